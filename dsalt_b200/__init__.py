@@ -15,6 +15,14 @@ from .ops import (  # noqa: F401
     select_landmarks,
     window_signals,
 )
+from .serving import (  # noqa: F401
+    SlotPlan,
+    append_cache,
+    cache_attention,
+    release_slots,
+    reserve_slots,
+    sample_tokens,
+)
 from .module import DSALTAttention  # noqa: F401
 from .model import DSALTConfig, DSALTLMHeadModel, DSALTTransformerBlock  # noqa: F401
 from ._lib import DsaltError  # noqa: F401

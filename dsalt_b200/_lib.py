@@ -56,6 +56,13 @@ SIGNATURES = {
     "dsalt_select_shard": (_I, [_I, _P, _P, _P, _P, _I64, _I, _I, _I, _I, _I, _I, _P, _SZ, _P, _P, _P]),
     "dsalt_attention_fwd_sharded": (_I, [_P, _P, _P, _I, _I64, _I, _I, _I, _I64, _I64, _I64, _I64, _I64, _I64,
                                          _P, _P, _P, _I, _I, _P, _P, _I64, _P, _I, _P, _P, _SZ, _P]),
+    "dsalt_reserve_slots": (_I, [_P, _I, _I, _P, _P, _P, _I64, _P, _I, _I64, _P, _P, _P, _P, _P, _P, _P]),
+    "dsalt_release_slots": (_I, [_P, _I, _I, _P, _P, _P, _I64, _P, _I, _P]),
+    "dsalt_append_cache": (_I, [_P, _P, _I, _I64, _I, _I, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I, _P, _P]),
+    "dsalt_cache_attention_workspace_bytes": (_SZ, [_I64, _I, _I, _I, _I]),
+    "dsalt_cache_attention": (_I, [_P, _I, _I64, _I, _I, _I, _I64, _P, _P, _P, _P, _I64, _I, _P, _I, _P, _I, _P, _P,
+                                   _P, _P, _I, _P, _I, _P, _P, _SZ, _P]),
+    "dsalt_sample": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _F, _P, _I, _P, _F, _P, _F, _P, _P, _P]),
     "dsalt_peer_barrier": (_I, [_P, _P, _I, _I, _I, _P]),
     "dsalt_peer_allgather": (_I, [_P, _P, _I, _I, _I64, _P]),
     "dsalt_peer_copy": (_I, [_P, _P, _I64, _P]),

@@ -6,6 +6,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/dsalt_b200.h"
 
 #if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ < 1000)
@@ -34,6 +36,20 @@ void set_error(const char* fmt, ...);
 int fail(int code, const char* fmt, ...);
 int check_cuda(cudaError_t e, const char* what);
 int* device_status_ptr();  // device address of the status word of the current device
+
+// Raises a kernel's dynamic shared-memory limit on the current device, once per device:
+// `ready` (one bit per device) belongs to the kernel.
+inline int allow_dynamic_smem(const void* kernel, int bytes, std::atomic<uint64_t>& ready) {
+  int dev = 0;
+  if (int rc = check_cuda(cudaGetDevice(&dev), "current device")) return rc;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (ready.load(std::memory_order_acquire) & bit)) return DSALT_OK;
+  if (int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
+                          "dynamic shared memory limit"))
+    return rc;
+  ready.fetch_or(bit, std::memory_order_release);
+  return DSALT_OK;
+}
 
 // device-side status word: the first kernel that gives up a bounded wait records a
 // code here; the host reads it with dsalt_device_status().

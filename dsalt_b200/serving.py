@@ -1,0 +1,256 @@
+"""Serving operators over the C ABI: a paged key/value cache in 8 bits, the attention that
+reads it, and sampling.
+
+* :func:`reserve_slots` / :func:`release_slots` — block tables and slot maps, built on the
+  GPU from the rows' lengths
+* :func:`append_cache`    — keys and values of new tokens into their slots, e4m3 with one
+  power-of-two scale per page and kv head
+* :func:`cache_attention` — window-and-landmark (or full) attention of one or a few query
+  tokens per sequence over the cache
+* :func:`sample_tokens`   — temperature, top-k, top-p and min-p from given uniforms
+
+The reference has no counterpart (it recomputes the whole sequence for every token). As in
+:mod:`dsalt_b200.ops`, tensors must be CUDA tensors and every call launches on the current
+stream of their device; lengths and tables stay on the device, so nothing here synchronises
+and every call can be captured into a CUDA graph.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib as L
+from .ops import _dt, _ptr, _workspace
+
+PAGE_SIZES = (16, 32, 64, 128)
+MAX_ROWS = 8192          # rows (sequences) of one call
+MAX_VOCAB = 1 << 20
+
+
+class SlotPlan(NamedTuple):
+    """What :func:`reserve_slots` found for the new tokens, packed row after row."""
+    slots: torch.Tensor      # [n_tokens] int64: page * page_size + offset, -1 = none
+    positions: torch.Tensor  # [n_tokens] int32: position within the sequence (0 where no slot)
+    cu_new: torch.Tensor     # [S + 1] int32: first token of each row
+    granted: torch.Tensor    # [S] bool
+    seq_lens: torch.Tensor   # [S] int32: lengths with the new tokens of granted rows
+    n_free: torch.Tensor     # [1] int32: pages left
+
+
+def _on_one_device(first: torch.Tensor, *rest) -> torch.device:
+    dev = first.device
+    if dev.type != "cuda":
+        raise RuntimeError("dsalt_b200 operators need CUDA tensors (no CPU path)")
+    for t in rest:
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"tensors on {dev} and {t.device} in one call")
+    return dev
+
+
+def _want(t: torch.Tensor, name: str, dtype: torch.dtype, shape) -> None:
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _run(dev: torch.device, name: str, *args) -> None:
+    """The C call on the current stream of the tensors' device."""
+    if dev.index == torch.cuda.current_device():
+        L.call(name, *args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            L.call(name, *args, torch.cuda.current_stream().cuda_stream)
+
+
+# --------------------------------------------------------------------------- slots
+def reserve_slots(block_tables, seq_lens, new_lens, free_pages, n_free, page_size: int, n_tokens: int, *,
+                  inplace: bool = False) -> SlotPlan:
+    """Pages and slots for ``new_lens [S]`` more tokens of rows that hold ``seq_lens [S]``.
+
+    ``block_tables [S, max_pages]`` int32 is extended in place with pages from the top of the
+    stack ``free_pages [N]`` (the first ``n_free [1]`` entries count). Rows are served in
+    order; a row whose table, or the room for ``n_tokens`` tokens, or the pool does not hold
+    its new tokens is not granted: it keeps its length and its tokens get slot -1. A row that
+    needs no page is not held up by rows that wait for one. With ``inplace`` the new lengths
+    and free count are written to ``seq_lens`` and ``n_free`` (as a captured step needs)."""
+    dev = _on_one_device(block_tables, seq_lens, new_lens, free_pages, n_free)
+    if block_tables.dim() != 2 or free_pages.dim() != 1:
+        raise ValueError("block_tables must be [S, max_pages] and free_pages [N]")
+    S, max_pages = block_tables.shape
+    i32 = torch.int32
+    _want(block_tables, "block_tables", i32, (S, max_pages))
+    _want(seq_lens, "seq_lens", i32, (S,))
+    _want(new_lens, "new_lens", i32, (S,))
+    _want(free_pages, "free_pages", i32, free_pages.shape)
+    _want(n_free, "n_free", i32, (1,))
+    n_tokens = int(n_tokens)
+    if n_tokens < 0:
+        raise ValueError("n_tokens must not be negative")
+    slots = torch.empty(n_tokens, dtype=torch.int64, device=dev)
+    ints = torch.empty(((n_tokens + 3) & ~3) + 2 * S + 2, dtype=i32, device=dev)
+    positions, _, cu_new, lens, left = ints.split_with_sizes([n_tokens, -n_tokens & 3, S + 1, S, 1])
+    granted = torch.empty(S, dtype=torch.bool, device=dev)
+    if inplace:
+        lens, left = seq_lens, n_free
+    _run(dev, "dsalt_reserve_slots", block_tables.data_ptr(), S, max_pages, seq_lens.data_ptr(), new_lens.data_ptr(),
+         free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(), int(page_size), n_tokens, slots.data_ptr(),
+         positions.data_ptr(), cu_new.data_ptr(), granted.data_ptr(), lens.data_ptr(), left.data_ptr())
+    return SlotPlan(slots, positions, cu_new, granted, lens, left)
+
+
+def release_slots(block_tables, seq_lens, release, free_pages, n_free, page_size: int) -> None:
+    """Gives the pages of the rows flagged in ``release [S]`` bool back to the stack, in place:
+    their table entries become -1 and their lengths 0. Pages go back in the order in which
+    :func:`reserve_slots` would take them again."""
+    dev = _on_one_device(block_tables, seq_lens, release, free_pages, n_free)
+    if block_tables.dim() != 2 or free_pages.dim() != 1:
+        raise ValueError("block_tables must be [S, max_pages] and free_pages [N]")
+    S, max_pages = block_tables.shape
+    i32 = torch.int32
+    _want(block_tables, "block_tables", i32, (S, max_pages))
+    _want(seq_lens, "seq_lens", i32, (S,))
+    _want(release, "release", torch.bool, (S,))
+    _want(free_pages, "free_pages", i32, free_pages.shape)
+    _want(n_free, "n_free", i32, (1,))
+    _run(dev, "dsalt_release_slots", block_tables.data_ptr(), S, max_pages, seq_lens.data_ptr(), release.data_ptr(),
+         free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(), int(page_size))
+
+
+# --------------------------------------------------------------------------- cache
+def _cache_shapes(k_cache, v_cache, k_scale, v_scale):
+    if k_cache.dim() != 4:
+        raise ValueError("k_cache must be [n_pages, H_kv, page_size, head_dim]")
+    n_pages, n_kv, page, D = k_cache.shape
+    _want(k_cache, "k_cache", torch.float8_e4m3fn, k_cache.shape)
+    _want(v_cache, "v_cache", torch.float8_e4m3fn, k_cache.shape)
+    _want(k_scale, "k_scale", torch.float32, (n_pages, n_kv))
+    _want(v_scale, "v_scale", torch.float32, (n_pages, n_kv))
+    return n_pages, n_kv, page, D
+
+
+def _rows_ok(x) -> bool:
+    """Rows of ``x [T, H, D]`` that 16-byte loads can take."""
+    es = x.element_size()
+    return (x.stride(2) == 1 and x.data_ptr() % 16 == 0 and x.stride(0) * es % 16 == 0 and x.stride(1) * es % 16 == 0)
+
+
+def append_cache(k, v, k_cache, v_cache, k_scale, v_scale, slots) -> None:
+    """Quantises ``k, v [T, H_kv, D]`` into their slots, in place.
+
+    ``k_cache, v_cache [n_pages, H_kv, page_size, D]`` float8_e4m3fn, ``k_scale, v_scale
+    [n_pages, H_kv]`` fp32 powers of two; ``slots [T]`` int64 from :func:`reserve_slots` (-1: the
+    token is left out). The slots of one page must be distinct and lie within ``page_size``
+    consecutive tokens of the call (:func:`reserve_slots` numbers them next to each other).
+    The scale of a page follows the largest magnitude written since its first token; when it
+    grows, the bytes already there are rescaled."""
+    dev = _on_one_device(k, v, k_cache, v_cache, k_scale, v_scale, slots)
+    n_pages, n_kv, page, D = _cache_shapes(k_cache, v_cache, k_scale, v_scale)
+    T = k.shape[0]
+    if tuple(k.shape) != (T, n_kv, D) or v.shape != k.shape:
+        raise ValueError(f"k and v must be [T, {n_kv}, {D}]")
+    if v.dtype != k.dtype:
+        raise TypeError("k and v must share a dtype")
+    _want(slots, "slots", torch.int64, (T,))
+    if not _rows_ok(k):
+        k = k.contiguous()
+    if not _rows_ok(v):
+        v = v.contiguous()
+    _run(dev, "dsalt_append_cache", k.data_ptr(), v.data_ptr(), _dt(k), T, n_kv, D, k.stride(0), k.stride(1), v.stride(0),
+         v.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_pages, page,
+         slots.data_ptr())
+
+
+def cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, *, cu_q=None, w_sizes=None,
+                    lmk_indices=None, lmk_bias=None, out_dtype=None, return_lse: bool = False):
+    """Attention of the last query tokens of each sequence over the cache: ``out [T, H, D]`` in
+    ``out_dtype`` (default the query's), with ``return_lse`` also ``lse [T, H]`` fp32.
+
+    ``seq_lens [S]`` int32 tokens in the cache, the query tokens included. ``cu_q [S + 1]`` int32
+    packs the query tokens; without it there is one per sequence. With ``w_sizes [T]`` int32 the
+    query at position ``i`` attends to its window ``[i - w + 1, i]`` and to the landmarks
+    ``lmk_indices [H, S, k]`` before it, as :func:`dsalt_b200.ops.dsalt_attention` does
+    (``lmk_bias`` is added to their logits); without, to ``[0, i]``."""
+    dev = _on_one_device(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, w_sizes, lmk_indices,
+                         lmk_bias)
+    n_pages, n_kv, page, D = _cache_shapes(k_cache, v_cache, k_scale, v_scale)
+    if q.dim() != 3 or q.shape[2] != D or q.shape[1] % n_kv:
+        raise ValueError(f"q must be [T, H, {D}] with H a multiple of {n_kv}")
+    T, H, _ = q.shape
+    if block_tables.dim() != 2:
+        raise ValueError("block_tables must be [S, max_pages]")
+    S, max_pages = block_tables.shape
+    i32 = torch.int32
+    _want(block_tables, "block_tables", i32, (S, max_pages))
+    _want(seq_lens, "seq_lens", i32, (S,))
+    if cu_q is not None:
+        _want(cu_q, "cu_q", i32, (S + 1,))
+    elif T != S:
+        raise ValueError(f"{T} query tokens for {S} sequences: pass cu_q")
+    if w_sizes is not None:
+        _want(w_sizes, "w_sizes", i32, (T,))
+    k_lmk = 0
+    if lmk_indices is not None:
+        if w_sizes is None:
+            raise ValueError("landmarks need w_sizes")
+        k_lmk = lmk_indices.shape[-1]
+        _want(lmk_indices, "lmk_indices", i32, (H, S, k_lmk))
+    if lmk_bias is not None:
+        if lmk_indices is None:
+            raise ValueError("lmk_bias needs lmk_indices")
+        _want(lmk_bias, "lmk_bias", torch.float32, (H, S, k_lmk))
+    if not (_rows_ok(q) and q.stride(1) == D):
+        q = q.contiguous()
+    out = torch.empty(T, H, D, dtype=out_dtype or q.dtype, device=dev)
+    lse = torch.empty(T, H, dtype=torch.float32, device=dev) if return_lse else None
+    ws = _workspace(L.query("dsalt_cache_attention_workspace_bytes", T, S, H, n_kv, D), dev)
+    _run(dev, "dsalt_cache_attention", q.data_ptr(), _dt(q), T, H, n_kv, D, q.stride(0), k_cache.data_ptr(),
+         v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_pages, page, block_tables.data_ptr(), max_pages,
+         seq_lens.data_ptr(), S, _ptr(cu_q), _ptr(w_sizes), _ptr(lmk_indices), _ptr(lmk_bias), k_lmk, out.data_ptr(),
+         _dt(out), _ptr(lse), ws.data_ptr(), ws.numel())
+    return (out, lse) if return_lse else out
+
+
+# --------------------------------------------------------------------------- sampling
+def _setting(v, name: str, B: int, dtype: torch.dtype, lo, hi):
+    """(device array or None, number) of a setting given per row or for all."""
+    if isinstance(v, torch.Tensor):
+        _want(v, name, dtype, (B,))
+        return v, 0
+    if not lo <= v <= hi:  # refuses NaN as well
+        raise ValueError(f"{name} must lie in [{lo}, {hi}], got {v}")
+    return None, v
+
+
+def sample_tokens(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, return_logprob: bool = False):
+    """One token per row of ``logits [B, V]`` from the given uniforms ``u [B]`` fp32 in [0, 1):
+    ``token [B]`` int64, with ``return_logprob`` also its log-probability ``[B]`` fp32 in the
+    distribution that it was drawn from.
+
+    Of the weights ``exp((l - max l) / temperature)`` ``top_k`` keeps the largest (equal logits:
+    lowest index first; 0 = off), ``top_p`` of those the shortest prefix whose mass reaches
+    ``top_p`` of theirs, ``min_p`` of those the weights of at least ``min_p``. The token is the
+    first index whose running sum of kept weights exceeds ``u`` times their total;
+    ``temperature`` 0 takes the largest logit. Each setting is a number or a ``[B]`` tensor
+    (fp32; ``top_k`` int32). A row gives the same token in every batch."""
+    per_row = [t for t in (temperature, top_k, top_p, min_p) if isinstance(t, torch.Tensor)]
+    dev = _on_one_device(logits, u, *per_row)
+    if logits.dim() != 2:
+        raise ValueError("logits must be [B, V]")
+    B, V = logits.shape
+    _want(u, "u", torch.float32, (B,))
+    f32, inf = torch.float32, float("inf")
+    t, tv = _setting(temperature, "temperature", B, f32, 0.0, 3e38)
+    k, kv = _setting(top_k, "top_k", B, torch.int32, 0, 2**31 - 1)
+    p, pv = _setting(top_p, "top_p", B, f32, 0.0, inf)
+    mp, mv = _setting(min_p, "min_p", B, f32, 0.0, 1.0)
+    if V > 1 and logits.stride(1) != 1 or (B > 1 and logits.stride(0) < V):
+        logits = logits.contiguous()
+    token = torch.empty(B, dtype=torch.int64, device=dev)
+    logprob = torch.empty(B, dtype=f32, device=dev) if return_logprob else None
+    _run(dev, "dsalt_sample", logits.data_ptr(), _dt(logits), B, V, logits.stride(0) if B > 1 else V, u.data_ptr(),
+         _ptr(t), tv, _ptr(k), kv, _ptr(p), pv, _ptr(mp), mv, token.data_ptr(), _ptr(logprob))
+    return (token, logprob) if return_logprob else token

@@ -313,6 +313,99 @@ int dsalt_core_forward(int mode, const void* x, int x_dtype, int d_model, int64_
                        const int32_t* cu_seqlens, int n_seqs, int64_t T, int max_seqlen, void* out, int out_dtype,
                        int32_t* w_out, int32_t* lmk_out, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Serving operators (no counterpart in the reference, which recomputes the whole sequence
+ * for every token): a paged key/value cache in 8 bits, the attention that reads it, and
+ * sampling. Lengths, tables and counts are device data, so a captured call follows them.
+ *
+ * Pages hold page_size tokens (16, 32, 64 or 128) of every kv head. block_tables
+ * [n_seqs, max_pages] int32 lists the pages of each row (sequence), -1 where none; the pages
+ * of no row are a stack free_pages [free_capacity] of which the first n_free [1] count.
+ *
+ * dsalt_reserve_slots: pages and slots for new_lens [n_seqs] more tokens of rows that hold
+ *   seq_lens [n_seqs] (negative numbers count as 0). Tokens are packed row after row;
+ *   n_tokens is the room in slots / positions. A row is granted when its table
+ *   (max_pages * page_size tokens) and the room hold its new tokens and either it needs no
+ *   page or the running sum of needed pages, over the rows that fit in order, is at most
+ *   n_free; a row that is not granted keeps its length and gets nothing. Page number j of
+ *   that order is free_pages[n_free - 1 - j]. Writes the new table entries, slots [n_tokens]
+ *   int64 (page * page_size + offset; -1 for tokens of rows not granted and behind the last
+ *   token), positions [n_tokens] (0 there), cu_new [n_seqs + 1] (first token of each row,
+ *   at most n_tokens), granted [n_seqs] bytes, seq_lens_out and n_free_out (which may be
+ *   seq_lens and n_free). At most 8192 rows. slots and positions 16-byte aligned.
+ * dsalt_release_slots: gives the pages of the rows flagged in release [n_seqs] bytes back to
+ *   the stack, in the order in which reserve would take them again; their entries become -1
+ *   and their lengths 0.
+ */
+int dsalt_reserve_slots(int32_t* block_tables, int n_seqs, int max_pages, const int32_t* seq_lens,
+                        const int32_t* new_lens, const int32_t* free_pages, int64_t free_capacity,
+                        const int32_t* n_free, int page_size, int64_t n_tokens, int64_t* slots, int32_t* positions,
+                        int32_t* cu_new, uint8_t* granted, int32_t* seq_lens_out, int32_t* n_free_out, void* stream);
+int dsalt_release_slots(int32_t* block_tables, int n_seqs, int max_pages, int32_t* seq_lens, const uint8_t* release,
+                        int32_t* free_pages, int64_t free_capacity, int32_t* n_free, int page_size, void* stream);
+
+/*
+ * dsalt_append_cache: quantises the keys and values of T new tokens into their slots.
+ * k, v [T, n_kv, head_dim] of dtype (token and head strides in elements; 16-byte aligned
+ *   rows; head_dim 64 or 128); k_cache, v_cache [n_pages, n_kv, page_size, head_dim] e4m3
+ *   bytes; k_scale, v_scale [n_pages, n_kv] fp32, powers of two: an element is byte * scale.
+ * The scale of a (page, kv head) is the smallest 2^e, e >= -110, with amax <= 448 * 2^e over
+ *   the tokens of the page; it starts afresh in a call that writes the page's first token,
+ *   otherwise it never falls, and when it grows the bytes already there are rescaled (rounded
+ *   to nearest even). Infinities are stored as the largest value (448 * 2^e) and do not count
+ *   for amax, NaN as NaN.
+ * slots [T] int64; negative or beyond the pool: the token is left out. The slots of one page
+ *   must be distinct and lie within page_size consecutive tokens of the call, in any order (as
+ *   dsalt_reserve_slots numbers them: next to each other).
+ */
+int dsalt_append_cache(const void* k, const void* v, int dtype, int64_t T, int n_kv, int head_dim,
+                       int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                       void* k_cache, void* v_cache, float* k_scale, float* v_scale, int64_t n_pages, int page_size,
+                       const int64_t* slots, void* stream);
+
+/*
+ * dsalt_cache_attention: attention of the last query tokens of each sequence over the cache.
+ * q [T, n_heads, head_dim] (token stride q_stride, 16-byte aligned rows; bf16, fp16 or fp32;
+ *   head_dim 64 or 128); cache, scales and tables as above; head h reads kv head
+ *   h / (n_heads / n_kv).
+ * seq_lens [n_seqs]: tokens in the cache, the query tokens included; cu_q [n_seqs + 1]
+ *   (starting at 0, at most T): query tokens of each sequence, the r-th of n at position
+ *   seq_len - n + r. Null: one per sequence, T = n_seqs.
+ * w [T] int32 widths (at least 1 is taken): the query at position i attends to
+ *   [max(0, i - w + 1), i] and to the landmarks lmk [n_heads, n_seqs, k_lmk] p with
+ *   0 <= p < i - w + 1 (any order, distinct, -1 = none), whose logits get lmk_bias (nullable).
+ *   w null: to [0, i], k_lmk = 0.
+ * out [T, n_heads, head_dim] in out_dtype, lse [T, n_heads] (nullable, natural log). A query
+ *   without keys and rows behind cu_q's last token give zeros and -inf.
+ * Keys on a page number outside [0, n_pages) are left out and reported in the device status
+ *   word. Deterministic. At most 8192 sequences.
+ */
+size_t dsalt_cache_attention_workspace_bytes(int64_t T, int n_seqs, int n_heads, int n_kv, int head_dim);
+int dsalt_cache_attention(const void* q, int dtype, int64_t T, int n_heads, int n_kv, int head_dim, int64_t q_stride,
+                          const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                          int64_t n_pages, int page_size, const int32_t* block_tables, int max_pages,
+                          const int32_t* seq_lens, int n_seqs, const int32_t* cu_q, const int32_t* w,
+                          const int32_t* lmk, const float* lmk_bias, int k_lmk, void* out, int out_dtype, float* lse,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * dsalt_sample: one token per row of logits [B, V] (row stride in elements, any alignment;
+ * fp32, bf16 or fp16; V at most 2^20) from given uniforms u [B] in [0, 1).
+ * With weights exp((l - max l) / temperature): top_k keeps the k first in the order (logit
+ *   descending, index ascending), top_p of those the shortest prefix whose mass reaches top_p
+ *   times theirs, min_p of those the weights of at least min_p; token is the first index
+ *   whose running sum of kept weights (index order) exceeds u times their total, logprob
+ *   (nullable) log of its share of that total.
+ * Each setting is a device array [B], or null and the value beside it. temperature <= 0 takes
+ *   the first index of the largest logit (logprob 0); top_k outside [1, V), top_p >= 1 and
+ *   min_p <= 0 are off. A NaN logit counts as -inf; +inf logits share the draw; a row of
+ *   nothing but -inf gives token 0 and logprob -inf.
+ */
+int dsalt_sample(const void* logits, int dtype, int64_t B, int64_t V, int64_t row_stride, const float* u,
+                 const float* temperature, float temperature_value, const int32_t* top_k, int top_k_value,
+                 const float* top_p, float top_p_value, const float* min_p, float min_p_value, int64_t* token,
+                 float* logprob, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
