@@ -13,8 +13,8 @@
 //   two per row to a largest magnitude in [2^13, 2^14), which keeps bf16 and fp16 values
 //   exact (those below 2^-27 of the row's largest fall short, under fp32's own rounding);
 // * the contraction order of a product is free, so lane (g, t) takes 16 consecutive bytes of
-//   key g for Q K^T and the D/8 bytes at D/8 g of keys 2t, 2t+1, 2t+8, 2t+9 for P V: whole
-//   sectors, no shared memory, no shuffles of data;
+//   one key for Q K^T and the D/8 bytes at D/8 g of four keys for P V, as they lie in the
+//   cache: no transposition, no shuffles of data;
 // * P is rounded to fp16 relative to the row's largest p * 2^e (half a step is 2^-12, under
 //   the 2^-9 of a bf16 result and as large as an fp16 result's own); fp32 queries take Q and
 //   P as two fp16 terms each (22 bits).
@@ -70,6 +70,13 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// cp.async of 16 bytes, zeros when !ok
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, bool ok) { cp_async_16(dst, src, ok ? 16 : 0); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // two e4m3 bytes -> two fp16
 __device__ __forceinline__ uint32_t widen_lo(uint32_t v) {
   uint32_t r;
@@ -138,40 +145,30 @@ __device__ __forceinline__ int2 block_before2(int2 v, int2* red, int2& all) {
   return make_int2(before.x + s.x - v.x, before.y + s.y - v.y);
 }
 
+// One stage of a warp's ring: 16 keys. K and V rows of D bytes, their 16-byte chunks placed so
+// that a warp's fragment loads meet no bank twice, and per key {scale of K, exponent of V's,
+// bias, position or -1}.
 template <int D>
-struct Frag {
-  uint32_t k[2][D / 16];   // key g of either half: D/4 bytes of this lane
-  uint32_t v[4][D / 32];   // keys 2t, 2t+1, 2t+8, 2t+9: D/8 bytes each
+struct Stage {
+  static constexpr int BYTES = 2 * 16 * D + 256;
+  static __device__ __forceinline__ int k_at(int r, int c) {
+    return D == 64 ? ((r ^ (r >> 2 & 1)) * 64 + c * 16) : (r * 128 + ((c ^ (r & 4)) * 16));
+  }
+  static __device__ __forceinline__ int v_at(int r, int c) {
+    return 16 * D + (D == 64 ? r * 64 + ((c ^ (r & 2)) * 16) : r * 128 + ((c ^ (r & 3) << 1) * 16));
+  }
+  static constexpr int META = 32 * D;
 };
+// Which key of the 16 is column n of half nt of S: so chosen that lane t's P columns 2t, 2t+1
+// of both halves are keys t, t+4, t+8, t+12, whose V rows lie together.
+__device__ __forceinline__ int slot_of(int nt, int n) { return nt * 8 + (n >> 1) + 4 * (n & 1); }
 
-// D/4 bytes of K (16 at 16 t of each 64) and D/8 bytes of V (at D/8 g) of one cache row
-template <int D>
-__device__ __forceinline__ void load_k(uint32_t (&r)[D / 16], const uint8_t* base, int row, int t, bool ok) {
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (ok) x = __ldg(reinterpret_cast<const uint4*>(base + (int64_t)row * D + i * 64 + t * 16));
-    r[4 * i] = x.x, r[4 * i + 1] = x.y, r[4 * i + 2] = x.z, r[4 * i + 3] = x.w;
-  }
-}
-template <int D>
-__device__ __forceinline__ void load_v(uint32_t (&r)[D / 32], const uint8_t* base, int row, int g, bool ok) {
-  if constexpr (D == 64) {
-    uint2 x = make_uint2(0, 0);
-    if (ok) x = __ldg(reinterpret_cast<const uint2*>(base + (int64_t)row * D + g * 8));
-    r[0] = x.x, r[1] = x.y;
-  } else {
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (ok) x = __ldg(reinterpret_cast<const uint4*>(base + (int64_t)row * D + g * 16));
-    r[0] = x.x, r[1] = x.y, r[2] = x.z, r[3] = x.w;
-  }
-}
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t v) {  // 0xff where a byte is an e4m3 NaN
   return __vcmpeq4(v & 0x7f7f7f7fu, 0x7f7f7f7fu);
 }
 
 // NS: fp16 terms that Q and P are held in (2 for fp32 queries)
-template <typename T, int D, int NS>
+template <typename T, int D, int NS, int STAGES>
 __global__ void __launch_bounds__(CA_THREADS) cache_attn_kernel(CacheAttnArgs a) {
   constexpr int KS = D / 16, NT = D / 8;
   extern __shared__ __align__(16) unsigned char dyn[];
@@ -250,7 +247,6 @@ __global__ void __launch_bounds__(CA_THREADS) cache_attn_kernel(CacheAttnArgs a)
   const int split = local % splits, item = local / splits;
   const int hk = item % a.Hkv, tile = item / a.Hkv;
   const int part0 = s_cut[s] + item * splits;
-  __syncthreads();  // the schedule's memory is used again below
   const int each = (groups + splits - 1) / splits;
   const int g_begin = split * each, g_end = min(g_begin + each, groups);
 
@@ -350,182 +346,307 @@ __global__ void __launch_bounds__(CA_THREADS) cache_attn_kernel(CacheAttnArgs a)
   const int lmk16 = (a.k_lmk + 15) >> 4;
   bool bad_page = false;
 
-  for (int gi = g_begin + warp; gi < g_end; gi += CA_WARPS) {
-    const bool window = gi < p.n_window;
-    const int key0 = p.lo16 + gi * 16;
-    if (window && (key0 + 16 <= lo_min || key0 >= hi_max)) continue;  // keys of the sequence's other tiles
-    // slot j = lane & 15 of the group: its cache row (or -1), scales, position
-    int key, row = -1, slot_head = 0;
-    float add = 0.f, ks = 0.f, ve = 0.f;
-    const int j = lane & 15;
-    if (window) key = key0 + j;
-    else {
-      const int l = gi - p.n_window, c = (l % lmk16) * 16 + j;
-      slot_head = l / lmk16;
-      key = -1;
-      if (c < a.k_lmk) {
-        const int64_t at = ((int64_t)(hk * a.G + slot_head) * a.n_seqs + s) * a.k_lmk + c;
-        key = a.lmk[at];
-        if (a.bias) add = a.bias[at] * 1.4426950408889634f;
-      }
-      if (key >= p.len) key = -1;  // no row attends to it, and it may lie outside the table
-    }
+  // ---- this warp's share of the unit: a stretch of window groups, then one of landmark groups
+  const int w0 = min(g_begin, p.n_window), w1 = min(g_end, p.n_window);
+  const int l0 = max(g_begin - p.n_window, 0), l1 = max(g_end - p.n_window, 0);
+  const int wq = (w1 - w0 + CA_WARPS - 1) / CA_WARPS, lq = (l1 - l0 + CA_WARPS - 1) / CA_WARPS;
+  int wb = min(w0 + warp * wq, w1), we = min(wb + wq, w1);
+  const int lb = min(l0 + warp * lq, l1), le = min(lb + lq, l1);
+  // (keys of the sequence's other tiles are passed over)
+  wb = max(wb, min(we, (lo_min < p.len ? lo_min - p.lo16 : 0x7ffffff0) >> 4));
+  we = min(we, max(wb, (hi_max - p.lo16 + 15) >> 4));
+  const int n_w = we - wb, n = n_w + le - lb;
+
+  // where keys lie: of 32 window groups ahead a lane each, of 2 landmark groups a lane per key
+  struct Where {
+    int row, key;
+    float ks, ve, add;
+  };
+  auto look_up = [&](int key, Where& o) {
+    o.row = -1;
+    o.ks = 0.f;
+    o.ve = 0.f;
     if (key >= 0 && key < p.len) {
       const int id = __ldg(table + (key >> a.page_shift));
       if ((unsigned)id < (unsigned)a.n_pages) {
         const int64_t head = (int64_t)id * a.Hkv + hk;
-        row = (int)(head << a.page_shift) + (key & page_mask);
-        ks = __ldg(a.ks + head);
-        ve = scale_log(__ldg(a.vs + head));
+        o.row = (int)(head << a.page_shift) + (key & page_mask);
+        o.ks = __ldg(a.ks + head);
+        o.ve = scale_log(__ldg(a.vs + head));
       } else {
         bad_page = true;
       }
     }
-    // valid for any row of the tile?  (a masked key's bytes are not looked at)
-    Frag<D> f;
-    {
-      const int r0 = __shfl_sync(0xffffffffu, row, g), r1 = __shfl_sync(0xffffffffu, row, g + 8);
-      load_k<D>(f.k[0], a.kc, r0, t, r0 >= 0);
-      load_k<D>(f.k[1], a.kc, r1, t, r1 >= 0);
+  };
+  auto find_window = [&](int i) {  // lane: group wb + i + lane
+    Where o;
+    o.add = 0.f;
+    o.key = i + lane < n_w ? p.lo16 + (wb + i + lane) * 16 : -1;
+    look_up(o.key, o);
+    return o;
+  };
+  auto find_lmk = [&](int i) {  // lane: key lane & 15 of group lb + i + (lane >> 4)
+    Where o;
+    o.add = 0.f;
+    o.key = -1;
+    const int l = lb + i + (lane >> 4), c = (l % max(lmk16, 1)) * 16 + (lane & 15);
+    if (l < le && c < a.k_lmk) {
+      const int64_t at = ((int64_t)(hk * a.G + l / lmk16) * a.n_seqs + s) * a.k_lmk + c;
+      o.key = a.lmk[at];
+      if (a.bias) o.add = a.bias[at] * 1.4426950408889634f;
+    }
+    if (o.key >= p.len) o.key = -1;  // no row attends to it, and it may lie outside the table
+    look_up(o.key, o);
+    return o;
+  };
+  Where ww = find_window(0), wn = ww, lw = ww, ln = ww;
+  if (n_w > 32) wn = find_window(32);
+  if (le > lb) {
+    lw = find_lmk(0);
+    ln = find_lmk(2);
+  }
+  uint8_t* ring = dyn + warp * (STAGES * Stage<D>::BYTES);
+  const uint32_t ring_s = smem_u32(ring);
+  auto issue = [&](int i) {
+    const uint32_t st_s = ring_s + (i % STAGES) * Stage<D>::BYTES;
+    uint8_t* st_p = ring + (i % STAGES) * Stage<D>::BYTES;
+    if (i < n) {
+      const bool window = i < n_w;
+      int row, key;  // of slot lane & 15
+      float ks, ve, add;
+      if (window) {
+        const int b = i & 31;
+        if (b == 0 && i > 0) {
+          ww = wn;
+          if (i + 32 < n_w) wn = find_window(i + 32);
+        }
+        row = __shfl_sync(0xffffffffu, ww.row, b);
+        key = __shfl_sync(0xffffffffu, ww.key, b) + (lane & 15);
+        ks = __shfl_sync(0xffffffffu, ww.ks, b);
+        ve = __shfl_sync(0xffffffffu, ww.ve, b);
+        add = 0.f;
+        row = row >= 0 && key < p.len ? row + (lane & 15) : -1;
+      } else {
+        const int li = i - n_w, b = li & 1;
+        if (b == 0 && li > 0) {
+          lw = ln;
+          if (lb + li + 2 < le) ln = find_lmk(li + 2);
+        }
+        const int from = b * 16 + (lane & 15);
+        row = __shfl_sync(0xffffffffu, lw.row, from);
+        key = __shfl_sync(0xffffffffu, lw.key, from);
+        ks = __shfl_sync(0xffffffffu, lw.ks, from);
+        ve = __shfl_sync(0xffffffffu, lw.ve, from);
+        add = __shfl_sync(0xffffffffu, lw.add, from);
+      }
+      if (lane < 16)
+        *reinterpret_cast<float4*>(st_p + Stage<D>::META + lane * 16) =
+            make_float4(ks, ve, add, __int_as_float(row >= 0 ? key : -1));
+      constexpr int CPR = D / 16, RPI = 32 / CPR;  // chunks per row, rows per step
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int rv = __shfl_sync(0xffffffffu, row, (i & 1) + 2 * t + (i >> 1) * 8);
-        load_v<D>(f.v[i], a.vc, rv, g, rv >= 0);
+      for (int x = 0; x < 16 / RPI; ++x) {
+        const int r = x * RPI + lane / CPR, c = lane % CPR;
+        const int rr = __shfl_sync(0xffffffffu, row, r);
+        const int64_t at = (int64_t)max(rr, 0) * D + c * 16;
+        copy16(st_s + Stage<D>::k_at(r, c), a.kc + at, rr >= 0);
+        copy16(st_s + Stage<D>::v_at(r, c), a.vc + at, rr >= 0);
       }
     }
+    copies_commit();
+  };
+  __syncthreads();  // the schedule's memory becomes the ring
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) issue(i);
+
+  for (int i = 0; i < n; ++i) {
+    copies_wait<STAGES - 2>();
+    __syncwarp();  // every lane's copies of stage i are there, and stage i - 1 is read
+    issue(i + STAGES - 1);
+    const uint8_t* stage = ring + (i % STAGES) * Stage<D>::BYTES;
+    const bool window = i < n_w;
+    float4 meta[4];  // keys t, t + 4, t + 8, t + 12: columns 2t, 2t + 1 of half 0, then of half 1
+#pragma unroll
+    for (int x = 0; x < 4; ++x) meta[x] = *reinterpret_cast<const float4*>(stage + Stage<D>::META + (t + 4 * x) * 16);
     // ---- S = Q K^T
     float sc[2][4];
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt) {
       sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const uint32_t b0 = widen_lo(f.k[nt][k]), b1 = widen_hi(f.k[nt][k]);
+      for (int b = 0; b < D / 64; ++b) {
+        const uint4 kw = *reinterpret_cast<const uint4*>(stage + Stage<D>::k_at(slot_of(nt, g), b * 4 + t));
+        const uint32_t kr[4] = {kw.x, kw.y, kw.z, kw.w};
 #pragma unroll
-        for (int n = 0; n < NS; ++n) mma_f16(sc[nt], qa[n][k][0], qa[n][k][1], qa[n][k][2], qa[n][k][3], b0, b1);
-      }
-    }
-    // ---- logits (base 2) of this lane's columns: keys 2t, 2t+1 of either half
-    const bool plain = window && key0 >= lo_max && key0 + 16 <= hi_min && !__any_sync(0xffffffffu, row < 0);
-    float ve_col[2][2];
-    uint32_t valid = 0;  // bit 4 nt + 2 r + c: row r attends to column c of half nt
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t b0 = widen_lo(kr[k]), b1 = widen_hi(kr[k]);
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int from = nt * 8 + 2 * t + c;
-        const float kscale = __shfl_sync(0xffffffffu, ks, from), badd = __shfl_sync(0xffffffffu, add, from);
-        ve_col[nt][c] = __shfl_sync(0xffffffffu, ve, from);
-        const int kk = __shfl_sync(0xffffffffu, key, from), rr = __shfl_sync(0xffffffffu, row, from);
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float x = fmaf(sc[nt][2 * r + c], kscale * row_f[r], badd);
-          const bool ok = plain || (rr >= 0 && (window ? kk >= row_lo[r] && kk < row_hi[r]
-                                                       : kk < row_lo[r] && kk < row_hi[r] && slot_head == row_head[r]));
-          if (ok) valid |= 1u << (4 * nt + 2 * r + c);
-          sc[nt][2 * r + c] = ok ? x : -INFINITY;
+          for (int x = 0; x < NS; ++x) {
+            const uint32_t(&q4)[4] = qa[x][b * 4 + k];
+            mma_f16(sc[nt], q4[0], q4[1], q4[2], q4[3], b0, b1);
+          }
         }
       }
+    }
+    // ---- logits (base 2); columns that a row does not attend to become -inf
+    const int key0 = p.lo16 + (wb + i) * 16;
+    const bool plain = window && key0 >= lo_max && key0 + 16 <= hi_min && __float_as_int(meta[0].w) >= 0;
+    uint32_t valid = 0xff;  // bit 4 nt + 2 r + c: row r attends to column c of half nt
+    if (plain) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float f = meta[0].x * row_f[r];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          sc[nt][2 * r] *= f;
+          sc[nt][2 * r + 1] *= f;
+        }
+      }
+    } else {
+      valid = 0;
+      const int head = window ? -1 : (lb + i - n_w) / lmk16;
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float4 mt = meta[2 * nt + c];
+          const int key = __float_as_int(mt.w);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const bool ok = key >= 0 && (window ? key >= row_lo[r] && key < row_hi[r]
+                                                : key < row_lo[r] && key < row_hi[r] && head == row_head[r]);
+            if (ok) valid |= 1u << (4 * nt + 2 * r + c);
+            sc[nt][2 * r + c] = ok ? fmaf(sc[nt][2 * r + c], mt.x * row_f[r], mt.z) : -INFINITY;
+          }
+        }
+    }
     // ---- online softmax with the two maxima
+    float gm[2], gM[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      gm[r] = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
+      gm[r] = fmaxf(gm[r], __shfl_xor_sync(0xffffffffu, gm[r], 1));
+      gm[r] = fmaxf(gm[r], __shfl_xor_sync(0xffffffffu, gm[r], 2));
+      if (window) {
+        gM[r] = gm[r] + meta[0].y;
+      } else {
+        gM[r] = fmaxf(fmaxf(sc[0][2 * r] + meta[0].y, sc[0][2 * r + 1] + meta[1].y),
+                      fmaxf(sc[1][2 * r] + meta[2].y, sc[1][2 * r + 1] + meta[3].y));
+        gM[r] = fmaxf(gM[r], __shfl_xor_sync(0xffffffffu, gM[r], 1));
+        gM[r] = fmaxf(gM[r], __shfl_xor_sync(0xffffffffu, gM[r], 2));
+      }
+    }
+    if (__any_sync(0xffffffffu, gm[0] > st[0].m || gm[1] > st[1].m || gM[0] > st[0].M || gM[1] > st[1].M)) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float m = fmaxf(st[r].m, gm[r]), M = fmaxf(st[r].M, gM[r]);
+        st[r].l *= m == -INFINITY ? 1.f : exp2_fast(st[r].m - m);
+        const float c = M == -INFINITY ? 1.f : exp2_fast(st[r].M - M);
+        st[r].m = m;
+        st[r].M = M;
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+          o[x][2 * r] *= c;
+          o[x][2 * r + 1] *= c;
+        }
+      }
+    }
     float pr[2][4];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      float gm = -INFINITY, gM = -INFINITY;
+      const float mu = st[r].m == -INFINITY ? 0.f : st[r].m, Mu = st[r].M == -INFINITY ? 0.f : st[r].M;
+      // 2^(x + e - M) = 2^(x - m) 2^(m + e - M); where the second factor is large the first is small
+      const float f = exp2_fast(fminf(mu - Mu + meta[0].y + CA_P_SHIFT, 126.f));
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          gm = fmaxf(gm, sc[nt][2 * r + c]);
-          gM = fmaxf(gM, sc[nt][2 * r + c] + ve_col[nt][c]);
+          const float x = sc[nt][2 * r + c], e = exp2_fast(x - mu);
+          st[r].l += e;
+          pr[nt][2 * r + c] = window ? e * f : exp2_fast(x + meta[2 * nt + c].y - Mu + CA_P_SHIFT);
         }
-#pragma unroll
-      for (int x = 1; x < 4; x <<= 1) {
-        gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, x));
-        gM = fmaxf(gM, __shfl_xor_sync(0xffffffffu, gM, x));
-      }
-      const float m = fmaxf(st[r].m, gm), M = fmaxf(st[r].M, gM);
-      const float mu = m == -INFINITY ? 0.f : m, Mu = M == -INFINITY ? 0.f : M;
-      const float cl = exp2_fast(st[r].m - mu), cO = exp2_fast(st[r].M - Mu);
-      float l = st[r].l * cl;
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float x = sc[nt][2 * r + c];
-          l += exp2_fast(x - mu);
-          pr[nt][2 * r + c] = exp2_fast(x + ve_col[nt][c] - Mu + CA_P_SHIFT);
-        }
-      st[r].m = m;
-      st[r].M = M;
-      st[r].l = l;
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        o[i][2 * r] *= cO;
-        o[i][2 * r + 1] *= cO;
-      }
     }
     // ---- O += P V
     uint32_t pa[NS][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int nt = i >> 1, r = i & 1;
+    for (int x = 0; x < 4; ++x) {
+      const int nt = x >> 1, r = x & 1;
       const float lo = pr[nt][2 * r], hi = pr[nt][2 * r + 1];
-      pa[0][i] = pack_f16x2(lo, hi);
+      pa[0][x] = pack_f16x2(lo, hi);
       if constexpr (NS == 2) {
-        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&pa[0][i]));
-        pa[1][i] = pack_f16x2(lo - b.x, hi - b.y);
+        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&pa[0][x]));
+        pa[1][x] = pack_f16x2(lo - b.x, hi - b.y);
+      }
+    }
+    uint32_t v[4][D / 32];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if constexpr (D == 64) {
+        const uint2 y = *reinterpret_cast<const uint2*>(stage + Stage<D>::v_at(t + 4 * x, g >> 1) + (g & 1) * 8);
+        v[x][0] = y.x, v[x][1] = y.y;
+      } else {
+        const uint4 y = *reinterpret_cast<const uint4*>(stage + Stage<D>::v_at(t + 4 * x, g));
+        v[x][0] = y.x, v[x][1] = y.y, v[x][2] = y.z, v[x][3] = y.w;
       }
     }
     bool nans = false;
     if (!plain) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int x = 0; x < 4; ++x)
 #pragma unroll
-        for (int x = 0; x < D / 32; ++x) nans |= nan_bytes(f.v[i][x]) != 0;
+        for (int y = 0; y < D / 32; ++y) nans |= nan_bytes(v[x][y]) != 0;
+      nans = __any_sync(0xffffffffu, nans);
     }
-    nans = !plain && __any_sync(0xffffffffu, nans);
-    uint32_t va[4] = {0, 0, 0, 0};
-    if (nans) {  // 1.0 where a row attends to a key: counts its NaNs, which P = 0 must not spread
+    if (nans) {
+      // P = 0 must not spread a NaN: count, per row and channel, the NaNs among the keys that the row
+      // attends to (a product of ones), and take the NaNs themselves out
+      uint32_t va[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        va[i] = (valid >> (4 * (i >> 1) + 2 * (i & 1)) & 1 ? 0x3c00u : 0u) |
-                (valid >> (4 * (i >> 1) + 2 * (i & 1) + 1) & 1 ? 0x3c000000u : 0u);
-    }
+      for (int x = 0; x < 4; ++x)
+        va[x] = (valid >> (4 * (x >> 1) + 2 * (x & 1)) & 1 ? 0x3c00u : 0u) |
+                (valid >> (4 * (x >> 1) + 2 * (x & 1) + 1) & 1 ? 0x3c000000u : 0u);
 #pragma unroll
-    for (int x = 0; x < D / 32; ++x) {
-      uint32_t v0 = f.v[0][x], v1 = f.v[1][x], v2 = f.v[2][x], v3 = f.v[3][x];
-      uint32_t n0 = 0, n1 = 0, n2 = 0, n3 = 0;
-      if (nans) {
-        n0 = nan_bytes(v0), n1 = nan_bytes(v1), n2 = nan_bytes(v2), n3 = nan_bytes(v3);
-        v0 &= ~n0, v1 &= ~n1, v2 &= ~n2, v3 &= ~n3;
-      }
+      for (int x = 0; x < D / 32; ++x) {
+        uint32_t nb[4];
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const uint32_t sel = y ? 0x7362 : 0x5140;
-        const uint32_t b0 = __byte_perm(v0, v1, sel), b1 = __byte_perm(v2, v3, sel);
+        for (int y = 0; y < 4; ++y) {
+          nb[y] = nan_bytes(v[y][x]);
+          v[y][x] &= ~nb[y];
+        }
 #pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const int nt = 4 * x + 2 * y + z;
-          const uint32_t w0 = z ? widen_hi(b0) : widen_lo(b0), w1 = z ? widen_hi(b1) : widen_lo(b1);
+        for (int y = 0; y < 2; ++y)
 #pragma unroll
-          for (int n = 0; n < NS; ++n) mma_f16(o[nt], pa[n][0], pa[n][1], pa[n][2], pa[n][3], w0, w1);
-          if (nans) {
-            // bytes 0xff -> fp16 1.0
-            const uint32_t m0 = __byte_perm(__byte_perm(n0, n1, sel), 0, z ? 0x3322 : 0x1100);
-            const uint32_t m1 = __byte_perm(__byte_perm(n2, n3, sel), 0, z ? 0x3322 : 0x1100);
+          for (int z = 0; z < 2; ++z) {
+            const uint32_t sel = y ? 0x7362 : 0x5140, half = z ? 0x3322 : 0x1100;
+            const uint32_t m0 = __byte_perm(__byte_perm(nb[0], nb[1], sel), 0, half);  // 0xffff per NaN
+            const uint32_t m1 = __byte_perm(__byte_perm(nb[2], nb[3], sel), 0, half);
             float cnt[4] = {0.f, 0.f, 0.f, 0.f};
             mma_f16(cnt, va[0], va[1], va[2], va[3], m0 & 0x3c003c00u, m1 & 0x3c003c00u);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (cnt[e] > 0.f) o[nt][e] = __int_as_float(0x7fffffff);
+              if (cnt[e] > 0.f) o[4 * x + 2 * y + z][e] = __int_as_float(0x7fffffff);
           }
-        }
       }
     }
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const uint32_t sel = y ? 0x7362 : 0x5140;
+        const uint32_t b0 = __byte_perm(v[0][x], v[1][x], sel), b1 = __byte_perm(v[2][x], v[3][x], sel);
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const uint32_t h0 = z ? widen_hi(b0) : widen_lo(b0), h1 = z ? widen_hi(b1) : widen_lo(b1);
+#pragma unroll
+          for (int q4 = 0; q4 < NS; ++q4)
+            mma_f16(o[4 * x + 2 * y + z], pa[q4][0], pa[q4][1], pa[q4][2], pa[q4][3], h0, h1);
+        }
+      }
   }
   if (bad_page) report_device_error(a.err, CA_ERR_PAGE);
 
   // ---- the warps' parts into one
+  copies_wait<0>();
+  __syncthreads();  // the rings' memory becomes the parts
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     float l = st[r].l;
@@ -629,14 +750,15 @@ static inline int64_t ca_items(int64_t T, int n_seqs, int G, int Hkv) { return (
 
 template <typename T, int D, int NS>
 static int launch_cache_attn(const CacheAttnArgs& a, unsigned grid, bool join, cudaStream_t stream) {
-  size_t smem = 2 * sizeof(int) * (size_t)a.n_seqs;
-  const size_t merge = sizeof(float) * CA_WARPS * 16 * D;
-  if (smem < merge) smem = merge;
+  constexpr int STAGES = D == 64 ? 6 : 4;
+  constexpr size_t RING = (size_t)CA_WARPS * STAGES * Stage<D>::BYTES;
+  static_assert(RING >= sizeof(float) * CA_WARPS * 16 * D, "the parts take the rings' place");
+  const size_t tables = 2 * sizeof(int) * (size_t)a.n_seqs, smem = tables > RING ? tables : RING;
   static std::atomic<uint64_t> ready{0};
-  if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(cache_attn_kernel<T, D, NS>),
-                                  (int)(2 * sizeof(int) * CA_MAX_SEQS), ready))
+  if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(cache_attn_kernel<T, D, NS, STAGES>),
+                                  (int)(2 * sizeof(int) * CA_MAX_SEQS > RING ? 2 * sizeof(int) * CA_MAX_SEQS : RING), ready))
     return rc;
-  cache_attn_kernel<T, D, NS><<<grid, CA_THREADS, smem, stream>>>(a);
+  cache_attn_kernel<T, D, NS, STAGES><<<grid, CA_THREADS, smem, stream>>>(a);
   if (int rc = check_cuda(cudaGetLastError(), "cache_attention launch")) return rc;
   if (!join) return DSALT_OK;
   cudaLaunchAttribute attr[1];
