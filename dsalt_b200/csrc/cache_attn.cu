@@ -22,10 +22,12 @@
 // denominator l = sum 2^(x - m), and M of x + e for the numerator O = sum 2^(x + e - M) byte;
 // out = O 2^(M - m) / l. Neither can overflow whatever the scales are.
 //
-// The keys of an item (sequence, kv head, tile of 16 rows) are a list of groups of 16: the
+// The keys of an item (sequence, kv head, tile of 16 rows) are a list of tiles of 32: the
 // window's, then the landmarks' of each head. Items are cut into units of about equal
 // length, by the lengths found on the device (no host copy of them is needed and a captured
 // call follows them); the parts of an item that was cut are joined by a second kernel.
+// Within a unit each of four warps has its own stretch of tiles and its own ring of
+// cp.async stages: nothing but the end is shared, so no warp waits for another.
 #include <type_traits>
 
 #include "common.cuh"
@@ -34,11 +36,20 @@ namespace dsalt {
 
 constexpr int CA_WARPS = 4;
 constexpr int CA_THREADS = 32 * CA_WARPS;
-constexpr int CA_TARGET = 148 * 4;     // units wanted where the keys can be cut into as many
-constexpr int CA_MIN_GROUPS = 16;      // groups of 16 keys that a unit takes at least
+constexpr int CA_MIN_TILES = 8;        // tiles of 32 keys that a unit takes at least: two per warp
 constexpr int CA_MAX_SEQS = 8192;
 constexpr int CA_ERR_PAGE = 41;        // device status: a page number outside the pool was met
 constexpr float CA_P_SHIFT = 14.f;     // P is held times 2^14: fp16 stays normal down to 2^-28
+constexpr float CA_SLACK = 1.f;        // P may exceed 2^14 by 2^1 before its reference moves (fp16 ends at 2^16)
+
+// blocks per SM that registers and rings allow; one round of them is the number of units wanted
+template <int D>
+struct Shape {
+  static constexpr int OCC = D == 64 ? 4 : 2;
+  static constexpr int STAGES = 3;
+  static constexpr int UNITS = 148 * OCC;
+};
+constexpr int CA_MAX_UNITS = 148 * 4;
 
 struct CacheAttnArgs {
   const void* q;
@@ -92,9 +103,9 @@ __device__ __forceinline__ float exp2_fast(float x) { return ex2_approx(x); }
 // e of a scale 2^e, as a float; 0 (a page never written) as the lowest
 __device__ __forceinline__ float scale_log(float s) { return (float)((int)(__float_as_uint(s) >> 23 & 0xff) - 127); }
 
-// query of sequence s: tokens, keys and the groups of 16 that they make
+// query of sequence s: tokens, keys and the tiles of 32 that they make
 struct SeqPlan {
-  int q0, n_q, len, lo16, n_window, n_lmk;  // lo16: first key of the first group
+  int q0, n_q, len, lo32, n_window, n_lmk;  // lo32: first key of the first window tile
 };
 __device__ __forceinline__ int first_key(const CacheAttnArgs& a, int t, int pos) {
   if (!a.w) return 0;
@@ -115,13 +126,13 @@ __device__ __forceinline__ SeqPlan plan_of(const CacheAttnArgs& a, int s) {
     lo = min(lo, f);
     top = max(top, f);
   }
-  // the last key is the sequence's last: groups behind a tile's own rows are passed over
-  p.lo16 = lo & ~15;
-  p.n_window = p.n_q > 0 && p.len > 0 ? (p.len - p.lo16 + 15) >> 4 : 0;
-  p.n_lmk = a.k_lmk > 0 && top > 0 ? a.G * ((a.k_lmk + 15) >> 4) : 0;  // none lies before a window from 0
+  // the last key is the sequence's last: tiles behind a row tile's own keys are passed over
+  p.lo32 = lo & ~31;
+  p.n_window = p.n_q > 0 && p.len > 0 ? (p.len - p.lo32 + 31) >> 5 : 0;
+  p.n_lmk = a.k_lmk > 0 && top > 0 ? a.G * ((a.k_lmk + 31) >> 5) : 0;  // none lies before a window from 0
   return p;
 }
-__device__ __forceinline__ int tiles_of(const CacheAttnArgs& a, int n_q) { return (n_q * a.G + 15) >> 4; }
+__device__ __forceinline__ int row_tiles(const CacheAttnArgs& a, int n_q) { return (n_q * a.G + 15) >> 4; }
 
 // sums of two numbers over the block's 128 threads, exclusive; totals in `all`
 __device__ __forceinline__ int2 block_before2(int2 v, int2* red, int2& all) {
@@ -145,22 +156,21 @@ __device__ __forceinline__ int2 block_before2(int2 v, int2* red, int2& all) {
   return make_int2(before.x + s.x - v.x, before.y + s.y - v.y);
 }
 
-// One stage of a warp's ring: 16 keys. K and V rows of D bytes, their 16-byte chunks placed so
-// that a warp's fragment loads meet no bank twice, and per key {scale of K, exponent of V's,
-// bias, position or -1}.
+// One stage of a warp's ring: 32 keys. K and V rows of D bytes, their 16-byte chunks placed so
+// that a warp's fragment loads meet no bank twice, and {scale of K, exponent of V's, bias,
+// position or -1}: of landmarks per key, of a window tile per half at keys 0 and 16.
 template <int D>
 struct Stage {
-  static constexpr int BYTES = 2 * 16 * D + 256;
+  static constexpr int V = 32 * D, META = 64 * D, BYTES = 64 * D + 512;
   static __device__ __forceinline__ int k_at(int r, int c) {
     return D == 64 ? ((r ^ (r >> 2 & 1)) * 64 + c * 16) : (r * 128 + ((c ^ (r & 4)) * 16));
   }
   static __device__ __forceinline__ int v_at(int r, int c) {
-    return 16 * D + (D == 64 ? r * 64 + ((c ^ (r & 2)) * 16) : r * 128 + ((c ^ (r & 3) << 1) * 16));
+    return V + (D == 64 ? r * 64 + ((c ^ (r & 2)) * 16) : r * 128 + ((c ^ (r & 3) << 1) * 16));
   }
-  static constexpr int META = 32 * D;
 };
-// Which key of the 16 is column n of half nt of S: so chosen that lane t's P columns 2t, 2t+1
-// of both halves are keys t, t+4, t+8, t+12, whose V rows lie together.
+// Which key of the tile is column n of block nt of S: so chosen that lane t's P columns 2t,
+// 2t+1 of blocks 2h, 2h+1 are keys t, t+4, t+8, t+12 of half h, whose V rows lie together.
 __device__ __forceinline__ int slot_of(int nt, int n) { return nt * 8 + (n >> 1) + 4 * (n & 1); }
 
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t v) {  // 0xff where a byte is an e4m3 NaN
@@ -168,42 +178,47 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t v) {  // 0xff where a byt
 }
 
 // NS: fp16 terms that Q and P are held in (2 for fp32 queries)
-template <typename T, int D, int NS, int STAGES>
-__global__ void __launch_bounds__(CA_THREADS) cache_attn_kernel(CacheAttnArgs a) {
-  constexpr int KS = D / 16, NT = D / 8;
+template <typename T, int D, int NS>
+__global__ void __launch_bounds__(CA_THREADS, NS == 1 ? Shape<D>::OCC : 1) cache_attn_kernel(CacheAttnArgs a) {
+  constexpr int KS = D / 16, NT = D / 8, STAGES = Shape<D>::STAGES;
+  constexpr bool Q_SMEM = D == 128 || NS == 2;  // registers hold Q only where there is room beside O
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ int2 red[CA_WARPS];
+  __shared__ long long s_sum[CA_WARPS];
   __shared__ float s_m[CA_WARPS][16], s_l[CA_WARPS][16], s_M[CA_WARPS][16];
+  __shared__ uint4 s_q[Q_SMEM ? NS * KS * 32 : 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   int* s_base = reinterpret_cast<int*>(dyn);  // [n_seqs] units of the sequences before s
   int* s_cut = s_base + a.n_seqs;             // [n_seqs] parts of cut items before s
-  float* s_o = reinterpret_cast<float*>(dyn);  // [warps][16][D], after the schedule has been read
+  int* s_len = s_cut + a.n_seqs;              // [n_seqs] tiles of an item of s
+  float* s_o = reinterpret_cast<float*>(dyn);  // [warps][16][D], after the rings
 
   // ---- schedule: every block derives the same one from the lengths
-  int2 all;
   int chunk;
   {
     long long mine = 0;
     for (int s = tid; s < a.n_seqs; s += CA_THREADS) {
       const SeqPlan p = plan_of(a, s);
-      mine += (long long)(p.n_window + p.n_lmk) * tiles_of(a, p.n_q) * a.Hkv;
+      const int items = row_tiles(a, p.n_q) * a.Hkv;
+      s_len[s] = p.n_window + p.n_lmk;
+      s_base[s] = items;
+      mine += (long long)s_len[s] * items;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    __shared__ long long s_sum[CA_WARPS];
     if (lane == 0) s_sum[warp] = mine;
     __syncthreads();
     const long long total = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-    chunk = (int)min(max((total + CA_TARGET - 1) / CA_TARGET, (long long)CA_MIN_GROUPS), 0x7fffffffLL);
+    constexpr int UNITS = Shape<D>::UNITS;
+    chunk = (int)min(max((total + UNITS - 1) / UNITS, (long long)CA_MIN_TILES), 0x7fffffffLL);
   }
   int2 carry = make_int2(0, 0);
   for (int base = 0; base < a.n_seqs; base += CA_THREADS) {
     const int s = base + tid;
-    int2 v = make_int2(0, 0);
+    int2 v = make_int2(0, 0), all;
     if (s < a.n_seqs) {
-      const SeqPlan p = plan_of(a, s);
-      const int splits = max(1, (p.n_window + p.n_lmk + chunk - 1) / chunk);
-      v.x = tiles_of(a, p.n_q) * a.Hkv * splits;
+      const int splits = max(1, (s_len[s] + chunk - 1) / chunk);
+      v.x = s_base[s] * splits;
       v.y = splits > 1 ? v.x : 0;
     }
     const int2 b = block_before2(v, red, all);
@@ -226,7 +241,7 @@ __global__ void __launch_bounds__(CA_THREADS) cache_attn_kernel(CacheAttnArgs a)
       }
       if (tid == 0) {
         if (a.lse) a.lse[r] = -INFINITY;
-        if (a.row_part) a.row_part[r] = make_int2(0, 1);
+        a.row_part[r] = make_int2(0, 1);
       }
     }
   }
@@ -242,32 +257,29 @@ __global__ void __launch_bounds__(CA_THREADS) cache_attn_kernel(CacheAttnArgs a)
     s = lo;
   }
   const SeqPlan p = plan_of(a, s);
-  const int groups = p.n_window + p.n_lmk, splits = max(1, (groups + chunk - 1) / chunk);
+  const int tiles = p.n_window + p.n_lmk, splits = max(1, (tiles + chunk - 1) / chunk);
   const int local = unit - s_base[s];
   const int split = local % splits, item = local / splits;
   const int hk = item % a.Hkv, tile = item / a.Hkv;
   const int part0 = s_cut[s] + item * splits;
-  const int each = (groups + splits - 1) / splits;
-  const int g_begin = split * each, g_end = min(g_begin + each, groups);
+  const int each = (tiles + splits - 1) / splits;
+  const int t_begin = min(split * each, tiles), t_end = min(t_begin + each, tiles);
 
   // ---- this lane's two query rows
   int row_lo[2], row_hi[2], row_head[2];
-  int64_t row_q[2];
   float row_f[2];
   bool row_ok[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    const int i = tile * 16 + g + r * 8, tok = i / a.G, h = hk * a.G + i % a.G;
+    const int i = tile * 16 + g + r * 8, tok = i / a.G;
     row_ok[r] = tok < p.n_q;
     const int pos = p.len - p.n_q + tok;
     const bool keys = row_ok[r] && pos >= 0;
     row_lo[r] = keys ? first_key(a, p.q0 + tok, pos) : 0x7fffffff;
     row_hi[r] = keys ? pos + 1 : 0;
     row_head[r] = i % a.G;
-    row_q[r] = (int64_t)(p.q0 + tok) * a.H + h;
-    row_f[r] = 0.f;
   }
-  uint32_t qa[NS][KS][4];
+  uint32_t qa[Q_SMEM ? 1 : KS][4];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     // 16 consecutive elements at 16 t of each 64
@@ -318,10 +330,15 @@ __global__ void __launch_bounds__(CA_THREADS) cache_attn_kernel(CacheAttnArgs a)
       for (int h = 0; h < 2; ++h) {
         const float lo = x[4 * k + 2 * h] * mul, hi = x[4 * k + 2 * h + 1] * mul;
         const uint32_t first = pack_f16x2(lo, hi);
-        qa[0][k][2 * h + r] = first;
-        if constexpr (NS == 2) {
-          const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&first));
-          qa[1][k][2 * h + r] = pack_f16x2(lo - b.x, hi - b.y);
+        if constexpr (!Q_SMEM) {
+          qa[k][2 * h + r] = first;
+        } else if (warp == 0) {
+          uint32_t* sq = reinterpret_cast<uint32_t*>(s_q);
+          sq[(k * 32 + lane) * 4 + 2 * h + r] = first;
+          if constexpr (NS == 2) {
+            const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&first));
+            sq[((KS + k) * 32 + lane) * 4 + 2 * h + r] = pack_f16x2(lo - b.x, hi - b.y);
+          }
         }
       }
   }
@@ -343,21 +360,21 @@ __global__ void __launch_bounds__(CA_THREADS) cache_attn_kernel(CacheAttnArgs a)
   RowState st[2] = {{-INFINITY, 0.f, -INFINITY}, {-INFINITY, 0.f, -INFINITY}};
   const int page_mask = (1 << a.page_shift) - 1;
   const int* table = a.tables + (int64_t)s * a.max_pages;
-  const int lmk16 = (a.k_lmk + 15) >> 4;
+  const int lmk32 = max((a.k_lmk + 31) >> 5, 1);
   bool bad_page = false;
 
-  // ---- this warp's share of the unit: a stretch of window groups, then one of landmark groups
-  const int w0 = min(g_begin, p.n_window), w1 = min(g_end, p.n_window);
-  const int l0 = max(g_begin - p.n_window, 0), l1 = max(g_end - p.n_window, 0);
+  // ---- this warp's share of the unit: a stretch of window tiles, then one of landmark tiles
+  const int w0 = min(t_begin, p.n_window), w1 = min(t_end, p.n_window);
+  const int l0 = max(t_begin - p.n_window, 0), l1 = max(t_end - p.n_window, 0);
   const int wq = (w1 - w0 + CA_WARPS - 1) / CA_WARPS, lq = (l1 - l0 + CA_WARPS - 1) / CA_WARPS;
   int wb = min(w0 + warp * wq, w1), we = min(wb + wq, w1);
   const int lb = min(l0 + warp * lq, l1), le = min(lb + lq, l1);
-  // (keys of the sequence's other tiles are passed over)
-  wb = max(wb, min(we, (lo_min < p.len ? lo_min - p.lo16 : 0x7ffffff0) >> 4));
-  we = min(we, max(wb, (hi_max - p.lo16 + 15) >> 4));
+  // (keys of the sequence's other row tiles are passed over)
+  wb = max(wb, min(we, (lo_min < p.len ? lo_min - p.lo32 : 0x7fffffe0) >> 5));
+  we = min(we, max(wb, (hi_max - p.lo32 + 31) >> 5));
   const int n_w = we - wb, n = n_w + le - lb;
 
-  // where keys lie: of 32 window groups ahead a lane each, of 2 landmark groups a lane per key
+  // where keys lie: of 16 window tiles ahead a lane per half, of the next landmark tile a lane per key
   struct Where {
     int row, key;
     float ks, ve, add;
@@ -378,20 +395,20 @@ __global__ void __launch_bounds__(CA_THREADS) cache_attn_kernel(CacheAttnArgs a)
       }
     }
   };
-  auto find_window = [&](int i) {  // lane: group wb + i + lane
+  auto find_window = [&](int i) {  // lane: half lane & 1 of tile wb + i + lane / 2
     Where o;
     o.add = 0.f;
-    o.key = i + lane < n_w ? p.lo16 + (wb + i + lane) * 16 : -1;
+    o.key = i + (lane >> 1) < n_w ? p.lo32 + (wb + i) * 32 + lane * 16 : -1;
     look_up(o.key, o);
     return o;
   };
-  auto find_lmk = [&](int i) {  // lane: key lane & 15 of group lb + i + (lane >> 4)
+  auto find_lmk = [&](int i) {  // lane: key `lane` of tile lb + i
     Where o;
     o.add = 0.f;
     o.key = -1;
-    const int l = lb + i + (lane >> 4), c = (l % max(lmk16, 1)) * 16 + (lane & 15);
+    const int l = lb + i, c = (l % lmk32) * 32 + lane;
     if (l < le && c < a.k_lmk) {
-      const int64_t at = ((int64_t)(hk * a.G + l / lmk16) * a.n_seqs + s) * a.k_lmk + c;
+      const int64_t at = ((int64_t)(hk * a.G + l / lmk32) * a.n_seqs + s) * a.k_lmk + c;
       o.key = a.lmk[at];
       if (a.bias) o.add = a.bias[at] * 1.4426950408889634f;
     }
@@ -399,62 +416,56 @@ __global__ void __launch_bounds__(CA_THREADS) cache_attn_kernel(CacheAttnArgs a)
     look_up(o.key, o);
     return o;
   };
-  Where ww = find_window(0), wn = ww, lw = ww, ln = ww;
-  if (n_w > 32) wn = find_window(32);
-  if (le > lb) {
-    lw = find_lmk(0);
-    ln = find_lmk(2);
-  }
+  Where ww = find_window(0), wn = ww, ln = ww;
+  if (n_w > 16) wn = find_window(16);
+  if (le > lb) ln = find_lmk(0);
   uint8_t* ring = dyn + warp * (STAGES * Stage<D>::BYTES);
   const uint32_t ring_s = smem_u32(ring);
+  int in_stage = 0, out_stage = 0;  // byte offsets of the stages written and read next
+  constexpr int CPR = D / 16, RPI = 32 / CPR;  // 16-byte chunks per row, rows per step of the warp
+  const int my_row = lane / CPR, my_chunk = lane % CPR;
   auto issue = [&](int i) {
-    const uint32_t st_s = ring_s + (i % STAGES) * Stage<D>::BYTES;
-    uint8_t* st_p = ring + (i % STAGES) * Stage<D>::BYTES;
     if (i < n) {
-      const bool window = i < n_w;
-      int row, key;  // of slot lane & 15
-      float ks, ve, add;
-      if (window) {
-        const int b = i & 31;
+      const uint32_t st_s = ring_s + in_stage;
+      float4* meta = reinterpret_cast<float4*>(ring + in_stage + Stage<D>::META);
+      if (i < n_w) {
+        const int b = i & 15;
         if (b == 0 && i > 0) {
           ww = wn;
-          if (i + 32 < n_w) wn = find_window(i + 32);
+          if (i + 16 < n_w) wn = find_window(i + 16);
         }
-        row = __shfl_sync(0xffffffffu, ww.row, b);
-        key = __shfl_sync(0xffffffffu, ww.key, b) + (lane & 15);
-        ks = __shfl_sync(0xffffffffu, ww.ks, b);
-        ve = __shfl_sync(0xffffffffu, ww.ve, b);
-        add = 0.f;
-        row = row >= 0 && key < p.len ? row + (lane & 15) : -1;
-      } else {
-        const int li = i - n_w, b = li & 1;
-        if (b == 0 && li > 0) {
-          lw = ln;
-          if (lb + li + 2 < le) ln = find_lmk(li + 2);
-        }
-        const int from = b * 16 + (lane & 15);
-        row = __shfl_sync(0xffffffffu, lw.row, from);
-        key = __shfl_sync(0xffffffffu, lw.key, from);
-        ks = __shfl_sync(0xffffffffu, lw.ks, from);
-        ve = __shfl_sync(0xffffffffu, lw.ve, from);
-        add = __shfl_sync(0xffffffffu, lw.add, from);
-      }
-      if (lane < 16)
-        *reinterpret_cast<float4*>(st_p + Stage<D>::META + lane * 16) =
-            make_float4(ks, ve, add, __int_as_float(row >= 0 ? key : -1));
-      constexpr int CPR = D / 16, RPI = 32 / CPR;  // chunks per row, rows per step
+        if ((lane >> 1) == b)
+          meta[(lane & 1) * 16] = make_float4(ww.ks, ww.ve, 0.f, __int_as_float(ww.row >= 0 ? ww.key : -1));
+        const int key = __shfl_sync(0xffffffffu, ww.key, 2 * b);
 #pragma unroll
-      for (int x = 0; x < 16 / RPI; ++x) {
-        const int r = x * RPI + lane / CPR, c = lane % CPR;
-        const int rr = __shfl_sync(0xffffffffu, row, r);
-        const int64_t at = (int64_t)max(rr, 0) * D + c * 16;
-        copy16(st_s + Stage<D>::k_at(r, c), a.kc + at, rr >= 0);
-        copy16(st_s + Stage<D>::v_at(r, c), a.vc + at, rr >= 0);
+        for (int h = 0; h < 2; ++h) {
+          const int row = __shfl_sync(0xffffffffu, ww.row, 2 * b + h);
+          const int left = row < 0 ? 0 : p.len - key - h * 16;  // rows from here that hold keys
+          const int64_t at = (int64_t)max(row, 0) * D + lane * 16;
+#pragma unroll
+          for (int x = 0; x < 16 / RPI; ++x) {
+            const int r = x * RPI + my_row;
+            copy16(st_s + Stage<D>::k_at(h * 16 + r, my_chunk), a.kc + at + x * 512, r < left);
+            copy16(st_s + Stage<D>::v_at(h * 16 + r, my_chunk), a.vc + at + x * 512, r < left);
+          }
+        }
+      } else {
+        const Where lw = ln;
+        if (i + 1 < n) ln = find_lmk(i + 1 - n_w);
+        meta[lane] = make_float4(lw.ks, lw.ve, lw.add, __int_as_float(lw.row >= 0 ? lw.key : -1));
+#pragma unroll
+        for (int x = 0; x < 32 / RPI; ++x) {
+          const int r = x * RPI + my_row, row = __shfl_sync(0xffffffffu, lw.row, r);
+          const int64_t at = (int64_t)max(row, 0) * D + my_chunk * 16;
+          copy16(st_s + Stage<D>::k_at(r, my_chunk), a.kc + at, row >= 0);
+          copy16(st_s + Stage<D>::v_at(r, my_chunk), a.vc + at, row >= 0);
+        }
       }
+      in_stage = in_stage == (STAGES - 1) * Stage<D>::BYTES ? 0 : in_stage + Stage<D>::BYTES;
     }
     copies_commit();
   };
-  __syncthreads();  // the schedule's memory becomes the ring
+  __syncthreads();  // Q is in place; the schedule's memory becomes the rings
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) issue(i);
 
@@ -462,54 +473,120 @@ __global__ void __launch_bounds__(CA_THREADS) cache_attn_kernel(CacheAttnArgs a)
     copies_wait<STAGES - 2>();
     __syncwarp();  // every lane's copies of stage i are there, and stage i - 1 is read
     issue(i + STAGES - 1);
-    const uint8_t* stage = ring + (i % STAGES) * Stage<D>::BYTES;
+    const uint8_t* stage = ring + out_stage;
+    out_stage = out_stage == (STAGES - 1) * Stage<D>::BYTES ? 0 : out_stage + Stage<D>::BYTES;
+    const float4* meta = reinterpret_cast<const float4*>(stage + Stage<D>::META);
     const bool window = i < n_w;
-    float4 meta[4];  // keys t, t + 4, t + 8, t + 12: columns 2t, 2t + 1 of half 0, then of half 1
-#pragma unroll
-    for (int x = 0; x < 4; ++x) meta[x] = *reinterpret_cast<const float4*>(stage + Stage<D>::META + (t + 4 * x) * 16);
     // ---- S = Q K^T
-    float sc[2][4];
+    float sc[4][4];
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
-      sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+    for (int nt = 0; nt < 4; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
 #pragma unroll
-      for (int b = 0; b < D / 64; ++b) {
+    for (int b = 0; b < D / 64; ++b) {
+      uint32_t kr[4][4];
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt) {
         const uint4 kw = *reinterpret_cast<const uint4*>(stage + Stage<D>::k_at(slot_of(nt, g), b * 4 + t));
-        const uint32_t kr[4] = {kw.x, kw.y, kw.z, kw.w};
+        kr[nt][0] = kw.x, kr[nt][1] = kw.y, kr[nt][2] = kw.z, kr[nt][3] = kw.w;
+      }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t b0 = widen_lo(kr[k]), b1 = widen_hi(kr[k]);
+      for (int k = 0; k < 4; ++k)
 #pragma unroll
-          for (int x = 0; x < NS; ++x) {
-            const uint32_t(&q4)[4] = qa[x][b * 4 + k];
-            mma_f16(sc[nt], q4[0], q4[1], q4[2], q4[3], b0, b1);
+        for (int x = 0; x < NS; ++x) {
+          uint32_t q4[4];
+          if constexpr (Q_SMEM) {
+            const uint4 y = s_q[(x * KS + b * 4 + k) * 32 + lane];
+            q4[0] = y.x, q4[1] = y.y, q4[2] = y.z, q4[3] = y.w;
+          } else {
+            q4[0] = qa[b * 4 + k][0], q4[1] = qa[b * 4 + k][1], q4[2] = qa[b * 4 + k][2], q4[3] = qa[b * 4 + k][3];
+          }
+#pragma unroll
+          for (int nt = 0; nt < 4; ++nt)
+            mma_f16(sc[nt], q4[0], q4[1], q4[2], q4[3], widen_lo(kr[nt][k]), widen_hi(kr[nt][k]));
+        }
+    }
+    // ---- P = 2^(x + e - M + 14), l += 2^(x - m)
+    const int key0 = p.lo32 + (wb + i) * 32;
+    const float4 mh[2] = {meta[0], meta[16]};  // of a window tile's halves
+    bool plain = window && key0 >= lo_max && key0 + 32 <= hi_min && __float_as_int(mh[0].w) >= 0 &&
+                 __float_as_int(mh[1].w) >= 0;
+    uint32_t valid = 0xffff;  // bit 4 nt + 2 r + c: row r attends to column c of block nt
+    if (plain) {
+      // m and M are references here, not exact maxima: they move when a logit passes them by
+      // the slack. One exponential per element: the sum of P is brought to l's reference.
+      float f[2][2], lm[2][2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          f[r][h] = mh[h].x * row_f[r];
+          lm[r][h] = f[r][h] * fmaxf(fmaxf(sc[2 * h][2 * r], sc[2 * h][2 * r + 1]), fmaxf(sc[2 * h + 1][2 * r], sc[2 * h + 1][2 * r + 1]));
+        }
+      bool over = false;
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        over |= fmaxf(lm[r][0], lm[r][1]) > st[r].m + CA_SLACK || fmaxf(lm[r][0] + mh[0].y, lm[r][1] + mh[1].y) > st[r].M + CA_SLACK;
+      if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float gm = fmaxf(lm[r][0], lm[r][1]), gM = fmaxf(lm[r][0] + mh[0].y, lm[r][1] + mh[1].y);
+          gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 1));
+          gM = fmaxf(gM, __shfl_xor_sync(0xffffffffu, gM, 1));
+          gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 2));
+          gM = fmaxf(gM, __shfl_xor_sync(0xffffffffu, gM, 2));
+          const float m = fmaxf(st[r].m, gm), M = fmaxf(st[r].M, gM);
+          st[r].l *= m == -INFINITY ? 1.f : exp2_fast(st[r].m - m);
+          const float c = M == -INFINITY ? 1.f : exp2_fast(st[r].M - M);
+          st[r].m = m;
+          st[r].M = M;
+#pragma unroll
+          for (int x = 0; x < NT; ++x) {
+            o[x][2 * r] *= c;
+            o[x][2 * r + 1] *= c;
           }
         }
       }
-    }
-    // ---- logits (base 2); columns that a row does not attend to become -inf
-    const int key0 = p.lo16 + (wb + i) * 16;
-    const bool plain = window && key0 >= lo_max && key0 + 16 <= hi_min && __float_as_int(meta[0].w) >= 0;
-    uint32_t valid = 0xff;  // bit 4 nt + 2 r + c: row r attends to column c of half nt
-    if (plain) {
+      // where V's scale is so small that P of a logit near m would vanish, l needs its own
+      // exponentials: the general path
+      const float e_min = fminf(mh[0].y, mh[1].y);
+      plain = !__any_sync(0xffffffffu, !(st[0].m + e_min - st[0].M > -90.f) || !(st[1].m + e_min - st[1].M > -90.f));
+      if (plain) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float f = meta[0].x * row_f[r];
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          sc[nt][2 * r] *= f;
-          sc[nt][2 * r + 1] *= f;
-        }
+          for (int h = 0; h < 2; ++h) {
+            const float shift = mh[h].y - st[r].M + CA_P_SHIFT;
+            float sum = 0.f;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                float& y = sc[2 * h + x][2 * r + c];
+                y = exp2_fast(fmaf(y, f[r][h], shift));
+                sum += y;
+              }
+            st[r].l = fmaf(sum, exp2_fast(-shift - st[r].m), st[r].l);
+          }
+      } else {
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[nt][e] *= f[e >> 1][nt >> 1];
       }
     } else {
       valid = 0;
-      const int head = window ? -1 : (lb + i - n_w) / lmk16;
+      const int head = window ? -1 : (lb + i - n_w) / lmk32;
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
+      for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const float4 mt = meta[2 * nt + c];
-          const int key = __float_as_int(mt.w);
+          const int slot = (nt >> 1) * 16 + (nt & 1) * 8 + t + 4 * c;
+          const float4 mt = window ? mh[nt >> 1] : meta[slot];
+          int key = __float_as_int(mt.w);
+          if (window && key >= 0) {
+            key += slot & 15;
+            if (key >= p.len) key = -1;
+          }
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const bool ok = key >= 0 && (window ? key >= row_lo[r] && key < row_hi[r]
@@ -519,128 +596,128 @@ __global__ void __launch_bounds__(CA_THREADS) cache_attn_kernel(CacheAttnArgs a)
           }
         }
     }
-    // ---- online softmax with the two maxima
-    float gm[2], gM[2];
+    if (!plain) {
+      float ve[4][2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      gm[r] = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
-      gm[r] = fmaxf(gm[r], __shfl_xor_sync(0xffffffffu, gm[r], 1));
-      gm[r] = fmaxf(gm[r], __shfl_xor_sync(0xffffffffu, gm[r], 2));
-      if (window) {
-        gM[r] = gm[r] + meta[0].y;
-      } else {
-        gM[r] = fmaxf(fmaxf(sc[0][2 * r] + meta[0].y, sc[0][2 * r + 1] + meta[1].y),
-                      fmaxf(sc[1][2 * r] + meta[2].y, sc[1][2 * r + 1] + meta[3].y));
-        gM[r] = fmaxf(gM[r], __shfl_xor_sync(0xffffffffu, gM[r], 1));
-        gM[r] = fmaxf(gM[r], __shfl_xor_sync(0xffffffffu, gM[r], 2));
-      }
-    }
-    if (__any_sync(0xffffffffu, gm[0] > st[0].m || gm[1] > st[1].m || gM[0] > st[0].M || gM[1] > st[1].M)) {
+      for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          ve[nt][c] = window ? mh[nt >> 1].y : meta[(nt >> 1) * 16 + (nt & 1) * 8 + t + 4 * c].y;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float m = fmaxf(st[r].m, gm[r]), M = fmaxf(st[r].M, gM[r]);
-        st[r].l *= m == -INFINITY ? 1.f : exp2_fast(st[r].m - m);
-        const float c = M == -INFINITY ? 1.f : exp2_fast(st[r].M - M);
-        st[r].m = m;
-        st[r].M = M;
+        float gm = -INFINITY, gM = -INFINITY;
 #pragma unroll
-        for (int x = 0; x < NT; ++x) {
-          o[x][2 * r] *= c;
-          o[x][2 * r + 1] *= c;
+        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            gm = fmaxf(gm, sc[nt][2 * r + c]);
+            gM = fmaxf(gM, sc[nt][2 * r + c] + ve[nt][c]);
+          }
+        gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 1));
+        gM = fmaxf(gM, __shfl_xor_sync(0xffffffffu, gM, 1));
+        gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 2));
+        gM = fmaxf(gM, __shfl_xor_sync(0xffffffffu, gM, 2));
+        const float m = fmaxf(st[r].m, gm), M = fmaxf(st[r].M, gM);
+        const float mu = m == -INFINITY ? 0.f : m, Mu = M == -INFINITY ? 0.f : M;
+        float l = st[r].l * exp2_fast(st[r].m - mu);
+        const float corr = exp2_fast(st[r].M - Mu);
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float x = sc[nt][2 * r + c];
+            l += exp2_fast(x - mu);
+            sc[nt][2 * r + c] = exp2_fast(x + ve[nt][c] - Mu + CA_P_SHIFT);
+          }
+        st[r] = {m, l, M};
+        if (__any_sync(0xffffffffu, corr != 1.f)) {
+#pragma unroll
+          for (int x = 0; x < NT; ++x) {
+            o[x][2 * r] *= corr;
+            o[x][2 * r + 1] *= corr;
+          }
         }
       }
     }
-    float pr[2][4];
+    // ---- O += P V, 16 keys at a time
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const float mu = st[r].m == -INFINITY ? 0.f : st[r].m, Mu = st[r].M == -INFINITY ? 0.f : st[r].M;
-      // 2^(x + e - M) = 2^(x - m) 2^(m + e - M); where the second factor is large the first is small
-      const float f = exp2_fast(fminf(mu - Mu + meta[0].y + CA_P_SHIFT, 126.f));
+    for (int h = 0; h < 2; ++h) {
+      uint32_t pa[NS][4];
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float x = sc[nt][2 * r + c], e = exp2_fast(x - mu);
-          st[r].l += e;
-          pr[nt][2 * r + c] = window ? e * f : exp2_fast(x + meta[2 * nt + c].y - Mu + CA_P_SHIFT);
+      for (int x = 0; x < 4; ++x) {
+        const float lo = sc[2 * h + (x >> 1)][2 * (x & 1)], hi = sc[2 * h + (x >> 1)][2 * (x & 1) + 1];
+        pa[0][x] = pack_f16x2(lo, hi);
+        if constexpr (NS == 2) {
+          const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&pa[0][x]));
+          pa[1][x] = pack_f16x2(lo - b.x, hi - b.y);
         }
-    }
-    // ---- O += P V
-    uint32_t pa[NS][4];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int nt = x >> 1, r = x & 1;
-      const float lo = pr[nt][2 * r], hi = pr[nt][2 * r + 1];
-      pa[0][x] = pack_f16x2(lo, hi);
-      if constexpr (NS == 2) {
-        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&pa[0][x]));
-        pa[1][x] = pack_f16x2(lo - b.x, hi - b.y);
       }
-    }
-    uint32_t v[4][D / 32];
+      uint32_t v[4][D / 32];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      if constexpr (D == 64) {
-        const uint2 y = *reinterpret_cast<const uint2*>(stage + Stage<D>::v_at(t + 4 * x, g >> 1) + (g & 1) * 8);
-        v[x][0] = y.x, v[x][1] = y.y;
-      } else {
-        const uint4 y = *reinterpret_cast<const uint4*>(stage + Stage<D>::v_at(t + 4 * x, g));
-        v[x][0] = y.x, v[x][1] = y.y, v[x][2] = y.z, v[x][3] = y.w;
+      for (int x = 0; x < 4; ++x) {
+        const int r = h * 16 + t + 4 * x;
+        if constexpr (D == 64) {
+          const uint2 y = *reinterpret_cast<const uint2*>(stage + Stage<D>::v_at(r, g >> 1) + (g & 1) * 8);
+          v[x][0] = y.x, v[x][1] = y.y;
+        } else {
+          const uint4 y = *reinterpret_cast<const uint4*>(stage + Stage<D>::v_at(r, g));
+          v[x][0] = y.x, v[x][1] = y.y, v[x][2] = y.z, v[x][3] = y.w;
+        }
       }
-    }
-    bool nans = false;
-    if (!plain) {
+      bool nans = false;
+      if (valid != 0xffff) {  // differs from lane to lane
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
+        for (int x = 0; x < 4; ++x)
 #pragma unroll
-        for (int y = 0; y < D / 32; ++y) nans |= nan_bytes(v[x][y]) != 0;
-      nans = __any_sync(0xffffffffu, nans);
-    }
-    if (nans) {
-      // P = 0 must not spread a NaN: count, per row and channel, the NaNs among the keys that the row
-      // attends to (a product of ones), and take the NaNs themselves out
-      uint32_t va[4];
+          for (int y = 0; y < D / 32; ++y) nans |= nan_bytes(v[x][y]) != 0;
+      }
+      if (__any_sync(0xffffffffu, nans)) {
+        // P = 0 must not spread a NaN: count, per row and channel, the NaNs among the keys that the
+        // row attends to (a product of ones), and take the NaNs themselves out
+        uint32_t va[4];
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        va[x] = (valid >> (4 * (x >> 1) + 2 * (x & 1)) & 1 ? 0x3c00u : 0u) |
-                (valid >> (4 * (x >> 1) + 2 * (x & 1) + 1) & 1 ? 0x3c000000u : 0u);
-#pragma unroll
-      for (int x = 0; x < D / 32; ++x) {
-        uint32_t nb[4];
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          nb[y] = nan_bytes(v[y][x]);
-          v[y][x] &= ~nb[y];
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t bits = valid >> (4 * (2 * h + (x >> 1)) + 2 * (x & 1));
+          va[x] = (bits & 1 ? 0x3c00u : 0u) | (bits & 2 ? 0x3c000000u : 0u);
         }
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
+        for (int x = 0; x < D / 32; ++x) {
+          uint32_t nb[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            nb[y] = nan_bytes(v[y][x]);
+            v[y][x] &= ~nb[y];
+          }
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              const uint32_t sel = y ? 0x7362 : 0x5140, half = z ? 0x3322 : 0x1100;
+              const uint32_t m0 = __byte_perm(__byte_perm(nb[0], nb[1], sel), 0, half);  // 0xffff per NaN
+              const uint32_t m1 = __byte_perm(__byte_perm(nb[2], nb[3], sel), 0, half);
+              float cnt[4] = {0.f, 0.f, 0.f, 0.f};
+              mma_f16(cnt, va[0], va[1], va[2], va[3], m0 & 0x3c003c00u, m1 & 0x3c003c00u);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (cnt[e] > 0.f) o[4 * x + 2 * y + z][e] = __int_as_float(0x7fffffff);
+            }
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const uint32_t sel = y ? 0x7362 : 0x5140;
+          const uint32_t b0 = __byte_perm(v[0][x], v[1][x], sel), b1 = __byte_perm(v[2][x], v[3][x], sel);
 #pragma unroll
           for (int z = 0; z < 2; ++z) {
-            const uint32_t sel = y ? 0x7362 : 0x5140, half = z ? 0x3322 : 0x1100;
-            const uint32_t m0 = __byte_perm(__byte_perm(nb[0], nb[1], sel), 0, half);  // 0xffff per NaN
-            const uint32_t m1 = __byte_perm(__byte_perm(nb[2], nb[3], sel), 0, half);
-            float cnt[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_f16(cnt, va[0], va[1], va[2], va[3], m0 & 0x3c003c00u, m1 & 0x3c003c00u);
+            const uint32_t h0 = z ? widen_hi(b0) : widen_lo(b0), h1 = z ? widen_hi(b1) : widen_lo(b1);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (cnt[e] > 0.f) o[4 * x + 2 * y + z][e] = __int_as_float(0x7fffffff);
+            for (int q4 = 0; q4 < NS; ++q4)
+              mma_f16(o[4 * x + 2 * y + z], pa[q4][0], pa[q4][1], pa[q4][2], pa[q4][3], h0, h1);
           }
-      }
-    }
-#pragma unroll
-    for (int x = 0; x < D / 32; ++x)
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const uint32_t sel = y ? 0x7362 : 0x5140;
-        const uint32_t b0 = __byte_perm(v[0][x], v[1][x], sel), b1 = __byte_perm(v[2][x], v[3][x], sel);
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const uint32_t h0 = z ? widen_hi(b0) : widen_lo(b0), h1 = z ? widen_hi(b1) : widen_lo(b1);
-#pragma unroll
-          for (int q4 = 0; q4 < NS; ++q4)
-            mma_f16(o[4 * x + 2 * y + z], pa[q4][0], pa[q4][1], pa[q4][2], pa[q4][3], h0, h1);
         }
-      }
+    }
   }
   if (bad_page) report_device_error(a.err, CA_ERR_PAGE);
 
@@ -690,7 +767,7 @@ __global__ void __launch_bounds__(CA_THREADS) cache_attn_kernel(CacheAttnArgs a)
       else reinterpret_cast<__half*>(a.out)[row * D + d] = __float2half_rn(res);
       if (d == 0) {
         if (a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-        if (a.row_part) a.row_part[row] = make_int2(0, 1);
+        a.row_part[row] = make_int2(0, 1);
       }
     } else {
       const int64_t part = part0 + split;
@@ -712,7 +789,7 @@ __global__ void __launch_bounds__(128) cache_attn_join_kernel(CacheAttnArgs a) {
   const int64_t row = blockIdx.x;
   const int2 rp = a.row_part[row];
   // one part: already written. Anything else than parts of this call: a row of no sequence.
-  if (rp.y <= 1 || rp.x < 0 || rp.y > 2 * CA_TARGET || rp.x / 16 + rp.y > 2 * CA_TARGET) return;
+  if (rp.y <= 1 || rp.x < 0 || rp.y > 2 * CA_MAX_UNITS || rp.x / 16 + rp.y > 2 * CA_MAX_UNITS) return;
   __shared__ float s_red[8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const float* ps = a.part_s + (int64_t)rp.x * 4;
@@ -750,15 +827,14 @@ static inline int64_t ca_items(int64_t T, int n_seqs, int G, int Hkv) { return (
 
 template <typename T, int D, int NS>
 static int launch_cache_attn(const CacheAttnArgs& a, unsigned grid, bool join, cudaStream_t stream) {
-  constexpr int STAGES = D == 64 ? 6 : 4;
-  constexpr size_t RING = (size_t)CA_WARPS * STAGES * Stage<D>::BYTES;
+  constexpr size_t RING = (size_t)CA_WARPS * Shape<D>::STAGES * Stage<D>::BYTES, TABLES = 3 * sizeof(int);
   static_assert(RING >= sizeof(float) * CA_WARPS * 16 * D, "the parts take the rings' place");
-  const size_t tables = 2 * sizeof(int) * (size_t)a.n_seqs, smem = tables > RING ? tables : RING;
+  const size_t smem = TABLES * (size_t)a.n_seqs > RING ? TABLES * (size_t)a.n_seqs : RING;
   static std::atomic<uint64_t> ready{0};
-  if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(cache_attn_kernel<T, D, NS, STAGES>),
-                                  (int)(2 * sizeof(int) * CA_MAX_SEQS > RING ? 2 * sizeof(int) * CA_MAX_SEQS : RING), ready))
+  if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(cache_attn_kernel<T, D, NS>),
+                                  (int)(TABLES * CA_MAX_SEQS > RING ? TABLES * CA_MAX_SEQS : RING), ready))
     return rc;
-  cache_attn_kernel<T, D, NS, STAGES><<<grid, CA_THREADS, smem, stream>>>(a);
+  cache_attn_kernel<T, D, NS><<<grid, CA_THREADS, smem, stream>>>(a);
   if (int rc = check_cuda(cudaGetLastError(), "cache_attention launch")) return rc;
   if (!join) return DSALT_OK;
   cudaLaunchAttribute attr[1];
@@ -782,8 +858,8 @@ extern "C" {
 size_t dsalt_cache_attention_workspace_bytes(int64_t T, int n_seqs, int n_heads, int n_kv, int head_dim) {
   if (T < 0 || n_seqs < 1 || n_heads < 1 || n_kv < 1 || head_dim < 1) return 0;
   // a cut item has at least two units of at least half the wanted length: at most twice the target
-  return ca_a256(sizeof(int2) * (size_t)T * n_heads) + ca_a256(sizeof(float) * 2 * CA_TARGET * 64) +
-         ca_a256(sizeof(float) * 2 * CA_TARGET * 16 * (size_t)head_dim);
+  return ca_a256(sizeof(int2) * (size_t)T * n_heads) + ca_a256(sizeof(float) * 2 * CA_MAX_UNITS * 64) +
+         ca_a256(sizeof(float) * 2 * CA_MAX_UNITS * 16 * (size_t)head_dim);
 }
 
 int dsalt_cache_attention(const void* q, int dtype, int64_t T, int n_heads, int n_kv, int head_dim, int64_t q_stride,
@@ -831,15 +907,15 @@ int dsalt_cache_attention(const void* q, int dtype, int64_t T, int n_heads, int 
   a.row_part = reinterpret_cast<int2*>(ws);
   ws += ca_a256(sizeof(int2) * (size_t)T * n_heads);
   a.part_s = reinterpret_cast<float*>(ws);
-  ws += ca_a256(sizeof(float) * 2 * CA_TARGET * 64);
+  ws += ca_a256(sizeof(float) * 2 * CA_MAX_UNITS * 64);
   a.part_o = reinterpret_cast<float*>(ws);
   a.err = device_status_ptr();
   const int64_t items = ca_items(T, n_seqs, a.G, n_kv);
-  const int64_t grid = items + CA_TARGET;
+  const int64_t grid = items + CA_MAX_UNITS;
   if (grid > 0x7fffff00LL) return fail(DSALT_ERR_UNSUPPORTED, "cache_attention: too many rows");
   // tables too short for any item to be cut: nothing to join
-  const int64_t most = ((int64_t)max_pages * page_size >> 4) + (int64_t)a.G * ((k_lmk + 15) >> 4);
-  const bool join = most > CA_MIN_GROUPS;
+  const int64_t most = (((int64_t)max_pages * page_size + 31) >> 5) + (int64_t)a.G * ((k_lmk + 31) >> 5);
+  const bool join = most > CA_MIN_TILES;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
 #define DSALT_CA(TT, NS)                                                              \
   (head_dim == 64 ? launch_cache_attn<TT, 64, NS>(a, (unsigned)grid, join, st)        \
