@@ -6,23 +6,24 @@
 // v_j; without widths A = [0, i]. k_j = byte * 2^e of its page and kv head, v_j likewise.
 //
 // Bytes decide: 2 D per key and kv head are read once and give 4 D * (query rows of the kv
-// head) operations, far below what the tensor cores do in that time. So every query row that
-// shares a kv head (the heads of a group, the tokens of a draft) goes into one 16-row tile of
-// mma.sync m16n8k16, whose operands can be built in registers straight from global loads:
+// head) operations, far below what the tensor cores do in that time; what has to be kept
+// small are the instructions per byte. Eight query rows that share a kv head (the heads of a
+// group, the tokens of a draft) are the narrow side of mma.sync m16n8k16, the keys and the
+// channels the wide one: S^T = K Q^T (16 keys x 8 rows), O^T = V^T P^T (16 channels x 8 rows),
+// with operands built in registers:
 // * an e4m3 value is exact in fp16, so K and V are widened exactly; Q is scaled by a power of
 //   two per row to a largest magnitude in [2^13, 2^14), which keeps bf16 and fp16 values
 //   exact (those below 2^-27 of the row's largest fall short, under fp32's own rounding);
 // * the contraction order of a product is free, so lane (g, t) takes 16 consecutive bytes of
-//   one key for Q K^T and the D/8 bytes at D/8 g of four keys for P V, as they lie in the
-//   cache: no transposition, no shuffles of data;
-// * P is rounded to fp16 relative to the row's largest p * 2^e (half a step is 2^-12, under
-//   the 2^-9 of a bf16 result and as large as an fp16 result's own); fp32 queries take Q and
-//   P as two fp16 terms each (22 bits).
+//   a key for K Q^T and the D/8 bytes at D/8 g of four keys for V^T P^T, as they lie in the
+//   cache; P alone is transposed, two movmatrix per 16 keys;
+// * P is rounded to fp16 relative to the row's largest p * 2^e (half a step is 2^-11 of a
+//   term, errors of either sign); fp32 queries take Q and P as two fp16 terms each (22 bits).
 // The scales of V differ from page to page, so a row keeps two maxima: m of x for the
 // denominator l = sum 2^(x - m), and M of x + e for the numerator O = sum 2^(x + e - M) byte;
 // out = O 2^(M - m) / l. Neither can overflow whatever the scales are.
 //
-// The keys of an item (sequence, kv head, tile of 16 rows) are a list of tiles of 32: the
+// The keys of an item (sequence, kv head, tile of 8 rows) are a list of tiles of 32: the
 // window's, then the landmarks' of each head. Items are cut into units of about equal
 // length, by the lengths found on the device (no host copy of them is needed and a captured
 // call follows them); the parts of an item that was cut are joined by a second kernel.
@@ -43,13 +44,20 @@ constexpr float CA_P_SHIFT = 14.f;     // P is held times 2^14: fp16 stays norma
 constexpr float CA_SLACK = 1.f;        // P may exceed 2^14 by 2^1 before its reference moves (fp16 ends at 2^16)
 
 // blocks per SM that registers and rings allow; one round of them is the number of units wanted
+#ifndef O64
+#define O64 4
+#define S64 3
+#define O128 3
+#define S128 2
+#endif
 template <int D>
 struct Shape {
-  static constexpr int OCC = D == 64 ? 4 : 2;
-  static constexpr int STAGES = 3;
-  static constexpr int UNITS = 148 * OCC;
+  static constexpr int OCC = D == 64 ? O64 : O128;
+  static constexpr int STAGES = D == 64 ? S64 : S128;
+  static constexpr int SLOTS = 148 * OCC;
 };
-constexpr int CA_MAX_UNITS = 148 * 4;
+constexpr int CA_ROWS = 8;
+constexpr int CA_MAX_SLOTS = 148 * 8;
 
 struct CacheAttnArgs {
   const void* q;
@@ -65,8 +73,8 @@ struct CacheAttnArgs {
   void* out;
   int out_dtype;
   float* lse;
-  float* part_o;   // [cut units][16][D]
-  float* part_s;   // [cut units][16][4]: m, l, M
+  float* part_o;   // [cut units][8][D]
+  float* part_s;   // [cut units][8][4]: m, l, M
   int2* row_part;  // [T * H] first part of the row and how many there are
   int* err;
 };
@@ -132,7 +140,7 @@ __device__ __forceinline__ SeqPlan plan_of(const CacheAttnArgs& a, int s) {
   p.n_lmk = a.k_lmk > 0 && top > 0 ? a.G * ((a.k_lmk + 31) >> 5) : 0;  // none lies before a window from 0
   return p;
 }
-__device__ __forceinline__ int row_tiles(const CacheAttnArgs& a, int n_q) { return (n_q * a.G + 15) >> 4; }
+__device__ __forceinline__ int row_tiles(const CacheAttnArgs& a, int n_q) { return (n_q * a.G + CA_ROWS - 1) / CA_ROWS; }
 
 // sums of two numbers over the block's 128 threads, exclusive; totals in `all`
 __device__ __forceinline__ int2 block_before2(int2 v, int2* red, int2& all) {
@@ -169,9 +177,15 @@ struct Stage {
     return V + (D == 64 ? r * 64 + ((c ^ (r & 2)) * 16) : r * 128 + ((c ^ (r & 3) << 1) * 16));
   }
 };
-// Which key of the tile is column n of block nt of S: so chosen that lane t's P columns 2t,
-// 2t+1 of blocks 2h, 2h+1 are keys t, t+4, t+8, t+12 of half h, whose V rows lie together.
-__device__ __forceinline__ int slot_of(int nt, int n) { return nt * 8 + (n >> 1) + 4 * (n & 1); }
+// Which key of eight is row n of S^T: so chosen that the keys 2t, 2t+1 (and 8 on) of P^T that
+// lane t contracts are t, t+4 (and 8 on), whose V rows lie together.
+__device__ __forceinline__ int slot_of(int n) { return (n >> 1) + 4 * (n & 1); }
+// transposes an 8 x 8 matrix of 16-bit values: lane (g, t) gives [g][2t, 2t+1] and gets [2t, 2t+1][g]
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t v) {  // 0xff where a byte is an e4m3 NaN
   return __vcmpeq4(v & 0x7f7f7f7fu, 0x7f7f7f7fu);
@@ -179,38 +193,45 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t v) {  // 0xff where a byt
 
 // NS: fp16 terms that Q and P are held in (2 for fp32 queries)
 template <typename T, int D, int NS>
-__global__ void __launch_bounds__(CA_THREADS, NS == 1 ? Shape<D>::OCC : 1) cache_attn_kernel(CacheAttnArgs a) {
-  constexpr int KS = D / 16, NT = D / 8, STAGES = Shape<D>::STAGES;
-  constexpr bool Q_SMEM = D == 128 || NS == 2;  // registers hold Q only where there is room beside O
+__global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(CacheAttnArgs a) {
+  constexpr int KS = D / 16, MT = D / 16, STAGES = Shape<D>::STAGES;
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ int2 red[CA_WARPS];
-  __shared__ long long s_sum[CA_WARPS];
-  __shared__ float s_m[CA_WARPS][16], s_l[CA_WARPS][16], s_M[CA_WARPS][16];
-  __shared__ uint4 s_q[Q_SMEM ? NS * KS * 32 : 1];
+  __shared__ long long s_sum[CA_WARPS][2];
+  __shared__ float s_m[CA_WARPS][CA_ROWS], s_l[CA_WARPS][CA_ROWS], s_M[CA_WARPS][CA_ROWS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   int* s_base = reinterpret_cast<int*>(dyn);  // [n_seqs] units of the sequences before s
   int* s_cut = s_base + a.n_seqs;             // [n_seqs] parts of cut items before s
   int* s_len = s_cut + a.n_seqs;              // [n_seqs] tiles of an item of s
-  float* s_o = reinterpret_cast<float*>(dyn);  // [warps][16][D], after the rings
+  float* s_o = reinterpret_cast<float*>(dyn);  // [warps][8][D], after the rings
 
   // ---- schedule: every block derives the same one from the lengths
   int chunk;
   {
-    long long mine = 0;
+    // tiles and items of the call; both stay below 2^40
+    long long mine = 0, count = 0;
     for (int s = tid; s < a.n_seqs; s += CA_THREADS) {
       const SeqPlan p = plan_of(a, s);
       const int items = row_tiles(a, p.n_q) * a.Hkv;
       s_len[s] = p.n_window + p.n_lmk;
       s_base[s] = items;
       mine += (long long)s_len[s] * items;
+      count += items;
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if (lane == 0) s_sum[warp] = mine;
+    for (int o = 16; o > 0; o >>= 1) {
+      mine += __shfl_xor_sync(0xffffffffu, mine, o);
+      count += __shfl_xor_sync(0xffffffffu, count, o);
+    }
+    if (lane == 0) s_sum[warp][0] = mine, s_sum[warp][1] = count;
     __syncthreads();
-    const long long total = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-    constexpr int UNITS = Shape<D>::UNITS;
-    chunk = (int)min(max((total + UNITS - 1) / UNITS, (long long)CA_MIN_TILES), 0x7fffffffLL);
+    const long long total = s_sum[0][0] + s_sum[1][0] + s_sum[2][0] + s_sum[3][0];
+    const long long items = s_sum[0][1] + s_sum[1][1] + s_sum[2][1] + s_sum[3][1];
+    // Cutting adds at most one unit per item: where the items leave room, all units run at once;
+    // where they do not, only items above an average slot's load are cut.
+    constexpr int SLOTS = Shape<D>::SLOTS;
+    const long long want = items < SLOTS ? max(SLOTS - items, (long long)SLOTS / 4) : SLOTS;
+    chunk = (int)min(max((total + want - 1) / want, (long long)CA_MIN_TILES), 0x7fffffffLL);
   }
   int2 carry = make_int2(0, 0);
   for (int base = 0; base < a.n_seqs; base += CA_THREADS) {
@@ -265,29 +286,39 @@ __global__ void __launch_bounds__(CA_THREADS, NS == 1 ? Shape<D>::OCC : 1) cache
   const int each = (tiles + splits - 1) / splits;
   const int t_begin = min(split * each, tiles), t_end = min(t_begin + each, tiles);
 
-  // ---- this lane's two query rows
+  // ---- rows 2t, 2t+1 of the tile are this lane's in S^T and O^T
   int row_lo[2], row_hi[2], row_head[2];
-  float row_f[2];
   bool row_ok[2];
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int i = tile * 16 + g + r * 8, tok = i / a.G;
-    row_ok[r] = tok < p.n_q;
+  for (int c = 0; c < 2; ++c) {
+    const int i = tile * CA_ROWS + 2 * t + c, tok = i / a.G;
+    row_ok[c] = tok < p.n_q;
     const int pos = p.len - p.n_q + tok;
-    const bool keys = row_ok[r] && pos >= 0;
-    row_lo[r] = keys ? first_key(a, p.q0 + tok, pos) : 0x7fffffff;
-    row_hi[r] = keys ? pos + 1 : 0;
-    row_head[r] = i % a.G;
+    const bool keys = row_ok[c] && pos >= 0;
+    row_lo[c] = keys ? first_key(a, p.q0 + tok, pos) : 0x7fffffff;
+    row_hi[c] = keys ? pos + 1 : 0;
+    row_head[c] = i % a.G;
   }
-  uint32_t qa[Q_SMEM ? 1 : KS][4];
+  // keys that every row of the tile attends to need no mask
+  int lo_min = min(row_lo[0], row_lo[1]), hi_max = max(row_hi[0], row_hi[1]);
+  int lo_max = max(row_ok[0] ? row_lo[0] : 0, row_ok[1] ? row_lo[1] : 0);
+  int hi_min = min(row_ok[0] ? row_hi[0] : 0x7fffffff, row_ok[1] ? row_hi[1] : 0x7fffffff);
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    // 16 consecutive elements at 16 t of each 64
+  for (int x = 1; x < 4; x <<= 1) {
+    lo_max = max(lo_max, __shfl_xor_sync(0xffffffffu, lo_max, x));
+    hi_min = min(hi_min, __shfl_xor_sync(0xffffffffu, hi_min, x));
+    lo_min = min(lo_min, __shfl_xor_sync(0xffffffffu, lo_min, x));
+    hi_max = max(hi_max, __shfl_xor_sync(0xffffffffu, hi_max, x));
+  }
+  // ---- Q of row g: the 16 consecutive elements at 16 t of each 64
+  uint32_t qb[NS][KS][2];
+  float row_f[2];
+  {
     float x[D / 4];
 #pragma unroll
     for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
-    if (row_ok[r]) {
-      const int i = tile * 16 + g + r * 8;
+    const int i = tile * CA_ROWS + g;
+    if (i / a.G < p.n_q) {
       const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)(p.q0 + i / a.G) * a.q_stride +
                      (int64_t)(hk * a.G + i % a.G) * D + t * 16;
 #pragma unroll
@@ -317,46 +348,31 @@ __global__ void __launch_bounds__(CA_THREADS, NS == 1 ? Shape<D>::OCC : 1) cache
     }
     float big = 0.f;
 #pragma unroll
-    for (int i = 0; i < D / 4; ++i) big = fmaxf(big, fabsf(x[i]));
+    for (int j = 0; j < D / 4; ++j) big = fmaxf(big, fabsf(x[j]));
     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
     const int eb = (int)(__float_as_uint(big) >> 23);  // biased exponent; 255: an infinity
     const int up = eb == 255 ? 0 : min(max(13 - (eb - 127), -126), 126);
     const float mul = __uint_as_float((uint32_t)(up + 127) << 23);
-    row_f[r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
+    const float f = a.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) row_f[c] = __shfl_sync(0xffffffffu, f, (2 * t + c) * 4);
 #pragma unroll
     for (int k = 0; k < KS; ++k)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float lo = x[4 * k + 2 * h] * mul, hi = x[4 * k + 2 * h + 1] * mul;
-        const uint32_t first = pack_f16x2(lo, hi);
-        if constexpr (!Q_SMEM) {
-          qa[k][2 * h + r] = first;
-        } else if (warp == 0) {
-          uint32_t* sq = reinterpret_cast<uint32_t*>(s_q);
-          sq[(k * 32 + lane) * 4 + 2 * h + r] = first;
-          if constexpr (NS == 2) {
-            const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&first));
-            sq[((KS + k) * 32 + lane) * 4 + 2 * h + r] = pack_f16x2(lo - b.x, hi - b.y);
-          }
+        qb[0][k][h] = pack_f16x2(lo, hi);
+        if constexpr (NS == 2) {
+          const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&qb[0][k][h]));
+          qb[1][k][h] = pack_f16x2(lo - b.x, hi - b.y);
         }
       }
   }
-  // keys that every row of the tile attends to need no mask
-  int lo_min = min(row_lo[0], row_lo[1]), hi_max = max(row_hi[0], row_hi[1]);
-  int lo_max = max(row_ok[0] ? row_lo[0] : 0, row_ok[1] ? row_lo[1] : 0);
-  int hi_min = min(row_ok[0] ? row_hi[0] : 0x7fffffff, row_ok[1] ? row_hi[1] : 0x7fffffff);
-#pragma unroll
-  for (int o = 4; o < 32; o <<= 1) {
-    lo_max = max(lo_max, __shfl_xor_sync(0xffffffffu, lo_max, o));
-    hi_min = min(hi_min, __shfl_xor_sync(0xffffffffu, hi_min, o));
-    lo_min = min(lo_min, __shfl_xor_sync(0xffffffffu, lo_min, o));
-    hi_max = max(hi_max, __shfl_xor_sync(0xffffffffu, hi_max, o));
-  }
 
-  float o[NT][4];
+  float o[MT][4];  // channels D/8 g + 2 i (0, 1) and one on (2, 3) of rows 2t, 2t+1
 #pragma unroll
-  for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   RowState st[2] = {{-INFINITY, 0.f, -INFINITY}, {-INFINITY, 0.f, -INFINITY}};
   const int page_mask = (1 << a.page_shift) - 1;
   const int* table = a.tables + (int64_t)s * a.max_pages;
@@ -465,7 +481,7 @@ __global__ void __launch_bounds__(CA_THREADS, NS == 1 ? Shape<D>::OCC : 1) cache
     }
     copies_commit();
   };
-  __syncthreads();  // Q is in place; the schedule's memory becomes the rings
+  __syncthreads();  // the schedule's memory becomes the rings
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) issue(i);
 
@@ -477,72 +493,63 @@ __global__ void __launch_bounds__(CA_THREADS, NS == 1 ? Shape<D>::OCC : 1) cache
     out_stage = out_stage == (STAGES - 1) * Stage<D>::BYTES ? 0 : out_stage + Stage<D>::BYTES;
     const float4* meta = reinterpret_cast<const float4*>(stage + Stage<D>::META);
     const bool window = i < n_w;
-    // ---- S = Q K^T
-    float sc[4][4];
+    // ---- S^T = K Q^T
+    float sc[2][4];  // half h: keys g (0, 1) and 8 on (2, 3) of rows 2t, 2t+1
 #pragma unroll
-    for (int nt = 0; nt < 4; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+    for (int h = 0; h < 2; ++h) {
+      sc[h][0] = sc[h][1] = sc[h][2] = sc[h][3] = 0.f;
 #pragma unroll
-    for (int b = 0; b < D / 64; ++b) {
-      uint32_t kr[4][4];
+      for (int b = 0; b < D / 64; ++b) {
+        const uint4 ka = *reinterpret_cast<const uint4*>(stage + Stage<D>::k_at(h * 16 + slot_of(g), b * 4 + t));
+        const uint4 kb = *reinterpret_cast<const uint4*>(stage + Stage<D>::k_at(h * 16 + 8 + slot_of(g), b * 4 + t));
+        const uint32_t k0[4] = {ka.x, ka.y, ka.z, ka.w}, k1[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
-        const uint4 kw = *reinterpret_cast<const uint4*>(stage + Stage<D>::k_at(slot_of(nt, g), b * 4 + t));
-        kr[nt][0] = kw.x, kr[nt][1] = kw.y, kr[nt][2] = kw.z, kr[nt][3] = kw.w;
-      }
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t a0 = widen_lo(k0[k]), a1 = widen_lo(k1[k]), a2 = widen_hi(k0[k]), a3 = widen_hi(k1[k]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int x = 0; x < NS; ++x) {
-          uint32_t q4[4];
-          if constexpr (Q_SMEM) {
-            const uint4 y = s_q[(x * KS + b * 4 + k) * 32 + lane];
-            q4[0] = y.x, q4[1] = y.y, q4[2] = y.z, q4[3] = y.w;
-          } else {
-            q4[0] = qa[b * 4 + k][0], q4[1] = qa[b * 4 + k][1], q4[2] = qa[b * 4 + k][2], q4[3] = qa[b * 4 + k][3];
-          }
-#pragma unroll
-          for (int nt = 0; nt < 4; ++nt)
-            mma_f16(sc[nt], q4[0], q4[1], q4[2], q4[3], widen_lo(kr[nt][k]), widen_hi(kr[nt][k]));
+          for (int x = 0; x < NS; ++x) mma_f16(sc[h], a0, a1, a2, a3, qb[x][b * 4 + k][0], qb[x][b * 4 + k][1]);
         }
+      }
     }
     // ---- P = 2^(x + e - M + 14), l += 2^(x - m)
     const int key0 = p.lo32 + (wb + i) * 32;
     const float4 mh[2] = {meta[0], meta[16]};  // of a window tile's halves
     bool plain = window && key0 >= lo_max && key0 + 32 <= hi_min && __float_as_int(mh[0].w) >= 0 &&
                  __float_as_int(mh[1].w) >= 0;
-    uint32_t valid = 0xffff;  // bit 4 nt + 2 r + c: row r attends to column c of block nt
+    uint32_t valid = 0xff;  // bit 4 h + e: element e of half h counts
     if (plain) {
       // m and M are references here, not exact maxima: they move when a logit passes them by
       // the slack. One exponential per element: the sum of P is brought to l's reference.
       float f[2][2], lm[2][2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          f[r][h] = mh[h].x * row_f[r];
-          lm[r][h] = f[r][h] * fmaxf(fmaxf(sc[2 * h][2 * r], sc[2 * h][2 * r + 1]), fmaxf(sc[2 * h + 1][2 * r], sc[2 * h + 1][2 * r + 1]));
-        }
       bool over = false;
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
-        over |= fmaxf(lm[r][0], lm[r][1]) > st[r].m + CA_SLACK || fmaxf(lm[r][0] + mh[0].y, lm[r][1] + mh[1].y) > st[r].M + CA_SLACK;
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          f[c][h] = mh[h].x * row_f[c];
+          lm[c][h] = f[c][h] * fmaxf(sc[h][c], sc[h][2 + c]);
+        }
+        over |= fmaxf(lm[c][0], lm[c][1]) > st[c].m + CA_SLACK ||
+                fmaxf(lm[c][0] + mh[0].y, lm[c][1] + mh[1].y) > st[c].M + CA_SLACK;
+      }
       if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float gm = fmaxf(lm[r][0], lm[r][1]), gM = fmaxf(lm[r][0] + mh[0].y, lm[r][1] + mh[1].y);
-          gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 1));
-          gM = fmaxf(gM, __shfl_xor_sync(0xffffffffu, gM, 1));
-          gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 2));
-          gM = fmaxf(gM, __shfl_xor_sync(0xffffffffu, gM, 2));
-          const float m = fmaxf(st[r].m, gm), M = fmaxf(st[r].M, gM);
-          st[r].l *= m == -INFINITY ? 1.f : exp2_fast(st[r].m - m);
-          const float c = M == -INFINITY ? 1.f : exp2_fast(st[r].M - M);
-          st[r].m = m;
-          st[r].M = M;
+        for (int c = 0; c < 2; ++c) {
+          float gm = fmaxf(lm[c][0], lm[c][1]), gM = fmaxf(lm[c][0] + mh[0].y, lm[c][1] + mh[1].y);
 #pragma unroll
-          for (int x = 0; x < NT; ++x) {
-            o[x][2 * r] *= c;
-            o[x][2 * r + 1] *= c;
+          for (int x = 4; x < 32; x <<= 1) {
+            gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, x));
+            gM = fmaxf(gM, __shfl_xor_sync(0xffffffffu, gM, x));
+          }
+          const float m = fmaxf(st[c].m, gm), M = fmaxf(st[c].M, gM);
+          st[c].l *= m == -INFINITY ? 1.f : exp2_fast(st[c].m - m);
+          const float corr = M == -INFINITY ? 1.f : exp2_fast(st[c].M - M);
+          st[c].m = m;
+          st[c].M = M;
+#pragma unroll
+          for (int x = 0; x < MT; ++x) {
+            o[x][c] *= corr;
+            o[x][2 + c] *= corr;
           }
         }
       }
@@ -552,107 +559,101 @@ __global__ void __launch_bounds__(CA_THREADS, NS == 1 ? Shape<D>::OCC : 1) cache
       plain = !__any_sync(0xffffffffu, !(st[0].m + e_min - st[0].M > -90.f) || !(st[1].m + e_min - st[1].M > -90.f));
       if (plain) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float shift = mh[h].y - st[r].M + CA_P_SHIFT;
-            float sum = 0.f;
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                float& y = sc[2 * h + x][2 * r + c];
-                y = exp2_fast(fmaf(y, f[r][h], shift));
-                sum += y;
-              }
-            st[r].l = fmaf(sum, exp2_fast(-shift - st[r].m), st[r].l);
+            const float shift = mh[h].y - st[c].M + CA_P_SHIFT;
+            sc[h][c] = exp2_fast(fmaf(sc[h][c], f[c][h], shift));
+            sc[h][2 + c] = exp2_fast(fmaf(sc[h][2 + c], f[c][h], shift));
+            st[c].l = fmaf(sc[h][c] + sc[h][2 + c], exp2_fast(-shift - st[c].m), st[c].l);
           }
       } else {
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[nt][e] *= f[e >> 1][nt >> 1];
+          for (int e = 0; e < 4; ++e) sc[h][e] *= f[e & 1][h];
       }
-    } else {
-      valid = 0;
-      const int head = window ? -1 : (lb + i - n_w) / lmk32;
-#pragma unroll
-      for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int slot = (nt >> 1) * 16 + (nt & 1) * 8 + t + 4 * c;
-          const float4 mt = window ? mh[nt >> 1] : meta[slot];
-          int key = __float_as_int(mt.w);
-          if (window && key >= 0) {
-            key += slot & 15;
-            if (key >= p.len) key = -1;
-          }
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const bool ok = key >= 0 && (window ? key >= row_lo[r] && key < row_hi[r]
-                                                : key < row_lo[r] && key < row_hi[r] && head == row_head[r]);
-            if (ok) valid |= 1u << (4 * nt + 2 * r + c);
-            sc[nt][2 * r + c] = ok ? fmaf(sc[nt][2 * r + c], mt.x * row_f[r], mt.z) : -INFINITY;
-          }
-        }
     }
     if (!plain) {
-      float ve[4][2];
+      float ve[2][2];
+      if (valid == 0xff && window && key0 >= lo_max && key0 + 32 <= hi_min && __float_as_int(mh[0].w) >= 0 &&
+          __float_as_int(mh[1].w) >= 0) {  // came from above, logits formed
+        ve[0][0] = ve[0][1] = mh[0].y;
+        ve[1][0] = ve[1][1] = mh[1].y;
+      } else {
+        valid = 0;
+        const int head = window ? -1 : (lb + i - n_w) / lmk32;
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-          ve[nt][c] = window ? mh[nt >> 1].y : meta[(nt >> 1) * 16 + (nt & 1) * 8 + t + 4 * c].y;
+          for (int b = 0; b < 2; ++b) {
+            const int slot = b * 8 + slot_of(g);  // within the half
+            const float4 mt = window ? mh[h] : meta[h * 16 + slot];
+            int key = __float_as_int(mt.w);
+            if (window && key >= 0) {
+              key += slot;
+              if (key >= p.len) key = -1;
+            }
+            ve[h][b] = mt.y;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
+            for (int c = 0; c < 2; ++c) {
+              const bool ok = key >= 0 && (window ? key >= row_lo[c] && key < row_hi[c]
+                                                  : key < row_lo[c] && key < row_hi[c] && head == row_head[c]);
+              if (ok) valid |= 1u << (4 * h + 2 * b + c);
+              sc[h][2 * b + c] = ok ? fmaf(sc[h][2 * b + c], mt.x * row_f[c], mt.z) : -INFINITY;
+            }
+          }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
         float gm = -INFINITY, gM = -INFINITY;
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            gm = fmaxf(gm, sc[nt][2 * r + c]);
-            gM = fmaxf(gM, sc[nt][2 * r + c] + ve[nt][c]);
+          for (int b = 0; b < 2; ++b) {
+            gm = fmaxf(gm, sc[h][2 * b + c]);
+            gM = fmaxf(gM, sc[h][2 * b + c] + ve[h][b]);
           }
-        gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 1));
-        gM = fmaxf(gM, __shfl_xor_sync(0xffffffffu, gM, 1));
-        gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 2));
-        gM = fmaxf(gM, __shfl_xor_sync(0xffffffffu, gM, 2));
-        const float m = fmaxf(st[r].m, gm), M = fmaxf(st[r].M, gM);
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) {
+          gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, x));
+          gM = fmaxf(gM, __shfl_xor_sync(0xffffffffu, gM, x));
+        }
+        const float m = fmaxf(st[c].m, gm), M = fmaxf(st[c].M, gM);
         const float mu = m == -INFINITY ? 0.f : m, Mu = M == -INFINITY ? 0.f : M;
-        float l = st[r].l * exp2_fast(st[r].m - mu);
-        const float corr = exp2_fast(st[r].M - Mu);
+        float l = st[c].l * exp2_fast(st[c].m - mu);
+        const float corr = exp2_fast(st[c].M - Mu);
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const float x = sc[nt][2 * r + c];
+          for (int b = 0; b < 2; ++b) {
+            const float x = sc[h][2 * b + c];
             l += exp2_fast(x - mu);
-            sc[nt][2 * r + c] = exp2_fast(x + ve[nt][c] - Mu + CA_P_SHIFT);
+            sc[h][2 * b + c] = exp2_fast(x + ve[h][b] - Mu + CA_P_SHIFT);
           }
-        st[r] = {m, l, M};
-        if (__any_sync(0xffffffffu, corr != 1.f)) {
+        st[c] = {m, l, M};
 #pragma unroll
-          for (int x = 0; x < NT; ++x) {
-            o[x][2 * r] *= corr;
-            o[x][2 * r + 1] *= corr;
-          }
+        for (int x = 0; x < MT; ++x) {
+          o[x][c] *= corr;
+          o[x][2 + c] *= corr;
         }
       }
     }
-    // ---- O += P V, 16 keys at a time
+    // ---- O^T += V^T P^T, 16 keys at a time
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      uint32_t pa[NS][4];
+      uint32_t pb[NS][2];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float lo = sc[2 * h + (x >> 1)][2 * (x & 1)], hi = sc[2 * h + (x >> 1)][2 * (x & 1) + 1];
-        pa[0][x] = pack_f16x2(lo, hi);
+      for (int b = 0; b < 2; ++b) {
+        const float lo = sc[h][2 * b], hi = sc[h][2 * b + 1];
+        const uint32_t first = pack_f16x2(lo, hi);
+        pb[0][b] = transpose8(first);
         if constexpr (NS == 2) {
-          const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&pa[0][x]));
-          pa[1][x] = pack_f16x2(lo - b.x, hi - b.y);
+          const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&first));
+          pb[1][b] = transpose8(pack_f16x2(lo - x.x, hi - x.y));
         }
       }
-      uint32_t v[4][D / 32];
+      uint32_t v[4][D / 32];  // keys t, t + 4, t + 8, t + 12
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const int r = h * 16 + t + 4 * x;
@@ -665,20 +666,21 @@ __global__ void __launch_bounds__(CA_THREADS, NS == 1 ? Shape<D>::OCC : 1) cache
         }
       }
       bool nans = false;
-      if (valid != 0xffff) {  // differs from lane to lane
+      if (!plain) {
 #pragma unroll
         for (int x = 0; x < 4; ++x)
 #pragma unroll
           for (int y = 0; y < D / 32; ++y) nans |= nan_bytes(v[x][y]) != 0;
+        nans = __any_sync(0xffffffffu, nans);
       }
-      if (__any_sync(0xffffffffu, nans)) {
-        // P = 0 must not spread a NaN: count, per row and channel, the NaNs among the keys that the
+      if (nans) {
+        // P = 0 must not spread a NaN: count, per channel and row, the NaNs among the keys that the
         // row attends to (a product of ones), and take the NaNs themselves out
-        uint32_t va[4];
+        uint32_t ones[2];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const uint32_t bits = valid >> (4 * (2 * h + (x >> 1)) + 2 * (x & 1));
-          va[x] = (bits & 1 ? 0x3c00u : 0u) | (bits & 2 ? 0x3c000000u : 0u);
+        for (int b = 0; b < 2; ++b) {
+          const uint32_t bits = valid >> (4 * h + 2 * b);
+          ones[b] = transpose8((bits & 1 ? 0x3c00u : 0u) | (bits & 2 ? 0x3c000000u : 0u));
         }
 #pragma unroll
         for (int x = 0; x < D / 32; ++x) {
@@ -689,18 +691,17 @@ __global__ void __launch_bounds__(CA_THREADS, NS == 1 ? Shape<D>::OCC : 1) cache
             v[y][x] &= ~nb[y];
           }
 #pragma unroll
-          for (int y = 0; y < 2; ++y)
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t sel = y ? 0x7362 : 0x5140;
+            const uint32_t b0 = __byte_perm(nb[0], nb[1], sel), b1 = __byte_perm(nb[2], nb[3], sel);
+            float cnt[4] = {0.f, 0.f, 0.f, 0.f};
+            // 0xff per NaN -> fp16 1.0
+            mma_f16(cnt, __byte_perm(b0, 0, 0x1100) & 0x3c003c00u, __byte_perm(b0, 0, 0x3322) & 0x3c003c00u,
+                    __byte_perm(b1, 0, 0x1100) & 0x3c003c00u, __byte_perm(b1, 0, 0x3322) & 0x3c003c00u, ones[0], ones[1]);
 #pragma unroll
-            for (int z = 0; z < 2; ++z) {
-              const uint32_t sel = y ? 0x7362 : 0x5140, half = z ? 0x3322 : 0x1100;
-              const uint32_t m0 = __byte_perm(__byte_perm(nb[0], nb[1], sel), 0, half);  // 0xffff per NaN
-              const uint32_t m1 = __byte_perm(__byte_perm(nb[2], nb[3], sel), 0, half);
-              float cnt[4] = {0.f, 0.f, 0.f, 0.f};
-              mma_f16(cnt, va[0], va[1], va[2], va[3], m0 & 0x3c003c00u, m1 & 0x3c003c00u);
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (cnt[e] > 0.f) o[4 * x + 2 * y + z][e] = __int_as_float(0x7fffffff);
-            }
+            for (int e = 0; e < 4; ++e)
+              if (cnt[e] > 0.f) o[2 * x + y][e] = __int_as_float(0x7fffffff);
+          }
         }
       }
 #pragma unroll
@@ -709,13 +710,9 @@ __global__ void __launch_bounds__(CA_THREADS, NS == 1 ? Shape<D>::OCC : 1) cache
         for (int y = 0; y < 2; ++y) {
           const uint32_t sel = y ? 0x7362 : 0x5140;
           const uint32_t b0 = __byte_perm(v[0][x], v[1][x], sel), b1 = __byte_perm(v[2][x], v[3][x], sel);
+          const uint32_t a0 = widen_lo(b0), a1 = widen_hi(b0), a2 = widen_lo(b1), a3 = widen_hi(b1);
 #pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            const uint32_t h0 = z ? widen_hi(b0) : widen_lo(b0), h1 = z ? widen_hi(b1) : widen_lo(b1);
-#pragma unroll
-            for (int q4 = 0; q4 < NS; ++q4)
-              mma_f16(o[4 * x + 2 * y + z], pa[q4][0], pa[q4][1], pa[q4][2], pa[q4][3], h0, h1);
-          }
+          for (int z = 0; z < NS; ++z) mma_f16(o[2 * x + y], a0, a1, a2, a3, pb[z][0], pb[z][1]);
         }
     }
   }
@@ -725,26 +722,23 @@ __global__ void __launch_bounds__(CA_THREADS, NS == 1 ? Shape<D>::OCC : 1) cache
   copies_wait<0>();
   __syncthreads();  // the rings' memory becomes the parts
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    float l = st[r].l;
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if (t == 0) {
-      s_m[warp][g + 8 * r] = st[r].m;
-      s_l[warp][g + 8 * r] = l;
-      s_M[warp][g + 8 * r] = st[r].M;
-    }
-    float* dst = s_o + (warp * 16 + g + 8 * r) * D + t * (D / 4);  // columns D/8 (2t) + i and D/8 (2t + 1) + i
+  for (int c = 0; c < 2; ++c) {
+    float l = st[c].l;
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      dst[i] = o[i][2 * r];
-      dst[NT + i] = o[i][2 * r + 1];
+    for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+    if (g == 0) {
+      s_m[warp][2 * t + c] = st[c].m;
+      s_l[warp][2 * t + c] = l;
+      s_M[warp][2 * t + c] = st[c].M;
     }
+    float* dst = s_o + (warp * CA_ROWS + 2 * t + c) * D + g * (D / 8);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(o[i][c], o[i][2 + c]);
   }
   __syncthreads();
-  for (int e = tid; e < 16 * D; e += CA_THREADS) {
+  for (int e = tid; e < CA_ROWS * D; e += CA_THREADS) {
     const int r = e / D, d = e % D;
-    const int i = tile * 16 + r, tok = i / a.G, h = hk * a.G + i % a.G;
+    const int i = tile * CA_ROWS + r, tok = i / a.G, h = hk * a.G + i % a.G;
     if (tok >= p.n_q) continue;
     float m = -INFINITY, M = -INFINITY;
 #pragma unroll
@@ -757,7 +751,7 @@ __global__ void __launch_bounds__(CA_THREADS, NS == 1 ? Shape<D>::OCC : 1) cache
 #pragma unroll
     for (int x = 0; x < CA_WARPS; ++x) {
       l += s_l[x][r] * exp2_fast(s_m[x][r] - mu);
-      v += s_o[(x * 16 + r) * D + d] * exp2_fast(s_M[x][r] - Mu);
+      v += s_o[(x * CA_ROWS + r) * D + d] * exp2_fast(s_M[x][r] - Mu);
     }
     const int64_t row = (int64_t)(p.q0 + tok) * a.H + h;
     if (splits == 1) {
@@ -771,11 +765,11 @@ __global__ void __launch_bounds__(CA_THREADS, NS == 1 ? Shape<D>::OCC : 1) cache
       }
     } else {
       const int64_t part = part0 + split;
-      a.part_o[(part * 16 + r) * D + d] = v;
+      a.part_o[(part * CA_ROWS + r) * D + d] = v;
       if (d == 0) {
-        float* ps = a.part_s + (part * 16 + r) * 4;
+        float* ps = a.part_s + (part * CA_ROWS + r) * 4;
         ps[0] = m, ps[1] = l, ps[2] = M;
-        if (split == 0) a.row_part[row] = make_int2(part0 * 16 + r, splits);
+        if (split == 0) a.row_part[row] = make_int2(part0 * CA_ROWS + r, splits);
       }
     }
   }
@@ -789,14 +783,14 @@ __global__ void __launch_bounds__(128) cache_attn_join_kernel(CacheAttnArgs a) {
   const int64_t row = blockIdx.x;
   const int2 rp = a.row_part[row];
   // one part: already written. Anything else than parts of this call: a row of no sequence.
-  if (rp.y <= 1 || rp.x < 0 || rp.y > 2 * CA_MAX_UNITS || rp.x / 16 + rp.y > 2 * CA_MAX_UNITS) return;
+  if (rp.y <= 1 || rp.x < 0 || rp.y > 2 * CA_MAX_SLOTS || rp.x / CA_ROWS + rp.y > 2 * CA_MAX_SLOTS) return;
   __shared__ float s_red[8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const float* ps = a.part_s + (int64_t)rp.x * 4;
   float m = -INFINITY, M = -INFINITY;
   for (int x = tid; x < rp.y; x += 128) {
-    m = fmaxf(m, ps[(int64_t)x * 64]);
-    M = fmaxf(M, ps[(int64_t)x * 64 + 2]);
+    m = fmaxf(m, ps[(int64_t)x * (4 * CA_ROWS)]);
+    M = fmaxf(M, ps[(int64_t)x * (4 * CA_ROWS) + 2]);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -809,11 +803,11 @@ __global__ void __launch_bounds__(128) cache_attn_join_kernel(CacheAttnArgs a) {
   M = fmaxf(fmaxf(s_red[4], s_red[5]), fmaxf(s_red[6], s_red[7]));
   const float mu = m == -INFINITY ? 0.f : m, Mu = M == -INFINITY ? 0.f : M;
   float l = 0.f;
-  for (int x = 0; x < rp.y; ++x) l += ps[(int64_t)x * 64 + 1] * exp2_fast(ps[(int64_t)x * 64] - mu);
+  for (int x = 0; x < rp.y; ++x) l += ps[(int64_t)x * (4 * CA_ROWS) + 1] * exp2_fast(ps[(int64_t)x * (4 * CA_ROWS)] - mu);
   if (tid < D) {
     float v = 0.f;
     for (int x = 0; x < rp.y; ++x)
-      v += a.part_o[((int64_t)rp.x + (int64_t)x * 16) * D + tid] * exp2_fast(ps[(int64_t)x * 64 + 2] - Mu);
+      v += a.part_o[((int64_t)rp.x + (int64_t)x * CA_ROWS) * D + tid] * exp2_fast(ps[(int64_t)x * (4 * CA_ROWS) + 2] - Mu);
     const float res = l == 0.f ? 0.f : v * exp2_fast(Mu - mu - CA_P_SHIFT) / l;
     if (a.out_dtype == DSALT_F32) reinterpret_cast<float*>(a.out)[row * D + tid] = res;
     else if (a.out_dtype == DSALT_BF16) reinterpret_cast<__nv_bfloat16*>(a.out)[row * D + tid] = __float2bfloat16_rn(res);
@@ -823,12 +817,12 @@ __global__ void __launch_bounds__(128) cache_attn_join_kernel(CacheAttnArgs a) {
 }
 
 static inline size_t ca_a256(size_t v) { return (v + 255) & ~(size_t)255; }
-static inline int64_t ca_items(int64_t T, int n_seqs, int G, int Hkv) { return ((T * G + 15 * (int64_t)n_seqs) / 16 + 1) * Hkv; }
+static inline int64_t ca_items(int64_t T, int n_seqs, int G, int Hkv) { return ((T * G + (CA_ROWS - 1) * (int64_t)n_seqs) / CA_ROWS + 1) * Hkv; }
 
 template <typename T, int D, int NS>
 static int launch_cache_attn(const CacheAttnArgs& a, unsigned grid, bool join, cudaStream_t stream) {
   constexpr size_t RING = (size_t)CA_WARPS * Shape<D>::STAGES * Stage<D>::BYTES, TABLES = 3 * sizeof(int);
-  static_assert(RING >= sizeof(float) * CA_WARPS * 16 * D, "the parts take the rings' place");
+  static_assert(RING >= sizeof(float) * CA_WARPS * CA_ROWS * D, "the parts take the rings' place");
   const size_t smem = TABLES * (size_t)a.n_seqs > RING ? TABLES * (size_t)a.n_seqs : RING;
   static std::atomic<uint64_t> ready{0};
   if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(cache_attn_kernel<T, D, NS>),
@@ -858,8 +852,8 @@ extern "C" {
 size_t dsalt_cache_attention_workspace_bytes(int64_t T, int n_seqs, int n_heads, int n_kv, int head_dim) {
   if (T < 0 || n_seqs < 1 || n_heads < 1 || n_kv < 1 || head_dim < 1) return 0;
   // a cut item has at least two units of at least half the wanted length: at most twice the target
-  return ca_a256(sizeof(int2) * (size_t)T * n_heads) + ca_a256(sizeof(float) * 2 * CA_MAX_UNITS * 64) +
-         ca_a256(sizeof(float) * 2 * CA_MAX_UNITS * 16 * (size_t)head_dim);
+  return ca_a256(sizeof(int2) * (size_t)T * n_heads) + ca_a256(sizeof(float) * 2 * CA_MAX_SLOTS * CA_ROWS * 4) +
+         ca_a256(sizeof(float) * 2 * CA_MAX_SLOTS * CA_ROWS * (size_t)head_dim);
 }
 
 int dsalt_cache_attention(const void* q, int dtype, int64_t T, int n_heads, int n_kv, int head_dim, int64_t q_stride,
@@ -907,11 +901,11 @@ int dsalt_cache_attention(const void* q, int dtype, int64_t T, int n_heads, int 
   a.row_part = reinterpret_cast<int2*>(ws);
   ws += ca_a256(sizeof(int2) * (size_t)T * n_heads);
   a.part_s = reinterpret_cast<float*>(ws);
-  ws += ca_a256(sizeof(float) * 2 * CA_MAX_UNITS * 64);
+  ws += ca_a256(sizeof(float) * 2 * CA_MAX_SLOTS * CA_ROWS * 4);
   a.part_o = reinterpret_cast<float*>(ws);
   a.err = device_status_ptr();
   const int64_t items = ca_items(T, n_seqs, a.G, n_kv);
-  const int64_t grid = items + CA_MAX_UNITS;
+  const int64_t grid = items + CA_MAX_SLOTS;
   if (grid > 0x7fffff00LL) return fail(DSALT_ERR_UNSUPPORTED, "cache_attention: too many rows");
   // tables too short for any item to be cut: nothing to join
   const int64_t most = (((int64_t)max_pages * page_size + 31) >> 5) + (int64_t)a.G * ((k_lmk + 31) >> 5);
