@@ -104,7 +104,7 @@ def load() -> ctypes.CDLL:
 
 
 def call(name: str, *args):
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != OK:
         msg = lib.dsalt_last_error().decode(errors="replace")

@@ -44,20 +44,14 @@ constexpr float CA_P_SHIFT = 14.f;     // P is held times 2^14: fp16 stays norma
 constexpr float CA_SLACK = 1.f;        // P may exceed 2^14 by 2^1 before its reference moves (fp16 ends at 2^16)
 
 // blocks per SM that registers and rings allow; one round of them is the number of units wanted
-#ifndef O64
-#define O64 4
-#define S64 3
-#define O128 3
-#define S128 2
-#endif
 template <int D>
 struct Shape {
-  static constexpr int OCC = D == 64 ? O64 : O128;
-  static constexpr int STAGES = D == 64 ? S64 : S128;
+  static constexpr int OCC = D == 64 ? 4 : 3;
+  static constexpr int STAGES = 2;
   static constexpr int SLOTS = 148 * OCC;
 };
 constexpr int CA_ROWS = 8;
-constexpr int CA_MAX_SLOTS = 148 * 8;
+constexpr int CA_MAX_SLOTS = 148 * 4;
 
 struct CacheAttnArgs {
   const void* q;
@@ -251,6 +245,7 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
     carry.y += all.y;
   }
   __syncthreads();
+  cudaTriggerProgrammaticLaunchCompletion();  // the join may take its places; it waits for this grid's end
   const int unit = blockIdx.x;
   // rows behind the last sequence's: zero, log-sum-exp -inf
   if (a.cu_q) {
@@ -775,45 +770,79 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
   }
 }
 
-// Joins the parts of the rows that were cut, a block of four warps per (token, head). Parts
-// are added in their order: the result does not depend on which finished first.
+// Joins the parts of the rows that were cut, a block per row (or several rows after one
+// another). The order of every sum is fixed by the parts' numbers: the result does not depend
+// on which finished first.
+constexpr int CJ_THREADS = 256;
 template <int D>
-__global__ void __launch_bounds__(128) cache_attn_join_kernel(CacheAttnArgs a) {
-  cudaGridDependencySynchronize();
-  const int64_t row = blockIdx.x;
-  const int2 rp = a.row_part[row];
-  // one part: already written. Anything else than parts of this call: a row of no sequence.
-  if (rp.y <= 1 || rp.x < 0 || rp.y > 2 * CA_MAX_SLOTS || rp.x / CA_ROWS + rp.y > 2 * CA_MAX_SLOTS) return;
-  __shared__ float s_red[8];
+__global__ void __launch_bounds__(CJ_THREADS) cache_attn_join_kernel(CacheAttnArgs a, int rows_per_block) {
+  constexpr int TPP = D / 4, GROUPS = CJ_THREADS / TPP;  // threads per part, parts at a time
+  __shared__ float s_w[2 * CA_MAX_SLOTS];
+  __shared__ float s_red[3][CJ_THREADS / 32];
+  __shared__ float4 s_v[GROUPS][TPP];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const float* ps = a.part_s + (int64_t)rp.x * 4;
-  float m = -INFINITY, M = -INFINITY;
-  for (int x = tid; x < rp.y; x += 128) {
-    m = fmaxf(m, ps[(int64_t)x * (4 * CA_ROWS)]);
-    M = fmaxf(M, ps[(int64_t)x * (4 * CA_ROWS) + 2]);
-  }
+  cudaGridDependencySynchronize();
+  const int64_t rows = (int64_t)a.T * a.H, row0 = (int64_t)blockIdx.x * rows_per_block;
+  for (int64_t row = row0; row < min(row0 + rows_per_block, rows); ++row) {
+    const int2 rp = a.row_part[row];
+    // one part: already written. Anything else than parts of this call: a row of no sequence.
+    if (rp.y <= 1 || rp.x < 0 || rp.y > 2 * CA_MAX_SLOTS || rp.x / CA_ROWS + rp.y > 2 * CA_MAX_SLOTS) continue;
+    const float4* ps = reinterpret_cast<const float4*>(a.part_s) + rp.x;
+    float m = -INFINITY, M = -INFINITY;
+    for (int x = tid; x < rp.y; x += CJ_THREADS) {
+      const float4 v = ps[(int64_t)x * CA_ROWS];
+      m = fmaxf(m, v.x);
+      M = fmaxf(M, v.z);
+      s_w[x] = v.z;
+    }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    for (int o = 16; o > 0; o >>= 1) {
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    }
+    if (lane == 0) s_red[0][warp] = m, s_red[1][warp] = M;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < CJ_THREADS / 32; ++w) {
+      m = fmaxf(m, s_red[0][w]);
+      M = fmaxf(M, s_red[1][w]);
+    }
+    const float mu = m == -INFINITY ? 0.f : m, Mu = M == -INFINITY ? 0.f : M;
+    float l = 0.f;
+    for (int x = tid; x < rp.y; x += CJ_THREADS) {
+      const float4 v = ps[(int64_t)x * CA_ROWS];
+      l += v.y * exp2_fast(v.x - mu);
+      s_w[x] = exp2_fast(s_w[x] - Mu);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (lane == 0) s_red[2][warp] = l;
+    __syncthreads();
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < CJ_THREADS / 32; ++w) l += s_red[2][w];
+    const float4* po = reinterpret_cast<const float4*>(a.part_o + (int64_t)rp.x * D) + tid % TPP;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int x = tid / TPP; x < rp.y; x += GROUPS) {
+      const float4 y = po[(int64_t)x * (CA_ROWS * TPP)];
+      const float w = s_w[x];
+      v.x += y.x * w, v.y += y.y * w, v.z += y.z * w, v.w += y.w * w;
+    }
+    s_v[tid / TPP][tid % TPP] = v;
+    __syncthreads();
+    if (tid < D) {
+      float sum = 0.f;
+#pragma unroll
+      for (int x = 0; x < GROUPS; ++x) sum += reinterpret_cast<const float*>(&s_v[x][0])[tid];
+      const float res = l == 0.f ? 0.f : sum * exp2_fast(Mu - mu - CA_P_SHIFT) / l;
+      if (a.out_dtype == DSALT_F32) reinterpret_cast<float*>(a.out)[row * D + tid] = res;
+      else if (a.out_dtype == DSALT_BF16) reinterpret_cast<__nv_bfloat16*>(a.out)[row * D + tid] = __float2bfloat16_rn(res);
+      else reinterpret_cast<__half*>(a.out)[row * D + tid] = __float2half_rn(res);
+    }
+    if (tid == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    __syncthreads();  // the shared arrays are used again
   }
-  if (lane == 0) s_red[warp] = m, s_red[4 + warp] = M;
-  __syncthreads();
-  m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-  M = fmaxf(fmaxf(s_red[4], s_red[5]), fmaxf(s_red[6], s_red[7]));
-  const float mu = m == -INFINITY ? 0.f : m, Mu = M == -INFINITY ? 0.f : M;
-  float l = 0.f;
-  for (int x = 0; x < rp.y; ++x) l += ps[(int64_t)x * (4 * CA_ROWS) + 1] * exp2_fast(ps[(int64_t)x * (4 * CA_ROWS)] - mu);
-  if (tid < D) {
-    float v = 0.f;
-    for (int x = 0; x < rp.y; ++x)
-      v += a.part_o[((int64_t)rp.x + (int64_t)x * CA_ROWS) * D + tid] * exp2_fast(ps[(int64_t)x * (4 * CA_ROWS) + 2] - Mu);
-    const float res = l == 0.f ? 0.f : v * exp2_fast(Mu - mu - CA_P_SHIFT) / l;
-    if (a.out_dtype == DSALT_F32) reinterpret_cast<float*>(a.out)[row * D + tid] = res;
-    else if (a.out_dtype == DSALT_BF16) reinterpret_cast<__nv_bfloat16*>(a.out)[row * D + tid] = __float2bfloat16_rn(res);
-    else reinterpret_cast<__half*>(a.out)[row * D + tid] = __float2half_rn(res);
-  }
-  if (tid == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 static inline size_t ca_a256(size_t v) { return (v + 255) & ~(size_t)255; }
@@ -835,12 +864,15 @@ static int launch_cache_attn(const CacheAttnArgs& a, unsigned grid, bool join, c
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((int64_t)a.T * a.H));
-  cfg.blockDim = dim3(128);
+  // up to two rounds of blocks; where there are more rows, few of them are cut
+  const int64_t rows = (int64_t)a.T * a.H;
+  const int per = (int)((rows + 148 * 8 - 1) / (148 * 8));
+  cfg.gridDim = dim3((unsigned)((rows + per - 1) / per));
+  cfg.blockDim = dim3(CJ_THREADS);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, cache_attn_join_kernel<D>, a), "cache_attention join launch");
+  return check_cuda(cudaLaunchKernelEx(&cfg, cache_attn_join_kernel<D>, a, per), "cache_attention join launch");
 }
 
 }  // namespace dsalt

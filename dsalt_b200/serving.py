@@ -16,7 +16,8 @@ and every call can be captured into a CUDA graph.
 """
 from __future__ import annotations
 
-from typing import NamedTuple, Optional
+import functools
+from typing import NamedTuple
 
 import torch
 
@@ -39,31 +40,38 @@ class SlotPlan(NamedTuple):
 
 
 def _on_one_device(first: torch.Tensor, *rest) -> torch.device:
-    dev = first.device
-    if dev.type != "cuda":
+    index = first.get_device()
+    if index < 0:
         raise RuntimeError("dsalt_b200 operators need CUDA tensors (no CPU path)")
     for t in rest:
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"tensors on {dev} and {t.device} in one call")
-    return dev
+        if t is not None and t.get_device() != index:
+            raise RuntimeError(f"tensors on {first.device} and {t.device} in one call")
+    return first.device
 
 
 def _want(t: torch.Tensor, name: str, dtype: torch.dtype, shape) -> None:
+    if t.dtype is dtype and t.shape == shape and t.is_contiguous():
+        return
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
+    raise ValueError(f"{name} must be contiguous")
 
 
 def _run(dev: torch.device, name: str, *args) -> None:
     """The C call on the current stream of the tensors' device."""
-    if dev.index == torch.cuda.current_device():
-        L.call(name, *args, torch.cuda.current_stream().cuda_stream)
+    index = dev.index
+    if index == torch.cuda.current_device():
+        L.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            L.call(name, *args, torch.cuda.current_stream().cuda_stream)
+            L.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_workspace(T: int, S: int, H: int, n_kv: int, D: int) -> int:
+    return L.query("dsalt_cache_attention_workspace_bytes", T, S, H, n_kv, D)
 
 
 # --------------------------------------------------------------------------- slots
@@ -206,7 +214,7 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_len
         q = q.contiguous()
     out = torch.empty(T, H, D, dtype=out_dtype or q.dtype, device=dev)
     lse = torch.empty(T, H, dtype=torch.float32, device=dev) if return_lse else None
-    ws = _workspace(L.query("dsalt_cache_attention_workspace_bytes", T, S, H, n_kv, D), dev)
+    ws = _workspace(_attention_workspace(T, S, H, n_kv, D), dev)
     _run(dev, "dsalt_cache_attention", q.data_ptr(), _dt(q), T, H, n_kv, D, q.stride(0), k_cache.data_ptr(),
          v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_pages, page, block_tables.data_ptr(), max_pages,
          seq_lens.data_ptr(), S, _ptr(cu_q), _ptr(w_sizes), _ptr(lmk_indices), _ptr(lmk_bias), k_lmk, out.data_ptr(),
