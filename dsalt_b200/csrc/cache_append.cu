@@ -13,10 +13,12 @@
 // enter amax, a NaN as NaN.
 //
 // A run is the tokens of one page among `page` consecutive tokens of the call, beginning with
-// the first of them. One group of threads owns a run of one head: it takes amax, settles e,
+// the first of them. One group of lanes owns a run of one head: it takes amax, settles e,
 // rewrites the older bytes if e grew and writes the new ones, so nothing is exchanged between
-// groups. A decode step is all runs of one token (a warp each), a prompt is runs of P
-// tokens (a block each).
+// groups. A decode step is all runs of one token: D/8 lanes each, so that a warp holds
+// 4 (2) heads at once. A prompt is runs of P tokens: a warp each, which keeps up to 64
+// vectors per row of lanes in registers between the two passes.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.cuh"
@@ -24,15 +26,19 @@
 namespace dsalt {
 
 constexpr int APPEND_THREADS = 256;
-constexpr int APPEND_MAX_WINDOW = 64;  // tokens whose runs one block looks for
+constexpr int APPEND_WARPS = APPEND_THREADS / 32;
+constexpr int APPEND_MAX_WINDOW = 32;  // tokens whose runs one block looks for
 constexpr int APPEND_MAX_PAGE = 128;
 constexpr int SCALE_E_MIN = -110;  // 2^-110 times the smallest byte is still a normal fp32
 
+struct AppendSide {  // k or v
+  const void* src;
+  uint8_t* cache;
+  float* scale;
+  int64_t token_stride, head_stride;
+};
 struct AppendArgs {
-  const void* src[2];  // k, v
-  uint8_t* cache[2];
-  float* scale[2];
-  int64_t token_stride[2], head_stride[2];
+  AppendSide k, v;
   const int64_t* slots;
   int64_t T, n_pages;
   int n_kv, page_shift, window;
@@ -111,96 +117,42 @@ __device__ __forceinline__ float amax8(const Vec8<T>& v, float amax) {
   return amax;
 }
 
-// One run of one head by the threads of a warp (BLOCK = false) or of the block: n tokens of
-// the call from `tok` on, those whose slot lies in page `id`; s_off: their offsets in the page,
-// -1 for the others.
-template <typename T, int D, bool BLOCK>
-__device__ __forceinline__ void append_run(const AppendArgs& a, int which, int head, int64_t tok, int n, int id,
-                                           bool fresh, const int16_t* s_off, float* s_red) {
-  constexpr int N = BLOCK ? APPEND_THREADS : 32;
-  constexpr int VPT = D / 8;  // vectors per token
-  constexpr int KEEP = sizeof(T) == 4 ? 2 : 4;
-  const int me = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & 31);
-  const int64_t stride = a.token_stride[which];
-  // N is a multiple of VPT: a thread keeps its place within the rows and steps by whole tokens
-  const T* src = reinterpret_cast<const T*>(a.src[which]) + tok * stride + head * a.head_stride[which] + (me % VPT) * 8;
-  const int64_t at = (int64_t)id * a.n_kv + head;
-  uint8_t* page_bytes = a.cache[which] + (at << a.page_shift) * D;
-  float* scale = a.scale[which] + at;
-  const float old_scale = *scale;
-  constexpr int STEP = N / VPT;  // tokens per step
-  const int first = me / VPT;
-  // the first KEEP of a thread's vectors stay in registers between the passes
-  Vec8<T> keep[KEEP];
-  int off[KEEP];
-#pragma unroll
-  for (int i = 0; i < KEEP; ++i) {
-    const int x = first + i * STEP;
-    off[i] = x < n ? s_off[x] : -1;
-    if (off[i] >= 0) keep[i] = load8(src + x * stride);
+// exponent of a run of one head, and the rewriting of the page's older bytes by the warp
+// where it grew (`own`: this lane holds the decision of its group; one group at a time)
+__device__ __forceinline__ void rewrite_page(uint8_t* bytes, int n16, int shrink) {
+  const float f = shrink < -126 ? 0.f : pow2f(shrink);
+  uint4* p = reinterpret_cast<uint4*>(bytes);
+  for (int i = threadIdx.x & 31; i < n16; i += 32) {
+    uint4 v = p[i];
+    v.x = rescale_e4m3x4(v.x, f);
+    v.y = rescale_e4m3x4(v.y, f);
+    v.z = rescale_e4m3x4(v.z, f);
+    v.w = rescale_e4m3x4(v.w, f);
+    p[i] = v;
   }
-  float amax = 0.f;
-#pragma unroll
-  for (int i = 0; i < KEEP; ++i)
-    if (off[i] >= 0) amax = amax8<T>(keep[i], amax);
-  for (int x = first + KEEP * STEP; x < n; x += STEP)
-    if (s_off[x] >= 0) amax = amax8<T>(load8(src + x * stride), amax);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if (BLOCK) {
-    if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = amax;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < APPEND_THREADS / 32; ++w) amax = fmaxf(amax, s_red[w]);
-  }
-  const int e_old = fresh ? SCALE_E_MIN : scale_exponent(old_scale);
-  const int e = max(e_old, need_exponent(amax));
-  if (!fresh && e > e_old) {
-    const float f = e_old - e < -126 ? 0.f : pow2f(e_old - e);
-    uint4* p = reinterpret_cast<uint4*>(page_bytes);
-    for (int i = me; i < (D << a.page_shift) / 16; i += N) {
-      uint4 v = p[i];
-      v.x = rescale_e4m3x4(v.x, f);
-      v.y = rescale_e4m3x4(v.y, f);
-      v.z = rescale_e4m3x4(v.z, f);
-      v.w = rescale_e4m3x4(v.w, f);
-      p[i] = v;
-    }
-    // the new tokens' bytes lie in the range just rewritten, by other threads
-    if (BLOCK) __syncthreads();
-    else __syncwarp();
-  }
-  const float inv = pow2f(-e);
-  uint8_t* dst = page_bytes + (me % VPT) * 8;
-  auto put = [&](int o, const Vec8<T>& v) {
-    float x[8];
-    widen8<T>(v, x);
-    uint2 b;
-    b.x = to_e4m3x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-    b.y = to_e4m3x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
-    *reinterpret_cast<uint2*>(dst + o * D) = b;
-  };
-#pragma unroll
-  for (int i = 0; i < KEEP; ++i)
-    if (off[i] >= 0) put(off[i], keep[i]);
-  for (int x = first + KEEP * STEP; x < n; x += STEP)
-    if (s_off[x] >= 0) put(s_off[x], load8(src + x * stride));
-  __syncwarp();  // every lane has read the old scale
-  if (me == 0) *scale = pow2f(e);
+}
+template <typename T>
+__device__ __forceinline__ uint2 quantise8(const Vec8<T>& v, float inv) {
+  float x[8];
+  widen8<T>(v, x);
+  return make_uint2(to_e4m3x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv),
+                    to_e4m3x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv));
 }
 
-// grid: (window of tokens, kv head, k | v)
+// grid: (window of tokens, share of the 2 n_kv planes: heads of k, then of v)
 template <typename T, int D>
-__global__ void __launch_bounds__(APPEND_THREADS) append_cache_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(APPEND_THREADS, 2) append_cache_kernel(AppendArgs a) {
+  constexpr int VPT = D / 8, STEP = 32 / VPT;          // lanes per token, tokens (or heads) per warp
+  constexpr int KEEP = sizeof(T) == 4 ? 8 : 16;        // vectors of a lane kept between the passes
   __shared__ int32_t s_page[APPEND_MAX_WINDOW + 2 * APPEND_MAX_PAGE];  // page of each token near the window, -1: none
   __shared__ int16_t s_in[APPEND_MAX_WINDOW + 2 * APPEND_MAX_PAGE];    // its offset in the page
-  __shared__ int16_t s_off[APPEND_THREADS / 32][APPEND_MAX_PAGE];      // per warp: offsets of a run's tokens
-  __shared__ int16_t s_len[APPEND_MAX_WINDOW];  // tokens that a run spans (0: none begins here), negative: afresh
-  __shared__ float s_red[APPEND_THREADS / 32];
+  __shared__ int16_t s_one[APPEND_MAX_WINDOW], s_run[APPEND_MAX_WINDOW], s_len[APPEND_MAX_WINDOW];
+  __shared__ int s_ones, s_runs;
   const int64_t t0 = (int64_t)blockIdx.x * a.window;
   const int page = 1 << a.page_shift, back = (int)min((int64_t)page - 1, t0);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int have = (int)min((int64_t)(back + a.window + page - 1), a.T - t0 + back);
+  if (threadIdx.x == 0) s_ones = s_runs = 0;
   for (int i = threadIdx.x; i < have; i += APPEND_THREADS) {
     const int64_t s = a.slots[t0 - back + i];
     const int64_t id = s >> a.page_shift;
@@ -209,49 +161,122 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_cache_kernel(AppendArgs
   }
   __syncthreads();
   // a run begins where none of the `page - 1` tokens before lies in the same page, and spans the
-  // last of the `page - 1` tokens behind that does
-  for (int i = warp; i < a.window; i += APPEND_THREADS / 32) {
+  // last of the `page - 1` tokens behind that does; s_len is negative where it starts the page
+  for (int i = warp; i < a.window; i += APPEND_WARPS) {
     const int x = back + i;
+    if (x >= have || s_page[x] < 0) continue;
+    const int id = s_page[x];
+    bool older = x > 0 && s_page[x - 1] == id;  // a prompt's: no need to look further
+    if (!older) {
+      for (int y = x - 1 - lane; y >= max(0, x - page + 1); y -= 32) older |= s_page[y] == id;
+      older = __any_sync(0xffffffffu, older);
+    }
+    if (older) continue;
+    bool fresh = false;
     int len = 0;
-    if (x < have && s_page[x] >= 0) {
-      const int id = s_page[x];
-      bool older = false;
-      for (int y = x - 1 - lane; !__any_sync(0xffffffffu, older) && __any_sync(0xffffffffu, y >= max(0, x - page + 1)); y -= 32)
-        older = y >= max(0, x - page + 1) && s_page[y] == id;
-      if (!__any_sync(0xffffffffu, older)) {
-        bool fresh = false;
-        for (int y = x + lane; __any_sync(0xffffffffu, y < min(have, x + page)); y += 32) {
-          const bool mine = y < min(have, x + page) && s_page[y] == id;
-          fresh |= mine && s_in[y] == 0;
-          if (mine) len = y - x + 1;
-        }
-        len = __reduce_max_sync(0xffffffffu, len);
-        if (__any_sync(0xffffffffu, fresh)) len = -len;
+    for (int y = x + lane; y < min(have, x + page); y += 32)
+      if (s_page[y] == id) {
+        len = y - x + 1;
+        fresh |= s_in[y] == 0;
+      }
+    len = __reduce_max_sync(0xffffffffu, len);
+    fresh = __any_sync(0xffffffffu, fresh);
+    if (lane == 0) {
+      if (len == 1) {
+        s_one[atomicAdd(&s_ones, 1)] = (int16_t)x;
+      } else {
+        const int r = atomicAdd(&s_runs, 1);
+        s_run[r] = (int16_t)x;
+        s_len[r] = (int16_t)(fresh ? -len : len);
       }
     }
-    if (lane == 0) s_len[i] = (int16_t)len;
   }
   __syncthreads();
-  const int head = blockIdx.y, which = blockIdx.z;
-  // up to what a warp keeps in registers: a warp each; longer ones: the block, one after another
-  constexpr int SHORT = 32 * (sizeof(T) == 4 ? 2 : 4) * 8 / D;
-  for (int i = warp; i < a.window; i += APPEND_THREADS / 32) {
-    const int n = abs(s_len[i]);
-    if (n == 0 || n > SHORT) continue;
-    const int x = back + i, id = s_page[x];
-    __syncwarp();
-    if (lane < n) s_off[warp][lane] = s_page[x + lane] == id ? s_in[x + lane] : -1;
-    __syncwarp();
-    append_run<T, D, false>(a, which, head, t0 + i, n, id, s_len[i] < 0, s_off[warp], s_red);
+  const int planes = 2 * a.n_kv, share = (planes + gridDim.y - 1) / gridDim.y;
+  const int p0 = blockIdx.y * share, p1 = min(p0 + share, planes), n_planes = max(p1 - p0, 0);
+  const int64_t tok0 = t0 - back;
+
+  // ---- runs of one token: D/8 lanes each
+  const int per_one = (n_planes + STEP - 1) / STEP, ones = s_ones * per_one;
+  for (int w = warp; w < ones; w += APPEND_WARPS) {
+    const int x = s_one[w / per_one], pl = p0 + (w % per_one) * STEP + lane / VPT;
+    const bool live = pl < p1;
+    const bool is_v = pl >= a.n_kv;
+    const AppendSide side = is_v ? a.v : a.k;
+    const int head = is_v ? pl - a.n_kv : pl;
+    const int id = s_page[x], off = s_in[x];
+    const int64_t at = (int64_t)id * a.n_kv + head;
+    Vec8<T> v;
+    float amax = 0.f, old = 0.f;
+    if (live) {
+      old = side.scale[at];
+      v = load8(reinterpret_cast<const T*>(side.src) + (tok0 + x) * side.token_stride +
+                head * side.head_stride + (lane % VPT) * 8);
+      amax = amax8<T>(v, 0.f);
+    }
+#pragma unroll
+    for (int o = VPT / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const int e_old = off == 0 ? SCALE_E_MIN : scale_exponent(old);
+    const int e = max(e_old, need_exponent(amax));
+    uint8_t* bytes = side.cache + (at << a.page_shift) * D;
+    uint32_t grown = __ballot_sync(0xffffffffu, live && off != 0 && e > e_old && lane % VPT == 0);
+    while (grown) {  // the warp rewrites the pages one after another
+      const int from = __ffs(grown) - 1;
+      grown &= grown - 1;
+      rewrite_page(reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(bytes), from)),
+                   (D << a.page_shift) / 16, __shfl_sync(0xffffffffu, e_old - e, from));
+    }
+    __syncwarp();  // the new bytes lie in the range just rewritten; every lane has read the old scale
+    if (live) {
+      *reinterpret_cast<uint2*>(bytes + off * D + (lane % VPT) * 8) = quantise8<T>(v, pow2f(-e));
+      if (lane % VPT == 0) side.scale[at] = pow2f(e);
+    }
   }
-  for (int i = 0; i < a.window; ++i) {
-    const int n = abs(s_len[i]);
-    if (n <= SHORT) continue;
-    const int x = back + i, id = s_page[x];
-    __syncthreads();  // s_off and s_red are used again
-    for (int y = threadIdx.x; y < n; y += APPEND_THREADS) s_off[0][y] = s_page[x + y] == id ? s_in[x + y] : -1;
-    __syncthreads();
-    append_run<T, D, true>(a, which, head, t0 + i, n, id, s_len[i] < 0, s_off[0], s_red);
+
+  // ---- longer runs: a warp each
+  for (int w = warp; w < s_runs * n_planes; w += APPEND_WARPS) {
+    const int r = w / n_planes, x0 = s_run[r], n = abs(s_len[r]), pl = p0 + w % n_planes;
+    const bool fresh = s_len[r] < 0;
+    const bool is_v = pl >= a.n_kv;
+    const AppendSide side = is_v ? a.v : a.k;
+    const int head = is_v ? pl - a.n_kv : pl;
+    const int id = s_page[x0];
+    const int64_t at = (int64_t)id * a.n_kv + head, stride = side.token_stride;
+    const T* src = reinterpret_cast<const T*>(side.src) + (tok0 + x0) * stride + head * side.head_stride +
+                   (lane % VPT) * 8;
+    const float old = side.scale[at];
+    const int first = lane / VPT;
+    Vec8<T> keep[KEEP];
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+      const int y = first + i * STEP;
+      if (y < n && s_page[x0 + y] == id) keep[i] = load8(src + y * stride);
+    }
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+      const int y = first + i * STEP;
+      if (y < n && s_page[x0 + y] == id) amax = amax8<T>(keep[i], amax);
+    }
+    for (int y = first + KEEP * STEP; y < n; y += STEP)
+      if (s_page[x0 + y] == id) amax = amax8<T>(load8(src + y * stride), amax);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const int e_old = fresh ? SCALE_E_MIN : scale_exponent(old);
+    const int e = max(e_old, need_exponent(amax));
+    uint8_t* bytes = side.cache + (at << a.page_shift) * D;
+    if (!fresh && e > e_old) rewrite_page(bytes, (D << a.page_shift) / 16, e_old - e);
+    __syncwarp();  // as above
+    const float inv = pow2f(-e);
+    uint8_t* dst = bytes + (lane % VPT) * 8;
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+      const int y = first + i * STEP;
+      if (y < n && s_page[x0 + y] == id) *reinterpret_cast<uint2*>(dst + s_in[x0 + y] * D) = quantise8<T>(keep[i], inv);
+    }
+    for (int y = first + KEEP * STEP; y < n; y += STEP)
+      if (s_page[x0 + y] == id) *reinterpret_cast<uint2*>(dst + s_in[x0 + y] * D) = quantise8<T>(load8(src + y * stride), inv);
+    if (lane == 0) side.scale[at] = pow2f(e);
   }
 }
 
@@ -279,17 +304,18 @@ extern "C" int dsalt_append_cache(const void* k, const void* v, int dtype, int64
       ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) * es) % 16)
     return fail(DSALT_ERR_INVALID, "append_cache: rows must be 16-byte aligned");
   AppendArgs a;
-  a.src[0] = k, a.src[1] = v;
-  a.cache[0] = reinterpret_cast<uint8_t*>(k_cache), a.cache[1] = reinterpret_cast<uint8_t*>(v_cache);
-  a.scale[0] = k_scale, a.scale[1] = v_scale;
-  a.token_stride[0] = k_token_stride, a.token_stride[1] = v_token_stride;
-  a.head_stride[0] = k_head_stride, a.head_stride[1] = v_head_stride;
+  a.k = {k, reinterpret_cast<uint8_t*>(k_cache), k_scale, k_token_stride, k_head_stride};
+  a.v = {v, reinterpret_cast<uint8_t*>(v_cache), v_scale, v_token_stride, v_head_stride};
   a.slots = slots, a.T = T, a.n_pages = n_pages, a.n_kv = n_kv;
   a.page_shift = page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7;
-  // few tokens: windows of a warp per token, so that a decode step fills the GPU; many: windows
-  // of 64, so that a prompt's blocks find about one run each
-  a.window = (T + 7) / 8 * n_kv * 2 <= 148 * 16 ? 8 : APPEND_MAX_WINDOW;
-  const dim3 grid((unsigned)((T + a.window - 1) / a.window), (unsigned)n_kv, 2);
+  // few tokens: small windows, so that a decode step's runs spread over the GPU; many: larger
+  // ones, so that fewer blocks find no run. Planes are shared out until there are blocks enough
+  // (or each has no more planes than warps).
+  a.window = T <= 2048 ? 8 : APPEND_MAX_WINDOW;
+  const int64_t windows = (T + a.window - 1) / a.window;
+  const int per_warp = a.window == 8 ? 32 * 8 / head_dim : 1, most = (2 * n_kv + per_warp - 1) / per_warp;
+  const int64_t shares = std::min<int64_t>(most, std::max<int64_t>((148 * 16 + windows - 1) / windows, 1));
+  const dim3 grid((unsigned)windows, (unsigned)shares);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
 #define DSALT_APPEND(TT)                                                                    \
   (head_dim == 64 ? append_cache_kernel<TT, 64><<<grid, APPEND_THREADS, 0, s>>>(a)         \
