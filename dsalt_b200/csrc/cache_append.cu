@@ -27,7 +27,7 @@ namespace dsalt {
 
 constexpr int APPEND_THREADS = 256;
 constexpr int APPEND_WARPS = APPEND_THREADS / 32;
-constexpr int APPEND_MAX_WINDOW = 32;  // tokens whose runs one block looks for
+constexpr int APPEND_MAX_WINDOW = 64;  // tokens whose runs one block looks for
 constexpr int APPEND_MAX_PAGE = 128;
 constexpr int SCALE_E_MIN = -110;  // 2^-110 times the smallest byte is still a normal fp32
 
@@ -105,16 +105,50 @@ __device__ __forceinline__ void widen8(const Vec8<T>& v, float (&x)[8]) {
     }
   }
 }
+// Largest magnitude, as ordered bits: 16-bit types two to a word. Infinities and NaN come out
+// above every finite number and are looked for afterwards.
 template <typename T>
-__device__ __forceinline__ float amax8(const Vec8<T>& v, float amax) {
+__device__ __forceinline__ uint32_t max8(const Vec8<T>& v, uint32_t m) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      m = max(m, max(v.w[i].x & 0x7fffffffu, v.w[i].y & 0x7fffffffu));
+      m = max(m, max(v.w[i].z & 0x7fffffffu, v.w[i].w & 0x7fffffffu));
+    }
+  } else {
+    m = __vmaxu2(m, __vmaxu2(v.w[0].x & 0x7fff7fffu, v.w[0].y & 0x7fff7fffu));
+    m = __vmaxu2(m, __vmaxu2(v.w[0].z & 0x7fff7fffu, v.w[0].w & 0x7fff7fffu));
+  }
+  return m;
+}
+// the same over finite numbers alone
+template <typename T>
+__device__ __forceinline__ uint32_t max8_finite(const Vec8<T>& v, uint32_t m) {
   float x[8];
   widen8<T>(v, x);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float m = fabsf(x[j]);
-    amax = m < INFINITY ? fmaxf(amax, m) : amax;  // false for NaN as well
+    const float f = fabsf(x[j]);
+    if (!(f < INFINITY)) continue;
+    if constexpr (sizeof(T) == 4) m = max(m, __float_as_uint(f));
+    else if constexpr (std::is_same<T, __half>::value) m = __vmaxu2(m, __half_as_ushort(__float2half_rn(f)));
+    else m = __vmaxu2(m, __float_as_uint(f) >> 16);
   }
-  return amax;
+  return m;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t fold(uint32_t m) {  // the larger of the two halves
+  return sizeof(T) == 4 ? m : max(m & 0xffffu, m >> 16);
+}
+template <typename T>
+__device__ __forceinline__ bool finite_bits(uint32_t m) {
+  return m < (sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u);
+}
+template <typename T>
+__device__ __forceinline__ float bits_value(uint32_t m) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(m);
+  else if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)m));
+  else return __uint_as_float(m << 16);
 }
 
 // exponent of a run of one head, and the rewriting of the page's older bytes by the warp
@@ -141,18 +175,19 @@ __device__ __forceinline__ uint2 quantise8(const Vec8<T>& v, float inv) {
 
 // grid: (window of tokens, share of the 2 n_kv planes: heads of k, then of v)
 template <typename T, int D>
-__global__ void __launch_bounds__(APPEND_THREADS, 2) append_cache_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(APPEND_THREADS, 3) append_cache_kernel(AppendArgs a) {
   constexpr int VPT = D / 8, STEP = 32 / VPT;          // lanes per token, tokens (or heads) per warp
-  constexpr int KEEP = sizeof(T) == 4 ? 8 : 16;        // vectors of a lane kept between the passes
+  constexpr int KEEP = sizeof(T) == 4 ? 4 : 8;         // vectors of a lane in one chunk
   __shared__ int32_t s_page[APPEND_MAX_WINDOW + 2 * APPEND_MAX_PAGE];  // page of each token near the window, -1: none
   __shared__ int16_t s_in[APPEND_MAX_WINDOW + 2 * APPEND_MAX_PAGE];    // its offset in the page
   __shared__ int16_t s_one[APPEND_MAX_WINDOW], s_run[APPEND_MAX_WINDOW], s_len[APPEND_MAX_WINDOW];
-  __shared__ int s_ones, s_runs;
+  __shared__ int16_t s_cand[APPEND_MAX_WINDOW];
+  __shared__ int s_cands, s_ones, s_runs;
   const int64_t t0 = (int64_t)blockIdx.x * a.window;
   const int page = 1 << a.page_shift, back = (int)min((int64_t)page - 1, t0);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int have = (int)min((int64_t)(back + a.window + page - 1), a.T - t0 + back);
-  if (threadIdx.x == 0) s_ones = s_runs = 0;
+  if (threadIdx.x == 0) s_cands = s_ones = s_runs = 0;
   for (int i = threadIdx.x; i < have; i += APPEND_THREADS) {
     const int64_t s = a.slots[t0 - back + i];
     const int64_t id = s >> a.page_shift;
@@ -161,33 +196,38 @@ __global__ void __launch_bounds__(APPEND_THREADS, 2) append_cache_kernel(AppendA
   }
   __syncthreads();
   // a run begins where none of the `page - 1` tokens before lies in the same page, and spans the
-  // last of the `page - 1` tokens behind that does; s_len is negative where it starts the page
-  for (int i = warp; i < a.window; i += APPEND_WARPS) {
-    const int x = back + i;
-    if (x >= have || s_page[x] < 0) continue;
-    const int id = s_page[x];
-    bool older = x > 0 && s_page[x - 1] == id;  // a prompt's: no need to look further
-    if (!older) {
-      for (int y = x - 1 - lane; y >= max(0, x - page + 1); y -= 32) older |= s_page[y] == id;
-      older = __any_sync(0xffffffffu, older);
-    }
-    if (older) continue;
-    bool fresh = false;
+  // last of the `page - 1` tokens behind that does; s_len: its length, 0x100 where it holds the
+  // page's first token, 0x200 where its tokens follow one another without gaps
+  // (in a prompt most tokens follow one of their page: only the others are looked at closely)
+  if ((int)threadIdx.x < a.window) {
+    const int x = back + threadIdx.x;
+    if (x < have && s_page[x] >= 0 && (x == 0 || s_page[x - 1] != s_page[x]))
+      s_cand[atomicAdd(&s_cands, 1)] = (int16_t)x;
+  }
+  __syncthreads();
+  for (int i = warp; i < s_cands; i += APPEND_WARPS) {
+    const int x = s_cand[i], id = s_page[x];
+    bool older = false;
+    for (int y = x - 2 - lane; y >= max(0, x - page + 1); y -= 32) older |= s_page[y] == id;
+    if (__any_sync(0xffffffffu, older)) continue;
+    bool fresh = false, dense = true;
     int len = 0;
     for (int y = x + lane; y < min(have, x + page); y += 32)
       if (s_page[y] == id) {
         len = y - x + 1;
         fresh |= s_in[y] == 0;
+        dense &= s_in[y] - s_in[x] == y - x && s_page[y - (y > x)] == id;
       }
     len = __reduce_max_sync(0xffffffffu, len);
     fresh = __any_sync(0xffffffffu, fresh);
+    dense = __all_sync(0xffffffffu, dense);
     if (lane == 0) {
       if (len == 1) {
         s_one[atomicAdd(&s_ones, 1)] = (int16_t)x;
       } else {
         const int r = atomicAdd(&s_runs, 1);
         s_run[r] = (int16_t)x;
-        s_len[r] = (int16_t)(fresh ? -len : len);
+        s_len[r] = (int16_t)(len | (fresh ? 0x100 : 0) | (dense ? 0x200 : 0));
       }
     }
   }
@@ -207,15 +247,18 @@ __global__ void __launch_bounds__(APPEND_THREADS, 2) append_cache_kernel(AppendA
     const int id = s_page[x], off = s_in[x];
     const int64_t at = (int64_t)id * a.n_kv + head;
     Vec8<T> v;
-    float amax = 0.f, old = 0.f;
+    uint32_t top = 0;
+    float old = 0.f;
     if (live) {
       old = side.scale[at];
       v = load8(reinterpret_cast<const T*>(side.src) + (tok0 + x) * side.token_stride +
                 head * side.head_stride + (lane % VPT) * 8);
-      amax = amax8<T>(v, 0.f);
+      top = fold<T>(max8<T>(v, 0));
+      if (!finite_bits<T>(top)) top = fold<T>(max8_finite<T>(v, 0));
     }
 #pragma unroll
-    for (int o = VPT / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    for (int o = VPT / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float amax = bits_value<T>(top);
     const int e_old = off == 0 ? SCALE_E_MIN : scale_exponent(old);
     const int e = max(e_old, need_exponent(amax));
     uint8_t* bytes = side.cache + (at << a.page_shift) * D;
@@ -235,47 +278,66 @@ __global__ void __launch_bounds__(APPEND_THREADS, 2) append_cache_kernel(AppendA
 
   // ---- longer runs: a warp each
   for (int w = warp; w < s_runs * n_planes; w += APPEND_WARPS) {
-    const int r = w / n_planes, x0 = s_run[r], n = abs(s_len[r]), pl = p0 + w % n_planes;
-    const bool fresh = s_len[r] < 0;
+    const int r = w / n_planes, x0 = s_run[r], n = s_len[r] & 0xff, pl = p0 + w % n_planes;
+    const bool fresh = s_len[r] & 0x100, dense = s_len[r] & 0x200;
     const bool is_v = pl >= a.n_kv;
     const AppendSide side = is_v ? a.v : a.k;
     const int head = is_v ? pl - a.n_kv : pl;
-    const int id = s_page[x0];
+    const int id = s_page[x0], first = lane / VPT;
     const int64_t at = (int64_t)id * a.n_kv + head, stride = side.token_stride;
-    const T* src = reinterpret_cast<const T*>(side.src) + (tok0 + x0) * stride + head * side.head_stride +
+    const T* src = reinterpret_cast<const T*>(side.src) + (tok0 + x0 + first) * stride + head * side.head_stride +
                    (lane % VPT) * 8;
     const float old = side.scale[at];
-    const int first = lane / VPT;
-    Vec8<T> keep[KEEP];
-    float amax = 0.f;
-#pragma unroll
-    for (int i = 0; i < KEEP; ++i) {
-      const int y = first + i * STEP;
-      if (y < n && s_page[x0 + y] == id) keep[i] = load8(src + y * stride);
-    }
-#pragma unroll
-    for (int i = 0; i < KEEP; ++i) {
-      const int y = first + i * STEP;
-      if (y < n && s_page[x0 + y] == id) amax = amax8<T>(keep[i], amax);
-    }
-    for (int y = first + KEEP * STEP; y < n; y += STEP)
-      if (s_page[x0 + y] == id) amax = amax8<T>(load8(src + y * stride), amax);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const int e_old = fresh ? SCALE_E_MIN : scale_exponent(old);
-    const int e = max(e_old, need_exponent(amax));
     uint8_t* bytes = side.cache + (at << a.page_shift) * D;
+    uint8_t* dst = bytes + (lane % VPT) * 8;
+    // Chunks of KEEP vectors: all of a chunk's loads are under way at once. The last chunk stays in
+    // registers for the second pass, which takes the others from L1 or L2 again. A run with gaps
+    // or out of order goes token by token.
+    constexpr int CHUNK = KEEP * STEP;
+    const int chunks = dense ? (n + CHUNK - 1) / CHUNK : 0;
+    Vec8<T> keep[KEEP];
+    const auto load_chunk = [&](int c) {
+      const T* p = src + (int64_t)c * CHUNK * stride;
+      const int left = n - first - c * CHUNK;
+#pragma unroll
+      for (int i = 0; i < KEEP; ++i) {
+        if (i * STEP < left) keep[i] = load8(p);
+        p += STEP * stride;
+      }
+      return left;
+    };
+    const auto sparse = [&](auto&& f) {
+      for (int y = first; !dense && y < n; y += STEP)
+        if (s_page[x0 + y] == id) f(load8(src + (y - first) * stride), s_in[x0 + y]);
+    };
+    uint32_t top = 0;
+    for (int c = 0; c < chunks; ++c) {
+      const int left = load_chunk(c);
+#pragma unroll
+      for (int i = 0; i < KEEP; ++i)
+        if (i * STEP < left) top = max8<T>(keep[i], top);
+    }
+    sparse([&](const Vec8<T>& v, int) { top = max8<T>(v, top); });
+    top = __reduce_max_sync(0xffffffffu, fold<T>(top));
+    if (!finite_bits<T>(top)) {
+      uint32_t m = 0;
+      for (int y = first; y < n; y += STEP)
+        if (s_page[x0 + y] == id) m = max8_finite<T>(load8(src + (y - first) * stride), m);
+      top = __reduce_max_sync(0xffffffffu, fold<T>(m));
+    }
+    const int e_old = fresh ? SCALE_E_MIN : scale_exponent(old);
+    const int e = max(e_old, need_exponent(bits_value<T>(top)));
     if (!fresh && e > e_old) rewrite_page(bytes, (D << a.page_shift) / 16, e_old - e);
     __syncwarp();  // as above
     const float inv = pow2f(-e);
-    uint8_t* dst = bytes + (lane % VPT) * 8;
+    uint8_t* out = dst + (s_in[x0] + first) * D;
+    for (int c = chunks - 1; c >= 0; --c) {
+      const int left = c == chunks - 1 ? n - first - c * CHUNK : load_chunk(c);
 #pragma unroll
-    for (int i = 0; i < KEEP; ++i) {
-      const int y = first + i * STEP;
-      if (y < n && s_page[x0 + y] == id) *reinterpret_cast<uint2*>(dst + s_in[x0 + y] * D) = quantise8<T>(keep[i], inv);
+      for (int i = 0; i < KEEP; ++i)
+        if (i * STEP < left) *reinterpret_cast<uint2*>(out + (c * CHUNK + i * STEP) * D) = quantise8<T>(keep[i], inv);
     }
-    for (int y = first + KEEP * STEP; y < n; y += STEP)
-      if (s_page[x0 + y] == id) *reinterpret_cast<uint2*>(dst + s_in[x0 + y] * D) = quantise8<T>(load8(src + y * stride), inv);
+    sparse([&](const Vec8<T>& v, int off) { *reinterpret_cast<uint2*>(dst + off * D) = quantise8<T>(v, inv); });
     if (lane == 0) side.scale[at] = pow2f(e);
   }
 }
@@ -311,10 +373,10 @@ extern "C" int dsalt_append_cache(const void* k, const void* v, int dtype, int64
   // few tokens: small windows, so that a decode step's runs spread over the GPU; many: larger
   // ones, so that fewer blocks find no run. Planes are shared out until there are blocks enough
   // (or each has no more planes than warps).
-  a.window = T <= 2048 ? 8 : APPEND_MAX_WINDOW;
+  a.window = T <= 2048 ? 8 : page_size >= 64 ? 64 : 32;
   const int64_t windows = (T + a.window - 1) / a.window;
-  const int per_warp = a.window == 8 ? 32 * 8 / head_dim : 1, most = (2 * n_kv + per_warp - 1) / per_warp;
-  const int64_t shares = std::min<int64_t>(most, std::max<int64_t>((148 * 16 + windows - 1) / windows, 1));
+  const int planes = 2 * n_kv, most = a.window == 8 ? (planes + 256 / head_dim - 1) / (256 / head_dim) : planes;
+  const int64_t shares = std::min<int64_t>(most, std::max<int64_t>((148 * 2 + windows - 1) / windows, (planes + 7) / 8));
   const dim3 grid((unsigned)windows, (unsigned)shares);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
 #define DSALT_APPEND(TT)                                                                    \
