@@ -11,20 +11,25 @@
 // the draw among themselves, a row of nothing but -inf gives token 0 with log-probability -inf.
 //
 // No sort of the row: all three filters keep a prefix of one order, so there is one element
-// (key, index) at which the row is cut, and it is found by histograms of counts or masses.
-// Where at most LIST_CAP elements can matter they are gathered and settled in one block's
-// shared memory; otherwise the histogram's bin is refined until the cut is one element, and
-// the row is passed over again with it.
+// (key, index) at which the row is cut. Where at most LIST_CAP elements can matter they are
+// gathered and sorted in one block's shared memory, and the row is settled there:
+//   top-k: the k-th largest of the threads' own maxima is at most the k-th largest logit, so
+//          the elements from there on up hold the k first and few more;
+//   top-p: masses and counts of 16 bins of (m - l) / T, then of 16 parts of the bin where p is
+//          reached. Each thread has bins of its own (no atomics: a word per thread and bin).
+// Otherwise the bin is refined by histograms over (key, index) until the cut is one element,
+// and the row is passed over again with it.
 //
-// Masses are whole numbers, w * 2^43 rounded from a 64-bit exp: their sums do not depend on
-// the order in which threads arrive, so a row gives the same token in every batch and in
+// Masses are whole numbers, w * 2^43 rounded from 64-bit arithmetic: their sums do not depend
+// on the order in which threads arrive, so a row gives the same token in every batch and in
 // every run, and a border lies within 2^20 roundings of 2^-44 (6e-8 of the largest weight at
 // the very worst, about 1e-11 in practice) of where sums in 64-bit floating point put it.
 //
-// One cluster of C blocks owns a row; each block holds its share of the logits in shared
-// memory, so the row is read from HBM once. Histograms and lists are joined through
-// distributed shared memory.
+// One cluster of C blocks owns a row, each a share of it. The row comes from HBM once; later
+// passes find it in L1 or L2, which hold it for all rows under way.
 #include <cooperative_groups.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -34,20 +39,23 @@ namespace cg = cooperative_groups;
 
 constexpr int SAMPLE_THREADS = 512;
 constexpr int SAMPLE_WARPS = SAMPLE_THREADS / 32;
-constexpr int NBINS = 2 * SAMPLE_THREADS;     // two per thread where they are summed
-constexpr int LIST_CAP = 2 * SAMPLE_THREADS;  // two per thread where they are ranked
+constexpr int PBINS = SAMPLE_WARPS;           // private bins, one per warp where they are summed
+constexpr int NBINS = 2 * SAMPLE_THREADS;     // of a joint histogram, two per thread where they are summed
+constexpr int LIST_CAP = 2 * SAMPLE_THREADS;
 constexpr int IDX_BITS = 20;                  // vocabulary of at most 2^20
-constexpr int SAMPLE_MAX_SHARE = 131072;      // elements of one block: 2^17 limbs of 15 bits fit 32 bits
-constexpr int SAMPLE_SMEM_SHARE = 160 * 1024;  // bytes of logits that one block keeps in shared memory
+constexpr int BLOCK_ELEMS = 256;              // a warp's step: eight consecutive elements per lane
+constexpr int MAX_SHARE = 131328;             // 2^20 / 8 and a skew, in whole steps: 513 of them
+constexpr int MAX_BLOCKS = MAX_SHARE / BLOCK_ELEMS;
 constexpr double MASS_ONE = 8796093022208.0;  // 2^43: 2^20 of them stay below 2^63
-constexpr float BIN_SPAN = 32.f;              // (m - l) / T of the first histogram; its last bin takes the rest
+constexpr float BIN_SPAN = 32.f;              // (m - l) / T that the joint histogram covers
+constexpr float MIN_LOG2 = -45.f;             // weights below 2^-45 round to no mass
 
 typedef unsigned long long u64;
 
 struct SampleArgs {
   const void* logits;
   int64_t row_stride;
-  int V, share, in_smem;  // share: elements of one block
+  int V, share;  // share: elements of one block, a multiple of BLOCK_ELEMS
   const float* u;
   const float *temperature, *top_p, *min_p;  // per row, or null and the value below
   const int32_t* top_k;
@@ -57,48 +65,72 @@ struct SampleArgs {
   float* logprob;
 };
 
-// The lists are formed after a histogram has been read, in its place.
+// What one block holds. The arrays of a group share their memory: none outlives the next use.
 struct SampleShared {
   union {
+    u64 priv[PBINS][SAMPLE_THREADS];  // count (12 bits) and mass (52) of each thread's elements per bin
     struct {
-      uint32_t count[NBINS], limb[3][NBINS];  // this block's histogram; masses as three limbs
+      uint32_t count[NBINS], limb[3][NBINS];  // this block's joint histogram; masses as three limbs
     };
     struct {
       u64 sorted[LIST_CAP], weight[LIST_CAP];  // the leader's candidates in order, and their masses
+      uint32_t by_index[LIST_CAP];
     };
+    u64 steps[MAX_BLOCKS];  // mass of each step of the last pass
   };
   union {
     u64 mass[NBINS];     // joined over the cluster, in the leader's copy
     u64 item[LIST_CAP];  // candidates as they arrive, in the leader's copy
   };
   uint32_t total[NBINS];  // joined counts, in the leader's copy
-  uint32_t n_items;
-  // small exchanges; `result` is written by the leader only
-  u64 best, share_mass, range[2], result[4];
+  u64 bin_mass[2][PBINS];
+  uint32_t bin_count[2][PBINS];
+  uint32_t n_items, first_index;
+  float best;
+  u64 share_mass, range[2], result[4];  // result: written by the leader only
   u64 warp_red[SAMPLE_WARPS];
+  double exp2_16[16];  // 2^(j / 16)
 };
 
-// logits as unsigned keys that order as the logits do; NaN as -inf, -0 as 0
-__device__ __forceinline__ uint32_t logit_key(float l) { return order_f32(l == l ? l + 0.0f : -INFINITY); }
-__device__ __forceinline__ float key_logit(uint32_t k) {
-  return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
-}
 // (key, index) as one number: larger comes first in the order of the filters
-__device__ __forceinline__ u64 compose(uint32_t key, int idx) {
-  return ((u64)key << IDX_BITS) | (u64)((1 << IDX_BITS) - 1 - idx);
+__device__ __forceinline__ u64 compose(float l, int idx) {
+  return ((u64)order_f32(l + 0.0f) << IDX_BITS) | (u64)((1 << IDX_BITS) - 1 - idx);  // -0 as 0
 }
 __device__ __forceinline__ int index_of(u64 c) { return (1 << IDX_BITS) - 1 - (int)(c & ((1u << IDX_BITS) - 1)); }
-
-__device__ __forceinline__ float as_float(float v) { return v; }
-__device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-
-__device__ __forceinline__ double weight_of(float l, float top, double inv_t) {
-  if (l == top) return 1.0;
-  if (l == -INFINITY) return 0.0;  // at any temperature
-  return exp(((double)l - (double)top) * inv_t);
+__device__ __forceinline__ float logit_of(u64 c) {
+  const uint32_t k = (uint32_t)(c >> IDX_BITS);
+  return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
 }
-__device__ __forceinline__ u64 mass_of(double w) { return (u64)__double2ull_rn(w * MASS_ONE); }
+
+// Weights of one row. 2^t, t = (l - m) log2(e) / T: t = k / 16 + g with |g| <= 1/32, then
+// 2^(k/16) from a table of 16 and the exponent, 2^g by its Taylor series to the sixth power
+// (the seventh term is below (ln 2 / 32)^7 / 7! = 4.4e-16).
+struct Weights {
+  float top, l_min;
+  double c;
+  const double* table;
+  __device__ __forceinline__ double operator()(float l) const {  // 0 below l_min and for NaN
+    if (l == top) return 1.0;
+    if (!(l >= l_min)) return 0.0;
+    constexpr double MAGIC = 422212465065984.0;  // 1.5 * 2^48: adding it leaves steps of 1/16
+    constexpr double C1 = 0.6931471805599453094, C2 = C1 * C1 / 2, C3 = C2 * C1 / 3, C4 = C3 * C1 / 4, C5 = C4 * C1 / 5,
+                     C6 = C5 * C1 / 6;
+    const double t = ((double)l - (double)top) * c, r = t + MAGIC;
+    const int k = __double2loint(r);
+    const double g = t - (r - MAGIC);
+    double p = fma(g, C6, C5);
+    p = fma(p, g, C4);
+    p = fma(p, g, C3);
+    p = fma(p, g, C2);
+    p = fma(p, g, C1);
+    p = fma(p, g, 1.0) * table[k & 15];
+    return __hiloint2double(__double2hiint(p) + ((k >> 4) << 20), __double2loint(p));
+  }
+  __device__ __forceinline__ u64 mass(double w) const {  // w * 2^43 to the nearest whole number
+    return (u64)__double_as_longlong(fma(w, MASS_ONE, 4503599627370496.0)) & 0xfffffffffffffull;  // + 2^52
+  }
+  __device__ __forceinline__ u64 mass(float l) const { return mass((*this)(l)); }
+};
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
 #pragma unroll
@@ -140,29 +172,6 @@ __device__ __forceinline__ u64 part_of(double p, u64 mass) {
   if (!(x >= 1.0)) return 1;
   return x >= (double)mass ? mass : (u64)x;
 }
-
-// Sorts the leader's n <= LIST_CAP items by counting the larger ones, and forms their masses.
-__device__ void sort_items(SampleShared& sh, int n, float top, double inv_t) {
-  __syncthreads();
-  const u64 a = (int)threadIdx.x < n ? sh.item[threadIdx.x] : 0;
-  const u64 b = (int)threadIdx.x + SAMPLE_THREADS < n ? sh.item[threadIdx.x + SAMPLE_THREADS] : 0;
-  int ra = 0, rb = 0;
-  for (int j = 0; j < n; ++j) {
-    const u64 o = sh.item[j];
-    ra += o > a;
-    rb += o > b;
-  }
-  if ((int)threadIdx.x < n) {
-    sh.sorted[ra] = a;
-    sh.weight[ra] = mass_of(weight_of(key_logit((uint32_t)(a >> IDX_BITS)), top, inv_t));
-  }
-  if ((int)threadIdx.x + SAMPLE_THREADS < n) {
-    sh.sorted[rb] = b;
-    sh.weight[rb] = mass_of(weight_of(key_logit((uint32_t)(b >> IDX_BITS)), top, inv_t));
-  }
-  __syncthreads();
-}
-
 // u * total as the whole number that the drawn running sum has to exceed
 __device__ __forceinline__ u64 target_of(float u, u64 total) {
   const double x = (double)u * (double)total;
@@ -170,48 +179,75 @@ __device__ __forceinline__ u64 target_of(float u, u64 total) {
   return x >= (double)total ? total - 1 : min((u64)x, total - 1);
 }
 
-// The leader's block settles a row whose candidates are all in its list: `keep` of them in
-// order are within top-k; `want` > 0 is the mass that top-p has to reach, else it is formed here.
-__device__ void settle_list(const SampleArgs& a, SampleShared& sh, int row, int keep, bool cut_p, double top_p, u64 want,
-                            double min_p, float u, float top, double inv_t) {
+// bitonic sort of size (a power of two) values in shared memory by the block
+template <typename T, bool DESCENDING>
+__device__ __forceinline__ void block_sort(T* v, int size) {
+  for (int k = 2; k <= size; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < size / 2; i += SAMPLE_THREADS) {
+        const int x = 2 * i - (i & (j - 1)), y = x + j;
+        const T a = v[x], b = v[y];
+        if (((x & k) == 0) == (DESCENDING ? a < b : a > b)) {
+          v[x] = b;
+          v[y] = a;
+        }
+      }
+    }
+  __syncthreads();
+}
+__device__ __forceinline__ int power_of_two(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
+
+// Sorts the leader's n <= LIST_CAP items and forms their masses.
+__device__ __forceinline__ void sort_items(SampleShared& sh, int n, const Weights& wt) {
+  const int size = power_of_two(n);
+  __syncthreads();
+  for (int i = threadIdx.x; i < size; i += SAMPLE_THREADS) sh.sorted[i] = i < n ? sh.item[i] : 0;
+  block_sort<u64, true>(sh.sorted, size);
+  for (int i = threadIdx.x; i < n; i += SAMPLE_THREADS) sh.weight[i] = wt.mass(logit_of(sh.sorted[i]));
+  __syncthreads();
+}
+
+// The leader's block settles a row whose candidates are all in its sorted list: `keep` of them
+// are within top-k; `want` > 0 is the mass that top-p has to reach, else it is formed here.
+__device__ __forceinline__ void settle_list(const SampleArgs& a, SampleShared& sh, int row, int keep, bool cut_p,
+                                            double top_p, u64 want, double min_p, float u, const Weights& wt) {
   const int i0 = 2 * threadIdx.x, i1 = i0 + 1;
-  u64 w0 = i0 < keep ? sh.weight[i0] : 0, w1 = i1 < keep ? sh.weight[i1] : 0;
+  const u64 w0 = i0 < keep ? sh.weight[i0] : 0, w1 = i1 < keep ? sh.weight[i1] : 0;
   if (cut_p) {
     if (want == 0) want = part_of(top_p, block_sum(w0 + w1, sh));
     const u64 before = block_before(w0 + w1, sh);
     keep = (int)block_sum((u64)(i0 < keep && before < want) + (u64)(i1 < keep && before + w0 < want), sh);
   }
   if (min_p > 0) {
-    const auto ok = [&](int i) {
-      return i < keep && weight_of(key_logit((uint32_t)(sh.sorted[i] >> IDX_BITS)), top, inv_t) >= min_p;
-    };
+    const auto ok = [&](int i) { return i < keep && wt(logit_of(sh.sorted[i])) >= min_p; };
     keep = max(1, (int)block_sum((u64)ok(i0) + (u64)ok(i1), sh));
   }
-  const u64 total = block_sum((i0 < keep ? w0 : 0) + (i1 < keep ? w1 : 0), sh);
-  const u64 target = target_of(u, total);
-  // running sum in index order: a lower index is a larger low part of the item
-  for (int i = threadIdx.x; i < keep; i += SAMPLE_THREADS) {
-    const int mine = index_of(sh.sorted[i]);
-    u64 before = 0;
-    for (int j = 0; j < keep; ++j) before += index_of(sh.sorted[j]) < mine ? sh.weight[j] : 0;
-    if (before <= target && target < before + sh.weight[i]) {
-      a.token[row] = mine;
-      if (a.logprob) a.logprob[row] = (float)log((double)sh.weight[i] / (double)total);
-    }
+  // in index order: (index, place) sorted, then a running sum
+  const int size = power_of_two(keep);
+  for (int i = threadIdx.x; i < size; i += SAMPLE_THREADS)
+    sh.by_index[i] = i < keep ? ((uint32_t)index_of(sh.sorted[i]) << 10) | (uint32_t)i : 0xffffffffu;
+  block_sort<uint32_t, false>(sh.by_index, size);
+  static_assert(LIST_CAP == 1 << 10 && IDX_BITS + 10 <= 30, "index and place share a word");
+  const u64 m0 = i0 < keep ? sh.weight[sh.by_index[i0] & 1023] : 0, m1 = i1 < keep ? sh.weight[sh.by_index[i1] & 1023] : 0;
+  const u64 total = block_sum(m0 + m1, sh), before = block_before(m0 + m1, sh), target = target_of(u, total);
+  if (before <= target && target < before + m0 + m1) {  // one thread
+    const bool second = target >= before + m0;
+    a.token[row] = sh.by_index[second ? i1 : i0] >> 10;
+    if (a.logprob) a.logprob[row] = (float)log((double)(second ? m1 : m0) / (double)total);
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(SampleArgs a) {
+__global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a) {
   extern __shared__ __align__(16) unsigned char dyn[];
-  __shared__ SampleShared sh;
+  SampleShared& sh = *reinterpret_cast<SampleShared*>(dyn);
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int row = blockIdx.x / C;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   SampleShared* lead = cluster.map_shared_rank(&sh, 0);
-  const int lo = min(rank * a.share, a.V), n = min(lo + a.share, a.V) - lo;
-  const T* src = reinterpret_cast<const T*>(a.logits) + (int64_t)row * a.row_stride + lo;
+  const T* src = reinterpret_cast<const T*>(a.logits) + (int64_t)row * a.row_stride;
 
   const float temp = a.temperature ? a.temperature[row] : a.temperature_v;
   const double top_p = a.top_p ? (double)a.top_p[row] : (double)a.top_p_v;
@@ -219,249 +255,416 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(SampleArgs a) {
   const int top_k = a.top_k ? a.top_k[row] : a.top_k_v;
   const float u = a.u[row];
   const bool cut_k = top_k > 0 && top_k < a.V, cut_p = top_p < 1.0;
-  const double inv_t = 1.0 / (double)temp;
-  const float bin_scale = (float)inv_t * (NBINS / BIN_SPAN);
 
-  // ---- the share into shared memory; its first element in the order
-  const T* val = src;
-  u64 best = 0;
-  auto see = [&](T v, int at) {
-    const u64 c = compose(logit_key(as_float(v)), lo + at);
-    best = c > best ? c : best;
+  // ---- the share, in steps of a warp: eight consecutive elements per lane. Places are counted
+  // from the 16-byte boundary at or before the row's start, so that whole vectors can be read.
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const int skew = (int)(((uintptr_t)src & 15) / sizeof(T));
+  const int place0 = rank * a.share, n_steps = (max(0, min(a.share, a.V + skew - place0)) + BLOCK_ELEMS - 1) / BLOCK_ELEMS;
+  const auto load = [&](int step, float (&l)[8]) -> int {  // NaN outside the row; returns the first index
+    const int i0 = place0 + step * BLOCK_ELEMS + lane * 8 - skew;
+    if (i0 >= 0 && i0 + 8 <= a.V) {
+#pragma unroll
+      for (int h = 0; h < 8 / VEC; ++h) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + i0) + h);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (sizeof(T) == 4) {
+            l[4 * h + e] = __uint_as_float(w[e]);
+          } else if constexpr (std::is_same<T, __half>::value) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+            l[2 * e] = f.x, l[2 * e + 1] = f.y;
+          } else {
+            l[2 * e] = __uint_as_float(w[e] << 16), l[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        l[e] = __int_as_float(0x7fffffff);
+        if (i0 + e >= 0 && i0 + e < a.V) {
+          if constexpr (sizeof(T) == 4) l[e] = src[i0 + e];
+          else if constexpr (std::is_same<T, __half>::value) l[e] = __half2float(src[i0 + e]);
+          else l[e] = __bfloat162float(src[i0 + e]);
+        }
+      }
+    }
+    return i0;
   };
-  if (a.in_smem) {
-    constexpr int VEC = 16 / (int)sizeof(T);
-    const int skew = (int)(((uintptr_t)src & 15) / sizeof(T));  // the copy keeps the source's alignment
-    T* buf = reinterpret_cast<T*>(dyn) + skew;
-    const int head = min(n, (VEC - skew) % VEC), body = (n - head) / VEC;
-    for (int i = tid; i < body; i += SAMPLE_THREADS) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + head) + i);
-      *reinterpret_cast<uint4*>(buf + head + i * VEC) = v;
-      const T* e = reinterpret_cast<const T*>(&v);
+  const auto for_each = [&](auto&& f) {  // every element of the share, NaN and places outside too
+#pragma unroll 2
+    for (int step = warp; step < n_steps; step += SAMPLE_WARPS) {
+      float l[8];
+      const int i0 = load(step, l);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) see(e[j], head + i * VEC + j);
+      for (int e = 0; e < 8; ++e) f(l[e], i0 + e);
     }
-    for (int i = tid; i < n - body * VEC; i += SAMPLE_THREADS) {
-      const int at = i < head ? i : i + body * VEC;
-      buf[at] = src[at];
-      see(src[at], at);
-    }
-    val = buf;
-  } else {
-    for (int i = tid; i < n; i += SAMPLE_THREADS) see(src[i], i);
-  }
+  };
+
+  // ---- the largest logit
+  float mine = -INFINITY;
+#pragma unroll 4
+  for (int step = warp; step < n_steps; step += SAMPLE_WARPS) {
+    float l[8];
+    load(step, l);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const u64 c = __shfl_xor_sync(0xffffffffu, best, o);
-    best = c > best ? c : best;
+    for (int e = 0; e < 8; ++e) mine = fmaxf(mine, l[e]);  // passes over NaN
   }
-  if (lane == 0) sh.warp_red[warp] = best;
-  auto clear_bins = [&] {
+  float top = mine;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) sh.warp_red[warp] = __float_as_uint(top);
+  if (tid < 16) sh.exp2_16[tid] = exp2((double)tid / 16);
+  if (tid == 0) {
+    sh.first_index = 0xffffffffu;
+    sh.n_items = 0;
+  }
+  const auto clear_bins = [&] {
     for (int i = tid; i < NBINS; i += SAMPLE_THREADS) sh.count[i] = sh.limb[0][i] = sh.limb[1][i] = sh.limb[2][i] = 0;
   };
   clear_bins();
   __syncthreads();
-  if (tid == 0) {
-    u64 b = 0;
-    for (int w = 0; w < SAMPLE_WARPS; ++w) b = sh.warp_red[w] > b ? sh.warp_red[w] : b;
-    sh.best = b;
-  }
+#pragma unroll
+  for (int w = 0; w < SAMPLE_WARPS; ++w) top = fmaxf(top, __uint_as_float((uint32_t)sh.warp_red[w]));
+  if (tid == 0) sh.best = top;
   cluster.sync();
-  for (int r = 0; r < C; ++r) {
-    const u64 b = cluster.map_shared_rank(&sh, r)->best;
-    best = b > best ? b : best;
-  }
-  const float top = key_logit((uint32_t)(best >> IDX_BITS));
+  for (int r = 0; r < C; ++r) top = fmaxf(top, cluster.map_shared_rank(&sh, r)->best);
   // every decision from here to the end is the same in all threads of the cluster
   if (!(temp > 0.f) || top == -INFINITY) {
+    if (top > -INFINITY) {
+      uint32_t first = 0xffffffffu;
+      for_each([&](float l, int i) {
+        if (l == top) first = min(first, (uint32_t)i);
+      });
+      first = __reduce_min_sync(0xffffffffu, first);
+      if (lane == 0 && first != 0xffffffffu) atomicMin(&lead->first_index, first);
+    }
+    cluster.sync();
     if (rank == 0 && tid == 0) {
-      a.token[row] = top == -INFINITY ? 0 : index_of(best);
+      a.token[row] = top == -INFINITY ? 0 : sh.first_index;
       if (a.logprob) a.logprob[row] = top == -INFINITY ? -INFINITY : 0.f;
     }
-    cluster.sync();  // a block's shared memory stays until the others have read it
-    return;
+    return;  // (the others' shared memory was last read before the barrier)
   }
+  Weights wt;
+  wt.top = top;
+  wt.c = 1.4426950408889634 / (double)temp;
+  wt.l_min = top == INFINITY ? INFINITY : fmaxf((float)((double)top + (double)MIN_LOG2 / wt.c), -3.402823466e38f);
+  wt.table = sh.exp2_16;
+  const float inv_t = (float)(1.0 / (double)temp);
+  const auto z_of = [&](float l) { return l == top ? 0.f : (top - l) * inv_t; };  // grows as l falls, at least 0
 
   u64 cut = 0;  // elements below it are dropped
-  bool listed = false;
-  for (int pass = cut_k ? 0 : 1; pass < (cut_p ? 2 : 1) && !listed; ++pass) {
-    const bool by_mass = pass == 1;
-    u64 want = by_mass ? 0 : (u64)top_k;  // the mass to reach is known once all masses are summed
-    u64 above = 0;                        // count or mass before the bins
-    u64 floor_c = cut, ceil_c = ~0ull;
-    int shift = -1;  // -1: bins of (m - l) / T; else bins of 2^shift composed numbers from ceil_c down
-    int bin = 0;
-    u64 bin_count = 0;
-    auto first_bin = [&](float l) { return l == top ? 0 : (int)fminf((top - l) * bin_scale, (float)(NBINS - 1)); };
-    while (true) {
-      for (int i = tid; i < n; i += SAMPLE_THREADS) {
-        const uint32_t key = logit_key(as_float(val[i]));
-        const u64 c = compose(key, lo + i);
-        if (c < floor_c || c > ceil_c) continue;
-        const float l = key_logit(key);
-        const int b = shift < 0 ? first_bin(l) : (int)((ceil_c - c) >> shift);
-        atomicAdd(&sh.count[b], 1u);
-        if (by_mass) {
-          const u64 w = mass_of(weight_of(l, top, inv_t));
-          atomicAdd(&sh.limb[0][b], (uint32_t)(w & 0x7fff));
-          atomicAdd(&sh.limb[1][b], (uint32_t)(w >> 15) & 0x7fff);
-          atomicAdd(&sh.limb[2][b], (uint32_t)(w >> 30));
-        }
+  // A list of all that can stay, from `in` on: sorted and settled by the leader.
+  const auto gather = [&](auto&& in) {
+    for_each([&](float l, int i) {
+      if (l > -INFINITY && in(l, i)) {
+        const uint32_t at = atomicAdd(&lead->n_items, 1u);
+        if (at < LIST_CAP) lead->item[at] = compose(l, i);
       }
-      cluster.sync();
-      // each block joins its part of the bins into the leader
-      for (int b = rank * SAMPLE_THREADS + tid; b < NBINS; b += C * SAMPLE_THREADS) {
-        uint32_t cnt = 0;
-        u64 ms = 0;
-        for (int r = 0; r < C; ++r) {
-          const SampleShared* o = cluster.map_shared_rank(&sh, r);
-          cnt += o->count[b];
-          if (by_mass) ms += (u64)o->limb[0][b] + ((u64)o->limb[1][b] << 15) + ((u64)o->limb[2][b] << 30);
-        }
-        lead->total[b] = cnt;
-        lead->mass[b] = ms;
+    });
+    cluster.sync();
+  };
+
+  // ---- a small top-k: elements down to the k-th largest of the threads' maxima
+  const auto joint_bin = [&](float l) { return (int)fminf(z_of(l) * (NBINS / BIN_SPAN), (float)(NBINS - 1)); };
+  const auto join_bins = [&](bool by_mass) {  // each block joins its part of the bins into the leader
+    cluster.sync();
+    for (int b = rank * SAMPLE_THREADS + tid; b < NBINS; b += C * SAMPLE_THREADS) {
+      uint32_t cnt = 0;
+      u64 ms = 0;
+      for (int r = 0; r < C; ++r) {
+        const SampleShared* o = cluster.map_shared_rank(&sh, r);
+        cnt += o->count[b];
+        if (by_mass) ms += (u64)o->limb[0][b] + ((u64)o->limb[1][b] << 15) + ((u64)o->limb[2][b] << 30);
       }
-      cluster.sync();
-      clear_bins();  // for the next histogram
-      if (rank == 0) {
-        // the first bin whose running sum reaches `want`
-        const uint32_t c0 = sh.total[2 * tid], c1 = sh.total[2 * tid + 1];
-        const u64 v0 = by_mass ? sh.mass[2 * tid] : c0, v1 = by_mass ? sh.mass[2 * tid + 1] : c1;
-        if (want == 0) want = part_of(top_p, block_sum(v0 + v1, sh));
-        const u64 before = above + block_before(v0 + v1, sh);
-        const u64 cnt_before = block_before((u64)c0 + c1, sh);
-        if (before < want && before + v0 + v1 >= want) {  // one thread: the sums only grow
-          const bool second = before + v0 < want;
-          sh.result[0] = (u64)(2 * tid + second) | ((u64)(second ? c1 : c0) << 32);
-          sh.result[1] = before + (second ? v0 : 0);
-          sh.result[2] = cnt_before + c0 + (second ? c1 : 0);  // elements up to and with the bin
-          sh.result[3] = want;
-        }
-        if (tid == 0) sh.n_items = 0;
-      }
-      cluster.sync();
-      bin = (int)(uint32_t)lead->result[0];
-      bin_count = lead->result[0] >> 32;
-      above = lead->result[1];
-      want = lead->result[3];
-      if (shift < 0) {
-        if (lead->result[2] <= LIST_CAP) {
-          listed = true;  // everything that can stay fits the list
-          break;
-        }
-        // the composed numbers that the bin spans
-        u64 first = ~0ull, last = 0;
-        for (int i = tid; i < n; i += SAMPLE_THREADS) {
-          const uint32_t key = logit_key(as_float(val[i]));
-          const u64 c = compose(key, lo + i);
-          if (c < floor_c || first_bin(key_logit(key)) != bin) continue;
-          first = min(first, c);
-          last = max(last, c);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
-          last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
-        }
-        __syncthreads();
-        if (tid == 0) {
-          sh.range[0] = ~0ull;
-          sh.range[1] = 0;
-        }
-        __syncthreads();
-        if (lane == 0) {
-          atomicMin(&sh.range[0], first);
-          atomicMax(&sh.range[1], last);
-        }
-        cluster.sync();
-        for (int r = 0; r < C; ++r) {
-          const SampleShared* o = cluster.map_shared_rank(&sh, r);
-          first = min(first, o->range[0]);
-          last = max(last, o->range[1]);
-        }
-        floor_c = first;
-        ceil_c = last;
-        cluster.sync();  // `range` may be used again
-      } else {
-        ceil_c -= (u64)bin << shift;
-        const u64 size = 1ull << shift;
-        if (ceil_c - floor_c >= size) floor_c = ceil_c - size + 1;
-      }
-      if (bin_count <= LIST_CAP) {
-        // the bin's elements decide: sort them, the cut is the one at which `want` is reached
-        for (int i = tid; i < n; i += SAMPLE_THREADS) {
-          const u64 c = compose(logit_key(as_float(val[i])), lo + i);
-          if (c >= floor_c && c <= ceil_c) lead->item[atomicAdd(&lead->n_items, 1u)] = c;
-        }
-        cluster.sync();
-        if (rank == 0) {
-          sort_items(sh, (int)bin_count, top, inv_t);
-          const int i0 = 2 * tid, i1 = i0 + 1, m = (int)bin_count;
-          const u64 w0 = i0 < m ? (by_mass ? sh.weight[i0] : 1) : 0, w1 = i1 < m ? (by_mass ? sh.weight[i1] : 1) : 0;
-          const u64 before = above + block_before(w0 + w1, sh);
-          if (before < want && before + w0 + w1 >= want) sh.result[0] = sh.sorted[before + w0 < want ? i1 : i0];
-        }
-        cluster.sync();
-        cut = lead->result[0];
-        clear_bins();  // the leader's held the list
-        __syncthreads();
-        break;
-      }
-      const u64 width = ceil_c - floor_c;
-      shift = max(0, 64 - __clzll((long long)width) - 10);  // width >> shift < NBINS = 2^10
+      lead->total[b] = cnt;
+      lead->mass[b] = ms;
     }
-    if (listed) {
-      for (int i = tid; i < n; i += SAMPLE_THREADS) {
-        const uint32_t key = logit_key(as_float(val[i]));
-        const u64 c = compose(key, lo + i);
-        if (c >= cut && first_bin(key_logit(key)) <= bin) lead->item[atomicAdd(&lead->n_items, 1u)] = c;
+    cluster.sync();
+  };
+  // the leader: the first bin whose running sum reaches `want` (there is one): result = bin and its
+  // count, sum before it, elements up to and with it
+  const auto find_bin = [&](bool by_mass, u64 above, u64 want) {
+    if (rank == 0) {
+      const uint32_t c0 = sh.total[2 * tid], c1 = sh.total[2 * tid + 1];
+      const u64 v0 = by_mass ? sh.mass[2 * tid] : c0, v1 = by_mass ? sh.mass[2 * tid + 1] : c1;
+      const u64 before = above + block_before(v0 + v1, sh);
+      const u64 cnt_before = block_before((u64)c0 + c1, sh);
+      if (before < want && before + v0 + v1 >= want) {  // one thread: the sums only grow
+        const bool second = before + v0 < want;
+        sh.result[0] = (u64)(2 * tid + second) | ((u64)(second ? c1 : c0) << 32);
+        sh.result[1] = before + (second ? v0 : 0);
+        sh.result[2] = cnt_before + c0 + (second ? c1 : 0);
       }
-      cluster.sync();
+      if (tid == 0) sh.n_items = 0;
+    }
+    cluster.sync();
+  };
+  bool k_done = !cut_k;
+  if (cut_k && top_k <= LIST_CAP / 2 && top_k <= C * SAMPLE_THREADS / 4) {
+    if (mine > -INFINITY) atomicAdd(&sh.count[joint_bin(mine)], 1u);
+    if (rank == 0 && tid == 0) sh.result[0] = NBINS - 1;  // fewer maxima than k: every element
+    join_bins(false);
+    find_bin(false, 0, (u64)top_k);
+    const int bin = (int)(uint32_t)lead->result[0];
+    gather([&](float l, int) { return joint_bin(l) <= bin; });
+    const uint32_t m = lead->n_items;
+    if (m <= LIST_CAP) {
       if (rank == 0) {
-        const int m = (int)sh.n_items;
-        sort_items(sh, m, top, inv_t);
-        settle_list(a, sh, row, by_mass ? m : min(m, top_k), cut_p, top_p, by_mass ? want : 0, min_p, u, top, inv_t);
+        sort_items(sh, (int)m, wt);
+        settle_list(a, sh, row, min((int)m, top_k), cut_p, top_p, 0, min_p, u, wt);
       }
-      // the others' shared memory is no longer read, theirs of the leader neither
+      cluster.sync();  // the leader's count may still be read
       return;
     }
+    cluster.sync();
+    if (rank == 0 && tid == 0) sh.n_items = 0;
   }
 
-  // ---- many elements stay: a pass over the row. Each thread sums a stretch of the share (an
-  // odd number of elements, so that the threads' stretches start in different banks).
-  const int per = ((n + SAMPLE_THREADS - 1) / SAMPLE_THREADS) | 1;
-  const int from = min(tid * per, n), to = min(from + per, n);
-  auto kept_mass = [&](int i) -> u64 {
-    const uint32_t key = logit_key(as_float(val[i]));
-    if (compose(key, lo + i) < cut) return 0;
-    const double w = weight_of(key_logit(key), top, inv_t);
-    return w >= min_p ? mass_of(w) : 0;
+  // ---- the cut of a wide top-k (by count), then of top-p (by mass)
+  for (int pass = k_done ? 1 : 0; pass < (cut_p ? 2 : 1); ++pass) {
+    const bool by_mass = pass == 1;
+    u64 want = by_mass ? 0 : (u64)top_k;  // the mass to reach is known once all masses are summed
+    u64 above = 0, upto = 0, bin_elems = 0;
+    float z0 = 0.f, z_scale = 1.f;  // bins of 1, then of 1/16 from z0
+    bool inside_last = false, enough = true;
+    const auto private_bin = [&](float l) -> int {  // -1: not in the range
+      const float z = z_of(l) - z0;
+      if (z < 0.f || (z_scale > 1.f && !inside_last && z >= 1.f)) return -1;
+      return (int)fminf(z * z_scale, (float)(PBINS - 1));
+    };
+    int bin = 0;
+    for (int level = 0; level < 2; ++level) {
+      __syncthreads();
+#pragma unroll
+      for (int b = 0; b < PBINS; ++b) sh.priv[b][tid] = 0;
+      for_each([&](float l, int i) {
+        if (!(l > -INFINITY) || (cut != 0 && compose(l, i) < cut)) return;
+        const int b = private_bin(l);
+        if (b >= 0) sh.priv[b][tid] += (1ull << 52) + (by_mass ? wt.mass(l) : 0);
+      });
+      __syncthreads();
+      {  // a warp per bin
+        u64 ms = 0;
+        uint32_t cnt = 0;
+        for (int i = lane; i < SAMPLE_THREADS; i += 32) {
+          const u64 v = sh.priv[warp][i];
+          ms += v & 0xfffffffffffffull;
+          cnt += (uint32_t)(v >> 52);
+        }
+        ms = warp_sum(ms);
+        cnt = __reduce_add_sync(0xffffffffu, cnt);
+        if (lane == 0) {
+          sh.bin_mass[level][warp] = ms;
+          sh.bin_count[level][warp] = cnt;
+        }
+      }
+      cluster.sync();
+      // every block finds the bin for itself
+      u64 ms = 0, cnt = 0;
+      if (lane < PBINS)
+        for (int r = 0; r < C; ++r) {
+          const SampleShared* o = cluster.map_shared_rank(&sh, r);
+          ms += o->bin_mass[level][lane];
+          cnt += o->bin_count[level][lane];
+        }
+      const u64 v = by_mass ? ms : cnt;
+      if (want == 0) want = part_of(top_p, warp_sum(v));
+      u64 sv = v, sc = cnt;
+#pragma unroll
+      for (int o = 1; o < PBINS; o <<= 1) {
+        const u64 x = __shfl_up_sync(0xffffffffu, sv, o), y = __shfl_up_sync(0xffffffffu, sc, o);
+        if (lane >= o) sv += x, sc += y;
+      }
+      const uint32_t reached = __ballot_sync(0xffffffffu, lane < PBINS && above + sv >= want);
+      if (reached == 0) {  // fewer finite logits than k: nothing to cut
+        enough = false;
+        break;
+      }
+      bin = __ffs(reached) - 1;
+      const u64 before_v = __shfl_sync(0xffffffffu, sv - v, bin), before_c = __shfl_sync(0xffffffffu, sc - cnt, bin);
+      bin_elems = __shfl_sync(0xffffffffu, cnt, bin);
+      above += before_v;
+      upto = (level == 0 ? 0 : upto) + before_c;  // elements before the bin
+      if (level == 0) {
+        if (bin_elems + upto <= LIST_CAP) break;
+        z0 = (float)bin;
+        z_scale = (float)PBINS;
+        inside_last = bin == PBINS - 1;
+      }
+    }
+    if (!enough) {
+      cluster.sync();  // the others' sums may still be read
+      continue;
+    }
+    const float z_low = z0 + (float)bin / z_scale;  // exact
+    const bool open = bin == PBINS - 1 && (z_scale == 1.f || inside_last);
+    const float z_high = z0 + (float)(bin + 1) / z_scale;
+    const auto in_bin = [&](float l, int i) {
+      const float z = z_of(l);
+      return z >= z_low && (open || z < z_high) && compose(l, i) >= cut;
+    };
+    if (upto + bin_elems <= LIST_CAP) {
+      // everything that can stay fits the list
+      gather([&](float l, int i) { return (open || z_of(l) < z_high) && compose(l, i) >= cut; });
+      if (rank == 0) {
+        const int m = (int)sh.n_items;
+        sort_items(sh, m, wt);
+        settle_list(a, sh, row, by_mass ? m : min(m, top_k), cut_p, top_p, by_mass ? want : 0, min_p, u, wt);
+      }
+      return;  // (what is read of the others was read before the last barrier)
+    }
+    // ---- refine the bin: bins of 2^shift composed numbers from ceil_c down
+    u64 floor_c = 0, ceil_c = ~0ull;
+    if (bin_elems > LIST_CAP) {
+      u64 first = ~0ull, last = 0;
+      for_each([&](float l, int i) {
+        if (!(l > -INFINITY) || !in_bin(l, i)) return;
+        const u64 c = compose(l, i);
+        first = min(first, c);
+        last = max(last, c);
+      });
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+        last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+      }
+      __syncthreads();
+      if (tid == 0) {
+        sh.range[0] = ~0ull;
+        sh.range[1] = 0;
+      }
+      __syncthreads();
+      if (lane == 0) {
+        atomicMin(&sh.range[0], first);
+        atomicMax(&sh.range[1], last);
+      }
+      cluster.sync();
+      for (int r = 0; r < C; ++r) {
+        const SampleShared* o = cluster.map_shared_rank(&sh, r);
+        first = min(first, o->range[0]);
+        last = max(last, o->range[1]);
+      }
+      floor_c = first;
+      ceil_c = last;
+      clear_bins();
+      cluster.sync();  // `range` and the bins may be used again
+      while (bin_elems > LIST_CAP) {
+        const int shift = max(0, 64 - __clzll((long long)(ceil_c - floor_c)) - 10);  // width >> shift < NBINS = 2^10
+        for_each([&](float l, int i) {
+          if (!(l > -INFINITY)) return;
+          const u64 c = compose(l, i);
+          if (c < floor_c || c > ceil_c) return;
+          const int b = (int)((ceil_c - c) >> shift);
+          atomicAdd(&sh.count[b], 1u);
+          if (by_mass) {
+            const u64 w = wt.mass(l);
+            atomicAdd(&sh.limb[0][b], (uint32_t)(w & 0x7fff));
+            atomicAdd(&sh.limb[1][b], (uint32_t)(w >> 15) & 0x7fff);
+            atomicAdd(&sh.limb[2][b], (uint32_t)(w >> 30));
+          }
+        });
+        join_bins(by_mass);
+        clear_bins();  // for the next histogram
+        find_bin(by_mass, above, want);
+        bin_elems = lead->result[0] >> 32;
+        above = lead->result[1];
+        ceil_c -= (u64)(uint32_t)lead->result[0] << shift;
+        const u64 size = 1ull << shift;
+        if (ceil_c - floor_c >= size) floor_c = ceil_c - size + 1;
+        cluster.sync();  // `result` may be written again
+      }
+      gather([&](float l, int i) {
+        const u64 c = compose(l, i);
+        return c >= floor_c && c <= ceil_c;
+      });
+    } else {
+      gather(in_bin);
+    }
+    // the bin's elements decide: sort them, the cut is the one at which `want` is reached
+    if (rank == 0) {
+      const int m = (int)sh.n_items;
+      sort_items(sh, m, wt);
+      const int i0 = 2 * tid, i1 = i0 + 1;
+      const u64 w0 = i0 < m ? (by_mass ? sh.weight[i0] : 1) : 0, w1 = i1 < m ? (by_mass ? sh.weight[i1] : 1) : 0;
+      const u64 before = above + block_before(w0 + w1, sh);
+      if (before < want && before + w0 + w1 >= want) sh.result[0] = sh.sorted[before + w0 < want ? i1 : i0];
+      __syncthreads();
+      if (tid == 0) sh.n_items = 0;
+    }
+    cluster.sync();
+    cut = lead->result[0];
+  }
+
+  // ---- many elements stay: a pass over the row, with the mass of each step of 256 elements
+  const auto kept_mass = [&](float l, int i) -> u64 {
+    if (!(l >= wt.l_min) || (cut != 0 && compose(l, i) < cut)) return 0;
+    const double w = wt(l);
+    return w >= min_p ? wt.mass(w) : 0;
   };
+  __syncthreads();
   u64 sum = 0;
-  for (int i = from; i < to; ++i) sum += kept_mass(i);
-  const u64 share = block_sum(sum, sh);
-  u64 before = block_before(sum, sh);
+  for (int step = warp; step < n_steps; step += SAMPLE_WARPS) {
+    float l[8];
+    const int i0 = load(step, l);
+    u64 m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m += kept_mass(l[e], i0 + e);
+    m = warp_sum(m);
+    if (lane == 0) sh.steps[step] = m;
+    sum += m;
+  }
+  const u64 share = block_sum(lane == 0 ? sum : 0, sh);  // its barriers publish `steps`
   if (tid == 0) sh.share_mass = share;
   cluster.sync();
-  u64 total = 0;
+  u64 total = 0, before = 0;
   for (int r = 0; r < C; ++r) {
     const u64 m = cluster.map_shared_rank(&sh, r)->share_mass;
     total += m;
     if (r < rank) before += m;
   }
   const u64 target = target_of(u, total);
-  if (before <= target && target < before + sum) {  // one thread of the cluster
-    for (int i = from; i < to; ++i) {
-      const u64 m = kept_mass(i);
-      if (target < before + m) {
-        a.token[row] = lo + i;
-        if (a.logprob) a.logprob[row] = (float)log((double)m / (double)total);
-        break;
+  if (before <= target && target < before + share) {  // one block of the cluster
+    // the step that holds the target, two steps per thread, then its elements, a lane's eight
+    const int s0 = 2 * tid, s1 = s0 + 1;
+    const u64 m0 = s0 < n_steps ? sh.steps[s0] : 0, m1 = s1 < n_steps ? sh.steps[s1] : 0;
+    u64 b = before + block_before(m0 + m1, sh);
+    if (b <= target && target < b + m0 + m1) {
+      const bool second = target >= b + m0;
+      sh.range[0] = second ? s1 : s0;
+      sh.range[1] = second ? b + m0 : b;
+    }
+    __syncthreads();
+    if (warp == 0) {
+      float l[8];
+      u64 m[8], lane_sum = 0;
+      const int i0 = load((int)sh.range[0], l);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        m[e] = kept_mass(l[e], i0 + e);
+        lane_sum += m[e];
       }
-      before += m;
+      u64 s = lane_sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 x = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += x;
+      }
+      b = sh.range[1] + s - lane_sum;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (b <= target && target < b + m[e]) {
+          a.token[row] = i0 + e;
+          if (a.logprob) a.logprob[row] = (float)log((double)m[e] / (double)total);
+        }
+        b += m[e];
+      }
     }
   }
-  cluster.sync();
+  cluster.sync();  // a block's shared memory stays until the others have read it
 }
 
 }  // namespace dsalt
@@ -481,16 +684,15 @@ extern "C" int dsalt_sample(const void* logits, int dtype, int64_t B, int64_t V,
   const int es = dtype == DSALT_F32 ? 4 : 2;
   if ((uintptr_t)logits % es) return fail(DSALT_ERR_INVALID, "sample: logits not aligned to their type");
   // blocks per row: as many as leave every row's cluster resident at once (two blocks per
-  // SM), at least so many that a share fits; a small row is one block's
+  // SM), eight where a share would be too long; a small row is one block's
   int C = 1;
-  while (C < 8 && (V / (2 * C) >= 2048 && B * (2 * C) <= 148 * 2)) C *= 2;
-  while (C < 8 && ((V + C - 1) / C > SAMPLE_MAX_SHARE || (V + C - 1) / C * es > SAMPLE_SMEM_SHARE)) C *= 2;
+  while (C < 8 && ((V / (2 * C) >= 2048 && B * (2 * C) <= 148 * 2) || V / C > MAX_SHARE / 2)) C *= 2;
   SampleArgs a;
   a.logits = logits;
   a.row_stride = row_stride;
   a.V = (int)V;
-  a.share = (int)(((V + C - 1) / C + 7) / 8 * 8);
-  a.in_smem = (int64_t)a.share * es <= SAMPLE_SMEM_SHARE + 64;
+  a.share = (int)((V + 7 + (int64_t)C * BLOCK_ELEMS - 1) / ((int64_t)C * BLOCK_ELEMS) * BLOCK_ELEMS);  // 7: the skew
+  if (a.share > MAX_SHARE) return fail(DSALT_ERR_UNSUPPORTED, "sample: share too long");
   a.u = u;
   a.temperature = temperature, a.top_k = top_k, a.top_p = top_p, a.min_p = min_p;
   a.temperature_v = temperature_value, a.top_k_v = top_k_value, a.top_p_v = top_p_value, a.min_p_v = min_p_value;
@@ -499,7 +701,7 @@ extern "C" int dsalt_sample(const void* logits, int dtype, int64_t B, int64_t V,
                        : dtype == DSALT_F16 ? reinterpret_cast<const void*>(sample_kernel<__half>)
                                             : reinterpret_cast<const void*>(sample_kernel<__nv_bfloat16>);
   static std::atomic<uint64_t> ready[3];
-  if (int rc = allow_dynamic_smem(kernel, SAMPLE_SMEM_SHARE + 256, ready[dtype])) return rc;
+  if (int rc = allow_dynamic_smem(kernel, (int)sizeof(SampleShared), ready[dtype])) return rc;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)C;
@@ -507,7 +709,7 @@ extern "C" int dsalt_sample(const void* logits, int dtype, int64_t B, int64_t V,
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(B * C));
   cfg.blockDim = dim3(SAMPLE_THREADS);
-  cfg.dynamicSmemBytes = a.in_smem ? (size_t)a.share * es + 32 : 0;
+  cfg.dynamicSmemBytes = sizeof(SampleShared);
   cfg.stream = reinterpret_cast<cudaStream_t>(stream);
   cfg.attrs = attr;
   cfg.numAttrs = 1;
