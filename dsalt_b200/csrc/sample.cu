@@ -13,12 +13,15 @@
 // No sort of the row: all three filters keep a prefix of one order, so there is one element
 // (key, index) at which the row is cut. Where at most LIST_CAP elements can matter they are
 // gathered and sorted in one block's shared memory, and the row is settled there:
-//   top-k: the k-th largest of the threads' own maxima is at most the k-th largest logit, so
-//          the elements from there on up hold the k first and few more;
+//   top-k: the k-th largest of the maxima of any threads is at most the k-th largest logit, so
+//          the elements from there on up hold the k first and few more (groups of 8 or 16 threads
+//          for a small k, every thread for a larger one);
 //   top-p: masses and counts of 16 bins of (m - l) / T, then of 16 parts of the bin where p is
-//          reached. Each thread has bins of its own (no atomics: a word per thread and bin).
-// Otherwise the bin is refined by histograms over (key, index) until the cut is one element,
-// and the row is passed over again with it.
+//          reached. Each thread has bins of its own (no atomics: a word per thread and bin), and
+//          each warp keeps a queue of its elements in that bin: only they are looked at again.
+// Otherwise the bin is refined by histograms over (key, index) until the cut is one element.
+// The mass of what stays is then known per warp, and the draw goes down from block to warp to
+// 256 elements to the token.
 //
 // Masses are whole numbers, w * 2^43 rounded from 64-bit arithmetic: their sums do not depend
 // on the order in which threads arrive, so a row gives the same token in every batch and in
@@ -45,7 +48,9 @@ constexpr int LIST_CAP = 2 * SAMPLE_THREADS;
 constexpr int IDX_BITS = 20;                  // vocabulary of at most 2^20
 constexpr int BLOCK_ELEMS = 256;              // a warp's step: eight consecutive elements per lane
 constexpr int MAX_SHARE = 131328;             // 2^20 / 8 and a skew, in whole steps: 513 of them
-constexpr int MAX_BLOCKS = MAX_SHARE / BLOCK_ELEMS;
+constexpr int MAX_STEPS = (MAX_SHARE / BLOCK_ELEMS + SAMPLE_WARPS - 1) / SAMPLE_WARPS;  // of one warp
+constexpr int QUEUE = 1024;                   // elements of the decisive bin that a warp keeps
+constexpr int MAX_GROUPS = 256;
 constexpr double MASS_ONE = 8796093022208.0;  // 2^43: 2^20 of them stay below 2^63
 constexpr float BIN_SPAN = 32.f;              // (m - l) / T that the joint histogram covers
 constexpr float MIN_LOG2 = -45.f;             // weights below 2^-45 round to no mass
@@ -76,17 +81,21 @@ struct SampleShared {
       u64 sorted[LIST_CAP], weight[LIST_CAP];  // the leader's candidates in order, and their masses
       uint32_t by_index[LIST_CAP];
     };
-    u64 steps[MAX_BLOCKS];  // mass of each step of the last pass
   };
+  uint16_t queue[SAMPLE_WARPS][QUEUE];  // places within the warp's stretch (below 2^16)
   union {
     u64 mass[NBINS];     // joined over the cluster, in the leader's copy
     u64 item[LIST_CAP];  // candidates as they arrive, in the leader's copy
   };
   uint32_t total[NBINS];  // joined counts, in the leader's copy
+  u64 warp_bin[PBINS][SAMPLE_WARPS];  // first level's masses, per warp
   u64 bin_mass[2][PBINS];
   uint32_t bin_count[2][PBINS];
+  u64 steps[MAX_STEPS];  // masses of the steps of the warp that holds the draw
+  u64 kept[SAMPLE_WARPS];
   uint32_t n_items, first_index;
-  float best;
+  float best, bound;
+  float group_max[64], all_max[MAX_GROUPS];  // of 8 or 16 threads: this block's, the cluster's
   u64 share_mass, range[2], result[4];  // result: written by the leader only
   u64 warp_red[SAMPLE_WARPS];
   double exp2_16[16];  // 2^(j / 16)
@@ -109,9 +118,8 @@ struct Weights {
   float top, l_min;
   double c;
   const double* table;
-  __device__ __forceinline__ double operator()(float l) const {  // 0 below l_min and for NaN
-    if (l == top) return 1.0;
-    if (!(l >= l_min)) return 0.0;
+  // no branch, so that several run side by side; 0 below l_min and for NaN
+  __device__ __forceinline__ double operator()(float l) const {
     constexpr double MAGIC = 422212465065984.0;  // 1.5 * 2^48: adding it leaves steps of 1/16
     constexpr double C1 = 0.6931471805599453094, C2 = C1 * C1 / 2, C3 = C2 * C1 / 3, C4 = C3 * C1 / 4, C5 = C4 * C1 / 5,
                      C6 = C5 * C1 / 6;
@@ -124,7 +132,9 @@ struct Weights {
     p = fma(p, g, C2);
     p = fma(p, g, C1);
     p = fma(p, g, 1.0) * table[k & 15];
-    return __hiloint2double(__double2hiint(p) + ((k >> 4) << 20), __double2loint(p));
+    p = __hiloint2double(__double2hiint(p) + ((k >> 4) << 20), __double2loint(p));
+    p = l >= l_min ? p : 0.0;
+    return l == top ? 1.0 : p;
   }
   __device__ __forceinline__ u64 mass(double w) const {  // w * 2^43 to the nearest whole number
     return (u64)__double_as_longlong(fma(w, MASS_ONE, 4503599627370496.0)) & 0xfffffffffffffull;  // + 2^52
@@ -238,6 +248,8 @@ __device__ __forceinline__ void settle_list(const SampleArgs& a, SampleShared& s
   }
 }
 
+static_assert(sizeof(SampleShared) <= (228 * 1024 - 2 * 1024) / 2, "two blocks per SM");
+
 template <typename T>
 __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a) {
   extern __shared__ __align__(16) unsigned char dyn[];
@@ -261,6 +273,13 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
   constexpr int VEC = 16 / (int)sizeof(T);
   const int skew = (int)(((uintptr_t)src & 15) / sizeof(T));
   const int place0 = rank * a.share, n_steps = (max(0, min(a.share, a.V + skew - place0)) + BLOCK_ELEMS - 1) / BLOCK_ELEMS;
+  const int per_warp = (n_steps + SAMPLE_WARPS - 1) / SAMPLE_WARPS;  // a warp's steps follow one another
+  const int step0 = min(warp * per_warp, n_steps), step1 = min(step0 + per_warp, n_steps);
+  const auto load_one = [&](int i) -> float {
+    if constexpr (sizeof(T) == 4) return src[i];
+    else if constexpr (std::is_same<T, __half>::value) return __half2float(src[i]);
+    else return __bfloat162float(src[i]);
+  };
   const auto load = [&](int step, float (&l)[8]) -> int {  // NaN outside the row; returns the first index
     const int i0 = place0 + step * BLOCK_ELEMS + lane * 8 - skew;
     if (i0 >= 0 && i0 + 8 <= a.V) {
@@ -285,17 +304,14 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
       for (int e = 0; e < 8; ++e) {
         l[e] = __int_as_float(0x7fffffff);
         if (i0 + e >= 0 && i0 + e < a.V) {
-          if constexpr (sizeof(T) == 4) l[e] = src[i0 + e];
-          else if constexpr (std::is_same<T, __half>::value) l[e] = __half2float(src[i0 + e]);
-          else l[e] = __bfloat162float(src[i0 + e]);
+          l[e] = load_one(i0 + e);
         }
       }
     }
     return i0;
   };
   const auto for_each = [&](auto&& f) {  // every element of the share, NaN and places outside too
-#pragma unroll 2
-    for (int step = warp; step < n_steps; step += SAMPLE_WARPS) {
+    for (int step = step0; step < step1; ++step) {
       float l[8];
       const int i0 = load(step, l);
 #pragma unroll
@@ -306,7 +322,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
   // ---- the largest logit
   float mine = -INFINITY;
 #pragma unroll 4
-  for (int step = warp; step < n_steps; step += SAMPLE_WARPS) {
+  for (int step = step0; step < step1; ++step) {
     float l[8];
     load(step, l);
 #pragma unroll
@@ -314,7 +330,12 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
   }
   float top = mine;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int o = 1; o < 32; o <<= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (o == 4 && C < 8 && (lane & 7) == 0) sh.group_max[tid >> 3] = top;
+    if (o == 8 && C == 8 && (lane & 15) == 0) sh.group_max[tid >> 4] = top;
+  }
+  const int groups = C < 8 ? 64 : 32;  // per block
   if (lane == 0) sh.warp_red[warp] = __float_as_uint(top);
   if (tid < 16) sh.exp2_16[tid] = exp2((double)tid / 16);
   if (tid == 0) {
@@ -331,6 +352,23 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
   if (tid == 0) sh.best = top;
   cluster.sync();
   for (int r = 0; r < C; ++r) top = fmaxf(top, cluster.map_shared_rank(&sh, r)->best);
+  // a small top-k's bound: the k-th largest of the groups' maxima. (Near the smallest of them
+  // the bound would fall off, so the last few are left to the larger k's way.)
+  const bool small_k = cut_k && temp > 0.f && top_k <= C * groups - C * groups / 8;
+  float bound = -INFINITY;
+  if (small_k) {
+    if (tid < C * groups) sh.all_max[tid] = cluster.map_shared_rank(&sh, tid / groups)->group_max[tid % groups];
+    __syncthreads();
+    if (tid < C * groups) {
+      const float v = sh.all_max[tid];
+      int before = 0;
+#pragma unroll 8
+      for (int i = 0; i < C * groups; ++i) before += sh.all_max[i] > v || (sh.all_max[i] == v && i < tid);
+      if (before == top_k - 1) sh.bound = v;
+    }
+    __syncthreads();
+    bound = sh.bound;
+  }
   // every decision from here to the end is the same in all threads of the cluster
   if (!(temp > 0.f) || top == -INFINITY) {
     if (top > -INFINITY) {
@@ -368,7 +406,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
     cluster.sync();
   };
 
-  // ---- a small top-k: elements down to the k-th largest of the threads' maxima
+  // ---- top-k by a bound from the threads' maxima
   const auto joint_bin = [&](float l) { return (int)fminf(z_of(l) * (NBINS / BIN_SPAN), (float)(NBINS - 1)); };
   const auto join_bins = [&](bool by_mass) {  // each block joins its part of the bins into the leader
     cluster.sync();
@@ -403,8 +441,20 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
     }
     cluster.sync();
   };
-  bool k_done = !cut_k;
-  if (cut_k && top_k <= LIST_CAP / 2 && top_k <= C * SAMPLE_THREADS / 4) {
+  if (small_k) {
+    gather([&](float l, int) { return l >= bound; });
+    const uint32_t m = lead->n_items;
+    if (m <= LIST_CAP) {
+      if (rank == 0) {
+        sort_items(sh, (int)m, wt);
+        settle_list(a, sh, row, min((int)m, top_k), cut_p, top_p, 0, min_p, u, wt);
+      }
+      cluster.sync();  // the leader's count may still be read
+      return;
+    }
+    cluster.sync();
+    if (rank == 0 && tid == 0) sh.n_items = 0;
+  } else if (cut_k && top_k <= LIST_CAP / 2 && top_k <= C * SAMPLE_THREADS / 4) {
     if (mine > -INFINITY) atomicAdd(&sh.count[joint_bin(mine)], 1u);
     if (rank == 0 && tid == 0) sh.result[0] = NBINS - 1;  // fewer maxima than k: every element
     join_bins(false);
@@ -425,45 +475,36 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
   }
 
   // ---- the cut of a wide top-k (by count), then of top-p (by mass)
-  for (int pass = k_done ? 1 : 0; pass < (cut_p ? 2 : 1); ++pass) {
+  bool kept_known = false;  // sh.kept holds the mass that stays, per warp
+  for (int pass = cut_k ? 0 : 1; pass < (cut_p ? 2 : 1); ++pass) {
     const bool by_mass = pass == 1;
     u64 want = by_mass ? 0 : (u64)top_k;  // the mass to reach is known once all masses are summed
     u64 above = 0, upto = 0, bin_elems = 0;
-    float z0 = 0.f, z_scale = 1.f;  // bins of 1, then of 1/16 from z0
-    bool inside_last = false, enough = true;
-    const auto private_bin = [&](float l) -> int {  // -1: not in the range
-      const float z = z_of(l) - z0;
-      if (z < 0.f || (z_scale > 1.f && !inside_last && z >= 1.f)) return -1;
-      return (int)fminf(z * z_scale, (float)(PBINS - 1));
-    };
-    int bin = 0;
-    for (int level = 0; level < 2; ++level) {
+    // bins of a level: every block adds up its own, the cluster's sums are found by each warp for
+    // itself. Returns whether `want` is reached, and where.
+    const auto find_private = [&](int level, int& bin) -> bool {
       __syncthreads();
-#pragma unroll
-      for (int b = 0; b < PBINS; ++b) sh.priv[b][tid] = 0;
-      for_each([&](float l, int i) {
-        if (!(l > -INFINITY) || (cut != 0 && compose(l, i) < cut)) return;
-        const int b = private_bin(l);
-        if (b >= 0) sh.priv[b][tid] += (1ull << 52) + (by_mass ? wt.mass(l) : 0);
-      });
-      __syncthreads();
-      {  // a warp per bin
+      {
+        // a thread for 16 of the 32 words of (bin, warp), from different banks; the pair joins
+        const int b = tid >> 5, w = (tid & 31) >> 1, h = tid & 1;
         u64 ms = 0;
         uint32_t cnt = 0;
-        for (int i = lane; i < SAMPLE_THREADS; i += 32) {
-          const u64 v = sh.priv[warp][i];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const u64 v = sh.priv[b][w * 32 + h * 16 + ((i + w) & 15)];
           ms += v & 0xfffffffffffffull;
           cnt += (uint32_t)(v >> 52);
         }
-        ms = warp_sum(ms);
+        ms += __shfl_xor_sync(0xffffffffu, ms, 1);
+        if (level == 0 && h == 0) sh.warp_bin[b][w] = ms;
+        ms = warp_sum(ms) >> 1;  // every pair counts twice
         cnt = __reduce_add_sync(0xffffffffu, cnt);
         if (lane == 0) {
-          sh.bin_mass[level][warp] = ms;
-          sh.bin_count[level][warp] = cnt;
+          sh.bin_mass[level][b] = ms;
+          sh.bin_count[level][b] = cnt;
         }
       }
       cluster.sync();
-      // every block finds the bin for itself
       u64 ms = 0, cnt = 0;
       if (lane < PBINS)
         for (int r = 0; r < C; ++r) {
@@ -480,49 +521,114 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
         if (lane >= o) sv += x, sc += y;
       }
       const uint32_t reached = __ballot_sync(0xffffffffu, lane < PBINS && above + sv >= want);
-      if (reached == 0) {  // fewer finite logits than k: nothing to cut
-        enough = false;
-        break;
-      }
+      if (reached == 0) return false;
       bin = __ffs(reached) - 1;
-      const u64 before_v = __shfl_sync(0xffffffffu, sv - v, bin), before_c = __shfl_sync(0xffffffffu, sc - cnt, bin);
+      above += __shfl_sync(0xffffffffu, sv - v, bin);
+      upto += __shfl_sync(0xffffffffu, sc - cnt, bin);  // elements before the bin
       bin_elems = __shfl_sync(0xffffffffu, cnt, bin);
-      above += before_v;
-      upto = (level == 0 ? 0 : upto) + before_c;  // elements before the bin
-      if (level == 0) {
-        if (bin_elems + upto <= LIST_CAP) break;
-        z0 = (float)bin;
-        z_scale = (float)PBINS;
-        inside_last = bin == PBINS - 1;
+      return true;
+    };
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < PBINS; ++b) sh.priv[b][tid] = 0;
+    __syncwarp();
+    for (int step = step0; step < step1; ++step) {
+      float l[8];
+      const int i0 = load(step, l);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        u64 m = 1ull << 52;
+        if (by_mass) m += wt.mass(l[e]);
+        if (l[e] > -INFINITY && (cut == 0 || compose(l[e], i0 + e) >= cut))
+          sh.priv[(int)fminf(z_of(l[e]), (float)(PBINS - 1))][tid] += m;
       }
     }
-    if (!enough) {
-      cluster.sync();  // the others' sums may still be read
+    int bin0 = 0, bin = 0;
+    if (!find_private(0, bin0)) {  // fewer finite logits than k: nothing to cut
+      cluster.sync();              // the others' sums may still be read
       continue;
     }
-    const float z_low = z0 + (float)bin / z_scale;  // exact
-    const bool open = bin == PBINS - 1 && (z_scale == 1.f || inside_last);
-    const float z_high = z0 + (float)(bin + 1) / z_scale;
-    const auto in_bin = [&](float l, int i) {
-      const float z = z_of(l);
-      return z >= z_low && (open || z < z_high) && compose(l, i) >= cut;
-    };
-    if (upto + bin_elems <= LIST_CAP) {
-      // everything that can stay fits the list
-      gather([&](float l, int i) { return (open || z_of(l) < z_high) && compose(l, i) >= cut; });
+    const float z0 = (float)bin0;
+    const bool last0 = bin0 == PBINS - 1;
+    const auto settle = [&](auto&& in) {  // everything that can stay fits the list
+      gather(in);
       if (rank == 0) {
         const int m = (int)sh.n_items;
         sort_items(sh, m, wt);
         settle_list(a, sh, row, by_mass ? m : min(m, top_k), cut_p, top_p, by_mass ? want : 0, min_p, u, wt);
       }
-      return;  // (what is read of the others was read before the last barrier)
+      // the others may leave: what is read of them was read before the last barrier
+    };
+    if (upto + bin_elems <= LIST_CAP) {
+      settle([&](float l, int i) { return (last0 || z_of(l) < z0 + 1.f) && (cut == 0 || compose(l, i) >= cut); });
+      return;
     }
-    // ---- refine the bin: bins of 2^shift composed numbers from ceil_c down
+    // ---- the bin's elements into the warps' queues; from here on only they are looked at
+    const int stretch = place0 + step0 * BLOCK_ELEMS - skew;  // index of the warp's first place
+    int queued = 0;
+    for (int step = step0; step < step1; ++step) {
+      float l[8];
+      const int i0 = load(step, l);
+      uint32_t in = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float z = z_of(l[e]);
+        if (z >= z0 && (last0 || z < z0 + 1.f) && l[e] > -INFINITY && (cut == 0 || compose(l[e], i0 + e) >= cut))
+          in |= 1u << e;
+      }
+      const int cnt = __popc(in);
+      int at = cnt;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, at, o);
+        if (lane >= o) at += x;
+      }
+      const int all = __shfl_sync(0xffffffffu, at, 31);
+      at += queued - cnt;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (in >> e & 1) {
+          if (at < QUEUE) sh.queue[warp][at] = (uint16_t)(i0 + e - stretch);
+          ++at;
+        }
+      queued += all;
+    }
+    __syncwarp();
+    const auto for_bin = [&](auto&& f) {  // every element of the bin that this warp owns
+      if (queued <= QUEUE) {
+        for (int q = lane; q < queued; q += 32) {
+          const int i = stretch + (int)sh.queue[warp][q];
+          f(load_one(i), i);
+        }
+      } else {
+        for_each([&](float l, int i) {
+          const float z = z_of(l);
+          if (z >= z0 && (last0 || z < z0 + 1.f) && l > -INFINITY && (cut == 0 || compose(l, i) >= cut)) f(l, i);
+        });
+      }
+    };
+    __syncthreads();  // the first level's bins have been read
+#pragma unroll
+    for (int b = 0; b < PBINS; ++b) sh.priv[b][tid] = 0;
+    // parts of 1/16: z - z0 is exact, as z lies within a factor of two of z0 (or z0 is 0)
+    const auto part_bin = [&](float l) { return (int)fminf((z_of(l) - z0) * PBINS, (float)(PBINS - 1)); };
+    for_bin([&](float l, int) { sh.priv[part_bin(l)][tid] += (1ull << 52) + (by_mass ? wt.mass(l) : 0); });
+    find_private(1, bin);
+    if (upto + bin_elems <= LIST_CAP) {
+      const int to = bin;
+      settle([&](float l, int i) {
+        const float z = z_of(l);
+        if (z < z0) return cut == 0 || compose(l, i) >= cut;
+        return (last0 || z < z0 + 1.f) && part_bin(l) <= to && (cut == 0 || compose(l, i) >= cut);
+      });
+      return;
+    }
+    // ---- refine the part: bins of 2^shift composed numbers from ceil_c down
     u64 floor_c = 0, ceil_c = ~0ull;
     if (bin_elems > LIST_CAP) {
       u64 first = ~0ull, last = 0;
-      for_each([&](float l, int i) {
-        if (!(l > -INFINITY) || !in_bin(l, i)) return;
+      for_bin([&](float l, int i) {
+        if (part_bin(l) != bin) return;
         const u64 c = compose(l, i);
         first = min(first, c);
         last = max(last, c);
@@ -554,8 +660,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
       cluster.sync();  // `range` and the bins may be used again
       while (bin_elems > LIST_CAP) {
         const int shift = max(0, 64 - __clzll((long long)(ceil_c - floor_c)) - 10);  // width >> shift < NBINS = 2^10
-        for_each([&](float l, int i) {
-          if (!(l > -INFINITY)) return;
+        for_bin([&](float l, int i) {
           const u64 c = compose(l, i);
           if (c < floor_c || c > ceil_c) return;
           const int b = (int)((ceil_c - c) >> shift);
@@ -577,47 +682,58 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
         if (ceil_c - floor_c >= size) floor_c = ceil_c - size + 1;
         cluster.sync();  // `result` may be written again
       }
-      gather([&](float l, int i) {
-        const u64 c = compose(l, i);
-        return c >= floor_c && c <= ceil_c;
-      });
-    } else {
-      gather(in_bin);
     }
-    // the bin's elements decide: sort them, the cut is the one at which `want` is reached
+    const bool by_part = ceil_c == ~0ull;
+    for_bin([&](float l, int i) {
+      const u64 c = compose(l, i);
+      if (by_part ? part_bin(l) == bin : c >= floor_c && c <= ceil_c) lead->item[atomicAdd(&lead->n_items, 1u)] = c;
+    });
+    cluster.sync();
+    // these elements decide: sort them, the cut is the one at which `want` is reached
     if (rank == 0) {
       const int m = (int)sh.n_items;
       sort_items(sh, m, wt);
       const int i0 = 2 * tid, i1 = i0 + 1;
       const u64 w0 = i0 < m ? (by_mass ? sh.weight[i0] : 1) : 0, w1 = i1 < m ? (by_mass ? sh.weight[i1] : 1) : 0;
       const u64 before = above + block_before(w0 + w1, sh);
-      if (before < want && before + w0 + w1 >= want) sh.result[0] = sh.sorted[before + w0 < want ? i1 : i0];
+      if (before < want && before + w0 + w1 >= want) {
+        const bool second = before + w0 < want;
+        sh.result[0] = sh.sorted[second ? i1 : i0];
+      }
       __syncthreads();
       if (tid == 0) sh.n_items = 0;
     }
     cluster.sync();
     cut = lead->result[0];
+    if (by_mass && !(min_p > 0)) {
+      // the mass that stays: all of the bins before, of the bin what the queue holds from the cut on
+      u64 m = 0;
+      for_bin([&](float l, int i) {
+        if (compose(l, i) >= cut) m += wt.mass(l);
+      });
+      m = warp_sum(m);
+      for (int b = 0; b < bin0; ++b) m += sh.warp_bin[b][warp];
+      if (lane == 0) sh.kept[warp] = m;
+      kept_known = true;
+    }
+    if (!by_mass) cluster.sync();  // `result` may be written again
   }
 
-  // ---- many elements stay: a pass over the row, with the mass of each step of 256 elements
+  // ---- the draw: block, warp, step of 256 elements, element
   const auto kept_mass = [&](float l, int i) -> u64 {
-    if (!(l >= wt.l_min) || (cut != 0 && compose(l, i) < cut)) return 0;
     const double w = wt(l);
-    return w >= min_p ? wt.mass(w) : 0;
+    return w >= min_p && (cut == 0 || compose(l, i) >= cut) && l >= wt.l_min ? wt.mass(w) : 0;
   };
-  __syncthreads();
-  u64 sum = 0;
-  for (int step = warp; step < n_steps; step += SAMPLE_WARPS) {
-    float l[8];
-    const int i0 = load(step, l);
+  if (!kept_known) {
     u64 m = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m += kept_mass(l[e], i0 + e);
+    for_each([&](float l, int i) { m += kept_mass(l, i); });
     m = warp_sum(m);
-    if (lane == 0) sh.steps[step] = m;
-    sum += m;
+    if (lane == 0) sh.kept[warp] = m;
   }
-  const u64 share = block_sum(lane == 0 ? sum : 0, sh);  // its barriers publish `steps`
+  __syncthreads();
+  u64 share = 0;
+#pragma unroll
+  for (int w = 0; w < SAMPLE_WARPS; ++w) share += sh.kept[w];
   if (tid == 0) sh.share_mass = share;
   cluster.sync();
   u64 total = 0, before = 0;
@@ -628,20 +744,26 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
   }
   const u64 target = target_of(u, total);
   if (before <= target && target < before + share) {  // one block of the cluster
-    // the step that holds the target, two steps per thread, then its elements, a lane's eight
-    const int s0 = 2 * tid, s1 = s0 + 1;
-    const u64 m0 = s0 < n_steps ? sh.steps[s0] : 0, m1 = s1 < n_steps ? sh.steps[s1] : 0;
-    u64 b = before + block_before(m0 + m1, sh);
-    if (b <= target && target < b + m0 + m1) {
-      const bool second = target >= b + m0;
-      sh.range[0] = second ? s1 : s0;
-      sh.range[1] = second ? b + m0 : b;
+    int owner = 0;
+    u64 b = before;
+    while (owner < SAMPLE_WARPS - 1 && target >= b + sh.kept[owner]) b += sh.kept[owner++];
+    const int first = min(owner * per_warp, n_steps), steps = min(first + per_warp, n_steps) - first;
+    for (int step = warp; step < steps; step += SAMPLE_WARPS) {
+      float l[8];
+      u64 m = 0;
+      const int i0 = load(first + step, l);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m += kept_mass(l[e], i0 + e);
+      m = warp_sum(m);
+      if (lane == 0) sh.steps[step] = m;
     }
     __syncthreads();
     if (warp == 0) {
+      int step = 0;
+      while (step < steps - 1 && target >= b + sh.steps[step]) b += sh.steps[step++];
       float l[8];
       u64 m[8], lane_sum = 0;
-      const int i0 = load((int)sh.range[0], l);
+      const int i0 = load(first + step, l);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         m[e] = kept_mass(l[e], i0 + e);
@@ -653,7 +775,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
         const u64 x = __shfl_up_sync(0xffffffffu, s, o);
         if (lane >= o) s += x;
       }
-      b = sh.range[1] + s - lane_sum;
+      b += s - lane_sum;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if (b <= target && target < b + m[e]) {
@@ -684,9 +806,10 @@ extern "C" int dsalt_sample(const void* logits, int dtype, int64_t B, int64_t V,
   const int es = dtype == DSALT_F32 ? 4 : 2;
   if ((uintptr_t)logits % es) return fail(DSALT_ERR_INVALID, "sample: logits not aligned to their type");
   // blocks per row: as many as leave every row's cluster resident at once (two blocks per
-  // SM), eight where a share would be too long; a small row is one block's
+  // SM), more where the decisive bin of a share would overrun the warps' queues; a small row is
+  // one block's
   int C = 1;
-  while (C < 8 && ((V / (2 * C) >= 2048 && B * (2 * C) <= 148 * 2) || V / C > MAX_SHARE / 2)) C *= 2;
+  while (C < 8 && ((V / (2 * C) >= 2048 && B * (2 * C) <= 148 * 2) || V / C > 80000)) C *= 2;
   SampleArgs a;
   a.logits = logits;
   a.row_stride = row_stride;
