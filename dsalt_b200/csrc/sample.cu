@@ -16,12 +16,12 @@
 //   top-k: the k-th largest of the maxima of any threads is at most the k-th largest logit, so
 //          the elements from there on up hold the k first and few more (groups of 8 or 16 threads
 //          for a small k, every thread for a larger one);
-//   top-p: masses and counts of 16 bins of (m - l) / T, then of 16 parts of the bin where p is
-//          reached. Each thread has bins of its own (no atomics: a word per thread and bin), and
-//          each warp keeps a queue of its elements in that bin: only they are looked at again.
-// Otherwise the bin is refined by histograms over (key, index) until the cut is one element.
-// The mass of what stays is then known per warp, and the draw goes down from block to warp to
-// 256 elements to the token.
+//   top-p: masses and counts of 16 bins of (m - l) / T. Each thread has bins of its own (no
+//          atomics: a word per thread and bin).
+// Otherwise each warp puts its elements of the bin where p is reached into a queue: only they
+// are looked at again, by a histogram of 1024 parts of the bin and, where a part still holds
+// more than the list, by histograms over (key, index). The mass of what stays is then known
+// per warp, and the draw goes down from block to warp to 256 elements to the token.
 //
 // Masses are whole numbers, w * 2^43 rounded from 64-bit arithmetic: their sums do not depend
 // on the order in which threads arrive, so a row gives the same token in every batch and in
@@ -89,8 +89,8 @@ struct SampleShared {
   };
   uint32_t total[NBINS];  // joined counts, in the leader's copy
   u64 warp_bin[PBINS][SAMPLE_WARPS];  // first level's masses, per warp
-  u64 bin_mass[2][PBINS];
-  uint32_t bin_count[2][PBINS];
+  u64 bin_mass[PBINS];
+  uint32_t bin_count[PBINS];
   u64 steps[MAX_STEPS];  // masses of the steps of the warp that holds the draw
   u64 kept[SAMPLE_WARPS];
   uint32_t n_items, first_index;
@@ -98,8 +98,14 @@ struct SampleShared {
   float group_max[64], all_max[MAX_GROUPS];  // of 8 or 16 threads: this block's, the cluster's
   u64 share_mass, range[2], result[4];  // result: written by the leader only
   u64 warp_red[SAMPLE_WARPS];
-  double exp2_16[16];  // 2^(j / 16)
+  double exp2_32[32];  // 2^(j / 32)
 };
+
+// the block's own, by its shared-memory address (a pointer handed to a function would be generic)
+__device__ __forceinline__ SampleShared& block_shared() {
+  extern __shared__ __align__(16) unsigned char sample_smem[];
+  return *reinterpret_cast<SampleShared*>(sample_smem);
+}
 
 // (key, index) as one number: larger comes first in the order of the filters
 __device__ __forceinline__ u64 compose(float l, int idx) {
@@ -111,32 +117,34 @@ __device__ __forceinline__ float logit_of(u64 c) {
   return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
 }
 
-// Weights of one row. 2^t, t = (l - m) log2(e) / T: t = k / 16 + g with |g| <= 1/32, then
-// 2^(k/16) from a table of 16 and the exponent, 2^g by its Taylor series to the sixth power
-// (the seventh term is below (ln 2 / 32)^7 / 7! = 4.4e-16).
+// Weights of one row. 2^t, t = (l - m) log2(e) / T: t = k / 32 + g with |g| <= 1/64, then
+// 2^(k/32) from a table of 32 and the exponent, 2^g by its Taylor series to the fifth power
+// (the sixth term is below (ln 2 / 64)^6 / 6! = 2.3e-15). The passes are bound by instructions, and
+// one in 64 bits takes two turns: eleven of them here, no branch and no selection.
 struct Weights {
-  float top, l_min;
+  float top;    // the largest logit
+  float floor;  // logits below it (and NaN) are taken as it
   double c;
-  const double* table;
-  // no branch, so that several run side by side; 0 below l_min and for NaN
-  __device__ __forceinline__ double operator()(float l) const {
-    constexpr double MAGIC = 422212465065984.0;  // 1.5 * 2^48: adding it leaves steps of 1/16
-    constexpr double C1 = 0.6931471805599453094, C2 = C1 * C1 / 2, C3 = C2 * C1 / 3, C4 = C3 * C1 / 4, C5 = C4 * C1 / 5,
-                     C6 = C5 * C1 / 6;
-    const double t = ((double)l - (double)top) * c, r = t + MAGIC;
+  bool only_top;   // +inf: equal ones have weight 1, all others none
+  bool vanishing;  // the floor's weight rounds to no mass (else -inf and NaN have to be left out)
+  __device__ __forceinline__ double finite(float l) const {  // where !only_top
+    constexpr double MAGIC = 211106232532992.0;  // 1.5 * 2^47: adding it leaves steps of 1/32
+    constexpr double C1 = 0.6931471805599453094, C2 = C1 * C1 / 2, C3 = C2 * C1 / 3, C4 = C3 * C1 / 4, C5 = C4 * C1 / 5;
+    const double d = (double)fmaxf(l, floor) - (double)top, r = fma(d, c, MAGIC);
     const int k = __double2loint(r);
-    const double g = t - (r - MAGIC);
-    double p = fma(g, C6, C5);
-    p = fma(p, g, C4);
+    const double g = fma(d, c, MAGIC - r);
+    double p = fma(g, C5, C4);
     p = fma(p, g, C3);
     p = fma(p, g, C2);
     p = fma(p, g, C1);
-    p = fma(p, g, 1.0) * table[k & 15];
-    p = __hiloint2double(__double2hiint(p) + ((k >> 4) << 20), __double2loint(p));
-    p = l >= l_min ? p : 0.0;
-    return l == top ? 1.0 : p;
+    p = fma(p, g, 1.0) * block_shared().exp2_32[k & 31];
+    return __hiloint2double(__double2hiint(p) + ((k >> 5) << 20), __double2loint(p));
   }
-  __device__ __forceinline__ u64 mass(double w) const {  // w * 2^43 to the nearest whole number
+  __device__ __forceinline__ double operator()(float l) const {
+    return only_top ? (l == top ? 1.0 : 0.0) : finite(l);
+  }
+  // w * 2^43 to the nearest whole number
+  static __device__ __forceinline__ u64 mass(double w) {
     return (u64)__double_as_longlong(fma(w, MASS_ONE, 4503599627370496.0)) & 0xfffffffffffffull;  // + 2^52
   }
   __device__ __forceinline__ u64 mass(float l) const { return mass((*this)(l)); }
@@ -189,21 +197,44 @@ __device__ __forceinline__ u64 target_of(float u, u64 total) {
   return x >= (double)total ? total - 1 : min((u64)x, total - 1);
 }
 
-// bitonic sort of size (a power of two) values in shared memory by the block
+// Bitonic sort of `size` (a power of two, at most two per thread) values in shared memory by
+// the block. A thread holds two neighbours: distances up to 32 are a warp's own business
+// (shuffles), only longer ones go through shared memory, twice at a time.
 template <typename T, bool DESCENDING>
 __device__ __forceinline__ void block_sort(T* v, int size) {
-  for (int k = 2; k <= size; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
+  static_assert(LIST_CAP == 2 * SAMPLE_THREADS, "two values per thread");
+  __syncthreads();
+  const int i0 = 2 * threadIdx.x;
+  const bool live = i0 < size;
+  T a = live ? v[i0] : T(0), b = live ? v[i0 + 1] : T(0);
+  const auto better = [](T x, T y, bool first) {  // the value that the lower (first) or upper place keeps
+    return (x > y) == (first == DESCENDING) ? x : y;
+  };
+  for (int k = 2; k <= size; k <<= 1) {
+    const bool up = (i0 & k) == 0;  // a block of k in the wanted order, else reversed
+    for (int j = k >> 1; j > 32; j >>= 1) {
       __syncthreads();
-      for (int i = threadIdx.x; i < size / 2; i += SAMPLE_THREADS) {
-        const int x = 2 * i - (i & (j - 1)), y = x + j;
-        const T a = v[x], b = v[y];
-        if (((x & k) == 0) == (DESCENDING ? a < b : a > b)) {
-          v[x] = b;
-          v[y] = a;
-        }
+      if (live) v[i0] = a, v[i0 + 1] = b;
+      __syncthreads();
+      if (live) {
+        const bool first = ((i0 & j) == 0) == up;
+        a = better(a, v[i0 ^ j], first);
+        b = better(b, v[(i0 ^ j) + 1], first);
       }
     }
+    if (i0 - 2 * (int)(threadIdx.x & 31) < size) {  // the warp holds values
+      for (int j = min(k >> 1, 32); j > 1; j >>= 1) {
+        const bool first = ((i0 & j) == 0) == up;
+        a = better(a, __shfl_xor_sync(0xffffffffu, a, j >> 1), first);
+        b = better(b, __shfl_xor_sync(0xffffffffu, b, j >> 1), first);
+      }
+      const T x = better(a, b, up), y = better(a, b, !up);
+      a = x;
+      b = y;
+    }
+  }
+  __syncthreads();
+  if (live) v[i0] = a, v[i0 + 1] = b;
   __syncthreads();
 }
 __device__ __forceinline__ int power_of_two(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
@@ -248,18 +279,276 @@ __device__ __forceinline__ void settle_list(const SampleArgs& a, SampleShared& s
   }
 }
 
+// One block's share of a row, in steps of a warp: eight consecutive elements per lane. Places are
+// counted from the 16-byte boundary at or before the row's start, so that whole vectors can be
+// read. A warp's steps follow one another.
+template <typename T>
+struct Share {
+  static constexpr int VEC = 16 / (int)sizeof(T), WORDS = 32 / VEC, PER = 4 / (int)sizeof(T);
+  static constexpr int AHEAD = 1;  // steps that loads run ahead (more of them cost registers that the weights need)
+  const T* src;
+  int V, start;  // index of the share's first place (negative where the row begins behind it)
+  int n_steps, per_warp;
+
+  __device__ __forceinline__ int first() const { return min((int)(threadIdx.x >> 5) * per_warp, n_steps); }
+  __device__ __forceinline__ int last() const { return min(first() + per_warp, n_steps); }
+  __device__ __forceinline__ int index(int step) const { return start + step * BLOCK_ELEMS + (threadIdx.x & 31) * 8; }
+  __device__ __forceinline__ float one(int i) const {
+    if constexpr (sizeof(T) == 4) return src[i];
+    else if constexpr (std::is_same<T, __half>::value) return __half2float(src[i]);
+    else return __bfloat162float(src[i]);
+  }
+  struct Raw {  // eight elements as they lie in memory
+    uint32_t w[WORDS];
+  };
+  __device__ __forceinline__ Raw load(int step) const {  // NaN outside the row
+    const int i0 = index(step);
+    Raw r;
+    if (i0 >= 0 && i0 + 8 <= V) {
+#pragma unroll
+      for (int h = 0; h < WORDS / 4; ++h) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + i0) + h);
+        r.w[4 * h] = v.x, r.w[4 * h + 1] = v.y, r.w[4 * h + 2] = v.z, r.w[4 * h + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < WORDS; ++e) {
+        r.w[e] = 0xffffffffu;
+#pragma unroll
+        for (int x = 0; x < PER; ++x) {
+          const int i = i0 + e * PER + x;
+          if (i < 0 || i >= V) continue;
+          if constexpr (sizeof(T) == 4) r.w[e] = __float_as_uint(src[i]);
+          else r.w[e] = (r.w[e] & ~(0xffffu << 16 * x)) | (uint32_t)reinterpret_cast<const uint16_t*>(src)[i] << 16 * x;
+        }
+      }
+    }
+    return r;
+  }
+  static __device__ __forceinline__ float2 pair(const Raw& r, int x) {  // elements 2 x, 2 x + 1
+    if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(r.w[2 * x]), __uint_as_float(r.w[2 * x + 1]));
+    else if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&r.w[x]));
+    else return make_float2(__uint_as_float(r.w[x] << 16), __uint_as_float(r.w[x] & 0xffff0000u));
+  }
+  // f(raw, first index) for the warp's steps
+  template <typename F>
+  __device__ __forceinline__ void steps(F&& f) const {
+    const int s0 = first(), s1 = last();
+    Raw next[AHEAD];
+#pragma unroll
+    for (int x = 0; x < AHEAD; ++x)
+      if (s0 + x < s1) next[x] = load(s0 + x);
+#pragma unroll 1
+    for (int step = s0; step < s1; ++step) {
+      const Raw now = next[0];
+#pragma unroll
+      for (int x = 0; x + 1 < AHEAD; ++x) next[x] = next[x + 1];
+      if (step + AHEAD < s1) next[AHEAD - 1] = load(step + AHEAD);
+      f(now, index(step));
+    }
+  }
+  // f(logit, index) for the warp's elements, NaN outside the row
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+    steps([&](const Raw& r, int i0) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float2 l = pair(r, x);
+        f(l.x, i0 + 2 * x);
+        f(l.y, i0 + 2 * x + 1);
+      }
+    });
+  }
+};
+
+// The passes over a share.
+struct Bin {  // logits [low, high) (from low up where `top`), of elements at or above `cut`
+  float low, high;
+  bool top;
+  u64 cut;
+  __device__ __forceinline__ bool has(float l, int i) const {
+    return l >= low && (top || l < high) && (cut == 0 || compose(l, i) >= cut);
+  }
+};
+__device__ __forceinline__ float place_of(float l, float top, float inv_t) {  // grows as l falls, at least 0
+  const float z = (top - l) * inv_t;
+  return z == z ? z : 0.f;  // of +inf against +inf
+}
+
+template <typename T>
+__device__ __forceinline__ float max_pass(Share<T> s) {
+  float m = -INFINITY;
+  s.each([&](float l, int) { m = fmaxf(m, l); });  // passes over NaN
+  return m;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t first_pass(Share<T> s, float top) {  // lowest index of the largest logit
+  uint32_t first = 0xffffffffu;
+  s.each([&](float l, int i) {
+    if (l == top) first = min(first, (uint32_t)i);
+  });
+  return first;
+}
+template <typename T>
+__device__ __forceinline__ void bins_pass(Share<T> s, Weights wt, float inv_t, u64 cut, bool by_mass) {
+  auto& priv = block_shared().priv;
+#pragma unroll
+  for (int b = 0; b < PBINS; ++b) priv[b][threadIdx.x] = 0;
+  const auto put = [&](float l, int i, float z, u64 m) {
+    if (l > -INFINITY && (cut == 0 || compose(l, i) >= cut)) priv[(int)fminf(z, (float)(PBINS - 1))][threadIdx.x] += m;
+  };
+  constexpr u64 ONE = 1ull << 52;
+  if (wt.only_top || !by_mass)
+    s.each([&](float l, int i) { put(l, i, place_of(l, wt.top, inv_t), ONE + (by_mass && l == wt.top ? (u64)MASS_ONE : 0)); });
+  else
+    s.each([&](float l, int i) { put(l, i, (wt.top - l) * inv_t, ONE + Weights::mass(wt.finite(l))); });
+}
+template <typename T>
+__device__ __forceinline__ int queue_pass(Share<T> s, Bin bin) {  // returns how many there are
+  uint16_t* const queue = block_shared().queue[threadIdx.x >> 5];
+  const int lane = threadIdx.x & 31, from = s.start + s.first() * BLOCK_ELEMS;
+  int queued = 0;
+  s.steps([&](const typename Share<T>::Raw& r, int i0) {
+    uint32_t in = 0;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float2 l = Share<T>::pair(r, x);
+      in |= (bin.has(l.x, i0 + 2 * x) ? 1u : 0u) << (2 * x) | (bin.has(l.y, i0 + 2 * x + 1) ? 2u : 0u) << (2 * x);
+    }
+    const int cnt = __popc(in);
+    int at = cnt;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += x;
+    }
+    const int all = __shfl_sync(0xffffffffu, at, 31);
+    at += queued - cnt;
+    for (; in; in &= in - 1, ++at)
+      if (at < QUEUE) queue[at] = (uint16_t)(i0 + __ffs(in) - 1 - from);
+    queued += all;
+  });
+  __syncwarp();
+  return queued;
+}
+// f(logit, index) for the elements of the bin that this warp owns
+template <typename T, typename F>
+__device__ __forceinline__ void for_bin(const Share<T>& s, const Bin& bin, int queued, F&& f) {
+  const uint16_t* const queue = block_shared().queue[threadIdx.x >> 5];
+  if (queued <= QUEUE) {
+    const int from = s.start + s.first() * BLOCK_ELEMS;
+    for (int q = threadIdx.x & 31; q < queued; q += 4 * 32) {  // four loads under way
+      float l[4];
+      int i[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (q + 32 * x < queued) {
+          i[x] = from + (int)queue[q + 32 * x];
+          l[x] = s.one(i[x]);
+        }
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (q + 32 * x < queued) f(l[x], i[x]);
+    }
+  } else {
+    s.each([&](float l, int i) {
+      if (bin.has(l, i)) f(l, i);
+    });
+  }
+}
+// Parts of the bin for a histogram: 1024 of (m - l) / T from z0 on (shift < 0), or 2^shift
+// composed numbers each from ceil_c down to floor_c.
+struct Parts {
+  float top, inv_t, z0, scale;
+  int shift;
+  u64 floor_c, ceil_c;
+  __device__ __forceinline__ int operator()(float l, int i) const {  // -1: outside
+    if (shift < 0) return (int)fminf((place_of(l, top, inv_t) - z0) * scale, (float)(NBINS - 1));
+    const u64 c = compose(l, i);
+    return c < floor_c || c > ceil_c ? -1 : (int)((ceil_c - c) >> shift);
+  }
+};
+template <typename T>
+__device__ __forceinline__ void histogram_pass(Share<T> s, Weights wt, Bin bin, Parts parts, bool by_mass, int queued) {
+  SampleShared& sh = block_shared();
+  for_bin(s, bin, queued, [&](float l, int i) {
+    const int b = parts(l, i);
+    if (b < 0) return;
+    atomicAdd(&sh.count[b], 1u);
+    if (by_mass) {
+      const u64 w = wt.mass(l);
+      atomicAdd(&sh.limb[0][b], (uint32_t)(w & 0x7fff));
+      atomicAdd(&sh.limb[1][b], (uint32_t)(w >> 15) & 0x7fff);
+      if (w >> 30) atomicAdd(&sh.limb[2][b], (uint32_t)(w >> 30));
+    }
+  });
+}
+template <typename T>
+__device__ __forceinline__ void range_pass(Share<T> s, Bin bin, Parts parts, int part, int queued, u64& first, u64& last) {
+  u64 lo = ~0ull, hi = 0;
+  for_bin(s, bin, queued, [&](float l, int i) {
+    if (parts(l, i) != part) return;
+    const u64 c = compose(l, i);
+    lo = min(lo, c);
+    hi = max(hi, c);
+  });
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  first = lo;
+  last = hi;
+}
+// into the leader's list: all elements from `low` up; or those of one part of the bin
+template <typename T>
+__device__ __forceinline__ void list_pass(Share<T> s, float low, u64 cut, SampleShared* lead) {
+  s.each([&](float l, int i) {
+    if (!(l >= low) || l == -INFINITY || (cut != 0 && compose(l, i) < cut)) return;
+    const uint32_t at = atomicAdd(&lead->n_items, 1u);
+    if (at < LIST_CAP) lead->item[at] = compose(l, i);
+  });
+}
+template <typename T>
+__device__ __forceinline__ void list_part_pass(Share<T> s, Bin bin, Parts parts, int part, int queued, SampleShared* lead) {
+  for_bin(s, bin, queued, [&](float l, int i) {
+    if (parts(l, i) == part) lead->item[atomicAdd(&lead->n_items, 1u)] = compose(l, i);
+  });
+}
+// the warp's mass of what stays: of its queue, of its elements, of one step
+struct Kept {
+  Weights wt;
+  u64 cut;
+  double min_p;
+  __device__ __forceinline__ u64 operator()(float l, int i) const {
+    const double w = wt(l);
+    return (min_p > 0 && !(w >= min_p)) || (cut != 0 && compose(l, i) < cut) || !(l > -INFINITY) ? 0 : wt.mass(w);
+  }
+};
+template <typename T>
+__device__ __forceinline__ u64 kept_queue_pass(Share<T> s, Kept kept, Bin bin, int queued) {
+  u64 m = 0;
+  for_bin(s, bin, queued, [&](float l, int i) { m += kept(l, i); });
+  return warp_sum(m);
+}
+template <typename T>
+__device__ __forceinline__ u64 kept_pass(Share<T> s, Kept kept) {
+  u64 m = 0;
+  if (kept.wt.only_top || !kept.wt.vanishing || kept.cut != 0 || kept.min_p > 0) s.each([&](float l, int i) { m += kept(l, i); });
+  else s.each([&](float l, int) { m += Weights::mass(kept.wt.finite(l)); });  // nothing is cut
+  return warp_sum(m);
+}
+
 static_assert(sizeof(SampleShared) <= (228 * 1024 - 2 * 1024) / 2, "two blocks per SM");
 
 template <typename T>
 __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a) {
-  extern __shared__ __align__(16) unsigned char dyn[];
-  SampleShared& sh = *reinterpret_cast<SampleShared*>(dyn);
+  SampleShared& sh = block_shared();
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int row = blockIdx.x / C;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   SampleShared* lead = cluster.map_shared_rank(&sh, 0);
-  const T* src = reinterpret_cast<const T*>(a.logits) + (int64_t)row * a.row_stride;
 
   const float temp = a.temperature ? a.temperature[row] : a.temperature_v;
   const double top_p = a.top_p ? (double)a.top_p[row] : (double)a.top_p_v;
@@ -268,66 +557,16 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
   const float u = a.u[row];
   const bool cut_k = top_k > 0 && top_k < a.V, cut_p = top_p < 1.0;
 
-  // ---- the share, in steps of a warp: eight consecutive elements per lane. Places are counted
-  // from the 16-byte boundary at or before the row's start, so that whole vectors can be read.
-  constexpr int VEC = 16 / (int)sizeof(T);
-  const int skew = (int)(((uintptr_t)src & 15) / sizeof(T));
-  const int place0 = rank * a.share, n_steps = (max(0, min(a.share, a.V + skew - place0)) + BLOCK_ELEMS - 1) / BLOCK_ELEMS;
-  const int per_warp = (n_steps + SAMPLE_WARPS - 1) / SAMPLE_WARPS;  // a warp's steps follow one another
-  const int step0 = min(warp * per_warp, n_steps), step1 = min(step0 + per_warp, n_steps);
-  const auto load_one = [&](int i) -> float {
-    if constexpr (sizeof(T) == 4) return src[i];
-    else if constexpr (std::is_same<T, __half>::value) return __half2float(src[i]);
-    else return __bfloat162float(src[i]);
-  };
-  const auto load = [&](int step, float (&l)[8]) -> int {  // NaN outside the row; returns the first index
-    const int i0 = place0 + step * BLOCK_ELEMS + lane * 8 - skew;
-    if (i0 >= 0 && i0 + 8 <= a.V) {
-#pragma unroll
-      for (int h = 0; h < 8 / VEC; ++h) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + i0) + h);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (sizeof(T) == 4) {
-            l[4 * h + e] = __uint_as_float(w[e]);
-          } else if constexpr (std::is_same<T, __half>::value) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-            l[2 * e] = f.x, l[2 * e + 1] = f.y;
-          } else {
-            l[2 * e] = __uint_as_float(w[e] << 16), l[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-          }
-        }
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        l[e] = __int_as_float(0x7fffffff);
-        if (i0 + e >= 0 && i0 + e < a.V) {
-          l[e] = load_one(i0 + e);
-        }
-      }
-    }
-    return i0;
-  };
-  const auto for_each = [&](auto&& f) {  // every element of the share, NaN and places outside too
-    for (int step = step0; step < step1; ++step) {
-      float l[8];
-      const int i0 = load(step, l);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f(l[e], i0 + e);
-    }
-  };
+  Share<T> s;
+  s.src = reinterpret_cast<const T*>(a.logits) + (int64_t)row * a.row_stride;
+  s.V = a.V;
+  const int skew = (int)(((uintptr_t)s.src & 15) / sizeof(T));
+  s.start = rank * a.share - skew;
+  s.n_steps = (max(0, min(a.share, a.V - s.start)) + BLOCK_ELEMS - 1) / BLOCK_ELEMS;
+  s.per_warp = (s.n_steps + SAMPLE_WARPS - 1) / SAMPLE_WARPS;
 
   // ---- the largest logit
-  float mine = -INFINITY;
-#pragma unroll 4
-  for (int step = step0; step < step1; ++step) {
-    float l[8];
-    load(step, l);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) mine = fmaxf(mine, l[e]);  // passes over NaN
-  }
+  const float mine = max_pass<T>(s);
   float top = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -337,7 +576,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
   }
   const int groups = C < 8 ? 64 : 32;  // per block
   if (lane == 0) sh.warp_red[warp] = __float_as_uint(top);
-  if (tid < 16) sh.exp2_16[tid] = exp2((double)tid / 16);
+  if (tid < 32) sh.exp2_32[tid] = exp2((double)tid / 32);
   if (tid == 0) {
     sh.first_index = 0xffffffffu;
     sh.n_items = 0;
@@ -351,7 +590,9 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
   for (int w = 0; w < SAMPLE_WARPS; ++w) top = fmaxf(top, __uint_as_float((uint32_t)sh.warp_red[w]));
   if (tid == 0) sh.best = top;
   cluster.sync();
-  for (int r = 0; r < C; ++r) top = fmaxf(top, cluster.map_shared_rank(&sh, r)->best);
+#pragma unroll
+  for (int r = 0; r < 8; ++r)
+    if (r < C) top = fmaxf(top, cluster.map_shared_rank(&sh, r)->best);
   // a small top-k's bound: the k-th largest of the groups' maxima. (Near the smallest of them
   // the bound would fall off, so the last few are left to the larger k's way.)
   const bool small_k = cut_k && temp > 0.f && top_k <= C * groups - C * groups / 8;
@@ -372,11 +613,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
   // every decision from here to the end is the same in all threads of the cluster
   if (!(temp > 0.f) || top == -INFINITY) {
     if (top > -INFINITY) {
-      uint32_t first = 0xffffffffu;
-      for_each([&](float l, int i) {
-        if (l == top) first = min(first, (uint32_t)i);
-      });
-      first = __reduce_min_sync(0xffffffffu, first);
+      const uint32_t first = __reduce_min_sync(0xffffffffu, first_pass<T>(s, top));
       if (lane == 0 && first != 0xffffffffu) atomicMin(&lead->first_index, first);
     }
     cluster.sync();
@@ -389,35 +626,43 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
   Weights wt;
   wt.top = top;
   wt.c = 1.4426950408889634 / (double)temp;
-  wt.l_min = top == INFINITY ? INFINITY : fmaxf((float)((double)top + (double)MIN_LOG2 / wt.c), -3.402823466e38f);
-  wt.table = sh.exp2_16;
-  const float inv_t = (float)(1.0 / (double)temp);
-  const auto z_of = [&](float l) { return l == top ? 0.f : (top - l) * inv_t; };  // grows as l falls, at least 0
+  // Where one step of fp32 below the largest logit is beyond 2^-900, a smaller slope says the same:
+  // everything below has no mass, and 2^t stays a normal number down to the floor.
+  const float below = nextafterf(top, -INFINITY);
+  wt.only_top = top == INFINITY || below == -INFINITY;
+  if (!wt.only_top) wt.c = fmin(wt.c, 900.0 / ((double)top - (double)below));
+  wt.floor = fmaxf(fminf((float)((double)top + (double)MIN_LOG2 / wt.c), below), -3.402823466e38f);
+  wt.vanishing = ((double)wt.floor - (double)top) * wt.c <= (double)MIN_LOG2 + 0.5;
+  // 1 / T as a finite number, so that a difference of 0 is place 0 at any temperature
+  const float inv_t = fminf((float)(1.0 / (double)temp), 3.402823466e38f);
 
-  u64 cut = 0;  // elements below it are dropped
-  // A list of all that can stay, from `in` on: sorted and settled by the leader.
-  const auto gather = [&](auto&& in) {
-    for_each([&](float l, int i) {
-      if (l > -INFINITY && in(l, i)) {
-        const uint32_t at = atomicAdd(&lead->n_items, 1u);
-        if (at < LIST_CAP) lead->item[at] = compose(l, i);
-      }
-    });
-    cluster.sync();
+  // the smallest logit whose place (m - l) / T lies below a bound, by a search of 32 steps at a time
+  const auto lowest = [&](float bound) -> float {
+    uint32_t lo = order_f32(-INFINITY), hi = order_f32(top);  // at or beyond the bound, below it
+    while (hi - lo > 1) {
+      const uint32_t step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step;
+      const bool in = at >= hi || place_of(logit_of((u64)at << IDX_BITS), top, inv_t) < bound;
+      const int f = __ffs(__ballot_sync(0xffffffffu, in)) - 1;  // the last lane's is at or above hi
+      hi = min(hi, lo + (f + 1) * step);
+      lo += f * step;
+    }
+    return logit_of((u64)hi << IDX_BITS);
   };
-
+  u64 cut = 0;  // elements below it are dropped
   // ---- top-k by a bound from the threads' maxima
-  const auto joint_bin = [&](float l) { return (int)fminf(z_of(l) * (NBINS / BIN_SPAN), (float)(NBINS - 1)); };
+  const auto joint_bin = [&](float l) { return (int)fminf(place_of(l, top, inv_t) * (NBINS / BIN_SPAN), (float)(NBINS - 1)); };
   const auto join_bins = [&](bool by_mass) {  // each block joins its part of the bins into the leader
     cluster.sync();
     for (int b = rank * SAMPLE_THREADS + tid; b < NBINS; b += C * SAMPLE_THREADS) {
       uint32_t cnt = 0;
       u64 ms = 0;
-      for (int r = 0; r < C; ++r) {
-        const SampleShared* o = cluster.map_shared_rank(&sh, r);
-        cnt += o->count[b];
-        if (by_mass) ms += (u64)o->limb[0][b] + ((u64)o->limb[1][b] << 15) + ((u64)o->limb[2][b] << 30);
-      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < C) {
+          const SampleShared* o = cluster.map_shared_rank(&sh, r);
+          cnt += o->count[b];
+          if (by_mass) ms += (u64)o->limb[0][b] + ((u64)o->limb[1][b] << 15) + ((u64)o->limb[2][b] << 30);
+        }
       lead->total[b] = cnt;
       lead->mass[b] = ms;
     }
@@ -442,7 +687,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
     cluster.sync();
   };
   if (small_k) {
-    gather([&](float l, int) { return l >= bound; });
+    list_pass<T>(s, bound, 0, lead);
+    cluster.sync();
     const uint32_t m = lead->n_items;
     if (m <= LIST_CAP) {
       if (rank == 0) {
@@ -460,7 +706,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
     join_bins(false);
     find_bin(false, 0, (u64)top_k);
     const int bin = (int)(uint32_t)lead->result[0];
-    gather([&](float l, int) { return joint_bin(l) <= bin; });
+    list_pass<T>(s, bin == NBINS - 1 ? -INFINITY : lowest((float)(bin + 1) / (NBINS / BIN_SPAN)), 0, lead);
+    cluster.sync();
     const uint32_t m = lead->n_items;
     if (m <= LIST_CAP) {
       if (rank == 0) {
@@ -480,164 +727,94 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
     const bool by_mass = pass == 1;
     u64 want = by_mass ? 0 : (u64)top_k;  // the mass to reach is known once all masses are summed
     u64 above = 0, upto = 0, bin_elems = 0;
-    // bins of a level: every block adds up its own, the cluster's sums are found by each warp for
-    // itself. Returns whether `want` is reached, and where.
-    const auto find_private = [&](int level, int& bin) -> bool {
-      __syncthreads();
-      {
-        // a thread for 16 of the 32 words of (bin, warp), from different banks; the pair joins
-        const int b = tid >> 5, w = (tid & 31) >> 1, h = tid & 1;
-        u64 ms = 0;
-        uint32_t cnt = 0;
+    __syncthreads();
+    bins_pass<T>(s, wt, inv_t, cut, by_mass);
+    __syncthreads();
+    {
+      // a thread for 16 of the 32 words of (bin, warp), from different banks; the pair joins
+      const int b = tid >> 5, w = (tid & 31) >> 1, h = tid & 1;
+      u64 ms = 0;
+      uint32_t cnt = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const u64 v = sh.priv[b][w * 32 + h * 16 + ((i + w) & 15)];
-          ms += v & 0xfffffffffffffull;
-          cnt += (uint32_t)(v >> 52);
-        }
-        ms += __shfl_xor_sync(0xffffffffu, ms, 1);
-        if (level == 0 && h == 0) sh.warp_bin[b][w] = ms;
-        ms = warp_sum(ms) >> 1;  // every pair counts twice
-        cnt = __reduce_add_sync(0xffffffffu, cnt);
-        if (lane == 0) {
-          sh.bin_mass[level][b] = ms;
-          sh.bin_count[level][b] = cnt;
-        }
+      for (int i = 0; i < 16; ++i) {
+        const u64 v = sh.priv[b][w * 32 + h * 16 + ((i + w) & 15)];
+        ms += v & 0xfffffffffffffull;
+        cnt += (uint32_t)(v >> 52);
       }
-      cluster.sync();
+      ms += __shfl_xor_sync(0xffffffffu, ms, 1);
+      if (h == 0) sh.warp_bin[b][w] = ms;
+      ms = warp_sum(ms) >> 1;  // every pair counts twice
+      cnt = __reduce_add_sync(0xffffffffu, cnt);
+      if (lane == 0) {
+        sh.bin_mass[b] = ms;
+        sh.bin_count[b] = cnt;
+      }
+    }
+    cluster.sync();
+    // every warp finds the bin for itself
+    int bin0;
+    {
       u64 ms = 0, cnt = 0;
-      if (lane < PBINS)
-        for (int r = 0; r < C; ++r) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < C && lane < PBINS) {
           const SampleShared* o = cluster.map_shared_rank(&sh, r);
-          ms += o->bin_mass[level][lane];
-          cnt += o->bin_count[level][lane];
+          ms += o->bin_mass[lane];
+          cnt += o->bin_count[lane];
         }
       const u64 v = by_mass ? ms : cnt;
       if (want == 0) want = part_of(top_p, warp_sum(v));
-      u64 sv = v, sc = cnt;
+      u64 sv = v;
+      uint32_t sc = (uint32_t)cnt;
 #pragma unroll
       for (int o = 1; o < PBINS; o <<= 1) {
-        const u64 x = __shfl_up_sync(0xffffffffu, sv, o), y = __shfl_up_sync(0xffffffffu, sc, o);
+        const u64 x = __shfl_up_sync(0xffffffffu, sv, o);
+        const uint32_t y = __shfl_up_sync(0xffffffffu, sc, o);
         if (lane >= o) sv += x, sc += y;
       }
-      const uint32_t reached = __ballot_sync(0xffffffffu, lane < PBINS && above + sv >= want);
-      if (reached == 0) return false;
-      bin = __ffs(reached) - 1;
-      above += __shfl_sync(0xffffffffu, sv - v, bin);
-      upto += __shfl_sync(0xffffffffu, sc - cnt, bin);  // elements before the bin
-      bin_elems = __shfl_sync(0xffffffffu, cnt, bin);
-      return true;
-    };
-    __syncthreads();
-#pragma unroll
-    for (int b = 0; b < PBINS; ++b) sh.priv[b][tid] = 0;
-    __syncwarp();
-    for (int step = step0; step < step1; ++step) {
-      float l[8];
-      const int i0 = load(step, l);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        u64 m = 1ull << 52;
-        if (by_mass) m += wt.mass(l[e]);
-        if (l[e] > -INFINITY && (cut == 0 || compose(l[e], i0 + e) >= cut))
-          sh.priv[(int)fminf(z_of(l[e]), (float)(PBINS - 1))][tid] += m;
+      const uint32_t reached = __ballot_sync(0xffffffffu, lane < PBINS && sv >= want);
+      if (reached == 0) {  // fewer finite logits than k: nothing to cut
+        cluster.sync();    // the others' sums may still be read
+        continue;
       }
+      bin0 = __ffs(reached) - 1;
+      above = __shfl_sync(0xffffffffu, sv - v, bin0);
+      upto = __shfl_sync(0xffffffffu, sc, bin0);  // elements up to and with the bin
     }
-    int bin0 = 0, bin = 0;
-    if (!find_private(0, bin0)) {  // fewer finite logits than k: nothing to cut
-      cluster.sync();              // the others' sums may still be read
-      continue;
-    }
-    const float z0 = (float)bin0;
-    const bool last0 = bin0 == PBINS - 1;
-    const auto settle = [&](auto&& in) {  // everything that can stay fits the list
-      gather(in);
+    // the bin [bin0, bin0 + 1) as a range of logits
+    const Bin bin{bin0 == PBINS - 1 ? -3.402823466e38f : lowest((float)(bin0 + 1)), bin0 == 0 ? 0.f : lowest((float)bin0),
+                  bin0 == 0, cut};
+    if (upto <= LIST_CAP) {  // everything that can stay fits the list
+      list_pass<T>(s, bin.low, cut, lead);
+      cluster.sync();
       if (rank == 0) {
         const int m = (int)sh.n_items;
         sort_items(sh, m, wt);
         settle_list(a, sh, row, by_mass ? m : min(m, top_k), cut_p, top_p, by_mass ? want : 0, min_p, u, wt);
       }
-      // the others may leave: what is read of them was read before the last barrier
-    };
-    if (upto + bin_elems <= LIST_CAP) {
-      settle([&](float l, int i) { return (last0 || z_of(l) < z0 + 1.f) && (cut == 0 || compose(l, i) >= cut); });
-      return;
+      return;  // (what is read of the others was read before the last barrier)
     }
     // ---- the bin's elements into the warps' queues; from here on only they are looked at
-    const int stretch = place0 + step0 * BLOCK_ELEMS - skew;  // index of the warp's first place
-    int queued = 0;
-    for (int step = step0; step < step1; ++step) {
-      float l[8];
-      const int i0 = load(step, l);
-      uint32_t in = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float z = z_of(l[e]);
-        if (z >= z0 && (last0 || z < z0 + 1.f) && l[e] > -INFINITY && (cut == 0 || compose(l[e], i0 + e) >= cut))
-          in |= 1u << e;
-      }
-      const int cnt = __popc(in);
-      int at = cnt;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, at, o);
-        if (lane >= o) at += x;
-      }
-      const int all = __shfl_sync(0xffffffffu, at, 31);
-      at += queued - cnt;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (in >> e & 1) {
-          if (at < QUEUE) sh.queue[warp][at] = (uint16_t)(i0 + e - stretch);
-          ++at;
-        }
-      queued += all;
-    }
-    __syncwarp();
-    const auto for_bin = [&](auto&& f) {  // every element of the bin that this warp owns
-      if (queued <= QUEUE) {
-        for (int q = lane; q < queued; q += 32) {
-          const int i = stretch + (int)sh.queue[warp][q];
-          f(load_one(i), i);
-        }
-      } else {
-        for_each([&](float l, int i) {
-          const float z = z_of(l);
-          if (z >= z0 && (last0 || z < z0 + 1.f) && l > -INFINITY && (cut == 0 || compose(l, i) >= cut)) f(l, i);
-        });
-      }
+    const int queued = queue_pass<T>(s, bin);
+    // a histogram over the bin's elements, joined in the leader: the part where `want` is reached
+    const auto histogram = [&](const Parts& parts) {
+      clear_bins();
+      __syncthreads();
+      histogram_pass<T>(s, wt, bin, parts, by_mass, queued);
+      join_bins(by_mass);
+      find_bin(by_mass, above, want);
+      bin_elems = lead->result[0] >> 32;
+      above = lead->result[1];
+      return (int)(uint32_t)lead->result[0];
     };
-    __syncthreads();  // the first level's bins have been read
-#pragma unroll
-    for (int b = 0; b < PBINS; ++b) sh.priv[b][tid] = 0;
-    // parts of 1/16: z - z0 is exact, as z lies within a factor of two of z0 (or z0 is 0)
-    const auto part_bin = [&](float l) { return (int)fminf((z_of(l) - z0) * PBINS, (float)(PBINS - 1)); };
-    for_bin([&](float l, int) { sh.priv[part_bin(l)][tid] += (1ull << 52) + (by_mass ? wt.mass(l) : 0); });
-    find_private(1, bin);
-    if (upto + bin_elems <= LIST_CAP) {
-      const int to = bin;
-      settle([&](float l, int i) {
-        const float z = z_of(l);
-        if (z < z0) return cut == 0 || compose(l, i) >= cut;
-        return (last0 || z < z0 + 1.f) && part_bin(l) <= to && (cut == 0 || compose(l, i) >= cut);
-      });
-      return;
-    }
-    // ---- refine the part: bins of 2^shift composed numbers from ceil_c down
-    u64 floor_c = 0, ceil_c = ~0ull;
+    // 1024 parts (of the open last bin: 1/64 each; z - bin0 is exact, as z lies within a factor of two
+    // of bin0 or bin0 is 0, and beyond that everything is in the last part)
+    Parts parts{top, inv_t, (float)bin0, bin0 == PBINS - 1 ? 64.f : (float)NBINS, -1, 0, 0};
+    int part = histogram(parts);
     if (bin_elems > LIST_CAP) {
-      u64 first = ~0ull, last = 0;
-      for_bin([&](float l, int i) {
-        if (part_bin(l) != bin) return;
-        const u64 c = compose(l, i);
-        first = min(first, c);
-        last = max(last, c);
-      });
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
-        last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
-      }
+      // ---- refine the part: bins of 2^shift composed numbers from ceil_c down
+      u64 first, last;
+      range_pass<T>(s, bin, parts, part, queued, first, last);
       __syncthreads();
       if (tid == 0) {
         sh.range[0] = ~0ull;
@@ -654,40 +831,19 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
         first = min(first, o->range[0]);
         last = max(last, o->range[1]);
       }
-      floor_c = first;
-      ceil_c = last;
-      clear_bins();
-      cluster.sync();  // `range` and the bins may be used again
+      parts.floor_c = first;
+      parts.ceil_c = last;
       while (bin_elems > LIST_CAP) {
-        const int shift = max(0, 64 - __clzll((long long)(ceil_c - floor_c)) - 10);  // width >> shift < NBINS = 2^10
-        for_bin([&](float l, int i) {
-          const u64 c = compose(l, i);
-          if (c < floor_c || c > ceil_c) return;
-          const int b = (int)((ceil_c - c) >> shift);
-          atomicAdd(&sh.count[b], 1u);
-          if (by_mass) {
-            const u64 w = wt.mass(l);
-            atomicAdd(&sh.limb[0][b], (uint32_t)(w & 0x7fff));
-            atomicAdd(&sh.limb[1][b], (uint32_t)(w >> 15) & 0x7fff);
-            atomicAdd(&sh.limb[2][b], (uint32_t)(w >> 30));
-          }
-        });
-        join_bins(by_mass);
-        clear_bins();  // for the next histogram
-        find_bin(by_mass, above, want);
-        bin_elems = lead->result[0] >> 32;
-        above = lead->result[1];
-        ceil_c -= (u64)(uint32_t)lead->result[0] << shift;
-        const u64 size = 1ull << shift;
-        if (ceil_c - floor_c >= size) floor_c = ceil_c - size + 1;
-        cluster.sync();  // `result` may be written again
+        // width >> shift < NBINS = 2^10
+        parts.shift = max(0, 64 - __clzll((long long)(parts.ceil_c - parts.floor_c)) - 10);
+        part = histogram(parts);
+        parts.ceil_c -= (u64)part << parts.shift;
+        const u64 size = 1ull << parts.shift;
+        if (parts.ceil_c - parts.floor_c >= size) parts.floor_c = parts.ceil_c - size + 1;
+        part = 0;  // of the narrowed range
       }
     }
-    const bool by_part = ceil_c == ~0ull;
-    for_bin([&](float l, int i) {
-      const u64 c = compose(l, i);
-      if (by_part ? part_bin(l) == bin : c >= floor_c && c <= ceil_c) lead->item[atomicAdd(&lead->n_items, 1u)] = c;
-    });
+    list_part_pass<T>(s, bin, parts, part, queued, lead);
     cluster.sync();
     // these elements decide: sort them, the cut is the one at which `want` is reached
     if (rank == 0) {
@@ -707,11 +863,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
     cut = lead->result[0];
     if (by_mass && !(min_p > 0)) {
       // the mass that stays: all of the bins before, of the bin what the queue holds from the cut on
-      u64 m = 0;
-      for_bin([&](float l, int i) {
-        if (compose(l, i) >= cut) m += wt.mass(l);
-      });
-      m = warp_sum(m);
+      u64 m = kept_queue_pass<T>(s, Kept{wt, cut, 0.0}, bin, queued);
       for (int b = 0; b < bin0; ++b) m += sh.warp_bin[b][warp];
       if (lane == 0) sh.kept[warp] = m;
       kept_known = true;
@@ -720,14 +872,9 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
   }
 
   // ---- the draw: block, warp, step of 256 elements, element
-  const auto kept_mass = [&](float l, int i) -> u64 {
-    const double w = wt(l);
-    return w >= min_p && (cut == 0 || compose(l, i) >= cut) && l >= wt.l_min ? wt.mass(w) : 0;
-  };
+  const Kept kept{wt, cut, min_p};
   if (!kept_known) {
-    u64 m = 0;
-    for_each([&](float l, int i) { m += kept_mass(l, i); });
-    m = warp_sum(m);
+    const u64 m = kept_pass<T>(s, kept);
     if (lane == 0) sh.kept[warp] = m;
   }
   __syncthreads();
@@ -737,23 +884,24 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
   if (tid == 0) sh.share_mass = share;
   cluster.sync();
   u64 total = 0, before = 0;
-  for (int r = 0; r < C; ++r) {
-    const u64 m = cluster.map_shared_rank(&sh, r)->share_mass;
-    total += m;
-    if (r < rank) before += m;
-  }
+#pragma unroll
+  for (int r = 0; r < 8; ++r)
+    if (r < C) {
+      const u64 m = cluster.map_shared_rank(&sh, r)->share_mass;
+      total += m;
+      if (r < rank) before += m;
+    }
   const u64 target = target_of(u, total);
   if (before <= target && target < before + share) {  // one block of the cluster
     int owner = 0;
     u64 b = before;
     while (owner < SAMPLE_WARPS - 1 && target >= b + sh.kept[owner]) b += sh.kept[owner++];
-    const int first = min(owner * per_warp, n_steps), steps = min(first + per_warp, n_steps) - first;
+    const int first = min(owner * s.per_warp, s.n_steps), steps = min(first + s.per_warp, s.n_steps) - first;
     for (int step = warp; step < steps; step += SAMPLE_WARPS) {
-      float l[8];
+      const int i0 = s.index(first + step);
       u64 m = 0;
-      const int i0 = load(first + step, l);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m += kept_mass(l[e], i0 + e);
+#pragma unroll 1
+      for (int i = max(i0, 0); i < min(i0 + 8, a.V); ++i) m += kept(s.one(i), i);
       m = warp_sum(m);
       if (lane == 0) sh.steps[step] = m;
     }
@@ -761,28 +909,28 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
     if (warp == 0) {
       int step = 0;
       while (step < steps - 1 && target >= b + sh.steps[step]) b += sh.steps[step++];
-      float l[8];
-      u64 m[8], lane_sum = 0;
-      const int i0 = load(first + step, l);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        m[e] = kept_mass(l[e], i0 + e);
-        lane_sum += m[e];
-      }
-      u64 s = lane_sum;
+      const int i0 = s.index(first + step), i1 = min(i0 + 8, a.V);
+      u64 lane_sum = 0;
+#pragma unroll 1
+      for (int i = max(i0, 0); i < i1; ++i) lane_sum += kept(s.one(i), i);
+      u64 upto_lane = lane_sum;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const u64 x = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += x;
+        const u64 x = __shfl_up_sync(0xffffffffu, upto_lane, o);
+        if (lane >= o) upto_lane += x;
       }
-      b += s - lane_sum;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (b <= target && target < b + m[e]) {
-          a.token[row] = i0 + e;
-          if (a.logprob) a.logprob[row] = (float)log((double)m[e] / (double)total);
+      b += upto_lane - lane_sum;
+      if (b <= target && target < b + lane_sum) {  // one lane
+#pragma unroll 1
+        for (int i = max(i0, 0); i < i1; ++i) {
+          const u64 m = kept(s.one(i), i);
+          if (target < b + m) {
+            a.token[row] = i;
+            if (a.logprob) a.logprob[row] = (float)log((double)m / (double)total);
+            break;
+          }
+          b += m;
         }
-        b += m[e];
       }
     }
   }

@@ -546,6 +546,13 @@ def test_sample_masked_and_odd_logits(V):
             if u == 0.0 and f.get("p"):
                 continue
             check_sample(V, rows, uu + 0.013, **f)
+    # the lowest finite number as the largest logit; temperatures at which one step of fp32 is everything
+    low = -torch.finfo(torch.float32).max
+    edge = torch.tensor([[-inf, low, -inf, low, low], [0.0, -1e-45, 0.0, 1e-45, -inf], [1.0, 1.0 - 2**-24, 1.0, -1.0, 0.5]],
+                        device="cuda")
+    for t in (1e-45, 1e-38, 1e-30, 1e-3, 1.0, 3e38):
+        for f in ({}, dict(p=0.4), dict(k=2)):
+            check_sample(V, edge, torch.full((3,), 0.57, device="cuda"), t=t, **f)
     tok, lp = V.sample_tokens(rows, torch.full((7,), 0.9, device="cuda"), return_logprob=True)
     assert tok.tolist()[1:4] == [0, 0, 2] and lp[1] == -inf and lp[2] == -inf
     # uniforms outside [0, 1): the nearest token
