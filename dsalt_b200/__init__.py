@@ -16,6 +16,7 @@ from .ops import (  # noqa: F401
     window_signals,
 )
 from .serving import (  # noqa: F401
+    PagedCache,
     SlotPlan,
     append_cache,
     cache_attention,

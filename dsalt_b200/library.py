@@ -8,6 +8,10 @@ keeps its kernels opaque (``_dynamo_opaque``, ``dsalt/kernels/dsalt_triton_attn.
 * ``torch.ops.dsalt_b200.dsalt_attention``  → :func:`dsalt_b200.ops.dsalt_attention`
 * ``torch.ops.dsalt_b200.core_forward``     → :func:`dsalt_b200.ops.core_forward`
 
+* ``torch.ops.dsalt_b200.append_cache`` / ``cache_attention`` / ``sample_tokens``
+  → the functions of :mod:`dsalt_b200.serving` of these names (``sample_tokens`` with its settings as
+  numbers and the log-probability)
+
 ``cu_list`` (the host copy of ``cu_seqlens``) is an ``int[]`` argument: the kernels size
 their launches and workspaces from it, so a compiled graph is specialised on the packing.
 The fake (meta) functions give the output shapes and dtypes; no real implementation runs
@@ -20,6 +24,7 @@ from typing import List, Optional
 import torch
 
 from . import ops
+from . import serving
 
 
 def _n_sets(cu_list: List[int], mode: str, block: int) -> int:
@@ -80,3 +85,40 @@ def core_forward(x: torch.Tensor, gate_weight: torch.Tensor, gate_bias: torch.Te
 def _(x, gate_weight, gate_bias, n_min, n_max, alpha, q, k, v, k_lmk, cu_seqlens, mode, block, norm_round, cu_list,
       out_dtype, logit):
     return q.new_empty(q.shape, dtype=out_dtype)
+
+
+@torch.library.custom_op("dsalt_b200::append_cache", mutates_args=("k_cache", "v_cache", "k_scale", "v_scale"))
+def append_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                 v_scale: torch.Tensor, slots: torch.Tensor) -> None:
+    serving.append_cache(k, v, k_cache, v_cache, k_scale, v_scale, slots)
+
+
+@append_cache.register_fake
+def _(k, v, k_cache, v_cache, k_scale, v_scale, slots):
+    return None
+
+
+@torch.library.custom_op("dsalt_b200::cache_attention", mutates_args=())
+def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                    v_scale: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                    cu_q: Optional[torch.Tensor], w_sizes: Optional[torch.Tensor], lmk_indices: Optional[torch.Tensor],
+                    lmk_bias: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
+    return serving.cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q=cu_q,
+                                   w_sizes=w_sizes, lmk_indices=lmk_indices, lmk_bias=lmk_bias, out_dtype=out_dtype)
+
+
+@cache_attention.register_fake
+def _(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, w_sizes, lmk_indices, lmk_bias, out_dtype):
+    return q.new_empty(q.shape, dtype=out_dtype)
+
+
+@torch.library.custom_op("dsalt_b200::sample_tokens", mutates_args=())
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: float, top_k: int, top_p: float,
+                  min_p: float) -> List[torch.Tensor]:
+    return list(serving.sample_tokens(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p,
+                                      return_logprob=True))
+
+
+@sample_tokens.register_fake
+def _(logits, u, temperature, top_k, top_p, min_p):
+    return [logits.new_empty(logits.shape[0], dtype=torch.int64), logits.new_empty(logits.shape[0], dtype=torch.float32)]

@@ -8,7 +8,9 @@ so a reference checkpoint loads unchanged. Every block's attention is
 :class:`dsalt_b200.DSALTAttention` (widths, landmark selection and the sparse attention on
 this package's kernels); norms, the SwiGLU MLP, embeddings and the LM head are library
 ops. Packed input only (``input_ids [T]`` with ``cu_seqlens``), inference only: training,
-the losses and the batched path are not part of this package.
+the losses and the batched path are not part of this package. ``generate`` (no counterpart in
+the reference) answers prompts token by token over the paged 8-bit cache of
+:mod:`dsalt_b200.serving`.
 """
 from __future__ import annotations
 
@@ -22,6 +24,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .module import DSALTAttention
+from .serving import PagedCache, sample_tokens
 
 
 @dataclass
@@ -127,6 +130,15 @@ class DSALTTransformerBlock(nn.Module):
         return x, aux
 
 
+    def prefill(self, x, cu_seqlens, cu_h, rope_cs, cache, plan):
+        x = x + self.attn.prefill(self.attn_norm(x), cu_seqlens, cu_h, rope_cs, cache, plan)
+        return x + self.ffn(self.ffn_norm(x))
+
+    def decode(self, x, rope_cs, cache, plan):
+        x = x + self.attn.decode(self.attn_norm(x), rope_cs, cache, plan)
+        return x + self.ffn(self.ffn_norm(x))
+
+
 class DSALTLMHeadModel(nn.Module):
     """Causal LM: embeddings, ``n_layers`` DSALT blocks, a final RMSNorm and the LM head
     (tied to the embedding by default); the reference's initialisation (``N(0, 0.02)``,
@@ -190,3 +202,87 @@ class DSALTLMHeadModel(nn.Module):
         if logits_to_keep > 0:
             x = x[T - logits_to_keep:]
         return {"loss": None, "logits": self.lm_head(x), "aux_loss": None}
+
+    # ---------------------------------------------------------------- generation
+    def new_cache(self, max_seqs: int, max_len: int, *, n_pages: int | None = None, page_size: int = 64) -> PagedCache:
+        """A cache of this model's shape for ``max_seqs`` sequences of up to ``max_len`` tokens."""
+        a = self.layers[0].attn
+        if a.selection != "block_causal":
+            raise NotImplementedError("generation needs selection='block_causal': whole-sequence landmarks depend on "
+                                      "tokens that are not there yet")
+        if max_len > a.max_seq_len:
+            raise ValueError(f"max_len {max_len} beyond the model's max_seq_len {a.max_seq_len}")
+        return PagedCache(self.n_layers, a.n_heads, a.n_kv_heads, a.head_dim, a.k_lmk, max_seqs=max_seqs,
+                          max_len=max_len, n_pages=n_pages, page_size=page_size, device=self.embed_tokens.weight.device)
+
+    def _embed(self, ids, positions):
+        x = self.embed_tokens(ids)
+        if x.is_cuda and torch.is_autocast_enabled("cuda"):
+            x = x.to(torch.get_autocast_dtype("cuda"))
+        attn0 = self.layers[0].attn
+        at = positions.long()
+        return x, (attn0.rope_cos.to(x.device)[at], attn0.rope_sin.to(x.device)[at])
+
+    @torch.no_grad()
+    def prefill(self, input_ids, cu_list, cache: PagedCache):
+        """Packed prompts (``cu_list``: the host list of their borders, one per row of the cache, whose
+        rows must be empty) into the cache; the logits of each prompt's last token ``[S, vocab]``."""
+        cu_h = [int(c) for c in cu_list]
+        lens = [b - a for a, b in zip(cu_h, cu_h[1:])]
+        if len(lens) != cache.max_seqs or min(lens) < 1 or cu_h[-1] != input_ids.shape[0]:
+            raise ValueError("cu_list must give one prompt of at least one token per row of the cache")
+        if any(cache.lens):
+            raise ValueError("prefill needs empty rows: release them first")
+        plan = cache.reserve(lens)
+        x, rope_cs = self._embed(input_ids, plan.positions)
+        for layer in self.layers:
+            x = layer.prefill(x, plan.cu_new, cu_h, rope_cs, cache, plan)
+        return self.lm_head(self.final_norm(x[plan.cu_new[1:].long() - 1]))
+
+    @torch.no_grad()
+    def decode(self, tokens, cache: PagedCache):
+        """One more token per row of the cache ``tokens [S]`` → the next token's logits ``[S, vocab]``."""
+        if min(cache.lens) < 1:
+            raise ValueError("decode needs a prompt in every row")
+        plan = cache.reserve([1] * cache.max_seqs)
+        x, rope_cs = self._embed(tokens, plan.positions)
+        for layer in self.layers:
+            x = layer.decode(x, rope_cs, cache, plan)
+        return self.lm_head(self.final_norm(x))
+
+    @torch.no_grad()
+    def generate(self, prompts, max_new_tokens: int, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                 eos_token: int | None = None, generator: torch.Generator | None = None, page_size: int = 64):
+        """Answers to ``prompts`` (a list of lists of token ids): a list of lists of up to
+        ``max_new_tokens`` ids each, ending with ``eos_token`` where it was drawn. The settings are those
+        of :func:`dsalt_b200.serving.sample_tokens`; the uniforms come from ``generator`` (a CUDA
+        generator; torch's own without one)."""
+        if self.training:
+            raise RuntimeError("generate needs eval mode")
+        if max_new_tokens < 1 or not prompts or min(len(p) for p in prompts) < 1:
+            raise ValueError("generate needs prompts of at least one token and max_new_tokens >= 1")
+        dev = self.embed_tokens.weight.device
+        lens = [len(p) for p in prompts]
+        S = len(prompts)
+        pages = sum(-(-(n + max_new_tokens - 1) // page_size) for n in lens)
+        cache = self.new_cache(S, max(lens) + max_new_tokens - 1, n_pages=pages, page_size=page_size)
+        cu_h = [0]
+        for n in lens:
+            cu_h.append(cu_h[-1] + n)
+        ids = torch.tensor([t for p in prompts for t in p], dtype=torch.long, device=dev)
+        logits = self.prefill(ids, cu_h, cache)
+        drawn, done = [], torch.zeros(S, dtype=torch.bool, device=dev)
+        for step in range(max_new_tokens):
+            u = torch.rand(S, device=dev, generator=generator)
+            token = sample_tokens(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+            drawn.append(token)
+            if eos_token is not None:
+                done |= token == eos_token
+                if bool(done.all()):
+                    break
+            if step + 1 < max_new_tokens:
+                logits = self.decode(token, cache)
+        answers = torch.stack(drawn, 1).tolist()
+        if eos_token is not None:
+            answers = [a[:a.index(eos_token) + 1] if eos_token in a else a for a in answers]
+        return answers

@@ -27,6 +27,11 @@ scores (differentiable in ``alpha_w``, ``x`` and ``v_proj``), and the soft-selec
 of :func:`dsalt_b200.ops.dsalt_train_attention`, whose backward carries the gradients of the
 soft window edge to ``win_gate`` and of the landmark weights to ``alpha_w``.
 
+``prefill`` and ``decode`` are the same attention with a paged 8-bit cache
+(:mod:`dsalt_b200.serving`): prompts as above, then a token at a time against what the cache
+holds. They need ``selection="block_causal"``, whose set for a position depends on earlier
+blocks only; the reference has no counterpart.
+
 Out of scope (raise): the batched ``[B, T, d]`` path, and training with
 ``selection="block_causal"`` (the training kernel takes one landmark set per sequence, as
 the reference's does).
@@ -187,9 +192,14 @@ class DSALTAttention(nn.Module):
 
     @torch.no_grad()
     def _packed(self, x, cu_seqlens, total_len, device, rope_cs=None, cu_list=None):
-        T, H, Hkv, D = total_len, self.n_heads, self.n_kv_heads, self.head_dim
         cu_h = ops._host_cu(cu_seqlens, cu_list)
-        q, k, v = self._qkv(x, cu_h, T, device, rope_cs)
+        out, q, k, _, w, _, _, alpha = self._packed_core(x, cu_seqlens, total_len, device, rope_cs, cu_h)
+        self._last_P = self._rebuild_last_P(x, q, k, w, alpha, cu_h) if self._collect_last_P else None
+        aux = torch.zeros((), device=x.device, dtype=x.dtype)
+        return self.out_proj(out.view(total_len, self.d_model).to(self.out_proj.weight.dtype)), aux
+
+    def _signals(self, x, v):
+        """Widths and selection norms of ``x`` (``v``: its value projection, as a head view)."""
         amp = torch.is_autocast_enabled("cuda") if x.is_cuda else False
         # the width logit comes from the same library op as the reference's
         # _window_continuous (win_gate(x), :275), so that the widths equal the reference's
@@ -201,16 +211,47 @@ class DSALTAttention(nn.Module):
         vs = v if self.v_proj.bias is None else F.linear(x, self.v_proj.weight.to(v.dtype))
         norm_round = (x.dtype != torch.float32) and not amp
         # the operators as registered torch.library ops: opaque nodes under torch.compile
-        w, xn, vn = torch.ops.dsalt_b200.window_signals(x, gw, gb, self.n_min, self.n_max, vs, D, norm_round, logit)
+        return torch.ops.dsalt_b200.window_signals(x, gw, gb, self.n_min, self.n_max, vs, self.head_dim, norm_round,
+                                                   logit)
+
+    def _packed_core(self, x, cu_seqlens, total_len, device, rope_cs, cu_h):
+        """Projections, signals, selection and attention of a pack: ``(out, q, k, v, w, xn, vn,
+        alpha)``."""
+        q, k, v = self._qkv(x, cu_h, total_len, device, rope_cs)
+        w, xn, vn = self._signals(x, v)
         alpha = self._alpha().detach().float()
         mode = "global" if self.selection == "global" else "block_causal"
-        lmk = torch.ops.dsalt_b200.select_landmarks(xn, vn, w, alpha, cu_seqlens, self.k_lmk, H, mode, self.block,
-                                                    cu_h)
+        lmk = torch.ops.dsalt_b200.select_landmarks(xn, vn, w, alpha, cu_seqlens, self.k_lmk, self.n_heads, mode,
+                                                    self.block, cu_h)
         out = torch.ops.dsalt_b200.dsalt_attention(q.contiguous(), k.contiguous(), v.contiguous(), lmk, None, w,
                                                    cu_seqlens, 0 if mode == "global" else self.block, cu_h, q.dtype)
-        self._last_P = self._rebuild_last_P(x, q, k, w, alpha, cu_h) if self._collect_last_P else None
-        aux = torch.zeros((), device=x.device, dtype=x.dtype)
-        return self.out_proj(out.view(T, self.d_model).to(self.out_proj.weight.dtype)), aux
+        return out, q, k, v, w, xn, vn, alpha
+
+    # ---------------------------------------------------------------- generation
+    @torch.no_grad()
+    def prefill(self, x, cu_seqlens, cu_h, rope_cs, cache, plan):
+        """Packed prompts as :meth:`forward` does, their keys, values and signals into the layer of
+        a :class:`dsalt_b200.serving.PagedCache` (``plan``: the cache's slots for them)."""
+        out, _, k, v, w, xn, vn, alpha = self._packed_core(x, cu_seqlens, x.shape[0], x.device, rope_cs, cu_h)
+        cache.append(self.layer_idx, k, v, w, xn, vn, plan)
+        cache.update_landmarks(self.layer_idx, alpha, self.k_lmk, self.block)
+        return self.out_proj(out.view(x.shape[0], self.d_model).to(self.out_proj.weight.dtype))
+
+    @torch.no_grad()
+    def decode(self, x, rope_cs, cache, plan):
+        """One token per row ``x [S, d_model]`` against the cached sequences: its window and its block's
+        landmarks, the query's own key and value included (all as the cache holds them, in 8 bits)."""
+        T = x.shape[0]
+        q = self.q_proj(x).view(T, self.n_heads, self.head_dim)
+        k = self.k_proj(x).view(T, self.n_kv_heads, self.head_dim)
+        v = self.v_proj(x).view(T, self.n_kv_heads, self.head_dim)
+        cos, sin = (t.to(q.dtype).unsqueeze(1) for t in rope_cs)
+        q, k = apply_rotary_emb(q, k, cos, sin)
+        w, xn, vn = self._signals(x, v)
+        cache.append(self.layer_idx, k, v, w, xn, vn, plan)
+        cache.update_landmarks(self.layer_idx, self._alpha().detach().float(), self.k_lmk, self.block)
+        out = cache.attention(self.layer_idx, q, w)
+        return self.out_proj(out.view(T, self.d_model).to(self.out_proj.weight.dtype))
 
     @torch.no_grad()
     def _rebuild_last_P(self, x, q, k, w, alpha, cu_h):

@@ -9,6 +9,9 @@ reads it, and sampling.
   tokens per sequence over the cache
 * :func:`sample_tokens`   — temperature, top-k, top-p and min-p from given uniforms
 
+:class:`PagedCache` holds the state of several sequences for a decoder stack and makes these
+calls for it (:meth:`dsalt_b200.model.DSALTLMHeadModel.generate`).
+
 The reference has no counterpart (it recomputes the whole sequence for every token). As in
 :mod:`dsalt_b200.ops`, tensors must be CUDA tensors and every call launches on the current
 stream of their device; lengths and tables stay on the device, so nothing here synchronises
@@ -22,6 +25,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib as L
+from . import ops
 from .ops import _dt, _ptr, _workspace
 
 PAGE_SIZES = (16, 32, 64, 128)
@@ -262,3 +266,109 @@ def sample_tokens(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     _run(dev, "dsalt_sample", logits.data_ptr(), _dt(logits), B, V, logits.stride(0) if B > 1 else V, u.data_ptr(),
          _ptr(t), tv, _ptr(k), kv, _ptr(p), pv, _ptr(mp), mv, token.data_ptr(), _ptr(logprob))
     return (token, logprob) if return_logprob else token
+
+
+# --------------------------------------------------------------------------- a decoder stack's state
+class PagedCache:
+    """Keys and values of ``max_seqs`` sequences for ``n_layers`` layers in pages of
+    ``page_size`` tokens, with what the landmark selection needs of them (norms and widths per
+    position) and the current landmark sets ``[H, max_seqs, k]`` per layer.
+
+    Rows are sequences. All rows are used together: :meth:`reserve` takes the number of new
+    tokens of each row. ``lens`` is the host's copy of the lengths, kept so that block borders
+    are known without reading the device; a row whose tokens the pool or the tables cannot
+    hold is refused here, before anything is launched."""
+
+    def __init__(self, n_layers: int, n_heads: int, n_kv_heads: int, head_dim: int, k_lmk: int, *, max_seqs: int,
+                 max_len: int, n_pages: int | None = None, page_size: int = 64, device="cuda"):
+        if page_size not in PAGE_SIZES:
+            raise ValueError(f"page_size must be one of {PAGE_SIZES}")
+        if not 1 <= max_seqs <= MAX_ROWS or max_len < 1:
+            raise ValueError(f"max_seqs must be in [1, {MAX_ROWS}] and max_len positive")
+        self.max_seqs, self.max_len, self.page_size = max_seqs, max_len, page_size
+        self.max_pages = -(-max_len // page_size)
+        self.n_pages = self.max_pages * max_seqs if n_pages is None else int(n_pages)
+        dev = torch.device(device)
+        i32 = torch.int32
+        self.block_tables = torch.full((max_seqs, self.max_pages), -1, dtype=i32, device=dev)
+        self.seq_lens = torch.zeros(max_seqs, dtype=i32, device=dev)
+        self.free_pages = torch.arange(self.n_pages - 1, -1, -1, dtype=i32, device=dev)
+        self.n_free = torch.full((1,), self.n_pages, dtype=i32, device=dev)
+        self.lens = [0] * max_seqs
+        kv = (n_layers, self.n_pages, n_kv_heads, page_size, head_dim)
+        self.k = torch.zeros(kv, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+        self.v = torch.zeros(kv, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+        self.k_scale = torch.zeros(n_layers, self.n_pages, n_kv_heads, device=dev)
+        self.v_scale = torch.zeros(n_layers, self.n_pages, n_kv_heads, device=dev)
+        self.xnorm = torch.zeros(n_layers, max_seqs, max_len, device=dev)
+        self.vnorm = torch.zeros(n_layers, max_seqs, max_len, n_kv_heads, device=dev)
+        self.width = torch.zeros(n_layers, max_seqs, max_len, dtype=i32, device=dev)
+        self.lmk = torch.full((n_layers, n_heads, max_seqs, k_lmk), -1, dtype=i32, device=dev)
+        self._rows = None
+        self._block_of = [[-1] * max_seqs for _ in range(n_layers)]  # whose set `lmk` holds
+
+    def pages_held(self) -> int:
+        return sum(-(-n // self.page_size) for n in self.lens)
+
+    def reserve(self, new_lens) -> SlotPlan:
+        """Slots for ``new_lens`` (a list, one number per row) more tokens, packed row after row."""
+        new_lens = [int(n) for n in new_lens]
+        if len(new_lens) != self.max_seqs or min(new_lens) < 0:
+            raise ValueError(f"new_lens must give {self.max_seqs} numbers of new tokens")
+        lens = [a + b for a, b in zip(self.lens, new_lens)]
+        if max(lens) > self.max_len:
+            raise ValueError(f"a sequence of {max(lens)} tokens in a cache for {self.max_len}")
+        need = sum(-(-n // self.page_size) for n in lens)
+        if need > self.n_pages:
+            raise ValueError(f"{need} pages wanted of a pool of {self.n_pages}")
+        dev = self.seq_lens.device
+        new = torch.tensor(new_lens, dtype=torch.int32, device=dev)
+        plan = reserve_slots(self.block_tables, self.seq_lens, new, self.free_pages, self.n_free, self.page_size,
+                             sum(new_lens), inplace=True)
+        self.lens = lens
+        self._rows = torch.repeat_interleave(torch.arange(self.max_seqs, device=dev), new.long(),
+                                             output_size=sum(new_lens))
+        return plan
+
+    def release(self, rows) -> None:
+        """Ends the sequences of these rows; their pages go back to the pool."""
+        flags = [False] * self.max_seqs
+        for r in rows:
+            flags[r] = True
+            self.lens[r] = 0
+            for blocks in self._block_of:
+                blocks[r] = -1
+        release_slots(self.block_tables, self.seq_lens, torch.tensor(flags, device=self.seq_lens.device), self.free_pages,
+                      self.n_free, self.page_size)
+
+    def append(self, layer: int, k, v, w, xn, vn, plan: SlotPlan) -> None:
+        """New tokens of all rows (packed as ``plan`` says) into one layer."""
+        append_cache(k, v, self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer], plan.slots)
+        at = (self._rows, plan.positions.long())
+        self.xnorm[layer].index_put_(at, xn)
+        self.vnorm[layer].index_put_(at, vn)
+        self.width[layer].index_put_(at, w)
+
+    def update_landmarks(self, layer: int, alpha, k_lmk: int, block: int) -> None:
+        """The set of the block that each row's last position lies in, where it is a new one: drawn
+        from the positions before the block, with their statistics, as
+        :func:`dsalt_b200.ops.select_landmarks` does in block-causal mode."""
+        H = self.lmk.shape[1]
+        for r, n in enumerate(self.lens):
+            b = (n - 1) // block
+            if n == 0 or k_lmk == 0 or self._block_of[layer][r] == b:
+                continue
+            self._block_of[layer][r] = b
+            if b == 0:
+                self.lmk[layer, :, r] = -1
+                continue
+            end = b * block + 1
+            sets = ops.select_block_range(self.xnorm[layer, r, :end], self.vnorm[layer, r, :end],
+                                          self.width[layer, r, :end], alpha, k_lmk, H, block, b, b + 1)
+            self.lmk[layer, :, r] = sets[:, 0]
+
+    def attention(self, layer: int, q, w):
+        """One query token per row over one layer."""
+        lmk = self.lmk[layer] if self.lmk.shape[-1] > 0 else None
+        return cache_attention(q.contiguous(), self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer],
+                               self.block_tables, self.seq_lens, w_sizes=w, lmk_indices=lmk)
