@@ -27,7 +27,7 @@
 // window's, then the landmarks' of each head. Items are cut into units of about equal
 // length, by the lengths found on the device (no host copy of them is needed and a captured
 // call follows them); the parts of an item that was cut are joined by a second kernel.
-// Within a unit each of four warps has its own stretch of tiles and its own ring of
+// Within a unit each of two warps has its own stretch of tiles and its own ring of
 // cp.async stages: nothing but the end is shared, so no warp waits for another.
 #include <type_traits>
 
@@ -35,9 +35,9 @@
 
 namespace dsalt {
 
-constexpr int CA_WARPS = 4;
+constexpr int CA_WARPS = 2;
 constexpr int CA_THREADS = 32 * CA_WARPS;
-constexpr int CA_MIN_TILES = 8;        // tiles of 32 keys that a unit takes at least: two per warp
+constexpr int CA_MIN_TILES = 8;        // tiles of 32 keys that a unit takes at least: four per warp
 constexpr int CA_MAX_SEQS = 8192;
 constexpr int CA_ERR_PAGE = 41;        // device status: a page number outside the pool was met
 constexpr float CA_P_SHIFT = 14.f;     // P is held times 2^14: fp16 stays normal down to 2^-28
@@ -46,12 +46,12 @@ constexpr float CA_SLACK = 1.f;        // P may exceed 2^14 by 2^1 before its re
 // blocks per SM that registers and rings allow; one round of them is the number of units wanted
 template <int D>
 struct Shape {
-  static constexpr int OCC = D == 64 ? 4 : 3;
+  static constexpr int OCC = D == 64 ? 8 : 6;
   static constexpr int STAGES = 2;
   static constexpr int SLOTS = 148 * OCC;
 };
 constexpr int CA_ROWS = 8;
-constexpr int CA_MAX_SLOTS = 148 * 4;
+constexpr int CA_MAX_SLOTS = 148 * 8;
 
 struct CacheAttnArgs {
   const void* q;
@@ -159,8 +159,8 @@ __device__ __forceinline__ int2 block_before2(int2 v, int2* red, int2& all) {
 }
 
 // One stage of a warp's ring: 32 keys. K and V rows of D bytes, their 16-byte chunks placed so
-// that a warp's fragment loads meet no bank twice, and {scale of K, exponent of V's, bias,
-// position or -1}: of landmarks per key, of a window tile per half at keys 0 and 16.
+// that a warp's fragment loads meet no bank twice, and {scale of K, scale of V, bias, position
+// or -1}: of landmarks per key, of a window tile per half at keys 0 and 16.
 template <int D>
 struct Stage {
   static constexpr int V = 32 * D, META = 64 * D, BYTES = 64 * D + 512;
@@ -194,21 +194,26 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
   __shared__ long long s_sum[CA_WARPS][2];
   __shared__ float s_m[CA_WARPS][CA_ROWS], s_l[CA_WARPS][CA_ROWS], s_M[CA_WARPS][CA_ROWS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  int* s_base = reinterpret_cast<int*>(dyn);  // [n_seqs] units of the sequences before s
-  int* s_cut = s_base + a.n_seqs;             // [n_seqs] parts of cut items before s
-  int* s_len = s_cut + a.n_seqs;              // [n_seqs] tiles of an item of s
+  __shared__ struct {
+    SeqPlan plan;
+    int s, local, splits, cut;  // sequence, unit within it, parts of its items, parts of cut items before it
+  } s_job;
+  int* s_items = reinterpret_cast<int*>(dyn);  // [n_seqs] items of the sequence
+  int* s_len = s_items + a.n_seqs;             // [n_seqs] tiles of one of them
   float* s_o = reinterpret_cast<float*>(dyn);  // [warps][8][D], after the rings
 
   // ---- schedule: every block derives the same one from the lengths
   int chunk;
+  SeqPlan first_plan{};
   {
     // tiles and items of the call; both stay below 2^40
     long long mine = 0, count = 0;
     for (int s = tid; s < a.n_seqs; s += CA_THREADS) {
       const SeqPlan p = plan_of(a, s);
+      if (s == tid) first_plan = p;
       const int items = row_tiles(a, p.n_q) * a.Hkv;
       s_len[s] = p.n_window + p.n_lmk;
-      s_base[s] = items;
+      s_items[s] = items;
       mine += (long long)s_len[s] * items;
       count += items;
     }
@@ -219,34 +224,40 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
     }
     if (lane == 0) s_sum[warp][0] = mine, s_sum[warp][1] = count;
     __syncthreads();
-    const long long total = s_sum[0][0] + s_sum[1][0] + s_sum[2][0] + s_sum[3][0];
-    const long long items = s_sum[0][1] + s_sum[1][1] + s_sum[2][1] + s_sum[3][1];
+    long long total = 0, items = 0;
+#pragma unroll
+    for (int w = 0; w < CA_WARPS; ++w) total += s_sum[w][0], items += s_sum[w][1];
     // Cutting adds at most one unit per item: where the items leave room, all units run at once;
     // where they do not, only items above an average slot's load are cut.
     constexpr int SLOTS = Shape<D>::SLOTS;
     const long long want = items < SLOTS ? max(SLOTS - items, (long long)SLOTS / 4) : SLOTS;
     chunk = (int)min(max((total + want - 1) / want, (long long)CA_MIN_TILES), 0x7fffffffLL);
   }
+  const int unit = blockIdx.x;
   int2 carry = make_int2(0, 0);
   for (int base = 0; base < a.n_seqs; base += CA_THREADS) {
     const int s = base + tid;
     int2 v = make_int2(0, 0), all;
+    int splits = 1;
     if (s < a.n_seqs) {
-      const int splits = max(1, (s_len[s] + chunk - 1) / chunk);
-      v.x = s_base[s] * splits;
+      splits = max(1, (s_len[s] + chunk - 1) / chunk);
+      v.x = s_items[s] * splits;
       v.y = splits > 1 ? v.x : 0;
     }
     const int2 b = block_before2(v, red, all);
-    if (s < a.n_seqs) {
-      s_base[s] = carry.x + b.x;
-      s_cut[s] = carry.y + b.y;
+    const int from = carry.x + b.x;
+    if (unit >= from && unit < from + v.x) {  // one thread, if any
+      s_job.plan = base == 0 ? first_plan : plan_of(a, s);
+      s_job.s = s;
+      s_job.local = unit - from;
+      s_job.splits = splits;
+      s_job.cut = carry.y + b.y;
     }
     carry.x += all.x;
     carry.y += all.y;
   }
   __syncthreads();
   cudaTriggerProgrammaticLaunchCompletion();  // the join may take its places; it waits for this grid's end
-  const int unit = blockIdx.x;
   // rows behind the last sequence's: zero, log-sum-exp -inf
   if (a.cu_q) {
     const int64_t rows0 = (int64_t)min(max(a.cu_q[a.n_seqs], 0), a.T) * a.H, rows1 = (int64_t)a.T * a.H;
@@ -262,22 +273,11 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
     }
   }
   if (unit >= carry.x) return;
-  int s = 0;
-  {
-    int lo = 0, hi = a.n_seqs - 1;  // the last sequence whose units begin at or before this one
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (s_base[mid] <= unit) lo = mid;
-      else hi = mid - 1;
-    }
-    s = lo;
-  }
-  const SeqPlan p = plan_of(a, s);
-  const int tiles = p.n_window + p.n_lmk, splits = max(1, (tiles + chunk - 1) / chunk);
-  const int local = unit - s_base[s];
-  const int split = local % splits, item = local / splits;
+  const SeqPlan p = s_job.plan;
+  const int s = s_job.s, splits = s_job.splits, tiles = p.n_window + p.n_lmk;
+  const int split = s_job.local % splits, item = s_job.local / splits;
   const int hk = item % a.Hkv, tile = item / a.Hkv;
-  const int part0 = s_cut[s] + item * splits;
+  const int part0 = s_job.cut + item * splits;
   const int each = (tiles + splits - 1) / splits;
   const int t_begin = min(split * each, tiles), t_end = min(t_begin + each, tiles);
 
@@ -305,6 +305,60 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
     lo_min = min(lo_min, __shfl_xor_sync(0xffffffffu, lo_min, x));
     hi_max = max(hi_max, __shfl_xor_sync(0xffffffffu, hi_max, x));
   }
+  const int page_mask = (1 << a.page_shift) - 1;
+  const int* table = a.tables + (int64_t)s * a.max_pages;
+  const int lmk32 = max((a.k_lmk + 31) >> 5, 1);
+  bool bad_page = false;
+
+  // ---- this warp's share of the unit: a stretch of window tiles, then one of landmark tiles
+  const int w0 = min(t_begin, p.n_window), w1 = min(t_end, p.n_window);
+  const int l0 = max(t_begin - p.n_window, 0), l1 = max(t_end - p.n_window, 0);
+  const int wq = (w1 - w0 + CA_WARPS - 1) / CA_WARPS, lq = (l1 - l0 + CA_WARPS - 1) / CA_WARPS;
+  int wb = min(w0 + warp * wq, w1), we = min(wb + wq, w1);
+  const int lb = min(l0 + warp * lq, l1), le = min(lb + lq, l1);
+  // (keys of the sequence's other row tiles are passed over)
+  wb = max(wb, min(we, (lo_min < p.len ? lo_min - p.lo32 : 0x7fffffe0) >> 5));
+  we = min(we, max(wb, (hi_max - p.lo32 + 31) >> 5));
+  const int n_w = we - wb, n = n_w + le - lb;
+
+  // where keys lie: of 16 window tiles ahead a lane per half, of the next landmark tile a lane per key
+  struct Where {
+    int key, page;  // -1 where none
+    float add;
+  };
+  const auto page_of = [&](int key) { return key >= 0 && key < p.len ? __ldg(table + (key >> a.page_shift)) : -1; };
+  // cache row of a key, or -1 (also for a page that does not exist)
+  const auto row_of = [&](const Where& o) -> int {
+    if (o.key < 0 || o.key >= p.len) return -1;
+    if ((unsigned)o.page >= (unsigned)a.n_pages) {
+      bad_page = true;
+      return -1;
+    }
+    return ((o.page * a.Hkv + hk) << a.page_shift) + (o.key & page_mask);
+  };
+  auto find_window = [&](int i) {  // lane: half lane & 1 of tile wb + i + lane / 2
+    Where o;
+    o.add = 0.f;
+    o.key = i + (lane >> 1) < n_w ? p.lo32 + (wb + i) * 32 + lane * 16 : -1;
+    o.page = page_of(o.key);
+    return o;
+  };
+  auto find_lmk = [&](int i) {  // lane: key `lane` of tile lb + i
+    Where o;
+    o.add = 0.f;
+    o.key = -1;
+    const int l = lb + i, c = (l % lmk32) * 32 + lane;
+    if (l < le && c < a.k_lmk) {
+      const int64_t at = ((int64_t)(hk * a.G + l / lmk32) * a.n_seqs + s) * a.k_lmk + c;
+      o.key = a.lmk[at];
+      if (a.bias) o.add = a.bias[at] * 1.4426950408889634f;
+    }
+    o.page = page_of(o.key);
+    return o;
+  };
+  Where ww = find_window(0), wn = ww, ln = ww;
+  if (n_w > 16) wn = find_window(16);
+  if (le > lb) ln = find_lmk(0);
   // ---- Q of row g: the 16 consecutive elements at 16 t of each 64
   uint32_t qb[NS][KS][2];
   float row_f[2];
@@ -369,72 +423,20 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
 #pragma unroll
   for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   RowState st[2] = {{-INFINITY, 0.f, -INFINITY}, {-INFINITY, 0.f, -INFINITY}};
-  const int page_mask = (1 << a.page_shift) - 1;
-  const int* table = a.tables + (int64_t)s * a.max_pages;
-  const int lmk32 = max((a.k_lmk + 31) >> 5, 1);
-  bool bad_page = false;
-
-  // ---- this warp's share of the unit: a stretch of window tiles, then one of landmark tiles
-  const int w0 = min(t_begin, p.n_window), w1 = min(t_end, p.n_window);
-  const int l0 = max(t_begin - p.n_window, 0), l1 = max(t_end - p.n_window, 0);
-  const int wq = (w1 - w0 + CA_WARPS - 1) / CA_WARPS, lq = (l1 - l0 + CA_WARPS - 1) / CA_WARPS;
-  int wb = min(w0 + warp * wq, w1), we = min(wb + wq, w1);
-  const int lb = min(l0 + warp * lq, l1), le = min(lb + lq, l1);
-  // (keys of the sequence's other row tiles are passed over)
-  wb = max(wb, min(we, (lo_min < p.len ? lo_min - p.lo32 : 0x7fffffe0) >> 5));
-  we = min(we, max(wb, (hi_max - p.lo32 + 31) >> 5));
-  const int n_w = we - wb, n = n_w + le - lb;
-
-  // where keys lie: of 16 window tiles ahead a lane per half, of the next landmark tile a lane per key
-  struct Where {
-    int row, key;
-    float ks, ve, add;
-  };
-  auto look_up = [&](int key, Where& o) {
-    o.row = -1;
-    o.ks = 0.f;
-    o.ve = 0.f;
-    if (key >= 0 && key < p.len) {
-      const int id = __ldg(table + (key >> a.page_shift));
-      if ((unsigned)id < (unsigned)a.n_pages) {
-        const int64_t head = (int64_t)id * a.Hkv + hk;
-        o.row = (int)(head << a.page_shift) + (key & page_mask);
-        o.ks = __ldg(a.ks + head);
-        o.ve = scale_log(__ldg(a.vs + head));
-      } else {
-        bad_page = true;
-      }
-    }
-  };
-  auto find_window = [&](int i) {  // lane: half lane & 1 of tile wb + i + lane / 2
-    Where o;
-    o.add = 0.f;
-    o.key = i + (lane >> 1) < n_w ? p.lo32 + (wb + i) * 32 + lane * 16 : -1;
-    look_up(o.key, o);
-    return o;
-  };
-  auto find_lmk = [&](int i) {  // lane: key `lane` of tile lb + i
-    Where o;
-    o.add = 0.f;
-    o.key = -1;
-    const int l = lb + i, c = (l % lmk32) * 32 + lane;
-    if (l < le && c < a.k_lmk) {
-      const int64_t at = ((int64_t)(hk * a.G + l / lmk32) * a.n_seqs + s) * a.k_lmk + c;
-      o.key = a.lmk[at];
-      if (a.bias) o.add = a.bias[at] * 1.4426950408889634f;
-    }
-    if (o.key >= p.len) o.key = -1;  // no row attends to it, and it may lie outside the table
-    look_up(o.key, o);
-    return o;
-  };
-  Where ww = find_window(0), wn = ww, ln = ww;
-  if (n_w > 16) wn = find_window(16);
-  if (le > lb) ln = find_lmk(0);
   uint8_t* ring = dyn + warp * (STAGES * Stage<D>::BYTES);
   const uint32_t ring_s = smem_u32(ring);
+  int ww_row = -1;                  // row of ww's key
   int in_stage = 0, out_stage = 0;  // byte offsets of the stages written and read next
   constexpr int CPR = D / 16, RPI = 32 / CPR;  // 16-byte chunks per row, rows per step of the warp
   const int my_row = lane / CPR, my_chunk = lane % CPR;
+  // scales come with the keys, by cp.async: nothing waits for them here
+  const auto put_meta = [&](uint32_t st_s, float4* meta, int slot, int row, const Where& o) {
+    const int head = max(row, 0) >> a.page_shift;
+    const uint32_t at = st_s + Stage<D>::META + slot * 16;
+    cp_async_4(at, a.ks + head, row >= 0 ? 4 : 0);
+    cp_async_4(at + 4, a.vs + head, row >= 0 ? 4 : 0);
+    *reinterpret_cast<float2*>(&meta[slot].z) = make_float2(o.add, __int_as_float(row >= 0 ? o.key : -1));
+  };
   auto issue = [&](int i) {
     if (i < n) {
       const uint32_t st_s = ring_s + in_stage;
@@ -445,12 +447,12 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
           ww = wn;
           if (i + 16 < n_w) wn = find_window(i + 16);
         }
-        if ((lane >> 1) == b)
-          meta[(lane & 1) * 16] = make_float4(ww.ks, ww.ve, 0.f, __int_as_float(ww.row >= 0 ? ww.key : -1));
+        if (b == 0) ww_row = row_of(ww);
+        if ((lane >> 1) == b) put_meta(st_s, meta, (lane & 1) * 16, ww_row, ww);
         const int key = __shfl_sync(0xffffffffu, ww.key, 2 * b);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int row = __shfl_sync(0xffffffffu, ww.row, 2 * b + h);
+          const int row = __shfl_sync(0xffffffffu, ww_row, 2 * b + h);
           const int left = row < 0 ? 0 : p.len - key - h * 16;  // rows from here that hold keys
           const int64_t at = (int64_t)max(row, 0) * D + lane * 16;
 #pragma unroll
@@ -463,10 +465,11 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
       } else {
         const Where lw = ln;
         if (i + 1 < n) ln = find_lmk(i + 1 - n_w);
-        meta[lane] = make_float4(lw.ks, lw.ve, lw.add, __int_as_float(lw.row >= 0 ? lw.key : -1));
+        const int mine = row_of(lw);
+        put_meta(st_s, meta, lane, mine, lw);
 #pragma unroll
         for (int x = 0; x < 32 / RPI; ++x) {
-          const int r = x * RPI + my_row, row = __shfl_sync(0xffffffffu, lw.row, r);
+          const int r = x * RPI + my_row, row = __shfl_sync(0xffffffffu, mine, r);
           const int64_t at = (int64_t)max(row, 0) * D + my_chunk * 16;
           copy16(st_s + Stage<D>::k_at(r, my_chunk), a.kc + at, row >= 0);
           copy16(st_s + Stage<D>::v_at(r, my_chunk), a.vc + at, row >= 0);
@@ -479,6 +482,33 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
   __syncthreads();  // the schedule's memory becomes the rings
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) issue(i);
+
+  // m and M are references, not exact maxima: they move when a lane's logit passes them by the
+  // slack, which after the first tiles is rare, and only then are maxima formed over the lanes
+  const auto raise = [&](const float (&lm)[2], const float (&lM)[2]) {
+    if (!__any_sync(0xffffffffu, lm[0] > st[0].m + CA_SLACK || lM[0] > st[0].M + CA_SLACK || lm[1] > st[1].m + CA_SLACK ||
+                                     lM[1] > st[1].M + CA_SLACK))
+      return;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float gm = lm[c], gM = lM[c];
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) {
+        gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, x));
+        gM = fmaxf(gM, __shfl_xor_sync(0xffffffffu, gM, x));
+      }
+      const float m = fmaxf(st[c].m, gm), M = fmaxf(st[c].M, gM);
+      st[c].l *= m == -INFINITY ? 1.f : exp2_fast(st[c].m - m);
+      const float corr = M == -INFINITY ? 1.f : exp2_fast(st[c].M - M);
+      st[c].m = m;
+      st[c].M = M;
+#pragma unroll
+      for (int x = 0; x < MT; ++x) {
+        o[x][c] *= corr;
+        o[x][2 + c] *= corr;
+      }
+    }
+  };
 
   for (int i = 0; i < n; ++i) {
     copies_wait<STAGES - 2>();
@@ -508,15 +538,16 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
     }
     // ---- P = 2^(x + e - M + 14), l += 2^(x - m)
     const int key0 = p.lo32 + (wb + i) * 32;
-    const float4 mh[2] = {meta[0], meta[16]};  // of a window tile's halves
+    float4 mh[2] = {meta[0], meta[16]};  // of a window tile's halves; .y: exponent of V's scale
+    mh[0].y = scale_log(mh[0].y);
+    mh[1].y = scale_log(mh[1].y);
     bool plain = window && key0 >= lo_max && key0 + 32 <= hi_min && __float_as_int(mh[0].w) >= 0 &&
                  __float_as_int(mh[1].w) >= 0;
+    const bool valid_all = plain;
     uint32_t valid = 0xff;  // bit 4 h + e: element e of half h counts
     if (plain) {
-      // m and M are references here, not exact maxima: they move when a logit passes them by
-      // the slack. One exponential per element: the sum of P is brought to l's reference.
-      float f[2][2], lm[2][2];
-      bool over = false;
+      // one exponential per element: the sum of P is brought to l's reference
+      float f[2][2], lm[2][2], top[2], top_e[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
@@ -524,30 +555,10 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
           f[c][h] = mh[h].x * row_f[c];
           lm[c][h] = f[c][h] * fmaxf(sc[h][c], sc[h][2 + c]);
         }
-        over |= fmaxf(lm[c][0], lm[c][1]) > st[c].m + CA_SLACK ||
-                fmaxf(lm[c][0] + mh[0].y, lm[c][1] + mh[1].y) > st[c].M + CA_SLACK;
+        top[c] = fmaxf(lm[c][0], lm[c][1]);
+        top_e[c] = fmaxf(lm[c][0] + mh[0].y, lm[c][1] + mh[1].y);
       }
-      if (__any_sync(0xffffffffu, over)) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float gm = fmaxf(lm[c][0], lm[c][1]), gM = fmaxf(lm[c][0] + mh[0].y, lm[c][1] + mh[1].y);
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) {
-            gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, x));
-            gM = fmaxf(gM, __shfl_xor_sync(0xffffffffu, gM, x));
-          }
-          const float m = fmaxf(st[c].m, gm), M = fmaxf(st[c].M, gM);
-          st[c].l *= m == -INFINITY ? 1.f : exp2_fast(st[c].m - m);
-          const float corr = M == -INFINITY ? 1.f : exp2_fast(st[c].M - M);
-          st[c].m = m;
-          st[c].M = M;
-#pragma unroll
-          for (int x = 0; x < MT; ++x) {
-            o[x][c] *= corr;
-            o[x][2 + c] *= corr;
-          }
-        }
-      }
+      raise(top, top_e);
       // where V's scale is so small that P of a logit near m would vanish, l needs its own
       // exponentials: the general path
       const float e_min = fminf(mh[0].y, mh[1].y);
@@ -571,8 +582,7 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
     }
     if (!plain) {
       float ve[2][2];
-      if (valid == 0xff && window && key0 >= lo_max && key0 + 32 <= hi_min && __float_as_int(mh[0].w) >= 0 &&
-          __float_as_int(mh[1].w) >= 0) {  // came from above, logits formed
+      if (valid_all) {  // came from above, logits formed
         ve[0][0] = ve[0][1] = mh[0].y;
         ve[1][0] = ve[1][1] = mh[1].y;
       } else {
@@ -583,7 +593,11 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
             const int slot = b * 8 + slot_of(g);  // within the half
-            const float4 mt = window ? mh[h] : meta[h * 16 + slot];
+            float4 mt = mh[h];
+            if (!window) {
+              mt = meta[h * 16 + slot];
+              mt.y = scale_log(mt.y);
+            }
             int key = __float_as_int(mt.w);
             if (window && key >= 0) {
               key += slot;
@@ -599,39 +613,24 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
             }
           }
       }
+      float lm[2], lM[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float gm = -INFINITY, gM = -INFINITY;
+        lm[c] = fmaxf(fmaxf(sc[0][c], sc[0][2 + c]), fmaxf(sc[1][c], sc[1][2 + c]));
+        lM[c] = fmaxf(fmaxf(sc[0][c] + ve[0][0], sc[0][2 + c] + ve[0][1]), fmaxf(sc[1][c] + ve[1][0], sc[1][2 + c] + ve[1][1]));
+      }
+      raise(lm, lM);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            gm = fmaxf(gm, sc[h][2 * b + c]);
-            gM = fmaxf(gM, sc[h][2 * b + c] + ve[h][b]);
-          }
-#pragma unroll
-        for (int x = 4; x < 32; x <<= 1) {
-          gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, x));
-          gM = fmaxf(gM, __shfl_xor_sync(0xffffffffu, gM, x));
-        }
-        const float m = fmaxf(st[c].m, gm), M = fmaxf(st[c].M, gM);
-        const float mu = m == -INFINITY ? 0.f : m, Mu = M == -INFINITY ? 0.f : M;
-        float l = st[c].l * exp2_fast(st[c].m - mu);
-        const float corr = exp2_fast(st[c].M - Mu);
+      for (int c = 0; c < 2; ++c) {
+        const float mu = st[c].m == -INFINITY ? 0.f : st[c].m, Mu = st[c].M == -INFINITY ? 0.f : st[c].M;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
             const float x = sc[h][2 * b + c];
-            l += exp2_fast(x - mu);
+            st[c].l += exp2_fast(x - mu);
             sc[h][2 * b + c] = exp2_fast(x + ve[h][b] - Mu + CA_P_SHIFT);
           }
-        st[c] = {m, l, M};
-#pragma unroll
-        for (int x = 0; x < MT; ++x) {
-          o[x][c] *= corr;
-          o[x][2 + c] *= corr;
-        }
       }
     }
     // ---- O^T += V^T P^T, 16 keys at a time
@@ -850,7 +849,7 @@ static inline int64_t ca_items(int64_t T, int n_seqs, int G, int Hkv) { return (
 
 template <typename T, int D, int NS>
 static int launch_cache_attn(const CacheAttnArgs& a, unsigned grid, bool join, cudaStream_t stream) {
-  constexpr size_t RING = (size_t)CA_WARPS * Shape<D>::STAGES * Stage<D>::BYTES, TABLES = 3 * sizeof(int);
+  constexpr size_t RING = (size_t)CA_WARPS * Shape<D>::STAGES * Stage<D>::BYTES, TABLES = 2 * sizeof(int);
   static_assert(RING >= sizeof(float) * CA_WARPS * CA_ROWS * D, "the parts take the rings' place");
   const size_t smem = TABLES * (size_t)a.n_seqs > RING ? TABLES * (size_t)a.n_seqs : RING;
   static std::atomic<uint64_t> ready{0};

@@ -10,25 +10,23 @@
 // A granted row's first page number is upto - need, whatever becomes of the rows behind it,
 // so no row waits for another: two running sums (need, new) over the rows and then one
 // independent computation per token.
-#include <cooperative_groups.h>
-
 #include <atomic>
 
 #include "common.cuh"
 
 namespace dsalt {
 
-namespace cg = cooperative_groups;
-
-constexpr int SLOT_THREADS = 1024;
 constexpr int SLOT_MAX_SEQS = 8192;  // three int32 per row in shared memory
+constexpr int SLOT_FILL_MAX = 1024;  // tokens that the rows' block numbers itself
 
 struct Pair64 {
   long long a, b;
 };
 
-// inclusive sums of a pair over the block's threads
-__device__ __forceinline__ Pair64 block_scan(Pair64 v, Pair64* warp_sums) {
+// inclusive sums of a pair over the block's threads, and the block's total
+template <int THREADS>
+__device__ __forceinline__ Pair64 block_scan(Pair64 v, Pair64* warp_sums, Pair64& all) {
+  constexpr int WARPS = THREADS / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -38,50 +36,50 @@ __device__ __forceinline__ Pair64 block_scan(Pair64 v, Pair64* warp_sums) {
       v.b += b;
     }
   }
+  __syncthreads();  // the sums of the call before have been read
   if (lane == 31) warp_sums[warp] = v;
   __syncthreads();
-  if (warp == 0) {
-    Pair64 s = warp_sums[lane];
+  Pair64 s = lane < WARPS ? warp_sums[lane] : Pair64{0, 0}, before{0, 0};
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long a = __shfl_up_sync(0xffffffffu, s.a, o), b = __shfl_up_sync(0xffffffffu, s.b, o);
-      if (lane >= o) {
-        s.a += a;
-        s.b += b;
-      }
+  for (int o = 1; o < WARPS; o <<= 1) {
+    const long long a = __shfl_up_sync(0xffffffffu, s.a, o), b = __shfl_up_sync(0xffffffffu, s.b, o);
+    if (lane >= o) {
+      s.a += a;
+      s.b += b;
     }
-    warp_sums[lane] = s;
   }
-  __syncthreads();
+  all.a = __shfl_sync(0xffffffffu, s.a, WARPS - 1);
+  all.b = __shfl_sync(0xffffffffu, s.b, WARPS - 1);
+  before.a = __shfl_sync(0xffffffffu, s.a, warp > 0 ? warp - 1 : 0);
+  before.b = __shfl_sync(0xffffffffu, s.b, warp > 0 ? warp - 1 : 0);
   if (warp > 0) {
-    v.a += warp_sums[warp - 1].a;
-    v.b += warp_sums[warp - 1].b;
+    v.a += before.a;
+    v.b += before.b;
   }
   return v;
 }
 
-// One cluster. Every CTA forms the running sums of all rows for itself (they are a few
-// loads and two shuffles deep; exchanging them would cost as much) and then fills its share
-// of the tokens and table rows. The lengths and the free count may be updated in place:
-// they are written behind a cluster barrier, after the last CTA has read them.
-__global__ void __launch_bounds__(SLOT_THREADS) reserve_slots_kernel(
+// The rows: one block, which also numbers the tokens where they are few (FILL). Lengths and
+// free count may be updated in place: each thread has read its rows, and everybody the free
+// count, before the barriers that come before the writes.
+template <int THREADS, bool FILL>
+__global__ void __launch_bounds__(THREADS) reserve_slots_kernel(
     int32_t* __restrict__ tables, int n_seqs, int max_pages, const int32_t* seq_lens, const int32_t* new_lens,
-    const int32_t* __restrict__ free_pages, int free_cap, const int32_t* n_free_in, int page, int64_t n_tokens,
+    const int32_t* __restrict__ free_pages, int free_cap, const int32_t* n_free_in, int page_shift, int64_t n_tokens,
     int64_t* __restrict__ slots, int32_t* __restrict__ positions, int32_t* __restrict__ cu_new, uint8_t* granted,
     int32_t* seq_lens_out, int32_t* n_free_out) {
   extern __shared__ int32_t sm[];
-  int32_t* s_cu = sm;                // [n_seqs + 1] first token of each row, at most n_tokens
+  int32_t* s_cu = sm;                  // [n_seqs + 1] first token of each row, at most n_tokens
   int32_t* s_old = s_cu + n_seqs + 1;  // [n_seqs] length before, -1 - length where the row is refused
   int32_t* s_first = s_old + n_seqs;   // [n_seqs] number of its first new page in the running order
-  __shared__ Pair64 warp_sums[32];
-  cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank(), n_ranks = (int)cluster.num_blocks();
-  const int tid = threadIdx.x;
+  __shared__ Pair64 warp_sums[THREADS / 32];
+  __shared__ int s_taken;
+  const int tid = threadIdx.x, page_mask = (1 << page_shift) - 1;
   int n_free = *n_free_in;
   n_free = n_free < 0 ? 0 : (n_free > free_cap ? free_cap : n_free);
+  if (tid == 0) s_taken = 0;
   Pair64 carry{0, 0};
-  long long taken = 0;  // pages of granted rows, this thread's rows
-  for (int base = 0; base < n_seqs; base += SLOT_THREADS) {
+  for (int base = 0; base < n_seqs; base += THREADS) {
     const int s = base + tid;
     long long old = 0, add = 0;
     if (s < n_seqs) {
@@ -89,118 +87,141 @@ __global__ void __launch_bounds__(SLOT_THREADS) reserve_slots_kernel(
       add = max(new_lens[s], 0);
     }
     // the token budget is judged on the running sum of the new tokens: that sum comes first
-    const long long end = carry.b + block_scan(Pair64{0, add}, warp_sums).b;
-    carry.b += warp_sums[31].b;
-    __syncthreads();
-    const long long have = (old + page - 1) / page, want = (old + add + page - 1) / page;
+    Pair64 all;
+    const long long end = carry.b + block_scan<THREADS>(Pair64{0, add}, warp_sums, all).b;
+    carry.b += all.b;
+    const long long have = (old + page_mask) >> page_shift, want = (old + add + page_mask) >> page_shift;
     const bool fits = want <= max_pages && end <= n_tokens && old + add <= 0x7fffffffLL;
     const long long need = s < n_seqs && fits ? want - have : 0;
-    const long long upto = carry.a + block_scan(Pair64{need, 0}, warp_sums).a;
-    carry.a += warp_sums[31].a;
-    __syncthreads();
+    const long long upto = carry.a + block_scan<THREADS>(Pair64{need, 0}, warp_sums, all).a;
+    carry.a += all.a;
     const bool ok = fits && (need == 0 || upto <= n_free);
     if (s < n_seqs) {
       s_cu[s + 1] = (int32_t)min(end, (long long)n_tokens);
       s_old[s] = ok ? (int32_t)old : (int32_t)(-1 - old);
       s_first[s] = ok ? (int32_t)(upto - need) : 0;
-      if (ok) taken += need;
+      // granted rows that need pages are the first that do: the last one's sum is what is taken
+      if (ok && need > 0) atomicMax(&s_taken, (int)upto);
     }
   }
   if (tid == 0) s_cu[0] = 0;
-  block_scan(Pair64{taken, 0}, warp_sums);  // its barriers also publish s_cu, s_old, s_first
-  const long long all_taken = warp_sums[31].a;
+  __syncthreads();
   // new table entries, a warp per row
   const int warp = tid >> 5, lane = tid & 31;
-  for (int s = rank * (SLOT_THREADS / 32) + warp; s < n_seqs; s += n_ranks * (SLOT_THREADS / 32)) {
+  for (int s = warp; s < n_seqs; s += THREADS / 32) {
     const int old = s_old[s];
     if (old < 0) continue;
-    const int add = s_cu[s + 1] - s_cu[s];
-    const int have = (old + page - 1) / page, want = (int)(((long long)old + add + page - 1) / page);
-    const int first = s_first[s];
+    const int add = s_cu[s + 1] - s_cu[s], first = s_first[s];
+    const int have = (int)(((long long)old + page_mask) >> page_shift), want = (int)(((long long)old + add + page_mask) >> page_shift);
     for (int c = have + lane; c < want; c += 32)
       tables[(int64_t)s * max_pages + c] = free_pages[n_free - 1 - (first + c - have)];
   }
-  // slots and positions: four consecutive tokens per thread, one search for the first's row
-  const int64_t quads = (n_tokens + 3) / 4;
-  for (int64_t qd = (int64_t)rank * SLOT_THREADS + tid; qd < quads; qd += (int64_t)n_ranks * SLOT_THREADS) {
-    const int64_t t0 = qd * 4;
-    int lo = 0, hi = n_seqs;  // first row whose end lies behind t0
+  for (int s = tid; s < n_seqs; s += THREADS) {
+    const int old = s_old[s];
+    const bool ok = old >= 0;
+    granted[s] = ok ? 1 : 0;
+    // a granted row's tokens all lie within the budget: its share of s_cu is its new length
+    seq_lens_out[s] = ok ? old + (s_cu[s + 1] - s_cu[s]) : -1 - old;
+  }
+  for (int s = tid; s <= n_seqs; s += THREADS) cu_new[s] = s_cu[s];
+  if (tid == 0) *n_free_out = n_free - s_taken;
+  if (!FILL) return;
+  for (int64_t t = tid; t < n_tokens; t += THREADS) {
+    int lo = 0, hi = n_seqs;  // first row whose end lies behind t
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (s_cu[mid + 1] > t0) hi = mid;
+      if (s_cu[mid + 1] > t) hi = mid;
       else lo = mid + 1;
     }
-    int s = lo;
-    int64_t sl[4];
-    int32_t ps[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t t = t0 + e;
-      while (s < n_seqs && s_cu[s + 1] <= t) ++s;
-      sl[e] = -1;
-      ps[e] = 0;
-      if (s < n_seqs && s_old[s] >= 0) {
-        const int old = s_old[s];
-        const int pos = old + (int)(t - s_cu[s]);
-        const int col = pos / page, have = (old + page - 1) / page;
-        const int id = col < have ? tables[(int64_t)s * max_pages + col]
-                                  : free_pages[n_free - 1 - (s_first[s] + col - have)];
-        ps[e] = pos;
-        if (id >= 0) sl[e] = (int64_t)id * page + pos % page;
-      }
+    int64_t slot = -1;
+    int pos = 0;
+    if (lo < n_seqs && s_old[lo] >= 0) {
+      const int old = s_old[lo], have = (int)(((long long)old + page_mask) >> page_shift);
+      pos = old + (int)(t - s_cu[lo]);
+      const int col = pos >> page_shift;
+      // entries just written are read from where they came
+      const int id = col < have ? tables[(int64_t)lo * max_pages + col]
+                                : free_pages[n_free - 1 - (s_first[lo] + col - have)];
+      if (id >= 0) slot = ((int64_t)id << page_shift) + (pos & page_mask);
     }
-    if (t0 + 4 <= n_tokens) {
-      reinterpret_cast<longlong2*>(slots + t0)[0] = make_longlong2(sl[0], sl[1]);
-      reinterpret_cast<longlong2*>(slots + t0)[1] = make_longlong2(sl[2], sl[3]);
-      *reinterpret_cast<int4*>(positions + t0) = make_int4(ps[0], ps[1], ps[2], ps[3]);
-    } else {
-      for (int e = 0; e < 4 && t0 + e < n_tokens; ++e) {
-        slots[t0 + e] = sl[e];
-        positions[t0 + e] = ps[e];
-      }
+    slots[t] = slot;
+    positions[t] = pos;
+  }
+}
+
+// The tokens, where they are many: four consecutive ones per thread, one search for the first's
+// row, from what the rows' kernel has written.
+__global__ void __launch_bounds__(256) fill_slots_kernel(const int32_t* __restrict__ tables, int n_seqs, int max_pages,
+                                                         const int32_t* __restrict__ seq_lens,
+                                                         const int32_t* __restrict__ cu, const uint8_t* __restrict__ granted,
+                                                         int page_shift, int64_t n_tokens, int64_t* __restrict__ slots,
+                                                         int32_t* __restrict__ positions) {
+  cudaGridDependencySynchronize();
+  const int64_t t0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (t0 >= n_tokens) return;
+  int lo = 0, hi = n_seqs;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid + 1] > t0) hi = mid;
+    else lo = mid + 1;
+  }
+  int s = lo;
+  int64_t sl[4];
+  int32_t ps[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int64_t t = t0 + e;
+    while (s < n_seqs && cu[s + 1] <= t) ++s;
+    sl[e] = -1;
+    ps[e] = 0;
+    if (s < n_seqs && granted[s]) {
+      const int pos = seq_lens[s] - (int)(cu[s + 1] - t);
+      const int id = tables[(int64_t)s * max_pages + (pos >> page_shift)];
+      ps[e] = pos;
+      if (id >= 0) sl[e] = ((int64_t)id << page_shift) + (pos & ((1 << page_shift) - 1));
     }
   }
-  if (n_ranks > 1) cluster.sync();  // every CTA has read the lengths and the free count
-  else __syncthreads();
-  if (rank == 0) {
-    for (int s = tid; s < n_seqs; s += SLOT_THREADS) {
-      const int old = s_old[s];
-      const bool ok = old >= 0;
-      granted[s] = ok ? 1 : 0;
-      // a granted row's tokens all lie within the budget: its share of s_cu is its new length
-      seq_lens_out[s] = ok ? old + (s_cu[s + 1] - s_cu[s]) : -1 - old;
+  if (t0 + 4 <= n_tokens) {
+    reinterpret_cast<longlong2*>(slots + t0)[0] = make_longlong2(sl[0], sl[1]);
+    reinterpret_cast<longlong2*>(slots + t0)[1] = make_longlong2(sl[2], sl[3]);
+    *reinterpret_cast<int4*>(positions + t0) = make_int4(ps[0], ps[1], ps[2], ps[3]);
+  } else {
+    for (int e = 0; e < 4 && t0 + e < n_tokens; ++e) {
+      slots[t0 + e] = sl[e];
+      positions[t0 + e] = ps[e];
     }
-    for (int s = tid; s <= n_seqs; s += SLOT_THREADS) cu_new[s] = s_cu[s];
-    if (tid == 0) *n_free_out = n_free - (int)all_taken;
   }
 }
 
 // The pages of the flagged rows go back on the stack, in the order in which reserve_slots
 // would take them again (page number j of the rows in order to free[n_free + total - 1 - j]);
 // their table entries become -1 and their lengths 0.
-__global__ void __launch_bounds__(SLOT_THREADS) release_slots_kernel(int32_t* __restrict__ tables, int n_seqs,
-                                                                     int max_pages, int32_t* __restrict__ seq_lens,
-                                                                     const uint8_t* __restrict__ release,
-                                                                     int32_t* __restrict__ free_pages, int free_cap,
-                                                                     int32_t* __restrict__ n_free_io, int page) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) release_slots_kernel(int32_t* __restrict__ tables, int n_seqs, int max_pages,
+                                                                int32_t* __restrict__ seq_lens,
+                                                                const uint8_t* __restrict__ release,
+                                                                int32_t* __restrict__ free_pages, int free_cap,
+                                                                int32_t* __restrict__ n_free_io, int page_shift) {
   extern __shared__ int32_t s_upto[];  // [n_seqs] pages of the flagged rows up to and with s
-  __shared__ Pair64 warp_sums[32];
-  const int tid = threadIdx.x;
+  __shared__ Pair64 warp_sums[THREADS / 32];
+  const int tid = threadIdx.x, page_mask = (1 << page_shift) - 1;
   int n_free = *n_free_io;
   n_free = n_free < 0 ? 0 : (n_free > free_cap ? free_cap : n_free);
   long long carry = 0;
-  for (int base = 0; base < n_seqs; base += SLOT_THREADS) {
+  for (int base = 0; base < n_seqs; base += THREADS) {
     const int s = base + tid;
     long long held = 0;
-    if (s < n_seqs && release[s]) held = min(((long long)max(seq_lens[s], 0) + page - 1) / page, (long long)max_pages);
-    const Pair64 p = block_scan(Pair64{held, 0}, warp_sums);
+    if (s < n_seqs && release[s]) held = min(((long long)max(seq_lens[s], 0) + page_mask) >> page_shift, (long long)max_pages);
+    Pair64 all;
+    const Pair64 p = block_scan<THREADS>(Pair64{held, 0}, warp_sums, all);
     if (s < n_seqs) s_upto[s] = (int32_t)(carry + p.a);
-    carry += warp_sums[31].a;
-    __syncthreads();
+    carry += all.a;
   }
+  __syncthreads();
   const int total = (int)carry;
-  // every flagged page: number j, its row by search
-  for (int j = tid; j < total; j += SLOT_THREADS) {
+  // every flagged page: number j, its row by search; four under way at a time
+#pragma unroll 4
+  for (int j = tid; j < total; j += THREADS) {
     int lo = 0, hi = n_seqs - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
@@ -213,12 +234,13 @@ __global__ void __launch_bounds__(SLOT_THREADS) release_slots_kernel(int32_t* __
     if (to < free_cap) free_pages[to] = *e;
     *e = -1;
   }
-  for (int s = tid; s < n_seqs; s += SLOT_THREADS)
+  for (int s = tid; s < n_seqs; s += THREADS)
     if (release[s]) seq_lens[s] = 0;
   if (tid == 0) *n_free_io = (int)min((long long)n_free + total, (long long)free_cap);
 }
 
 static bool page_ok(int page) { return page == 16 || page == 32 || page == 64 || page == 128; }
+static int shift_of(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
 
 }  // namespace dsalt
 
@@ -242,26 +264,40 @@ int dsalt_reserve_slots(int32_t* block_tables, int n_seqs, int max_pages, const 
   if (((uintptr_t)slots | (uintptr_t)positions) & 15)
     return fail(DSALT_ERR_INVALID, "reserve_slots: slots and positions must be 16-byte aligned");
   const size_t smem = sizeof(int32_t) * (3 * (size_t)n_seqs + 1);
-  static std::atomic<uint64_t> ready{0};
-  if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(reserve_slots_kernel),
-                                  (int)(sizeof(int32_t) * (3 * (size_t)SLOT_MAX_SEQS + 1)), ready))
-    return rc;
+  const int most = (int)(sizeof(int32_t) * (3 * (size_t)SLOT_MAX_SEQS + 1));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int shift = shift_of(page_size);
+  // one block of 256 threads is quicker round its barriers than one of 1024; with more rows than
+  // it takes at once the larger one is
+  const bool fill = n_tokens <= SLOT_FILL_MAX, wide = n_seqs > 256 || n_tokens > 512;
+  static std::atomic<uint64_t> ready[3];
+#define DSALT_RESERVE(N, F, R)                                                                                       \
+  do {                                                                                                               \
+    if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(reserve_slots_kernel<N, F>), most, ready[R]))      \
+      return rc;                                                                                                     \
+    reserve_slots_kernel<N, F><<<1, N, smem, st>>>(block_tables, n_seqs, max_pages, seq_lens, new_lens, free_pages,  \
+                                                   (int)free_capacity, n_free, shift, n_tokens, slots, positions,    \
+                                                   cu_new, granted, seq_lens_out, n_free_out);                       \
+  } while (0)
+  if (!fill) DSALT_RESERVE(1024, false, 0);
+  else if (wide) DSALT_RESERVE(1024, true, 1);
+  else DSALT_RESERVE(256, true, 2);
+#undef DSALT_RESERVE
+  if (int rc = check_cuda(cudaGetLastError(), "reserve_slots launch")) return rc;
+  if (fill) return DSALT_OK;
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  const unsigned ctas = n_tokens > 4 * SLOT_THREADS ? 8 : 1;  // one CTA covers a decode step's tokens in one go
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(SLOT_THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+  cfg.gridDim = dim3((unsigned)((n_tokens + 1023) / 1024));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, reserve_slots_kernel, block_tables, n_seqs, max_pages, seq_lens, new_lens,
-                                       free_pages, (int)free_capacity, n_free, page_size, n_tokens, slots, positions,
-                                       cu_new, granted, seq_lens_out, n_free_out),
-                    "reserve_slots launch");
+  return check_cuda(cudaLaunchKernelEx(&cfg, fill_slots_kernel, (const int32_t*)block_tables, n_seqs, max_pages,
+                                       (const int32_t*)seq_lens_out, (const int32_t*)cu_new, (const uint8_t*)granted, shift,
+                                       n_tokens, slots, positions),
+                    "reserve_slots fill launch");
 }
 
 int dsalt_release_slots(int32_t* block_tables, int n_seqs, int max_pages, int32_t* seq_lens, const uint8_t* release,
@@ -272,8 +308,9 @@ int dsalt_release_slots(int32_t* block_tables, int n_seqs, int max_pages, int32_
   if (free_capacity > 0x7fffff00LL) return fail(DSALT_ERR_UNSUPPORTED, "release_slots: pool too large");
   if (!block_tables || !seq_lens || !release || (free_capacity > 0 && !free_pages) || !n_free)
     return fail(DSALT_ERR_INVALID, "release_slots: null pointer");
-  release_slots_kernel<<<1, SLOT_THREADS, sizeof(int32_t) * (size_t)n_seqs, reinterpret_cast<cudaStream_t>(stream)>>>(
-      block_tables, n_seqs, max_pages, seq_lens, release, free_pages, (int)free_capacity, n_free, page_size);
+  const size_t smem = sizeof(int32_t) * (size_t)n_seqs;  // at most 32 KB
+  release_slots_kernel<1024><<<1, 1024, smem, reinterpret_cast<cudaStream_t>(stream)>>>(
+      block_tables, n_seqs, max_pages, seq_lens, release, free_pages, (int)free_capacity, n_free, shift_of(page_size));
   return check_cuda(cudaGetLastError(), "release_slots launch");
 }
 
