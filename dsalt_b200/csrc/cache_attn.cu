@@ -84,6 +84,9 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // cp.async of 16 bytes, zeros when !ok
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(__cvta_generic_to_global(src)) : "memory");
+}
 __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, bool ok) { cp_async_16(dst, src, ok ? 16 : 0); }
 template <int N>
 __device__ __forceinline__ void copies_wait() {
@@ -429,6 +432,11 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
   int in_stage = 0, out_stage = 0;  // byte offsets of the stages written and read next
   constexpr int CPR = D / 16, RPI = 32 / CPR;  // 16-byte chunks per row, rows per step of the warp
   const int my_row = lane / CPR, my_chunk = lane % CPR;
+  // places of this lane's chunks and fragments in a stage; whole steps and halves are added (the
+  // swizzle looks at the lowest bits of the row alone, save one bit that K's odd steps flip)
+  const int k_put = Stage<D>::k_at(my_row, my_chunk), v_put = Stage<D>::v_at(my_row, my_chunk);
+  const auto k_step = [&](int x) { return D == 64 ? k_put + x * RPI * D : (k_put ^ (x & 1) * 64) + x * RPI * D; };
+  const int k_get = Stage<D>::k_at(slot_of(g), t), v_get = D == 64 ? Stage<D>::v_at(t, g >> 1) + (g & 1) * 8 : Stage<D>::v_at(t, g);
   // scales come with the keys, by cp.async: nothing waits for them here
   const auto put_meta = [&](uint32_t st_s, float4* meta, int slot, int row, const Where& o) {
     const int head = max(row, 0) >> a.page_shift;
@@ -455,11 +463,19 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
           const int row = __shfl_sync(0xffffffffu, ww_row, 2 * b + h);
           const int left = row < 0 ? 0 : p.len - key - h * 16;  // rows from here that hold keys
           const int64_t at = (int64_t)max(row, 0) * D + lane * 16;
+          const uint8_t *ksrc = a.kc + at, *vsrc = a.vc + at;
+          if (left >= 16) {
 #pragma unroll
-          for (int x = 0; x < 16 / RPI; ++x) {
-            const int r = x * RPI + my_row;
-            copy16(st_s + Stage<D>::k_at(h * 16 + r, my_chunk), a.kc + at + x * 512, r < left);
-            copy16(st_s + Stage<D>::v_at(h * 16 + r, my_chunk), a.vc + at + x * 512, r < left);
+            for (int x = 0; x < 16 / RPI; ++x) {
+              copy16(st_s + k_step(x) + h * 16 * D, ksrc + x * 512);
+              copy16(st_s + v_put + (h * 16 + x * RPI) * D, vsrc + x * 512);
+            }
+          } else {
+#pragma unroll
+            for (int x = 0; x < 16 / RPI; ++x) {
+              copy16(st_s + k_step(x) + h * 16 * D, ksrc + x * 512, x * RPI + my_row < left);
+              copy16(st_s + v_put + (h * 16 + x * RPI) * D, vsrc + x * 512, x * RPI + my_row < left);
+            }
           }
         }
       } else {
@@ -471,8 +487,8 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
         for (int x = 0; x < 32 / RPI; ++x) {
           const int r = x * RPI + my_row, row = __shfl_sync(0xffffffffu, mine, r);
           const int64_t at = (int64_t)max(row, 0) * D + my_chunk * 16;
-          copy16(st_s + Stage<D>::k_at(r, my_chunk), a.kc + at, row >= 0);
-          copy16(st_s + Stage<D>::v_at(r, my_chunk), a.vc + at, row >= 0);
+          copy16(st_s + k_step(x), a.kc + at, row >= 0);
+          copy16(st_s + v_put + x * RPI * D, a.vc + at, row >= 0);
         }
       }
       in_stage = in_stage == (STAGES - 1) * Stage<D>::BYTES ? 0 : in_stage + Stage<D>::BYTES;
@@ -525,8 +541,8 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
       sc[h][0] = sc[h][1] = sc[h][2] = sc[h][3] = 0.f;
 #pragma unroll
       for (int b = 0; b < D / 64; ++b) {
-        const uint4 ka = *reinterpret_cast<const uint4*>(stage + Stage<D>::k_at(h * 16 + slot_of(g), b * 4 + t));
-        const uint4 kb = *reinterpret_cast<const uint4*>(stage + Stage<D>::k_at(h * 16 + 8 + slot_of(g), b * 4 + t));
+        const uint4 ka = *reinterpret_cast<const uint4*>(stage + (k_get ^ b * 64) + h * 16 * D);
+        const uint4 kb = *reinterpret_cast<const uint4*>(stage + (k_get ^ b * 64) + (h * 16 + 8) * D);
         const uint32_t k0[4] = {ka.x, ka.y, ka.z, ka.w}, k1[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -650,12 +666,12 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
       uint32_t v[4][D / 32];  // keys t, t + 4, t + 8, t + 12
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const int r = h * 16 + t + 4 * x;
+        const uint8_t* at = stage + v_get + (h * 16 + 4 * x) * D;
         if constexpr (D == 64) {
-          const uint2 y = *reinterpret_cast<const uint2*>(stage + Stage<D>::v_at(r, g >> 1) + (g & 1) * 8);
+          const uint2 y = *reinterpret_cast<const uint2*>(at);
           v[x][0] = y.x, v[x][1] = y.y;
         } else {
-          const uint4 y = *reinterpret_cast<const uint4*>(stage + Stage<D>::v_at(r, g));
+          const uint4 y = *reinterpret_cast<const uint4*>(at);
           v[x][0] = y.x, v[x][1] = y.y, v[x][2] = y.z, v[x][3] = y.w;
         }
       }
