@@ -29,6 +29,7 @@
 // call follows them); the parts of an item that was cut are joined by a second kernel.
 // Within a unit each of two warps has its own stretch of tiles and its own ring of
 // cp.async stages: nothing but the end is shared, so no warp waits for another.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.cuh"
@@ -286,6 +287,7 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
 
   // ---- rows 2t, 2t+1 of the tile are this lane's in S^T and O^T
   int row_lo[2], row_hi[2], row_head[2];
+  unsigned row_span[2], row_before[2];  // keys of the window; positions before it, where landmarks count
   bool row_ok[2];
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
@@ -296,6 +298,8 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
     row_lo[c] = keys ? first_key(a, p.q0 + tok, pos) : 0x7fffffff;
     row_hi[c] = keys ? pos + 1 : 0;
     row_head[c] = i % a.G;
+    row_span[c] = keys ? row_hi[c] - row_lo[c] : 0;
+    row_before[c] = keys ? row_lo[c] : 0;
   }
   // keys that every row of the tile attends to need no mask
   int lo_min = min(row_lo[0], row_lo[1]), hi_max = max(row_hi[0], row_hi[1]);
@@ -553,89 +557,89 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
       }
     }
     // ---- P = 2^(x + e - M + 14), l += 2^(x - m)
-    const int key0 = p.lo32 + (wb + i) * 32;
+    const int key0 = p.lo32 + (wb + i) * 32, slot = slot_of(g);
     float4 mh[2] = {meta[0], meta[16]};  // of a window tile's halves; .y: exponent of V's scale
-    mh[0].y = scale_log(mh[0].y);
-    mh[1].y = scale_log(mh[1].y);
-    bool plain = window && key0 >= lo_max && key0 + 32 <= hi_min && __float_as_int(mh[0].w) >= 0 &&
-                 __float_as_int(mh[1].w) >= 0;
-    const bool valid_all = plain;
-    uint32_t valid = 0xff;  // bit 4 h + e: element e of half h counts
-    if (plain) {
+    const bool whole = window && key0 >= lo_max && key0 + 32 <= hi_min && __float_as_int(mh[0].w) >= 0 &&
+                       __float_as_int(mh[1].w) >= 0;  // every row attends to every key
+    const int head = window ? 0 : (lb + i - n_w) / lmk32;
+    // does row c attend to this lane's key b of half h?
+    const auto attends = [&](int h, int b, int c) -> bool {
+      if (window)
+        return (unsigned)(key0 + h * 16 + b * 8 + slot - row_lo[c]) < (__float_as_int(mh[h].w) >= 0 ? row_span[c] : 0u);
+      return __float_as_uint(meta[h * 16 + b * 8 + slot].w) < (head == row_head[c] ? row_before[c] : 0u);
+    };
+    float ve[2][2];
+    bool formed = !window;  // sc holds logits
+    if (window) {
+      mh[0].y = scale_log(mh[0].y);
+      mh[1].y = scale_log(mh[1].y);
+      if (!whole) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+              if (!attends(h, b, c)) sc[h][2 * b + c] = -INFINITY;
+      }
       // one exponential per element: the sum of P is brought to l's reference
-      float f[2][2], lm[2][2], top[2], top_e[2];
+      float f[2][2], lm[2][2], top[2], top_e[2], mu[2], Mu[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          f[c][h] = mh[h].x * row_f[c];
+          f[c][h] = fmaxf(mh[h].x * row_f[c], 1.17549435e-38f);  // above 0, so that -inf stays what it is
           lm[c][h] = f[c][h] * fmaxf(sc[h][c], sc[h][2 + c]);
         }
         top[c] = fmaxf(lm[c][0], lm[c][1]);
         top_e[c] = fmaxf(lm[c][0] + mh[0].y, lm[c][1] + mh[1].y);
       }
       raise(top, top_e);
-      // where V's scale is so small that P of a logit near m would vanish, l needs its own
-      // exponentials: the general path
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        mu[c] = st[c].m == -INFINITY ? 0.f : st[c].m;
+        Mu[c] = st[c].M == -INFINITY ? 0.f : st[c].M;
+      }
+      // where V's scale is so small that P of a logit near m would vanish, l needs its own exponentials
       const float e_min = fminf(mh[0].y, mh[1].y);
-      plain = !__any_sync(0xffffffffu, !(st[0].m + e_min - st[0].M > -90.f) || !(st[1].m + e_min - st[1].M > -90.f));
-      if (plain) {
+      formed = __any_sync(0xffffffffu, !(fminf(mu[0] - Mu[0], mu[1] - Mu[1]) + e_min > -90.f));
+      if (!formed) {
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float shift = mh[h].y - st[c].M + CA_P_SHIFT;
+            const float shift = mh[h].y - Mu[c] + CA_P_SHIFT;
             sc[h][c] = exp2_fast(fmaf(sc[h][c], f[c][h], shift));
             sc[h][2 + c] = exp2_fast(fmaf(sc[h][2 + c], f[c][h], shift));
-            st[c].l = fmaf(sc[h][c] + sc[h][2 + c], exp2_fast(-shift - st[c].m), st[c].l);
+            st[c].l = fmaf(sc[h][c] + sc[h][2 + c], exp2_fast(-shift - mu[c]), st[c].l);
           }
       } else {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
+          ve[h][0] = ve[h][1] = mh[h].y;
 #pragma unroll
           for (int e = 0; e < 4; ++e) sc[h][e] *= f[e & 1][h];
+        }
       }
-    }
-    if (!plain) {
-      float ve[2][2];
-      if (valid_all) {  // came from above, logits formed
-        ve[0][0] = ve[0][1] = mh[0].y;
-        ve[1][0] = ve[1][1] = mh[1].y;
-      } else {
-        valid = 0;
-        const int head = window ? -1 : (lb + i - n_w) / lmk32;
+    } else {
+      float lm[2] = {-INFINITY, -INFINITY}, lM[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const int slot = b * 8 + slot_of(g);  // within the half
-            float4 mt = mh[h];
-            if (!window) {
-              mt = meta[h * 16 + slot];
-              mt.y = scale_log(mt.y);
-            }
-            int key = __float_as_int(mt.w);
-            if (window && key >= 0) {
-              key += slot;
-              if (key >= p.len) key = -1;
-            }
-            ve[h][b] = mt.y;
+        for (int b = 0; b < 2; ++b) {
+          const float4 mt = meta[h * 16 + b * 8 + slot];
+          ve[h][b] = scale_log(mt.y);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const bool ok = key >= 0 && (window ? key >= row_lo[c] && key < row_hi[c]
-                                                  : key < row_lo[c] && key < row_hi[c] && head == row_head[c]);
-              if (ok) valid |= 1u << (4 * h + 2 * b + c);
-              sc[h][2 * b + c] = ok ? fmaf(sc[h][2 * b + c], mt.x * row_f[c], mt.z) : -INFINITY;
-            }
+          for (int c = 0; c < 2; ++c) {
+            float& x = sc[h][2 * b + c];
+            x = attends(h, b, c) ? fmaf(x, mt.x * row_f[c], mt.z) : -INFINITY;
+            lm[c] = fmaxf(lm[c], x);
+            lM[c] = fmaxf(lM[c], x + ve[h][b]);
           }
-      }
-      float lm[2], lM[2];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        lm[c] = fmaxf(fmaxf(sc[0][c], sc[0][2 + c]), fmaxf(sc[1][c], sc[1][2 + c]));
-        lM[c] = fmaxf(fmaxf(sc[0][c] + ve[0][0], sc[0][2 + c] + ve[0][1]), fmaxf(sc[1][c] + ve[1][0], sc[1][2 + c] + ve[1][1]));
-      }
+        }
       raise(lm, lM);
+    }
+    if (formed) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const float mu = st[c].m == -INFINITY ? 0.f : st[c].m, Mu = st[c].M == -INFINITY ? 0.f : st[c].M;
@@ -676,12 +680,13 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
         }
       }
       bool nans = false;
-      if (!plain) {
+      if (!whole) {
+        uint32_t hit = 0;  // 0x7f, the only NaN, is what a carry takes to the eighth bit
 #pragma unroll
         for (int x = 0; x < 4; ++x)
 #pragma unroll
-          for (int y = 0; y < D / 32; ++y) nans |= nan_bytes(v[x][y]) != 0;
-        nans = __any_sync(0xffffffffu, nans);
+          for (int y = 0; y < D / 32; ++y) hit |= (v[x][y] & 0x7f7f7f7fu) + 0x01010101u;
+        nans = __any_sync(0xffffffffu, (hit & 0x80808080u) != 0);
       }
       if (nans) {
         // P = 0 must not spread a NaN: count, per channel and row, the NaNs among the keys that the
@@ -689,8 +694,7 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
         uint32_t ones[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const uint32_t bits = valid >> (4 * h + 2 * b);
-          ones[b] = transpose8((bits & 1 ? 0x3c00u : 0u) | (bits & 2 ? 0x3c000000u : 0u));
+          ones[b] = transpose8((attends(h, b, 0) ? 0x3c00u : 0u) | (attends(h, b, 1) ? 0x3c000000u : 0u));
         }
 #pragma unroll
         for (int x = 0; x < D / 32; ++x) {
@@ -798,10 +802,19 @@ __global__ void __launch_bounds__(CJ_THREADS) cache_attn_join_kernel(CacheAttnAr
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   cudaGridDependencySynchronize();
   const int64_t rows = (int64_t)a.T * a.H, row0 = (int64_t)blockIdx.x * rows_per_block;
+  // which of the block's rows were cut. One part: already written. Anything else than parts of
+  // this call: a row of no sequence.
+  __shared__ int2 s_part[CJ_THREADS];
+  bool cut = false;
+  if (tid < rows_per_block && row0 + tid < rows) {
+    const int2 rp = a.row_part[row0 + tid];
+    cut = rp.y > 1 && rp.x >= 0 && rp.y <= 2 * CA_MAX_SLOTS && rp.x / CA_ROWS + rp.y <= 2 * CA_MAX_SLOTS;
+    s_part[tid] = cut ? rp : make_int2(0, 0);
+  }
+  if (!__syncthreads_or(cut)) return;
   for (int64_t row = row0; row < min(row0 + rows_per_block, rows); ++row) {
-    const int2 rp = a.row_part[row];
-    // one part: already written. Anything else than parts of this call: a row of no sequence.
-    if (rp.y <= 1 || rp.x < 0 || rp.y > 2 * CA_MAX_SLOTS || rp.x / CA_ROWS + rp.y > 2 * CA_MAX_SLOTS) continue;
+    const int2 rp = s_part[row - row0];
+    if (rp.y == 0) continue;
     const float4* ps = reinterpret_cast<const float4*>(a.part_s) + rp.x;
     float m = -INFINITY, M = -INFINITY;
     for (int x = tid; x < rp.y; x += CJ_THREADS) {
@@ -879,9 +892,9 @@ static int launch_cache_attn(const CacheAttnArgs& a, unsigned grid, bool join, c
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  // up to two rounds of blocks; where there are more rows, few of them are cut
+  // a block per row up to one round of blocks; where there are more rows, few of them are cut
   const int64_t rows = (int64_t)a.T * a.H;
-  const int per = (int)((rows + 148 * 8 - 1) / (148 * 8));
+  const int per = (int)std::min<int64_t>((rows + 148 * 4 - 1) / (148 * 4), CJ_THREADS);
   cfg.gridDim = dim3((unsigned)((rows + per - 1) / per));
   cfg.blockDim = dim3(CJ_THREADS);
   cfg.stream = stream;
