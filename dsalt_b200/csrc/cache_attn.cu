@@ -40,6 +40,7 @@ constexpr int CA_WARPS = 2;
 constexpr int CA_THREADS = 32 * CA_WARPS;
 constexpr int CA_MIN_TILES = 8;        // tiles of 32 keys that a unit takes at least: four per warp
 constexpr int CA_MAX_SEQS = 8192;
+constexpr int CA_OWN_SCHED = 128;      // sequences up to which every block makes the schedule for itself
 constexpr int CA_ERR_PAGE = 41;        // device status: a page number outside the pool was met
 constexpr float CA_P_SHIFT = 14.f;     // P is held times 2^14: fp16 stays normal down to 2^-28
 constexpr float CA_SLACK = 1.f;        // P may exceed 2^14 by 2^1 before its reference moves (fp16 ends at 2^16)
@@ -71,6 +72,7 @@ struct CacheAttnArgs {
   float* part_o;   // [cut units][8][D]
   float* part_s;   // [cut units][8][4]: m, l, M
   int2* row_part;  // [T * H] first part of the row and how many there are
+  int2* sched;     // many sequences: {chunk, units}, then {units, parts} before each sequence; else null
   int* err;
 };
 
@@ -140,7 +142,8 @@ __device__ __forceinline__ SeqPlan plan_of(const CacheAttnArgs& a, int s) {
 }
 __device__ __forceinline__ int row_tiles(const CacheAttnArgs& a, int n_q) { return (n_q * a.G + CA_ROWS - 1) / CA_ROWS; }
 
-// sums of two numbers over the block's 128 threads, exclusive; totals in `all`
+// sums of two numbers over the block's threads, exclusive; totals in `all`
+template <int WARPS>
 __device__ __forceinline__ int2 block_before2(int2 v, int2* red, int2& all) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int2 s = v;
@@ -155,11 +158,65 @@ __device__ __forceinline__ int2 block_before2(int2 v, int2* red, int2& all) {
   int2 before = make_int2(0, 0);
   all = make_int2(0, 0);
 #pragma unroll
-  for (int i = 0; i < CA_WARPS; ++i) {
+  for (int i = 0; i < WARPS; ++i) {
     if (i < warp) before.x += red[i].x, before.y += red[i].y;
     all.x += red[i].x, all.y += red[i].y;
   }
   return make_int2(before.x + s.x - v.x, before.y + s.y - v.y);
+}
+
+// Tiles that a unit takes. Cutting adds at most one unit per item: where the items leave room,
+// all units run at once; where they do not, only items above an average slot's load are cut.
+__device__ __forceinline__ int chunk_of(long long tiles, long long items, int slots) {
+  const long long want = items < slots ? max(slots - items, (long long)slots / 4) : slots;
+  return (int)min(max((tiles + want - 1) / want, (long long)CA_MIN_TILES), 0x7fffffffLL);
+}
+
+// The schedule of many sequences, made once: for few, each block's own takes less time than a
+// launch; its time grows with the sequences, in every block.
+constexpr int CP_THREADS = 1024;
+__global__ void __launch_bounds__(CP_THREADS) cache_attn_plan_kernel(CacheAttnArgs a, int slots) {
+  __shared__ long long s_sum[CP_THREADS / 32][2];
+  __shared__ int2 red[CP_THREADS / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int MINE = CA_MAX_SEQS / CP_THREADS;  // sequences of one thread
+  int len[MINE], count[MINE];
+  long long tiles = 0, items = 0;
+#pragma unroll
+  for (int i = 0; i < MINE; ++i) {
+    const int s = i * CP_THREADS + tid;
+    len[i] = count[i] = 0;
+    if (s < a.n_seqs) {
+      const SeqPlan p = plan_of(a, s);
+      len[i] = p.n_window + p.n_lmk;
+      count[i] = row_tiles(a, p.n_q) * a.Hkv;
+      tiles += (long long)len[i] * count[i];
+      items += count[i];
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+    items += __shfl_xor_sync(0xffffffffu, items, o);
+  }
+  if (lane == 0) s_sum[warp][0] = tiles, s_sum[warp][1] = items;
+  __syncthreads();
+  tiles = items = 0;
+  for (int w = 0; w < CP_THREADS / 32; ++w) tiles += s_sum[w][0], items += s_sum[w][1];
+  const int chunk = chunk_of(tiles, items, slots);
+  int2 carry = make_int2(0, 0);
+#pragma unroll
+  for (int i = 0; i < MINE; ++i) {
+    const int s = i * CP_THREADS + tid;
+    const int splits = max(1, (len[i] + chunk - 1) / chunk);
+    const int2 v = make_int2(count[i] * splits, splits > 1 ? count[i] * splits : 0);
+    int2 all;
+    const int2 b = block_before2<CP_THREADS / 32>(v, red, all);
+    if (s < a.n_seqs) a.sched[1 + s] = make_int2(carry.x + b.x, carry.y + b.y);
+    carry.x += all.x;
+    carry.y += all.y;
+  }
+  if (tid == 0) a.sched[0] = make_int2(chunk, carry.x);
 }
 
 // One stage of a warp's ring: 32 keys. K and V rows of D bytes, their 16-byte chunks placed so
@@ -206,10 +263,33 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
   int* s_len = s_items + a.n_seqs;             // [n_seqs] tiles of one of them
   float* s_o = reinterpret_cast<float*>(dyn);  // [warps][8][D], after the rings
 
-  // ---- schedule: every block derives the same one from the lengths
-  int chunk;
-  SeqPlan first_plan{};
-  {
+  const int unit = blockIdx.x;
+  int n_units;
+  if (a.sched) {
+    // ---- the schedule is there: the last sequence whose units begin at or before this one
+    const int2 head = a.sched[0];
+    n_units = head.y;
+    if (warp == 0 && unit < n_units) {
+      int lo = 0, hi = a.n_seqs;  // sched[1 + lo].x <= unit, sched[1 + hi].x > unit (or hi is the end)
+      while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const uint32_t in = __ballot_sync(0xffffffffu, at < hi && a.sched[1 + at].x <= unit);  // lane 0 always
+        const int f = 31 - __clz(in);
+        hi = min(hi, lo + (f + 1) * step);
+        lo += f * step;
+      }
+      if (lane == 0) {
+        const int2 from = a.sched[1 + lo];
+        s_job.plan = plan_of(a, lo);
+        s_job.s = lo;
+        s_job.local = unit - from.x;
+        s_job.splits = max(1, (s_job.plan.n_window + s_job.plan.n_lmk + head.x - 1) / head.x);
+        s_job.cut = from.y;
+      }
+    }
+  } else {
+    // ---- schedule: every block derives the same one from the lengths
+    SeqPlan first_plan{};
     // tiles and items of the call; both stay below 2^40
     long long mine = 0, count = 0;
     for (int s = tid; s < a.n_seqs; s += CA_THREADS) {
@@ -231,34 +311,30 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
     long long total = 0, items = 0;
 #pragma unroll
     for (int w = 0; w < CA_WARPS; ++w) total += s_sum[w][0], items += s_sum[w][1];
-    // Cutting adds at most one unit per item: where the items leave room, all units run at once;
-    // where they do not, only items above an average slot's load are cut.
-    constexpr int SLOTS = Shape<D>::SLOTS;
-    const long long want = items < SLOTS ? max(SLOTS - items, (long long)SLOTS / 4) : SLOTS;
-    chunk = (int)min(max((total + want - 1) / want, (long long)CA_MIN_TILES), 0x7fffffffLL);
-  }
-  const int unit = blockIdx.x;
-  int2 carry = make_int2(0, 0);
-  for (int base = 0; base < a.n_seqs; base += CA_THREADS) {
-    const int s = base + tid;
-    int2 v = make_int2(0, 0), all;
-    int splits = 1;
-    if (s < a.n_seqs) {
-      splits = max(1, (s_len[s] + chunk - 1) / chunk);
-      v.x = s_items[s] * splits;
-      v.y = splits > 1 ? v.x : 0;
+    const int chunk = chunk_of(total, items, Shape<D>::SLOTS);
+    int2 carry = make_int2(0, 0);
+    for (int base = 0; base < a.n_seqs; base += CA_THREADS) {
+      const int s = base + tid;
+      int2 v = make_int2(0, 0), all;
+      int splits = 1;
+      if (s < a.n_seqs) {
+        splits = max(1, (s_len[s] + chunk - 1) / chunk);
+        v.x = s_items[s] * splits;
+        v.y = splits > 1 ? v.x : 0;
+      }
+      const int2 b = block_before2<CA_WARPS>(v, red, all);
+      const int from = carry.x + b.x;
+      if (unit >= from && unit < from + v.x) {  // one thread, if any
+        s_job.plan = base == 0 ? first_plan : plan_of(a, s);
+        s_job.s = s;
+        s_job.local = unit - from;
+        s_job.splits = splits;
+        s_job.cut = carry.y + b.y;
+      }
+      carry.x += all.x;
+      carry.y += all.y;
     }
-    const int2 b = block_before2(v, red, all);
-    const int from = carry.x + b.x;
-    if (unit >= from && unit < from + v.x) {  // one thread, if any
-      s_job.plan = base == 0 ? first_plan : plan_of(a, s);
-      s_job.s = s;
-      s_job.local = unit - from;
-      s_job.splits = splits;
-      s_job.cut = carry.y + b.y;
-    }
-    carry.x += all.x;
-    carry.y += all.y;
+    n_units = carry.x;
   }
   __syncthreads();
   cudaTriggerProgrammaticLaunchCompletion();  // the join may take its places; it waits for this grid's end
@@ -266,9 +342,9 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
   if (a.cu_q) {
     const int64_t rows0 = (int64_t)min(max(a.cu_q[a.n_seqs], 0), a.T) * a.H, rows1 = (int64_t)a.T * a.H;
     for (int64_t r = rows0 + unit; r < rows1; r += gridDim.x) {
-      if (tid < D) {
-        if (a.out_dtype == DSALT_F32) reinterpret_cast<float*>(a.out)[r * D + tid] = 0.f;
-        else reinterpret_cast<uint16_t*>(a.out)[r * D + tid] = 0;
+      for (int d = tid; d < D; d += CA_THREADS) {
+        if (a.out_dtype == DSALT_F32) reinterpret_cast<float*>(a.out)[r * D + d] = 0.f;
+        else reinterpret_cast<uint16_t*>(a.out)[r * D + d] = 0;
       }
       if (tid == 0) {
         if (a.lse) a.lse[r] = -INFINITY;
@@ -276,7 +352,7 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
       }
     }
   }
-  if (unit >= carry.x) return;
+  if (unit >= n_units) return;
   const SeqPlan p = s_job.plan;
   const int s = s_job.s, splits = s_job.splits, tiles = p.n_window + p.n_lmk;
   const int split = s_job.local % splits, item = s_job.local / splits;
@@ -878,14 +954,16 @@ static inline int64_t ca_items(int64_t T, int n_seqs, int G, int Hkv) { return (
 
 template <typename T, int D, int NS>
 static int launch_cache_attn(const CacheAttnArgs& a, unsigned grid, bool join, cudaStream_t stream) {
-  constexpr size_t RING = (size_t)CA_WARPS * Shape<D>::STAGES * Stage<D>::BYTES, TABLES = 2 * sizeof(int);
+  constexpr size_t RING = (size_t)CA_WARPS * Shape<D>::STAGES * Stage<D>::BYTES;
   static_assert(RING >= sizeof(float) * CA_WARPS * CA_ROWS * D, "the parts take the rings' place");
-  const size_t smem = TABLES * (size_t)a.n_seqs > RING ? TABLES * (size_t)a.n_seqs : RING;
+  static_assert(RING >= 2 * sizeof(int) * CA_OWN_SCHED, "so does the schedule");
   static std::atomic<uint64_t> ready{0};
-  if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(cache_attn_kernel<T, D, NS>),
-                                  (int)(TABLES * CA_MAX_SEQS > RING ? TABLES * CA_MAX_SEQS : RING), ready))
-    return rc;
-  cache_attn_kernel<T, D, NS><<<grid, CA_THREADS, smem, stream>>>(a);
+  if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(cache_attn_kernel<T, D, NS>), (int)RING, ready)) return rc;
+  if (a.sched) {
+    cache_attn_plan_kernel<<<1, CP_THREADS, 0, stream>>>(a, Shape<D>::SLOTS);
+    if (int rc = check_cuda(cudaGetLastError(), "cache_attention plan launch")) return rc;
+  }
+  cache_attn_kernel<T, D, NS><<<grid, CA_THREADS, RING, stream>>>(a);
   if (int rc = check_cuda(cudaGetLastError(), "cache_attention launch")) return rc;
   if (!join) return DSALT_OK;
   cudaLaunchAttribute attr[1];
@@ -911,9 +989,10 @@ extern "C" {
 
 size_t dsalt_cache_attention_workspace_bytes(int64_t T, int n_seqs, int n_heads, int n_kv, int head_dim) {
   if (T < 0 || n_seqs < 1 || n_heads < 1 || n_kv < 1 || head_dim < 1) return 0;
-  // a cut item has at least two units of at least half the wanted length: at most twice the target
+  // cut items: two parts or more each of more than half the wanted length, so at most twice as many as slots
   return ca_a256(sizeof(int2) * (size_t)T * n_heads) + ca_a256(sizeof(float) * 2 * CA_MAX_SLOTS * CA_ROWS * 4) +
-         ca_a256(sizeof(float) * 2 * CA_MAX_SLOTS * CA_ROWS * (size_t)head_dim);
+         ca_a256(sizeof(float) * 2 * CA_MAX_SLOTS * CA_ROWS * (size_t)head_dim) +
+         (n_seqs > CA_OWN_SCHED ? ca_a256(sizeof(int2) * (size_t)(n_seqs + 1)) : 0);
 }
 
 int dsalt_cache_attention(const void* q, int dtype, int64_t T, int n_heads, int n_kv, int head_dim, int64_t q_stride,
@@ -963,6 +1042,8 @@ int dsalt_cache_attention(const void* q, int dtype, int64_t T, int n_heads, int 
   a.part_s = reinterpret_cast<float*>(ws);
   ws += ca_a256(sizeof(float) * 2 * CA_MAX_SLOTS * CA_ROWS * 4);
   a.part_o = reinterpret_cast<float*>(ws);
+  ws += ca_a256(sizeof(float) * 2 * CA_MAX_SLOTS * CA_ROWS * (size_t)head_dim);
+  a.sched = n_seqs > CA_OWN_SCHED ? reinterpret_cast<int2*>(ws) : nullptr;
   a.err = device_status_ptr();
   const int64_t items = ca_items(T, n_seqs, a.G, n_kv);
   const int64_t grid = items + CA_MAX_SLOTS;

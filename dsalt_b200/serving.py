@@ -167,10 +167,10 @@ def append_cache(k, v, k_cache, v_cache, k_scale, v_scale, slots) -> None:
     if v.dtype != k.dtype:
         raise TypeError("k and v must share a dtype")
     _want(slots, "slots", torch.int64, (T,))
-    if not _rows_ok(k):
-        k = k.contiguous()
-    if not _rows_ok(v):
-        v = v.contiguous()
+    if not (k.is_contiguous() and k.data_ptr() % 16 == 0 or _rows_ok(k)):
+        k = k.clone(memory_format=torch.contiguous_format)
+    if not (v.is_contiguous() and v.data_ptr() % 16 == 0 or _rows_ok(v)):
+        v = v.clone(memory_format=torch.contiguous_format)
     _run(dev, "dsalt_append_cache", k.data_ptr(), v.data_ptr(), _dt(k), T, n_kv, D, k.stride(0), k.stride(1), v.stride(0),
          v.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_pages, page,
          slots.data_ptr())
@@ -214,8 +214,8 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_len
         if lmk_indices is None:
             raise ValueError("lmk_bias needs lmk_indices")
         _want(lmk_bias, "lmk_bias", torch.float32, (H, S, k_lmk))
-    if not (_rows_ok(q) and q.stride(1) == D):
-        q = q.contiguous()
+    if not (q.is_contiguous() and q.data_ptr() % 16 == 0 or _rows_ok(q) and q.stride(1) == D):
+        q = q.clone(memory_format=torch.contiguous_format)
     out = torch.empty(T, H, D, dtype=out_dtype or q.dtype, device=dev)
     lse = torch.empty(T, H, dtype=torch.float32, device=dev) if return_lse else None
     ws = _workspace(_attention_workspace(T, S, H, n_kv, D), dev)
@@ -260,7 +260,7 @@ def sample_tokens(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     p, pv = _setting(top_p, "top_p", B, f32, 0.0, inf)
     mp, mv = _setting(min_p, "min_p", B, f32, 0.0, 1.0)
     if V > 1 and logits.stride(1) != 1 or (B > 1 and logits.stride(0) < V):
-        logits = logits.contiguous()
+        logits = logits.contiguous()  # also of a row given to all by expand
     token = torch.empty(B, dtype=torch.int64, device=dev)
     logprob = torch.empty(B, dtype=f32, device=dev) if return_logprob else None
     _run(dev, "dsalt_sample", logits.data_ptr(), _dt(logits), B, V, logits.stride(0) if B > 1 else V, u.data_ptr(),

@@ -306,7 +306,7 @@ def test_attention_over_windows_and_landmarks(V, dtype, H, Hkv, D, page, lens, q
 
 
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("lens", [[2500], [1500, 7, 900], [300] * 40])
+@pytest.mark.parametrize("lens", [[2500], [1500, 7, 900], [300] * 40, [3] * 127 + [400], [3] * 128 + [0, 900], [1, 60] * 700])
 def test_attention_with_cut_keys(V, D, lens):
     # keys split over blocks, short sequences beside long ones
     run_attend(V, attend_case(3, lens, [1] * len(lens), 2, 1, D, 64, torch.bfloat16))
@@ -401,14 +401,8 @@ def test_attention_bytes_behind_the_end_do_not_count(V):
 
 
 def test_attention_rows_behind_the_last_sequence_and_empty_ones(V):
-    c = attend_case(11, [50, 0, 9], [2, 1, 1], 4, 2, 64, 16, torch.bfloat16)
-    c["cu"] = np.array([0, 2, 3, 4], np.int32)
-    gpu = to_gpu(c)
-    gpu["q"] = torch.cat([gpu["q"], torch.full((5, 4, 64), float("nan"), dtype=torch.bfloat16, device="cuda")])
-    out, lse = V.cache_attention(**gpu, return_lse=True)
-    check_attend(c, out[:4], lse[:4])
-    assert (out[4:] == 0).all() and torch.isneginf(lse[4:]).all()
-    assert (out[2] == 0).all()  # a query of an empty sequence
+    for D in (64, 128):
+        rows_behind(V, attend_case(11, [50, 0, 9], [2, 1, 1], 4, 2, D, 16, torch.bfloat16))
     # more query tokens than the sequence has: those before its start have no keys
     c = attend_case(12, [2, 60], [4, 1], 4, 2, 64, 16, torch.bfloat16)
     out, _ = run_attend(V, c)
@@ -420,6 +414,15 @@ def test_attention_rows_behind_the_last_sequence_and_empty_ones(V):
     assert out.shape == (0, 4, 64)
     out = V.cache_attention(**gpu)
     assert (out == 0).all()
+
+
+def rows_behind(V, c):
+    gpu = to_gpu(c)
+    gpu["q"] = torch.cat([gpu["q"], torch.full((5, *c["q"].shape[1:]), float("nan"), dtype=torch.bfloat16, device="cuda")])
+    out, lse = V.cache_attention(**gpu, return_lse=True)
+    check_attend(c, out[:4], lse[:4])
+    assert (out[4:] == 0).all() and torch.isneginf(lse[4:]).all()
+    assert (out[2] == 0).all()  # a query of an empty sequence
 
 
 def test_attention_bad_pages_are_left_out_and_reported(V):
@@ -604,7 +607,50 @@ def test_sample_largest_vocabulary_and_batch(V, dtype):
     assert V.sample_tokens(many[:0], u[:0]).shape == (0,)
 
 
-# ------------------------------------------------------------------ the operators together
+# ------------------------------------------------------------------ graphs, streams, the operators together
+def test_a_captured_decode_step_follows_the_state(V):
+    """Slots, append, attention and sampling in one graph, on a stream of its own; each replay is a
+    step, and equals the same calls made one by one on a copy of the state."""
+    S, H, Hkv, D, page, max_pages, n_pages = 3, 4, 2, 64, 16, 6, 20
+    g = torch.Generator(device="cuda").manual_seed(1)
+    new = torch.tensor([1, 1, 0], dtype=torch.int32, device="cuda")
+    k, v = (torch.randn(S, Hkv, D, device="cuda", generator=g).bfloat16() for _ in range(2))
+    q, head = torch.randn(S, H, D, device="cuda", generator=g).bfloat16(), torch.randn(H * D, 500, device="cuda", generator=g)
+    u = torch.rand(S, device="cuda", generator=g)
+
+    def state():
+        kc = torch.zeros(n_pages, Hkv, page, D, device="cuda").to(F8)
+        sc = torch.zeros(n_pages, Hkv, device="cuda")
+        t = torch.full((S, max_pages), -1, dtype=torch.int32, device="cuda")
+        t[0, 0], t[2, 0] = 18, 19  # the pages of the tokens already there
+        return dict(t=t, n=torch.tensor([14, 0, 3], dtype=torch.int32, device="cuda"),
+                    free=torch.arange(n_pages, dtype=torch.int32, device="cuda"),
+                    nf=torch.tensor([18], dtype=torch.int32, device="cuda"), kc=kc, vc=kc.clone(), ks=sc, vs=sc.clone())
+
+    def step(s):
+        plan = V.reserve_slots(s["t"], s["n"], new, s["free"], s["nf"], page, S, inplace=True)
+        V.append_cache(k, v, s["kc"], s["vc"], s["ks"], s["vs"], plan.slots)
+        out = V.cache_attention(q, s["kc"], s["vc"], s["ks"], s["vs"], s["t"], s["n"], cu_q=plan.cu_new)
+        tok, lp = V.sample_tokens(out.flatten(1).float() @ head, u, temperature=0.7, top_k=40, top_p=0.9, return_logprob=True)
+        return plan.slots, plan.positions, out, tok, lp
+
+    a, b = state(), state()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(state())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            captured = step(a)
+        for _ in range(20):
+            graph.replay()
+            for x, y in zip(captured, step(b)):
+                assert torch.equal(x, y)
+    side.synchronize()
+    assert a["n"].tolist() == [34, 20, 3] and torch.equal(a["t"], b["t"]) and int(a["nf"]) == 18 - 2 - 2
+    assert status() == 0
+
+
 def test_serving_steps_together(V):
     """Admission, prompts, decode steps and release of several requests, each step checked."""
     g = np.random.default_rng(20)
