@@ -19,6 +19,10 @@
 //   cache; P alone is transposed, two movmatrix per 16 keys;
 // * P is rounded to fp16 relative to the row's largest p * 2^e (half a step is 2^-11 of a
 //   term, errors of either sign); fp32 queries take Q and P as two fp16 terms each (22 bits).
+// * the tensor cores cut off what does not fit a sum's 24 bits, which over a long cache adds up
+//   (3.4e-4 of the result after 4096 products in a row); so O is added up by them over
+//   CA_CHAIN tiles at most and then, rounded, to an array in local memory (1e-6 remains), for
+//   fp32 queries over 16 keys only.
 // The scales of V differ from page to page, so a row keeps two maxima: m of x for the
 // denominator l = sum 2^(x - m), and M of x + e for the numerator O = sum 2^(x + e - M) byte;
 // out = O 2^(M - m) / l. Neither can overflow whatever the scales are.
@@ -43,6 +47,7 @@ constexpr int CA_MAX_SEQS = 8192;
 constexpr int CA_OWN_SCHED = 128;      // sequences up to which every block makes the schedule for itself
 constexpr int CA_ERR_PAGE = 41;        // device status: a page number outside the pool was met
 constexpr float CA_P_SHIFT = 14.f;     // P is held times 2^14: fp16 stays normal down to 2^-28
+constexpr int CA_CHAIN = 64;            // tiles that O is added up over by the tensor cores alone
 constexpr float CA_SLACK = 1.f;        // P may exceed 2^14 by 2^1 before its reference moves (fp16 ends at 2^16)
 
 // blocks per SM that registers and rings allow; one round of them is the number of units wanted
@@ -606,7 +611,40 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
     }
   };
 
+  // o to the sum over the tiles before; that sum, in o, with `all`
+  [[maybe_unused]] volatile float far_o[D == 64 ? 1 : MT][4];
+  [[maybe_unused]] float* const far_s =
+      reinterpret_cast<float*>(dyn + CA_WARPS * STAGES * Stage<D>::BYTES) + warp * (MT * 4 * 32) + lane;
+  [[maybe_unused]] const auto far_get = [&](int x, int e) -> float {
+    if constexpr (D == 64) return far_s[(x * 4 + e) * 32];
+    else return far_o[x][e];
+  };
+  [[maybe_unused]] const auto far_put = [&](int x, int e, float v) {
+    if constexpr (D == 64) far_s[(x * 4 + e) * 32] = v;
+    else far_o[x][e] = v;
+  };
+  [[maybe_unused]] float far_M[2];
+  [[maybe_unused]] const auto put_by = [&](bool first, bool all) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float corr = first || st[c].M == -INFINITY ? 1.f : exp2_fast(far_M[c] - st[c].M);
+#pragma unroll
+      for (int x = 0; x < MT; ++x)
+#pragma unroll
+        for (int e = c; e < 4; e += 2) {
+          if (!first) o[x][e] = fmaf(far_get(x, e), corr, o[x][e]);
+          if (!all) {
+            far_put(x, e, o[x][e]);
+            o[x][e] = 0.f;
+          }
+        }
+      far_M[c] = st[c].M;
+    }
+  };
+
   for (int i = 0; i < n; ++i) {
+    if constexpr (NS == 1)
+      if (i % CA_CHAIN == 0 && i > 0) put_by(i == CA_CHAIN, false);
     copies_wait<STAGES - 2>();
     __syncwarp();  // every lane's copies of stage i are there, and stage i - 1 is read
     issue(i + STAGES - 1);
@@ -801,11 +839,20 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
           const uint32_t sel = y ? 0x7362 : 0x5140;
           const uint32_t b0 = __byte_perm(v[0][x], v[1][x], sel), b1 = __byte_perm(v[2][x], v[3][x], sel);
           const uint32_t a0 = widen_lo(b0), a1 = widen_hi(b0), a2 = widen_lo(b1), a3 = widen_hi(b1);
+          if constexpr (NS == 1) {
+            mma_f16(o[2 * x + y], a0, a1, a2, a3, pb[0][0], pb[0][1]);
+          } else {
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_f16(c, a0, a1, a2, a3, pb[1][0], pb[1][1]);
+            mma_f16(c, a0, a1, a2, a3, pb[0][0], pb[0][1]);
 #pragma unroll
-          for (int z = 0; z < NS; ++z) mma_f16(o[2 * x + y], a0, a1, a2, a3, pb[z][0], pb[z][1]);
+            for (int e = 0; e < 4; ++e) o[2 * x + y][e] += c[e];
+          }
         }
     }
   }
+  if constexpr (NS == 1)
+    if (n > CA_CHAIN) put_by(false, true);
   if (bad_page) report_device_error(a.err, CA_ERR_PAGE);
 
   // ---- the warps' parts into one
@@ -955,15 +1002,16 @@ static inline int64_t ca_items(int64_t T, int n_seqs, int G, int Hkv) { return (
 template <typename T, int D, int NS>
 static int launch_cache_attn(const CacheAttnArgs& a, unsigned grid, bool join, cudaStream_t stream) {
   constexpr size_t RING = (size_t)CA_WARPS * Shape<D>::STAGES * Stage<D>::BYTES;
+  constexpr size_t SMEM = RING + (NS == 1 && D == 64 ? sizeof(float) * CA_THREADS * D / 4 : 0);
   static_assert(RING >= sizeof(float) * CA_WARPS * CA_ROWS * D, "the parts take the rings' place");
   static_assert(RING >= 2 * sizeof(int) * CA_OWN_SCHED, "so does the schedule");
   static std::atomic<uint64_t> ready{0};
-  if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(cache_attn_kernel<T, D, NS>), (int)RING, ready)) return rc;
+  if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(cache_attn_kernel<T, D, NS>), (int)SMEM, ready)) return rc;
   if (a.sched) {
     cache_attn_plan_kernel<<<1, CP_THREADS, 0, stream>>>(a, Shape<D>::SLOTS);
     if (int rc = check_cuda(cudaGetLastError(), "cache_attention plan launch")) return rc;
   }
-  cache_attn_kernel<T, D, NS><<<grid, CA_THREADS, RING, stream>>>(a);
+  cache_attn_kernel<T, D, NS><<<grid, CA_THREADS, SMEM, stream>>>(a);
   if (int rc = check_cuda(cudaGetLastError(), "cache_attention launch")) return rc;
   if (!join) return DSALT_OK;
   cudaLaunchAttribute attr[1];

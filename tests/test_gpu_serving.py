@@ -312,6 +312,32 @@ def test_attention_with_cut_keys(V, D, lens):
     run_attend(V, attend_case(3, lens, [1] * len(lens), 2, 1, D, 64, torch.bfloat16))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_of_long_uncut_rows_loses_nothing_on_the_way(V, D, dtype):
+    # More sequences than places, so that none is cut: each warp adds up 65536 keys of positive V.
+    # What a rounding or a cut of the running sum may cost, relative to the result:
+    # * fp16 P: half a step of 2^-11 per key, either sign: 8 * 2^-11 / sqrt(131072) = 1.1e-5;
+    # * at most 128 products in a row, each cut by one step of 2^-23 of a sum that grows evenly:
+    #   64 * 2^-23 = 7.6e-6;
+    # * fp32 sums with rounding, at most 4096 of them, either sign, growing evenly:
+    #   8 * 2^-24 * sqrt(4096 / 3) = 1.8e-5 (fp32 queries; 32 of them, 1.6e-6, for the others).
+    # Both kinds stay below 3e-5; 4096 products in a row, each cut, come to 2e-4 and more.
+    S, n, page = 1200, 131072, 128
+    g = torch.Generator(device="cuda").manual_seed(D)
+    k = torch.randn(n // page, 1, page, D, device="cuda", generator=g).to(F8)
+    v = (torch.rand(n // page, 1, page, D, device="cuda", generator=g) + 0.5).to(F8)
+    scale = torch.ones(n // page, 1, device="cuda")
+    tables = torch.arange(n // page, device="cuda", dtype=torch.int32).repeat(S, 1)
+    q = (torch.randn(S, 1, D, device="cuda", generator=g) * 0.3).to(dtype)
+    out = V.cache_attention(q, k, v, scale, scale, tables, torch.full((S,), n, device="cuda", dtype=torch.int32),
+                            out_dtype=torch.float32)
+    some = torch.arange(0, S, 97, device="cuda")
+    x = q[some, 0].double() @ k.double().reshape(n, D).T / D ** 0.5
+    want = torch.softmax(x, -1) @ v.double().reshape(n, D)
+    assert ((out[some, 0].double() - want) / want).abs().max().item() < 3e-5
+
+
 def test_attention_widths_and_landmarks_at_their_limits(V):
     c = attend_case(4, [200, 90, 64], [2, 1, 1], 4, 2, 64, 16, torch.float16, 50, 9, True)
     c["w"] = np.array([0, -7, 2**31 - 1, 90], np.int32)  # below 1: 1; beyond the start: every key
