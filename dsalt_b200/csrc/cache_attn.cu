@@ -125,6 +125,11 @@ __device__ __forceinline__ int first_key(const CacheAttnArgs& a, int t, int pos)
   const int w = max(a.w[t], 1);
   return max(pos - w + 1, 0);  // no overflow: pos < 2^31, w >= 1
 }
+// The rows of a kv head go head by head, each head's tokens after one another: a tile meets the
+// landmarks of few heads, where token by token it would meet those of all. How many at most:
+__device__ __forceinline__ int tile_heads(const CacheAttnArgs& a, int n_q) {
+  return n_q > 0 ? min(a.G, (CA_ROWS - 2) / n_q + 2) : 0;
+}
 __device__ __forceinline__ SeqPlan plan_of(const CacheAttnArgs& a, int s) {
   SeqPlan p;
   p.q0 = a.cu_q ? min(max(a.cu_q[s], 0), a.T) : s;
@@ -142,7 +147,7 @@ __device__ __forceinline__ SeqPlan plan_of(const CacheAttnArgs& a, int s) {
   // the last key is the sequence's last: tiles behind a row tile's own keys are passed over
   p.lo32 = lo & ~31;
   p.n_window = p.n_q > 0 && p.len > 0 ? (p.len - p.lo32 + 31) >> 5 : 0;
-  p.n_lmk = a.k_lmk > 0 && top > 0 ? a.G * ((a.k_lmk + 31) >> 5) : 0;  // none lies before a window from 0
+  p.n_lmk = a.k_lmk > 0 && top > 0 ? tile_heads(a, p.n_q) * ((a.k_lmk + 31) >> 5) : 0;  // none lies before a window from 0
   return p;
 }
 __device__ __forceinline__ int row_tiles(const CacheAttnArgs& a, int n_q) { return (n_q * a.G + CA_ROWS - 1) / CA_ROWS; }
@@ -366,19 +371,21 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
   const int each = (tiles + splits - 1) / splits;
   const int t_begin = min(split * each, tiles), t_end = min(t_begin + each, tiles);
 
+  const int n_rows = p.n_q * a.G, head0 = tile * CA_ROWS / p.n_q;  // first head of the tile
+  const int n_heads = (min(tile * CA_ROWS + CA_ROWS, n_rows) - 1) / p.n_q - head0 + 1;
   // ---- rows 2t, 2t+1 of the tile are this lane's in S^T and O^T
   int row_lo[2], row_hi[2], row_head[2];
   unsigned row_span[2], row_before[2];  // keys of the window; positions before it, where landmarks count
   bool row_ok[2];
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    const int i = tile * CA_ROWS + 2 * t + c, tok = i / a.G;
-    row_ok[c] = tok < p.n_q;
+    const int i = tile * CA_ROWS + 2 * t + c, tok = i % p.n_q;
+    row_ok[c] = i < n_rows;
     const int pos = p.len - p.n_q + tok;
     const bool keys = row_ok[c] && pos >= 0;
     row_lo[c] = keys ? first_key(a, p.q0 + tok, pos) : 0x7fffffff;
     row_hi[c] = keys ? pos + 1 : 0;
-    row_head[c] = i % a.G;
+    row_head[c] = i / p.n_q - head0;
     row_span[c] = keys ? row_hi[c] - row_lo[c] : 0;
     row_before[c] = keys ? row_lo[c] : 0;
   }
@@ -400,7 +407,7 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
 
   // ---- this warp's share of the unit: a stretch of window tiles, then one of landmark tiles
   const int w0 = min(t_begin, p.n_window), w1 = min(t_end, p.n_window);
-  const int l0 = max(t_begin - p.n_window, 0), l1 = max(t_end - p.n_window, 0);
+  const int l1 = min(max(t_end - p.n_window, 0), n_heads * lmk32), l0 = min(max(t_begin - p.n_window, 0), l1);
   const int wq = (w1 - w0 + CA_WARPS - 1) / CA_WARPS, lq = (l1 - l0 + CA_WARPS - 1) / CA_WARPS;
   int wb = min(w0 + warp * wq, w1), we = min(wb + wq, w1);
   const int lb = min(l0 + warp * lq, l1), le = min(lb + lq, l1);
@@ -437,7 +444,7 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
     o.key = -1;
     const int l = lb + i, c = (l % lmk32) * 32 + lane;
     if (l < le && c < a.k_lmk) {
-      const int64_t at = ((int64_t)(hk * a.G + l / lmk32) * a.n_seqs + s) * a.k_lmk + c;
+      const int64_t at = ((int64_t)(hk * a.G + head0 + l / lmk32) * a.n_seqs + s) * a.k_lmk + c;
       o.key = a.lmk[at];
       if (a.bias) o.add = a.bias[at] * 1.4426950408889634f;
     }
@@ -455,9 +462,9 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
 #pragma unroll
     for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
     const int i = tile * CA_ROWS + g;
-    if (i / a.G < p.n_q) {
-      const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)(p.q0 + i / a.G) * a.q_stride +
-                     (int64_t)(hk * a.G + i % a.G) * D + t * 16;
+    if (i < n_rows) {
+      const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)(p.q0 + i % p.n_q) * a.q_stride +
+                     (int64_t)(hk * a.G + i / p.n_q) * D + t * 16;
 #pragma unroll
       for (int b = 0; b < D / 64; ++b) {
         if constexpr (sizeof(T) == 4) {
@@ -875,8 +882,8 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
   __syncthreads();
   for (int e = tid; e < CA_ROWS * D; e += CA_THREADS) {
     const int r = e / D, d = e % D;
-    const int i = tile * CA_ROWS + r, tok = i / a.G, h = hk * a.G + i % a.G;
-    if (tok >= p.n_q) continue;
+    const int i = tile * CA_ROWS + r, tok = i % p.n_q, h = hk * a.G + i / p.n_q;
+    if (i >= n_rows) continue;
     float m = -INFINITY, M = -INFINITY;
 #pragma unroll
     for (int x = 0; x < CA_WARPS; ++x) {
