@@ -188,11 +188,27 @@ __global__ void __launch_bounds__(APPEND_THREADS, 3) append_cache_kernel(AppendA
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int have = (int)min((int64_t)(back + a.window + page - 1), a.T - t0 + back);
   if (threadIdx.x == 0) s_cands = s_ones = s_runs = 0;
+  const int planes = 2 * a.n_kv, share = (planes + gridDim.y - 1) / gridDim.y;
+  const int p0 = blockIdx.y * share, p1 = min(p0 + share, planes), n_planes = max(p1 - p0, 0);
   for (int i = threadIdx.x; i < have; i += APPEND_THREADS) {
     const int64_t s = a.slots[t0 - back + i];
     const int64_t id = s >> a.page_shift;
     s_page[i] = id < a.n_pages ? (int32_t)max(id, (int64_t)-1) : -1;  // outside the pool: not written
     s_in[i] = (int16_t)(s & (page - 1));
+  }
+  // the rows are on their way to L2 while the runs are looked for
+  if (a.window > 8) {
+    constexpr int LINES = D * (int)sizeof(T) / 128;
+    const int n = (int)min((int64_t)a.window, a.T - t0);
+    for (int i = threadIdx.x; i < n * n_planes; i += APPEND_THREADS) {
+      const int y = i / n_planes, pl = p0 + i % n_planes;
+      const bool is_v = pl >= a.n_kv;
+      const int64_t token = t0 + y, at = is_v ? token * a.v.token_stride + (pl - a.n_kv) * a.v.head_stride
+                                             : token * a.k.token_stride + pl * a.k.head_stride;
+      const T* p = reinterpret_cast<const T*>(is_v ? a.v.src : a.k.src) + at;
+#pragma unroll
+      for (int l = 0; l < LINES; ++l) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + l * (128 / (int)sizeof(T))));
+    }
   }
   __syncthreads();
   // a run begins where none of the `page - 1` tokens before lies in the same page, and spans the
@@ -232,8 +248,6 @@ __global__ void __launch_bounds__(APPEND_THREADS, 3) append_cache_kernel(AppendA
     }
   }
   __syncthreads();
-  const int planes = 2 * a.n_kv, share = (planes + gridDim.y - 1) / gridDim.y;
-  const int p0 = blockIdx.y * share, p1 = min(p0 + share, planes), n_planes = max(p1 - p0, 0);
   const int64_t tok0 = t0 - back;
 
   // ---- runs of one token: D/8 lanes each
