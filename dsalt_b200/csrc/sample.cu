@@ -347,6 +347,18 @@ struct Share {
       f(now, index(step));
     }
   }
+  // f(four logits, index of the first) for the warp's elements, NaN outside the row
+  template <typename F>
+  __device__ __forceinline__ void fours(F&& f) const {
+    steps([&](const Raw& r, int i0) {
+#pragma unroll
+      for (int x = 0; x < 4; x += 2) {
+        const float2 a = pair(r, x), b = pair(r, x + 1);
+        const float l[4] = {a.x, a.y, b.x, b.y};
+        f(l, i0 + 2 * x);
+      }
+    });
+  }
   // f(logit, index) for the warp's elements, NaN outside the row
   template <typename F>
   __device__ __forceinline__ void each(F&& f) const {
@@ -394,14 +406,28 @@ __device__ __forceinline__ void bins_pass(Share<T> s, Weights wt, float inv_t, u
   auto& priv = block_shared().priv;
 #pragma unroll
   for (int b = 0; b < PBINS; ++b) priv[b][threadIdx.x] = 0;
-  const auto put = [&](float l, int i, float z, u64 m) {
-    if (l > -INFINITY && (cut == 0 || compose(l, i) >= cut)) priv[(int)fminf(z, (float)(PBINS - 1))][threadIdx.x] += m;
-  };
   constexpr u64 ONE = 1ull << 52;
-  if (wt.only_top || !by_mass)
-    s.each([&](float l, int i) { put(l, i, place_of(l, wt.top, inv_t), ONE + (by_mass && l == wt.top ? (u64)MASS_ONE : 0)); });
-  else
-    s.each([&](float l, int i) { put(l, i, (wt.top - l) * inv_t, ONE + Weights::mass(wt.finite(l))); });
+  // four elements at a time, and no branch: their chains of 64-bit instructions run side by side
+  const auto put = [&](auto&& mass) {
+    s.fours([&](const float (&l)[4], int i0) {
+      u64 m[4];
+      int b[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        m[e] = mass(l[e], i0 + e);
+        b[e] = (int)fminf(place_of(l[e], wt.top, inv_t), (float)(PBINS - 1));
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) priv[b[e]][threadIdx.x] += m[e];
+    });
+  };
+  if (!by_mass) put([&](float l, int) { return l > -INFINITY ? ONE : 0; });
+  else if (wt.only_top) put([&](float l, int i) { return l > -INFINITY && compose(l, i) >= cut ? ONE + wt.mass(l) : 0; });
+  else if (cut == 0) put([&](float l, int) { const u64 m = ONE + Weights::mass(wt.finite(l)); return l > -INFINITY ? m : 0; });
+  else put([&](float l, int i) {
+    const u64 m = ONE + Weights::mass(wt.finite(l));
+    return (l > -INFINITY) & (compose(l, i) >= cut) ? m : 0;
+  });
 }
 template <typename T>
 __device__ __forceinline__ int queue_pass(Share<T> s, Bin bin) {  // returns how many there are
@@ -899,9 +925,13 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
     const int first = min(owner * s.per_warp, s.n_steps), steps = min(first + s.per_warp, s.n_steps) - first;
     for (int step = warp; step < steps; step += SAMPLE_WARPS) {
       const int i0 = s.index(first + step);
+      const typename Share<T>::Raw raw = s.load(first + step);
       u64 m = 0;
-#pragma unroll 1
-      for (int i = max(i0, 0); i < min(i0 + 8, a.V); ++i) m += kept(s.one(i), i);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float2 l = Share<T>::pair(raw, x);
+        m += kept(l.x, i0 + 2 * x) + kept(l.y, i0 + 2 * x + 1);
+      }
       m = warp_sum(m);
       if (lane == 0) sh.steps[step] = m;
     }
