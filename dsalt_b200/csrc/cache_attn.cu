@@ -44,7 +44,8 @@ constexpr int CA_WARPS = 2;
 constexpr int CA_THREADS = 32 * CA_WARPS;
 constexpr int CA_MIN_TILES = 8;        // tiles of 32 keys that a unit takes at least: four per warp
 constexpr int CA_MAX_SEQS = 8192;
-constexpr int CA_OWN_SCHED = 128;      // sequences up to which every block makes the schedule for itself
+constexpr int CA_OWN_SCHED = 192;      // sequences up to which every block makes the schedule for itself,
+constexpr int CA_OWN_ROWS = 1024;      // and query tokens beyond one of each
 constexpr int CA_ERR_PAGE = 41;        // device status: a page number outside the pool was met
 constexpr float CA_P_SHIFT = 14.f;     // P is held times 2^14: fp16 stays normal down to 2^-28
 constexpr int CA_CHAIN = 64;            // tiles that O is added up over by the tensor cores alone
@@ -77,7 +78,8 @@ struct CacheAttnArgs {
   float* part_o;   // [cut units][8][D]
   float* part_s;   // [cut units][8][4]: m, l, M
   int2* row_part;  // [T * H] first part of the row and how many there are
-  int2* sched;     // many sequences: {chunk, units}, then {units, parts} before each sequence; else null
+  int2* sched;     // many sequences or tokens: {chunk, units}, then {units, parts} before each sequence; else null
+  struct SeqPlan* plans;  // with sched: [n_seqs]
   int* err;
 };
 
@@ -130,19 +132,24 @@ __device__ __forceinline__ int first_key(const CacheAttnArgs& a, int t, int pos)
 __device__ __forceinline__ int tile_heads(const CacheAttnArgs& a, int n_q) {
   return n_q > 0 ? min(a.G, (CA_ROWS - 2) / n_q + 2) : 0;
 }
-__device__ __forceinline__ SeqPlan plan_of(const CacheAttnArgs& a, int s) {
+// (lane, lanes: who looks at which of the tokens; the lanes' findings are joined)
+__device__ __forceinline__ SeqPlan plan_of(const CacheAttnArgs& a, int s, int lane = 0, int lanes = 1) {
   SeqPlan p;
   p.q0 = a.cu_q ? min(max(a.cu_q[s], 0), a.T) : s;
   p.n_q = a.cu_q ? max(min(a.cu_q[s + 1], a.T) - p.q0, 0) : 1;
   p.len = min(max(a.seq_lens[s], 0), a.max_pages << a.page_shift);
   int lo = p.len, top = 0;
   if (!a.w) lo = 0;
-  else for (int r = 0; r < p.n_q; ++r) {
+  else for (int r = lane; r < p.n_q; r += lanes) {
     const int pos = p.len - p.n_q + r;
     if (pos < 0) continue;
     const int f = first_key(a, p.q0 + r, pos);
     lo = min(lo, f);
     top = max(top, f);
+  }
+  if (lanes > 1) {
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    top = __reduce_max_sync(0xffffffffu, top);
   }
   // the last key is the sequence's last: tiles behind a row tile's own keys are passed over
   p.lo32 = lo & ~31;
@@ -182,8 +189,8 @@ __device__ __forceinline__ int chunk_of(long long tiles, long long items, int sl
   return (int)min(max((tiles + want - 1) / want, (long long)CA_MIN_TILES), 0x7fffffffLL);
 }
 
-// The schedule of many sequences, made once: for few, each block's own takes less time than a
-// launch; its time grows with the sequences, in every block.
+// The schedule of many sequences or tokens, made once: for few, each block's own takes less time
+// than a launch; its time grows with their number, in every block.
 constexpr int CP_THREADS = 1024;
 __global__ void __launch_bounds__(CP_THREADS) cache_attn_plan_kernel(CacheAttnArgs a, int slots) {
   __shared__ long long s_sum[CP_THREADS / 32][2];
@@ -192,12 +199,17 @@ __global__ void __launch_bounds__(CP_THREADS) cache_attn_plan_kernel(CacheAttnAr
   constexpr int MINE = CA_MAX_SEQS / CP_THREADS;  // sequences of one thread
   int len[MINE], count[MINE];
   long long tiles = 0, items = 0;
+  for (int s = warp; s < a.n_seqs; s += CP_THREADS / 32) {
+    const SeqPlan p = plan_of(a, s, lane, 32);
+    if (lane == 0) a.plans[s] = p;
+  }
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < MINE; ++i) {
     const int s = i * CP_THREADS + tid;
     len[i] = count[i] = 0;
     if (s < a.n_seqs) {
-      const SeqPlan p = plan_of(a, s);
+      const SeqPlan p = a.plans[s];
       len[i] = p.n_window + p.n_lmk;
       count[i] = row_tiles(a, p.n_q) * a.Hkv;
       tiles += (long long)len[i] * count[i];
@@ -217,6 +229,7 @@ __global__ void __launch_bounds__(CP_THREADS) cache_attn_plan_kernel(CacheAttnAr
   int2 carry = make_int2(0, 0);
 #pragma unroll
   for (int i = 0; i < MINE; ++i) {
+    if (i * CP_THREADS >= a.n_seqs) break;
     const int s = i * CP_THREADS + tid;
     const int splits = max(1, (len[i] + chunk - 1) / chunk);
     const int2 v = make_int2(count[i] * splits, splits > 1 ? count[i] * splits : 0);
@@ -269,8 +282,7 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
     SeqPlan plan;
     int s, local, splits, cut;  // sequence, unit within it, parts of its items, parts of cut items before it
   } s_job;
-  int* s_items = reinterpret_cast<int*>(dyn);  // [n_seqs] items of the sequence
-  int* s_len = s_items + a.n_seqs;             // [n_seqs] tiles of one of them
+  SeqPlan* s_plans = reinterpret_cast<SeqPlan*>(dyn);  // [n_seqs], before the rings
   float* s_o = reinterpret_cast<float*>(dyn);  // [warps][8][D], after the rings
 
   const int unit = blockIdx.x;
@@ -290,7 +302,7 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
       }
       if (lane == 0) {
         const int2 from = a.sched[1 + lo];
-        s_job.plan = plan_of(a, lo);
+        s_job.plan = a.plans[lo];
         s_job.s = lo;
         s_job.local = unit - from.x;
         s_job.splits = max(1, (s_job.plan.n_window + s_job.plan.n_lmk + head.x - 1) / head.x);
@@ -299,17 +311,21 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
     }
   } else {
     // ---- schedule: every block derives the same one from the lengths
-    SeqPlan first_plan{};
     // tiles and items of the call; both stay below 2^40
     long long mine = 0, count = 0;
-    for (int s = tid; s < a.n_seqs; s += CA_THREADS) {
-      const SeqPlan p = plan_of(a, s);
-      if (s == tid) first_plan = p;
+    const auto add = [&](int s, const SeqPlan& p) {
       const int items = row_tiles(a, p.n_q) * a.Hkv;
-      s_len[s] = p.n_window + p.n_lmk;
-      s_items[s] = items;
-      mine += (long long)s_len[s] * items;
+      s_plans[s] = p;
+      mine += (long long)(p.n_window + p.n_lmk) * items;
       count += items;
+    };
+    if (a.w && a.T >= 32 * a.n_seqs) {  // many tokens each: a warp looks at their widths
+      for (int s = warp; s < a.n_seqs; s += CA_WARPS) {
+        const SeqPlan p = plan_of(a, s, lane, 32);
+        if (lane == 0) add(s, p);
+      }
+    } else {
+      for (int s = tid; s < a.n_seqs; s += CA_THREADS) add(s, plan_of(a, s));
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -328,14 +344,15 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
       int2 v = make_int2(0, 0), all;
       int splits = 1;
       if (s < a.n_seqs) {
-        splits = max(1, (s_len[s] + chunk - 1) / chunk);
-        v.x = s_items[s] * splits;
+        const SeqPlan& p = s_plans[s];
+        splits = max(1, (p.n_window + p.n_lmk + chunk - 1) / chunk);
+        v.x = row_tiles(a, p.n_q) * a.Hkv * splits;
         v.y = splits > 1 ? v.x : 0;
       }
       const int2 b = block_before2<CA_WARPS>(v, red, all);
       const int from = carry.x + b.x;
       if (unit >= from && unit < from + v.x) {  // one thread, if any
-        s_job.plan = base == 0 ? first_plan : plan_of(a, s);
+        s_job.plan = s_plans[s];
         s_job.s = s;
         s_job.local = unit - from;
         s_job.splits = splits;
@@ -1004,6 +1021,8 @@ __global__ void __launch_bounds__(CJ_THREADS) cache_attn_join_kernel(CacheAttnAr
 }
 
 static inline size_t ca_a256(size_t v) { return (v + 255) & ~(size_t)255; }
+// is the schedule made by a kernel of its own?
+static inline bool ca_plans(int64_t T, int n_seqs) { return n_seqs > CA_OWN_SCHED || T - n_seqs > CA_OWN_ROWS; }
 static inline int64_t ca_items(int64_t T, int n_seqs, int G, int Hkv) { return ((T * G + (CA_ROWS - 1) * (int64_t)n_seqs) / CA_ROWS + 1) * Hkv; }
 
 template <typename T, int D, int NS>
@@ -1011,7 +1030,7 @@ static int launch_cache_attn(const CacheAttnArgs& a, unsigned grid, bool join, c
   constexpr size_t RING = (size_t)CA_WARPS * Shape<D>::STAGES * Stage<D>::BYTES;
   constexpr size_t SMEM = RING + (NS == 1 && D == 64 ? sizeof(float) * CA_THREADS * D / 4 : 0);
   static_assert(RING >= sizeof(float) * CA_WARPS * CA_ROWS * D, "the parts take the rings' place");
-  static_assert(RING >= 2 * sizeof(int) * CA_OWN_SCHED, "so does the schedule");
+  static_assert(RING >= sizeof(SeqPlan) * CA_OWN_SCHED, "so does the schedule");
   static std::atomic<uint64_t> ready{0};
   if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(cache_attn_kernel<T, D, NS>), (int)SMEM, ready)) return rc;
   if (a.sched) {
@@ -1047,7 +1066,7 @@ size_t dsalt_cache_attention_workspace_bytes(int64_t T, int n_seqs, int n_heads,
   // cut items: two parts or more each of more than half the wanted length, so at most twice as many as slots
   return ca_a256(sizeof(int2) * (size_t)T * n_heads) + ca_a256(sizeof(float) * 2 * CA_MAX_SLOTS * CA_ROWS * 4) +
          ca_a256(sizeof(float) * 2 * CA_MAX_SLOTS * CA_ROWS * (size_t)head_dim) +
-         (n_seqs > CA_OWN_SCHED ? ca_a256(sizeof(int2) * (size_t)(n_seqs + 1)) : 0);
+         (ca_plans(T, n_seqs) ? ca_a256(sizeof(int2) * (size_t)(n_seqs + 1)) + ca_a256(sizeof(SeqPlan) * (size_t)n_seqs) : 0);
 }
 
 int dsalt_cache_attention(const void* q, int dtype, int64_t T, int n_heads, int n_kv, int head_dim, int64_t q_stride,
@@ -1098,7 +1117,9 @@ int dsalt_cache_attention(const void* q, int dtype, int64_t T, int n_heads, int 
   ws += ca_a256(sizeof(float) * 2 * CA_MAX_SLOTS * CA_ROWS * 4);
   a.part_o = reinterpret_cast<float*>(ws);
   ws += ca_a256(sizeof(float) * 2 * CA_MAX_SLOTS * CA_ROWS * (size_t)head_dim);
-  a.sched = n_seqs > CA_OWN_SCHED ? reinterpret_cast<int2*>(ws) : nullptr;
+  a.sched = ca_plans(T, n_seqs) ? reinterpret_cast<int2*>(ws) : nullptr;
+  ws += ca_a256(sizeof(int2) * (size_t)(n_seqs + 1));
+  a.plans = reinterpret_cast<SeqPlan*>(ws);
   a.err = device_status_ptr();
   const int64_t items = ca_items(T, n_seqs, a.G, n_kv);
   const int64_t grid = items + CA_MAX_SLOTS;

@@ -229,7 +229,7 @@ class DSALTLMHeadModel(nn.Module):
         rows must be empty) into the cache; the logits of each prompt's last token ``[S, vocab]``."""
         cu_h = [int(c) for c in cu_list]
         lens = [b - a for a, b in zip(cu_h, cu_h[1:])]
-        if len(lens) != cache.max_seqs or min(lens) < 1 or cu_h[-1] != input_ids.shape[0]:
+        if len(lens) != cache.max_seqs or min(lens) < 1 or cu_h[0] != 0 or input_ids.shape != (cu_h[-1],):
             raise ValueError("cu_list must give one prompt of at least one token per row of the cache")
         if any(cache.lens):
             raise ValueError("prefill needs empty rows: release them first")
@@ -244,6 +244,8 @@ class DSALTLMHeadModel(nn.Module):
         """One more token per row of the cache ``tokens [S]`` → the next token's logits ``[S, vocab]``."""
         if min(cache.lens) < 1:
             raise ValueError("decode needs a prompt in every row")
+        if tokens.shape != (cache.max_seqs,):
+            raise ValueError(f"decode needs {cache.max_seqs} tokens, one per row")
         plan = cache.reserve([1] * cache.max_seqs)
         x, rope_cs = self._embed(tokens, plan.positions)
         for layer in self.layers:
@@ -261,6 +263,9 @@ class DSALTLMHeadModel(nn.Module):
             raise RuntimeError("generate needs eval mode")
         if max_new_tokens < 1 or not prompts or min(len(p) for p in prompts) < 1:
             raise ValueError("generate needs prompts of at least one token and max_new_tokens >= 1")
+        vocab = self.embed_tokens.num_embeddings
+        if any(not 0 <= t < vocab for p in prompts for t in p):
+            raise ValueError(f"token ids must lie in [0, {vocab})")
         dev = self.embed_tokens.weight.device
         lens = [len(p) for p in prompts]
         S = len(prompts)

@@ -14,8 +14,9 @@ calls for it (:meth:`dsalt_b200.model.DSALTLMHeadModel.generate`).
 
 The reference has no counterpart (it recomputes the whole sequence for every token). As in
 :mod:`dsalt_b200.ops`, tensors must be CUDA tensors and every call launches on the current
-stream of their device; lengths and tables stay on the device, so nothing here synchronises
-and every call can be captured into a CUDA graph.
+stream of their device; lengths and tables stay on the device, so the operators do not
+synchronise and every call can be captured into a CUDA graph. They are for answering, not for
+training: no gradient goes through them.
 """
 from __future__ import annotations
 
@@ -144,10 +145,21 @@ def _cache_shapes(k_cache, v_cache, k_scale, v_scale):
     return n_pages, n_kv, page, D
 
 
-def _rows_ok(x) -> bool:
-    """Rows of ``x [T, H, D]`` that 16-byte loads can take."""
-    es = x.element_size()
-    return (x.stride(2) == 1 and x.data_ptr() % 16 == 0 and x.stride(0) * es % 16 == 0 and x.stride(1) * es % 16 == 0)
+def _rows(x, packed: bool = False):
+    """``x [T, H, D]``, its token and head strides, as 16-byte loads can take its rows (``packed``: a
+    token's heads must follow one another, and its row must not overlap the next); else a copy."""
+    T, H, D = x.shape
+    if x.data_ptr() % 16 == 0:
+        if x.is_contiguous():  # strides of single tokens or heads may be anything
+            return x, H * D, D
+        es, (token, head, one) = x.element_size(), x.stride()
+        if T == 1:
+            token = H * D
+        if H == 1:
+            head = D
+        if one == 1 and token * es % 16 == 0 and head * es % 16 == 0 and not (packed and (head != D or token < H * D)):
+            return x, token, head
+    return x.clone(memory_format=torch.contiguous_format), H * D, D
 
 
 def append_cache(k, v, k_cache, v_cache, k_scale, v_scale, slots) -> None:
@@ -167,13 +179,10 @@ def append_cache(k, v, k_cache, v_cache, k_scale, v_scale, slots) -> None:
     if v.dtype != k.dtype:
         raise TypeError("k and v must share a dtype")
     _want(slots, "slots", torch.int64, (T,))
-    if not (k.is_contiguous() and k.data_ptr() % 16 == 0 or _rows_ok(k)):
-        k = k.clone(memory_format=torch.contiguous_format)
-    if not (v.is_contiguous() and v.data_ptr() % 16 == 0 or _rows_ok(v)):
-        v = v.clone(memory_format=torch.contiguous_format)
-    _run(dev, "dsalt_append_cache", k.data_ptr(), v.data_ptr(), _dt(k), T, n_kv, D, k.stride(0), k.stride(1), v.stride(0),
-         v.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_pages, page,
-         slots.data_ptr())
+    k, k_token, k_head = _rows(k)
+    v, v_token, v_head = _rows(v)
+    _run(dev, "dsalt_append_cache", k.data_ptr(), v.data_ptr(), _dt(k), T, n_kv, D, k_token, k_head, v_token, v_head,
+         k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_pages, page, slots.data_ptr())
 
 
 def cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, *, cu_q=None, w_sizes=None,
@@ -182,7 +191,8 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_len
     ``out_dtype`` (default the query's), with ``return_lse`` also ``lse [T, H]`` fp32.
 
     ``seq_lens [S]`` int32 tokens in the cache, the query tokens included. ``cu_q [S + 1]`` int32
-    packs the query tokens; without it there is one per sequence. With ``w_sizes [T]`` int32 the
+    (from 0, not falling) packs the query tokens, rows behind its last entry come out as zeros;
+    without it there is one per sequence. With ``w_sizes [T]`` int32 the
     query at position ``i`` attends to its window ``[i - w + 1, i]`` and to the landmarks
     ``lmk_indices [H, S, k]`` before it, as :func:`dsalt_b200.ops.dsalt_attention` does
     (``lmk_bias`` is added to their logits); without, to ``[0, i]``."""
@@ -214,12 +224,11 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_len
         if lmk_indices is None:
             raise ValueError("lmk_bias needs lmk_indices")
         _want(lmk_bias, "lmk_bias", torch.float32, (H, S, k_lmk))
-    if not (q.is_contiguous() and q.data_ptr() % 16 == 0 or _rows_ok(q) and q.stride(1) == D):
-        q = q.clone(memory_format=torch.contiguous_format)
+    q, q_stride, _ = _rows(q, packed=True)
     out = torch.empty(T, H, D, dtype=out_dtype or q.dtype, device=dev)
     lse = torch.empty(T, H, dtype=torch.float32, device=dev) if return_lse else None
     ws = _workspace(_attention_workspace(T, S, H, n_kv, D), dev)
-    _run(dev, "dsalt_cache_attention", q.data_ptr(), _dt(q), T, H, n_kv, D, q.stride(0), k_cache.data_ptr(),
+    _run(dev, "dsalt_cache_attention", q.data_ptr(), _dt(q), T, H, n_kv, D, q_stride, k_cache.data_ptr(),
          v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_pages, page, block_tables.data_ptr(), max_pages,
          seq_lens.data_ptr(), S, _ptr(cu_q), _ptr(w_sizes), _ptr(lmk_indices), _ptr(lmk_bias), k_lmk, out.data_ptr(),
          _dt(out), _ptr(lse), ws.data_ptr(), ws.numel())
@@ -332,6 +341,9 @@ class PagedCache:
 
     def release(self, rows) -> None:
         """Ends the sequences of these rows; their pages go back to the pool."""
+        rows = [int(r) for r in rows]
+        if any(not 0 <= r < self.max_seqs for r in rows):
+            raise ValueError(f"rows must lie in [0, {self.max_seqs})")
         flags = [False] * self.max_seqs
         for r in rows:
             flags[r] = True

@@ -154,6 +154,29 @@ def test_generation_refuses_what_it_cannot_hold():
         m.prefill(torch.ones(10, dtype=torch.long, device="cuda"), [0, 4, 10], cache)
 
 
+def test_refused_calls_leave_the_cache_as_it_was():
+    m = _model()
+    vocab = m.embed_tokens.num_embeddings
+    for bad in (-1, vocab):
+        with pytest.raises(ValueError, match="token ids"):
+            m.generate([[1, bad]], 2)
+    cache = m.new_cache(2, 40, page_size=16)
+    ids = torch.ones(10, dtype=torch.long, device="cuda")
+    for cu in ([2, 4, 10], [0, 4, 9], [0, 10]):
+        with pytest.raises(ValueError, match="one prompt"):
+            m.prefill(ids, cu, cache)
+    assert cache.lens == [0, 0]
+    m.prefill(ids, [0, 4, 10], cache)
+    with pytest.raises(ValueError, match="one per row"):
+        m.decode(ids[:1], cache)
+    for rows in ([0, 2], [-1]):
+        with pytest.raises(ValueError, match="rows must lie"):
+            cache.release(rows)
+    assert cache.lens == [4, 6] and cache.seq_lens.tolist() == [4, 6]
+    cache.release([1, 1])  # the same row twice
+    assert cache.lens == [4, 0] and int(cache.n_free) == cache.n_pages - 1
+
+
 def test_registered_operators():
     """The torch.library forms: opcheck (schema, mutation, shape functions) and equality."""
     from dsalt_b200 import library, serving  # noqa: F401

@@ -312,6 +312,36 @@ def test_attention_with_cut_keys(V, D, lens):
     run_attend(V, attend_case(3, lens, [1] * len(lens), 2, 1, D, 64, torch.bfloat16))
 
 
+@pytest.mark.parametrize("H,Hkv,D,page,lens,q_lens,w_max,k", [
+    (4, 2, 64, 16, [420, 900], [300, 2], 90, 40), (8, 1, 128, 64, [261, 0, 40], [261, 0, 35], 70, 33),
+    (2, 2, 64, 32, [700], [513], 0, 0), (3, 1, 64, 16, [30] * 9, [30] * 9, 12, 5)])
+def test_attention_of_many_tokens_per_sequence(V, H, Hkv, D, page, lens, q_lens, w_max, k):
+    run_attend(V, attend_case(5, lens, q_lens, H, Hkv, D, page, torch.bfloat16, w_max, k))
+
+
+def test_single_tokens_and_heads_of_any_stride(V):
+    # a dimension of one element may have any stride, an expanded row the stride 0
+    c = attend_case(6, [40], [1], 1, 1, 64, 16, torch.bfloat16)
+    plain, args = to_gpu(c)["q"], to_gpu(c)
+    for strides in ((1, 1, 1), (0, 0, 1), (7, 3, 1)):
+        args["q"] = plain.as_strided((1, 1, 64), strides)
+        out, lse = V.cache_attention(**args, return_lse=True)
+        check_attend(c, out, lse)
+    c = attend_case(7, [40, 33], [1, 1], 2, 1, 64, 16, torch.bfloat16)
+    args = to_gpu(c)
+    args["q"] = args["q"][:1].expand(2, -1, -1)
+    same = dict(args, q=args["q"].contiguous())
+    assert torch.equal(V.cache_attention(**args), V.cache_attention(**same))
+    k = torch.randn(64, device="cuda").to(torch.bfloat16)
+    caches = [[torch.zeros(2, 1, 16, 64, dtype=torch.uint8, device="cuda").view(F8) for _ in range(2)]
+              + [torch.zeros(2, 1, device="cuda") for _ in range(2)] for _ in range(2)]
+    slot = torch.tensor([17], device="cuda")
+    V.append_cache(k.as_strided((1, 1, 64), (1, 5, 1)), k.as_strided((1, 1, 64), (0, 0, 1)), *caches[0], slot)
+    V.append_cache(k.view(1, 1, 64), k.view(1, 1, 64), *caches[1], slot)
+    for a, b in zip(*caches):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("D", [64, 128])
 def test_attention_of_long_uncut_rows_loses_nothing_on_the_way(V, D, dtype):
