@@ -619,9 +619,10 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
 #pragma unroll
   for (int r = 0; r < 8; ++r)
     if (r < C) top = fmaxf(top, cluster.map_shared_rank(&sh, r)->best);
-  // a small top-k's bound: the k-th largest of the groups' maxima. (Near the smallest of them
-  // the bound would fall off, so the last few are left to the larger k's way.)
-  const bool small_k = cut_k && temp > 0.f && top_k <= C * groups - C * groups / 8;
+  // a small top-k's bound: the k-th largest of the groups' maxima. (Towards the smallest of them
+  // the bound falls off: k = 200 of 256 in a row of 16384 took 26.5 us, by the threads' maxima 15.4;
+  // k = 64 takes 12.4 this way and 13.7 that way.)
+  const bool small_k = cut_k && temp > 0.f && top_k <= C * groups / 2;
   float bound = -INFINITY;
   if (small_k) {
     if (tid < C * groups) sh.all_max[tid] = cluster.map_shared_rank(&sh, tid / groups)->group_max[tid % groups];

@@ -17,7 +17,9 @@
 namespace dsalt {
 
 constexpr int SLOT_MAX_SEQS = 8192;  // three int32 per row in shared memory
-constexpr int SLOT_FILL_MAX = 1024;  // tokens that the rows' block numbers itself
+constexpr int SLOT_THREADS = 1024;
+constexpr int SLOT_FILL_MAX = 4096;  // tokens that the rows' block numbers itself: 4096 in 64 rows take 7.1 us
+                                     // either way, 2048 in 4 rows 4.6 against 6.2, 8192 in 64 rows 9.9 against 7.3
 
 struct Pair64 {
   long long a, b;
@@ -106,16 +108,19 @@ __global__ void __launch_bounds__(THREADS) reserve_slots_kernel(
   }
   if (tid == 0) s_cu[0] = 0;
   __syncthreads();
-  // new table entries, a warp per row
+  // new table entries: of a row that gets few pages by a thread, of others by a warp
   const int warp = tid >> 5, lane = tid & 31;
-  for (int s = warp; s < n_seqs; s += THREADS / 32) {
+  const auto enter = [&](int s, int from, int step, bool few) {
     const int old = s_old[s];
-    if (old < 0) continue;
+    if (old < 0) return;
     const int add = s_cu[s + 1] - s_cu[s], first = s_first[s];
     const int have = (int)(((long long)old + page_mask) >> page_shift), want = (int)(((long long)old + add + page_mask) >> page_shift);
-    for (int c = have + lane; c < want; c += 32)
+    if ((want - have <= 4) != few) return;
+    for (int c = have + from; c < want; c += step)
       tables[(int64_t)s * max_pages + c] = free_pages[n_free - 1 - (first + c - have)];
-  }
+  };
+  for (int s = tid; s < n_seqs; s += THREADS) enter(s, 0, 1, true);
+  for (int s = warp; s < n_seqs; s += THREADS / 32) enter(s, lane, 32, false);
   for (int s = tid; s < n_seqs; s += THREADS) {
     const int old = s_old[s];
     const bool ok = old >= 0;
@@ -196,24 +201,23 @@ __global__ void __launch_bounds__(256) fill_slots_kernel(const int32_t* __restri
 // The pages of the flagged rows go back on the stack, in the order in which reserve_slots
 // would take them again (page number j of the rows in order to free[n_free + total - 1 - j]);
 // their table entries become -1 and their lengths 0.
-template <int THREADS>
-__global__ void __launch_bounds__(THREADS) release_slots_kernel(int32_t* __restrict__ tables, int n_seqs, int max_pages,
+__global__ void __launch_bounds__(SLOT_THREADS) release_slots_kernel(int32_t* __restrict__ tables, int n_seqs, int max_pages,
                                                                 int32_t* __restrict__ seq_lens,
                                                                 const uint8_t* __restrict__ release,
                                                                 int32_t* __restrict__ free_pages, int free_cap,
                                                                 int32_t* __restrict__ n_free_io, int page_shift) {
   extern __shared__ int32_t s_upto[];  // [n_seqs] pages of the flagged rows up to and with s
-  __shared__ Pair64 warp_sums[THREADS / 32];
+  __shared__ Pair64 warp_sums[SLOT_THREADS / 32];
   const int tid = threadIdx.x, page_mask = (1 << page_shift) - 1;
   int n_free = *n_free_io;
   n_free = n_free < 0 ? 0 : (n_free > free_cap ? free_cap : n_free);
   long long carry = 0;
-  for (int base = 0; base < n_seqs; base += THREADS) {
+  for (int base = 0; base < n_seqs; base += SLOT_THREADS) {
     const int s = base + tid;
     long long held = 0;
     if (s < n_seqs && release[s]) held = min(((long long)max(seq_lens[s], 0) + page_mask) >> page_shift, (long long)max_pages);
     Pair64 all;
-    const Pair64 p = block_scan<THREADS>(Pair64{held, 0}, warp_sums, all);
+    const Pair64 p = block_scan<SLOT_THREADS>(Pair64{held, 0}, warp_sums, all);
     if (s < n_seqs) s_upto[s] = (int32_t)(carry + p.a);
     carry += all.a;
   }
@@ -221,7 +225,7 @@ __global__ void __launch_bounds__(THREADS) release_slots_kernel(int32_t* __restr
   const int total = (int)carry;
   // every flagged page: number j, its row by search; four under way at a time
 #pragma unroll 4
-  for (int j = tid; j < total; j += THREADS) {
+  for (int j = tid; j < total; j += SLOT_THREADS) {
     int lo = 0, hi = n_seqs - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
@@ -234,7 +238,7 @@ __global__ void __launch_bounds__(THREADS) release_slots_kernel(int32_t* __restr
     if (to < free_cap) free_pages[to] = *e;
     *e = -1;
   }
-  for (int s = tid; s < n_seqs; s += THREADS)
+  for (int s = tid; s < n_seqs; s += SLOT_THREADS)
     if (release[s]) seq_lens[s] = 0;
   if (tid == 0) *n_free_io = (int)min((long long)n_free + total, (long long)free_cap);
 }
@@ -267,22 +271,19 @@ int dsalt_reserve_slots(int32_t* block_tables, int n_seqs, int max_pages, const 
   const int most = (int)(sizeof(int32_t) * (3 * (size_t)SLOT_MAX_SEQS + 1));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int shift = shift_of(page_size);
-  // one block of 256 threads is quicker round its barriers than one of 1024; with more rows than
-  // it takes at once the larger one is
-  const bool fill = n_tokens <= SLOT_FILL_MAX, wide = n_seqs > 256 || n_tokens > 512;
+  const bool fill = n_tokens <= SLOT_FILL_MAX;
+  // one block of 256 threads is quicker round its barriers than one of 1024 (64 rows of a decode
+  // step 3.8 against 4.6 us); with more rows or tokens than it takes at once the larger one is
+  // (512 rows 7.4 against 21.8)
+  const bool wide = n_seqs > 256 || n_tokens > 512;
   static std::atomic<uint64_t> ready[3];
-#define DSALT_RESERVE(N, F, R)                                                                                       \
-  do {                                                                                                               \
-    if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(reserve_slots_kernel<N, F>), most, ready[R]))      \
-      return rc;                                                                                                     \
-    reserve_slots_kernel<N, F><<<1, N, smem, st>>>(block_tables, n_seqs, max_pages, seq_lens, new_lens, free_pages,  \
-                                                   (int)free_capacity, n_free, shift, n_tokens, slots, positions,    \
-                                                   cu_new, granted, seq_lens_out, n_free_out);                       \
-  } while (0)
-  if (!fill) DSALT_RESERVE(1024, false, 0);
-  else if (wide) DSALT_RESERVE(1024, true, 1);
-  else DSALT_RESERVE(256, true, 2);
-#undef DSALT_RESERVE
+  const auto kernel = !fill ? reserve_slots_kernel<SLOT_THREADS, false>
+                      : wide ? reserve_slots_kernel<SLOT_THREADS, true>
+                             : reserve_slots_kernel<256, true>;
+  if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), most, ready[!fill ? 0 : wide ? 1 : 2])) return rc;
+  kernel<<<1, fill && !wide ? 256 : SLOT_THREADS, smem, st>>>(block_tables, n_seqs, max_pages, seq_lens, new_lens, free_pages,
+                                        (int)free_capacity, n_free, shift, n_tokens, slots, positions, cu_new, granted,
+                                        seq_lens_out, n_free_out);
   if (int rc = check_cuda(cudaGetLastError(), "reserve_slots launch")) return rc;
   if (fill) return DSALT_OK;
   cudaLaunchAttribute attr[1];
@@ -309,7 +310,7 @@ int dsalt_release_slots(int32_t* block_tables, int n_seqs, int max_pages, int32_
   if (!block_tables || !seq_lens || !release || (free_capacity > 0 && !free_pages) || !n_free)
     return fail(DSALT_ERR_INVALID, "release_slots: null pointer");
   const size_t smem = sizeof(int32_t) * (size_t)n_seqs;  // at most 32 KB
-  release_slots_kernel<1024><<<1, 1024, smem, reinterpret_cast<cudaStream_t>(stream)>>>(
+  release_slots_kernel<<<1, SLOT_THREADS, smem, reinterpret_cast<cudaStream_t>(stream)>>>(
       block_tables, n_seqs, max_pages, seq_lens, release, free_pages, (int)free_capacity, n_free, shift_of(page_size));
   return check_cuda(cudaGetLastError(), "release_slots launch");
 }
