@@ -120,7 +120,7 @@ __device__ __forceinline__ float scale_log(float s) { return (float)((int)(__flo
 
 // query of sequence s: tokens, keys and the tiles of 32 that they make
 struct SeqPlan {
-  int q0, n_q, len, lo32, n_window, n_lmk;  // lo32: first key of the first window tile
+  int q0, n_q, len, n_window, n_lmk;  // tiles of one row tile, at most
 };
 __device__ __forceinline__ int first_key(const CacheAttnArgs& a, int t, int pos) {
   if (!a.w) return 0;
@@ -128,9 +128,12 @@ __device__ __forceinline__ int first_key(const CacheAttnArgs& a, int t, int pos)
   return max(pos - w + 1, 0);  // no overflow: pos < 2^31, w >= 1
 }
 // The rows of a kv head go head by head, each head's tokens after one another: a tile meets the
-// landmarks of few heads, where token by token it would meet those of all. How many at most:
-__device__ __forceinline__ int tile_heads(const CacheAttnArgs& a, int n_q) {
-  return n_q > 0 ? min(a.G, (CA_ROWS - 2) / n_q + 2) : 0;
+// landmarks of few heads, where token by token it would meet those of all. From 8 tokens on a
+// head has tiles of its own, each with the windows of 8 neighbours.
+__device__ __forceinline__ int head_rows(int n_q) { return n_q < CA_ROWS ? n_q : (n_q + CA_ROWS - 1) & ~(CA_ROWS - 1); }
+__device__ __forceinline__ int tile_heads(const CacheAttnArgs& a, int n_q) {  // of one tile, at most
+  if (n_q <= 1) return n_q <= 0 ? 0 : min(a.G, CA_ROWS);
+  return n_q >= CA_ROWS ? 1 : min(a.G, n_q == 2 || n_q == 4 ? CA_ROWS / n_q : (CA_ROWS - 2) / n_q + 2);
 }
 // (lane, lanes: who looks at which of the tokens; the lanes' findings are joined)
 __device__ __forceinline__ SeqPlan plan_of(const CacheAttnArgs& a, int s, int lane = 0, int lanes = 1) {
@@ -138,7 +141,7 @@ __device__ __forceinline__ SeqPlan plan_of(const CacheAttnArgs& a, int s, int la
   p.q0 = a.cu_q ? min(max(a.cu_q[s], 0), a.T) : s;
   p.n_q = a.cu_q ? max(min(a.cu_q[s + 1], a.T) - p.q0, 0) : 1;
   p.len = min(max(a.seq_lens[s], 0), a.max_pages << a.page_shift);
-  int lo = p.len, top = 0;
+  int lo = p.len, top = 0, span = 0;
   if (!a.w) lo = 0;
   else for (int r = lane; r < p.n_q; r += lanes) {
     const int pos = p.len - p.n_q + r;
@@ -146,18 +149,21 @@ __device__ __forceinline__ SeqPlan plan_of(const CacheAttnArgs& a, int s, int la
     const int f = first_key(a, p.q0 + r, pos);
     lo = min(lo, f);
     top = max(top, f);
+    span = max(span, pos + 1 - f);
   }
   if (lanes > 1) {
     lo = __reduce_min_sync(0xffffffffu, lo);
     top = __reduce_max_sync(0xffffffffu, top);
+    span = __reduce_max_sync(0xffffffffu, span);
   }
-  // the last key is the sequence's last: tiles behind a row tile's own keys are passed over
-  p.lo32 = lo & ~31;
-  p.n_window = p.n_q > 0 && p.len > 0 ? (p.len - p.lo32 + 31) >> 5 : 0;
+  // tiles of 32 keys from the first key on, to the sequence's last; 8 neighbours have at most
+  // span + 7 keys
+  p.n_window = p.n_q > 0 && p.len > 0 ? (p.len - (lo & ~31) + 31) >> 5 : 0;
+  if (a.w && p.n_q >= CA_ROWS) p.n_window = min(p.n_window, (span + (CA_ROWS - 1) + 30) / 32 + 1);
   p.n_lmk = a.k_lmk > 0 && top > 0 ? tile_heads(a, p.n_q) * ((a.k_lmk + 31) >> 5) : 0;  // none lies before a window from 0
   return p;
 }
-__device__ __forceinline__ int row_tiles(const CacheAttnArgs& a, int n_q) { return (n_q * a.G + CA_ROWS - 1) / CA_ROWS; }
+__device__ __forceinline__ int row_tiles(const CacheAttnArgs& a, int n_q) { return (head_rows(n_q) * a.G + CA_ROWS - 1) / CA_ROWS; }
 
 // sums of two numbers over the block's threads, exclusive; totals in `all`
 template <int WARPS>
@@ -188,6 +194,8 @@ __device__ __forceinline__ int chunk_of(long long tiles, long long items, int sl
   const long long want = items < slots ? max(slots - items, (long long)slots / 4) : slots;
   return (int)min(max((tiles + want - 1) / want, (long long)CA_MIN_TILES), 0x7fffffffLL);
 }
+
+__device__ __forceinline__ int parts_of(int tiles, int chunk) { return max(1, (tiles + chunk - 1) / chunk); }
 
 // The schedule of many sequences or tokens, made once: for few, each block's own takes less time
 // than a launch; its time grows with their number, in every block.
@@ -231,7 +239,7 @@ __global__ void __launch_bounds__(CP_THREADS) cache_attn_plan_kernel(CacheAttnAr
   for (int i = 0; i < MINE; ++i) {
     if (i * CP_THREADS >= a.n_seqs) break;
     const int s = i * CP_THREADS + tid;
-    const int splits = max(1, (len[i] + chunk - 1) / chunk);
+    const int splits = parts_of(len[i], chunk);
     const int2 v = make_int2(count[i] * splits, splits > 1 ? count[i] * splits : 0);
     int2 all;
     const int2 b = block_before2<CP_THREADS / 32>(v, red, all);
@@ -305,7 +313,7 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
         s_job.plan = a.plans[lo];
         s_job.s = lo;
         s_job.local = unit - from.x;
-        s_job.splits = max(1, (s_job.plan.n_window + s_job.plan.n_lmk + head.x - 1) / head.x);
+        s_job.splits = parts_of(s_job.plan.n_window + s_job.plan.n_lmk, head.x);
         s_job.cut = from.y;
       }
     }
@@ -345,7 +353,7 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
       int splits = 1;
       if (s < a.n_seqs) {
         const SeqPlan& p = s_plans[s];
-        splits = max(1, (p.n_window + p.n_lmk + chunk - 1) / chunk);
+        splits = parts_of(p.n_window + p.n_lmk, chunk);
         v.x = row_tiles(a, p.n_q) * a.Hkv * splits;
         v.y = splits > 1 ? v.x : 0;
       }
@@ -388,21 +396,25 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
   const int each = (tiles + splits - 1) / splits;
   const int t_begin = min(split * each, tiles), t_end = min(t_begin + each, tiles);
 
-  const int n_rows = p.n_q * a.G, head0 = tile * CA_ROWS / p.n_q;  // first head of the tile
-  const int n_heads = (min(tile * CA_ROWS + CA_ROWS, n_rows) - 1) / p.n_q - head0 + 1;
+  // row r of the tile: head head0 + head_of(tok0 + r), token what is left
+  const int per_head = head_rows(p.n_q), n_rows = min(per_head * a.G - tile * CA_ROWS, CA_ROWS);
+  const int head0 = tile * CA_ROWS / per_head, tok0 = tile * CA_ROWS - head0 * per_head;
+  const int inverse = per_head < CA_ROWS ? (255 + per_head) / per_head : 0;  // exact for quotients of 14 and less
+  const auto head_of = [&](int x) { return per_head < CA_ROWS ? x * inverse >> 8 : 0; };
+  const int n_heads = head_of(tok0 + n_rows - 1) + 1;
   // ---- rows 2t, 2t+1 of the tile are this lane's in S^T and O^T
   int row_lo[2], row_hi[2], row_head[2];
   unsigned row_span[2], row_before[2];  // keys of the window; positions before it, where landmarks count
   bool row_ok[2];
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    const int i = tile * CA_ROWS + 2 * t + c, tok = i % p.n_q;
-    row_ok[c] = i < n_rows;
+    const int x = tok0 + 2 * t + c, head = head_of(x), tok = x - head * per_head;
+    row_ok[c] = 2 * t + c < n_rows && tok < p.n_q;
     const int pos = p.len - p.n_q + tok;
     const bool keys = row_ok[c] && pos >= 0;
     row_lo[c] = keys ? first_key(a, p.q0 + tok, pos) : 0x7fffffff;
     row_hi[c] = keys ? pos + 1 : 0;
-    row_head[c] = i / p.n_q - head0;
+    row_head[c] = head;
     row_span[c] = keys ? row_hi[c] - row_lo[c] : 0;
     row_before[c] = keys ? row_lo[c] : 0;
   }
@@ -426,11 +438,11 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
   const int w0 = min(t_begin, p.n_window), w1 = min(t_end, p.n_window);
   const int l1 = min(max(t_end - p.n_window, 0), n_heads * lmk32), l0 = min(max(t_begin - p.n_window, 0), l1);
   const int wq = (w1 - w0 + CA_WARPS - 1) / CA_WARPS, lq = (l1 - l0 + CA_WARPS - 1) / CA_WARPS;
-  int wb = min(w0 + warp * wq, w1), we = min(wb + wq, w1);
+  const int wb = min(w0 + warp * wq, w1);
+  int we = min(wb + wq, w1);
   const int lb = min(l0 + warp * lq, l1), le = min(lb + lq, l1);
-  // (keys of the sequence's other row tiles are passed over)
-  wb = max(wb, min(we, (lo_min < p.len ? lo_min - p.lo32 : 0x7fffffe0) >> 5));
-  we = min(we, max(wb, (hi_max - p.lo32 + 31) >> 5));
+  const int lo32 = lo_min < p.len ? lo_min & ~31 : 0;  // window tiles begin here
+  we = min(we, max(wb, (hi_max - lo32 + 31) >> 5));
   const int n_w = we - wb, n = n_w + le - lb;
 
   // where keys lie: of 16 window tiles ahead a lane per half, of the next landmark tile a lane per key
@@ -451,7 +463,7 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
   auto find_window = [&](int i) {  // lane: half lane & 1 of tile wb + i + lane / 2
     Where o;
     o.add = 0.f;
-    o.key = i + (lane >> 1) < n_w ? p.lo32 + (wb + i) * 32 + lane * 16 : -1;
+    o.key = i + (lane >> 1) < n_w ? lo32 + (wb + i) * 32 + lane * 16 : -1;
     o.page = page_of(o.key);
     return o;
   };
@@ -478,10 +490,10 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
     float x[D / 4];
 #pragma unroll
     for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
-    const int i = tile * CA_ROWS + g;
-    if (i < n_rows) {
-      const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)(p.q0 + i % p.n_q) * a.q_stride +
-                     (int64_t)(hk * a.G + i / p.n_q) * D + t * 16;
+    const int head = head_of(tok0 + g), tok = tok0 + g - head * per_head;
+    if (g < n_rows && tok < p.n_q) {
+      const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)(p.q0 + tok) * a.q_stride +
+                     (int64_t)(hk * a.G + head0 + head) * D + t * 16;
 #pragma unroll
       for (int b = 0; b < D / 64; ++b) {
         if constexpr (sizeof(T) == 4) {
@@ -695,7 +707,7 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
       }
     }
     // ---- P = 2^(x + e - M + 14), l += 2^(x - m)
-    const int key0 = p.lo32 + (wb + i) * 32, slot = slot_of(g);
+    const int key0 = lo32 + (wb + i) * 32, slot = slot_of(g);
     float4 mh[2] = {meta[0], meta[16]};  // of a window tile's halves; .y: exponent of V's scale
     const bool whole = window && key0 >= lo_max && key0 + 32 <= hi_min && __float_as_int(mh[0].w) >= 0 &&
                        __float_as_int(mh[1].w) >= 0;  // every row attends to every key
@@ -899,8 +911,8 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
   __syncthreads();
   for (int e = tid; e < CA_ROWS * D; e += CA_THREADS) {
     const int r = e / D, d = e % D;
-    const int i = tile * CA_ROWS + r, tok = i % p.n_q, h = hk * a.G + i / p.n_q;
-    if (i >= n_rows) continue;
+    const int head = head_of(tok0 + r), tok = tok0 + r - head * per_head, h = hk * a.G + head0 + head;
+    if (r >= n_rows || tok >= p.n_q) continue;
     float m = -INFINITY, M = -INFINITY;
 #pragma unroll
     for (int x = 0; x < CA_WARPS; ++x) {
@@ -936,8 +948,9 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
   }
 }
 
-// Joins the parts of the rows that were cut, a block per row (or several rows after one
-// another). The order of every sum is fixed by the parts' numbers: the result does not depend
+// Joins the parts of the rows that were cut: of few parts by a warp, of many by the block, one row
+// after another. (256 rows of 27 parts, a block each: 40.8 us with the attention, by warps 43.5;
+// 2576 rows of two parts, five to a block: 24.1 us, by warps 22.0.) The order of every sum is fixed by the parts' numbers: the result does not depend
 // on which finished first.
 constexpr int CJ_THREADS = 256;
 template <int D>
@@ -959,9 +972,53 @@ __global__ void __launch_bounds__(CJ_THREADS) cache_attn_join_kernel(CacheAttnAr
     s_part[tid] = cut ? rp : make_int2(0, 0);
   }
   if (!__syncthreads_or(cut)) return;
-  for (int64_t row = row0; row < min(row0 + rows_per_block, rows); ++row) {
+  const auto put = [&](int64_t at, float v) {
+    if (a.out_dtype == DSALT_F32) reinterpret_cast<float*>(a.out)[at] = v;
+    else if (a.out_dtype == DSALT_BF16) reinterpret_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
+    else reinterpret_cast<__half*>(a.out)[at] = __float2half_rn(v);
+  };
+  const int here = (int)min((int64_t)rows_per_block, rows - row0), few = min(32, 8 * rows_per_block);
+  for (int r = warp; r < here; r += CJ_THREADS / 32) {
+    const int2 rp = s_part[r];
+    if (rp.y == 0 || rp.y > few) continue;
+    float4 v = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+    if (lane < rp.y) v = reinterpret_cast<const float4*>(a.part_s)[rp.x + lane * CA_ROWS];
+    float m = v.x, M = v.z;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    }
+    const float mu = m == -INFINITY ? 0.f : m, Mu = M == -INFINITY ? 0.f : M;
+    float l = v.y * exp2_fast(v.x - mu);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    const float weight = exp2_fast(v.z - Mu);
+    const float2* po = reinterpret_cast<const float2*>(a.part_o + (int64_t)rp.x * D) + lane;
+    float2 sum[D / 64];
+#pragma unroll
+    for (int d = 0; d < D / 64; ++d) sum[d] = make_float2(0.f, 0.f);
+#pragma unroll 4
+    for (int x = 0; x < rp.y; ++x) {
+      const float w = __shfl_sync(0xffffffffu, weight, x);
+#pragma unroll
+      for (int d = 0; d < D / 64; ++d) {
+        const float2 y = po[(int64_t)x * (CA_ROWS * D / 2) + d * 32];
+        sum[d].x += y.x * w, sum[d].y += y.y * w;
+      }
+    }
+    const float f = l == 0.f ? 0.f : exp2_fast(Mu - mu - CA_P_SHIFT) / l;
+    const int64_t row = row0 + r;
+#pragma unroll
+    for (int d = 0; d < D / 64; ++d) {
+      put(row * D + d * 64 + 2 * lane, l == 0.f ? 0.f : sum[d].x * f);
+      put(row * D + d * 64 + 2 * lane + 1, l == 0.f ? 0.f : sum[d].y * f);
+    }
+    if (lane == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  }
+  for (int64_t row = row0; row < row0 + here; ++row) {
     const int2 rp = s_part[row - row0];
-    if (rp.y == 0) continue;
+    if (rp.y <= few) continue;
     const float4* ps = reinterpret_cast<const float4*>(a.part_s) + rp.x;
     float m = -INFINITY, M = -INFINITY;
     for (int x = tid; x < rp.y; x += CJ_THREADS) {
@@ -1010,10 +1067,7 @@ __global__ void __launch_bounds__(CJ_THREADS) cache_attn_join_kernel(CacheAttnAr
       float sum = 0.f;
 #pragma unroll
       for (int x = 0; x < GROUPS; ++x) sum += reinterpret_cast<const float*>(&s_v[x][0])[tid];
-      const float res = l == 0.f ? 0.f : sum * exp2_fast(Mu - mu - CA_P_SHIFT) / l;
-      if (a.out_dtype == DSALT_F32) reinterpret_cast<float*>(a.out)[row * D + tid] = res;
-      else if (a.out_dtype == DSALT_BF16) reinterpret_cast<__nv_bfloat16*>(a.out)[row * D + tid] = __float2bfloat16_rn(res);
-      else reinterpret_cast<__half*>(a.out)[row * D + tid] = __float2half_rn(res);
+      put(row * D + tid, l == 0.f ? 0.f : sum * exp2_fast(Mu - mu - CA_P_SHIFT) / l);
     }
     if (tid == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
     __syncthreads();  // the shared arrays are used again
@@ -1023,7 +1077,10 @@ __global__ void __launch_bounds__(CJ_THREADS) cache_attn_join_kernel(CacheAttnAr
 static inline size_t ca_a256(size_t v) { return (v + 255) & ~(size_t)255; }
 // is the schedule made by a kernel of its own?
 static inline bool ca_plans(int64_t T, int n_seqs) { return n_seqs > CA_OWN_SCHED || T - n_seqs > CA_OWN_ROWS; }
-static inline int64_t ca_items(int64_t T, int n_seqs, int G, int Hkv) { return ((T * G + (CA_ROWS - 1) * (int64_t)n_seqs) / CA_ROWS + 1) * Hkv; }
+// items of the kernel at most: from 8 tokens on a sequence's heads are filled up to whole tiles
+static inline int64_t ca_items(int64_t T, int n_seqs, int G, int Hkv) {
+  return ((T * G + (CA_ROWS - 1) * (n_seqs + G * std::min<int64_t>(n_seqs, T / CA_ROWS))) / CA_ROWS + 1) * Hkv;
+}
 
 template <typename T, int D, int NS>
 static int launch_cache_attn(const CacheAttnArgs& a, unsigned grid, bool join, cudaStream_t stream) {
