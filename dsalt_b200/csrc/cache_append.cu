@@ -16,8 +16,15 @@
 // the first of them. One group of lanes owns a run of one head: it takes amax, settles e,
 // rewrites the older bytes if e grew and writes the new ones, so nothing is exchanged between
 // groups. A decode step is all runs of one token: D/8 lanes each, so that a warp holds
-// 4 (2) heads at once. A prompt is runs of P tokens: a warp each, which keeps up to 64
-// vectors per row of lanes in registers between the two passes.
+// 4 (2) heads at once. A prompt is runs of P tokens: a warp each, which reads a run in chunks of
+// 8 vectors per lane (4 of fp32), keeps the last one between the two passes and takes the others
+// from L1 or L2 again.
+//
+// Measured on a B200 (device time): 4 prompts of 8192 tokens, 12 heads of 64 in bf16 with pages of
+// 64 (132 MB: the prompts are ragged) 29.7 us (4.5 TB/s; copying as much takes 20.5): bound by memory and by the chain
+// that each block goes through (slots, runs, first pass, second pass), which the other two
+// blocks of an SM cover; without the fetches to L2 it takes 34.1 us. 64 decode rows of 16 heads
+// 3.1 us, next to nothing of which is bytes.
 #include <algorithm>
 #include <type_traits>
 
@@ -384,8 +391,9 @@ extern "C" int dsalt_append_cache(const void* k, const void* v, int dtype, int64
   a.v = {v, reinterpret_cast<uint8_t*>(v_cache), v_scale, v_token_stride, v_head_stride};
   a.slots = slots, a.T = T, a.n_pages = n_pages, a.n_kv = n_kv;
   a.page_shift = page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7;
-  // few tokens: small windows, so that a decode step's runs spread over the GPU; many: larger
-  // ones, so that fewer blocks find no run. Planes are shared out until there are blocks enough
+  // few tokens: small windows, so that a decode step's runs spread over the GPU (512 rows of 12 heads
+  // 4.6 us, in windows of 64 13.2); many: larger ones, so that fewer blocks find no run (4096
+  // tokens of a prompt 6.2 us, in windows of 8 9.7). Planes are shared out until there are blocks enough
   // (or each has no more planes than warps).
   a.window = T <= 2048 ? 8 : page_size >= 64 ? 64 : 32;
   const int64_t windows = (T + a.window - 1) / a.window;

@@ -21,8 +21,8 @@
 //   term, errors of either sign); fp32 queries take Q and P as two fp16 terms each (22 bits).
 // * the tensor cores cut off what does not fit a sum's 24 bits, which over a long cache adds up
 //   (3.4e-4 of the result after 4096 products in a row); so O is added up by them over
-//   CA_CHAIN tiles at most and then, rounded, to an array in local memory (1e-6 remains), for
-//   fp32 queries over 16 keys only.
+//   CA_CHAIN tiles at most and then, with rounding, to a sum in shared memory (local memory
+//   where head_dim 128 leaves no room; 2e-6 remains), for fp32 queries over 16 keys only.
 // The scales of V differ from page to page, so a row keeps two maxima: m of x for the
 // denominator l = sum 2^(x - m), and M of x + e for the numerator O = sum 2^(x + e - M) byte;
 // out = O 2^(M - m) / l. Neither can overflow whatever the scales are.
@@ -33,6 +33,15 @@
 // call follows them); the parts of an item that was cut are joined by a second kernel.
 // Within a unit each of two warps has its own stretch of tiles and its own ring of
 // cp.async stages: nothing but the end is shared, so no warp waits for another.
+//
+// Measured on a B200 (device time): one row of 131072 keys over 16 heads of 64 in bf16, 268 MB,
+// 53 us (5.1 TB/s; copying as much takes 41.6); 16 rows of up to 32768 keys, 8 heads to a kv head
+// of 128, 174 MB, 40.6 us (4.3 TB/s); 64 rows with windows up to 512 and 128 landmarks 25 us.
+// About 10 us of a call are the schedule and the queries (4), the warps' joining and the second
+// kernel. Inside the loop no pipe is full (issue 39 %, ALU 40 %, tensor 15 %, DRAM 51 % of the
+// 16 rows' time, shared by all of it): a tile of 32 keys is a chain of copy, widening, product,
+// exponential and product that takes a warp about 1.5 us, and registers end the number of
+// warps that could overlap it.
 #include <algorithm>
 #include <type_traits>
 
@@ -40,18 +49,28 @@
 
 namespace dsalt {
 
+// Warps of a unit. Four (and half as many units) take 28.2 us against 25.1 for 64 rows with
+// landmarks and 42.4 against 40.6 for 16 rows of 32768 keys, and win 1.7 us for a row alone.
 constexpr int CA_WARPS = 2;
 constexpr int CA_THREADS = 32 * CA_WARPS;
-constexpr int CA_MIN_TILES = 8;        // tiles of 32 keys that a unit takes at least: four per warp
+// tiles of 32 keys that a unit takes at least: four per warp (drafts of 23 rows: 24.3 us; 12 tiles
+// 25.8, 16 tiles 27.7, before the join was made cheaper)
+constexpr int CA_MIN_TILES = 8;
 constexpr int CA_MAX_SEQS = 8192;
-constexpr int CA_OWN_SCHED = 192;      // sequences up to which every block makes the schedule for itself,
-constexpr int CA_OWN_ROWS = 1024;      // and query tokens beyond one of each
+// Sequences, and query tokens beyond one of each, up to which every block makes the schedule for
+// itself: 129 rows 30.8 us (by a kernel of its own 37.2), 200 rows 47.4 (48.3), 400 rows 103.9
+// (84.5); 32 rows of 40 tokens 78.3 (48.4), 8 of 128 take 41 either way.
+constexpr int CA_OWN_SCHED = 192;
+constexpr int CA_OWN_ROWS = 1024;
 constexpr int CA_ERR_PAGE = 41;        // device status: a page number outside the pool was met
 constexpr float CA_P_SHIFT = 14.f;     // P is held times 2^14: fp16 stays normal down to 2^-28
-constexpr int CA_CHAIN = 64;            // tiles that O is added up over by the tensor cores alone
+constexpr int CA_CHAIN = 64;           // tiles that O is added up over by the tensor cores alone
 constexpr float CA_SLACK = 1.f;        // P may exceed 2^14 by 2^1 before its reference moves (fp16 ends at 2^16)
 
-// blocks per SM that registers and rings allow; one round of them is the number of units wanted
+// Blocks per SM that registers and rings allow; one round of them is the number of units wanted.
+// Two stages: a third costs blocks, and at head_dim 64 with 7 of them one row of 131072 keys
+// takes 57.1 us against 54.2, with 6 of them 52.2 but 64 rows 33.9 against 25.2; at head_dim 128
+// with 4 of them 41.9 us against 40.8.
 template <int D>
 struct Shape {
   static constexpr int OCC = D == 64 ? 8 : 6;
@@ -114,7 +133,6 @@ __device__ __forceinline__ uint32_t widen_hi(uint32_t v) {
   asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, h;}" : "=r"(r) : "r"(v));
   return r;
 }
-__device__ __forceinline__ float exp2_fast(float x) { return ex2_approx(x); }
 // e of a scale 2^e, as a float; 0 (a page never written) as the lowest
 __device__ __forceinline__ float scale_log(float s) { return (float)((int)(__float_as_uint(s) >> 23 & 0xff) - 127); }
 
@@ -635,8 +653,8 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
         gM = fmaxf(gM, __shfl_xor_sync(0xffffffffu, gM, x));
       }
       const float m = fmaxf(st[c].m, gm), M = fmaxf(st[c].M, gM);
-      st[c].l *= m == -INFINITY ? 1.f : exp2_fast(st[c].m - m);
-      const float corr = M == -INFINITY ? 1.f : exp2_fast(st[c].M - M);
+      st[c].l *= m == -INFINITY ? 1.f : ex2_approx(st[c].m - m);
+      const float corr = M == -INFINITY ? 1.f : ex2_approx(st[c].M - M);
       st[c].m = m;
       st[c].M = M;
 #pragma unroll
@@ -663,7 +681,7 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
   [[maybe_unused]] const auto put_by = [&](bool first, bool all) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const float corr = first || st[c].M == -INFINITY ? 1.f : exp2_fast(far_M[c] - st[c].M);
+      const float corr = first || st[c].M == -INFINITY ? 1.f : ex2_approx(far_M[c] - st[c].M);
 #pragma unroll
       for (int x = 0; x < MT; ++x)
 #pragma unroll
@@ -759,9 +777,9 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float shift = mh[h].y - Mu[c] + CA_P_SHIFT;
-            sc[h][c] = exp2_fast(fmaf(sc[h][c], f[c][h], shift));
-            sc[h][2 + c] = exp2_fast(fmaf(sc[h][2 + c], f[c][h], shift));
-            st[c].l = fmaf(sc[h][c] + sc[h][2 + c], exp2_fast(-shift - mu[c]), st[c].l);
+            sc[h][c] = ex2_approx(fmaf(sc[h][c], f[c][h], shift));
+            sc[h][2 + c] = ex2_approx(fmaf(sc[h][2 + c], f[c][h], shift));
+            st[c].l = fmaf(sc[h][c] + sc[h][2 + c], ex2_approx(-shift - mu[c]), st[c].l);
           }
       } else {
 #pragma unroll
@@ -798,8 +816,8 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
             const float x = sc[h][2 * b + c];
-            st[c].l += exp2_fast(x - mu);
-            sc[h][2 * b + c] = exp2_fast(x + ve[h][b] - Mu + CA_P_SHIFT);
+            st[c].l += ex2_approx(x - mu);
+            sc[h][2 * b + c] = ex2_approx(x + ve[h][b] - Mu + CA_P_SHIFT);
           }
       }
     }
@@ -923,12 +941,12 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
     float l = 0.f, v = 0.f;
 #pragma unroll
     for (int x = 0; x < CA_WARPS; ++x) {
-      l += s_l[x][r] * exp2_fast(s_m[x][r] - mu);
-      v += s_o[(x * CA_ROWS + r) * D + d] * exp2_fast(s_M[x][r] - Mu);
+      l += s_l[x][r] * ex2_approx(s_m[x][r] - mu);
+      v += s_o[(x * CA_ROWS + r) * D + d] * ex2_approx(s_M[x][r] - Mu);
     }
     const int64_t row = (int64_t)(p.q0 + tok) * a.H + h;
     if (splits == 1) {
-      const float res = l == 0.f ? 0.f : v * exp2_fast(Mu - mu - CA_P_SHIFT) / l;
+      const float res = l == 0.f ? 0.f : v * ex2_approx(Mu - mu - CA_P_SHIFT) / l;
       if (a.out_dtype == DSALT_F32) reinterpret_cast<float*>(a.out)[row * D + d] = res;
       else if (a.out_dtype == DSALT_BF16) reinterpret_cast<__nv_bfloat16*>(a.out)[row * D + d] = __float2bfloat16_rn(res);
       else reinterpret_cast<__half*>(a.out)[row * D + d] = __float2half_rn(res);
@@ -950,8 +968,8 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
 
 // Joins the parts of the rows that were cut: of few parts by a warp, of many by the block, one row
 // after another. (256 rows of 27 parts, a block each: 40.8 us with the attention, by warps 43.5;
-// 2576 rows of two parts, five to a block: 24.1 us, by warps 22.0.) The order of every sum is fixed by the parts' numbers: the result does not depend
-// on which finished first.
+// 2576 rows of two parts, five to a block: 24.1 us, by warps 22.0.) The order of every sum is
+// fixed by the parts' numbers: the result does not depend on which finished first.
 constexpr int CJ_THREADS = 256;
 template <int D>
 __global__ void __launch_bounds__(CJ_THREADS) cache_attn_join_kernel(CacheAttnArgs a, int rows_per_block) {
@@ -990,10 +1008,10 @@ __global__ void __launch_bounds__(CJ_THREADS) cache_attn_join_kernel(CacheAttnAr
       M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     }
     const float mu = m == -INFINITY ? 0.f : m, Mu = M == -INFINITY ? 0.f : M;
-    float l = v.y * exp2_fast(v.x - mu);
+    float l = v.y * ex2_approx(v.x - mu);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    const float weight = exp2_fast(v.z - Mu);
+    const float weight = ex2_approx(v.z - Mu);
     const float2* po = reinterpret_cast<const float2*>(a.part_o + (int64_t)rp.x * D) + lane;
     float2 sum[D / 64];
 #pragma unroll
@@ -1007,7 +1025,7 @@ __global__ void __launch_bounds__(CJ_THREADS) cache_attn_join_kernel(CacheAttnAr
         sum[d].x += y.x * w, sum[d].y += y.y * w;
       }
     }
-    const float f = l == 0.f ? 0.f : exp2_fast(Mu - mu - CA_P_SHIFT) / l;
+    const float f = l == 0.f ? 0.f : ex2_approx(Mu - mu - CA_P_SHIFT) / l;
     const int64_t row = row0 + r;
 #pragma unroll
     for (int d = 0; d < D / 64; ++d) {
@@ -1043,8 +1061,8 @@ __global__ void __launch_bounds__(CJ_THREADS) cache_attn_join_kernel(CacheAttnAr
     float l = 0.f;
     for (int x = tid; x < rp.y; x += CJ_THREADS) {
       const float4 v = ps[(int64_t)x * CA_ROWS];
-      l += v.y * exp2_fast(v.x - mu);
-      s_w[x] = exp2_fast(s_w[x] - Mu);
+      l += v.y * ex2_approx(v.x - mu);
+      s_w[x] = ex2_approx(s_w[x] - Mu);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
@@ -1067,7 +1085,7 @@ __global__ void __launch_bounds__(CJ_THREADS) cache_attn_join_kernel(CacheAttnAr
       float sum = 0.f;
 #pragma unroll
       for (int x = 0; x < GROUPS; ++x) sum += reinterpret_cast<const float*>(&s_v[x][0])[tid];
-      put(row * D + tid, l == 0.f ? 0.f : sum * exp2_fast(Mu - mu - CA_P_SHIFT) / l);
+      put(row * D + tid, l == 0.f ? 0.f : sum * ex2_approx(Mu - mu - CA_P_SHIFT) / l);
     }
     if (tid == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
     __syncthreads();  // the shared arrays are used again

@@ -30,6 +30,15 @@
 //
 // One cluster of C blocks owns a row, each a share of it. The row comes from HBM once; later
 // passes find it in L1 or L2, which hold it for all rows under way.
+//
+// Measured on a B200 (device time, 64 rows of 151936 in bf16, 19 MB): the largest logit 9.9 us,
+// temperature alone 27.7, top-k 50 19.8, top-p 0.9 88, every row its own settings 95. Bytes are
+// 3 us of each. Temperature alone is bound by the 64-bit instructions of the weights (11 per
+// element), the draws of a wide nucleus by latency: some ten steps of one cluster one after
+// another, of which the pass over the bins takes 15 us, the queue 11, the histogram and its
+// joining 14, list and sort 14. Measured and not kept: a rough pass in 32 bits before one exact
+// pass that also queues (107 us for top-p 0.9: the queue's places cost more beside the
+// weights than in a pass of their own), queues per lane (112), queues by votes (93).
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -984,9 +993,11 @@ extern "C" int dsalt_sample(const void* logits, int dtype, int64_t B, int64_t V,
   if (!logits || !u || !token) return fail(DSALT_ERR_INVALID, "sample: null pointer");
   const int es = dtype == DSALT_F32 ? 4 : 2;
   if ((uintptr_t)logits % es) return fail(DSALT_ERR_INVALID, "sample: logits not aligned to their type");
-  // blocks per row: as many as leave every row's cluster resident at once (two blocks per
-  // SM), more where the decisive bin of a share would overrun the warps' queues; a small row is
-  // one block's
+  // Blocks per row: as many as leave every row's cluster resident at once (two blocks per SM; 64
+  // rows of 151936, top-p 0.9, by 4 blocks 91 us, by 8 129), more where the decisive bin of a share
+  // would overrun the warps' queues. A share below 2048 does not pay (a row of 4096, top-p 0.9, by
+  // one block 28.0 us with shares of 2048, 30.6 with 512; a row of 50257 by shares of 8192 42.9
+  // against 36.1).
   int C = 1;
   while (C < 8 && ((V / (2 * C) >= 2048 && B * (2 * C) <= 148 * 2) || V / C > 80000)) C *= 2;
   SampleArgs a;
