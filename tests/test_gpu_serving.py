@@ -707,6 +707,58 @@ def test_a_captured_decode_step_follows_the_state(V):
     assert status() == 0
 
 
+def test_offsets_beyond_32_bits(V):
+    # a cache of more than 2^32 bytes a side, tokens and rows more than 2^31 elements apart
+    Hkv, page, D = 2, 128, 128
+    n_pages = (1 << 32) // (Hkv * page * D) + 3
+    ids = [n_pages - 1, n_pages // 2 + 1, n_pages - 2, 0]
+    big = [torch.empty(n_pages, Hkv, page, D, dtype=torch.uint8, device="cuda").view(F8) for _ in range(2)]
+    big += [torch.zeros(n_pages, Hkv, device="cuda") for _ in range(2)]
+    small = [torch.empty(4, Hkv, page, D, dtype=torch.uint8, device="cuda").view(F8) for _ in range(2)]
+    small += [torch.zeros(4, Hkv, device="cuda") for _ in range(2)]
+    T = 4 * page - 5
+    g = torch.Generator(device="cuda").manual_seed(11)
+    k, v = (torch.randn(T, Hkv, D, device="cuda", generator=g).to(torch.bfloat16) for _ in range(2))
+    within = torch.arange(T, device="cuda") % page
+    slots = lambda pages: torch.tensor(pages, device="cuda")[torch.arange(T, device="cuda") // page] * page + within  # noqa: E731
+    V.append_cache(k, v, *big, slots(ids))
+    V.append_cache(k, v, *small, slots([0, 1, 2, 3]))
+    for a, b in zip(big, small):
+        a = a.view(torch.uint8) if a.dtype == F8 else a
+        b = b.view(torch.uint8) if b.dtype == F8 else b
+        for i, p in enumerate(ids):
+            n = min(page, T - i * page)
+            assert torch.equal(a[p][:, :n] if a.dim() == 4 else a[p], b[i][:, :n] if b.dim() == 4 else b[i])
+    q = torch.randn(1, 4, D, device="cuda", generator=g).to(torch.bfloat16)
+    lens = torch.tensor([T], dtype=torch.int32, device="cuda")
+    table = lambda pages: torch.tensor([pages], dtype=torch.int32, device="cuda")  # noqa: E731
+    w = torch.tensor([100], dtype=torch.int32, device="cuda")
+    lmk = torch.tensor([3, 130, 290], dtype=torch.int32, device="cuda").expand(4, 1, 3).contiguous()
+    for kw in ({}, dict(w_sizes=w, lmk_indices=lmk)):
+        assert torch.equal(V.cache_attention(q, *big, table(ids), lens, **kw),
+                           V.cache_attention(q, *small, table([0, 1, 2, 3]), lens, **kw))
+    del big
+    far = torch.empty((1 << 31) + 2 * 40 * 128, dtype=torch.bfloat16, device="cuda")
+    x = far.as_strided((2, 1, 64), (1 << 31, 64, 1))
+    x.copy_(torch.randn(2, 1, 64, device="cuda", generator=g))
+    caches = [[torch.zeros(2, 1, 16, 64, dtype=torch.uint8, device="cuda").view(F8) for _ in range(2)]
+              + [torch.zeros(2, 1, device="cuda") for _ in range(2)] for _ in range(2)]
+    at = torch.tensor([0, 16], device="cuda")
+    V.append_cache(x, x, *caches[0], at)
+    V.append_cache(x.contiguous(), x.contiguous(), *caches[1], at)
+    for a, b in zip(*caches):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    one = torch.tensor([1, 1], dtype=torch.int32, device="cuda")
+    tab = torch.tensor([[0], [1]], dtype=torch.int32, device="cuda")
+    assert torch.equal(V.cache_attention(x, *caches[0], tab, one), V.cache_attention(x.contiguous(), *caches[0], tab, one))
+    logits = far.as_strided((2, 5000), (1 << 31, 1))
+    logits.copy_(torch.randn(2, 5000, device="cuda", generator=g))
+    u = torch.tensor([0.3, 0.8], device="cuda")
+    for f in ({}, dict(top_k=50), dict(top_p=0.9)):
+        assert torch.equal(V.sample_tokens(logits, u, **f), V.sample_tokens(logits.contiguous(), u, **f))
+    assert status() == 0
+
+
 def test_serving_steps_together(V):
     """Admission, prompts, decode steps and release of several requests, each step checked."""
     g = np.random.default_rng(20)
