@@ -38,7 +38,8 @@
 // another, of which the pass over the bins takes 15 us, the queue 11, the histogram and its
 // joining 14, list and sort 14. Measured and not kept: a rough pass in 32 bits before one exact
 // pass that also queues (107 us for top-p 0.9: the queue's places cost more beside the
-// weights than in a pass of their own), queues per lane (112), queues by votes (93).
+// weights than in a pass of their own), queues per lane (112), queues by votes (93), queues
+// that hold the logits too (91).
 #include <cooperative_groups.h>
 
 #include <type_traits>
