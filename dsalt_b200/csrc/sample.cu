@@ -32,8 +32,8 @@
 // passes find it in L1 or L2, which hold it for all rows under way.
 //
 // Measured on a B200 (device time, 64 rows of 151936 in bf16, 19 MB): the largest logit 9.9 us,
-// temperature alone 27.7, top-k 50 19.8, top-p 0.9 88, every row its own settings 95. Bytes are
-// 3 us of each. Temperature alone is bound by the 64-bit instructions of the weights (11 per
+// temperature alone 26.9, top-k 50 19.8, top-p 0.9 88, every row its own settings 95. Bytes are
+// 3 us of each. Temperature alone is bound by the 64-bit instructions of the weights (10 per
 // element), the draws of a wide nucleus by latency: some ten steps of one cluster one after
 // another, of which the pass over the bins takes 15 us, the queue 11, the histogram and its
 // joining 14, list and sort 14. Measured and not kept: a rough pass in 32 bits before one exact
@@ -59,7 +59,7 @@ constexpr int IDX_BITS = 20;                  // vocabulary of at most 2^20
 constexpr int BLOCK_ELEMS = 256;              // a warp's step: eight consecutive elements per lane
 constexpr int MAX_SHARE = 131328;             // 2^20 / 8 and a skew, in whole steps: 513 of them
 constexpr int MAX_STEPS = (MAX_SHARE / BLOCK_ELEMS + SAMPLE_WARPS - 1) / SAMPLE_WARPS;  // of one warp
-constexpr int QUEUE = 1024;                   // elements of the decisive bin that a warp keeps
+constexpr int QUEUE = 992;                    // elements of the decisive bin that a warp keeps
 constexpr int MAX_GROUPS = 256;
 constexpr double MASS_ONE = 8796093022208.0;  // 2^43: 2^20 of them stay below 2^63
 constexpr float BIN_SPAN = 32.f;              // (m - l) / T that the joint histogram covers
@@ -108,7 +108,7 @@ struct SampleShared {
   float group_max[64], all_max[MAX_GROUPS];  // of 8 or 16 threads: this block's, the cluster's
   u64 share_mass, range[2], result[4];  // result: written by the leader only
   u64 warp_red[SAMPLE_WARPS];
-  double exp2_32[32];  // 2^(j / 32)
+  double exp2_128[128];  // 2^(j / 128)
 };
 
 // the block's own, by its shared-memory address (a pointer handed to a function would be generic)
@@ -127,10 +127,11 @@ __device__ __forceinline__ float logit_of(u64 c) {
   return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
 }
 
-// Weights of one row. 2^t, t = (l - m) log2(e) / T: t = k / 32 + g with |g| <= 1/64, then
-// 2^(k/32) from a table of 32 and the exponent, 2^g by its Taylor series to the fifth power
-// (the sixth term is below (ln 2 / 64)^6 / 6! = 2.3e-15). The passes are bound by instructions, and
-// one in 64 bits takes two turns: eleven of them here, no branch and no selection.
+// Weights of one row. 2^t, t = (l - m) log2(e) / T: t = k / 128 + g with |g| <= 1/256,
+// then 2^(k/128) from a table of 128 and the exponent, 2^g by its Taylor series to the fourth power
+// (the fifth term is below (ln 2 / 256)^5 / 5! = 1.3e-15). The passes are bound by instructions, and
+// one in 64 bits takes two turns: ten of them here, no branch and no selection (a table of 32 and
+// the fifth power: 27.7 us at temperature alone, 26.9 so).
 struct Weights {
   float top;    // the largest logit
   float floor;  // logits below it (and NaN) are taken as it
@@ -138,17 +139,16 @@ struct Weights {
   bool only_top;   // +inf: equal ones have weight 1, all others none
   bool vanishing;  // the floor's weight rounds to no mass (else -inf and NaN have to be left out)
   __device__ __forceinline__ double finite(float l) const {  // where !only_top
-    constexpr double MAGIC = 211106232532992.0;  // 1.5 * 2^47: adding it leaves steps of 1/32
-    constexpr double C1 = 0.6931471805599453094, C2 = C1 * C1 / 2, C3 = C2 * C1 / 3, C4 = C3 * C1 / 4, C5 = C4 * C1 / 5;
+    constexpr double MAGIC = 52776558133248.0;  // 1.5 * 2^45: adding it leaves steps of 1/128
+    constexpr double C1 = 0.6931471805599453094, C2 = C1 * C1 / 2, C3 = C2 * C1 / 3, C4 = C3 * C1 / 4;
     const double d = (double)fmaxf(l, floor) - (double)top, r = fma(d, c, MAGIC);
     const int k = __double2loint(r);
     const double g = fma(d, c, MAGIC - r);
-    double p = fma(g, C5, C4);
-    p = fma(p, g, C3);
+    double p = fma(g, C4, C3);
     p = fma(p, g, C2);
     p = fma(p, g, C1);
-    p = fma(p, g, 1.0) * block_shared().exp2_32[k & 31];
-    return __hiloint2double(__double2hiint(p) + ((k >> 5) << 20), __double2loint(p));
+    p = fma(p, g, 1.0) * block_shared().exp2_128[k & 127];
+    return __hiloint2double(__double2hiint(p) + ((k >> 7) << 20), __double2loint(p));
   }
   __device__ __forceinline__ double operator()(float l) const {
     return only_top ? (l == top ? 1.0 : 0.0) : finite(l);
@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
   }
   const int groups = C < 8 ? 64 : 32;  // per block
   if (lane == 0) sh.warp_red[warp] = __float_as_uint(top);
-  if (tid < 32) sh.exp2_32[tid] = exp2((double)tid / 32);
+  if (tid < 128) sh.exp2_128[tid] = exp2((double)tid / 128);
   if (tid == 0) {
     sh.first_index = 0xffffffffu;
     sh.n_items = 0;
@@ -629,10 +629,13 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
 #pragma unroll
   for (int r = 0; r < 8; ++r)
     if (r < C) top = fmaxf(top, cluster.map_shared_rank(&sh, r)->best);
-  // a small top-k's bound: the k-th largest of the groups' maxima. (Towards the smallest of them
-  // the bound falls off: k = 200 of 256 in a row of 16384 took 26.5 us, by the threads' maxima 15.4;
-  // k = 64 takes 12.4 this way and 13.7 that way.)
-  const bool small_k = cut_k && temp > 0.f && top_k <= C * groups / 2;
+  // a small top-k's bound: the k-th largest of the groups' maxima. (About -n ln(1 - k / n) elements lie
+  // above it with n groups that hold elements: towards the smallest of them the bound falls off. k =
+  // 200 of 256 in a row of 16384, where half of the warps have nothing, took 26.5 us, by the threads'
+  // maxima 15.4; k = 64 takes 12.4 this way and 13.7 that way.)
+  const int full = a.share / BLOCK_ELEMS, stretch = (full + SAMPLE_WARPS - 1) / SAMPLE_WARPS;
+  const int filled = C * groups * ((full + stretch - 1) / stretch) / SAMPLE_WARPS;
+  const bool small_k = cut_k && temp > 0.f && 5 * top_k <= 4 * filled;
   float bound = -INFINITY;
   if (small_k) {
     if (tid < C * groups) sh.all_max[tid] = cluster.map_shared_rank(&sh, tid / groups)->group_max[tid % groups];
