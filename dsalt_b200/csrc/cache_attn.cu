@@ -162,9 +162,10 @@ __device__ __forceinline__ SeqPlan plan_of(const CacheAttnArgs& a, int s, int la
   int lo = p.len, top = 0, span = 0;
   if (!a.w) lo = 0;
   else for (int r = lane; r < p.n_q; r += lanes) {
+    const int w = max(__ldg(a.w + p.q0 + r), 1);  // on its way beside the lengths
     const int pos = p.len - p.n_q + r;
     if (pos < 0) continue;
-    const int f = first_key(a, p.q0 + r, pos);
+    const int f = max(pos - w + 1, 0);
     lo = min(lo, f);
     top = max(top, f);
     span = max(span, pos + 1 - f);

@@ -314,7 +314,8 @@ def test_attention_with_cut_keys(V, D, lens):
 
 @pytest.mark.parametrize("H,Hkv,D,page,lens,q_lens,w_max,k", [
     (4, 2, 64, 16, [420, 900], [300, 2], 90, 40), (8, 1, 128, 64, [261, 0, 40], [261, 0, 35], 70, 33),
-    (2, 2, 64, 32, [700], [513], 0, 0), (3, 1, 64, 16, [30] * 9, [30] * 9, 12, 5)])
+    (2, 2, 64, 32, [700], [513], 0, 0), (3, 1, 64, 16, [30] * 9, [30] * 9, 12, 5), (2, 1, 64, 16, [20, 3, 50], [40, 9, 12], 30, 8),
+    (16, 2, 64, 64, [600, 8], [8, 8], 2**31 - 1, 20), (3, 1, 64, 16, [500, 77, 9], [9, 15, 3], 100, 64)])
 def test_attention_of_many_tokens_per_sequence(V, H, Hkv, D, page, lens, q_lens, w_max, k):
     run_attend(V, attend_case(5, lens, q_lens, H, Hkv, D, page, torch.bfloat16, w_max, k))
 
