@@ -67,7 +67,7 @@ def _want(t: torch.Tensor, name: str, dtype: torch.dtype, shape) -> None:
 def _run(dev: torch.device, name: str, *args) -> None:
     """The C call on the current stream of the tensors' device."""
     index = dev.index
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         L.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
@@ -104,11 +104,13 @@ def reserve_slots(block_tables, seq_lens, new_lens, free_pages, n_free, page_siz
     if n_tokens < 0:
         raise ValueError("n_tokens must not be negative")
     slots = torch.empty(n_tokens, dtype=torch.int64, device=dev)
-    ints = torch.empty(((n_tokens + 3) & ~3) + 2 * S + 2, dtype=i32, device=dev)
-    positions, _, cu_new, lens, left = ints.split_with_sizes([n_tokens, -n_tokens & 3, S + 1, S, 1])
     granted = torch.empty(S, dtype=torch.bool, device=dev)
     if inplace:
+        positions, cu_new = torch.empty(n_tokens + S + 1, dtype=i32, device=dev).split_with_sizes((n_tokens, S + 1))
         lens, left = seq_lens, n_free
+    else:
+        positions, cu_new, lens, left = torch.empty(n_tokens + 2 * S + 2, dtype=i32, device=dev).split_with_sizes(
+            (n_tokens, S + 1, S, 1))
     _run(dev, "dsalt_reserve_slots", block_tables.data_ptr(), S, max_pages, seq_lens.data_ptr(), new_lens.data_ptr(),
          free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(), int(page_size), n_tokens, slots.data_ptr(),
          positions.data_ptr(), cu_new.data_ptr(), granted.data_ptr(), lens.data_ptr(), left.data_ptr())
@@ -225,7 +227,10 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_len
             raise ValueError("lmk_bias needs lmk_indices")
         _want(lmk_bias, "lmk_bias", torch.float32, (H, S, k_lmk))
     q, q_stride, _ = _rows(q, packed=True)
-    out = torch.empty(T, H, D, dtype=out_dtype or q.dtype, device=dev)
+    if (out_dtype is None or out_dtype is q.dtype) and q_stride == H * D:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        out = torch.empty(T, H, D, dtype=out_dtype or q.dtype, device=dev)
     lse = torch.empty(T, H, dtype=torch.float32, device=dev) if return_lse else None
     ws = _workspace(_attention_workspace(T, S, H, n_kv, D), dev)
     _run(dev, "dsalt_cache_attention", q.data_ptr(), _dt(q), T, H, n_kv, D, q_stride, k_cache.data_ptr(),
