@@ -502,70 +502,23 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
   Where ww = find_window(0), wn = ww, ln = ww;
   if (n_w > 16) wn = find_window(16);
   if (le > lb) ln = find_lmk(0);
-  // ---- Q of row g: the 16 consecutive elements at 16 t of each 64
-  uint32_t qb[NS][KS][2];
-  float row_f[2];
+  // ---- Q of row g: the 16 consecutive elements at 16 t of each 64, on their way while the first
+  // tiles are asked for
+  constexpr int QV = (int)sizeof(T);  // vectors of 16 bytes per 64 channels
+  uint4 q_raw[D / 64][QV];
   {
-    float x[D / 4];
-#pragma unroll
-    for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
     const int head = head_of(tok0 + g), tok = tok0 + g - head * per_head;
-    if (g < n_rows && tok < p.n_q) {
-      const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)(p.q0 + tok) * a.q_stride +
-                     (int64_t)(hk * a.G + head0 + head) * D + t * 16;
+    const bool live = g < n_rows && tok < p.n_q;
+    const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)(p.q0 + (live ? tok : 0)) * a.q_stride +
+                   (int64_t)(hk * a.G + head0 + (live ? head : 0)) * D + t * 16;
 #pragma unroll
-      for (int b = 0; b < D / 64; ++b) {
-        if constexpr (sizeof(T) == 4) {
+    for (int b = 0; b < D / 64; ++b)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float4 f = __ldg(reinterpret_cast<const float4*>(src + b * 64) + j);
-            x[b * 16 + 4 * j] = f.x, x[b * 16 + 4 * j + 1] = f.y, x[b * 16 + 4 * j + 2] = f.z, x[b * 16 + 4 * j + 3] = f.w;
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(src + b * 64) + j);
-            const uint32_t wd[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float2 f;
-              if constexpr (std::is_same<T, __half>::value) f = __half22float2(*reinterpret_cast<const __half2*>(&wd[e]));
-              else f = make_float2(__uint_as_float(wd[e] << 16), __uint_as_float(wd[e] & 0xffff0000u));
-              x[b * 16 + j * 8 + 2 * e] = f.x;
-              x[b * 16 + j * 8 + 2 * e + 1] = f.y;
-            }
-          }
-        }
-      }
-    }
-    float big = 0.f;
-#pragma unroll
-    for (int j = 0; j < D / 4; ++j) big = fmaxf(big, fabsf(x[j]));
-    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-    const int eb = (int)(__float_as_uint(big) >> 23);  // biased exponent; 255: an infinity
-    const int up = eb == 255 ? 0 : min(max(13 - (eb - 127), -126), 126);
-    const float mul = __uint_as_float((uint32_t)(up + 127) << 23);
-    const float f = a.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
-#pragma unroll
-    for (int c = 0; c < 2; ++c) row_f[c] = __shfl_sync(0xffffffffu, f, (2 * t + c) * 4);
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float lo = x[4 * k + 2 * h] * mul, hi = x[4 * k + 2 * h + 1] * mul;
-        qb[0][k][h] = pack_f16x2(lo, hi);
-        if constexpr (NS == 2) {
-          const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&qb[0][k][h]));
-          qb[1][k][h] = pack_f16x2(lo - b.x, hi - b.y);
-        }
+      for (int j = 0; j < QV; ++j) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + b * 64) + j);
+        q_raw[b][j] = live ? v : make_uint4(0, 0, 0, 0);
       }
   }
-
-  float o[MT][4];  // channels D/8 g + 2 i (0, 1) and one on (2, 3) of rows 2t, 2t+1
-#pragma unroll
-  for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  RowState st[2] = {{-INFINITY, 0.f, -INFINITY}, {-INFINITY, 0.f, -INFINITY}};
   uint8_t* ring = dyn + warp * (STAGES * Stage<D>::BYTES);
   const uint32_t ring_s = smem_u32(ring);
   int ww_row = -1;                  // row of ww's key
@@ -635,9 +588,60 @@ __global__ void __launch_bounds__(CA_THREADS, Shape<D>::OCC) cache_attn_kernel(C
     }
     copies_commit();
   };
-  __syncthreads();  // the schedule's memory becomes the rings
+  // (the schedule's memory becomes the rings: it was last read before the barrier behind it)
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) issue(i);
+  uint32_t qb[NS][KS][2];
+  float row_f[2];
+  {
+    float x[D / 4];
+#pragma unroll
+    for (int b = 0; b < D / 64; ++b)
+#pragma unroll
+      for (int j = 0; j < QV; ++j) {
+        const uint4 u = q_raw[b][j];
+        const uint32_t wd[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (sizeof(T) == 4) {
+            x[b * 16 + j * 4 + e] = __uint_as_float(wd[e]);
+          } else {
+            float2 f;
+            if constexpr (std::is_same<T, __half>::value) f = __half22float2(*reinterpret_cast<const __half2*>(&wd[e]));
+            else f = make_float2(__uint_as_float(wd[e] << 16), __uint_as_float(wd[e] & 0xffff0000u));
+            x[b * 16 + j * 8 + 2 * e] = f.x;
+            x[b * 16 + j * 8 + 2 * e + 1] = f.y;
+          }
+        }
+      }
+    float big = 0.f;
+#pragma unroll
+    for (int j = 0; j < D / 4; ++j) big = fmaxf(big, fabsf(x[j]));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    const int eb = (int)(__float_as_uint(big) >> 23);  // biased exponent; 255: an infinity
+    const int up = eb == 255 ? 0 : min(max(13 - (eb - 127), -126), 126);
+    const float mul = __uint_as_float((uint32_t)(up + 127) << 23);
+    const float f = a.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) row_f[c] = __shfl_sync(0xffffffffu, f, (2 * t + c) * 4);
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float lo = x[4 * k + 2 * h] * mul, hi = x[4 * k + 2 * h + 1] * mul;
+        qb[0][k][h] = pack_f16x2(lo, hi);
+        if constexpr (NS == 2) {
+          const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&qb[0][k][h]));
+          qb[1][k][h] = pack_f16x2(lo - b.x, hi - b.y);
+        }
+      }
+  }
+
+  float o[MT][4];  // channels D/8 g + 2 i (0, 1) and one on (2, 3) of rows 2t, 2t+1
+#pragma unroll
+  for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  RowState st[2] = {{-INFINITY, 0.f, -INFINITY}, {-INFINITY, 0.f, -INFINITY}};
 
   // m and M are references, not exact maxima: they move when a lane's logit passes them by the
   // slack, which after the first tiles is rare, and only then are maxima formed over the lanes
