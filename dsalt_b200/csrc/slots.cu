@@ -159,12 +159,12 @@ __global__ void __launch_bounds__(THREADS) reserve_slots_kernel(
 }
 
 // The tokens, where they are many: four consecutive ones per thread, one search for the first's
-// row, from what the rows' kernel has written.
-__global__ void __launch_bounds__(256) fill_slots_kernel(const int32_t* __restrict__ tables, int n_seqs, int max_pages,
-                                                         const int32_t* __restrict__ seq_lens,
-                                                         const int32_t* __restrict__ cu, const uint8_t* __restrict__ granted,
-                                                         int page_shift, int64_t n_tokens, int64_t* __restrict__ slots,
-                                                         int32_t* __restrict__ positions) {
+// row, from what the rows' kernel has written. (That kernel may still be under way when this one
+// begins: its results are read by ordinary loads, not by those for constant data.)
+__global__ void __launch_bounds__(256) fill_slots_kernel(const int32_t* tables, int n_seqs, int max_pages,
+                                                         const int32_t* seq_lens, const int32_t* cu,
+                                                         const uint8_t* granted, int page_shift, int64_t n_tokens,
+                                                         int64_t* slots, int32_t* positions) {
   cudaGridDependencySynchronize();
   const int64_t t0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (t0 >= n_tokens) return;
