@@ -70,7 +70,7 @@ constexpr float CA_SLACK = 1.f;        // P may exceed 2^14 by 2^1 before its re
 // Blocks per SM that registers and rings allow; one round of them is the number of units wanted.
 // Two stages: a third costs blocks, and at head_dim 64 with 7 of them one row of 131072 keys
 // takes 57.1 us against 54.2, with 6 of them 52.2 but 64 rows 33.9 against 25.2; at head_dim 128
-// with 4 of them 41.9 us against 40.8.
+// with 4 of them 41.9 us against 40.8. Nine blocks of head_dim 64 leave 112 registers: 69 us.
 template <int D>
 struct Shape {
   static constexpr int OCC = D == 64 ? 8 : 6;
