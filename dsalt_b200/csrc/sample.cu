@@ -61,7 +61,14 @@ constexpr int MAX_SHARE = 131328;             // 2^20 / 8 and a skew, in whole s
 constexpr int MAX_STEPS = (MAX_SHARE / BLOCK_ELEMS + SAMPLE_WARPS - 1) / SAMPLE_WARPS;  // of one warp
 constexpr int QUEUE = 992;                    // elements of the decisive bin that a warp keeps
 constexpr int MAX_GROUPS = 256;
-constexpr double MASS_ONE = 8796093022208.0;  // 2^43: 2^20 of them stay below 2^63
+constexpr int MASS_BITS = 43;
+constexpr double MASS_ONE = 8796093022208.0;  // 2^43: 2^20 of them are 2^63, within 64 bits without a sign
+// A mass (at most 2^43) in the joint histogram's 32-bit words: limbs of 14 bits, so that no word overflows
+// where a whole share falls into one bin (131328 limbs of 15 bits would reach past 2^32).
+constexpr int LIMBS = 4, LIMB_BITS = 14;
+constexpr uint32_t LIMB_MAX = (1u << LIMB_BITS) - 1;
+static_assert((uint64_t)MAX_SHARE * LIMB_MAX <= 0xffffffffull, "a limb's sum over a share");
+static_assert(MASS_BITS < LIMBS * LIMB_BITS, "the limbs hold a mass");
 constexpr float BIN_SPAN = 32.f;              // (m - l) / T that the joint histogram covers
 constexpr float MIN_LOG2 = -45.f;             // weights below 2^-45 round to no mass
 
@@ -85,7 +92,7 @@ struct SampleShared {
   union {
     u64 priv[PBINS][SAMPLE_THREADS];  // count (12 bits) and mass (52) of each thread's elements per bin
     struct {
-      uint32_t count[NBINS], limb[3][NBINS];  // this block's joint histogram; masses as three limbs
+      uint32_t count[NBINS], limb[LIMBS][NBINS];  // this block's joint histogram; masses in limbs
     };
     struct {
       u64 sorted[LIST_CAP], weight[LIST_CAP];  // the leader's candidates in order, and their masses
@@ -513,9 +520,11 @@ __device__ __forceinline__ void histogram_pass(Share<T> s, Weights wt, Bin bin, 
     atomicAdd(&sh.count[b], 1u);
     if (by_mass) {
       const u64 w = wt.mass(l);
-      atomicAdd(&sh.limb[0][b], (uint32_t)(w & 0x7fff));
-      atomicAdd(&sh.limb[1][b], (uint32_t)(w >> 15) & 0x7fff);
-      if (w >> 30) atomicAdd(&sh.limb[2][b], (uint32_t)(w >> 30));
+      atomicAdd(&sh.limb[0][b], (uint32_t)w & LIMB_MAX);
+      atomicAdd(&sh.limb[1][b], (uint32_t)(w >> LIMB_BITS) & LIMB_MAX);
+#pragma unroll
+      for (int x = 2; x < LIMBS; ++x)  // of weights above 2^-15, and above 1/2
+        if (w >> x * LIMB_BITS) atomicAdd(&sh.limb[x][b], (uint32_t)(w >> x * LIMB_BITS) & LIMB_MAX);
     }
   });
 }
@@ -548,7 +557,9 @@ __device__ __forceinline__ void list_pass(Share<T> s, float low, u64 cut, Sample
 template <typename T>
 __device__ __forceinline__ void list_part_pass(Share<T> s, Bin bin, Parts parts, int part, int queued, SampleShared* lead) {
   for_bin(s, bin, queued, [&](float l, int i) {
-    if (parts(l, i) == part) lead->item[atomicAdd(&lead->n_items, 1u)] = compose(l, i);
+    if (parts(l, i) != part) return;
+    const uint32_t at = atomicAdd(&lead->n_items, 1u);
+    if (at < LIST_CAP) lead->item[at] = compose(l, i);
   });
 }
 // the warp's mass of what stays: of its queue, of its elements, of one step
@@ -618,7 +629,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
     sh.n_items = 0;
   }
   const auto clear_bins = [&] {
-    for (int i = tid; i < NBINS; i += SAMPLE_THREADS) sh.count[i] = sh.limb[0][i] = sh.limb[1][i] = sh.limb[2][i] = 0;
+    for (int i = tid; i < NBINS; i += SAMPLE_THREADS) sh.count[i] = sh.limb[0][i] = sh.limb[1][i] = sh.limb[2][i] = sh.limb[3][i] = 0;
   };
   clear_bins();
   __syncthreads();
@@ -701,22 +712,27 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
         if (r < C) {
           const SampleShared* o = cluster.map_shared_rank(&sh, r);
           cnt += o->count[b];
-          if (by_mass) ms += (u64)o->limb[0][b] + ((u64)o->limb[1][b] << 15) + ((u64)o->limb[2][b] << 30);
+          if (by_mass) {
+#pragma unroll
+            for (int x = 0; x < LIMBS; ++x) ms += (u64)o->limb[x][b] << x * LIMB_BITS;
+          }
         }
       lead->total[b] = cnt;
       lead->mass[b] = ms;
     }
     cluster.sync();
   };
-  // the leader: the first bin whose running sum reaches `want` (there is one): result = bin and its
-  // count, sum before it, elements up to and with it
+  // the leader: the first bin whose running sum reaches `want`, else the last: result = bin and its
+  // count, sum before it, elements up to and with it. (Where a bin is refined the sums reach it, unless
+  // the logits are written to meanwhile.)
   const auto find_bin = [&](bool by_mass, u64 above, u64 want) {
     if (rank == 0) {
       const uint32_t c0 = sh.total[2 * tid], c1 = sh.total[2 * tid + 1];
       const u64 v0 = by_mass ? sh.mass[2 * tid] : c0, v1 = by_mass ? sh.mass[2 * tid + 1] : c1;
       const u64 before = above + block_before(v0 + v1, sh);
       const u64 cnt_before = block_before((u64)c0 + c1, sh);
-      if (before < want && before + v0 + v1 >= want) {  // one thread: the sums only grow
+      // one thread: the sums only grow
+      if (before < want && (before + v0 + v1 >= want || tid == SAMPLE_THREADS - 1)) {
         const bool second = before + v0 < want;
         sh.result[0] = (u64)(2 * tid + second) | ((u64)(second ? c1 : c0) << 32);
         sh.result[1] = before + (second ? v0 : 0);
@@ -742,9 +758,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
     if (rank == 0 && tid == 0) sh.n_items = 0;
   } else if (cut_k && top_k <= LIST_CAP / 2 && top_k <= C * SAMPLE_THREADS / 4) {
     if (mine > -INFINITY) atomicAdd(&sh.count[joint_bin(mine)], 1u);
-    if (rank == 0 && tid == 0) sh.result[0] = NBINS - 1;  // fewer maxima than k: every element
     join_bins(false);
-    find_bin(false, 0, (u64)top_k);
+    find_bin(false, 0, (u64)top_k);  // fewer maxima than k: the last bin, every element
     const int bin = (int)(uint32_t)lead->result[0];
     list_pass<T>(s, bin == NBINS - 1 ? -INFINITY : lowest((float)(bin + 1) / (NBINS / BIN_SPAN)), 0, lead);
     cluster.sync();
@@ -828,7 +843,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
       list_pass<T>(s, bin.low, cut, lead);
       cluster.sync();
       if (rank == 0) {
-        const int m = (int)sh.n_items;
+        const int m = min((int)sh.n_items, LIST_CAP);
         sort_items(sh, m, wt);
         settle_list(a, sh, row, by_mass ? m : min(m, top_k), cut_p, top_p, by_mass ? want : 0, min_p, u, wt);
       }
@@ -873,7 +888,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
       }
       parts.floor_c = first;
       parts.ceil_c = last;
-      while (bin_elems > LIST_CAP) {
+      while (bin_elems > LIST_CAP && parts.shift != 0) {  // with 0 a bin is one element
         // width >> shift < NBINS = 2^10
         parts.shift = max(0, 64 - __clzll((long long)(parts.ceil_c - parts.floor_c)) - 10);
         part = histogram(parts);
@@ -887,8 +902,9 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
     cluster.sync();
     // these elements decide: sort them, the cut is the one at which `want` is reached
     if (rank == 0) {
-      const int m = (int)sh.n_items;
+      const int m = min((int)sh.n_items, LIST_CAP);
       sort_items(sh, m, wt);
+      if (tid == 0) sh.result[0] = m > 0 ? sh.sorted[m - 1] : 0;  // the last one, should none be found
       const int i0 = 2 * tid, i1 = i0 + 1;
       const u64 w0 = i0 < m ? (by_mass ? sh.weight[i0] : 1) : 0, w1 = i1 < m ? (by_mass ? sh.weight[i1] : 1) : 0;
       const u64 before = above + block_before(w0 + w1, sh);
