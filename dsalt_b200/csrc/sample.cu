@@ -4,7 +4,7 @@
 // Of a row of logits l, with m = max l and weights w = exp((l - m) / T):
 //   top-k: the k first in the order (logit descending, index ascending)
 //   top-p: of those the shortest prefix whose mass reaches p times theirs
-//   min-p: of those the weights of at least min_p (the largest weight is 1)
+//   min-p: of those the weights of at least min_p (the largest weight is 1), or the first alone
 //   token: the first index whose running sum of kept weights, in index order, exceeds u
 //          times their total.
 // T <= 0 takes the first index of the largest logit. A NaN counts as -inf, +inf logits share
@@ -597,9 +597,10 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   SampleShared* lead = cluster.map_shared_rank(&sh, 0);
 
-  const float temp = a.temperature ? a.temperature[row] : a.temperature_v;
   const double top_p = a.top_p ? (double)a.top_p[row] : (double)a.top_p_v;
   const double min_p = a.min_p ? (double)a.min_p[row] : (double)a.min_p_v;
+  // no weight reaches a min_p above 1, and the first of the order stays: what temperature 0 takes
+  const float temp = min_p > 1.0 ? 0.f : a.temperature ? a.temperature[row] : a.temperature_v;
   const int top_k = a.top_k ? a.top_k[row] : a.top_k_v;
   const float u = a.u[row];
   const bool cut_k = top_k > 0 && top_k < a.V, cut_p = top_p < 1.0;

@@ -258,10 +258,10 @@ def sample_tokens(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
 
     Of the weights ``exp((l - max l) / temperature)`` ``top_k`` keeps the largest (equal logits:
     lowest index first; 0 = off), ``top_p`` of those the shortest prefix whose mass reaches
-    ``top_p`` of theirs, ``min_p`` of those the weights of at least ``min_p``. The token is the
-    first index whose running sum of kept weights exceeds ``u`` times their total;
-    ``temperature`` 0 takes the largest logit. Each setting is a number or a ``[B]`` tensor
-    (fp32; ``top_k`` int32). A row gives the same token in every batch."""
+    ``top_p`` of theirs, ``min_p`` of those the weights of at least ``min_p``; the first of the
+    order always stays. The token is the first index whose running sum of kept weights exceeds
+    ``u`` times their total; ``temperature`` 0 takes the largest logit. Each setting is a number
+    or a ``[B]`` tensor (fp32; ``top_k`` int32). A row gives the same token in every batch."""
     per_row = [t for t in (temperature, top_k, top_p, min_p) if isinstance(t, torch.Tensor)]
     dev = _on_one_device(logits, u, *per_row)
     if logits.dim() != 2:

@@ -398,7 +398,8 @@ int dsalt_cache_attention(const void* q, int dtype, int64_t T, int n_heads, int 
  *   (nullable) log of its share of that total.
  * Each setting is a device array [B], or null and the value beside it. temperature <= 0 takes
  *   the first index of the largest logit (logprob 0); top_k outside [1, V), top_p >= 1 and
- *   min_p <= 0 are off. A NaN logit counts as -inf; +inf logits share the draw; a row of
+ *   min_p <= 0 are off; of a min_p above 1, which no weight reaches, the first of the order stays.
+ *   A NaN logit counts as -inf; +inf logits share the draw; a row of
  *   nothing but -inf gives token 0 and logprob -inf.
  */
 int dsalt_sample(const void* logits, int dtype, int64_t B, int64_t V, int64_t row_stride, const float* u,

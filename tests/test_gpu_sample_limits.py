@@ -32,3 +32,27 @@ def test_largest_vocabulary_of_two_values(V, low, dtype):
         assert margin >= 2.0 ** -43 * vocab
         assert int(tok) == t
         assert abs(float(lp) - l) <= 2.0 ** -23 * (abs(l) + 1)
+
+
+# ------------------------------------------------------------------ min_p above 1
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab,top_k,top_p", [(40, 0, 1.0), (5000, 0, 1.0), (5000, 0, 0.999), (5000, 3000, 1.0),
+                                               (5000, 20, 0.9), (151936, 0, 0.9999)])
+def test_min_p_above_one_leaves_the_first_of_the_order(V, dtype, vocab, top_k, top_p):
+    """The largest weight is 1: nothing reaches a larger min_p, and the first of the order stays, as it does under
+    every filter. Rows with such a min_p stand among ordinary ones."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    lg = (torch.randn(6, vocab, device="cuda", generator=g) * 2).to(dtype)
+    lg[2, 31] = lg[2, 7] = 40.0  # two largest: the lower index
+    min_p = torch.tensor([1.5, 0.0, 1.5, 0.01, float("inf"), 1.0], device="cuda")
+    u = torch.tensor([0.9, 0.3, 0.999, 0.6, 0.0, 0.7], device="cuda")
+    tok, lp = V.sample_tokens(lg, u, temperature=1.7, top_k=top_k, top_p=top_p, min_p=min_p, return_logprob=True)
+    f32 = lambda x: float(np.float32(x))  # noqa: E731
+    for i in range(6):
+        t, l, margin = O.sample(lg[i].double().cpu().numpy(), float(u[i]), f32(1.7), top_k, f32(top_p), float(min_p[i]))
+        if i in (0, 2, 4):
+            assert (t, l) == (int(lg[i].float().argmax()) if i != 2 else 7, 0.0)
+        if margin >= 2.0 ** -43 * vocab:  # as far as the order of sums may move a border
+            assert int(tok[i]) == t
+            assert abs(float(lp[i]) - l) <= 2.0 ** -23 * (abs(l) + 1)
+    assert (lp[[0, 2, 4]] == 0).all()
