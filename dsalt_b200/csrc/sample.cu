@@ -26,7 +26,8 @@
 // Masses are whole numbers, w * 2^43 rounded from 64-bit arithmetic: their sums do not depend
 // on the order in which threads arrive, so a row gives the same token in every batch and in
 // every run, and a border lies within 2^20 roundings of 2^-44 (6e-8 of the largest weight at
-// the very worst, about 1e-11 in practice) of where sums in 64-bit floating point put it.
+// the very worst, about 1e-11 in practice) of where sums in 64-bit floating point put it. The
+// log-probability is formed from the drawn logit and the sum, not from the token's own mass.
 //
 // One cluster of C blocks owns a row, each a share of it. The row comes from HBM once; later
 // passes find it in L1 or L2, which hold it for all rows under way.
@@ -165,6 +166,12 @@ struct Weights {
     return (u64)__double_as_longlong(fma(w, MASS_ONE, 4503599627370496.0)) & 0xfffffffffffffull;  // + 2^52
   }
   __device__ __forceinline__ u64 mass(float l) const { return mass((*this)(l)); }
+  // log of a drawn logit's share of the kept masses, from the logit itself: a rare token's mass has
+  // few bits (weight 2^-40: three)
+  __device__ __forceinline__ float log_share(float l, u64 total) const {
+    const double z = l == top ? 0.0 : ((double)l - (double)top) * (c * 0.6931471805599453094);
+    return (float)(z - log((double)total / MASS_ONE));
+  }
 };
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
@@ -290,9 +297,9 @@ __device__ __forceinline__ void settle_list(const SampleArgs& a, SampleShared& s
   const u64 m0 = i0 < keep ? sh.weight[sh.by_index[i0] & 1023] : 0, m1 = i1 < keep ? sh.weight[sh.by_index[i1] & 1023] : 0;
   const u64 total = block_sum(m0 + m1, sh), before = block_before(m0 + m1, sh), target = target_of(u, total);
   if (before <= target && target < before + m0 + m1) {  // one thread
-    const bool second = target >= before + m0;
-    a.token[row] = sh.by_index[second ? i1 : i0] >> 10;
-    if (a.logprob) a.logprob[row] = (float)log((double)(second ? m1 : m0) / (double)total);
+    const uint32_t drawn = sh.by_index[target >= before + m0 ? i1 : i0];
+    a.token[row] = drawn >> 10;
+    if (a.logprob) a.logprob[row] = wt.log_share(logit_of(sh.sorted[drawn & 1023]), total);
   }
 }
 
@@ -984,10 +991,11 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleArgs a)
       if (b <= target && target < b + lane_sum) {  // one lane
 #pragma unroll 1
         for (int i = max(i0, 0); i < i1; ++i) {
-          const u64 m = kept(s.one(i), i);
+          const float l = s.one(i);
+          const u64 m = kept(l, i);
           if (target < b + m) {
             a.token[row] = i;
-            if (a.logprob) a.logprob[row] = (float)log((double)m / (double)total);
+            if (a.logprob) a.logprob[row] = wt.log_share(l, total);
             break;
           }
           b += m;

@@ -56,3 +56,39 @@ def test_min_p_above_one_leaves_the_first_of_the_order(V, dtype, vocab, top_k, t
             assert int(tok[i]) == t
             assert abs(float(lp[i]) - l) <= 2.0 ** -23 * (abs(l) + 1)
     assert (lp[[0, 2, 4]] == 0).all()
+
+
+# ------------------------------------------------------------------ rare tokens
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("vocab", [5, 3000, 60000])
+def test_log_probability_of_rare_tokens(V, dtype, vocab):
+    """The log-probability is that of the drawn logit, whatever its weight: log w - log of the sum. Bound: the
+    result's own rounding, half a step of |lp|, and the sum's: at most V + 1 roundings of 2^-44 against a sum of
+    at least 1, 2^-28 here, both well within 2^-23 (|lp| + 1)."""
+    ones = -(2.0 ** -6) * (torch.arange(vocab, device="cuda") % 3)
+    rows = torch.stack([ones] * 5).to(dtype)
+    rare = [-25.0, -28.0, -29.25, -27.0, -20.0]
+    for i, x in enumerate(rare):
+        rows[i, 0] = x  # the first in index order: a small u draws it
+    mass = torch.exp(rows.double()).sum(1)
+    u = (torch.exp(rows[:, 0].double()) / mass * 0.4).float()
+    for min_p in (0.0, 1e-15):
+        tok, lp = V.sample_tokens(rows, u, min_p=min_p, return_logprob=True)
+        for i in range(5):
+            t, l, _ = O.sample(rows[i].double().cpu().numpy(), float(u[i]), 1.0, 0, 1.0, min_p)
+            assert t == 0 and int(tok[i]) == 0
+            assert abs(float(lp[i]) - l) <= 2.0 ** -23 * (abs(l) + 1), (i, float(lp[i]), l)
+
+
+def test_log_probability_of_rare_tokens_in_a_list(V):
+    # five candidates of 100, as top-k leaves them: settled in the list of one block
+    lg = torch.full((1, 100), -60.0, device="cuda")
+    lg[0, 2], lg[0, 50:54] = -26.0, torch.tensor([0.0, -0.5, -1.0, 0.25], device="cuda")
+    row = lg[0].double().cpu().numpy()
+    keep = np.sort(np.argsort(-row, kind="stable")[:5])
+    p = np.exp(row[keep] - row.max())
+    u = torch.tensor([0.4 * p[0] / p.sum()], device="cuda").float()
+    tok, lp = V.sample_tokens(lg, u, top_k=5, return_logprob=True)
+    t, l, _ = O.sample(row, float(u[0]), 1.0, 5, 1.0, 0.0)
+    assert t == 2 and int(tok) == 2
+    assert abs(float(lp) - l) <= 2.0 ** -23 * (abs(l) + 1)
