@@ -225,32 +225,41 @@ class DSALTLMHeadModel(nn.Module):
 
     @torch.no_grad()
     def prefill(self, input_ids, cu_list, cache: PagedCache):
-        """Packed prompts (``cu_list``: the host list of their borders, one per row of the cache, whose
-        rows must be empty) into the cache; the logits of each prompt's last token ``[S, vocab]``."""
+        """Packed prompts (``cu_list``: the host list of their borders, one per row of the cache) into
+        rows of the cache that are empty; the logits of each prompt's last token ``[S, vocab]``. Rows whose
+        prompt has no tokens are passed over, whether they hold a sequence or not; their logits are 0."""
         cu_h = [int(c) for c in cu_list]
         lens = [b - a for a, b in zip(cu_h, cu_h[1:])]
-        if len(lens) != cache.max_seqs or min(lens) < 1 or cu_h[0] != 0 or input_ids.shape != (cu_h[-1],):
-            raise ValueError("cu_list must give one prompt of at least one token per row of the cache")
-        if any(cache.lens):
+        if len(lens) != cache.max_seqs or min(lens) < 0 or cu_h[0] != 0 or input_ids.shape != (cu_h[-1],):
+            raise ValueError("cu_list must give one prompt (or none: no tokens) per row of the cache")
+        if not any(lens):
+            raise ValueError("prefill needs a prompt of at least one token")
+        if any(held and new for held, new in zip(cache.lens, lens)):
             raise ValueError("prefill needs empty rows: release them first")
         plan = cache.reserve(lens)
         x, rope_cs = self._embed(input_ids, plan.positions)
+        cu = plan.cu_new
+        if not all(lens):  # the layers see the prompts alone
+            cu_h = [0] + [c for c, n in zip(cu_h[1:], lens) if n]
+            cu = torch.tensor(cu_h, dtype=torch.int32, device=x.device)
         for layer in self.layers:
-            x = layer.prefill(x, plan.cu_new, cu_h, rope_cs, cache, plan)
-        return self.lm_head(self.final_norm(x[plan.cu_new[1:].long() - 1]))
+            x = layer.prefill(x, cu, cu_h, rope_cs, cache, plan)
+        return cache.spread(self.lm_head(self.final_norm(x[cu[1:].long() - 1])))
 
     @torch.no_grad()
     def decode(self, tokens, cache: PagedCache):
-        """One more token per row of the cache ``tokens [S]`` → the next token's logits ``[S, vocab]``."""
-        if min(cache.lens) < 1:
-            raise ValueError("decode needs a prompt in every row")
+        """One more token for each row of the cache that holds a sequence, ``tokens [S]`` → the next
+        token's logits ``[S, vocab]``. Rows without a sequence are passed over: their tokens are not looked
+        at, their logits are 0."""
+        if not any(cache.lens):
+            raise ValueError("decode needs a prompt in every row that is to go on, and no row holds one")
         if tokens.shape != (cache.max_seqs,):
             raise ValueError(f"decode needs {cache.max_seqs} tokens, one per row")
-        plan = cache.reserve([1] * cache.max_seqs)
-        x, rope_cs = self._embed(tokens, plan.positions)
+        plan = cache.reserve([min(n, 1) for n in cache.lens])
+        x, rope_cs = self._embed(cache.pick(tokens), plan.positions)
         for layer in self.layers:
             x = layer.decode(x, rope_cs, cache, plan)
-        return self.lm_head(self.final_norm(x))
+        return cache.spread(self.lm_head(self.final_norm(x)))
 
     @torch.no_grad()
     def generate(self, prompts, max_new_tokens: int, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,

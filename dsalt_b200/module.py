@@ -230,8 +230,9 @@ class DSALTAttention(nn.Module):
     # ---------------------------------------------------------------- generation
     @torch.no_grad()
     def prefill(self, x, cu_seqlens, cu_h, rope_cs, cache, plan):
-        """Packed prompts as :meth:`forward` does, their keys, values and signals into the layer of
-        a :class:`dsalt_b200.serving.PagedCache` (``plan``: the cache's slots for them)."""
+        """Packed prompts as :meth:`forward` does (``cu_seqlens``, ``cu_h``: their borders), their keys,
+        values and signals into the layer of a :class:`dsalt_b200.serving.PagedCache` (``plan``: the cache's
+        slots for them)."""
         out, _, k, v, w, xn, vn, alpha = self._packed_core(x, cu_seqlens, x.shape[0], x.device, rope_cs, cu_h)
         cache.append(self.layer_idx, k, v, w, xn, vn, plan)
         cache.update_landmarks(self.layer_idx, alpha, self.k_lmk, self.block)
@@ -239,8 +240,8 @@ class DSALTAttention(nn.Module):
 
     @torch.no_grad()
     def decode(self, x, rope_cs, cache, plan):
-        """One token per row ``x [S, d_model]`` against the cached sequences: its window and its block's
-        landmarks, the query's own key and value included (all as the cache holds them, in 8 bits)."""
+        """One token for each row that goes on ``x [n, d_model]`` against the cached sequences: its window
+        and its block's landmarks, the query's own key and value included (all as the cache holds them, in 8 bits)."""
         T = x.shape[0]
         q = self.q_proj(x).view(T, self.n_heads, self.head_dim)
         k = self.k_proj(x).view(T, self.n_kv_heads, self.head_dim)

@@ -288,10 +288,11 @@ class PagedCache:
     ``page_size`` tokens, with what the landmark selection needs of them (norms and widths per
     position) and the current landmark sets ``[H, max_seqs, k]`` per layer.
 
-    Rows are sequences. All rows are used together: :meth:`reserve` takes the number of new
-    tokens of each row. ``lens`` is the host's copy of the lengths, kept so that block borders
-    are known without reading the device; a row whose tokens the pool or the tables cannot
-    hold is refused here, before anything is launched."""
+    Rows are sequences, which begin and end on their own: :meth:`reserve` takes the number of
+    new tokens of each row, 0 among them, and what follows (:meth:`append`, :meth:`attention`)
+    packs the tokens of the rows that have some. ``lens`` is the host's copy of the lengths, kept
+    so that block borders are known without reading the device; a row whose tokens the pool or
+    the tables cannot hold is refused here, before anything is launched."""
 
     def __init__(self, n_layers: int, n_heads: int, n_kv_heads: int, head_dim: int, k_lmk: int, *, max_seqs: int,
                  max_len: int, n_pages: int | None = None, page_size: int = 64, device="cuda"):
@@ -318,7 +319,8 @@ class PagedCache:
         self.vnorm = torch.zeros(n_layers, max_seqs, max_len, n_kv_heads, device=dev)
         self.width = torch.zeros(n_layers, max_seqs, max_len, dtype=i32, device=dev)
         self.lmk = torch.full((n_layers, n_heads, max_seqs, k_lmk), -1, dtype=i32, device=dev)
-        self._rows = None
+        self._rows = self._cu_new = None  # of the tokens reserved last: each one's row, each row's first
+        self._new_lens = [0] * max_seqs
         self._block_of = [[-1] * max_seqs for _ in range(n_layers)]  # whose set `lmk` holds
 
     def pages_held(self) -> int:
@@ -342,7 +344,21 @@ class PagedCache:
         self.lens = lens
         self._rows = torch.repeat_interleave(torch.arange(self.max_seqs, device=dev), new.long(),
                                              output_size=sum(new_lens))
+        self._cu_new, self._new_lens = plan.cu_new, new_lens
         return plan
+
+    def pick(self, x):
+        """The lines of ``x [max_seqs, ...]`` of the rows that got tokens last, packed."""
+        rows = [r for r, n in enumerate(self._new_lens) if n]
+        return x if len(rows) == self.max_seqs else x[torch.tensor(rows, device=x.device)]
+
+    def spread(self, x):
+        """The reverse: ``x``, a line for each row that got tokens last, as ``[max_seqs, ...]`` with
+        zeros for the other rows."""
+        rows = [r for r, n in enumerate(self._new_lens) if n]
+        if len(rows) == self.max_seqs:
+            return x
+        return x.new_zeros(self.max_seqs, *x.shape[1:]).index_copy_(0, torch.tensor(rows, device=x.device), x)
 
     def release(self, rows) -> None:
         """Ends the sequences of these rows; their pages go back to the pool."""
@@ -385,7 +401,11 @@ class PagedCache:
             self.lmk[layer, :, r] = sets[:, 0]
 
     def attention(self, layer: int, q, w):
-        """One query token per row over one layer."""
+        """One query token for each row that got one last (packed: rows without are passed over) over
+        one layer."""
+        if max(self._new_lens) > 1:  # the landmark sets are those of each row's last position
+            raise ValueError("attention takes one query token per row")
         lmk = self.lmk[layer] if self.lmk.shape[-1] > 0 else None
         return cache_attention(q.contiguous(), self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer],
-                               self.block_tables, self.seq_lens, w_sizes=w, lmk_indices=lmk)
+                               self.block_tables, self.seq_lens, cu_q=None if min(self._new_lens) else self._cu_new,
+                               w_sizes=w, lmk_indices=lmk)
