@@ -24,7 +24,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .module import DSALTAttention
-from .serving import PagedCache, sample_tokens
+from .serving import MAX_VOCAB, PagedCache, sample_tokens
 
 
 @dataclass
@@ -273,6 +273,8 @@ class DSALTLMHeadModel(nn.Module):
         if max_new_tokens < 1 or not prompts or min(len(p) for p in prompts) < 1:
             raise ValueError("generate needs prompts of at least one token and max_new_tokens >= 1")
         vocab = self.embed_tokens.num_embeddings
+        if vocab > MAX_VOCAB:
+            raise ValueError(f"a vocabulary of {vocab}: sampling takes {MAX_VOCAB} at most")
         if any(not 0 <= t < vocab for p in prompts for t in p):
             raise ValueError(f"token ids must lie in [0, {vocab})")
         dev = self.embed_tokens.weight.device

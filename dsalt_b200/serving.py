@@ -30,8 +30,10 @@ from . import ops
 from .ops import _dt, _ptr, _workspace
 
 PAGE_SIZES = (16, 32, 64, 128)
+HEAD_SIZES = (64, 128)
 MAX_ROWS = 8192          # rows (sequences) of one call
 MAX_VOCAB = 1 << 20
+MAX_POSITIONS = 0x7fffff00  # of a row, and of the pool times its kv heads
 
 
 class SlotPlan(NamedTuple):
@@ -298,11 +300,17 @@ class PagedCache:
                  max_len: int, n_pages: int | None = None, page_size: int = 64, device="cuda"):
         if page_size not in PAGE_SIZES:
             raise ValueError(f"page_size must be one of {PAGE_SIZES}")
-        if not 1 <= max_seqs <= MAX_ROWS or max_len < 1:
-            raise ValueError(f"max_seqs must be in [1, {MAX_ROWS}] and max_len positive")
+        if head_dim not in HEAD_SIZES:
+            raise ValueError(f"head size {head_dim}: the cache holds heads of {' or '.join(map(str, HEAD_SIZES))}")
+        if n_kv_heads < 1 or n_heads % n_kv_heads:
+            raise ValueError(f"n_heads ({n_heads}) must be a multiple of n_kv_heads ({n_kv_heads})")
+        if not 1 <= max_seqs <= MAX_ROWS or not 1 <= max_len <= MAX_POSITIONS - page_size:
+            raise ValueError(f"max_seqs must be in [1, {MAX_ROWS}] and max_len in [1, {MAX_POSITIONS - page_size}]")
         self.max_seqs, self.max_len, self.page_size = max_seqs, max_len, page_size
         self.max_pages = -(-max_len // page_size)
         self.n_pages = self.max_pages * max_seqs if n_pages is None else int(n_pages)
+        if not 0 <= self.n_pages * n_kv_heads * page_size <= MAX_POSITIONS:
+            raise ValueError(f"a pool of {self.n_pages} pages: it holds {MAX_POSITIONS} positions of all kv heads at most")
         dev = torch.device(device)
         i32 = torch.int32
         self.block_tables = torch.full((max_seqs, self.max_pages), -1, dtype=i32, device=dev)
