@@ -23,9 +23,10 @@
 //   (3.4e-4 of the result after 4096 products in a row); so O is added up by them over
 //   CA_CHAIN tiles at most and then, with rounding, to a sum in shared memory (local memory
 //   where head_dim 128 leaves no room; 2e-6 remains), for fp32 queries over 16 keys only.
-// The scales of V differ from page to page, so a row keeps two maxima: m of x for the
+// The scales 2^e of V differ from page to page, so a row keeps two maxima: m of x for the
 // denominator l = sum 2^(x - m), and M of x + e for the numerator O = sum 2^(x + e - M) byte;
-// out = O 2^(M - m) / l. Neither can overflow whatever the scales are.
+// out = O 2^(M - m) / l. Neither can overflow whatever the scales are. The cache's own scales are
+// powers of two; of others, written by another program, e is a logarithm good to 2^-22.
 //
 // The keys of an item (sequence, kv head, tile of 8 rows) are a list of tiles of 32: the
 // window's, then the landmarks' of each head. Items are cut into units of about equal
@@ -133,8 +134,14 @@ __device__ __forceinline__ uint32_t widen_hi(uint32_t v) {
   asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, h;}" : "=r"(r) : "r"(v));
   return r;
 }
-// e of a scale 2^e, as a float; 0 (a page never written) as the lowest
-__device__ __forceinline__ float scale_log(float s) { return (float)((int)(__float_as_uint(s) >> 23 & 0xff) - 127); }
+// log2 of a scale; of 0 (a page never written) -127: its exponent (put into the significand of 2^23, and
+// 2^23 + 127 taken off), and the logarithm of its significand, exactly 0 for a power of two
+__device__ __forceinline__ float scale_log(float s) {
+  const uint32_t u = __float_as_uint(s);
+  float f;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(f) : "f"(__uint_as_float((u & 0x7fffffu) | 0x3f800000u)));
+  return __uint_as_float(0x4b000000u + (u >> 23)) - 8388735.f + f;
+}
 
 // query of sequence s: tokens, keys and the tiles of 32 that they make
 struct SeqPlan {

@@ -199,7 +199,8 @@ def cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_len
     without it there is one per sequence. With ``w_sizes [T]`` int32 the
     query at position ``i`` attends to its window ``[i - w + 1, i]`` and to the landmarks
     ``lmk_indices [H, S, k]`` before it, as :func:`dsalt_b200.ops.dsalt_attention` does
-    (``lmk_bias`` is added to their logits); without, to ``[0, i]``."""
+    (``lmk_bias`` is added to their logits); without, to ``[0, i]``. The scales may be any
+    positive numbers, or 0, not only the powers of two that :func:`append_cache` writes."""
     dev = _on_one_device(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, cu_q, w_sizes, lmk_indices,
                          lmk_bias)
     n_pages, n_kv, page, D = _cache_shapes(k_cache, v_cache, k_scale, v_scale)

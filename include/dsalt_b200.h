@@ -375,6 +375,7 @@ int dsalt_append_cache(const void* k, const void* v, int dtype, int64_t T, int n
  *   [max(0, i - w + 1), i] and to the landmarks lmk [n_heads, n_seqs, k_lmk] p with
  *   0 <= p < i - w + 1 (any order, distinct, -1 = none), whose logits get lmk_bias (nullable).
  *   w null: to [0, i], k_lmk = 0.
+ * k_scale, v_scale: any positive numbers (dsalt_append_cache writes powers of two), or 0.
  * out [T, n_heads, head_dim] in out_dtype, lse [T, n_heads] (nullable, natural log). A query
  *   without keys and rows behind cu_q's last token give zeros and -inf.
  * Keys on a page number outside [0, n_pages) are left out and reported in the device status
