@@ -242,8 +242,9 @@ class DSALTLMHeadModel(nn.Module):
         if not all(lens):  # the layers see the prompts alone
             cu_h = [0] + [c for c, n in zip(cu_h[1:], lens) if n]
             cu = torch.tensor(cu_h, dtype=torch.int32, device=x.device)
-        for layer in self.layers:
-            x = layer.prefill(x, cu, cu_h, rope_cs, cache, plan)
+        with torch.cuda.device(x.device):  # the prompts' operators launch on the current device
+            for layer in self.layers:
+                x = layer.prefill(x, cu, cu_h, rope_cs, cache, plan)
         return cache.spread(self.lm_head(self.final_norm(x[cu[1:].long() - 1])))
 
     @torch.no_grad()
@@ -257,8 +258,9 @@ class DSALTLMHeadModel(nn.Module):
             raise ValueError(f"decode needs {cache.max_seqs} tokens, one per row")
         plan = cache.reserve([min(n, 1) for n in cache.lens])
         x, rope_cs = self._embed(cache.pick(tokens), plan.positions)
-        for layer in self.layers:
-            x = layer.decode(x, rope_cs, cache, plan)
+        with torch.cuda.device(x.device):
+            for layer in self.layers:
+                x = layer.decode(x, rope_cs, cache, plan)
         return cache.spread(self.lm_head(self.final_norm(x)))
 
     @torch.no_grad()

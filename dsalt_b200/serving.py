@@ -405,8 +405,9 @@ class PagedCache:
                 self.lmk[layer, :, r] = -1
                 continue
             end = b * block + 1
-            sets = ops.select_block_range(self.xnorm[layer, r, :end], self.vnorm[layer, r, :end],
-                                          self.width[layer, r, :end], alpha, k_lmk, H, block, b, b + 1)
+            with torch.cuda.device(self.lmk.device):
+                sets = ops.select_block_range(self.xnorm[layer, r, :end], self.vnorm[layer, r, :end],
+                                              self.width[layer, r, :end], alpha, k_lmk, H, block, b, b + 1)
             self.lmk[layer, :, r] = sets[:, 0]
 
     def attention(self, layer: int, q, w):

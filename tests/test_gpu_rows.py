@@ -115,3 +115,31 @@ def test_refusals_name_rows_that_hold_sequences():
     cache.release([0, 1])
     with pytest.raises(ValueError, match="prompt"):
         m.decode(a[:2], cache)
+
+
+def test_prompts_and_steps_make_their_device_the_current_one(monkeypatch):
+    """The signals, the selection and the packed attention launch on the current device: a model that is
+    elsewhere has to make its own the current one first (seen here by the guards that are entered)."""
+    from dsalt_b200 import ops
+    m = _model()
+    cache = m.new_cache(2, 200, page_size=16)
+    a, b = _prompts(140, 9)
+    guard, inside, calls = torch.cuda.device, [], []
+
+    class Recorded(guard):
+        def __enter__(self):
+            inside.append(self.idx)
+            return super().__enter__()
+
+        def __exit__(self, *args):
+            inside.pop()
+            return super().__exit__(*args)
+
+    monkeypatch.setattr(torch.cuda, "device", Recorded)
+    run = ops.L.call
+    monkeypatch.setattr(ops.L, "call", lambda name, *args: calls.append((name, list(inside))) or run(name, *args))
+    x = m.prefill(torch.cat([a, b]), _cu(140, 9), cache)
+    m.decode(x.argmax(1), cache)
+    older = [c for c in calls if c[0] in ("dsalt_token_signals", "dsalt_select_landmarks", "dsalt_attention_fwd",
+                                          "dsalt_select_block_range")]
+    assert len(older) >= 2 * 5 and all(at and at[-1] == cache.lmk.device.index for _, at in older)
