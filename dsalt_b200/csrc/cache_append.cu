@@ -21,10 +21,10 @@
 // from L1 or L2 again.
 //
 // Measured on a B200 (device time): 4 prompts of 8192 tokens, 12 heads of 64 in bf16 with pages of
-// 64 (132 MB: the prompts are ragged) 29.7 us (4.5 TB/s; copying as much takes 20.5): bound by memory and by the chain
+// 64 (132 MB: the prompts are ragged) 30.0 us (4.4 TB/s; copying as much takes 20.5): bound by memory and by the chain
 // that each block goes through (slots, runs, first pass, second pass), which the other two
 // blocks of an SM cover; without the fetches to L2 it takes 34.1 us. 64 decode rows of 16 heads
-// 3.1 us, next to nothing of which is bytes.
+// 3.0 us, next to nothing of which is bytes.
 #include <algorithm>
 #include <type_traits>
 

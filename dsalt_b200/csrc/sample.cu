@@ -33,7 +33,7 @@
 // passes find it in L1 or L2, which hold it for all rows under way.
 //
 // Measured on a B200 (device time, 64 rows of 151936 in bf16, 19 MB): the largest logit 9.9 us,
-// temperature alone 26.9, top-k 50 19.8, top-p 0.9 88, every row its own settings 95. Bytes are
+// temperature alone 27.1, top-k 50 19.8, top-p 0.9 88.5, every row its own settings 94.4. Bytes are
 // 3 us of each. Temperature alone is bound by the 64-bit instructions of the weights (10 per
 // element), the draws of a wide nucleus by latency: some ten steps of one cluster one after
 // another, of which the pass over the bins takes 15 us, the queue 11, the histogram and its

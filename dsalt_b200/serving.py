@@ -122,7 +122,8 @@ def reserve_slots(block_tables, seq_lens, new_lens, free_pages, n_free, page_siz
 def release_slots(block_tables, seq_lens, release, free_pages, n_free, page_size: int) -> None:
     """Gives the pages of the rows flagged in ``release [S]`` bool back to the stack, in place:
     their table entries become -1 and their lengths 0. Pages go back in the order in which
-    :func:`reserve_slots` would take them again."""
+    :func:`reserve_slots` would take them again. Rows that share a page are not counted: each
+    flagged row gives back every page of its table."""
     dev = _on_one_device(block_tables, seq_lens, release, free_pages, n_free)
     if block_tables.dim() != 2 or free_pages.dim() != 1:
         raise ValueError("block_tables must be [S, max_pages] and free_pages [N]")
@@ -295,7 +296,8 @@ class PagedCache:
     new tokens of each row, 0 among them, and what follows (:meth:`append`, :meth:`attention`)
     packs the tokens of the rows that have some. ``lens`` is the host's copy of the lengths, kept
     so that block borders are known without reading the device; a row whose tokens the pool or
-    the tables cannot hold is refused here, before anything is launched."""
+    the tables cannot hold is refused here, before anything is launched. The norms and widths are
+    not paged: ``8 + 4 n_kv_heads`` bytes per layer, row and position of ``max_len``."""
 
     def __init__(self, n_layers: int, n_heads: int, n_kv_heads: int, head_dim: int, k_lmk: int, *, max_seqs: int,
                  max_len: int, n_pages: int | None = None, page_size: int = 64, device="cuda"):

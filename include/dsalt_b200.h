@@ -335,7 +335,7 @@ int dsalt_core_forward(int mode, const void* x, int x_dtype, int d_model, int64_
  *   seq_lens and n_free). At most 8192 rows. slots and positions 16-byte aligned.
  * dsalt_release_slots: gives the pages of the rows flagged in release [n_seqs] bytes back to
  *   the stack, in the order in which reserve would take them again; their entries become -1
- *   and their lengths 0.
+ *   and their lengths 0. A page in the tables of two flagged rows is given back twice.
  */
 int dsalt_reserve_slots(int32_t* block_tables, int n_seqs, int max_pages, const int32_t* seq_lens,
                         const int32_t* new_lens, const int32_t* free_pages, int64_t free_capacity,
