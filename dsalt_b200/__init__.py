@@ -24,6 +24,12 @@ from .serving import (  # noqa: F401
     reserve_slots,
     sample_tokens,
 )
+from .layers import (  # noqa: F401
+    gated_ffn,
+    pack8,
+    qk_norm_rope,
+    unpack8,
+)
 from .module import DSALTAttention  # noqa: F401
 from .model import DSALTConfig, DSALTLMHeadModel, DSALTTransformerBlock  # noqa: F401
 from ._lib import DsaltError  # noqa: F401

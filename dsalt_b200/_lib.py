@@ -19,6 +19,8 @@ NOALLOC_MAX_SEQS = 4096  # DSALT_NOALLOC_MAX_SEQS
 NOALLOC_MAX_TOKENS = 1048576  # DSALT_NOALLOC_MAX_TOKENS
 SELECT_GLOBAL, SELECT_BLOCK_CAUSAL = 0, 1
 NORM_F32, NORM_INPUT = 0, 1
+ACT_SILU, ACT_GELU = 0, 1
+KEEP_NONE, KEEP_INPUT, KEEP_8BIT = 0, 1, 2
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -63,6 +65,19 @@ SIGNATURES = {
     "dsalt_cache_attention": (_I, [_P, _I, _I64, _I, _I, _I, _I64, _P, _P, _P, _P, _I64, _I, _P, _I, _P, _I, _P, _P,
                                    _P, _P, _I, _P, _I, _P, _P, _SZ, _P]),
     "dsalt_sample": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _F, _P, _I, _P, _F, _P, _F, _P, _P, _P]),
+    "dsalt_pack8": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _P]),
+    "dsalt_unpack8": (_I, [_P, _P, _I64, _I64, _P, _I, _P]),
+    "dsalt_qk_norm_rope": (_I, [_P, _P, _I, _I64, _I, _I, _I, _I64, _I64, _I64, _I64, _P, _P, _I, _F, _P, _P, _I64, _I64,
+                                _P, _P, _P, _P]),
+    "dsalt_qk_norm_rope_bwd_workspace_bytes": (_SZ, [_I]),
+    "dsalt_qk_norm_rope_bwd": (_I, [_P, _P, _P, _P, _I, _I64, _I, _I, _I] + [_I64] * 8 + [_P, _P, _I, _F, _P, _P, _I64,
+                                                                                         _I64] + [_P] * 6 + [_SZ, _P]),
+    "dsalt_gated_ffn_pitch": (_I64, [_I]),
+    "dsalt_gated_ffn_workspace_bytes": (_SZ, [_I, _I64, _I, _I, _I]),
+    "dsalt_gated_ffn": (_I, [_P, _I, _I64, _I, _I64, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _SZ, _P]),
+    "dsalt_gated_ffn_bwd_workspace_bytes": (_SZ, [_I, _I64, _I, _I, _I, _I]),
+    "dsalt_gated_ffn_bwd": (_I, [_P, _I, _I64, _I, _I64, _P, _I64, _P, _P, _P, _P, _I, _I, _I, _I] + [_P] * 7
+                            + [_SZ, _P]),
     "dsalt_peer_barrier": (_I, [_P, _P, _I, _I, _I, _P]),
     "dsalt_peer_allgather": (_I, [_P, _P, _I, _I, _I64, _P]),
     "dsalt_peer_copy": (_I, [_P, _P, _I64, _P]),

@@ -1,0 +1,61 @@
+// Shared by the kernels of the gated feed-forward block (ffn.cu, ffn_tc.cu).
+#pragma once
+
+#include "pack8.cuh"
+
+namespace dsalt {
+namespace ffn {
+
+// act(g) and act'(g) in fp32. silu: g p with p = 1 / (1 + e^-g); gelu: g p with p the normal
+// distribution's share below g.
+template <int ACT>
+__device__ __forceinline__ float activate(float g) {
+  if constexpr (ACT == DSALT_ACT_SILU) return __fdividef(g, 1.f + __expf(-g));
+  else return g * normcdff(g);
+}
+template <int ACT>
+__device__ __forceinline__ void activate_grad(float g, float& a, float& da) {
+  if constexpr (ACT == DSALT_ACT_SILU) {
+    const float p = __fdividef(1.f, 1.f + __expf(-g));
+    a = g * p;
+    da = p * (1.f + g * (1.f - p));
+  } else {
+    const float p = normcdff(g);
+    a = g * p;
+    da = p + g * 0.3989422804014327f * __expf(-0.5f * g * g);
+  }
+}
+
+inline int64_t pitch_of(int64_t d_ff) { return (d_ff + GROUP8 - 1) / GROUP8 * GROUP8; }
+
+// One call's sizes and operands. Rows of h, dg, du and of what is kept are `pitch` values long.
+struct Ffn {
+  int dtype, act, keep;
+  int64_t T;
+  int d, F, d_out;
+  int64_t pitch;
+  const void* w_gate;
+  const void* w_up;
+  const void* w_down;
+  const void* x;
+  int64_t x_stride;
+  void* kept;       // gate's and up's [2, T, pitch], in the input type or as codes
+  uint8_t* exps;    // [2, T, pitch / 32]
+  // forward
+  void* y;
+  void* h;          // [T, pitch]
+  // backward
+  const void* dy;
+  int64_t dy_stride;
+  void* dg;
+  void* du;
+  void* dx;
+  void* dw_gate;
+  void* dw_up;
+  void* dw_down;
+  float* wide;      // [T, pitch] fp32 once or twice (the path of ffn.cu's own products)
+  cudaStream_t stream;
+};
+
+}  // namespace ffn
+}  // namespace dsalt

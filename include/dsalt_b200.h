@@ -408,6 +408,82 @@ int dsalt_sample(const void* logits, int dtype, int64_t B, int64_t V, int64_t ro
                  const float* top_p, float top_p_value, const float* min_p, float min_p_value, int64_t* token,
                  float* logprob, void* stream);
 
+/*
+ * What a decoder block computes around its attention.
+ *
+ * dsalt_pack8, dsalt_unpack8: activations in 8 bits. Of a row, 32 neighbouring values (the last
+ *   group may be shorter) share the scale 2^(s - 127), kept as the byte s; a value is code *
+ *   2^(s - 127) with code = clamp(rint(x * 2^(127 - s)), -127, 127), s = max(E - 6, 1), E the fp32
+ *   exponent field of the group's largest magnitude. A group with a NaN or an infinity gets s = 255
+ *   and reads as NaN as a whole.
+ * x [rows, cols] of dtype (row stride in elements), codes [rows, cols] int8, exps
+ *   [rows, ceil(cols / 32)] bytes, out [rows, cols] contiguous (rounded to nearest even where its
+ *   type holds fewer bits).
+ */
+int dsalt_pack8(const void* x, int dtype, int64_t rows, int64_t cols, int64_t x_stride, int8_t* codes, uint8_t* exps,
+                void* stream);
+int dsalt_unpack8(const int8_t* codes, const uint8_t* exps, int64_t rows, int64_t cols, void* out, int dtype,
+                  void* stream);
+
+/*
+ * dsalt_qk_norm_rope: per head, RMS norm with a weight per channel (q_weight, k_weight [head_dim] of
+ * w_dtype; both null: no norm), then the half-split rotation by the token's angles.
+ * q [T, n_heads, head_dim], k [T, n_kv, head_dim] of dtype (token and head strides in elements;
+ *   16-byte aligned rows), q_out and k_out contiguous. head_dim a multiple of 16 (fp32: 8) up to 256.
+ * cos, sin [table_rows, at least head_dim / 2] fp32 (row stride table_stride, 16-byte aligned rows);
+ *   the angles of the first half's channels are read, the second half turns by the same. Token t
+ *   takes row positions[t], or row t where positions is null. A position outside the tables is
+ *   reported in the device status word (51) and taken as 0.
+ * dsalt_qk_norm_rope_bwd: gradients of q, k (contiguous, of dtype) and of the weights (of w_dtype)
+ *   from those of the outputs, dq_out and dk_out (token and head strides as above). Deterministic.
+ */
+int dsalt_qk_norm_rope(const void* q, const void* k, int dtype, int64_t T, int n_heads, int n_kv, int head_dim,
+                       int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
+                       const void* q_weight, const void* k_weight, int w_dtype, float eps, const float* cos,
+                       const float* sin, int64_t table_rows, int64_t table_stride, const int32_t* positions, void* q_out,
+                       void* k_out, void* stream);
+size_t dsalt_qk_norm_rope_bwd_workspace_bytes(int head_dim);
+int dsalt_qk_norm_rope_bwd(const void* q, const void* k, const void* dq_out, const void* dk_out, int dtype, int64_t T,
+                           int n_heads, int n_kv, int head_dim, int64_t q_token_stride, int64_t q_head_stride,
+                           int64_t k_token_stride, int64_t k_head_stride, int64_t dq_token_stride,
+                           int64_t dq_head_stride, int64_t dk_token_stride, int64_t dk_head_stride,
+                           const void* q_weight, const void* k_weight, int w_dtype, float eps, const float* cos,
+                           const float* sin, int64_t table_rows, int64_t table_stride, const int32_t* positions,
+                           void* dq, void* dk, void* dq_weight, void* dk_weight, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/*
+ * dsalt_gated_ffn: y = (act(x Wg^T) * (x Wu^T)) Wd^T.
+ * x [T, d_model] of dtype (row stride x_stride), w_gate, w_up [d_ff, d_model], w_down [d_out, d_ff], y
+ *   [T, d_out], contiguous, all of dtype. The product of gate and up is rounded to dtype before the
+ *   last product; sums are fp32. activation: DSALT_ACT_SILU, or DSALT_ACT_GELU (by the error function).
+ * keep: what the backward pass needs of x Wg^T and x Wu^T goes to kept [2, T, pitch], in dtype
+ *   (DSALT_KEEP_INPUT) or as codes with scales in kept_exps [2, T, pitch / 32] (DSALT_KEEP_8BIT, as
+ *   dsalt_pack8 forms them); pitch = dsalt_gated_ffn_pitch(d_ff), a multiple of 32. kept and workspace
+ *   256-byte aligned.
+ * dsalt_gated_ffn_bwd: the gradients (contiguous, of dtype; null: not wanted, dw_gate and dw_up go
+ *   together) from dy [T, d_out] (row stride dy_stride). With DSALT_KEEP_8BIT x holds the codes and
+ *   x_exps the scales of dsalt_pack8 (contiguous), else x is the forward's. x may be null where dw_gate is.
+ * 16-bit types whose sizes are multiples of 8 and whose rows are 16-byte aligned run on the tensor
+ *   cores, everything else on the CUDA cores. Deterministic.
+ */
+#define DSALT_ACT_SILU 0
+#define DSALT_ACT_GELU 1
+#define DSALT_KEEP_NONE 0
+#define DSALT_KEEP_INPUT 1
+#define DSALT_KEEP_8BIT 2
+int64_t dsalt_gated_ffn_pitch(int d_ff);
+size_t dsalt_gated_ffn_workspace_bytes(int dtype, int64_t T, int d_model, int d_ff, int d_out);
+int dsalt_gated_ffn(const void* x, int dtype, int64_t T, int d_model, int64_t x_stride, const void* w_gate,
+                    const void* w_up, const void* w_down, int d_ff, int d_out, int activation, int keep, void* kept,
+                    uint8_t* kept_exps, void* y, void* workspace, size_t workspace_bytes, void* stream);
+size_t dsalt_gated_ffn_bwd_workspace_bytes(int dtype, int64_t T, int d_model, int d_ff, int d_out, int keep);
+int dsalt_gated_ffn_bwd(const void* dy, int dtype, int64_t T, int d_model, int64_t dy_stride, const void* x,
+                        int64_t x_stride, const uint8_t* x_exps, const void* w_gate, const void* w_up,
+                        const void* w_down, int d_ff, int d_out, int activation, int keep, const void* kept,
+                        const uint8_t* kept_exps, void* dx, void* dw_gate, void* dw_up, void* dw_down, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
