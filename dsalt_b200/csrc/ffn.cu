@@ -194,6 +194,7 @@ int run_plain(const Ffn& f, bool backward) {
 }
 
 int run(const Ffn& f, bool backward) {
+  if (takes_tensor_cores(f)) return run_tensor_cores(f, backward);
   if (f.dtype == DSALT_F32) return run_plain<float>(f, backward);
   if (f.dtype == DSALT_BF16) return run_plain<__nv_bfloat16>(f, backward);
   return run_plain<__half>(f, backward);
@@ -201,6 +202,7 @@ int run(const Ffn& f, bool backward) {
 
 size_t a256(size_t v) { return (v + 255) & ~(size_t)255; }
 size_t elem_bytes(int dtype) { return dtype == DSALT_F32 ? 4 : 2; }
+bool off256(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 255) != 0; }
 bool known_dtype(int dt) { return dt == DSALT_F32 || dt == DSALT_BF16 || dt == DSALT_F16; }
 
 int check(const char* fn, int dtype, int64_t T, int d, int F, int d_out, int act, int keep) {
@@ -239,12 +241,13 @@ int dsalt_gated_ffn(const void* x, int dtype, int64_t T, int d_model, int64_t x_
   if (T > 1 && x_stride < d_model) return fail(DSALT_ERR_INVALID, "%s: rows overlap", FN);
   if (!x || !w_gate || !w_up || !w_down || !y || !workspace || (keep && !kept) || (keep == DSALT_KEEP_8BIT && !kept_exps))
     return fail(DSALT_ERR_INVALID, "%s: null pointer", FN);
+  if (off256(kept) || off256(workspace)) return fail(DSALT_ERR_INVALID, "%s: kept and workspace must be 256-byte aligned", FN);
   if (workspace_bytes < dsalt_gated_ffn_workspace_bytes(dtype, T, d_model, d_ff, d_out))
     return fail(DSALT_ERR_WORKSPACE, "%s: workspace of %zu bytes is too small", FN, workspace_bytes);
   Ffn f{};
   f.dtype = dtype, f.act = activation, f.keep = keep, f.T = T, f.d = d_model, f.F = d_ff, f.d_out = d_out;
   f.pitch = pitch_of(d_ff);
-  f.w_gate = w_gate, f.w_up = w_up, f.w_down = w_down, f.x = x, f.x_stride = x_stride, f.kept = kept, f.exps = kept_exps;
+  f.w_gate = w_gate, f.w_up = w_up, f.w_down = w_down, f.x = x, f.x_stride = T > 1 ? x_stride : d_model, f.kept = kept, f.exps = kept_exps;
   f.y = y;
   f.h = workspace;
   f.wide = reinterpret_cast<float*>(static_cast<char*>(workspace) + a256((size_t)T * f.pitch * elem_bytes(dtype)));
@@ -282,6 +285,7 @@ int dsalt_gated_ffn_bwd(const void* dy, int dtype, int64_t T, int d_model, int64
   if (T > 1 && (dy_stride < d_out || (!coded && x_stride < d_model))) return fail(DSALT_ERR_INVALID, "%s: rows overlap", FN);
   if (!dy || (dw_gate && (!x || (coded && !x_exps))) || !w_gate || !w_up || !w_down || !kept || (coded && !kept_exps) || !workspace)
     return fail(DSALT_ERR_INVALID, "%s: null pointer", FN);
+  if (off256(kept) || off256(workspace)) return fail(DSALT_ERR_INVALID, "%s: kept and workspace must be 256-byte aligned", FN);
   if (workspace_bytes < dsalt_gated_ffn_bwd_workspace_bytes(dtype, T, d_model, d_ff, d_out, keep))
     return fail(DSALT_ERR_WORKSPACE, "%s: workspace of %zu bytes is too small", FN, workspace_bytes);
   Ffn f{};
@@ -289,12 +293,12 @@ int dsalt_gated_ffn_bwd(const void* dy, int dtype, int64_t T, int d_model, int64
   f.pitch = pitch_of(d_ff);
   f.w_gate = w_gate, f.w_up = w_up, f.w_down = w_down;
   f.kept = const_cast<void*>(kept), f.exps = const_cast<uint8_t*>(kept_exps);
-  f.dy = dy, f.dy_stride = dy_stride, f.dx = dx, f.dw_gate = dw_gate, f.dw_up = dw_up, f.dw_down = dw_down;
+  f.dy = dy, f.dy_stride = T > 1 ? dy_stride : d_out, f.dx = dx, f.dw_gate = dw_gate, f.dw_up = dw_up, f.dw_down = dw_down;
   f.stream = s;
   const size_t n = a256((size_t)T * f.pitch * es);
   char* ws = static_cast<char*>(workspace);
   f.dg = ws, f.du = ws + n, f.h = ws + 2 * n, f.wide = reinterpret_cast<float*>(ws + 3 * n);
-  f.x = x, f.x_stride = x_stride;
+  f.x = coded ? nullptr : x, f.x_stride = T > 1 ? x_stride : d_model;
   if (coded && dw_gate) {
     void* wide_x = ws + 3 * n + a256((size_t)T * f.pitch * sizeof(float));
     if (int rc = launch_unpack8(static_cast<const int8_t*>(x), x_exps, T, d_model, wide_x, dtype, s)) return rc;

@@ -57,5 +57,9 @@ struct Ffn {
   cudaStream_t stream;
 };
 
+// 16-bit types whose sizes are multiples of 8 and whose rows are 16-byte aligned
+bool takes_tensor_cores(const Ffn& f);
+int run_tensor_cores(const Ffn& f, bool backward);
+
 }  // namespace ffn
 }  // namespace dsalt

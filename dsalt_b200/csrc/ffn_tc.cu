@@ -1,0 +1,619 @@
+// The gated feed-forward block on the tensor cores (bf16, fp16): one persistent matrix kernel whose
+// epilogue is the activation, its gradient, or a plain store.
+//
+//   forward    gate, up = x [Wg | Wu]^T -> epilogue: h = act(gate) up, gate and up kept if a gradient
+//              will be wanted;  y = h Wd^T
+//   backward   dh = dy Wd -> epilogue: dg = dh up act'(gate), du = dh act(gate), h again;
+//              dx = dg Wg + du Wu (one sum over both);  dWg = dg^T x, dWu = du^T x, dWd = dy^T h (one
+//              launch, so that the tiles of the three fill the GPU together)
+//
+// Two CTAs share a tile of 256 x 256 outputs (tcgen05.mma of the pair: each holds 128 rows of A
+// and 128 of B, and reads the other's B through it), 64 values of K a stage, five stages of 32 KB a CTA. The
+// accumulators of two tiles lie in TMEM (2 x 256 columns), so that a tile's epilogue runs under the
+// next one's products. A tile of the first product is 128 columns of gate beside the same 128 of up:
+// one CTA of the pair loads gate's rows, the other up's, and a thread finds both in its row. Operands whose
+// K runs along memory rows or across them (weights and gradients as they lie) are both read as they
+// are, by the major-ness of the matrix descriptors; nothing is transposed in memory.
+//
+// Bound by the tensor cores where K is long; the backward's first product moves 6 bytes out and 2 to 4
+// in for each of its T x d_ff outputs and is bound by memory where d_out is below about 1000.
+#include <cuda.h>
+
+#include "ffn.cuh"
+
+namespace dsalt {
+namespace ffn {
+namespace {
+
+constexpr int PAIR_M = 256, CTA_M = 128, PAIR_N = 256, KB = 64, STAGES = 5;
+constexpr int OPERAND_BYTES = CTA_M * KB * 2, STAGE_BYTES = 2 * OPERAND_BYTES;
+constexpr int EPI_WARPS = 8, THREADS = 32 * (4 + EPI_WARPS);
+constexpr int BOX = 32, BOX_BYTES = BOX * BOX * 2, BOXES = 3;  // a warp's staged outputs
+constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + EPI_WARPS * BOXES * BOX_BYTES + 256;
+constexpr uint32_t TMEM_COLS = 512;
+constexpr int GROUP_M = 8;  // tiles of 256 rows whose A stays in L2 while N is walked
+
+enum Epilogue { PLAIN = 0, GATE_UP = 1, GRADS = 2 };
+
+struct alignas(64) Job {
+  CUtensorMap a[2], b[2];  // of both segments of K; the first product: gate's and up's rows
+  CUtensorMap c[3];
+  int tiles_m, tiles_n, blocks0, blocks;  // blocks of K in the first segment and in all
+  int rows, cols;                         // of the outputs
+};
+struct Kept {
+  void* p;           // gate's and up's [2, T, pitch]
+  uint8_t* exps;
+  int64_t T, pitch;
+};
+template <int NJ>
+struct Args {
+  Job job[NJ];
+  Kept kept;
+  int tiles;
+  uint32_t idesc;
+  int* err;
+};
+
+// ---------------------------------------------------------------- pair-wide forms
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t in_cta(uint32_t smem_addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// load into this CTA's shared memory, counted on a barrier of the pair
+__device__ __forceinline__ void load_2d(uint32_t dst, const void* map, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], "
+      "[%2];" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void store_2d(const void* map, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src),
+               "r"(c0), "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void store_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void pair_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// arrives on the barrier at this offset in both CTAs once the thread's products so far are done
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+// ---------------------------------------------------------------- shared memory
+struct Bars {
+  uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
+  uint32_t tmem;
+};
+
+struct Tile {
+  int job, m, n;
+};
+template <int NJ>
+__device__ __forceinline__ Tile find_tile(const Args<NJ>& a, int t) {
+  int j = 0;
+#pragma unroll
+  for (int i = 0; i + 1 < NJ; ++i) {
+    const int n = a.job[i].tiles_m * a.job[i].tiles_n;
+    if (j == i && t >= n) {
+      t -= n;
+      ++j;
+    }
+  }
+  const int tm = a.job[j].tiles_m, tn = a.job[j].tiles_n;
+  const int group = t / (GROUP_M * tn), first = group * GROUP_M, rows = min(GROUP_M, tm - first);
+  const int r = t - group * GROUP_M * tn;
+  return {j, first + r % rows, r / rows};
+}
+
+// 32 values of a row as fp32 into the warp's box (64 bytes a row, 16-byte pieces swizzled as the
+// store's map has it: piece ^ row / 2)
+template <typename T>
+__device__ __forceinline__ void stage_row(uint32_t box, int lane, const float (&f)[BOX]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint32_t at = box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4);
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(narrow2<T>(f[8 * c], f[8 * c + 1])),
+                 "r"(narrow2<T>(f[8 * c + 2], f[8 * c + 3])), "r"(narrow2<T>(f[8 * c + 4], f[8 * c + 5])),
+                 "r"(narrow2<T>(f[8 * c + 6], f[8 * c + 7]))
+                 : "memory");
+  }
+}
+__device__ __forceinline__ void load_acc(uint32_t taddr, float (&f)[BOX]) {
+  uint32_t r[32];
+  DSALT_TMEM_LD32(taddr, r);
+  tmem_wait_ld();
+#pragma unroll
+  for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void load_32b(uint32_t (&u)[8], const void* p) {
+  asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
+               : "l"(__cvta_generic_to_global(p)));
+}
+// one value per row and group of 32 columns: the scale byte, and the codes into `at`
+__device__ __forceinline__ uint32_t store_codes(const float (&f)[BOX], int8_t* at) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < BOX; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+  const uint32_t s = scale_byte(top);
+  uint32_t w[8];
+  pack_codes<BOX>(f, s, w);
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(__cvta_generic_to_global(at)), "r"(w[0]), "r"(w[1]),
+               "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+  return s;
+}
+
+// what the backward's first epilogue reads for 32 columns of a row
+template <typename T, int KEEP>
+struct KeptRow {
+  uint32_t g[KEEP == DSALT_KEEP_8BIT ? 8 : 16], u[KEEP == DSALT_KEEP_8BIT ? 8 : 16];
+  uint32_t sg, su;
+  __device__ __forceinline__ void load(const Kept& k, int64_t row, int64_t col) {
+    const int64_t plane = k.T * k.pitch, at = row * k.pitch + col;
+    const bool in = row < k.T && col < k.pitch;
+    if constexpr (KEEP == DSALT_KEEP_8BIT) {
+      sg = su = 127;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) g[i] = u[i] = 0;
+      if (in) {
+        load_32b(g, static_cast<const int8_t*>(k.p) + at);
+        load_32b(u, static_cast<const int8_t*>(k.p) + plane + at);
+        sg = k.exps[at / GROUP8];
+        su = k.exps[(plane + at) / GROUP8];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) g[i] = u[i] = 0;
+      if (in) {
+        const T* p = static_cast<const T*>(k.p) + at;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t a[8], b[8];
+          load_32b(a, p + 16 * i);
+          load_32b(b, p + plane + 16 * i);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) g[8 * i + j] = a[j], u[8 * i + j] = b[j];
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void values(float (&a)[BOX], float (&b)[BOX]) const {
+    if constexpr (KEEP == DSALT_KEEP_8BIT) {
+      unpack_codes<BOX>(g, scale_of(sg), a);
+      unpack_codes<BOX>(u, scale_of(su), b);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        widen2<T>(g[i], a[2 * i], a[2 * i + 1]);
+        widen2<T>(u[i], b[2 * i], b[2 * i + 1]);
+      }
+    }
+  }
+};
+
+// ---------------------------------------------------------------- the kernel
+template <int EPI, bool A_MN, bool B_MN, typename T, int ACT, int KEEP, int NJ>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    ffn_pair_kernel(const __grid_constant__ Args<NJ> args) {
+  extern __shared__ uint8_t raw[];
+  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+  const uint32_t staging = base + STAGES * STAGE_BYTES;
+  Bars& bars = *reinterpret_cast<Bars*>(raw + (staging + EPI_WARPS * BOXES * BOX_BYTES - smem_u32(raw)));
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = cluster_rank() & 1u;
+  const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&bars.full[i], 1);
+      mbar_init(&bars.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.acc_full[i], 1);
+      mbar_init(&bars.acc_empty[i], 2 * EPI_WARPS);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem)),
+                 "r"(TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem;
+
+  if (warp == 0) {
+    if (lane == 0) {  // loads of this CTA's halves of A and B
+      int s = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair; ok && t < args.tiles; t += pairs) {
+        const Tile tile = find_tile<NJ>(args, t);
+        const Job& job = args.job[tile.job];
+        const int m0 = tile.m * PAIR_M + (int)rank * CTA_M;
+        const int n0 = EPI == GATE_UP ? tile.n * (PAIR_N / 2) : tile.n * PAIR_N + (int)rank * (PAIR_N / 2);
+        for (int kb = 0; kb < job.blocks; ++kb) {
+          if (!mbar_wait(&bars.empty[s], phase ^ 1, args.err, 61)) {
+            ok = false;
+            break;
+          }
+          if (rank == 0) mbar_arrive_expect_tx(&bars.full[s], 2 * STAGE_BYTES);
+          const uint32_t full = in_cta(smem_u32(&bars.full[s]), 0);
+          const int seg = kb >= job.blocks0, k = (seg ? kb - job.blocks0 : kb) * KB;
+          const uint32_t a = base + s * STAGE_BYTES, b = a + OPERAND_BYTES;
+          const CUtensorMap* ma = &job.a[seg];
+          const CUtensorMap* mb = &job.b[EPI == GATE_UP ? (int)rank : seg];
+          if constexpr (A_MN) {
+            load_2d(a, ma, full, m0, k);
+            load_2d(a + OPERAND_BYTES / 2, ma, full, m0 + 64, k);
+          } else {
+            load_2d(a, ma, full, k, m0);
+          }
+          if constexpr (B_MN) {
+            load_2d(b, mb, full, n0, k);
+            load_2d(b + OPERAND_BYTES / 2, mb, full, n0 + 64, k);
+          } else {
+            load_2d(b, mb, full, k, n0);
+          }
+          if (++s == STAGES) {
+            s = 0;
+            phase ^= 1;
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0 && lane == 0) {  // products of the pair
+      int s = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair; ok && t < args.tiles; t += pairs, ++it) {
+        const Tile tile = find_tile<NJ>(args, t);
+        const int blocks = args.job[tile.job].blocks, acc = it & 1;
+        if (!mbar_wait(&bars.acc_empty[acc], ((it >> 1) & 1) ^ 1, args.err, 62)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + acc * PAIR_N;
+        for (int kb = 0; kb < blocks; ++kb) {
+          if (!mbar_wait(&bars.full[s], phase, args.err, 63)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a = base + s * STAGE_BYTES, b = a + OPERAND_BYTES;
+#pragma unroll
+          for (int ks = 0; ks < KB / 16; ++ks) {
+            // K along rows of 128 bytes: 16 values are 32 bytes on; across: 16 rows of 128 bytes
+            const uint64_t da = A_MN ? sw128_desc(a + ks * 2048, OPERAND_BYTES / 2, 1024) : sw128_desc(a + ks * 32, 16, 1024);
+            const uint64_t db = B_MN ? sw128_desc(b + ks * 2048, OPERAND_BYTES / 2, 1024) : sw128_desc(b + ks * 32, 16, 1024);
+            pair_mma(d, da, db, args.idesc, kb | ks);
+          }
+          pair_commit(&bars.empty[s]);
+          if (++s == STAGES) {
+            s = 0;
+            phase ^= 1;
+          }
+        }
+        if (ok) pair_commit(&bars.acc_full[acc]);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    const int quad = warp % 4, side = (warp - 4) / 4;  // 32 rows, a half of the columns
+    const uint32_t boxes = staging + (warp - 4) * BOXES * BOX_BYTES;
+    int it = 0, slot = 0;
+    for (int t = pair; t < args.tiles; t += pairs, ++it) {
+      const Tile tile = find_tile<NJ>(args, t);
+      const Job& job = args.job[tile.job];
+      const int acc = it & 1;
+      const int row0 = tile.m * PAIR_M + (int)rank * CTA_M + quad * 32;
+      const uint32_t ta = tmem + acc * PAIR_N + ((uint32_t)(quad * 32) << 16);
+      // the boxes are written once earlier stores have read them
+      auto free_boxes = [&]() {
+        if (lane == 0) store_wait_read<0>();
+        __syncwarp();
+      };
+      auto send = [&](int box, const CUtensorMap* map, int col) {
+        if (lane == 0 && row0 < job.rows && col < job.cols) store_2d(map, boxes + box * BOX_BYTES, col, row0);
+      };
+      if constexpr (EPI == GRADS) {
+        const int col0 = tile.n * PAIR_N + side * (PAIR_N / 2);
+        KeptRow<T, KEEP> kept;
+        kept.load(args.kept, row0 + lane, col0);
+        if (!mbar_wait(&bars.acc_full[acc], (it >> 1) & 1, args.err, 64)) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < PAIR_N / 2; c += BOX) {
+          float a[BOX], b[BOX], d[BOX];
+          kept.values(a, b);
+          if (c + BOX < PAIR_N / 2) kept.load(args.kept, row0 + lane, col0 + c + BOX);
+          load_acc(ta + side * (PAIR_N / 2) + c, d);
+#pragma unroll
+          for (int i = 0; i < BOX; ++i) {
+            float v, dv;
+            activate_grad<ACT>(a[i], v, dv);
+            a[i] = d[i] * b[i] * dv;
+            b[i] *= v;
+            d[i] *= v;
+          }
+          free_boxes();
+          stage_row<T>(boxes, lane, b);
+          stage_row<T>(boxes + BOX_BYTES, lane, a);
+          stage_row<T>(boxes + 2 * BOX_BYTES, lane, d);
+          fence_proxy_async_smem();
+          __syncwarp();
+          send(0, &job.c[0], col0 + c);
+          send(1, &job.c[1], col0 + c);
+          send(2, &job.c[2], col0 + c);
+          if (lane == 0) store_commit();
+        }
+      } else if constexpr (EPI == GATE_UP) {
+        if (!mbar_wait(&bars.acc_full[acc], (it >> 1) & 1, args.err, 64)) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = side * 64; c < side * 64 + 64; c += BOX) {
+          const int col = tile.n * (PAIR_N / 2) + c;
+          float g[BOX], u[BOX], h[BOX];
+          load_acc(ta + c, g);
+          load_acc(ta + PAIR_N / 2 + c, u);
+#pragma unroll
+          for (int i = 0; i < BOX; ++i) h[i] = activate<ACT>(g[i]) * u[i];
+          if constexpr (KEEP == DSALT_KEEP_8BIT) {
+            const int64_t row = row0 + lane, at = row * args.kept.pitch + col, plane = args.kept.T * args.kept.pitch;
+            if (row < args.kept.T && col < args.kept.pitch) {
+              int8_t* codes = static_cast<int8_t*>(args.kept.p);
+              args.kept.exps[at / GROUP8] = (uint8_t)store_codes(g, codes + at);
+              args.kept.exps[(plane + at) / GROUP8] = (uint8_t)store_codes(u, codes + plane + at);
+            }
+          }
+          free_boxes();
+          stage_row<T>(boxes, lane, h);
+          if constexpr (KEEP == DSALT_KEEP_INPUT) {
+            stage_row<T>(boxes + BOX_BYTES, lane, g);
+            stage_row<T>(boxes + 2 * BOX_BYTES, lane, u);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          send(0, &job.c[0], col);
+          if constexpr (KEEP == DSALT_KEEP_INPUT) {
+            send(1, &job.c[1], col);
+            send(2, &job.c[2], col);
+          }
+          if (lane == 0) store_commit();
+        }
+      } else {
+        if (!mbar_wait(&bars.acc_full[acc], (it >> 1) & 1, args.err, 64)) break;
+        tc_fence_after();
+        const int col0 = tile.n * PAIR_N + side * (PAIR_N / 2);
+#pragma unroll 1
+        for (int c = 0; c < PAIR_N / 2; c += BOX) {
+          float d[BOX];
+          load_acc(ta + side * (PAIR_N / 2) + c, d);
+          if (lane == 0) store_wait_read<BOXES - 1>();
+          __syncwarp();
+          stage_row<T>(boxes + slot * BOX_BYTES, lane, d);
+          fence_proxy_async_smem();
+          __syncwarp();
+          send(slot, &job.c[0], col0 + c);
+          if (lane == 0) store_commit();
+          slot = slot + 1 == BOXES ? 0 : slot + 1;
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_remote(in_cta(smem_u32(&bars.acc_empty[acc]), 0));
+    }
+    if (lane == 0) store_wait_all();
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // the other CTA's barriers and operands are not touched after this
+  if (warp == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+}
+
+// ---------------------------------------------------------------- host side
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn get_encode() {
+  static const EncodeTiledFn fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+                    q == cudaDriverEntryPointSuccess;
+    return ok ? reinterpret_cast<EncodeTiledFn>(ptr) : nullptr;
+  }();
+  return fn;
+}
+
+// rows x cols values of 16 bits, `stride` values from row to row, in boxes of box_rows x box_cols
+int make_map(CUtensorMap* m, const void* p, int dtype, int64_t rows, int64_t cols, int64_t stride, int box_rows,
+             int box_cols, bool store) {
+  const EncodeTiledFn enc = get_encode();
+  if (!enc) return fail(DSALT_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
+  const cuuint32_t step[2] = {1, 1};
+  const CUresult r = enc(m, dtype == DSALT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                         const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         store ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(DSALT_ERR_CUDA, "gated_ffn: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return DSALT_OK;
+}
+// an operand: K along its rows (128 rows of 64 values of K), or across them (64 rows of K, 64 columns)
+int operand(CUtensorMap* m, const void* p, const Ffn& f, int64_t rows, int64_t cols, int64_t stride, bool across) {
+  return make_map(m, p, f.dtype, rows, cols, stride, across ? KB : CTA_M, 64, false);
+}
+int output(CUtensorMap* m, void* p, const Ffn& f, int64_t rows, int64_t cols, int64_t stride) {
+  return make_map(m, p, f.dtype, rows, cols, stride, BOX, BOX, true);
+}
+int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+void size_job(Job& j, int64_t M, int64_t N, int64_t K, int tile_n) {
+  j.tiles_m = ceil_div(M, PAIR_M);
+  j.tiles_n = ceil_div(N, tile_n);
+  j.blocks0 = j.blocks = ceil_div(K, KB);
+  j.rows = (int)M;
+  j.cols = (int)N;
+}
+
+template <int EPI, bool A_MN, bool B_MN, typename T, int ACT, int KEEP, int NJ>
+int launch_pair(Args<NJ>& a, const Ffn& f, const char* what) {
+  static std::atomic<uint64_t> ready{0};
+  auto kernel = ffn_pair_kernel<EPI, A_MN, B_MN, T, ACT, KEEP, NJ>;
+  if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), SMEM_BYTES, ready)) return rc;
+  a.tiles = 0;
+  for (int i = 0; i < NJ; ++i) a.tiles += a.job[i].tiles_m * a.job[i].tiles_n;
+  a.idesc = umma_idesc_f16(f.dtype == DSALT_BF16 ? 1 : 0, A_MN, B_MN, PAIR_M, PAIR_N);
+  a.err = device_status_ptr();
+  const int pairs = a.tiles < 74 ? a.tiles : 74;
+  kernel<<<2 * pairs, THREADS, SMEM_BYTES, f.stream>>>(a);
+  return check_cuda(cudaGetLastError(), what);
+}
+
+template <typename T, int ACT, int KEEP>
+int gate_up(const Ffn& f) {
+  Args<1> a{};
+  Job& j = a.job[0];
+  size_job(j, f.T, f.F, f.d, PAIR_N / 2);
+  int rc;
+  if ((rc = operand(&j.a[0], f.x, f, f.T, f.d, f.x_stride, false)) || (rc = operand(&j.b[0], f.w_gate, f, f.F, f.d, f.d, false)) ||
+      (rc = operand(&j.b[1], f.w_up, f, f.F, f.d, f.d, false)) || (rc = output(&j.c[0], f.h, f, f.T, f.F, f.pitch)))
+    return rc;
+  if (KEEP == DSALT_KEEP_INPUT) {
+    T* kept = static_cast<T*>(f.kept);
+    if ((rc = output(&j.c[1], kept, f, f.T, f.F, f.pitch)) || (rc = output(&j.c[2], kept + f.T * f.pitch, f, f.T, f.F, f.pitch)))
+      return rc;
+  }
+  a.kept = {f.kept, f.exps, f.T, f.pitch};
+  return launch_pair<GATE_UP, false, false, T, ACT, KEEP, 1>(a, f, "gated_ffn gate and up launch");
+}
+
+template <typename T, int ACT>
+int forward(const Ffn& f) {
+  int rc = f.keep == DSALT_KEEP_NONE ? gate_up<T, ACT, DSALT_KEEP_NONE>(f)
+           : f.keep == DSALT_KEEP_INPUT ? gate_up<T, ACT, DSALT_KEEP_INPUT>(f)
+                                        : gate_up<T, ACT, DSALT_KEEP_8BIT>(f);
+  if (rc) return rc;
+  Args<1> a{};
+  Job& j = a.job[0];
+  size_job(j, f.T, f.d_out, f.F, PAIR_N);
+  if ((rc = operand(&j.a[0], f.h, f, f.T, f.F, f.pitch, false)) ||
+      (rc = operand(&j.b[0], f.w_down, f, f.d_out, f.F, f.F, false)) || (rc = output(&j.c[0], f.y, f, f.T, f.d_out, f.d_out)))
+    return rc;
+  return launch_pair<PLAIN, false, false, T, 0, 0, 1>(a, f, "gated_ffn down launch");
+}
+
+template <typename T, int ACT, int KEEP>
+int grads(const Ffn& f) {
+  Args<1> a{};
+  Job& j = a.job[0];
+  size_job(j, f.T, f.F, f.d_out, PAIR_N);
+  int rc;
+  if ((rc = operand(&j.a[0], f.dy, f, f.T, f.d_out, f.dy_stride, false)) ||
+      (rc = operand(&j.b[0], f.w_down, f, f.d_out, f.F, f.F, true)) || (rc = output(&j.c[0], f.h, f, f.T, f.F, f.pitch)) ||
+      (rc = output(&j.c[1], f.dg, f, f.T, f.F, f.pitch)) || (rc = output(&j.c[2], f.du, f, f.T, f.F, f.pitch)))
+    return rc;
+  a.kept = {f.kept, f.exps, f.T, f.pitch};
+  return launch_pair<GRADS, false, true, T, ACT, KEEP, 1>(a, f, "gated_ffn_bwd hidden gradients launch");
+}
+
+int weight_job(Job& j, const Ffn& f, const void* a, int64_t M, int64_t a_stride, const void* b, int64_t N, int64_t b_stride,
+               void* c) {
+  size_job(j, M, N, f.T, PAIR_N);
+  int rc;
+  if ((rc = operand(&j.a[0], a, f, f.T, M, a_stride, true)) || (rc = operand(&j.b[0], b, f, f.T, N, b_stride, true))) return rc;
+  return output(&j.c[0], c, f, M, N, N);
+}
+
+template <typename T, int ACT>
+int backward(const Ffn& f) {
+  int rc = f.keep == DSALT_KEEP_8BIT ? grads<T, ACT, DSALT_KEEP_8BIT>(f) : grads<T, ACT, DSALT_KEEP_INPUT>(f);
+  if (rc) return rc;
+  if (f.dx) {
+    Args<1> a{};
+    Job& j = a.job[0];
+    size_job(j, f.T, f.d, f.F, PAIR_N);
+    j.blocks = 2 * j.blocks0;
+    if ((rc = operand(&j.a[0], f.dg, f, f.T, f.F, f.pitch, false)) || (rc = operand(&j.a[1], f.du, f, f.T, f.F, f.pitch, false)) ||
+        (rc = operand(&j.b[0], f.w_gate, f, f.F, f.d, f.d, true)) || (rc = operand(&j.b[1], f.w_up, f, f.F, f.d, f.d, true)) ||
+        (rc = output(&j.c[0], f.dx, f, f.T, f.d, f.d)))
+      return rc;
+    if ((rc = launch_pair<PLAIN, false, true, T, 0, 0, 1>(a, f, "gated_ffn_bwd dx launch"))) return rc;
+  }
+  if (!f.dw_gate && !f.dw_down) return DSALT_OK;
+  Args<3> a{};
+  if (f.dw_down && (rc = weight_job(a.job[0], f, f.dy, f.d_out, f.dy_stride, f.h, f.F, f.pitch, f.dw_down))) return rc;
+  if (f.dw_gate && ((rc = weight_job(a.job[1], f, f.dg, f.F, f.pitch, f.x, f.d, f.x_stride, f.dw_gate)) ||
+                    (rc = weight_job(a.job[2], f, f.du, f.F, f.pitch, f.x, f.d, f.x_stride, f.dw_up))))
+    return rc;
+  return launch_pair<PLAIN, true, true, T, 0, 0, 3>(a, f, "gated_ffn_bwd weights launch");
+}
+
+template <typename T>
+int run_typed(const Ffn& f, bool back) {
+  if (f.act == DSALT_ACT_SILU) return back ? backward<T, DSALT_ACT_SILU>(f) : forward<T, DSALT_ACT_SILU>(f);
+  return back ? backward<T, DSALT_ACT_GELU>(f) : forward<T, DSALT_ACT_GELU>(f);
+}
+
+bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+
+}  // namespace
+
+bool takes_tensor_cores(const Ffn& f) {
+  if (f.dtype == DSALT_F32 || f.d % 8 || f.F % 8 || f.d_out % 8) return false;
+  if (off16(f.w_gate) || off16(f.w_up) || off16(f.w_down)) return false;
+  if ((f.x && (off16(f.x) || f.x_stride % 8)) || (f.dy && (off16(f.dy) || f.dy_stride % 8))) return false;
+  for (const void* p : {(const void*)f.y, (const void*)f.dx, (const void*)f.dw_gate, (const void*)f.dw_up, (const void*)f.dw_down})
+    if (off16(p)) return false;
+  return true;
+}
+
+int run_tensor_cores(const Ffn& f, bool back) {
+  // the tensor maps are made by the driver, which wants the thread's context: a thread that autograd
+  // started has the device set, but no context until the runtime is told so
+  int dev = 0;
+  int rc;
+  if ((rc = check_cuda(cudaGetDevice(&dev), "current device")) || (rc = check_cuda(cudaSetDevice(dev), "current device"))) return rc;
+  return f.dtype == DSALT_BF16 ? run_typed<__nv_bfloat16>(f, back) : run_typed<__half>(f, back);
+}
+
+}  // namespace ffn
+}  // namespace dsalt

@@ -375,7 +375,7 @@ def ffn_inputs(T, d, F, d_out, dtype, seed=0):
 @pytest.mark.parametrize("T,d,F,d_out,act", [
     (1, 64, 96, 64, "silu"), (1, 8, 8, 8, "gelu"), (3, 72, 40, 24, "silu"), (17, 256, 768, 256, "gelu"),
     (64, 512, 1408, 512, "silu"), (127, 128, 136, 200, "silu"), (300, 264, 520, 136, "gelu"), (513, 768, 2048, 768, "silu"),
-    (1000, 200, 328, 200, "silu")])
+    (1000, 200, 328, 200, "silu"), (2500, 512, 1408, 512, "silu"), (4100, 264, 2824, 520, "gelu")])
 def test_ffn_matches_the_oracle(Y, dtype, keep, T, d, F, d_out, act):
     x, wg, wu, wd, dy = ffn_inputs(T, d, F, d_out, TYPES[dtype])
     check_ffn(Y, x, wg, wu, wd, act, keep, dy)
