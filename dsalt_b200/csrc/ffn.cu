@@ -105,7 +105,8 @@ __global__ void __launch_bounds__(THREADS) act_kernel(const float* __restrict__ 
 template <typename T, int ACT>
 __global__ void __launch_bounds__(THREADS) act_grad_kernel(const float* __restrict__ dh, int64_t T_, int F, int64_t pitch,
                                                            const void* kept, const uint8_t* __restrict__ exps, int keep,
-                                                           T* __restrict__ h, T* __restrict__ dg, T* __restrict__ du) {
+                                                           T* __restrict__ h,  // nullable: it was kept
+                                                           T* __restrict__ dg, T* __restrict__ du) {
   const int64_t total = T_ * pitch;
   for (int64_t at = (int64_t)blockIdx.x * THREADS + threadIdx.x; at < total; at += (int64_t)gridDim.x * THREADS) {
     float a, b;
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(THREADS) act_grad_kernel(const float* __restri
     const float d = at % pitch < F ? dh[at] : 0.f;
     float v, dv;
     activate_grad<ACT>(a, v, dv);
-    h[at] = from_float<T>(v * b);
+    if (h) h[at] = from_float<T>(v * b);
     dg[at] = from_float<T>(d * b * dv);
     du[at] = from_float<T>(d * v);
   }
@@ -169,7 +170,8 @@ int backward_plain(const Ffn& f) {
   const Product dh = {{{f.dy, f.dy_stride, 1}}, {{f.w_down, 1, f.F}}, 1, f.T, f.F, f.d_out, f.pitch};
   if ((rc = product<T, float>(dh, f.wide, f.stream, "gated_ffn_bwd product launch"))) return rc;
   act_grad_kernel<T, ACT><<<blocks_for(f.T * f.pitch), THREADS, 0, f.stream>>>(
-      f.wide, f.T, f.F, f.pitch, f.kept, f.exps, f.keep, static_cast<T*>(f.h), static_cast<T*>(f.dg), static_cast<T*>(f.du));
+      f.wide, f.T, f.F, f.pitch, f.kept, f.exps, f.keep, f.keep == DSALT_KEEP_8BIT ? static_cast<T*>(f.h) : nullptr,
+      static_cast<T*>(f.dg), static_cast<T*>(f.du));
   if ((rc = check_cuda(cudaGetLastError(), "gated_ffn_bwd activation launch"))) return rc;
   if (f.dx) {
     const Product p = {{{f.dg, f.pitch, 1}, {f.du, f.pitch, 1}}, {{f.w_gate, 1, f.d}, {f.w_up, 1, f.d}}, 2, f.T, f.d, f.F, f.d};
@@ -249,7 +251,7 @@ int dsalt_gated_ffn(const void* x, int dtype, int64_t T, int d_model, int64_t x_
   f.pitch = pitch_of(d_ff);
   f.w_gate = w_gate, f.w_up = w_up, f.w_down = w_down, f.x = x, f.x_stride = T > 1 ? x_stride : d_model, f.kept = kept, f.exps = kept_exps;
   f.y = y;
-  f.h = workspace;
+  f.h = keep == DSALT_KEEP_INPUT ? static_cast<char*>(kept) + 2 * T * f.pitch * elem_bytes(dtype) : workspace;
   f.wide = reinterpret_cast<float*>(static_cast<char*>(workspace) + a256((size_t)T * f.pitch * elem_bytes(dtype)));
   f.stream = static_cast<cudaStream_t>(stream);
   return run(f, false);
@@ -297,7 +299,8 @@ int dsalt_gated_ffn_bwd(const void* dy, int dtype, int64_t T, int d_model, int64
   f.stream = s;
   const size_t n = a256((size_t)T * f.pitch * es);
   char* ws = static_cast<char*>(workspace);
-  f.dg = ws, f.du = ws + n, f.h = ws + 2 * n, f.wide = reinterpret_cast<float*>(ws + 3 * n);
+  f.dg = ws, f.du = ws + n, f.wide = reinterpret_cast<float*>(ws + 3 * n);
+  f.h = coded ? ws + 2 * n : static_cast<char*>(f.kept) + 2 * T * f.pitch * es;
   f.x = coded ? nullptr : x, f.x_stride = T > 1 ? x_stride : d_model;
   if (coded && dw_gate) {
     void* wide_x = ws + 3 * n + a256((size_t)T * f.pitch * sizeof(float));

@@ -39,7 +39,7 @@ struct Ffn {
   const void* w_down;
   const void* x;
   int64_t x_stride;
-  void* kept;       // gate's and up's [2, T, pitch], in the input type or as codes
+  void* kept;       // gate's, up's and h [3, T, pitch] in the input type, or gate's and up's codes [2, T, pitch]
   uint8_t* exps;    // [2, T, pitch / 32]
   // forward
   void* y;

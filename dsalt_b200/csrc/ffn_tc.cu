@@ -3,20 +3,22 @@
 //
 //   forward    gate, up = x [Wg | Wu]^T -> epilogue: h = act(gate) up, gate and up kept if a gradient
 //              will be wanted;  y = h Wd^T
-//   backward   dh = dy Wd -> epilogue: dg = dh up act'(gate), du = dh act(gate), h again;
+//   backward   dh = dy Wd -> epilogue: dg = dh up act'(gate), du = dh act(gate), of 8-bit
+//              activations h again;
 //              dx = dg Wg + du Wu (one sum over both);  dWg = dg^T x, dWu = du^T x, dWd = dy^T h (one
 //              launch, so that the tiles of the three fill the GPU together)
 //
 // Two CTAs share a tile of 256 x 256 outputs (tcgen05.mma of the pair: each holds 128 rows of A
-// and 128 of B, and reads the other's B through it), 64 values of K a stage, five stages of 32 KB a CTA. The
+// and 128 of B, and reads the other's B through it), 64 values of K and 32 KB a CTA in a stage. The
 // accumulators of two tiles lie in TMEM (2 x 256 columns), so that a tile's epilogue runs under the
 // next one's products. A tile of the first product is 128 columns of gate beside the same 128 of up:
 // one CTA of the pair loads gate's rows, the other up's, and a thread finds both in its row. Operands whose
 // K runs along memory rows or across them (weights and gradients as they lie) are both read as they
 // are, by the major-ness of the matrix descriptors; nothing is transposed in memory.
 //
-// Bound by the tensor cores where K is long; the backward's first product moves 6 bytes out and 2 to 4
-// in for each of its T x d_ff outputs and is bound by memory where d_out is below about 1000.
+// Bound by what an SM can take from L2, 64 bytes a cycle: a stage of 32 KB feeds 512 cycles of products, so
+// at the tensor cores' full rate the operands alone fill that path (85 to 90 % of the rate is reached),
+// and what an epilogue writes and reads (up to 6 and 4 bytes for each of T x d_ff values) comes on top.
 #include <cuda.h>
 
 #include "ffn.cuh"
@@ -25,11 +27,10 @@ namespace dsalt {
 namespace ffn {
 namespace {
 
-constexpr int PAIR_M = 256, CTA_M = 128, PAIR_N = 256, KB = 64, STAGES = 5;
+constexpr int PAIR_M = 256, CTA_M = 128, PAIR_N = 256, KB = 64;
 constexpr int OPERAND_BYTES = CTA_M * KB * 2, STAGE_BYTES = 2 * OPERAND_BYTES;
+constexpr int BOX = 32, BOX_BYTES = 32 * BOX * 2;  // a warp's staged outputs: 32 rows of 32 columns
 constexpr int EPI_WARPS = 8, THREADS = 32 * (4 + EPI_WARPS);
-constexpr int BOX = 32, BOX_BYTES = BOX * BOX * 2, BOXES = 3;  // a warp's staged outputs
-constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + EPI_WARPS * BOXES * BOX_BYTES + 256;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr int GROUP_M = 8;  // tiles of 256 rows whose A stays in L2 while N is walked
 
@@ -44,6 +45,7 @@ struct alignas(64) Job {
 struct Kept {
   void* p;           // gate's and up's [2, T, pitch]
   uint8_t* exps;
+  void* h;           // [T, pitch]
   int64_t T, pitch;
 };
 template <int NJ>
@@ -108,6 +110,20 @@ __device__ __forceinline__ void pair_commit(uint64_t* bar) {
 }
 
 // ---------------------------------------------------------------- shared memory
+// The outputs that an epilogue stages for the store engine, in how many sets of boxes, and what that
+// leaves for the operands. The first product's epilogue writes its rows from registers instead: at three
+// outputs of 128 columns that measured 177 us against 183 (32768 x 768 -> 2048), but the backward's, which
+// also reads rows, 192 us against 173.
+template <int EPI, int KEEP>
+struct Shape {
+  static constexpr int OUTPUTS = EPI == GATE_UP ? 0 : EPI == PLAIN ? 1 : KEEP == DSALT_KEEP_8BIT ? 3 : 2;
+  static constexpr int SETS = OUTPUTS == 1 ? 4 : 2, STAGES = OUTPUTS == 0 ? 6 : OUTPUTS == 3 ? 4 : 5;
+  static constexpr int SET_BYTES = OUTPUTS * BOX_BYTES, WARP_BYTES = SETS * SET_BYTES;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + EPI_WARPS * WARP_BYTES + 256;
+  // columns of the accumulator that a warp works on (of the first product: as many of gate and of up)
+  static constexpr int COLS = (EPI == GATE_UP ? PAIR_N / 2 : PAIR_N) / (EPI_WARPS / 4);
+};
+template <int STAGES>
 struct Bars {
   uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
   uint32_t tmem;
@@ -133,88 +149,122 @@ __device__ __forceinline__ Tile find_tile(const Args<NJ>& a, int t) {
   return {j, first + r % rows, r / rows};
 }
 
-// 32 values of a row as fp32 into the warp's box (64 bytes a row, 16-byte pieces swizzled as the
-// store's map has it: piece ^ row / 2)
-template <typename T>
-__device__ __forceinline__ void stage_row(uint32_t box, int lane, const float (&f)[BOX]) {
+// N values of a row as fp32 from column `first` of the warp's box (64 bytes a row, 16-byte pieces
+// swizzled as the store's map has it: piece ^ row / 2)
+template <typename T, int N>
+__device__ __forceinline__ void stage_row(uint32_t box, int lane, const float (&f)[N], int first) {
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const uint32_t at = box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4);
+  for (int c = 0; c < N / 8; ++c) {
+    const uint32_t at = box + lane * 64 + (((c + first / 8) ^ ((lane >> 1) & 3)) << 4);
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(narrow2<T>(f[8 * c], f[8 * c + 1])),
                  "r"(narrow2<T>(f[8 * c + 2], f[8 * c + 3])), "r"(narrow2<T>(f[8 * c + 4], f[8 * c + 5])),
                  "r"(narrow2<T>(f[8 * c + 6], f[8 * c + 7]))
                  : "memory");
   }
 }
-__device__ __forceinline__ void load_acc(uint32_t taddr, float (&f)[BOX]) {
-  uint32_t r[32];
-  DSALT_TMEM_LD32(taddr, r);
-  tmem_wait_ld();
+// N columns of the accumulator, in flight until take_acc
+template <int N>
+__device__ __forceinline__ void ask_acc(uint32_t taddr, uint32_t (&r)[N]) {
+  if constexpr (N == 32) {
+    DSALT_TMEM_LD32(taddr, r);
+  } else {
+    DSALT_TMEM_LD16(taddr, r);
+  }
+}
+// waits for what was asked; the registers pass through the wait, so that nothing reads them before it
+template <int N>
+__device__ __forceinline__ void take_acc(uint32_t (&r)[N], float (&f)[N]) {
+  if constexpr (N == 32) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                   "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                   "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+  } else {
+    static_assert(N == 16, "16 or 32 columns");
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+  }
 #pragma unroll
-  for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
+  for (int i = 0; i < N; ++i) f[i] = __uint_as_float(r[i]);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_row(T* p, const float (&f)[N]) {
+#pragma unroll
+  for (int c = 0; c < N / 16; ++c)
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(__cvta_generic_to_global(p + 16 * c)),
+                 "r"(narrow2<T>(f[16 * c], f[16 * c + 1])), "r"(narrow2<T>(f[16 * c + 2], f[16 * c + 3])),
+                 "r"(narrow2<T>(f[16 * c + 4], f[16 * c + 5])), "r"(narrow2<T>(f[16 * c + 6], f[16 * c + 7])),
+                 "r"(narrow2<T>(f[16 * c + 8], f[16 * c + 9])), "r"(narrow2<T>(f[16 * c + 10], f[16 * c + 11])),
+                 "r"(narrow2<T>(f[16 * c + 12], f[16 * c + 13])), "r"(narrow2<T>(f[16 * c + 14], f[16 * c + 15]))
+                 : "memory");
 }
 __device__ __forceinline__ void load_32b(uint32_t (&u)[8], const void* p) {
   asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
                : "l"(__cvta_generic_to_global(p)));
 }
-// one value per row and group of 32 columns: the scale byte, and the codes into `at`
-__device__ __forceinline__ uint32_t store_codes(const float (&f)[BOX], int8_t* at) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < BOX; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-  const uint32_t s = scale_byte(top);
-  uint32_t w[8];
-  pack_codes<BOX>(f, s, w);
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(__cvta_generic_to_global(at)), "r"(w[0]), "r"(w[1]),
+__device__ __forceinline__ void store_32b(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(__cvta_generic_to_global(p)), "r"(w[0]), "r"(w[1]),
                "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
+}
+// a group of 32 columns of a row: its scale byte and its codes
+__device__ __forceinline__ uint32_t form_codes(const float (&f)[GROUP8], uint32_t (&w)[8]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < GROUP8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+  const uint32_t s = scale_byte(top);
+  pack_codes<GROUP8>(f, s, w);
   return s;
 }
 
-// what the backward's first epilogue reads for 32 columns of a row
+// what the backward's first epilogue reads: 32 columns of a row of gate and up
 template <typename T, int KEEP>
 struct KeptRow {
-  uint32_t g[KEEP == DSALT_KEEP_8BIT ? 8 : 16], u[KEEP == DSALT_KEEP_8BIT ? 8 : 16];
+  static constexpr int WORDS = KEEP == DSALT_KEEP_8BIT ? 8 : 16;
+  uint32_t g[WORDS], u[WORDS];
   uint32_t sg, su;
   __device__ __forceinline__ void load(const Kept& k, int64_t row, int64_t col) {
     const int64_t plane = k.T * k.pitch, at = row * k.pitch + col;
-    const bool in = row < k.T && col < k.pitch;
-    if constexpr (KEEP == DSALT_KEEP_8BIT) {
-      sg = su = 127;
+    constexpr int ES = KEEP == DSALT_KEEP_8BIT ? 1 : (int)sizeof(T);
+    sg = su = 127;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[i] = u[i] = 0;
-      if (in) {
-        load_32b(g, static_cast<const int8_t*>(k.p) + at);
-        load_32b(u, static_cast<const int8_t*>(k.p) + plane + at);
-        sg = k.exps[at / GROUP8];
-        su = k.exps[(plane + at) / GROUP8];
+    for (int i = 0; i < WORDS; ++i) g[i] = u[i] = 0;
+    if (row < k.T && col < k.pitch) {
+      const char* p = static_cast<const char*>(k.p) + at * ES;
+#pragma unroll
+      for (int i = 0; i < WORDS / 8; ++i) {
+        uint32_t a[8], b[8];
+        load_32b(a, p + 32 * i);
+        load_32b(b, p + plane * ES + 32 * i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[8 * i + j] = a[j], u[8 * i + j] = b[j];
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) g[i] = u[i] = 0;
-      if (in) {
-        const T* p = static_cast<const T*>(k.p) + at;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t a[8], b[8];
-          load_32b(a, p + 16 * i);
-          load_32b(b, p + plane + 16 * i);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) g[8 * i + j] = a[j], u[8 * i + j] = b[j];
-        }
+      if constexpr (KEEP == DSALT_KEEP_8BIT) {
+        sg = __ldg(k.exps + at / GROUP8);
+        su = __ldg(k.exps + (plane + at) / GROUP8);
       }
     }
   }
-  __device__ __forceinline__ void values(float (&a)[BOX], float (&b)[BOX]) const {
+  // values 16 half .. 16 half + 15
+  __device__ __forceinline__ void values(int half, float (&a)[16], float (&b)[16]) const {
     if constexpr (KEEP == DSALT_KEEP_8BIT) {
-      unpack_codes<BOX>(g, scale_of(sg), a);
-      unpack_codes<BOX>(u, scale_of(su), b);
+      uint32_t x[4], y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = g[4 * half + i], y[i] = u[4 * half + i];
+      unpack_codes<16>(x, scale_of(sg), a);
+      unpack_codes<16>(y, scale_of(su), b);
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        widen2<T>(g[i], a[2 * i], a[2 * i + 1]);
-        widen2<T>(u[i], b[2 * i], b[2 * i + 1]);
+      for (int i = 0; i < 8; ++i) {
+        widen2<T>(g[8 * half + i], a[2 * i], a[2 * i + 1]);
+        widen2<T>(u[8 * half + i], b[2 * i], b[2 * i + 1]);
       }
     }
   }
@@ -224,10 +274,12 @@ struct KeptRow {
 template <int EPI, bool A_MN, bool B_MN, typename T, int ACT, int KEEP, int NJ>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     ffn_pair_kernel(const __grid_constant__ Args<NJ> args) {
+  using S = Shape<EPI, KEEP>;
+  constexpr int STAGES = S::STAGES;
   extern __shared__ uint8_t raw[];
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t staging = base + STAGES * STAGE_BYTES;
-  Bars& bars = *reinterpret_cast<Bars*>(raw + (staging + EPI_WARPS * BOXES * BOX_BYTES - smem_u32(raw)));
+  Bars<STAGES>& bars = *reinterpret_cast<Bars<STAGES>*>(raw + (staging + EPI_WARPS * S::WARP_BYTES - smem_u32(raw)));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = cluster_rank() & 1u;
   const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
@@ -332,104 +384,129 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
     __syncwarp();
   } else if (warp >= 4) {
-    const int quad = warp % 4, side = (warp - 4) / 4;  // 32 rows, a half of the columns
-    const uint32_t boxes = staging + (warp - 4) * BOXES * BOX_BYTES;
-    int it = 0, slot = 0;
+    const int quad = warp % 4, side = (warp - 4) / 4;  // 32 rows, a share of the columns
+    const uint32_t boxes = staging + (warp - 4) * S::WARP_BYTES;
+    int it = 0, set = 0;
     for (int t = pair; t < args.tiles; t += pairs, ++it) {
       const Tile tile = find_tile<NJ>(args, t);
       const Job& job = args.job[tile.job];
       const int acc = it & 1;
       const int row0 = tile.m * PAIR_M + (int)rank * CTA_M + quad * 32;
       const uint32_t ta = tmem + acc * PAIR_N + ((uint32_t)(quad * 32) << 16);
-      // the boxes are written once earlier stores have read them
-      auto free_boxes = [&]() {
-        if (lane == 0) store_wait_read<0>();
+      // the next set of boxes, once the stores that read it are done
+      auto next_boxes = [&]() {
+        set = set + 1 == S::SETS ? 0 : set + 1;
+        if (lane == 0) store_wait_read<S::SETS - 1>();
         __syncwarp();
+        return boxes + set * S::SET_BYTES;
       };
-      auto send = [&](int box, const CUtensorMap* map, int col) {
-        if (lane == 0 && row0 < job.rows && col < job.cols) store_2d(map, boxes + box * BOX_BYTES, col, row0);
+      auto send = [&](uint32_t to, int col) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (row0 < job.rows && col < job.cols)
+#pragma unroll
+            for (int i = 0; i < S::OUTPUTS; ++i) store_2d(&job.c[i], to + i * BOX_BYTES, col, row0);
+          store_commit();
+        }
       };
+      const uint32_t mine = ta + side * S::COLS;
       if constexpr (EPI == GRADS) {
-        const int col0 = tile.n * PAIR_N + side * (PAIR_N / 2);
+        const int col0 = tile.n * PAIR_N + side * S::COLS;
+        const int64_t row = row0 + lane;
         KeptRow<T, KEEP> kept;
-        kept.load(args.kept, row0 + lane, col0);
+        kept.load(args.kept, row, col0);
         if (!mbar_wait(&bars.acc_full[acc], (it >> 1) & 1, args.err, 64)) break;
         tc_fence_after();
+        uint32_t r[32];
+        ask_acc<32>(mine, r);
 #pragma unroll 1
-        for (int c = 0; c < PAIR_N / 2; c += BOX) {
-          float a[BOX], b[BOX], d[BOX];
-          kept.values(a, b);
-          if (c + BOX < PAIR_N / 2) kept.load(args.kept, row0 + lane, col0 + c + BOX);
-          load_acc(ta + side * (PAIR_N / 2) + c, d);
-#pragma unroll
-          for (int i = 0; i < BOX; ++i) {
-            float v, dv;
-            activate_grad<ACT>(a[i], v, dv);
-            a[i] = d[i] * b[i] * dv;
-            b[i] *= v;
-            d[i] *= v;
+        for (int c = 0; c < S::COLS; c += 32) {
+          float d[32];
+          take_acc<32>(r, d);
+          const KeptRow<T, KEEP> now = kept;
+          if (c + 32 < S::COLS) {
+            kept.load(args.kept, row, col0 + c + 32);
+            ask_acc<32>(mine + c + 32, r);
           }
-          free_boxes();
-          stage_row<T>(boxes, lane, b);
-          stage_row<T>(boxes + BOX_BYTES, lane, a);
-          stage_row<T>(boxes + 2 * BOX_BYTES, lane, d);
-          fence_proxy_async_smem();
-          __syncwarp();
-          send(0, &job.c[0], col0 + c);
-          send(1, &job.c[1], col0 + c);
-          send(2, &job.c[2], col0 + c);
-          if (lane == 0) store_commit();
+          uint32_t to = 0;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float a[16], b[16], e[16];
+            now.values(half, a, b);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float v, dv;
+              activate_grad<ACT>(a[i], v, dv);
+              a[i] = d[16 * half + i] * b[i] * dv;
+              b[i] *= v;
+              e[i] = d[16 * half + i] * v;
+            }
+            if (half == 0) to = next_boxes();
+            stage_row<T, 16>(to, lane, a, 16 * half);
+            stage_row<T, 16>(to + BOX_BYTES, lane, e, 16 * half);
+            if constexpr (KEEP == DSALT_KEEP_8BIT) stage_row<T, 16>(to + 2 * BOX_BYTES, lane, b, 16 * half);
+          }
+          send(to, col0 + c);
         }
       } else if constexpr (EPI == GATE_UP) {
+        static_assert(S::COLS == 64, "a warp takes two groups of 32 columns");
         if (!mbar_wait(&bars.acc_full[acc], (it >> 1) & 1, args.err, 64)) break;
         tc_fence_after();
-#pragma unroll 1
-        for (int c = side * 64; c < side * 64 + 64; c += BOX) {
-          const int col = tile.n * (PAIR_N / 2) + c;
-          float g[BOX], u[BOX], h[BOX];
-          load_acc(ta + c, g);
-          load_acc(ta + PAIR_N / 2 + c, u);
+        const int col = tile.n * (PAIR_N / 2) + side * 64;
+        const int64_t row = row0 + lane, at = row * args.kept.pitch + col, plane = args.kept.T * args.kept.pitch;
+        uint32_t rg[32], ru[32], cg[2][8], cu[2][8], sg[2], su[2];
+        ask_acc<32>(mine, rg);
+        ask_acc<32>(mine + PAIR_N / 2, ru);
 #pragma unroll
-          for (int i = 0; i < BOX; ++i) h[i] = activate<ACT>(g[i]) * u[i];
-          if constexpr (KEEP == DSALT_KEEP_8BIT) {
-            const int64_t row = row0 + lane, at = row * args.kept.pitch + col, plane = args.kept.T * args.kept.pitch;
-            if (row < args.kept.T && col < args.kept.pitch) {
-              int8_t* codes = static_cast<int8_t*>(args.kept.p);
-              args.kept.exps[at / GROUP8] = (uint8_t)store_codes(g, codes + at);
-              args.kept.exps[(plane + at) / GROUP8] = (uint8_t)store_codes(u, codes + plane + at);
+        for (int half = 0; half < 2; ++half) {
+          float g[32], u[32];
+          take_acc<32>(rg, g);
+          take_acc<32>(ru, u);
+          if (half == 0) {
+            ask_acc<32>(mine + 32, rg);
+            ask_acc<32>(mine + PAIR_N / 2 + 32, ru);
+          }
+          const bool in = row < args.kept.T && col + 32 * half < args.kept.pitch;
+          if constexpr (KEEP == DSALT_KEEP_INPUT) {
+            if (in) {
+              store_row<T, 32>(static_cast<T*>(args.kept.p) + at + 32 * half, g);
+              store_row<T, 32>(static_cast<T*>(args.kept.p) + plane + at + 32 * half, u);
             }
           }
-          free_boxes();
-          stage_row<T>(boxes, lane, h);
-          if constexpr (KEEP == DSALT_KEEP_INPUT) {
-            stage_row<T>(boxes + BOX_BYTES, lane, g);
-            stage_row<T>(boxes + 2 * BOX_BYTES, lane, u);
+          if constexpr (KEEP == DSALT_KEEP_8BIT) {
+            sg[half] = form_codes(g, cg[half]);
+            su[half] = form_codes(u, cu[half]);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          send(0, &job.c[0], col);
-          if constexpr (KEEP == DSALT_KEEP_INPUT) {
-            send(1, &job.c[1], col);
-            send(2, &job.c[2], col);
-          }
-          if (lane == 0) store_commit();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) g[i] = activate<ACT>(g[i]) * u[i];
+          if (in) store_row<T, 32>(static_cast<T*>(args.kept.h) + at + 32 * half, g);
+        }
+        if constexpr (KEEP == DSALT_KEEP_8BIT) {
+          int8_t* codes = static_cast<int8_t*>(args.kept.p);
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            if (row < args.kept.T && col + 32 * half < args.kept.pitch) {
+              store_32b(codes + at + half * 32, cg[half]);
+              store_32b(codes + plane + at + half * 32, cu[half]);
+              args.kept.exps[at / GROUP8 + half] = (uint8_t)sg[half];
+              args.kept.exps[(plane + at) / GROUP8 + half] = (uint8_t)su[half];
+            }
         }
       } else {
         if (!mbar_wait(&bars.acc_full[acc], (it >> 1) & 1, args.err, 64)) break;
         tc_fence_after();
-        const int col0 = tile.n * PAIR_N + side * (PAIR_N / 2);
+        const int col0 = tile.n * PAIR_N + side * S::COLS;
+        uint32_t r[BOX];
+        ask_acc<BOX>(mine, r);
 #pragma unroll 1
-        for (int c = 0; c < PAIR_N / 2; c += BOX) {
+        for (int c = 0; c < S::COLS; c += BOX) {
           float d[BOX];
-          load_acc(ta + side * (PAIR_N / 2) + c, d);
-          if (lane == 0) store_wait_read<BOXES - 1>();
-          __syncwarp();
-          stage_row<T>(boxes + slot * BOX_BYTES, lane, d);
-          fence_proxy_async_smem();
-          __syncwarp();
-          send(slot, &job.c[0], col0 + c);
-          if (lane == 0) store_commit();
-          slot = slot + 1 == BOXES ? 0 : slot + 1;
+          take_acc<BOX>(r, d);
+          if (c + BOX < S::COLS) ask_acc<BOX>(mine + c + BOX, r);
+          const uint32_t to = next_boxes();
+          stage_row<T, BOX>(to, lane, d, 0);
+          send(to, col0 + c);
         }
       }
       tc_fence_before();
@@ -462,9 +539,10 @@ EncodeTiledFn get_encode() {
   return fn;
 }
 
-// rows x cols values of 16 bits, `stride` values from row to row, in boxes of box_rows x box_cols
+// rows x cols values of 16 bits, `stride` values from row to row, in boxes of box_rows x box_cols (as wide as the swizzle:
+// 64 or 32 columns)
 int make_map(CUtensorMap* m, const void* p, int dtype, int64_t rows, int64_t cols, int64_t stride, int box_rows,
-             int box_cols, bool store) {
+             int box_cols) {
   const EncodeTiledFn enc = get_encode();
   if (!enc) return fail(DSALT_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
@@ -473,17 +551,17 @@ int make_map(CUtensorMap* m, const void* p, int dtype, int64_t rows, int64_t col
   const cuuint32_t step[2] = {1, 1};
   const CUresult r = enc(m, dtype == DSALT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
                          const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         store ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(DSALT_ERR_CUDA, "gated_ffn: cuTensorMapEncodeTiled failed (%d)", (int)r);
   return DSALT_OK;
 }
 // an operand: K along its rows (128 rows of 64 values of K), or across them (64 rows of K, 64 columns)
 int operand(CUtensorMap* m, const void* p, const Ffn& f, int64_t rows, int64_t cols, int64_t stride, bool across) {
-  return make_map(m, p, f.dtype, rows, cols, stride, across ? KB : CTA_M, 64, false);
+  return make_map(m, p, f.dtype, rows, cols, stride, across ? KB : CTA_M, 64);
 }
 int output(CUtensorMap* m, void* p, const Ffn& f, int64_t rows, int64_t cols, int64_t stride) {
-  return make_map(m, p, f.dtype, rows, cols, stride, BOX, BOX, true);
+  return make_map(m, p, f.dtype, rows, cols, stride, 32, BOX);
 }
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 void size_job(Job& j, int64_t M, int64_t N, int64_t K, int tile_n) {
@@ -497,14 +575,16 @@ void size_job(Job& j, int64_t M, int64_t N, int64_t K, int tile_n) {
 template <int EPI, bool A_MN, bool B_MN, typename T, int ACT, int KEEP, int NJ>
 int launch_pair(Args<NJ>& a, const Ffn& f, const char* what) {
   static std::atomic<uint64_t> ready{0};
+  constexpr int bytes = Shape<EPI, KEEP>::SMEM_BYTES;
+  static_assert(bytes <= 232448, "shared memory of a block");
   auto kernel = ffn_pair_kernel<EPI, A_MN, B_MN, T, ACT, KEEP, NJ>;
-  if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), SMEM_BYTES, ready)) return rc;
+  if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), bytes, ready)) return rc;
   a.tiles = 0;
   for (int i = 0; i < NJ; ++i) a.tiles += a.job[i].tiles_m * a.job[i].tiles_n;
   a.idesc = umma_idesc_f16(f.dtype == DSALT_BF16 ? 1 : 0, A_MN, B_MN, PAIR_M, PAIR_N);
   a.err = device_status_ptr();
   const int pairs = a.tiles < 74 ? a.tiles : 74;
-  kernel<<<2 * pairs, THREADS, SMEM_BYTES, f.stream>>>(a);
+  kernel<<<2 * pairs, THREADS, bytes, f.stream>>>(a);
   return check_cuda(cudaGetLastError(), what);
 }
 
@@ -515,14 +595,9 @@ int gate_up(const Ffn& f) {
   size_job(j, f.T, f.F, f.d, PAIR_N / 2);
   int rc;
   if ((rc = operand(&j.a[0], f.x, f, f.T, f.d, f.x_stride, false)) || (rc = operand(&j.b[0], f.w_gate, f, f.F, f.d, f.d, false)) ||
-      (rc = operand(&j.b[1], f.w_up, f, f.F, f.d, f.d, false)) || (rc = output(&j.c[0], f.h, f, f.T, f.F, f.pitch)))
+      (rc = operand(&j.b[1], f.w_up, f, f.F, f.d, f.d, false)))
     return rc;
-  if (KEEP == DSALT_KEEP_INPUT) {
-    T* kept = static_cast<T*>(f.kept);
-    if ((rc = output(&j.c[1], kept, f, f.T, f.F, f.pitch)) || (rc = output(&j.c[2], kept + f.T * f.pitch, f, f.T, f.F, f.pitch)))
-      return rc;
-  }
-  a.kept = {f.kept, f.exps, f.T, f.pitch};
+  a.kept = {f.kept, f.exps, f.h, f.T, f.pitch};
   return launch_pair<GATE_UP, false, false, T, ACT, KEEP, 1>(a, f, "gated_ffn gate and up launch");
 }
 
@@ -548,10 +623,10 @@ int grads(const Ffn& f) {
   size_job(j, f.T, f.F, f.d_out, PAIR_N);
   int rc;
   if ((rc = operand(&j.a[0], f.dy, f, f.T, f.d_out, f.dy_stride, false)) ||
-      (rc = operand(&j.b[0], f.w_down, f, f.d_out, f.F, f.F, true)) || (rc = output(&j.c[0], f.h, f, f.T, f.F, f.pitch)) ||
-      (rc = output(&j.c[1], f.dg, f, f.T, f.F, f.pitch)) || (rc = output(&j.c[2], f.du, f, f.T, f.F, f.pitch)))
+      (rc = operand(&j.b[0], f.w_down, f, f.d_out, f.F, f.F, true)) || (rc = output(&j.c[0], f.dg, f, f.T, f.F, f.pitch)) ||
+      (rc = output(&j.c[1], f.du, f, f.T, f.F, f.pitch)) || (KEEP == DSALT_KEEP_8BIT && (rc = output(&j.c[2], f.h, f, f.T, f.F, f.pitch))))
     return rc;
-  a.kept = {f.kept, f.exps, f.T, f.pitch};
+  a.kept = {f.kept, f.exps, f.h, f.T, f.pitch};
   return launch_pair<GRADS, false, true, T, ACT, KEEP, 1>(a, f, "gated_ffn_bwd hidden gradients launch");
 }
 

@@ -251,8 +251,9 @@ def _ffn_forward(x2, stride, w_gate, w_up, w_down, sizes, act, keep):
     kept = exps = None
     if keep:
         pitch = _ffn_pitch(F)
-        kept = torch.empty(2, T, pitch, dtype=torch.int8 if keep == L.KEEP_8BIT else x2.dtype, device=dev)
-        if keep == L.KEEP_8BIT:
+        coded = keep == L.KEEP_8BIT
+        kept = torch.empty(2 if coded else 3, T, pitch, dtype=torch.int8 if coded else x2.dtype, device=dev)
+        if coded:
             exps = torch.empty(2, T, pitch // GROUP, dtype=torch.uint8, device=dev)
     ws = _workspace(_ffn_workspace(_dt(x2), T, d, F, d_out, 0), dev)
     _run(dev, "dsalt_gated_ffn", x2.data_ptr(), _dt(x2), T, d, stride, w_gate.data_ptr(), w_up.data_ptr(),
@@ -262,8 +263,8 @@ def _ffn_forward(x2, stride, w_gate, w_up, w_down, sizes, act, keep):
 
 class GatedFFNFunction(torch.autograd.Function):
     """Autograd of :func:`gated_ffn`. Kept for the backward pass: ``x Wgᵀ`` and ``x Wuᵀ`` (written by
-    the epilogue that forms them) and ``x``, in the input's dtype or in 8 bits; the product of gate and up
-    is formed again."""
+    the epilogue that forms them) and ``x``, in the input's dtype or in 8 bits. In the input's dtype the rows
+    that the last product read are kept too; in 8 bits they are formed again."""
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, activation, keep):
