@@ -19,7 +19,8 @@ CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(OUT_DIR, "libdsalt_b200.so")
 SOURCES = ["capi.cu", "signals.cu", "select.cu", "attn_simt.cu", "attn_tc.cu", "attn_bwd.cu", "attn_train.cu", "peer.cu",
-           "slots.cu", "cache_append.cu", "cache_attn.cu", "sample.cu", "pack8.cu", "rope.cu", "ffn.cu", "ffn_tc.cu"]
+           "slots.cu", "cache_append.cu", "cache_attn.cu", "sample.cu", "pack8.cu", "rope.cu", "ffn.cu", "ffn_tc.cu",
+           "ffn_few.cu", "ffn_token.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -19,9 +19,7 @@
 // Bound by what an SM can take from L2, 64 bytes a cycle: a stage of 32 KB feeds 512 cycles of products, so
 // at the tensor cores' full rate the operands alone fill that path (85 to 90 % of the rate is reached),
 // and what an epilogue writes and reads (up to 6 and 4 bytes for each of T x d_ff values) comes on top.
-#include <cuda.h>
-
-#include "ffn.cuh"
+#include "ffn_tc.cuh"
 
 namespace dsalt {
 namespace ffn {
@@ -34,6 +32,12 @@ constexpr int EPI_WARPS = 8, THREADS = 32 * (4 + EPI_WARPS);
 constexpr uint32_t TMEM_COLS = 512;
 constexpr int GROUP_M = 8;  // tiles of 256 rows whose A stays in L2 while N is walked
 
+#ifndef FEW_TOKENS
+#define FEW_TOKENS 256
+#endif
+#ifndef TOKENS
+#define TOKENS 8
+#endif
 enum Epilogue { PLAIN = 0, GATE_UP = 1, GRADS = 2 };
 
 struct alignas(64) Job {
@@ -58,19 +62,6 @@ struct Args {
 };
 
 // ---------------------------------------------------------------- pair-wide forms
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t in_cta(uint32_t smem_addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 __device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -161,37 +152,6 @@ __device__ __forceinline__ void stage_row(uint32_t box, int lane, const float (&
                  "r"(narrow2<T>(f[8 * c + 6], f[8 * c + 7]))
                  : "memory");
   }
-}
-// N columns of the accumulator, in flight until take_acc
-template <int N>
-__device__ __forceinline__ void ask_acc(uint32_t taddr, uint32_t (&r)[N]) {
-  if constexpr (N == 32) {
-    DSALT_TMEM_LD32(taddr, r);
-  } else {
-    DSALT_TMEM_LD16(taddr, r);
-  }
-}
-// waits for what was asked; the registers pass through the wait, so that nothing reads them before it
-template <int N>
-__device__ __forceinline__ void take_acc(uint32_t (&r)[N], float (&f)[N]) {
-  if constexpr (N == 32) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
-                   "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
-                   "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-                 :
-                 : "memory");
-  } else {
-    static_assert(N == 16, "16 or 32 columns");
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-                 :
-                 : "memory");
-  }
-#pragma unroll
-  for (int i = 0; i < N; ++i) f[i] = __uint_as_float(r[i]);
 }
 template <typename T, int N>
 __device__ __forceinline__ void store_row(T* p, const float (&f)[N]) {
@@ -524,38 +484,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 }
 
 // ---------------------------------------------------------------- host side
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn get_encode() {
-  static const EncodeTiledFn fn = [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-                    q == cudaDriverEntryPointSuccess;
-    return ok ? reinterpret_cast<EncodeTiledFn>(ptr) : nullptr;
-  }();
-  return fn;
-}
-
-// rows x cols values of 16 bits, `stride` values from row to row, in boxes of box_rows x box_cols (as wide as the swizzle:
-// 64 or 32 columns)
-int make_map(CUtensorMap* m, const void* p, int dtype, int64_t rows, int64_t cols, int64_t stride, int box_rows,
-             int box_cols) {
-  const EncodeTiledFn enc = get_encode();
-  if (!enc) return fail(DSALT_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
-  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
-  const cuuint32_t step[2] = {1, 1};
-  const CUresult r = enc(m, dtype == DSALT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-                         const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(DSALT_ERR_CUDA, "gated_ffn: cuTensorMapEncodeTiled failed (%d)", (int)r);
-  return DSALT_OK;
-}
 // an operand: K along its rows (128 rows of 64 values of K), or across them (64 rows of K, 64 columns)
 int operand(CUtensorMap* m, const void* p, const Ffn& f, int64_t rows, int64_t cols, int64_t stride, bool across) {
   return make_map(m, p, f.dtype, rows, cols, stride, across ? KB : CTA_M, 64);
@@ -563,7 +491,6 @@ int operand(CUtensorMap* m, const void* p, const Ffn& f, int64_t rows, int64_t c
 int output(CUtensorMap* m, void* p, const Ffn& f, int64_t rows, int64_t cols, int64_t stride) {
   return make_map(m, p, f.dtype, rows, cols, stride, 32, BOX);
 }
-int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 void size_job(Job& j, int64_t M, int64_t N, int64_t K, int tile_n) {
   j.tiles_m = ceil_div(M, PAIR_M);
   j.tiles_n = ceil_div(N, tile_n);
@@ -687,6 +614,8 @@ int run_tensor_cores(const Ffn& f, bool back) {
   int dev = 0;
   int rc;
   if ((rc = check_cuda(cudaGetDevice(&dev), "current device")) || (rc = check_cuda(cudaSetDevice(dev), "current device"))) return rc;
+  if (!back && f.keep == DSALT_KEEP_NONE && f.T <= TOKENS) return forward_tokens(f);
+  if (!back && f.keep == DSALT_KEEP_NONE && f.T <= FEW_TOKENS) return forward_few(f);
   return f.dtype == DSALT_BF16 ? run_typed<__nv_bfloat16>(f, back) : run_typed<__half>(f, back);
 }
 
