@@ -21,12 +21,6 @@ namespace {
 
 constexpr int THREADS = 256;
 
-template <typename T>
-struct Vec32 {  // 32 bytes of T
-  static constexpr int N = 32 / sizeof(T);
-  uint32_t u[8];
-};
-
 __device__ __forceinline__ void ld32(uint32_t (&u)[8], const void* p) {
   asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
@@ -50,18 +44,19 @@ __device__ __forceinline__ void widen(const uint32_t (&u)[8], float (&f)[32 / si
 }
 
 // rows of n values in chunks of 32 bytes, a chunk per thread; a row's chunk count is rounded up
-// to whole groups, so that the lanes of a group are neighbours in a warp
-template <typename T>
+// to whole groups, so that the lanes of a group are neighbours in a warp. I: 32 bits where they count the
+// chunks, whose division is a few instructions
+template <typename T, typename I>
 __global__ void __launch_bounds__(THREADS) pack_rows_kernel(const T* __restrict__ x, int64_t rows, int n,
                                                             int64_t x_stride, int8_t* __restrict__ codes,
                                                             uint8_t* __restrict__ exps, int groups) {
   constexpr int N = 32 / (int)sizeof(T), LANES = GROUP8 / N;
-  const int64_t chunks = (int64_t)groups * LANES, total = rows * chunks;
-  for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i - threadIdx.x % 32 < total;
-       i += (int64_t)gridDim.x * THREADS) {
+  const I chunks = (I)groups * LANES, total = (I)rows * chunks;
+  for (I i = (I)blockIdx.x * THREADS + threadIdx.x; i - threadIdx.x % 32 < total; i += (I)gridDim.x * THREADS) {
     const bool in = i < total;
-    const int64_t row = in ? i / chunks : 0;
-    const int chunk = in ? (int)(i - row * chunks) : 0, col = chunk * N;
+    const I at_row = in ? i / chunks : 0;
+    const int64_t row = at_row;
+    const int chunk = in ? (int)(i - at_row * chunks) : 0, col = chunk * N;
     const bool held = in && col < n;
     uint32_t u[8] = {};
     if (held) ld32(u, x + row * x_stride + col);
@@ -102,15 +97,16 @@ __global__ void __launch_bounds__(THREADS) pack_any_kernel(const T* __restrict__
   }
 }
 
-template <typename T>
+template <typename T, typename I>
 __global__ void __launch_bounds__(THREADS) unpack_rows_kernel(const int8_t* __restrict__ codes,
                                                               const uint8_t* __restrict__ exps, int64_t rows, int n,
                                                               int groups, T* __restrict__ out) {
   constexpr int N = 32 / (int)sizeof(T);
-  const int64_t chunks = n / N, total = rows * chunks;
-  for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < total; i += (int64_t)gridDim.x * THREADS) {
-    const int64_t row = i / chunks;
-    const int col = (int)(i - row * chunks) * N;
+  const I chunks = n / N, total = (I)rows * chunks;
+  for (I i = (I)blockIdx.x * THREADS + threadIdx.x; i < total; i += (I)gridDim.x * THREADS) {
+    const I at_row = i / chunks;
+    const int64_t row = at_row;
+    const int col = (int)(i - at_row * chunks) * N;
     const float scale = scale_of(exps[row * groups + col / GROUP8]);
     uint32_t w[N / 4];
     if constexpr (N == 16) {
@@ -155,10 +151,13 @@ template <typename T>
 int pack(const T* x, int64_t rows, int n, int64_t x_stride, int8_t* codes, uint8_t* exps, cudaStream_t stream) {
   constexpr int N = 32 / (int)sizeof(T);
   const int groups = (n + GROUP8 - 1) / GROUP8;
-  if (n % N == 0 && x_stride % N == 0 && aligned(x, 32) && aligned(codes, 16))
-    pack_rows_kernel<T><<<blocks_for(rows * groups * (GROUP8 / N)), THREADS, 0, stream>>>(x, rows, n, x_stride, codes,
-                                                                                          exps, groups);
-  else
+  if (n % N == 0 && x_stride % N == 0 && aligned(x, 32) && aligned(codes, 16)) {
+    const int64_t chunks = rows * groups * (GROUP8 / N);
+    if (chunks < 1ll << 31)
+      pack_rows_kernel<T, uint32_t><<<blocks_for(chunks), THREADS, 0, stream>>>(x, rows, n, x_stride, codes, exps, groups);
+    else
+      pack_rows_kernel<T, int64_t><<<blocks_for(chunks), THREADS, 0, stream>>>(x, rows, n, x_stride, codes, exps, groups);
+  } else
     pack_any_kernel<T><<<blocks_for(rows * groups * 32), THREADS, 0, stream>>>(x, rows, n, x_stride, codes, exps, groups);
   return check_cuda(cudaGetLastError(), "pack8 launch");
 }
@@ -167,9 +166,13 @@ template <typename T>
 int unpack(const int8_t* codes, const uint8_t* exps, int64_t rows, int n, T* out, cudaStream_t stream) {
   constexpr int N = 32 / (int)sizeof(T);
   const int groups = (n + GROUP8 - 1) / GROUP8;
-  if (n % N == 0 && aligned(out, 32) && aligned(codes, 16))
-    unpack_rows_kernel<T><<<blocks_for(rows * (n / N)), THREADS, 0, stream>>>(codes, exps, rows, n, groups, out);
-  else
+  if (n % N == 0 && aligned(out, 32) && aligned(codes, 16)) {
+    const int64_t chunks = rows * (n / N);
+    if (chunks < 1ll << 31)
+      unpack_rows_kernel<T, uint32_t><<<blocks_for(chunks), THREADS, 0, stream>>>(codes, exps, rows, n, groups, out);
+    else
+      unpack_rows_kernel<T, int64_t><<<blocks_for(chunks), THREADS, 0, stream>>>(codes, exps, rows, n, groups, out);
+  } else
     unpack_any_kernel<T><<<blocks_for(rows * n), THREADS, 0, stream>>>(codes, exps, rows, n, groups, out);
   return check_cuda(cudaGetLastError(), "unpack8 launch");
 }

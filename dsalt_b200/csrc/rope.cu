@@ -12,7 +12,7 @@
 //
 // Bound by memory: an element is read once (backward: x and its gradient) and written once. A lane
 // holds 16 bytes of each half of a head, so that the rotation needs no exchange and the norm a sum over
-// G lanes (4 for 64 values of 16 bits); its angles, 4 bytes a value, are read once for HEADS
+// G lanes (4 for 64 values of 16 bits); its angles, 4 bytes a value, are read once for several
 // heads of the token, whose loads are all under way before the first is used. Queries and keys
 // are two sides of one launch: a block works on one of them, so that a thread's share of the
 // weights' gradient stays in registers until the block ends. The blocks' sums are joined by a second
@@ -22,8 +22,15 @@
 namespace dsalt {
 namespace {
 
-constexpr int THREADS = 256, HEADS = 4;
+constexpr int THREADS = 256;
 constexpr int MAX_HEAD_DIM = 256;
+
+// Heads whose loads are under way at once, and blocks an SM has room for. Measured at 131072 tokens, 16 + 16
+// heads of 64 in bf16 (forward / backward us; the bytes take 164 / 246): 4 and 2 heads, two blocks 186 / 291;
+// 2 and 2, three and two blocks 196 / 300; 4 and 4, two and one block 187 / 358; whatever makes registers spill
+// (three backward blocks and more) 400 to 500 backward.
+constexpr int FWD_HEADS = 4, BWD_HEADS = 2, PER_SM = 2;
+constexpr int FWD_BLOCKS = 148 * 8, BWD_BLOCKS = 148 * PER_SM;  // backward: one share of the weights' gradient a block
 
 struct Side {
   const void* x;
@@ -32,7 +39,7 @@ struct Side {
   const void* w;        // nullable
   int64_t x_token, x_head, d_token, d_head;
   int heads, chunks;    // chunks of HEADS heads in a token
-  int64_t items;        // tokens * chunks
+  uint32_t items;       // tokens * chunks
 };
 struct Args {
   Side side[2];
@@ -86,8 +93,8 @@ __device__ __forceinline__ float group_sum(float v) {
 
 // G lanes to a head, of which those below D / (2 V) hold values; a warp takes 32 / G chunks at a time
 template <typename T, int G, bool BWD>
-__global__ void __launch_bounds__(THREADS) qk_norm_rope_kernel(const __grid_constant__ Args a) {
-  constexpr int V = 16 / (int)sizeof(T), SLOTS = THREADS / G;
+__global__ void __launch_bounds__(THREADS, PER_SM) qk_norm_rope_kernel(const __grid_constant__ Args a) {
+  constexpr int V = 16 / (int)sizeof(T), SLOTS = THREADS / G, HEADS = BWD ? BWD_HEADS : FWD_HEADS;
   const int which = (int)blockIdx.x >= a.q_blocks;
   const Side& s = a.side[which];
   const int block = which ? blockIdx.x - a.q_blocks : blockIdx.x, blocks = which ? gridDim.x - a.q_blocks : a.q_blocks;
@@ -102,12 +109,12 @@ __global__ void __launch_bounds__(THREADS) qk_norm_rope_kernel(const __grid_cons
     ga[i] = gb[i] = 0.f;
   }
   const float inv_d = 1.f / (float)a.D;
-  const int64_t first = (int64_t)block * SLOTS + threadIdx.x / G;
+  const uint32_t first = block * SLOTS + threadIdx.x / G;
   // the lanes of a warp leave the loop together: the sums over a head need them all
-  for (int64_t item = first; item - (threadIdx.x % 32) / G < s.items; item += (int64_t)blocks * SLOTS) {
+  for (uint32_t item = first; item - (threadIdx.x % 32) / G < s.items; item += blocks * SLOTS) {
     const bool in = item < s.items;
-    const int64_t t = in ? item / s.chunks : 0;
-    const int h0 = in ? (int)(item - t * s.chunks) * HEADS : 0;
+    const int64_t t = in ? item / (uint32_t)s.chunks : 0;
+    const int h0 = in ? (int)(item - (uint32_t)t * s.chunks) * HEADS : 0;
     const int n = in && held ? min(HEADS, s.heads - h0) : 0;
     const T* x = static_cast<const T*>(s.x) + t * s.x_token + h0 * s.x_head + col;
     uint4 xr[HEADS][2] = {}, dr[HEADS][2] = {};
@@ -218,27 +225,32 @@ __global__ void __launch_bounds__(THREADS) qk_norm_rope_kernel(const __grid_cons
   }
 }
 
-// block (32 columns, side): 32 columns x 8 runs of partial sums
-__global__ void __launch_bounds__(256) weight_grad_kernel(const float* __restrict__ partial, int q_blocks, int blocks,
+// block (32 columns, side): 32 columns x 32 runs of partial sums
+__global__ void __launch_bounds__(1024) weight_grad_kernel(const float* __restrict__ partial, int q_blocks, int blocks,
                                                           int D, void* dwq, void* dwk, int dtype) {
-  __shared__ float sums[8][32];
-  const int col = blockIdx.x * 32 + threadIdx.x % 32, run = threadIdx.x / 32;
+  __shared__ float sums[32][33];
+  const int run = threadIdx.x / 32;
+  int col = blockIdx.x * 32 + threadIdx.x % 32;
   const int lo = blockIdx.y ? q_blocks : 0, hi = blockIdx.y ? blocks : q_blocks;
   void* out = blockIdx.y ? dwk : dwq;
   float v = 0.f;
-  if (col < D)
-    for (int b = lo + run; b < hi; b += 8) v += partial[(int64_t)b * D + col];
-  sums[run][threadIdx.x % 32] = v;
+  if (col < D) {
+#pragma unroll 8
+    for (int b = lo + run; b < hi; b += 32) v += partial[b * D + col];
+  }
+  sums[threadIdx.x % 32][run] = v;
   __syncthreads();
-  if (run == 0 && col < D) {
-    for (int i = 1; i < 8; ++i) v += sums[i][threadIdx.x];
+  // a warp per column
+  v = sums[run][threadIdx.x % 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  col = blockIdx.x * 32 + run;
+  if (threadIdx.x % 32 == 0 && col < D) {
     if (dtype == DSALT_F32) static_cast<float*>(out)[col] = v;
     else if (dtype == DSALT_BF16) static_cast<__nv_bfloat16*>(out)[col] = __float2bfloat16_rn(v);
     else static_cast<__half*>(out)[col] = __float2half_rn(v);
   }
 }
-
-constexpr int FWD_BLOCKS = 148 * 8, BWD_BLOCKS = 148 * 2;
 
 int elem_bytes(int dtype) { return dtype == DSALT_F32 ? 4 : 2; }
 int lanes_for(int D, int es) {
@@ -263,14 +275,15 @@ int launch_typed(const Args& a, int blocks, int G, int dtype, cudaStream_t strea
 }
 
 // blocks of both sides, as many as their items need (at most `most`), shared in proportion to their heads
-void share_blocks(Args& a, int64_t T, int G, int most, int& blocks) {
+int share_blocks(Args& a, const char* fn, int64_t T, int G, int heads, int most, int& blocks) {
   const int slots = THREADS / G;
   int64_t need[2];
   for (int i = 0; i < 2; ++i) {
     Side& s = a.side[i];
-    s.chunks = (s.heads + HEADS - 1) / HEADS;
-    s.items = T * s.chunks;
-    need[i] = (s.items + slots - 1) / slots;
+    s.chunks = (s.heads + heads - 1) / heads;
+    if (T * s.chunks > 1ll << 30) return fail(DSALT_ERR_UNSUPPORTED, "%s: more than 2^30 groups of %d heads", fn, heads);
+    s.items = (uint32_t)(T * s.chunks);
+    need[i] = ((int64_t)s.items + slots - 1) / slots;
   }
   if (need[0] + need[1] > most) {
     const int64_t q = most * need[0] / (need[0] + need[1]);
@@ -279,6 +292,7 @@ void share_blocks(Args& a, int64_t T, int G, int most, int& blocks) {
   }
   a.q_blocks = (int)need[0];
   blocks = (int)(need[0] + need[1]);
+  return DSALT_OK;
 }
 
 bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
@@ -338,7 +352,7 @@ int dsalt_qk_norm_rope(const void* q, const void* k, int dtype, int64_t T, int n
   a.eps = eps, a.w_dtype = w_dtype, a.D = head_dim, a.err = device_status_ptr();
   const int G = lanes_for(head_dim, elem_bytes(dtype));
   int blocks;
-  share_blocks(a, T, G, FWD_BLOCKS, blocks);
+  if ((rc = share_blocks(a, FN, T, G, FWD_HEADS, FWD_BLOCKS, blocks))) return rc;
   return launch_typed<false>(a, blocks, G, dtype, static_cast<cudaStream_t>(stream));
 }
 
@@ -385,9 +399,9 @@ int dsalt_qk_norm_rope_bwd(const void* q, const void* k, const void* dq_out, con
   a.partial = static_cast<float*>(workspace);
   const int G = lanes_for(head_dim, elem_bytes(dtype));
   int blocks;
-  share_blocks(a, T, G, BWD_BLOCKS, blocks);
+  if ((rc = share_blocks(a, FN, T, G, BWD_HEADS, BWD_BLOCKS, blocks))) return rc;
   if ((rc = launch_typed<true>(a, blocks, G, dtype, s)) || !norm) return rc;
-  weight_grad_kernel<<<dim3((head_dim + 31) / 32, 2), 256, 0, s>>>(a.partial, a.q_blocks, blocks, head_dim, dq_weight,
+  weight_grad_kernel<<<dim3((head_dim + 31) / 32, 2), 1024, 0, s>>>(a.partial, a.q_blocks, blocks, head_dim, dq_weight,
                                                                    dk_weight, w_dtype);
   return check_cuda(cudaGetLastError(), "qk_norm_rope_bwd weights launch");
 }

@@ -16,7 +16,6 @@ from __future__ import annotations
 import functools
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from .ops import _dt, _ptr, _workspace
@@ -27,19 +26,30 @@ ACTIVATIONS = {"silu": L.ACT_SILU, "gelu": L.ACT_GELU}
 KEEP = {"16bit": L.KEEP_INPUT, "8bit": L.KEEP_8BIT}
 
 
+def _no_second_derivative() -> None:
+    if torch.is_grad_enabled():  # only with create_graph=True
+        raise RuntimeError("dsalt_b200 operators have no second derivative")
+
+
 # --------------------------------------------------------------------------- 8 bits
 def _matrix(x: torch.Tensor):
-    """``x [..., n]`` as rows of consecutive values (a copy where its strides do not allow that)."""
-    x2 = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
-    if x2.shape[1] > 1 and x2.stride(1) != 1 or x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]:
-        x2 = x2.contiguous()
-    return x2, (x2.stride(0) if x2.shape[0] > 1 else x2.shape[1])
+    """``x [..., n]`` as rows of consecutive values and their stride (a copy where its strides do not
+    allow that)."""
+    n = x.shape[-1]
+    if x.is_contiguous():
+        return (x if x.dim() == 2 else x.view(-1, n)), n
+    if x.dim() != 2:
+        x = x.reshape(-1, n)
+    row, one = x.stride()
+    if n > 1 and one != 1 or x.shape[0] > 1 and row < n:
+        return x.contiguous(), n
+    return x, (row if x.shape[0] > 1 else n)
 
 
 def _pack(dev, x2, stride):
     rows, n = x2.shape
-    codes = torch.empty(rows, n, dtype=torch.int8, device=dev)
-    exps = torch.empty(rows, -(-n // GROUP), dtype=torch.uint8, device=dev)
+    codes = torch.empty((rows, n), dtype=torch.int8, device=dev)
+    exps = torch.empty((rows, -(-n // GROUP)), dtype=torch.uint8, device=dev)
     _run(dev, "dsalt_pack8", x2.data_ptr(), _dt(x2), rows, n, stride, codes.data_ptr(), exps.data_ptr())
     return codes, exps
 
@@ -52,12 +62,15 @@ def pack8(x):
     dev = _on_one_device(x)
     if x.dim() < 1:
         raise ValueError("pack8 needs at least one axis")
+    shape = x.shape
+    if len(shape) == 2 and shape[1]:
+        return _pack(dev, *_matrix(x))
     if x.numel() == 0:
         _dt(x)
-        return (torch.empty(x.shape, dtype=torch.int8, device=dev),
-                torch.empty(x.shape[:-1] + (-(-x.shape[-1] // GROUP),), dtype=torch.uint8, device=dev))
+        return (torch.empty(shape, dtype=torch.int8, device=dev),
+                torch.empty(shape[:-1] + (-(-shape[-1] // GROUP),), dtype=torch.uint8, device=dev))
     codes, exps = _pack(dev, *_matrix(x.detach()))
-    return codes.view(x.shape), exps.view(x.shape[:-1] + (-1,))
+    return codes.view(shape), exps.view(shape[:-1] + (-1,))
 
 
 def unpack8(codes, exps, dtype=torch.bfloat16):
@@ -65,60 +78,60 @@ def unpack8(codes, exps, dtype=torch.bfloat16):
     dev = _on_one_device(codes, exps)
     if codes.dim() < 1:
         raise ValueError("codes need at least one axis")
-    n = codes.shape[-1]
-    _want(codes, "codes", torch.int8, codes.shape)
-    _want(exps, "exps", torch.uint8, codes.shape[:-1] + (-(-n // GROUP),))
-    out = torch.empty(codes.shape, dtype=dtype, device=dev)
-    rows = codes.numel() // n if n else 0
-    _run(dev, "dsalt_unpack8", codes.data_ptr(), exps.data_ptr(), rows, n, out.data_ptr(), _dt(out))
+    shape = codes.shape
+    n = shape[-1]
+    _want(codes, "codes", torch.int8, shape)
+    _want(exps, "exps", torch.uint8, shape[:-1] + (-(-n // GROUP),))
+    out = torch.empty(shape, dtype=dtype, device=dev)
+    _run(dev, "dsalt_unpack8", codes.data_ptr(), exps.data_ptr(), codes.numel() // n if n else 0, n, out.data_ptr(),
+         _dt(out))
     return out
 
 
 # --------------------------------------------------------------------------- heads
-def _tables(cos, sin, D: int):
-    """Both tables as fp32 with 16-byte aligned rows of one stride: ``(cos, sin, stride)``."""
-    if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] not in (D, D // 2):
-        raise ValueError(f"cos and sin must be [rows, {D}] or [rows, {D // 2}], both alike")
-    out = []
-    for t in (cos, sin):
+def _table(t, D: int):
+    """A table of angles as fp32 with 16-byte aligned rows, and their stride."""
+    if t.dtype is not torch.float32:
         t = t.float()
-        one_row = t.shape[0] <= 1
-        if t.stride(1) != 1 or t.data_ptr() % 16 or not one_row and (t.stride(0) % 4 or t.stride(0) < D // 2):
-            t = t.clone(memory_format=torch.contiguous_format)
-        out.append(t)
-    cos, sin = out
-    if cos.shape[0] <= 1:
-        return cos, sin, -(-D // 4) * 4
-    if cos.stride(0) != sin.stride(0):
-        cos, sin = cos.contiguous(), sin.contiguous()
-    return cos, sin, cos.stride(0)
+    row, one = t.stride()
+    several = t.shape[0] > 1
+    if one != 1 or t.data_ptr() % 16 or several and (row % 4 or row < D // 2):
+        t = t.clone(memory_format=torch.contiguous_format)
+        row = t.stride(0)
+    return t, (row if several else -(-D // 4) * 4)
 
 
 def _rope_args(q, k, cos, sin, positions, q_weight, k_weight):
-    """Checked arguments: ``(dev, T, H, H_kv, D, stride of the tables, cos, sin, positions,
-    q_weight, k_weight)``."""
+    """Checked arguments: ``(dev, T, H, H_kv, D, stride of the tables, cos, sin, positions, q_weight,
+    k_weight)``."""
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError("q must be [T, H, D] and k [T, H_kv, D]")
     dev = _on_one_device(q, k, cos, sin, positions, q_weight, k_weight)
     T, H, D = q.shape
-    Hk = k.shape[1]
-    if k.shape[0] != T or k.shape[2] != D:
+    Tk, Hk, Dk = k.shape
+    if Tk != T or Dk != D:
         raise ValueError(f"k must be [{T}, H_kv, {D}], got {tuple(k.shape)}")
-    if k.dtype != q.dtype:
+    if k.dtype is not q.dtype:
         raise TypeError("q and k must share a dtype")
     if (q_weight is None) != (k_weight is None):
         raise ValueError("q_weight and k_weight go together")
     if q_weight is not None:
         _want(q_weight, "q_weight", q_weight.dtype, (D,))
         _want(k_weight, "k_weight", q_weight.dtype, (D,))
-        _dt(q_weight)
     if D % 2:
         raise ValueError(f"head_dim {D} is odd")
-    cos, sin, stride = _tables(cos, sin, D)
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] not in (D, D // 2):
+        raise ValueError(f"cos and sin must be [rows, {D}] or [rows, {D // 2}], both alike")
+    cos, stride = _table(cos, D)
+    sin, other = _table(sin, D)
+    if other != stride:
+        cos, sin = cos.contiguous(), sin.contiguous()
+        stride = cos.stride(0)
     if positions is not None:
         if positions.shape != (T,) or positions.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"positions must be [{T}] whole numbers")
-        positions = positions.to(torch.int32).contiguous()
+        if positions.dtype is not torch.int32 or not positions.is_contiguous():
+            positions = positions.to(torch.int32).contiguous()
         if cos.shape[0] == 0 and T:
             raise ValueError("empty tables")
     elif cos.shape[0] < T:
@@ -128,8 +141,8 @@ def _rope_args(q, k, cos, sin, positions, q_weight, k_weight):
 
 def _rope_forward(q, k, args, eps):
     dev, T, H, Hk, D, stride, cos, sin, positions, q_weight, k_weight = args
-    qo = torch.empty(T, H, D, dtype=q.dtype, device=dev)
-    ko = torch.empty(T, Hk, D, dtype=q.dtype, device=dev)
+    qo = torch.empty((T, H, D), dtype=q.dtype, device=dev)
+    ko = torch.empty((T, Hk, D), dtype=q.dtype, device=dev)
     q, q_token, q_head = _rows(q)
     k, k_token, k_head = _rows(k)
     _run(dev, "dsalt_qk_norm_rope", q.data_ptr(), k.data_ptr(), _dt(q), T, H, Hk, D, q_token, q_head, k_token, k_head,
@@ -150,12 +163,12 @@ class QKNormRopeFunction(torch.autograd.Function):
         return _rope_forward(q, k, args, eps)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gq, gk):
+        _no_second_derivative()
         q, k, cos, sin, positions, q_weight, k_weight = ctx.saved_tensors
         dev, (T, H, D), Hk = q.device, q.shape, k.shape[1]
-        dq = torch.empty(T, H, D, dtype=q.dtype, device=dev)
-        dk = torch.empty(T, Hk, D, dtype=q.dtype, device=dev)
+        dq = torch.empty((T, H, D), dtype=q.dtype, device=dev)
+        dk = torch.empty((T, Hk, D), dtype=q.dtype, device=dev)
         norm = q_weight is not None
         dwq, dwk = (torch.empty_like(q_weight), torch.empty_like(k_weight)) if norm else (None, None)
         ws = _workspace(_rope_workspace(D) if norm else 0, dev)
@@ -186,24 +199,25 @@ def qk_norm_rope(q, k, cos, sin, *, positions=None, q_weight=None, k_weight=None
     not read, or ``[rows, D/2]``); token ``t`` takes row ``positions[t]``, or row ``t``. A position outside
     the tables is taken as 0 and reported by :func:`dsalt_b200.device_status` (51). Differentiable in
     ``q``, ``k`` and the weights."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight is not None and q_weight.requires_grad
+                                    or k_weight is not None and k_weight.requires_grad):
         return QKNormRopeFunction.apply(q, k, q_weight, k_weight, cos, sin, positions, eps)
     return _rope_forward(q, k, _rope_args(q, k, cos, sin, positions, q_weight, k_weight), eps)
 
 
 # --------------------------------------------------------------------------- feed-forward
-def _aligned(t):
-    """``t`` with 16-byte aligned rows, where its sizes allow that without padding."""
+def _aligned(t, stride: int) -> bool:
+    """Whether the rows of ``t`` are 16-byte aligned, or their length does not allow that anyway."""
     es = t.element_size()
-    if t.shape[1] * es % 16 == 0 and (t.data_ptr() % 16 or t.shape[0] > 1 and t.stride(0) * es % 16):
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
+    return t.shape[1] * es % 16 != 0 or t.data_ptr() % 16 == 0 and stride * es % 16 == 0
 
 
 def _ffn_rows(x):
-    x2, stride = _matrix(x)
-    y = _aligned(x2)
-    return (x2, stride) if y is x2 else (y, y.shape[1])
+    x, stride = _matrix(x)
+    if not _aligned(x, stride):
+        x = x.clone(memory_format=torch.contiguous_format)
+        stride = x.shape[1]
+    return x, stride
 
 
 def _ffn_args(x, w_gate, w_up, w_down, activation, keep):
@@ -214,7 +228,7 @@ def _ffn_args(x, w_gate, w_up, w_down, activation, keep):
     if x.shape[-1] != d or w_up.shape != w_gate.shape or w_down.shape[1] != F:
         raise ValueError(f"x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)} and w_down "
                          f"{tuple(w_down.shape)} do not fit together")
-    if not (x.dtype == w_gate.dtype == w_up.dtype == w_down.dtype):
+    if not (x.dtype is w_gate.dtype is w_up.dtype is w_down.dtype):
         raise TypeError("x and the weights must share a dtype")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}")
@@ -239,15 +253,18 @@ def _ffn_pitch(F: int) -> int:
     return L.query("dsalt_gated_ffn_pitch", F)
 
 
-def _weights(*ws):
-    return [_aligned(w.contiguous()) for w in ws]
+def _weight(w):
+    if w.is_contiguous():
+        return w if _aligned(w, w.shape[1]) else w.clone()
+    return w.contiguous()
 
 
 def _ffn_forward(x2, stride, w_gate, w_up, w_down, sizes, act, keep):
     """``(y, kept, exps)`` of rows ``x2``; nothing is kept with ``L.KEEP_NONE``."""
     dev, d, F, d_out = sizes
     T = x2.shape[0]
-    y = torch.empty(T, d_out, dtype=x2.dtype, device=dev)
+    dt = _dt(x2)
+    y = torch.empty((T, d_out), dtype=x2.dtype, device=dev)
     kept = exps = None
     if keep:
         pitch = _ffn_pitch(F)
@@ -255,8 +272,8 @@ def _ffn_forward(x2, stride, w_gate, w_up, w_down, sizes, act, keep):
         kept = torch.empty(2 if coded else 3, T, pitch, dtype=torch.int8 if coded else x2.dtype, device=dev)
         if coded:
             exps = torch.empty(2, T, pitch // GROUP, dtype=torch.uint8, device=dev)
-    ws = _workspace(_ffn_workspace(_dt(x2), T, d, F, d_out, 0), dev)
-    _run(dev, "dsalt_gated_ffn", x2.data_ptr(), _dt(x2), T, d, stride, w_gate.data_ptr(), w_up.data_ptr(),
+    ws = torch.empty(_ffn_workspace(dt, T, d, F, d_out, 0), dtype=torch.uint8, device=dev)
+    _run(dev, "dsalt_gated_ffn", x2.data_ptr(), dt, T, d, stride, w_gate.data_ptr(), w_up.data_ptr(),
          w_down.data_ptr(), F, d_out, act, keep, _ptr(kept), _ptr(exps), y.data_ptr(), ws.data_ptr(), ws.numel())
     return y, kept, exps
 
@@ -271,7 +288,7 @@ class GatedFFNFunction(torch.autograd.Function):
         sizes = _ffn_args(x, w_gate, w_up, w_down, activation, keep)
         act, mode = ACTIVATIONS[activation], KEEP[keep]
         x2, stride = _ffn_rows(x)
-        ws = _weights(w_gate, w_up, w_down)
+        ws = _weight(w_gate), _weight(w_up), _weight(w_down)
         y, kept, exps = _ffn_forward(x2, stride, *ws, sizes, act, mode)
         x_exps = None
         if not (ctx.needs_input_grad[1] or ctx.needs_input_grad[2]):
@@ -280,11 +297,11 @@ class GatedFFNFunction(torch.autograd.Function):
             x2, x_exps = _pack(sizes[0], x2, stride)
         ctx.save_for_backward(x2, x_exps, kept, exps, *ws)
         ctx.act, ctx.mode, ctx.sizes, ctx.shape, ctx.stride = act, mode, sizes, x.shape, stride
-        return y.view(*x.shape[:-1], sizes[3])
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], sizes[3])
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _no_second_derivative()
         x2, x_exps, kept, exps, w_gate, w_up, w_down = ctx.saved_tensors
         dev, d, F, d_out = ctx.sizes
         need_x, need_gate, need_up, need_down = ctx.needs_input_grad[:4]
@@ -317,9 +334,9 @@ def gated_ffn(x, w_gate, w_up, w_down, *, activation: str = "silu", keep: str = 
     if x.is_cuda and torch.is_autocast_enabled("cuda"):
         dt = torch.get_autocast_dtype("cuda")
         x, w_gate, w_up, w_down = (t.to(dt) for t in (x, w_gate, w_up, w_down))
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate, w_up, w_down)):
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
         return GatedFFNFunction.apply(x, w_gate, w_up, w_down, activation, keep)
     sizes = _ffn_args(x, w_gate, w_up, w_down, activation, keep)
     x2, stride = _ffn_rows(x)
-    y, _, _ = _ffn_forward(x2, stride, *_weights(w_gate, w_up, w_down), sizes, ACTIVATIONS[activation], L.KEEP_NONE)
-    return y.view(*x.shape[:-1], sizes[3])
+    y, _, _ = _ffn_forward(x2, stride, _weight(w_gate), _weight(w_up), _weight(w_down), sizes, ACTIVATIONS[activation], L.KEEP_NONE)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], sizes[3])
