@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(THREADS) act_kernel(const float* __restrict__ 
     const int64_t at = i * GROUP8 + lane;
     const bool in = at % pitch < F;
     const float a = in ? g[at] : 0.f, b = in ? u[at] : 0.f;
-    h[at] = from_float<T>(activate<ACT>(a) * b);
+    h[at] = from_float<T>(activate<ACT, false>(a) * b);
     if (keep == DSALT_KEEP_INPUT) {
       static_cast<T*>(kept)[at] = from_float<T>(a);
       static_cast<T*>(kept)[plane + at] = from_float<T>(b);
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(THREADS) act_grad_kernel(const float* __restri
     }
     const float d = at % pitch < F ? dh[at] : 0.f;
     float v, dv;
-    activate_grad<ACT>(a, v, dv);
+    activate_grad<ACT, false>(a, v, dv);
     if (h) h[at] = from_float<T>(v * b);
     dg[at] = from_float<T>(d * b * dv);
     du[at] = from_float<T>(d * v);

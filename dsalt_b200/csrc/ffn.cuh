@@ -7,22 +7,33 @@ namespace dsalt {
 namespace ffn {
 
 // act(g) and act'(g) in fp32. silu: g p with p = 1 / (1 + e^-g); gelu: g p with p the normal
-// distribution's share below g.
-template <int ACT>
+// distribution's share below g. FAST (the tensor cores' epilogues, whose results are rounded to 16 bits and
+// added up with others of the size of u): p by Hastings' approximation (Abramowitz and Stegun 7.1.26),
+// off by 7.5e-8 at most, with the exponential that the derivative needs as well; CUDA's function, which
+// keeps the relative error of far negative g, takes about three times the instructions (first epilogue of
+// 1999 x 768 -> 2048: 30 us against 25).
+__device__ __forceinline__ float share_below(float g, float e) {  // e = exp(-g^2 / 2)
+  const float t = __fdividef(1.f, fmaf(0.3275911f * 0.70710678f, fabsf(g), 1.f));
+  const float tail =
+      0.5f * e * t * fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t, -0.284496736f), t, 0.254829592f);
+  return g < 0.f ? tail : 1.f - tail;
+}
+template <int ACT, bool FAST>
 __device__ __forceinline__ float activate(float g) {
   if constexpr (ACT == DSALT_ACT_SILU) return __fdividef(g, 1.f + __expf(-g));
+  else if constexpr (FAST) return g * share_below(g, __expf(-0.5f * g * g));
   else return g * normcdff(g);
 }
-template <int ACT>
+template <int ACT, bool FAST>
 __device__ __forceinline__ void activate_grad(float g, float& a, float& da) {
   if constexpr (ACT == DSALT_ACT_SILU) {
     const float p = __fdividef(1.f, 1.f + __expf(-g));
     a = g * p;
     da = p * (1.f + g * (1.f - p));
   } else {
-    const float p = normcdff(g);
+    const float e = __expf(-0.5f * g * g), p = FAST ? share_below(g, e) : normcdff(g);
     a = g * p;
-    da = p + g * 0.3989422804014327f * __expf(-0.5f * g * g);
+    da = p + g * 0.3989422804014327f * e;
   }
 }
 

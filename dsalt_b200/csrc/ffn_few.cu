@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(THREADS) ffn_few_kernel(const __grid_constant_
       const int r = 2 * lane;
       if (r < a.box && f0 + r < a.rows) {
         const float2 g = load_peer2(base + (t * ROWS + r) * 4), u = load_peer2(base + (t * ROWS + a.box + r) * 4);
-        *reinterpret_cast<uint32_t*>(out + r) = narrow2<T>(activate<ACT>(g.x) * u.x, activate<ACT>(g.y) * u.y);
+        *reinterpret_cast<uint32_t*>(out + r) = narrow2<T>(activate<ACT, true>(g.x) * u.x, activate<ACT, true>(g.y) * u.y);
       }
     } else {
       float2 v[2][MAX_SPLIT];

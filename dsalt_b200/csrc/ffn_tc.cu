@@ -45,6 +45,7 @@ struct alignas(64) Job {
   CUtensorMap c[3];
   int tiles_m, tiles_n, blocks0, blocks;  // blocks of K in the first segment and in all
   int rows, cols;                         // of the outputs
+  void* out;                              // of c[0], for a plain store's sums of several parts
 };
 struct Kept {
   void* p;           // gate's and up's [2, T, pitch]
@@ -56,7 +57,7 @@ template <int NJ>
 struct Args {
   Job job[NJ];
   Kept kept;
-  int tiles;
+  int tiles, split;  // split > 1: a cluster of so many pairs shares a tile, each takes a part of K
   uint32_t idesc;
   int* err;
 };
@@ -91,12 +92,13 @@ __device__ __forceinline__ void pair_mma(uint32_t d, uint64_t a, uint64_t b, uin
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// arrives on the barrier at this offset in both CTAs once the thread's products so far are done
-__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+// arrives on the barrier at this offset in both CTAs of the pair (ranks leader, leader + 1) once the
+// thread's products so far are done
+__device__ __forceinline__ void pair_commit(uint64_t* bar, uint32_t leader) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
           smem_u32(bar)),
-      "h"((uint16_t)3)
+      "h"((uint16_t)(3u << leader))
       : "memory");
 }
 
@@ -232,7 +234,7 @@ struct KeptRow {
 
 // ---------------------------------------------------------------- the kernel
 template <int EPI, bool A_MN, bool B_MN, typename T, int ACT, int KEEP, int NJ>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(THREADS, 1)
     ffn_pair_kernel(const __grid_constant__ Args<NJ> args) {
   using S = Shape<EPI, KEEP>;
   constexpr int STAGES = S::STAGES;
@@ -241,8 +243,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   const uint32_t staging = base + STAGES * STAGE_BYTES;
   Bars<STAGES>& bars = *reinterpret_cast<Bars<STAGES>*>(raw + (staging + EPI_WARPS * S::WARP_BYTES - smem_u32(raw)));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const uint32_t rank = cluster_rank() & 1u;
-  const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+  const uint32_t cta = cluster_rank(), rank = cta & 1u, leader = cta & ~1u;
+  const int part = EPI == PLAIN ? (int)cta / 2 : 0, split = EPI == PLAIN ? args.split : 1;
+  const int pair = blockIdx.x / 2 / split, pairs = gridDim.x / 2 / split;  // or cluster and clusters
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
@@ -266,6 +270,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // a product before this one may still be running
 
   if (warp == 0) {
     if (lane == 0) {  // loads of this CTA's halves of A and B
@@ -277,13 +282,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const Job& job = args.job[tile.job];
         const int m0 = tile.m * PAIR_M + (int)rank * CTA_M;
         const int n0 = EPI == GATE_UP ? tile.n * (PAIR_N / 2) : tile.n * PAIR_N + (int)rank * (PAIR_N / 2);
-        for (int kb = 0; kb < job.blocks; ++kb) {
+        const int last = (part + 1) * job.blocks / split;
+        for (int kb = part * job.blocks / split; kb < last; ++kb) {
           if (!mbar_wait(&bars.empty[s], phase ^ 1, args.err, 61)) {
             ok = false;
             break;
           }
           if (rank == 0) mbar_arrive_expect_tx(&bars.full[s], 2 * STAGE_BYTES);
-          const uint32_t full = in_cta(smem_u32(&bars.full[s]), 0);
+          const uint32_t full = in_cta(smem_u32(&bars.full[s]), leader);
           const int seg = kb >= job.blocks0, k = (seg ? kb - job.blocks0 : kb) * KB;
           const uint32_t a = base + s * STAGE_BYTES, b = a + OPERAND_BYTES;
           const CUtensorMap* ma = &job.a[seg];
@@ -315,7 +321,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       bool ok = true;
       for (int t = pair; ok && t < args.tiles; t += pairs, ++it) {
         const Tile tile = find_tile<NJ>(args, t);
-        const int blocks = args.job[tile.job].blocks, acc = it & 1;
+        const int all = args.job[tile.job].blocks, blocks = (part + 1) * all / split - part * all / split, acc = it & 1;
         if (!mbar_wait(&bars.acc_empty[acc], ((it >> 1) & 1) ^ 1, args.err, 62)) break;
         tc_fence_after();
         const uint32_t d = tmem + acc * PAIR_N;
@@ -333,13 +339,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             const uint64_t db = B_MN ? sw128_desc(b + ks * 2048, OPERAND_BYTES / 2, 1024) : sw128_desc(b + ks * 32, 16, 1024);
             pair_mma(d, da, db, args.idesc, kb | ks);
           }
-          pair_commit(&bars.empty[s]);
+          pair_commit(&bars.empty[s], leader);
           if (++s == STAGES) {
             s = 0;
             phase ^= 1;
           }
         }
-        if (ok) pair_commit(&bars.acc_full[acc]);
+        if (ok) pair_commit(&bars.acc_full[acc], leader);
       }
     }
     __syncwarp();
@@ -397,7 +403,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               float v, dv;
-              activate_grad<ACT>(a[i], v, dv);
+              activate_grad<ACT, true>(a[i], v, dv);
               a[i] = d[16 * half + i] * b[i] * dv;
               b[i] *= v;
               e[i] = d[16 * half + i] * v;
@@ -439,7 +445,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             su[half] = form_codes(u, cu[half]);
           }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) g[i] = activate<ACT>(g[i]) * u[i];
+          for (int i = 0; i < 32; ++i) g[i] = activate<ACT, true>(g[i]) * u[i];
           if (in) store_row<T, 32>(static_cast<T*>(args.kept.h) + at + 32 * half, g);
         }
         if constexpr (KEEP == DSALT_KEEP_8BIT) {
@@ -464,6 +470,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           float d[BOX];
           take_acc<BOX>(r, d);
           if (c + BOX < S::COLS) ask_acc<BOX>(mine + c + BOX, r);
+          if (split > 1) {  // sums of this part of K, as [column][row], where the operands were
+#pragma unroll
+            for (int i = 0; i < BOX; ++i)
+              asm volatile("st.shared.f32 [%0], %1;" ::"r"(base + ((side * S::COLS + c + i) * CTA_M + quad * 32 + lane) * 4),
+                           "f"(d[i])
+                           : "memory");
+            continue;
+          }
           const uint32_t to = next_boxes();
           stage_row<T, BOX>(to, lane, d, 0);
           send(to, col0 + c);
@@ -471,14 +485,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_remote(in_cta(smem_u32(&bars.acc_empty[acc]), 0));
+      if (lane == 0) arrive_remote(in_cta(smem_u32(&bars.acc_empty[acc]), leader));
     }
     if (lane == 0) store_wait_all();
     __syncwarp();
   }
   tc_fence_before();
+  if constexpr (EPI == PLAIN) {
+    if (split > 1) {
+      // the parts' sums, in the order of the parts: each pair adds up and stores its share of the columns
+      cluster_sync();
+      const Tile tile = find_tile<NJ>(args, pair);
+      const Job& job = args.job[tile.job];
+      const int row = warp % 4 * 32 + lane, m = tile.m * PAIR_M + (int)rank * CTA_M + row;
+      const int lo = part * 32 / split, hi = (part + 1) * 32 / split;  // in groups of 8 columns
+#pragma unroll 2
+      for (int g = lo + warp / 4; g < hi; g += THREADS / 128) {
+        float v[4][8];  // all parts' loads under way at once
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const uint32_t from = in_cta(base + (g * 8 * CTA_M + row) * 4, 2 * (p < split ? p : 0) + rank);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            v[p][i] = 0.f;
+            if (p < split)
+              asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[p][i]) : "r"(from + i * CTA_M * 4) : "memory");
+          }
+        }
+#pragma unroll
+        for (int p = 1; p < 4; ++p)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[0][i] += v[p][i];
+        const int n = tile.n * PAIR_N + g * 8;
+        if (m < job.rows && n < job.cols)
+          *reinterpret_cast<uint4*>(static_cast<T*>(job.out) + (int64_t)m * job.cols + n) =
+              make_uint4(narrow2<T>(v[0][0], v[0][1]), narrow2<T>(v[0][2], v[0][3]), narrow2<T>(v[0][4], v[0][5]),
+                         narrow2<T>(v[0][6], v[0][7]));
+      }
+    }
+  }
   __syncthreads();
-  cluster_sync();  // the other CTA's barriers and operands are not touched after this
+  cluster_sync();  // the other CTAs' barriers, operands and sums are not touched after this
   if (warp == 2)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
 }
@@ -499,20 +546,45 @@ void size_job(Job& j, int64_t M, int64_t N, int64_t K, int tile_n) {
   j.cols = (int)N;
 }
 
+// `after`: the launch before it in the stream is one of this call, whose end it may overlap
 template <int EPI, bool A_MN, bool B_MN, typename T, int ACT, int KEEP, int NJ>
-int launch_pair(Args<NJ>& a, const Ffn& f, const char* what) {
+int launch_pair(Args<NJ>& a, const Ffn& f, bool after, const char* what) {
   static std::atomic<uint64_t> ready{0};
-  constexpr int bytes = Shape<EPI, KEEP>::SMEM_BYTES;
+  constexpr int bytes = Shape<EPI, KEEP>::SMEM_BYTES, PAIRS = 74;
   static_assert(bytes <= 232448, "shared memory of a block");
+  static_assert(EPI != PLAIN || Shape<EPI, KEEP>::STAGES * STAGE_BYTES >= CTA_M * PAIR_N * 4, "the sums of a part do not fit");
   auto kernel = ffn_pair_kernel<EPI, A_MN, B_MN, T, ACT, KEEP, NJ>;
   if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), bytes, ready)) return rc;
   a.tiles = 0;
-  for (int i = 0; i < NJ; ++i) a.tiles += a.job[i].tiles_m * a.job[i].tiles_n;
+  int blocks = 1 << 30;
+  for (int i = 0; i < NJ; ++i)
+    if (a.job[i].tiles_m) {
+      a.tiles += a.job[i].tiles_m * a.job[i].tiles_n;
+      blocks = a.job[i].blocks < blocks ? a.job[i].blocks : blocks;
+    }
+  // Where the tiles leave half of the pairs idle, K is split over 2 to 4 pairs of a cluster, as far as all
+  // clusters run at once: of 4, 6 and 8 CTAs of this size the GPU holds 33, 22 and 15 (its processing
+  // clusters have odd numbers of SMs left over). 24 tiles of K = 2048: two parts 12 us, three 25, one 16.
+  constexpr int AT_ONCE[5] = {0, PAIRS, 33, 22, 15};
+  a.split = 1;
+  if (EPI == PLAIN)
+    while (a.split < 4 && a.tiles <= AT_ONCE[a.split + 1] && 4 * (a.split + 1) <= blocks) ++a.split;
   a.idesc = umma_idesc_f16(f.dtype == DSALT_BF16 ? 1 : 0, A_MN, B_MN, PAIR_M, PAIR_N);
   a.err = device_status_ptr();
-  const int pairs = a.tiles < 74 ? a.tiles : 74;
-  kernel<<<2 * pairs, THREADS, bytes, f.stream>>>(a);
-  return check_cuda(cudaGetLastError(), what);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * a.split * (a.split > 1 || a.tiles < PAIRS ? a.tiles : PAIRS));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = f.stream;
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2 * a.split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = after ? 2 : 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, a), what);
 }
 
 template <typename T, int ACT, int KEEP>
@@ -525,7 +597,7 @@ int gate_up(const Ffn& f) {
       (rc = operand(&j.b[1], f.w_up, f, f.F, f.d, f.d, false)))
     return rc;
   a.kept = {f.kept, f.exps, f.h, f.T, f.pitch};
-  return launch_pair<GATE_UP, false, false, T, ACT, KEEP, 1>(a, f, "gated_ffn gate and up launch");
+  return launch_pair<GATE_UP, false, false, T, ACT, KEEP, 1>(a, f, false, "gated_ffn gate and up launch");
 }
 
 template <typename T, int ACT>
@@ -540,7 +612,8 @@ int forward(const Ffn& f) {
   if ((rc = operand(&j.a[0], f.h, f, f.T, f.F, f.pitch, false)) ||
       (rc = operand(&j.b[0], f.w_down, f, f.d_out, f.F, f.F, false)) || (rc = output(&j.c[0], f.y, f, f.T, f.d_out, f.d_out)))
     return rc;
-  return launch_pair<PLAIN, false, false, T, 0, 0, 1>(a, f, "gated_ffn down launch");
+  j.out = f.y;
+  return launch_pair<PLAIN, false, false, T, 0, 0, 1>(a, f, true, "gated_ffn down launch");
 }
 
 template <typename T, int ACT, int KEEP>
@@ -554,7 +627,7 @@ int grads(const Ffn& f) {
       (rc = output(&j.c[1], f.du, f, f.T, f.F, f.pitch)) || (KEEP == DSALT_KEEP_8BIT && (rc = output(&j.c[2], f.h, f, f.T, f.F, f.pitch))))
     return rc;
   a.kept = {f.kept, f.exps, f.h, f.T, f.pitch};
-  return launch_pair<GRADS, false, true, T, ACT, KEEP, 1>(a, f, "gated_ffn_bwd hidden gradients launch");
+  return launch_pair<GRADS, false, true, T, ACT, KEEP, 1>(a, f, false, "gated_ffn_bwd hidden gradients launch");
 }
 
 int weight_job(Job& j, const Ffn& f, const void* a, int64_t M, int64_t a_stride, const void* b, int64_t N, int64_t b_stride,
@@ -562,6 +635,7 @@ int weight_job(Job& j, const Ffn& f, const void* a, int64_t M, int64_t a_stride,
   size_job(j, M, N, f.T, PAIR_N);
   int rc;
   if ((rc = operand(&j.a[0], a, f, f.T, M, a_stride, true)) || (rc = operand(&j.b[0], b, f, f.T, N, b_stride, true))) return rc;
+  j.out = c;
   return output(&j.c[0], c, f, M, N, N);
 }
 
@@ -578,7 +652,8 @@ int backward(const Ffn& f) {
         (rc = operand(&j.b[0], f.w_gate, f, f.F, f.d, f.d, true)) || (rc = operand(&j.b[1], f.w_up, f, f.F, f.d, f.d, true)) ||
         (rc = output(&j.c[0], f.dx, f, f.T, f.d, f.d)))
       return rc;
-    if ((rc = launch_pair<PLAIN, false, true, T, 0, 0, 1>(a, f, "gated_ffn_bwd dx launch"))) return rc;
+    j.out = f.dx;
+    if ((rc = launch_pair<PLAIN, false, true, T, 0, 0, 1>(a, f, true, "gated_ffn_bwd dx launch"))) return rc;
   }
   if (!f.dw_gate && !f.dw_down) return DSALT_OK;
   Args<3> a{};
@@ -586,7 +661,7 @@ int backward(const Ffn& f) {
   if (f.dw_gate && ((rc = weight_job(a.job[1], f, f.dg, f.F, f.pitch, f.x, f.d, f.x_stride, f.dw_gate)) ||
                     (rc = weight_job(a.job[2], f, f.du, f.F, f.pitch, f.x, f.d, f.x_stride, f.dw_up))))
     return rc;
-  return launch_pair<PLAIN, true, true, T, 0, 0, 3>(a, f, "gated_ffn_bwd weights launch");
+  return launch_pair<PLAIN, true, true, T, 0, 0, 3>(a, f, true, "gated_ffn_bwd weights launch");
 }
 
 template <typename T>

@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(THREADS) ffn_token_kernel(const __grid_constan
       for (int c = 0; c < MAX_SPLIT; ++c) v += x[c][0], u += x[c][MATS - 1];
     }
     const int tok = i / ROWS, f = f0 + i % ROWS;
-    if constexpr (GATED) v = activate<ACT>(v) * u;
+    if constexpr (GATED) v = activate<ACT, true>(v) * u;
     if (tok < a.T && f < a.rows) static_cast<T*>(a.out)[tok * a.out_stride + f] = from_float<T>(v);
   }
   if (a.split > 1) cluster_sync();  // the others' reads of this block's sums
