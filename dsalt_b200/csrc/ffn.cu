@@ -1,7 +1,6 @@
 // The gated feed-forward block y = (act(x Wg^T) * (x Wu^T)) Wd^T and its gradients
 // (dsalt_gated_ffn, dsalt_gated_ffn_bwd): arguments, workspaces, and the path for what the tensor
-// cores do not take: fp32 inputs, and 16-bit ones whose rows are not 16-byte aligned. That path is
-// plain: products on the CUDA cores in fp32 (128 x 128 tiles, 8 x 8 outputs a thread), the
+// cores do not take: fp32 inputs, and sizes that are not multiples of 8. That path is plain: products on the CUDA cores in fp32 (128 x 128 tiles, 8 x 8 outputs a thread), the
 // activation and its gradient as kernels of their own between them.
 #include "ffn.cuh"
 
@@ -195,8 +194,10 @@ int run_plain(const Ffn& f, bool backward) {
   return backward ? backward_plain<T, DSALT_ACT_GELU>(f) : forward_plain<T, DSALT_ACT_GELU>(f);
 }
 
+bool tensor_cores(int dtype, int d, int F, int d_out);
+
 int run(const Ffn& f, bool backward) {
-  if (takes_tensor_cores(f)) return run_tensor_cores(f, backward);
+  if (tensor_cores(f.dtype, f.d, f.F, f.d_out)) return run_tensor_cores(f, backward);
   if (f.dtype == DSALT_F32) return run_plain<float>(f, backward);
   if (f.dtype == DSALT_BF16) return run_plain<__nv_bfloat16>(f, backward);
   return run_plain<__half>(f, backward);
@@ -204,6 +205,17 @@ int run(const Ffn& f, bool backward) {
 
 size_t a256(size_t v) { return (v + 255) & ~(size_t)255; }
 size_t elem_bytes(int dtype) { return dtype == DSALT_F32 ? 4 : 2; }
+// what the tensor cores take; their operands' rows have to be 16-byte aligned
+bool tensor_cores(int dtype, int d, int F, int d_out) { return dtype != DSALT_F32 && d % 8 == 0 && F % 8 == 0 && d_out % 8 == 0; }
+int check_rows(const char* fn, const Ffn& f) {
+  if (!tensor_cores(f.dtype, f.d, f.F, f.d_out)) return DSALT_OK;
+  for (const void* p : {f.x, f.dy, f.w_gate, f.w_up, f.w_down, (const void*)f.y, (const void*)f.dx, (const void*)f.dw_gate,
+                        (const void*)f.dw_up, (const void*)f.dw_down})
+    if (reinterpret_cast<uintptr_t>(p) & 15) return fail(DSALT_ERR_INVALID, "%s: operands must be 16-byte aligned", fn);
+  if ((f.x && f.x_stride % 8) || (f.dy && f.dy_stride % 8))
+    return fail(DSALT_ERR_INVALID, "%s: rows must be 16-byte aligned", fn);
+  return DSALT_OK;
+}
 bool off256(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 255) != 0; }
 bool known_dtype(int dt) { return dt == DSALT_F32 || dt == DSALT_BF16 || dt == DSALT_F16; }
 
@@ -231,7 +243,7 @@ int64_t dsalt_gated_ffn_pitch(int d_ff) { return d_ff < 1 ? 0 : pitch_of(d_ff); 
 size_t dsalt_gated_ffn_workspace_bytes(int dtype, int64_t T, int d_model, int d_ff, int d_out) {
   if (check("gated_ffn", dtype, T, d_model, d_ff, d_out, 0, 0)) return 0;
   const size_t n = (size_t)T * pitch_of(d_ff);
-  return a256(n * elem_bytes(dtype)) + a256(2 * n * sizeof(float)) + 256;
+  return a256(n * elem_bytes(dtype)) + (tensor_cores(dtype, d_model, d_ff, d_out) ? 0 : a256(2 * n * sizeof(float))) + 256;
 }
 
 int dsalt_gated_ffn(const void* x, int dtype, int64_t T, int d_model, int64_t x_stride, const void* w_gate,
@@ -254,14 +266,17 @@ int dsalt_gated_ffn(const void* x, int dtype, int64_t T, int d_model, int64_t x_
   f.h = keep == DSALT_KEEP_INPUT ? static_cast<char*>(kept) + 2 * T * f.pitch * elem_bytes(dtype) : workspace;
   f.wide = reinterpret_cast<float*>(static_cast<char*>(workspace) + a256((size_t)T * f.pitch * elem_bytes(dtype)));
   f.stream = static_cast<cudaStream_t>(stream);
+  if (int rc = check_rows(FN, f)) return rc;
   return run(f, false);
 }
 
 size_t dsalt_gated_ffn_bwd_workspace_bytes(int dtype, int64_t T, int d_model, int d_ff, int d_out, int keep) {
   if (check("gated_ffn_bwd", dtype, T, d_model, d_ff, d_out, 0, keep)) return 0;
   const size_t n = (size_t)T * pitch_of(d_ff);
-  return 3 * a256(n * elem_bytes(dtype)) + a256(n * sizeof(float)) +
-         (keep == DSALT_KEEP_8BIT ? a256((size_t)T * d_model * elem_bytes(dtype)) : 0) + 256;
+  // dg and du; of 8-bit activations h and x as well; the plain path's dh
+  return (keep == DSALT_KEEP_8BIT ? 3 : 2) * a256(n * elem_bytes(dtype)) +
+         (keep == DSALT_KEEP_8BIT ? a256((size_t)T * d_model * elem_bytes(dtype)) : 0) +
+         (tensor_cores(dtype, d_model, d_ff, d_out) ? 0 : a256(n * sizeof(float))) + 256;
 }
 
 int dsalt_gated_ffn_bwd(const void* dy, int dtype, int64_t T, int d_model, int64_t dy_stride, const void* x,
@@ -299,11 +314,13 @@ int dsalt_gated_ffn_bwd(const void* dy, int dtype, int64_t T, int d_model, int64
   f.stream = s;
   const size_t n = a256((size_t)T * f.pitch * es);
   char* ws = static_cast<char*>(workspace);
-  f.dg = ws, f.du = ws + n, f.wide = reinterpret_cast<float*>(ws + 3 * n);
+  f.dg = ws, f.du = ws + n;
+  char* wide_x = ws + 3 * n;
+  f.wide = reinterpret_cast<float*>(coded ? wide_x + a256((size_t)T * d_model * es) : ws + 2 * n);
   f.h = coded ? ws + 2 * n : static_cast<char*>(f.kept) + 2 * T * f.pitch * es;
   f.x = coded ? nullptr : x, f.x_stride = T > 1 ? x_stride : d_model;
+  if (int rc = check_rows(FN, f)) return rc;
   if (coded && dw_gate) {
-    void* wide_x = ws + 3 * n + a256((size_t)T * f.pitch * sizeof(float));
     if (int rc = launch_unpack8(static_cast<const int8_t*>(x), x_exps, T, d_model, wide_x, dtype, s)) return rc;
     f.x = wide_x, f.x_stride = d_model;
   }

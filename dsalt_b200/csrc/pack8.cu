@@ -20,6 +20,7 @@ namespace dsalt {
 namespace {
 
 constexpr int THREADS = 256;
+constexpr int64_t MAX_CHUNKS = 1ll << 31;  // of a launch: 64 GB and more
 
 __device__ __forceinline__ void ld32(uint32_t (&u)[8], const void* p) {
   asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -44,17 +45,17 @@ __device__ __forceinline__ void widen(const uint32_t (&u)[8], float (&f)[32 / si
 }
 
 // rows of n values in chunks of 32 bytes, a chunk per thread; a row's chunk count is rounded up
-// to whole groups, so that the lanes of a group are neighbours in a warp. I: 32 bits where they count the
-// chunks, whose division is a few instructions
-template <typename T, typename I>
-__global__ void __launch_bounds__(THREADS) pack_rows_kernel(const T* __restrict__ x, int64_t rows, int n,
+// to whole groups, so that the lanes of a group are neighbours in a warp. Chunks are counted in 32 bits, whose
+// division is a few instructions; the host calls for as many rows as that allows
+template <typename T>
+__global__ void __launch_bounds__(THREADS) pack_rows_kernel(const T* __restrict__ x, uint32_t rows, int n,
                                                             int64_t x_stride, int8_t* __restrict__ codes,
                                                             uint8_t* __restrict__ exps, int groups) {
   constexpr int N = 32 / (int)sizeof(T), LANES = GROUP8 / N;
-  const I chunks = (I)groups * LANES, total = (I)rows * chunks;
-  for (I i = (I)blockIdx.x * THREADS + threadIdx.x; i - threadIdx.x % 32 < total; i += (I)gridDim.x * THREADS) {
+  const uint32_t chunks = groups * LANES, total = rows * chunks;
+  for (uint32_t i = blockIdx.x * THREADS + threadIdx.x; i - threadIdx.x % 32 < total; i += gridDim.x * THREADS) {
     const bool in = i < total;
-    const I at_row = in ? i / chunks : 0;
+    const uint32_t at_row = in ? i / chunks : 0;
     const int64_t row = at_row;
     const int chunk = in ? (int)(i - at_row * chunks) : 0, col = chunk * N;
     const bool held = in && col < n;
@@ -97,14 +98,14 @@ __global__ void __launch_bounds__(THREADS) pack_any_kernel(const T* __restrict__
   }
 }
 
-template <typename T, typename I>
+template <typename T>
 __global__ void __launch_bounds__(THREADS) unpack_rows_kernel(const int8_t* __restrict__ codes,
-                                                              const uint8_t* __restrict__ exps, int64_t rows, int n,
+                                                              const uint8_t* __restrict__ exps, uint32_t rows, int n,
                                                               int groups, T* __restrict__ out) {
   constexpr int N = 32 / (int)sizeof(T);
-  const I chunks = n / N, total = (I)rows * chunks;
-  for (I i = (I)blockIdx.x * THREADS + threadIdx.x; i < total; i += (I)gridDim.x * THREADS) {
-    const I at_row = i / chunks;
+  const uint32_t chunks = n / N, total = rows * chunks;
+  for (uint32_t i = blockIdx.x * THREADS + threadIdx.x; i < total; i += gridDim.x * THREADS) {
+    const uint32_t at_row = i / chunks;
     const int64_t row = at_row;
     const int col = (int)(i - at_row * chunks) * N;
     const float scale = scale_of(exps[row * groups + col / GROUP8]);
@@ -151,30 +152,36 @@ template <typename T>
 int pack(const T* x, int64_t rows, int n, int64_t x_stride, int8_t* codes, uint8_t* exps, cudaStream_t stream) {
   constexpr int N = 32 / (int)sizeof(T);
   const int groups = (n + GROUP8 - 1) / GROUP8;
-  if (n % N == 0 && x_stride % N == 0 && aligned(x, 32) && aligned(codes, 16)) {
-    const int64_t chunks = rows * groups * (GROUP8 / N);
-    if (chunks < 1ll << 31)
-      pack_rows_kernel<T, uint32_t><<<blocks_for(chunks), THREADS, 0, stream>>>(x, rows, n, x_stride, codes, exps, groups);
-    else
-      pack_rows_kernel<T, int64_t><<<blocks_for(chunks), THREADS, 0, stream>>>(x, rows, n, x_stride, codes, exps, groups);
-  } else
+  if (n % N || x_stride % N || !aligned(x, 32) || !aligned(codes, 16)) {
     pack_any_kernel<T><<<blocks_for(rows * groups * 32), THREADS, 0, stream>>>(x, rows, n, x_stride, codes, exps, groups);
-  return check_cuda(cudaGetLastError(), "pack8 launch");
+    return check_cuda(cudaGetLastError(), "pack8 launch");
+  }
+  const int64_t most = MAX_CHUNKS / (groups * (GROUP8 / N));
+  for (int64_t r = 0; r < rows; r += most) {
+    const int64_t part = rows - r < most ? rows - r : most;
+    pack_rows_kernel<T><<<blocks_for(part * groups * (GROUP8 / N)), THREADS, 0, stream>>>(
+        x + r * x_stride, (uint32_t)part, n, x_stride, codes + r * n, exps + r * groups, groups);
+    if (int rc = check_cuda(cudaGetLastError(), "pack8 launch")) return rc;
+  }
+  return DSALT_OK;
 }
 
 template <typename T>
 int unpack(const int8_t* codes, const uint8_t* exps, int64_t rows, int n, T* out, cudaStream_t stream) {
   constexpr int N = 32 / (int)sizeof(T);
   const int groups = (n + GROUP8 - 1) / GROUP8;
-  if (n % N == 0 && aligned(out, 32) && aligned(codes, 16)) {
-    const int64_t chunks = rows * (n / N);
-    if (chunks < 1ll << 31)
-      unpack_rows_kernel<T, uint32_t><<<blocks_for(chunks), THREADS, 0, stream>>>(codes, exps, rows, n, groups, out);
-    else
-      unpack_rows_kernel<T, int64_t><<<blocks_for(chunks), THREADS, 0, stream>>>(codes, exps, rows, n, groups, out);
-  } else
+  if (n % N || !aligned(out, 32) || !aligned(codes, 16)) {
     unpack_any_kernel<T><<<blocks_for(rows * n), THREADS, 0, stream>>>(codes, exps, rows, n, groups, out);
-  return check_cuda(cudaGetLastError(), "unpack8 launch");
+    return check_cuda(cudaGetLastError(), "unpack8 launch");
+  }
+  const int64_t most = MAX_CHUNKS / (n / N);
+  for (int64_t r = 0; r < rows; r += most) {
+    const int64_t part = rows - r < most ? rows - r : most;
+    unpack_rows_kernel<T><<<blocks_for(part * (n / N)), THREADS, 0, stream>>>(codes + r * n, exps + r * groups, (uint32_t)part,
+                                                                              n, groups, out + r * n);
+    if (int rc = check_cuda(cudaGetLastError(), "unpack8 launch")) return rc;
+  }
+  return DSALT_OK;
 }
 
 int check_sizes(const char* fn, int dtype, int64_t rows, int64_t cols) {

@@ -320,6 +320,14 @@ class GatedFFNFunction(torch.autograd.Function):
                 None, None)
 
 
+def autocast_all(*ts):
+    """The tensors as a linear layer takes them: in autocast's dtype where that is on."""
+    if torch.is_autocast_enabled("cuda") and ts[0].is_cuda:
+        dt = torch.get_autocast_dtype("cuda")
+        return tuple(t.to(dt) for t in ts)
+    return ts
+
+
 def gated_ffn(x, w_gate, w_up, w_down, *, activation: str = "silu", keep: str = "16bit"):
     """``(act(x Wgᵀ) · (x Wuᵀ)) Wdᵀ``: ``x [..., d_model]``, ``w_gate, w_up [d_ff, d_model]``, ``w_down [d_out,
     d_ff]`` → ``[..., d_out]`` in ``x``'s dtype. Sums are fp32; the product of gate and up is rounded to the
@@ -331,9 +339,7 @@ def gated_ffn(x, w_gate, w_up, w_down, *, activation: str = "silu", keep: str = 
     are then those at the held values). bf16 and fp16 run on the tensor cores where sizes are
     multiples of 8; fp32 and other sizes on the CUDA cores. Under autocast all four are cast first, as
     a linear layer's are."""
-    if x.is_cuda and torch.is_autocast_enabled("cuda"):
-        dt = torch.get_autocast_dtype("cuda")
-        x, w_gate, w_up, w_down = (t.to(dt) for t in (x, w_gate, w_up, w_down))
+    x, w_gate, w_up, w_down = autocast_all(x, w_gate, w_up, w_down)
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
         return GatedFFNFunction.apply(x, w_gate, w_up, w_down, activation, keep)
     sizes = _ffn_args(x, w_gate, w_up, w_down, activation, keep)

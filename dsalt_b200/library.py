@@ -12,6 +12,9 @@ keeps its kernels opaque (``_dynamo_opaque``, ``dsalt/kernels/dsalt_triton_attn.
   → the functions of :mod:`dsalt_b200.serving` of these names (``sample_tokens`` with its settings as
   numbers and the log-probability)
 
+* ``torch.ops.dsalt_b200.qk_norm_rope`` / ``gated_ffn`` / ``pack8`` / ``unpack8``
+  → the functions of :mod:`dsalt_b200.layers` of these names, without gradients
+
 ``cu_list`` (the host copy of ``cu_seqlens``) is an ``int[]`` argument: the kernels size
 their launches and workspaces from it, so a compiled graph is specialised on the packing.
 The fake (meta) functions give the output shapes and dtypes; no real implementation runs
@@ -23,6 +26,7 @@ from typing import List, Optional
 
 import torch
 
+from . import layers
 from . import ops
 from . import serving
 
@@ -122,3 +126,47 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: float, top
 @sample_tokens.register_fake
 def _(logits, u, temperature, top_k, top_p, min_p):
     return [logits.new_empty(logits.shape[0], dtype=torch.int64), logits.new_empty(logits.shape[0], dtype=torch.float32)]
+
+
+@torch.library.custom_op("dsalt_b200::qk_norm_rope", mutates_args=())
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                 positions: Optional[torch.Tensor], q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                 eps: float) -> List[torch.Tensor]:
+    return list(layers.qk_norm_rope(q, k, cos, sin, positions=positions, q_weight=q_weight, k_weight=k_weight, eps=eps))
+
+
+@qk_norm_rope.register_fake
+def _(q, k, cos, sin, positions, q_weight, k_weight, eps):
+    return [q.new_empty(q.shape), k.new_empty(k.shape)]
+
+
+@torch.library.custom_op("dsalt_b200::gated_ffn", mutates_args=())
+def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+              activation: str) -> torch.Tensor:
+    return layers.gated_ffn(x, w_gate, w_up, w_down, activation=activation)
+
+
+@gated_ffn.register_fake
+def _(x, w_gate, w_up, w_down, activation):
+    return x.new_empty(x.shape[:-1] + (w_down.shape[0],))
+
+
+@torch.library.custom_op("dsalt_b200::pack8", mutates_args=())
+def pack8(x: torch.Tensor) -> List[torch.Tensor]:
+    return list(layers.pack8(x))
+
+
+@pack8.register_fake
+def _(x):
+    return [x.new_empty(x.shape, dtype=torch.int8),
+            x.new_empty(x.shape[:-1] + ((x.shape[-1] + layers.GROUP - 1) // layers.GROUP,), dtype=torch.uint8)]
+
+
+@torch.library.custom_op("dsalt_b200::unpack8", mutates_args=())
+def unpack8(codes: torch.Tensor, exps: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    return layers.unpack8(codes, exps, dtype)
+
+
+@unpack8.register_fake
+def _(codes, exps, dtype):
+    return codes.new_empty(codes.shape, dtype=dtype)

@@ -6,11 +6,12 @@ Same configuration fields, module names and state-dict keys as the reference's
 (``dsalt/kernels/RMSENorm.py``) and ``DSALTLMHeadModel`` (``dsalt/model/dsalt_lm.py:64-284``),
 so a reference checkpoint loads unchanged. Every block's attention is
 :class:`dsalt_b200.DSALTAttention` (widths, landmark selection and the sparse attention on
-this package's kernels); norms, the SwiGLU MLP, embeddings and the LM head are library
-ops. Packed input only (``input_ids [T]`` with ``cu_seqlens``), inference only: training,
-the losses and the batched path are not part of this package. ``generate`` (no counterpart in
-the reference) answers prompts token by token over the paged 8-bit cache of
-:mod:`dsalt_b200.serving`.
+this package's kernels); norms, embeddings and the LM head are library ops, the SwiGLU MLP too
+unless ``ffn`` asks for :func:`dsalt_b200.layers.gated_ffn` (``"fused"``; ``"fused_8bit"`` keeps its
+activations in 8 bits while training). Packed input only (``input_ids [T]`` with ``cu_seqlens``),
+inference only: training, the losses and the batched path are not part of this package (the blocks
+alone train). ``generate`` (no counterpart in the reference) answers prompts token by token over the
+paged 8-bit cache of :mod:`dsalt_b200.serving`.
 """
 from __future__ import annotations
 
@@ -23,14 +24,19 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import layers
 from .module import DSALTAttention
 from .serving import MAX_VOCAB, PagedCache, sample_tokens
+
+
+FFN_KINDS = ("library", "fused", "fused_8bit")
 
 
 @dataclass
 class DSALTConfig:
     """Hyperparameters of :class:`DSALTLMHeadModel` (the reference's fields and defaults;
-    ``selection`` / ``block`` choose this package's landmark selection mode)."""
+    ``selection`` / ``block`` choose this package's landmark selection mode, ``qk_norm`` norms query and
+    key heads, ``ffn`` chooses the feed-forward block's kernels: one of :data:`FFN_KINDS`)."""
     vocab_size: int
     d_model: int
     n_layers: int
@@ -52,8 +58,12 @@ class DSALTConfig:
     aux_loss_weight: float = 0.0
     selection: str = "global"
     block: int = 512
+    qk_norm: bool = False
+    ffn: str = "library"
 
     def __post_init__(self) -> None:
+        if self.ffn not in FFN_KINDS:
+            raise ValueError(f"ffn must be one of {FFN_KINDS}, got {self.ffn!r}")
         if self.d_model % self.n_heads != 0:
             raise ValueError(f"d_model ({self.d_model}) must be divisible by n_heads ({self.n_heads})")
         if not (0 <= self.n_min <= self.n_max):
@@ -93,34 +103,46 @@ class RMSENorm(nn.Module):
 
 
 class SwiGLUFFN(nn.Module):
-    """``down(silu(gate(x)) * up(x))``."""
+    """``down(silu(gate(x)) * up(x))``: by library products, or (``kind`` ``"fused"``, ``"fused_8bit"``) by
+    :func:`dsalt_b200.layers.gated_ffn`, whose backward pass finds its activations in the weights' dtype or
+    in 8 bits."""
 
-    def __init__(self, d_model: int, d_ff: int, dropout: float = 0.0):
+    def __init__(self, d_model: int, d_ff: int, dropout: float = 0.0, kind: str = "library"):
         super().__init__()
+        if kind not in FFN_KINDS:
+            raise ValueError(f"kind must be one of {FFN_KINDS}, got {kind!r}")
+        self.kind = kind
         self.gate_proj = nn.Linear(d_model, d_ff, bias=False)
         self.up_proj = nn.Linear(d_model, d_ff, bias=False)
         self.down_proj = nn.Linear(d_ff, d_model, bias=False)
 
     def forward(self, x):
-        return self.down_proj(F.silu(self.gate_proj(x)) * self.up_proj(x))
+        if self.kind == "library":
+            return self.down_proj(F.silu(self.gate_proj(x)) * self.up_proj(x))
+        weights = self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight
+        if torch.compiler.is_compiling():
+            return torch.ops.dsalt_b200.gated_ffn(*layers.autocast_all(x, *weights), "silu")
+        return layers.gated_ffn(x, *weights, keep="8bit" if self.kind == "fused_8bit" else "16bit")
 
 
 class DSALTTransformerBlock(nn.Module):
     """Pre-norm block: RMSNorm → DSALTAttention → residual, RMSNorm → SwiGLU → residual."""
 
     def __init__(self, d_model, n_heads, n_min, n_max, k_lmk, max_seq_len, d_ff, dropout=0.0, yarn_scale=1.0,
-                 layer_idx=0, n_kv_heads=None, qkv_bias=False, rope_base=10000.0, selection="global", block=512):
+                 layer_idx=0, n_kv_heads=None, qkv_bias=False, rope_base=10000.0, selection="global", block=512,
+                 qk_norm=False, ffn="library"):
         super().__init__()
         self.layer_idx = layer_idx
         self.attn_norm = RMSENorm(d_model)
         self.ffn_norm = RMSENorm(d_model)
         self.attn = DSALTAttention(d_model, n_heads, n_min, n_max, k_lmk, max_seq_len, dropout=dropout,
                                    yarn_scale=yarn_scale, layer_idx=layer_idx, n_kv_heads=n_kv_heads,
-                                   qkv_bias=qkv_bias, rope_base=rope_base, selection=selection, block=block)
+                                   qkv_bias=qkv_bias, rope_base=rope_base, selection=selection, block=block,
+                                   qk_norm=qk_norm)
         # the dense [H, T0, T0] _last_P rebuild is off in the decoder stack: at prefill lengths it
         # does not fit (set attn._collect_last_P = True on a layer whose metrics are wanted)
         self.attn._collect_last_P = False
-        self.ffn = SwiGLUFFN(d_model, d_ff, dropout)
+        self.ffn = SwiGLUFFN(d_model, d_ff, dropout, ffn)
 
     def forward(self, x, cu_seqlens=None, max_seqlen=None, gradient_checkpointing=False, rope_cs=None, cu_list=None):
         a, aux = self.attn(self.attn_norm(x), cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, rope_cs=rope_cs,
@@ -147,7 +169,7 @@ class DSALTLMHeadModel(nn.Module):
     def __init__(self, vocab_size, d_model, n_layers, n_heads, n_min, n_max, k_lmk, max_seq_len, d_ff=None,
                  dropout=0.0, yarn_scale=1.0, tie_weights=True, padding_idx=None, lm_head_chunk_size=2048,
                  loss_fn="chunked", aux_loss_weight=0.0, n_kv_heads=None, qkv_bias=False, rope_base=10000.0,
-                 selection="global", block=512):
+                 selection="global", block=512, qk_norm=False, ffn="library"):
         super().__init__()
         del lm_head_chunk_size, loss_fn, aux_loss_weight  # training-only settings of the reference
         self.d_model, self.n_layers, self.vocab_size = d_model, n_layers, vocab_size
@@ -156,7 +178,7 @@ class DSALTLMHeadModel(nn.Module):
         self.embed_tokens = nn.Embedding(vocab_size, d_model, padding_idx=padding_idx)
         self.layers = nn.ModuleList([
             DSALTTransformerBlock(d_model, n_heads, n_min, n_max, k_lmk, max_seq_len, d_ff, dropout, yarn_scale, i,
-                                  n_kv_heads, qkv_bias, rope_base, selection, block)
+                                  n_kv_heads, qkv_bias, rope_base, selection, block, qk_norm, ffn)
             for i in range(n_layers)])
         self.final_norm = RMSENorm(d_model)
         self.lm_head = nn.Linear(d_model, vocab_size, bias=False)

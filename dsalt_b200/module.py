@@ -32,6 +32,10 @@ soft window edge to ``win_gate`` and of the landmark weights to ``alpha_w``.
 holds. They need ``selection="block_causal"``, whose set for a position depends on earlier
 blocks only; the reference has no counterpart.
 
+``qk_norm=True`` norms each query and key head (RMS, a learnable weight per channel, ``q_norm`` and
+``k_norm``) before the rotation, both in the one pass of :func:`dsalt_b200.layers.qk_norm_rope`, in
+training, prompts and single tokens; the reference has no such norm.
+
 Out of scope (raise): the batched ``[B, T, d]`` path, and training with
 ``selection="block_causal"`` (the training kernel takes one landmark set per sequence, as
 the reference's does).
@@ -44,6 +48,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import layers
 from . import library  # noqa: F401  (registers torch.ops.dsalt_b200.*)
 from . import ops
 
@@ -84,9 +89,19 @@ def apply_rotary_emb(q, k, cos, sin):
     return q * cos + rot(q) * sin, k * cos + rot(k) * sin
 
 
+class HeadNorm(nn.Module):
+    """The weight of a head's RMS norm (applied by :func:`dsalt_b200.layers.qk_norm_rope`)."""
+
+    def __init__(self, head_dim: int, eps: float = 1e-6):
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(head_dim))
+
+
 class DSALTAttention(nn.Module):
     def __init__(self, d_model, n_heads, n_min, n_max, k_lmk, max_seq_len, dropout=0.0, yarn_scale=1.0,
-                 layer_idx=0, n_kv_heads=None, qkv_bias=False, rope_base=10000.0, selection="global", block=512):
+                 layer_idx=0, n_kv_heads=None, qkv_bias=False, rope_base=10000.0, selection="global", block=512,
+                 qk_norm=False):
         super().__init__()
         assert d_model % n_heads == 0
         if selection not in ("global", "block_causal"):
@@ -112,6 +127,9 @@ class DSALTAttention(nn.Module):
         self.out_proj = nn.Linear(d_model, d_model, bias=False)
         self.win_gate = nn.Linear(d_model, 1, bias=True)
         self.alpha_w = nn.Parameter(torch.full((n_heads,), math.log(0.6 / 0.4)))
+        self.qk_norm = qk_norm
+        if qk_norm:
+            self.q_norm, self.k_norm = HeadNorm(self.head_dim), HeadNorm(self.head_dim)
         self.tau_win, self.tau_lmk, self.win_edge = 1.0, 2.0, 4
         self._last_P = None
         self._collect_last_P = True  # the reference's default (dsalt_attention.py:639)
@@ -141,6 +159,12 @@ class DSALTAttention(nn.Module):
         q = self.q_proj(x).view(T, H, D)
         k = self.k_proj(x).view(T, Hkv, D)
         v = self.v_proj(x).view(T, Hkv, D)
+        if self.qk_norm:
+            if rope_cs is not None:
+                return *self._norm_rope(q, k, *rope_cs, None), v
+            pos = torch.cat([torch.arange(cu_h[i + 1] - cu_h[i], device=device, dtype=torch.int32)
+                             for i in range(len(cu_h) - 1)])
+            return *self._norm_rope(q, k, self.rope_cos.to(device), self.rope_sin.to(device), pos), v
         if rope_cs is None:
             pos = torch.cat([torch.arange(cu_h[i + 1] - cu_h[i], device=device) for i in range(len(cu_h) - 1)])
             cos, sin = self.rope_cos.to(device)[pos], self.rope_sin.to(device)[pos]
@@ -149,6 +173,14 @@ class DSALTAttention(nn.Module):
         cos, sin = cos.to(q.dtype), sin.to(q.dtype)
         q, k = apply_rotary_emb(q, k, cos.unsqueeze(1), sin.unsqueeze(1))
         return q, k, v
+
+    def _norm_rope(self, q, k, cos, sin, positions):
+        """Head norms and rotation, by the rows ``positions`` of the tables (``None``: row by row)."""
+        if torch.compiler.is_compiling():
+            return torch.ops.dsalt_b200.qk_norm_rope(q, k, cos, sin, positions, self.q_norm.weight, self.k_norm.weight,
+                                                     self.q_norm.eps)
+        return layers.qk_norm_rope(q, k, cos, sin, positions=positions, q_weight=self.q_norm.weight,
+                                   k_weight=self.k_norm.weight, eps=self.q_norm.eps)
 
     def _packed_train(self, x, cu_seqlens, total_len, device, rope_cs=None, cu_list=None):
         """Training forward (``_packed`` ``:596-605`` → ``_packed_train_triton`` ``:438-455``)."""
@@ -246,8 +278,11 @@ class DSALTAttention(nn.Module):
         q = self.q_proj(x).view(T, self.n_heads, self.head_dim)
         k = self.k_proj(x).view(T, self.n_kv_heads, self.head_dim)
         v = self.v_proj(x).view(T, self.n_kv_heads, self.head_dim)
-        cos, sin = (t.to(q.dtype).unsqueeze(1) for t in rope_cs)
-        q, k = apply_rotary_emb(q, k, cos, sin)
+        if self.qk_norm:
+            q, k = self._norm_rope(q, k, *rope_cs, None)
+        else:
+            cos, sin = (t.to(q.dtype).unsqueeze(1) for t in rope_cs)
+            q, k = apply_rotary_emb(q, k, cos, sin)
         w, xn, vn = self._signals(x, v)
         cache.append(self.layer_idx, k, v, w, xn, vn, plan)
         cache.update_landmarks(self.layer_idx, self._alpha().detach().float(), self.k_lmk, self.block)

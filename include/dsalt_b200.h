@@ -433,7 +433,8 @@ int dsalt_unpack8(const int8_t* codes, const uint8_t* exps, int64_t rows, int64_
  * cos, sin [table_rows, at least head_dim / 2] fp32 (row stride table_stride, 16-byte aligned rows);
  *   the angles of the first half's channels are read, the second half turns by the same. Token t
  *   takes row positions[t], or row t where positions is null. A position outside the tables is
- *   reported in the device status word (51) and taken as 0.
+ *   reported in the device status word (51) and taken as 0. At most 4096 heads, and 2^30 groups of up to
+ *   four heads (forward) or two (backward).
  * dsalt_qk_norm_rope_bwd: gradients of q, k (contiguous, of dtype) and of the weights (of w_dtype)
  *   from those of the outputs, dq_out and dk_out (token and head strides as above). Deterministic.
  */
@@ -464,8 +465,8 @@ int dsalt_qk_norm_rope_bwd(const void* q, const void* k, const void* dq_out, con
  * dsalt_gated_ffn_bwd: the gradients (contiguous, of dtype; null: not wanted, dw_gate and dw_up go
  *   together) from dy [T, d_out] (row stride dy_stride). With DSALT_KEEP_8BIT x holds the codes and
  *   x_exps the scales of dsalt_pack8 (contiguous), else x is the forward's. x may be null where dw_gate is.
- * 16-bit types whose sizes are multiples of 8 and whose rows are 16-byte aligned run on the tensor
- *   cores, everything else on the CUDA cores. Deterministic.
+ * 16-bit types whose sizes are multiples of 8 run on the tensor cores (operands and their rows 16-byte
+ *   aligned), everything else on the CUDA cores. Deterministic.
  */
 #define DSALT_ACT_SILU 0
 #define DSALT_ACT_GELU 1

@@ -166,6 +166,12 @@ def test_ffn_arguments_are_rejected(lib):
     assert fwd(x=None) == L.ERR_INVALID and fwd(y=None) == L.ERR_INVALID and fwd(ws=None) == L.ERR_INVALID
     assert fwd(keep=L.KEEP_INPUT) == L.ERR_INVALID and fwd(keep=L.KEEP_8BIT, kept=FAKE) == L.ERR_INVALID
     assert fwd(n=need - 1) == L.ERR_WORKSPACE
+    assert fwd(ws=ODD) == L.ERR_INVALID and fwd(keep=L.KEEP_INPUT, kept=ODD) == L.ERR_INVALID
+    assert fwd(x=ODD) == L.ERR_INVALID and fwd(y=ODD) == L.ERR_INVALID and b"aligned" in lib.dsalt_last_error()
+    assert fwd(stride=68) == L.ERR_INVALID and b"aligned" in lib.dsalt_last_error()
+    # what only the plain path takes needs more workspace
+    assert lib.dsalt_gated_ffn_workspace_bytes(L.BF16, 8, 64, 100, 64) > need
+    assert lib.dsalt_gated_ffn_workspace_bytes(L.F32, 8, 64, 96, 64) > need
     assert fwd(T=0, x=None, y=None, ws=None) == L.OK
 
     need_b = lib.dsalt_gated_ffn_bwd_workspace_bytes(L.BF16, 8, 64, 96, 64, L.KEEP_8BIT)
@@ -180,6 +186,7 @@ def test_ffn_arguments_are_rejected(lib):
     assert bwd(dwg=None) == L.ERR_INVALID and b"go together" in lib.dsalt_last_error()
     assert bwd(dy=None) == L.ERR_INVALID and bwd(x=None) == L.ERR_INVALID and bwd(x_exps=None) == L.ERR_INVALID
     assert bwd(kept=None) == L.ERR_INVALID and bwd(exps=None) == L.ERR_INVALID and bwd(ws=None) == L.ERR_INVALID
+    assert bwd(dy=ODD) == L.ERR_INVALID and bwd(dwg=ODD) == L.ERR_INVALID and bwd(stride=68) == L.ERR_INVALID
     assert bwd(stride=8) == L.ERR_INVALID and bwd(n=need_b - 1) == L.ERR_WORKSPACE and bwd(dt=4) == L.ERR_INVALID
 
 
@@ -197,3 +204,33 @@ def test_functions_refuse_cpu_tensors():
     q, k, t = torch.zeros(4, 2, 64), torch.zeros(4, 1, 64), torch.zeros(4, 64)
     with pytest.raises(RuntimeError, match="CUDA"):
         Y.qk_norm_rope(q, k, t, t)
+
+
+# ------------------------------------------------------------------ the decoder stack
+def test_config_and_modules_offer_the_kinds():
+    from dsalt_b200.model import DSALTConfig, DSALTLMHeadModel, SwiGLUFFN
+    small = dict(vocab_size=100, d_model=64, n_layers=1, n_heads=2, n_min=4, n_max=16, k_lmk=4, max_seq_len=64)
+    with pytest.raises(ValueError, match="ffn must be one of"):
+        DSALTConfig(**small, ffn="other")
+    with pytest.raises(ValueError, match="kind must be one of"):
+        SwiGLUFFN(64, 128, kind="8bit")
+    plain, new = (DSALTLMHeadModel.from_config(DSALTConfig(**small, **kw)) for kw in ({}, dict(qk_norm=True, ffn="fused")))
+    keys = set(new.state_dict())
+    assert keys - set(plain.state_dict()) == {"layers.0.attn.q_norm.weight", "layers.0.attn.k_norm.weight"}
+    assert set(plain.state_dict()) <= keys and new.layers[0].ffn.kind == "fused"
+    assert DSALTConfig.from_dict(DSALTConfig(**small, qk_norm=True, ffn="fused_8bit").to_dict()).ffn == "fused_8bit"
+
+
+def test_registered_forms_have_shape_functions():
+    import dsalt_b200  # noqa: F401
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        new = lambda *s, dt=torch.bfloat16: torch.empty(*s, dtype=dt, device="cuda")  # noqa: E731
+        q, k = torch.ops.dsalt_b200.qk_norm_rope(new(9, 4, 64), new(9, 2, 64), new(20, 64), new(20, 64),
+                                                 new(9, dt=torch.int32), new(64), new(64), 1e-6)
+        assert (q.shape, k.shape, q.dtype) == ((9, 4, 64), (9, 2, 64), torch.bfloat16)
+        y = torch.ops.dsalt_b200.gated_ffn(new(2, 9, 64), new(96, 64), new(96, 64), new(48, 96), "gelu")
+        assert y.shape == (2, 9, 48) and y.dtype == torch.bfloat16
+        codes, exps = torch.ops.dsalt_b200.pack8(new(5, 70))
+        assert (codes.shape, codes.dtype, exps.shape, exps.dtype) == ((5, 70), torch.int8, (5, 3), torch.uint8)
+        assert torch.ops.dsalt_b200.unpack8(codes, exps, torch.float16).dtype == torch.float16
