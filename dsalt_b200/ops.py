@@ -40,6 +40,8 @@ def _cuda(*ts):
 
 
 def _ptr(t):
+    """The address of a tensor that the caller holds until the launch: that of a temporary may be
+    given to the next temporary before the kernel has read it."""
     return None if t is None else t.data_ptr()
 
 
@@ -141,9 +143,9 @@ def select_landmarks(xnorm, vnorm, w, alpha, cu_seqlens, k_lmk: int, n_heads: in
         return (lmk, zx, zv) if return_z else lmk
     ws_n = L.query("dsalt_select_workspace_bytes", m, T, S, maxL, n_heads, n_kv, k_lmk, block)
     ws = _workspace(ws_n, dev)
-    a = alpha.float().contiguous()
-    L.call("dsalt_select_landmarks", m, _ptr(xnorm.contiguous()), _ptr(vnorm.contiguous()),
-           _ptr(w.to(torch.int32).contiguous()), _ptr(a), _ptr(_cu_i32(cu_seqlens)), S, T, maxL, n_heads, n_kv,
+    xnorm, vnorm, w, a, cu = (xnorm.contiguous(), vnorm.contiguous(), w.to(torch.int32).contiguous(),
+                              alpha.float().contiguous(), _cu_i32(cu_seqlens))
+    L.call("dsalt_select_landmarks", m, _ptr(xnorm), _ptr(vnorm), _ptr(w), _ptr(a), _ptr(cu), S, T, maxL, n_heads, n_kv,
            k_lmk, block, _ptr(lmk), _ptr(zx), _ptr(zv), _ptr(ws), ws.numel(), _stream())
     return (lmk, zx, zv) if return_z else lmk
 
@@ -233,9 +235,9 @@ def dsalt_attention(q, k, v, lmk_indices, lmk_bias, w_sizes, cu_seqlens, *, lmk_
     lse = torch.empty(T, H, dtype=torch.float32, device=q.device) if return_lse else None
     ws_n = L.query("dsalt_attention_workspace_bytes", T, S, H, kl, int(lmk_block))
     ws = _workspace(ws_n, q.device)
+    w, cu = w_sizes.to(torch.int32).contiguous(), _cu_i32(cu_seqlens)
     L.call("dsalt_attention_fwd", _ptr(qc), _ptr(kc), _ptr(vc), _dt(qc), T, H, n_kv, D, qc.stride(0), kc.stride(0),
-           _ptr(w_sizes.to(torch.int32).contiguous()), _ptr(lmk), _ptr(bias), kl, int(lmk_block),
-           _ptr(_cu_i32(cu_seqlens)), S, maxL, _ptr(out), _dt(out), _ptr(lse), _ptr(ws), ws.numel(), _stream())
+           _ptr(w), _ptr(lmk), _ptr(bias), kl, int(lmk_block), _ptr(cu), S, maxL, _ptr(out), _dt(out), _ptr(lse), _ptr(ws), ws.numel(), _stream())
     if out_dtype is None:
         out = out.float()
     return (out, lse) if return_lse else out
@@ -271,9 +273,10 @@ def dsalt_attention_backward(grad_out, q, k, v, out, lse, lmk_indices, lmk_bias,
     dv = torch.empty(T, n_kv, D, dtype=torch.float32, device=q.device)
     db = torch.empty(H, n_sets, kl, dtype=torch.float32, device=q.device)
     ws = _workspace(L.query("dsalt_attention_bwd_workspace_bytes", T, S), q.device)
+    lc, w, cu = lse.contiguous(), w_sizes.to(torch.int32).contiguous(), _cu_i32(cu_seqlens)
     L.call("dsalt_attention_bwd", _ptr(qc), _ptr(kc), _ptr(vc), _dt(qc), T, H, n_kv, D, qc.stride(0), kc.stride(0),
-           _ptr(oc), _dt(oc), _ptr(do), _dt(do), _ptr(lse.contiguous()), _ptr(w_sizes.to(torch.int32).contiguous()),
-           _ptr(lmk), _ptr(bias), kl, int(lmk_block), n_sets, _ptr(_cu_i32(cu_seqlens)), S, _ptr(dq), _ptr(dk),
+           _ptr(oc), _dt(oc), _ptr(do), _dt(do), _ptr(lc), _ptr(w), _ptr(lmk), _ptr(bias), kl, int(lmk_block), n_sets,
+           _ptr(cu), S, _ptr(dq), _ptr(dk),
            _ptr(dv), _ptr(db), _ptr(ws), ws.numel(), _stream())
     # back to the caller's slot order (normalize_landmarks sorted each set)
     raw = lmk_indices.to(torch.int32)
@@ -333,9 +336,10 @@ def train_attention_forward(q, k, v, lmk_pos, lmk_logw, w_cont, cu_seqlens, tau_
     out = torch.empty(T, H, D, dtype=out_dtype or q.dtype, device=q.device)
     lse = torch.empty(T, H, dtype=torch.float32, device=q.device)
     ws = _workspace(L.query("dsalt_train_attention_fwd_workspace_bytes", T, H, S, kl), q.device)
+    w, pos, logw, cu = (w_cont.float().contiguous(), lmk_pos.to(torch.int32).contiguous(), lmk_logw.float().contiguous(),
+                        _cu_i32(cu_seqlens))
     L.call("dsalt_train_attention_fwd", _ptr(qc), _ptr(kc), _ptr(vc), _dt(qc), T, H, n_kv, D, qc.stride(0),
-           kc.stride(0), _ptr(w_cont.float().contiguous()), _ptr(lmk_pos.to(torch.int32).contiguous()),
-           _ptr(lmk_logw.float().contiguous()), kl, _ptr(_cu_i32(cu_seqlens)), S, float(tau_win), float(win_edge),
+           kc.stride(0), _ptr(w), _ptr(pos), _ptr(logw), kl, _ptr(cu), S, float(tau_win), float(win_edge),
            _ptr(out), _dt(out), _ptr(lse), _ptr(ws), ws.numel(), _stream())
     return out, lse
 
@@ -360,10 +364,11 @@ def train_attention_backward(grad_out, q, k, v, out, lse, lmk_pos, lmk_logw, w_c
     dlw = torch.empty(H, S, kl, dtype=torch.float32, device=q.device)
     dw = torch.empty(T, dtype=torch.float32, device=q.device)
     ws = _workspace(L.query("dsalt_attention_bwd_workspace_bytes", T, S), q.device)
+    lc, w, pos, logw, cu = (lse.contiguous(), w_cont.float().contiguous(), lmk_pos.to(torch.int32).contiguous(),
+                            lmk_logw.float().contiguous(), _cu_i32(cu_seqlens))
     L.call("dsalt_train_attention_bwd", _ptr(qc), _ptr(kc), _ptr(vc), _dt(qc), T, H, n_kv, D, qc.stride(0),
-           kc.stride(0), _ptr(oc), _dt(oc), _ptr(do), _dt(do), _ptr(lse.contiguous()),
-           _ptr(w_cont.float().contiguous()), _ptr(lmk_pos.to(torch.int32).contiguous()),
-           _ptr(lmk_logw.float().contiguous()), kl, _ptr(_cu_i32(cu_seqlens)), S, float(tau_win), float(win_edge),
+           kc.stride(0), _ptr(oc), _dt(oc), _ptr(do), _dt(do), _ptr(lc), _ptr(w), _ptr(pos), _ptr(logw), kl, _ptr(cu), S,
+           float(tau_win), float(win_edge),
            _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dlw), _ptr(dw), _ptr(ws), ws.numel(), _stream())
     return dq, dk, dv, dlw, dw
 
@@ -431,10 +436,11 @@ def core_forward(x, gate_weight, gate_bias, n_min, n_max, alpha, q, k, v, k_lmk,
     need = L.query("dsalt_core_workspace_bytes", m, T, S, maxL, H, n_kv, D, k_lmk, block)
     ws = workspace if (workspace is not None and workspace.numel() >= need) else _workspace(need, dev)
     lin = _logit_in(logit, T, gw.dtype)
+    a, cu = alpha.float().contiguous(), _cu_i32(cu_seqlens)
     L.call("dsalt_core_forward", m, _ptr(x), _dt(x), x.shape[1], x.stride(0), _ptr(gw), _ptr(gb), _dt(gw), _ptr(lin),
-           int(n_min), int(n_max), _ptr(alpha.float().contiguous()), L.NORM_INPUT if norm_round else L.NORM_F32,
+           int(n_min), int(n_max), _ptr(a), L.NORM_INPUT if norm_round else L.NORM_F32,
            _ptr(q), _ptr(k), _ptr(v), _dt(q), H, n_kv, D, q.stride(0), k.stride(0), int(k_lmk), int(block),
-           _ptr(_cu_i32(cu_seqlens)), S, T, maxL, _ptr(out), _dt(out), _ptr(w), _ptr(lmk), _ptr(ws), ws.numel(),
+           _ptr(cu), S, T, maxL, _ptr(out), _dt(out), _ptr(w), _ptr(lmk), _ptr(ws), ws.numel(),
            _stream())
     if return_aux:
         return out, w, lmk
@@ -470,8 +476,9 @@ def select_block_range(xnorm, vnorm, w, alpha, k_lmk: int, n_heads: int, block: 
     out = torch.empty(n_heads, set_hi - set_lo, k_lmk, dtype=torch.int32, device=xnorm.device)
     n = L.query("dsalt_select_block_range_workspace_bytes", Lseq, n_heads, n_kv, k_lmk, block, set_hi)
     ws = workspace if workspace is not None and workspace.numel() >= n else _workspace(n, xnorm.device)
-    L.call("dsalt_select_block_range", _ptr(xnorm.contiguous()), _ptr(vnorm.contiguous()),
-           _ptr(w.to(torch.int32).contiguous()), _ptr(alpha.float().contiguous()), Lseq, n_heads, n_kv, k_lmk, block,
+    xnorm, vnorm, w, alpha = (xnorm.contiguous(), vnorm.contiguous(), w.to(torch.int32).contiguous(),
+                              alpha.float().contiguous())
+    L.call("dsalt_select_block_range", _ptr(xnorm), _ptr(vnorm), _ptr(w), _ptr(alpha), Lseq, n_heads, n_kv, k_lmk, block,
            set_lo, set_hi, _ptr(out), _ptr(ws), ws.numel(), _stream())
     return out
 
