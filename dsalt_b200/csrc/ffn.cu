@@ -85,14 +85,21 @@ __global__ void __launch_bounds__(THREADS) act_kernel(const float* __restrict__ 
     const bool in = at % pitch < F;
     const float a = in ? g[at] : 0.f, b = in ? u[at] : 0.f;
     h[at] = from_float<T>(activate<ACT, false>(a) * b);
-    if (keep == DSALT_KEEP_INPUT) {
-      static_cast<T*>(kept)[at] = from_float<T>(a);
-      static_cast<T*>(kept)[plane + at] = from_float<T>(b);
-    } else if (keep == DSALT_KEEP_8BIT) {
-      const uint32_t sa = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(a) & 0x7fffffffu));
-      const uint32_t sb = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(b) & 0x7fffffffu));
-      static_cast<int8_t*>(kept)[at] = (int8_t)code_of(a, sa);
-      static_cast<int8_t*>(kept)[plane + at] = (int8_t)code_of(b, sb);
+    if (sizeof(T) == 4 && keep == DSALT_KEEP_INPUT) {
+      static_cast<float*>(kept)[at] = a;
+      static_cast<float*>(kept)[plane + at] = b;
+    } else if (keep != DSALT_KEEP_NONE) {
+      const uint32_t top_a = __reduce_max_sync(0xffffffffu, __float_as_uint(a) & 0x7fffffffu);
+      const uint32_t top_b = __reduce_max_sync(0xffffffffu, __float_as_uint(b) & 0x7fffffffu);
+      const bool wide = keep == DSALT_KEEP_INPUT;
+      const uint32_t sa = wide ? scale_byte16(top_a) : scale_byte(top_a), sb = wide ? scale_byte16(top_b) : scale_byte(top_b);
+      if (wide) {
+        static_cast<uint16_t*>(kept)[at] = (uint16_t)code_bits16(a, inverse_scale(sa));
+        static_cast<uint16_t*>(kept)[plane + at] = (uint16_t)code_bits16(b, inverse_scale(sb));
+      } else {
+        static_cast<int8_t*>(kept)[at] = (int8_t)code_of(a, sa);
+        static_cast<int8_t*>(kept)[plane + at] = (int8_t)code_of(b, sb);
+      }
       if (lane == 0) {
         exps[i] = (uint8_t)sa;
         exps[total + i] = (uint8_t)sb;
@@ -109,13 +116,15 @@ __global__ void __launch_bounds__(THREADS) act_grad_kernel(const float* __restri
   const int64_t total = T_ * pitch;
   for (int64_t at = (int64_t)blockIdx.x * THREADS + threadIdx.x; at < total; at += (int64_t)gridDim.x * THREADS) {
     float a, b;
-    if (keep == DSALT_KEEP_8BIT) {
-      const int8_t* c = static_cast<const int8_t*>(kept);
-      a = (float)c[at] * scale_of(exps[at / GROUP8]);
-      b = (float)c[total + at] * scale_of(exps[(total + at) / GROUP8]);
+    if (sizeof(T) == 4 && keep == DSALT_KEEP_INPUT) {
+      a = static_cast<const float*>(kept)[at];
+      b = static_cast<const float*>(kept)[total + at];
     } else {
-      a = to_float(static_cast<const T*>(kept)[at]);
-      b = to_float(static_cast<const T*>(kept)[total + at]);
+      const int8_t* c = static_cast<const int8_t*>(kept);
+      const int16_t* w = static_cast<const int16_t*>(kept);
+      const bool wide = keep == DSALT_KEEP_INPUT;
+      a = (float)(wide ? w[at] : c[at]) * scale_of(exps[at / GROUP8]);
+      b = (float)(wide ? w[total + at] : c[total + at]) * scale_of(exps[(total + at) / GROUP8]);
     }
     const float d = at % pitch < F ? dh[at] : 0.f;
     float v, dv;
@@ -205,6 +214,8 @@ int run(const Ffn& f, bool backward) {
 
 size_t a256(size_t v) { return (v + 255) & ~(size_t)255; }
 size_t elem_bytes(int dtype) { return dtype == DSALT_F32 ? 4 : 2; }
+// whether what is kept of gate and up are codes with scales
+bool scaled(int dtype, int keep) { return keep == DSALT_KEEP_8BIT || (keep == DSALT_KEEP_INPUT && dtype != DSALT_F32); }
 // what the tensor cores take; their operands' rows have to be 16-byte aligned
 bool tensor_cores(int dtype, int d, int F, int d_out) { return dtype != DSALT_F32 && d % 8 == 0 && F % 8 == 0 && d_out % 8 == 0; }
 int check_rows(const char* fn, const Ffn& f) {
@@ -253,7 +264,7 @@ int dsalt_gated_ffn(const void* x, int dtype, int64_t T, int d_model, int64_t x_
   if (int rc = check(FN, dtype, T, d_model, d_ff, d_out, activation, keep)) return rc;
   if (T == 0) return DSALT_OK;
   if (T > 1 && x_stride < d_model) return fail(DSALT_ERR_INVALID, "%s: rows overlap", FN);
-  if (!x || !w_gate || !w_up || !w_down || !y || !workspace || (keep && !kept) || (keep == DSALT_KEEP_8BIT && !kept_exps))
+  if (!x || !w_gate || !w_up || !w_down || !y || !workspace || (keep && !kept) || (scaled(dtype, keep) && !kept_exps))
     return fail(DSALT_ERR_INVALID, "%s: null pointer", FN);
   if (off256(kept) || off256(workspace)) return fail(DSALT_ERR_INVALID, "%s: kept and workspace must be 256-byte aligned", FN);
   if (workspace_bytes < dsalt_gated_ffn_workspace_bytes(dtype, T, d_model, d_ff, d_out))
@@ -300,7 +311,7 @@ int dsalt_gated_ffn_bwd(const void* dy, int dtype, int64_t T, int d_model, int64
   }
   const bool coded = keep == DSALT_KEEP_8BIT;
   if (T > 1 && (dy_stride < d_out || (!coded && x_stride < d_model))) return fail(DSALT_ERR_INVALID, "%s: rows overlap", FN);
-  if (!dy || (dw_gate && (!x || (coded && !x_exps))) || !w_gate || !w_up || !w_down || !kept || (coded && !kept_exps) || !workspace)
+  if (!dy || (dw_gate && (!x || (coded && !x_exps))) || !w_gate || !w_up || !w_down || !kept || (scaled(dtype, keep) && !kept_exps) || !workspace)
     return fail(DSALT_ERR_INVALID, "%s: null pointer", FN);
   if (off256(kept) || off256(workspace)) return fail(DSALT_ERR_INVALID, "%s: kept and workspace must be 256-byte aligned", FN);
   if (workspace_bytes < dsalt_gated_ffn_bwd_workspace_bytes(dtype, T, d_model, d_ff, d_out, keep))

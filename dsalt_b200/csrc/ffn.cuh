@@ -50,8 +50,8 @@ struct Ffn {
   const void* w_down;
   const void* x;
   int64_t x_stride;
-  void* kept;       // gate's, up's and h [3, T, pitch] in the input type, or gate's and up's codes [2, T, pitch]
-  uint8_t* exps;    // [2, T, pitch / 32]
+  void* kept;       // gate's and up's [2, T, pitch], as fp32 or as codes of 16 bits with h behind them, or codes of 8
+  uint8_t* exps;    // [2, T, pitch / 32] of codes
   // forward
   void* y;
   void* h;          // [T, pitch]

@@ -170,25 +170,37 @@ __device__ __forceinline__ void store_32b(void* p, const uint32_t (&w)[8]) {
                "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
 }
-// a group of 32 columns of a row: its scale byte and its codes
-__device__ __forceinline__ uint32_t form_codes(const float (&f)[GROUP8], uint32_t (&w)[8]) {
+// a group of 32 columns of a row: its scale byte and its codes of 8 or 16 bits
+template <int WORDS>
+__device__ __forceinline__ uint32_t form_codes(const float (&f)[GROUP8], uint32_t (&w)[WORDS]) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < GROUP8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-  const uint32_t s = scale_byte(top);
-  pack_codes<GROUP8>(f, s, w);
+  const uint32_t s = WORDS == 8 ? scale_byte(top) : scale_byte16(top);
+  if constexpr (WORDS == 8) pack_codes<GROUP8>(f, s, w);
+  else pack_codes16<GROUP8>(f, s, w);
   return s;
+}
+template <int WORDS>
+__device__ __forceinline__ void store_codes(void* p, const uint32_t (&w)[WORDS]) {
+#pragma unroll
+  for (int i = 0; i < WORDS; i += 8) {
+    uint32_t part[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) part[j] = w[i + j];
+    store_32b(static_cast<char*>(p) + 4 * i, part);
+  }
 }
 
 // what the backward's first epilogue reads: 32 columns of a row of gate and up
-template <typename T, int KEEP>
+template <int KEEP>
 struct KeptRow {
   static constexpr int WORDS = KEEP == DSALT_KEEP_8BIT ? 8 : 16;
   uint32_t g[WORDS], u[WORDS];
   uint32_t sg, su;
   __device__ __forceinline__ void load(const Kept& k, int64_t row, int64_t col) {
     const int64_t plane = k.T * k.pitch, at = row * k.pitch + col;
-    constexpr int ES = KEEP == DSALT_KEEP_8BIT ? 1 : (int)sizeof(T);
+    constexpr int ES = KEEP == DSALT_KEEP_8BIT ? 1 : 2;
     sg = su = 127;
 #pragma unroll
     for (int i = 0; i < WORDS; ++i) g[i] = u[i] = 0;
@@ -202,26 +214,21 @@ struct KeptRow {
 #pragma unroll
         for (int j = 0; j < 8; ++j) g[8 * i + j] = a[j], u[8 * i + j] = b[j];
       }
-      if constexpr (KEEP == DSALT_KEEP_8BIT) {
-        sg = __ldg(k.exps + at / GROUP8);
-        su = __ldg(k.exps + (plane + at) / GROUP8);
-      }
+      sg = __ldg(k.exps + at / GROUP8);
+      su = __ldg(k.exps + (plane + at) / GROUP8);
     }
   }
   // values 16 half .. 16 half + 15
   __device__ __forceinline__ void values(int half, float (&a)[16], float (&b)[16]) const {
-    if constexpr (KEEP == DSALT_KEEP_8BIT) {
-      uint32_t x[4], y[4];
+    uint32_t x[WORDS / 2], y[WORDS / 2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = g[4 * half + i], y[i] = u[4 * half + i];
+    for (int i = 0; i < WORDS / 2; ++i) x[i] = g[WORDS / 2 * half + i], y[i] = u[WORDS / 2 * half + i];
+    if constexpr (KEEP == DSALT_KEEP_8BIT) {
       unpack_codes<16>(x, scale_of(sg), a);
       unpack_codes<16>(y, scale_of(su), b);
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        widen2<T>(g[8 * half + i], a[2 * i], a[2 * i + 1]);
-        widen2<T>(u[8 * half + i], b[2 * i], b[2 * i + 1]);
-      }
+      unpack_codes16<16>(x, scale_of(sg), a);
+      unpack_codes16<16>(y, scale_of(su), b);
     }
   }
 };
@@ -374,7 +381,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if constexpr (EPI == GRADS) {
         const int col0 = tile.n * PAIR_N + side * S::COLS;
         const int64_t row = row0 + lane;
-        KeptRow<T, KEEP> kept;
+        KeptRow<KEEP> kept;
         kept.load(args.kept, row, col0);
         if (!mbar_wait(&bars.acc_full[acc], (it >> 1) & 1, args.err, 64)) break;
         tc_fence_after();
@@ -384,7 +391,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int c = 0; c < S::COLS; c += 32) {
           float d[32];
           take_acc<32>(r, d);
-          const KeptRow<T, KEEP> now = kept;
+          const KeptRow<KEEP> now = kept;
           if (c + 32 < S::COLS) {
             kept.load(args.kept, row, col0 + c + 32);
             ask_acc<32>(mine + c + 32, r);
@@ -415,7 +422,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tc_fence_after();
         const int col = tile.n * (PAIR_N / 2) + side * 64;
         const int64_t row = row0 + lane, at = row * args.kept.pitch + col, plane = args.kept.T * args.kept.pitch;
-        uint32_t rg[32], ru[32], cg[2][8], cu[2][8], sg[2], su[2];
+        uint32_t rg[32], ru[32];
         ask_acc<32>(mine, rg);
         ask_acc<32>(mine + PAIR_N / 2, ru);
 #pragma unroll
@@ -428,30 +435,24 @@ __global__ void __launch_bounds__(THREADS, 1)
             ask_acc<32>(mine + PAIR_N / 2 + 32, ru);
           }
           const bool in = row < args.kept.T && col + 32 * half < args.kept.pitch;
-          if constexpr (KEEP == DSALT_KEEP_INPUT) {
+          if constexpr (KEEP != DSALT_KEEP_NONE) {
+            constexpr int WORDS = KEEP == DSALT_KEEP_8BIT ? 8 : 16;
+            uint32_t c[WORDS];
+            char* codes = static_cast<char*>(args.kept.p) + (at + 32 * half) * (WORDS / 8);
+            uint32_t s = form_codes(g, c);
             if (in) {
-              store_row<T, 32>(static_cast<T*>(args.kept.p) + at + 32 * half, g);
-              store_row<T, 32>(static_cast<T*>(args.kept.p) + plane + at + 32 * half, u);
+              store_codes(codes, c);
+              args.kept.exps[at / GROUP8 + half] = (uint8_t)s;
             }
-          }
-          if constexpr (KEEP == DSALT_KEEP_8BIT) {
-            sg[half] = form_codes(g, cg[half]);
-            su[half] = form_codes(u, cu[half]);
+            s = form_codes(u, c);
+            if (in) {
+              store_codes(codes + plane * (WORDS / 8), c);
+              args.kept.exps[(plane + at) / GROUP8 + half] = (uint8_t)s;
+            }
           }
 #pragma unroll
           for (int i = 0; i < 32; ++i) g[i] = activate<ACT, true>(g[i]) * u[i];
           if (in) store_row<T, 32>(static_cast<T*>(args.kept.h) + at + 32 * half, g);
-        }
-        if constexpr (KEEP == DSALT_KEEP_8BIT) {
-          int8_t* codes = static_cast<int8_t*>(args.kept.p);
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-            if (row < args.kept.T && col + 32 * half < args.kept.pitch) {
-              store_32b(codes + at + half * 32, cg[half]);
-              store_32b(codes + plane + at + half * 32, cu[half]);
-              args.kept.exps[at / GROUP8 + half] = (uint8_t)sg[half];
-              args.kept.exps[(plane + at) / GROUP8 + half] = (uint8_t)su[half];
-            }
         }
       } else {
         if (!mbar_wait(&bars.acc_full[acc], (it >> 1) & 1, args.err, 64)) break;

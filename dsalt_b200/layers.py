@@ -270,7 +270,7 @@ def _ffn_forward(x2, stride, w_gate, w_up, w_down, sizes, act, keep):
         pitch = _ffn_pitch(F)
         coded = keep == L.KEEP_8BIT
         kept = torch.empty(2 if coded else 3, T, pitch, dtype=torch.int8 if coded else x2.dtype, device=dev)
-        if coded:
+        if coded or x2.dtype is not torch.float32:
             exps = torch.empty(2, T, pitch // GROUP, dtype=torch.uint8, device=dev)
     ws = torch.empty(_ffn_workspace(dt, T, d, F, d_out, 0), dtype=torch.uint8, device=dev)
     _run(dev, "dsalt_gated_ffn", x2.data_ptr(), dt, T, d, stride, w_gate.data_ptr(), w_up.data_ptr(),
@@ -280,8 +280,9 @@ def _ffn_forward(x2, stride, w_gate, w_up, w_down, sizes, act, keep):
 
 class GatedFFNFunction(torch.autograd.Function):
     """Autograd of :func:`gated_ffn`. Kept for the backward pass: ``x Wgᵀ`` and ``x Wuᵀ`` (written by
-    the epilogue that forms them) and ``x``, in the input's dtype or in 8 bits. In the input's dtype the rows
-    that the last product read are kept too; in 8 bits they are formed again."""
+    the epilogue that forms them) and ``x``, the first two in 16 bits with a scale for 32 (of fp32 inputs in
+    fp32), or all three in 8 bits. With 16 bits the rows that the last product read are kept too; with 8 they
+    are formed again."""
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, activation, keep):
@@ -334,9 +335,9 @@ def gated_ffn(x, w_gate, w_up, w_down, *, activation: str = "silu", keep: str = 
     dtype once, as the operand of the last product.
 
     ``activation`` is ``"silu"`` or ``"gelu"`` (by the error function). Differentiable in all four;
-    ``keep`` says in what form the backward pass finds ``x``, ``x Wgᵀ`` and ``x Wuᵀ``: ``"16bit"``, the input's
-    dtype (fp32 inputs: fp32), or ``"8bit"``, as :func:`pack8` holds them (half the memory; the gradients
-    are then those at the held values). bf16 and fp16 run on the tensor cores where sizes are
+    ``keep`` says in what form the backward pass finds ``x``, ``x Wgᵀ`` and ``x Wuᵀ``: ``"16bit"``, ``x`` as it is
+    and the others in 16 bits with a scale for 32 values (fp32 inputs: fp32), or ``"8bit"``, as
+    :func:`pack8` holds them (a third of the memory; the gradients are then those at the held values). bf16 and fp16 run on the tensor cores where sizes are
     multiples of 8; fp32 and other sizes on the CUDA cores. Under autocast all four are cast first, as
     a linear layer's are."""
     x, w_gate, w_up, w_down = autocast_all(x, w_gate, w_up, w_down)

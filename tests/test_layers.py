@@ -165,8 +165,9 @@ def test_ffn_arguments_are_rejected(lib):
     assert fwd(stride=56) == L.ERR_INVALID and b"overlap" in lib.dsalt_last_error()
     assert fwd(x=None) == L.ERR_INVALID and fwd(y=None) == L.ERR_INVALID and fwd(ws=None) == L.ERR_INVALID
     assert fwd(keep=L.KEEP_INPUT) == L.ERR_INVALID and fwd(keep=L.KEEP_8BIT, kept=FAKE) == L.ERR_INVALID
+    assert fwd(keep=L.KEEP_INPUT, kept=FAKE) == L.ERR_INVALID  # codes of 16 bits have scales
     assert fwd(n=need - 1) == L.ERR_WORKSPACE
-    assert fwd(ws=ODD) == L.ERR_INVALID and fwd(keep=L.KEEP_INPUT, kept=ODD) == L.ERR_INVALID
+    assert fwd(ws=ODD) == L.ERR_INVALID and fwd(keep=L.KEEP_INPUT, kept=ODD, exps=FAKE) == L.ERR_INVALID
     assert fwd(x=ODD) == L.ERR_INVALID and fwd(y=ODD) == L.ERR_INVALID and b"aligned" in lib.dsalt_last_error()
     assert fwd(stride=68) == L.ERR_INVALID and b"aligned" in lib.dsalt_last_error()
     # what only the plain path takes needs more workspace
