@@ -101,8 +101,8 @@ __global__ void __launch_bounds__(THREADS) act_kernel(const float* __restrict__ 
         static_cast<int8_t*>(kept)[plane + at] = (int8_t)code_of(b, sb);
       }
       if (lane == 0) {
-        exps[i] = (uint8_t)sa;
-        exps[total + i] = (uint8_t)sb;
+        exps[i % groups * T_ + i / groups] = (uint8_t)sa;
+        exps[(groups + i % groups) * T_ + i / groups] = (uint8_t)sb;
       }
     }
   }
@@ -123,8 +123,9 @@ __global__ void __launch_bounds__(THREADS) act_grad_kernel(const float* __restri
       const int8_t* c = static_cast<const int8_t*>(kept);
       const int16_t* w = static_cast<const int16_t*>(kept);
       const bool wide = keep == DSALT_KEEP_INPUT;
-      a = (float)(wide ? w[at] : c[at]) * scale_of(exps[at / GROUP8]);
-      b = (float)(wide ? w[total + at] : c[total + at]) * scale_of(exps[(total + at) / GROUP8]);
+      const int64_t scale = at % pitch / GROUP8 * T_ + at / pitch;
+      a = (float)(wide ? w[at] : c[at]) * scale_of(exps[scale]);
+      b = (float)(wide ? w[total + at] : c[total + at]) * scale_of(exps[pitch / GROUP8 * T_ + scale]);
     }
     const float d = at % pitch < F ? dh[at] : 0.f;
     float v, dv;

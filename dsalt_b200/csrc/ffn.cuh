@@ -51,7 +51,7 @@ struct Ffn {
   const void* x;
   int64_t x_stride;
   void* kept;       // gate's and up's [2, T, pitch], as fp32 or as codes of 16 bits with h behind them, or codes of 8
-  uint8_t* exps;    // [2, T, pitch / 32] of codes
+  uint8_t* exps;    // [2, pitch / 32, T] of codes
   // forward
   void* y;
   void* h;          // [T, pitch]

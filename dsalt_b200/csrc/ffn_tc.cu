@@ -28,7 +28,7 @@ namespace {
 constexpr int PAIR_M = 256, CTA_M = 128, PAIR_N = 256, KB = 64;
 constexpr int OPERAND_BYTES = CTA_M * KB * 2, STAGE_BYTES = 2 * OPERAND_BYTES;
 constexpr int BOX = 32, BOX_BYTES = 32 * BOX * 2;  // a warp's staged outputs: 32 rows of 32 columns
-constexpr int EPI_WARPS = 8, THREADS = 32 * (4 + EPI_WARPS);
+constexpr int EPI_WARPS = 8, THREADS = 32 * (4 + EPI_WARPS);  // 16 warps in the first epilogue: no faster
 constexpr uint32_t TMEM_COLS = 512;
 constexpr int GROUP_M = 8;  // tiles of 256 rows whose A stays in L2 while N is walked
 
@@ -43,7 +43,7 @@ struct alignas(64) Job {
 };
 struct Kept {
   void* p;           // gate's and up's [2, T, pitch]
-  uint8_t* exps;
+  uint8_t* exps;     // their scales [2, pitch / 32, T]: the lanes of a warp, rows of a tile, find theirs side by side
   void* h;           // [T, pitch]
   int64_t T, pitch;
 };
@@ -170,12 +170,21 @@ __device__ __forceinline__ void store_32b(void* p, const uint32_t (&w)[8]) {
                "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
 }
+// bits of the largest magnitude of 32, NaN if there is one
+__device__ __forceinline__ uint32_t largest_of(const float (&f)[GROUP8]) {
+  float top[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top[i] = fabsf(f[i]);
+#pragma unroll
+  for (int i = 4; i < GROUP8; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top[i % 4]) : "f"(fabsf(f[i])));
+#pragma unroll
+  for (int i = 1; i < 4; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top[0]) : "f"(top[i]));
+  return __float_as_uint(top[0]) & 0x7fffffffu;
+}
 // a group of 32 columns of a row: its scale byte and its codes of 8 or 16 bits
 template <int WORDS>
 __device__ __forceinline__ uint32_t form_codes(const float (&f)[GROUP8], uint32_t (&w)[WORDS]) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < GROUP8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+  const uint32_t top = largest_of(f);
   const uint32_t s = WORDS == 8 ? scale_byte(top) : scale_byte16(top);
   if constexpr (WORDS == 8) pack_codes<GROUP8>(f, s, w);
   else pack_codes16<GROUP8>(f, s, w);
@@ -214,8 +223,8 @@ struct KeptRow {
 #pragma unroll
         for (int j = 0; j < 8; ++j) g[8 * i + j] = a[j], u[8 * i + j] = b[j];
       }
-      sg = __ldg(k.exps + at / GROUP8);
-      su = __ldg(k.exps + (plane + at) / GROUP8);
+      sg = __ldg(k.exps + col / GROUP8 * k.T + row);
+      su = __ldg(k.exps + (k.pitch + col) / GROUP8 * k.T + row);
     }
   }
   // values 16 half .. 16 half + 15
@@ -417,20 +426,19 @@ __global__ void __launch_bounds__(THREADS, 1)
           send(to, col0 + c);
         }
       } else if constexpr (EPI == GATE_UP) {
-        static_assert(S::COLS == 64, "a warp takes two groups of 32 columns");
         if (!mbar_wait(&bars.acc_full[acc], (it >> 1) & 1, args.err, 64)) break;
         tc_fence_after();
-        const int col = tile.n * (PAIR_N / 2) + side * 64;
+        const int col = tile.n * (PAIR_N / 2) + side * S::COLS;
         const int64_t row = row0 + lane, at = row * args.kept.pitch + col, plane = args.kept.T * args.kept.pitch;
         uint32_t rg[32], ru[32];
         ask_acc<32>(mine, rg);
         ask_acc<32>(mine + PAIR_N / 2, ru);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+        for (int half = 0; half < S::COLS / 32; ++half) {
           float g[32], u[32];
           take_acc<32>(rg, g);
           take_acc<32>(ru, u);
-          if (half == 0) {
+          if (half + 1 < S::COLS / 32) {
             ask_acc<32>(mine + 32, rg);
             ask_acc<32>(mine + PAIR_N / 2 + 32, ru);
           }
@@ -442,12 +450,12 @@ __global__ void __launch_bounds__(THREADS, 1)
             uint32_t s = form_codes(g, c);
             if (in) {
               store_codes(codes, c);
-              args.kept.exps[at / GROUP8 + half] = (uint8_t)s;
+              args.kept.exps[(col / GROUP8 + half) * args.kept.T + row] = (uint8_t)s;
             }
             s = form_codes(u, c);
             if (in) {
               store_codes(codes + plane * (WORDS / 8), c);
-              args.kept.exps[(plane + at) / GROUP8 + half] = (uint8_t)s;
+              args.kept.exps[((args.kept.pitch + col) / GROUP8 + half) * args.kept.T + row] = (uint8_t)s;
             }
           }
 #pragma unroll

@@ -271,7 +271,7 @@ def _ffn_forward(x2, stride, w_gate, w_up, w_down, sizes, act, keep):
         coded = keep == L.KEEP_8BIT
         kept = torch.empty(2 if coded else 3, T, pitch, dtype=torch.int8 if coded else x2.dtype, device=dev)
         if coded or x2.dtype is not torch.float32:
-            exps = torch.empty(2, T, pitch // GROUP, dtype=torch.uint8, device=dev)
+            exps = torch.empty(2, pitch // GROUP, T, dtype=torch.uint8, device=dev)
     ws = torch.empty(_ffn_workspace(dt, T, d, F, d_out, 0), dtype=torch.uint8, device=dev)
     _run(dev, "dsalt_gated_ffn", x2.data_ptr(), dt, T, d, stride, w_gate.data_ptr(), w_up.data_ptr(),
          w_down.data_ptr(), F, d_out, act, keep, _ptr(kept), _ptr(exps), y.data_ptr(), ws.data_ptr(), ws.numel())
