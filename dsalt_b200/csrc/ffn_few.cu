@@ -34,13 +34,6 @@ struct FewBars {
   uint32_t tmem;
 };
 
-__device__ __forceinline__ void load_2d(uint32_t dst, const void* map, uint64_t* bar, int c0, int c1) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
-          dst),
-      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
-      : "memory");
-}
 __device__ __forceinline__ float2 load_peer2(uint32_t addr) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
@@ -85,11 +78,11 @@ __global__ void __launch_bounds__(THREADS) ffn_few_kernel(const __grid_constant_
     auto weights = [&](int i, int s) {
       const uint32_t at = base + s * stage_bytes;
       mbar_arrive_expect_tx(&bars.full[s], stage_bytes);
-      load_2d(at, &a.w[0], &bars.full[s], (lo + i) * KB, f0);
-      load_2d(at + w_bytes / 2, &a.w[1], &bars.full[s], (lo + i) * KB, GATED ? f0 : f0 + a.box);
+      load_own_2d(at, &a.w[0], &bars.full[s], (lo + i) * KB, f0);
+      load_own_2d(at + w_bytes / 2, &a.w[1], &bars.full[s], (lo + i) * KB, GATED ? f0 : f0 + a.box);
     };
     auto tokens = [&](int i, int s) {
-      load_2d(base + s * stage_bytes + w_bytes, &a.x, &bars.full[s], (lo + i) * KB, t0);
+      load_own_2d(base + s * stage_bytes + w_bytes, &a.x, &bars.full[s], (lo + i) * KB, t0);
     };
     const int first = min(n, a.stages);
     for (int i = 0; i < first; ++i) weights(i, i);

@@ -30,7 +30,7 @@ constexpr int OPERAND_BYTES = CTA_M * KB * 2, STAGE_BYTES = 2 * OPERAND_BYTES;
 constexpr int BOX = 32, BOX_BYTES = 32 * BOX * 2;  // a warp's staged outputs: 32 rows of 32 columns
 constexpr int EPI_WARPS = 8, THREADS = 32 * (4 + EPI_WARPS);  // 16 warps in the first epilogue: no faster
 constexpr uint32_t TMEM_COLS = 512;
-constexpr int GROUP_M = 8;  // tiles of 256 rows whose A stays in L2 while N is walked
+constexpr int GROUP_M = 4;  // tiles of 256 rows whose A stays in L2 while N is walked; 1 to 16 differ by 2 %
 
 enum Epilogue { PLAIN = 0, GATE_UP = 1, GRADS = 2 };
 
@@ -50,6 +50,7 @@ struct Kept {
 template <int NJ>
 struct Args {
   Job job[NJ];
+  CUtensorMap kept_map[2];  // gate's and up's, where they are read
   Kept kept;
   int tiles, split;  // split > 1: a cluster of so many pairs shares a tile, each takes a part of K
   uint32_t idesc;
@@ -97,22 +98,26 @@ __device__ __forceinline__ void pair_commit(uint64_t* bar, uint32_t leader) {
 }
 
 // ---------------------------------------------------------------- shared memory
-// The outputs that an epilogue stages for the store engine, in how many sets of boxes, and what that
-// leaves for the operands. The first product's epilogue writes its rows from registers instead: at three
-// outputs of 128 columns that measured 177 us against 183 (32768 x 768 -> 2048), but the backward's, which
-// also reads rows, 192 us against 173.
+// What an epilogue keeps in shared memory, and the stages that this leaves for the operands. The first
+// product's writes its rows from registers. A plain store stages its output for the store engine, in four
+// sets of boxes. The backward's has what was kept brought in by the load engine, a warp's 32 rows x 32
+// columns of gate and of up at a time, three of them under way (read row by row by the threads it took
+// 165 us at 32768 x 768 -> 2048, 148 so); codes of 16 bits are replaced by
+// the gradients where they lie, codes of 8 have a set of boxes for three outputs besides.
 template <int EPI, int KEEP>
 struct Shape {
-  static constexpr int OUTPUTS = EPI == GATE_UP ? 0 : EPI == PLAIN ? 1 : KEEP == DSALT_KEEP_8BIT ? 3 : 2;
-  static constexpr int SETS = OUTPUTS == 1 ? 4 : 2, STAGES = OUTPUTS == 0 ? 6 : OUTPUTS == 3 ? 4 : 5;
-  static constexpr int SET_BYTES = OUTPUTS * BOX_BYTES, WARP_BYTES = SETS * SET_BYTES;
-  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + EPI_WARPS * WARP_BYTES + 256;
+  static constexpr bool IN_PLACE = EPI == GRADS && KEEP == DSALT_KEEP_INPUT;
+  static constexpr int OUTPUTS = EPI == GATE_UP ? 0 : EPI == PLAIN ? 1 : IN_PLACE ? 2 : 3;
+  static constexpr int SETS = EPI == PLAIN ? 4 : IN_PLACE ? 0 : 1, STAGES = EPI == GATE_UP ? 6 : EPI == GRADS ? 4 : 5;
+  static constexpr int KEPT_SETS = EPI == GRADS ? 3 : 0, KEPT_BOX = BOX * BOX * (KEEP == DSALT_KEEP_8BIT ? 1 : 2);
+  static constexpr int SET_BYTES = OUTPUTS * BOX_BYTES, WARP_BYTES = SETS * SET_BYTES + KEPT_SETS * 2 * KEPT_BOX;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + EPI_WARPS * WARP_BYTES + 512;
   // columns of the accumulator that a warp works on (of the first product: as many of gate and of up)
   static constexpr int COLS = (EPI == GATE_UP ? PAIR_N / 2 : PAIR_N) / (EPI_WARPS / 4);
 };
 template <int STAGES>
 struct Bars {
-  uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
+  uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], kept_full[EPI_WARPS][3];
   uint32_t tmem;
 };
 
@@ -160,11 +165,6 @@ __device__ __forceinline__ void store_row(T* p, const float (&f)[N]) {
                  "r"(narrow2<T>(f[16 * c + 12], f[16 * c + 13])), "r"(narrow2<T>(f[16 * c + 14], f[16 * c + 15]))
                  : "memory");
 }
-__device__ __forceinline__ void load_32b(uint32_t (&u)[8], const void* p) {
-  asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
-               : "l"(__cvta_generic_to_global(p)));
-}
 __device__ __forceinline__ void store_32b(void* p, const uint32_t (&w)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(__cvta_generic_to_global(p)), "r"(w[0]), "r"(w[1]),
                "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
@@ -201,46 +201,28 @@ __device__ __forceinline__ void store_codes(void* p, const uint32_t (&w)[WORDS])
   }
 }
 
-// what the backward's first epilogue reads: 32 columns of a row of gate and up
+__device__ __forceinline__ uint4 load_shared(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+// values 16 half .. 16 half + 15 of a row of a box of codes, as the load engine wrote it
 template <int KEEP>
-struct KeptRow {
-  static constexpr int WORDS = KEEP == DSALT_KEEP_8BIT ? 8 : 16;
-  uint32_t g[WORDS], u[WORDS];
-  uint32_t sg, su;
-  __device__ __forceinline__ void load(const Kept& k, int64_t row, int64_t col) {
-    const int64_t plane = k.T * k.pitch, at = row * k.pitch + col;
-    constexpr int ES = KEEP == DSALT_KEEP_8BIT ? 1 : 2;
-    sg = su = 127;
+__device__ __forceinline__ void kept_values(uint32_t box, int lane, int half, float scale, float (&f)[16]) {
+  if constexpr (KEEP == DSALT_KEEP_8BIT) {
+    const uint4 v = load_shared(box + lane * 32 + half * 16);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    unpack_codes<16>(w, scale, f);
+  } else {
+    uint32_t w[8];
 #pragma unroll
-    for (int i = 0; i < WORDS; ++i) g[i] = u[i] = 0;
-    if (row < k.T && col < k.pitch) {
-      const char* p = static_cast<const char*>(k.p) + at * ES;
-#pragma unroll
-      for (int i = 0; i < WORDS / 8; ++i) {
-        uint32_t a[8], b[8];
-        load_32b(a, p + 32 * i);
-        load_32b(b, p + plane * ES + 32 * i);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) g[8 * i + j] = a[j], u[8 * i + j] = b[j];
-      }
-      sg = __ldg(k.exps + col / GROUP8 * k.T + row);
-      su = __ldg(k.exps + (k.pitch + col) / GROUP8 * k.T + row);
+    for (int i = 0; i < 2; ++i) {
+      const uint4 v = load_shared(box + lane * 64 + (((2 * half + i) ^ ((lane >> 1) & 3)) << 4));
+      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
     }
+    unpack_codes16<16>(w, scale, f);
   }
-  // values 16 half .. 16 half + 15
-  __device__ __forceinline__ void values(int half, float (&a)[16], float (&b)[16]) const {
-    uint32_t x[WORDS / 2], y[WORDS / 2];
-#pragma unroll
-    for (int i = 0; i < WORDS / 2; ++i) x[i] = g[WORDS / 2 * half + i], y[i] = u[WORDS / 2 * half + i];
-    if constexpr (KEEP == DSALT_KEEP_8BIT) {
-      unpack_codes<16>(x, scale_of(sg), a);
-      unpack_codes<16>(y, scale_of(su), b);
-    } else {
-      unpack_codes16<16>(x, scale_of(sg), a);
-      unpack_codes16<16>(y, scale_of(su), b);
-    }
-  }
-};
+}
 
 // ---------------------------------------------------------------- the kernel
 template <int EPI, bool A_MN, bool B_MN, typename T, int ACT, int KEEP, int NJ>
@@ -267,6 +249,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&bars.acc_full[i], 1);
       mbar_init(&bars.acc_empty[i], 2 * EPI_WARPS);
     }
+    if constexpr (EPI == GRADS)
+      for (int i = 0; i < EPI_WARPS * 3; ++i) mbar_init(&bars.kept_full[i / 3][i % 3], 1);
     fence_barrier_init();
   }
   if (warp == 2) {
@@ -363,6 +347,48 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int quad = warp % 4, side = (warp - 4) / 4;  // 32 rows, a share of the columns
     const uint32_t boxes = staging + (warp - 4) * S::WARP_BYTES;
     int it = 0, set = 0;
+    // The backward's first epilogue: a warp's chunks of 32 columns are numbered through its tiles. What was
+    // kept of the two or three after the present one is under way, in this tile or the next.
+    constexpr int CHUNKS = S::COLS / 32;
+    uint64_t* kept_full = bars.kept_full[warp - 4];
+    const uint32_t kept_boxes = boxes + S::SETS * S::SET_BYTES;
+    int rows[2] = {0, 0}, cols[2] = {0, 0};  // of this tile and the next
+    bool more = pair < args.tiles;           // whether there is a next one
+    auto look_ahead = [&](int t) {
+      more = t < args.tiles;
+      if (more) {
+        const Tile tile = find_tile<NJ>(args, t);
+        rows[1] = tile.m * PAIR_M + (int)rank * CTA_M + quad * 32;
+        cols[1] = tile.n * PAIR_N + side * S::COLS;
+      }
+    };
+    auto ask_kept = [&](int n, int c) {  // by lane 0: chunk number n, the c-th of this tile
+      const bool next = c >= CHUNKS;
+      if (next && !more) return;
+      const int row = next ? rows[1] : rows[0], col = (next ? cols[1] - CHUNKS * 32 : cols[0]) + c * 32;
+      const uint32_t to = kept_boxes + n % 3 * 2 * S::KEPT_BOX;
+      mbar_arrive_expect_tx(&kept_full[n % 3], 2 * S::KEPT_BOX);
+      load_own_2d(to, &args.kept_map[0], &kept_full[n % 3], col, row);
+      load_own_2d(to + S::KEPT_BOX, &args.kept_map[1], &kept_full[n % 3], col, row);
+    };
+    uint32_t sg = 127, su = 127;
+    auto ask_scales = [&](int c) {
+      const bool next = c >= CHUNKS;
+      const int64_t row = (next ? rows[1] : rows[0]) + lane, group = ((next ? cols[1] - CHUNKS * 32 : cols[0]) + c * 32) / GROUP8;
+      sg = su = 127;
+      if ((!next || more) && row < args.kept.T && group < args.kept.pitch / GROUP8) {
+        const uint8_t* at = args.kept.exps + group * args.kept.T + row;
+        sg = __ldg(at);
+        su = __ldg(at + args.kept.pitch / GROUP8 * args.kept.T);
+      }
+    };
+    if constexpr (EPI == GRADS) {
+      look_ahead(pair);
+      ask_scales(CHUNKS);
+      if (lane == 0)
+        for (int n = 0; n < (S::IN_PLACE ? 2 : 3); ++n) ask_kept(n, CHUNKS + n);
+      __syncwarp();
+    }
     for (int t = pair; t < args.tiles; t += pairs, ++it) {
       const Tile tile = find_tile<NJ>(args, t);
       const Job& job = args.job[tile.job];
@@ -372,7 +398,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // the next set of boxes, once the stores that read it are done
       auto next_boxes = [&]() {
         set = set + 1 == S::SETS ? 0 : set + 1;
-        if (lane == 0) store_wait_read<S::SETS - 1>();
+        if (lane == 0) store_wait_read<(S::SETS > 0 ? S::SETS - 1 : 0)>();
         __syncwarp();
         return boxes + set * S::SET_BYTES;
       };
@@ -388,28 +414,29 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       const uint32_t mine = ta + side * S::COLS;
       if constexpr (EPI == GRADS) {
-        const int col0 = tile.n * PAIR_N + side * S::COLS;
-        const int64_t row = row0 + lane;
-        KeptRow<KEEP> kept;
-        kept.load(args.kept, row, col0);
+        rows[0] = rows[1], cols[0] = cols[1];
+        look_ahead(t + pairs);
         if (!mbar_wait(&bars.acc_full[acc], (it >> 1) & 1, args.err, 64)) break;
         tc_fence_after();
         uint32_t r[32];
         ask_acc<32>(mine, r);
+        bool ok = true;
 #pragma unroll 1
         for (int c = 0; c < S::COLS; c += 32) {
+          const int n = it * CHUNKS + c / 32;
+          const uint32_t from = kept_boxes + n % 3 * 2 * S::KEPT_BOX;
+          const float scale_g = scale_of(sg), scale_u = scale_of(su);
+          ask_scales(c / 32 + 1);
+          if (!(ok = mbar_wait(&kept_full[n % 3], n / 3 & 1, args.err, 65))) break;
           float d[32];
           take_acc<32>(r, d);
-          const KeptRow<KEEP> now = kept;
-          if (c + 32 < S::COLS) {
-            kept.load(args.kept, row, col0 + c + 32);
-            ask_acc<32>(mine + c + 32, r);
-          }
-          uint32_t to = 0;
+          if (c + 32 < S::COLS) ask_acc<32>(mine + c + 32, r);
+          uint32_t to = from;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             float a[16], b[16], e[16];
-            now.values(half, a, b);
+            kept_values<KEEP>(from, lane, half, scale_g, a);
+            kept_values<KEEP>(from + S::KEPT_BOX, lane, half, scale_u, b);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               float v, dv;
@@ -418,13 +445,24 @@ __global__ void __launch_bounds__(THREADS, 1)
               b[i] *= v;
               e[i] = d[16 * half + i] * v;
             }
-            if (half == 0) to = next_boxes();
+            if constexpr (!S::IN_PLACE)
+              if (half == 0) to = next_boxes();
             stage_row<T, 16>(to, lane, a, 16 * half);
             stage_row<T, 16>(to + BOX_BYTES, lane, e, 16 * half);
-            if constexpr (KEEP == DSALT_KEEP_8BIT) stage_row<T, 16>(to + 2 * BOX_BYTES, lane, b, 16 * half);
+            if constexpr (!S::IN_PLACE) stage_row<T, 16>(to + 2 * BOX_BYTES, lane, b, 16 * half);
           }
-          send(to, col0 + c);
+          send(to, cols[0] + c);
+          if (lane == 0) {
+            if constexpr (S::IN_PLACE) {
+              store_wait_read<1>();  // the chunk before this one has left its boxes
+              ask_kept(n + 2, c / 32 + 2);
+            } else {
+              ask_kept(n + 3, c / 32 + 3);  // every lane has read this one's
+            }
+          }
+          __syncwarp();
         }
+        if (!ok) break;
       } else if constexpr (EPI == GATE_UP) {
         if (!mbar_wait(&bars.acc_full[acc], (it >> 1) & 1, args.err, 64)) break;
         tc_fence_after();
@@ -554,7 +592,7 @@ template <int EPI, bool A_MN, bool B_MN, typename T, int ACT, int KEEP, int NJ>
 int launch_pair(Args<NJ>& a, const Ffn& f, bool after, const char* what) {
   static std::atomic<uint64_t> ready{0};
   constexpr int bytes = Shape<EPI, KEEP>::SMEM_BYTES, PAIRS = 74;
-  static_assert(bytes <= 232448, "shared memory of a block");
+  static_assert(sizeof(Bars<6>) <= 512 && bytes <= 232448, "shared memory of a block");
   static_assert(EPI != PLAIN || Shape<EPI, KEEP>::STAGES * STAGE_BYTES >= CTA_M * PAIR_N * 4, "the sums of a part do not fit");
   auto kernel = ffn_pair_kernel<EPI, A_MN, B_MN, T, ACT, KEEP, NJ>;
   if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), bytes, ready)) return rc;
@@ -630,6 +668,12 @@ int grads(const Ffn& f) {
       (rc = output(&j.c[1], f.du, f, f.T, f.F, f.pitch)) || (KEEP == DSALT_KEEP_8BIT && (rc = output(&j.c[2], f.h, f, f.T, f.F, f.pitch))))
     return rc;
   a.kept = {f.kept, f.exps, f.h, f.T, f.pitch};
+  for (int i = 0; i < 2; ++i) {
+    const char* p = static_cast<const char*>(f.kept) + i * f.T * f.pitch * (KEEP == DSALT_KEEP_8BIT ? 1 : 2);
+    if ((rc = KEEP == DSALT_KEEP_8BIT ? make_map(&a.kept_map[i], p, DTYPE_BYTES, f.T, f.pitch, f.pitch, 32, 32)
+                                      : make_map(&a.kept_map[i], p, f.dtype, f.T, f.pitch, f.pitch, 32, BOX)))
+      return rc;
+  }
   return launch_pair<GRADS, false, true, T, ACT, KEEP, 1>(a, f, false, "gated_ffn_bwd hidden gradients launch");
 }
 

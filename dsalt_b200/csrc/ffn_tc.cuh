@@ -52,6 +52,14 @@ __device__ __forceinline__ void take_acc(uint32_t (&r)[N], float (&f)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) f[i] = __uint_as_float(r[i]);
 }
+// load into this CTA's shared memory, counted on its own barrier
+__device__ __forceinline__ void load_own_2d(uint32_t dst, const void* map, uint64_t* bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+          dst),
+      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
+      : "memory");
+}
 inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -69,20 +77,27 @@ inline EncodeTiledFn get_encode() {
   return fn;
 }
 
-// rows x cols values of 16 bits, `stride` values from row to row, in boxes of box_rows x box_cols (as wide as the swizzle:
-// 64 or 32 columns)
+// rows x cols values of 16 bits, `stride` values from row to row, in boxes of box_rows x box_cols (as wide as
+// the swizzle: 64 or 32 columns), or DTYPE_BYTES in boxes of 32 columns without a swizzle
+constexpr int DTYPE_BYTES = -1;
 inline int make_map(CUtensorMap* m, const void* p, int dtype, int64_t rows, int64_t cols, int64_t stride, int box_rows,
-             int box_cols) {
+                    int box_cols) {
   const EncodeTiledFn enc = get_encode();
   if (!enc) return fail(DSALT_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const bool bytes = dtype == DTYPE_BYTES;
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
+  const cuuint64_t strides[1] = {(cuuint64_t)stride * (bytes ? 1 : 2)};
   const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
   const cuuint32_t step[2] = {1, 1};
-  const CUresult r = enc(m, dtype == DSALT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-                         const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = enc(m,
+                         bytes                 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                         : dtype == DSALT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                         2, const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         bytes            ? CU_TENSOR_MAP_SWIZZLE_NONE
+                         : box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                          : CU_TENSOR_MAP_SWIZZLE_64B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(DSALT_ERR_CUDA, "gated_ffn: cuTensorMapEncodeTiled failed (%d)", (int)r);
   return DSALT_OK;
 }
