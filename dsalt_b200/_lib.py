@@ -12,6 +12,7 @@ import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "_lib", "libdsalt_b200.so")
+TORCH_LIB_PATH = os.path.join(HERE, "_lib", "_torch_layers.so")
 
 F32, BF16, F16 = 0, 1, 2
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_CUDA, ERR_WORKSPACE, ERR_DEVICE = range(6)
@@ -91,6 +92,7 @@ SIGNATURES = {
 
 _lock = threading.Lock()
 _lib = None
+_torch_layers = None
 
 
 class DsaltError(RuntimeError):
@@ -116,6 +118,24 @@ def load() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = lib
     return _lib
+
+
+def torch_layers():
+    """The compiled module over these entry points that :mod:`dsalt_b200.layers` calls (raises if it is not
+    built)."""
+    global _torch_layers
+    if _torch_layers is None:
+        load()
+        if not os.path.exists(TORCH_LIB_PATH):
+            raise RuntimeError(f"{TORCH_LIB_PATH} not built; run `python -m dsalt_b200.build`")
+        import importlib.util
+
+        import torch  # noqa: F401  (the module's own libraries)
+        spec = importlib.util.spec_from_file_location("dsalt_b200._torch_layers", TORCH_LIB_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _torch_layers = module
+    return _torch_layers
 
 
 def call(name: str, *args):

@@ -1,4 +1,5 @@
-"""Builds the C-ABI library ``dsalt_b200/_lib/libdsalt_b200.so`` with nvcc for sm_100a.
+"""Builds the C-ABI library ``dsalt_b200/_lib/libdsalt_b200.so`` with nvcc for sm_100a, and torch's side of
+the operators of :mod:`dsalt_b200.layers` (``dsalt_b200/_lib/_torch_layers.so``) with g++ against it.
 
     python -m dsalt_b200.build
 
@@ -18,6 +19,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(OUT_DIR, "libdsalt_b200.so")
+TORCH_SOURCE = os.path.join(CSRC, "torch_layers.cpp")
+TORCH_LIB = os.path.join(OUT_DIR, "_torch_layers.so")
 SOURCES = ["capi.cu", "signals.cu", "select.cu", "attn_simt.cu", "attn_tc.cu", "attn_bwd.cu", "attn_train.cu", "peer.cu",
            "slots.cu", "cache_append.cu", "cache_attn.cu", "sample.cu", "pack8.cu", "rope.cu", "ffn.cu", "ffn_tc.cu",
            "ffn_few.cu", "ffn_token.cu"]
@@ -40,9 +43,32 @@ def _newer(target: str, deps) -> bool:
 
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OUT_DIR, exist_ok=True)
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(ROOT, "include", "dsalt_b200.h")]
-    if not force and _newer(LIB, deps):
-        return LIB
+    header = os.path.join(ROOT, "include", "dsalt_b200.h")
+    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh"))] + [header]
+    if force or not _newer(LIB, deps):
+        _build_kernels(verbose)
+    if force or not _newer(TORCH_LIB, [TORCH_SOURCE, header]):
+        _build_torch_side()
+    return LIB
+
+
+def _build_torch_side() -> None:
+    import sysconfig
+
+    from torch.utils.cpp_extension import include_paths, library_paths
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    include = [*include_paths(), sysconfig.get_path("include"), os.path.join(cuda, "include")]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_torch_layers",
+           "-D_GLIBCXX_USE_CXX11_ABI=1", *[a for p in include for a in ("-isystem", p)], "-I", os.path.join(ROOT, "include"),
+           TORCH_SOURCE, "-o", TORCH_LIB + ".tmp", "-L" + OUT_DIR, "-ldsalt_b200", "-Wl,-rpath,$ORIGIN",
+           *["-L" + p for p in library_paths()], "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError("g++ failed:\n" + res.stderr[-8000:])
+    os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+
+
+def _build_kernels(verbose: bool) -> None:
     cmd = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
            "-I", os.path.join(ROOT, "include"), "-o", LIB + ".tmp"]
     if verbose:
@@ -54,7 +80,6 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if verbose:
         sys.stderr.write(res.stderr)
     os.replace(LIB + ".tmp", LIB)
-    return LIB
 
 
 if __name__ == "__main__":

@@ -1,0 +1,394 @@
+// Torch's side of the operators around the attention (dsalt_b200/layers.py): checks of arguments, outputs
+// and workspaces from torch's allocator, and autograd nodes, over the C entry points.
+//
+// Compiled, because these calls are short: from Python the checks, the outputs and the call of 23 to 33
+// arguments take 15 to 20 us and a backward node some 50 us more than an empty one, several times
+// the device time of a decode step (4 us for the heads of 64 tokens) and as much as that of a
+// training step's head norms over 24000 tokens.
+#include <torch/extension.h>
+
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+
+#include "../../include/dsalt_b200.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+constexpr int64_t GROUP = 32;
+
+template <typename... Args>
+std::string words(const Args&... args) { return c10::str(args...); }
+
+void check(int rc, const char* fn) {
+  if (rc == DSALT_OK) return;
+  const std::string msg = dsalt_last_error();
+  if (PyGILState_Check()) {
+    const py::object cls = py::module_::import("dsalt_b200._lib").attr("DsaltError");
+    PyErr_SetObject(cls.ptr(), cls(rc, fn, msg).ptr());
+    throw py::error_already_set();
+  }
+  TORCH_CHECK(false, fn, " failed (status ", rc, "): ", msg);  // in autograd's own threads
+}
+
+int type_code(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return DSALT_F32;
+    case at::kBFloat16: return DSALT_BF16;
+    case at::kHalf: return DSALT_F16;
+    default: throw py::type_error(words("unsupported dtype ", t.dtype()));
+  }
+}
+
+// every defined tensor on one CUDA device
+c10::Device one_device(std::initializer_list<const Tensor*> ts) {
+  const Tensor& first = **ts.begin();
+  TORCH_CHECK(first.is_cuda(), "dsalt_b200 operators need CUDA tensors (no CPU path)");
+  for (const Tensor* t : ts)
+    TORCH_CHECK(!t->defined() || t->device() == first.device(), "tensors on ", first.device(), " and ", t->device(),
+                " in one call");
+  return first.device();
+}
+
+void want(const Tensor& t, const char* name, at::ScalarType type, at::IntArrayRef shape) {
+  if (t.scalar_type() != type) throw py::type_error(words(name, " must be ", type, ", got ", t.scalar_type()));
+  if (t.sizes() != shape) throw py::value_error(words(name, " must have shape ", shape, ", got ", t.sizes()));
+  if (!t.is_contiguous()) throw py::value_error(words(name, " must be contiguous"));
+}
+
+bool at16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+Tensor empty(at::IntArrayRef shape, at::ScalarType type, c10::Device dev) {
+  return at::empty(shape, at::TensorOptions().dtype(type).device(dev));
+}
+Tensor workspace(size_t bytes, c10::Device dev) { return empty({(int64_t)std::max<size_t>(bytes, 256)}, at::kByte, dev); }
+void no_second_derivative() {
+  TORCH_CHECK(!at::GradMode::is_enabled(), "dsalt_b200 operators have no second derivative");  // create_graph=True
+}
+
+// The tensor's device as the current one, and its current stream, while a call is made
+struct Launch {
+  c10::cuda::CUDAGuard guard;
+  void* stream;
+  explicit Launch(c10::Device dev) : guard(dev), stream(c10::cuda::getCurrentCUDAStream(dev.index()).stream()) {}
+};
+
+// --------------------------------------------------------------------------- 8 bits
+// x [..., n] as rows of consecutive values and their stride (a copy where its strides do not allow that)
+std::pair<Tensor, int64_t> matrix(const Tensor& x) {
+  const int64_t n = x.size(-1);
+  if (x.is_contiguous()) return {x.dim() == 2 ? x : x.view({-1, n}), n};
+  Tensor m = x.dim() == 2 ? x : x.reshape({-1, n});
+  const bool several = m.size(0) > 1;
+  if ((n > 1 && m.stride(1) != 1) || (several && m.stride(0) < n)) return {m.contiguous(), n};
+  return {m, several ? m.stride(0) : n};
+}
+
+std::tuple<Tensor, Tensor> pack_rows(const Tensor& m, int64_t stride, c10::Device dev) {
+  const int64_t rows = m.size(0), n = m.size(1);
+  Tensor codes = empty({rows, n}, at::kChar, dev), exps = empty({rows, (n + GROUP - 1) / GROUP}, at::kByte, dev);
+  const Launch launch(dev);
+  check(dsalt_pack8(m.data_ptr(), type_code(m), rows, n, stride, codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(),
+                    launch.stream),
+        "dsalt_pack8");
+  return {codes, exps};
+}
+
+std::tuple<Tensor, Tensor> pack8(const Tensor& x) {
+  const c10::Device dev = one_device({&x});
+  if (x.dim() < 1) throw py::value_error("pack8 needs at least one axis");
+  type_code(x);
+  std::vector<int64_t> groups = x.sizes().vec();
+  groups.back() = (groups.back() + GROUP - 1) / GROUP;
+  if (x.numel() == 0) return {empty(x.sizes(), at::kChar, dev), empty(groups, at::kByte, dev)};
+  const at::NoGradGuard no_grad;
+  const auto [m, stride] = matrix(x);
+  auto [codes, exps] = pack_rows(m, stride, dev);
+  if (x.dim() == 2) return {codes, exps};
+  return {codes.view(x.sizes()), exps.view(groups)};
+}
+
+Tensor unpack8(const Tensor& codes, const Tensor& exps, int dtype) {
+  const c10::Device dev = one_device({&codes, &exps});
+  if (codes.dim() < 1) throw py::value_error("codes need at least one axis");
+  std::vector<int64_t> groups = codes.sizes().vec();
+  const int64_t n = groups.back();
+  groups.back() = (n + GROUP - 1) / GROUP;
+  want(codes, "codes", at::kChar, codes.sizes());
+  want(exps, "exps", at::kByte, groups);
+  Tensor out = empty(codes.sizes(), dtype == DSALT_F32 ? at::kFloat : dtype == DSALT_BF16 ? at::kBFloat16 : at::kHalf, dev);
+  const Launch launch(dev);
+  check(dsalt_unpack8(codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), n ? codes.numel() / n : 0, n, out.data_ptr(), dtype,
+                      launch.stream),
+        "dsalt_unpack8");
+  return out;
+}
+
+// --------------------------------------------------------------------------- heads
+// x [T, H, D] with its token and head strides, as 16-byte loads can take its rows; else a copy
+struct Heads {
+  Tensor t;
+  int64_t token, head;
+};
+Heads heads(const Tensor& x) {
+  const int64_t T = x.size(0), H = x.size(1), D = x.size(2);
+  if (at16(x.data_ptr())) {
+    if (x.is_contiguous()) return {x, H * D, D};
+    const int64_t es = x.element_size(), token = T == 1 ? H * D : x.stride(0), head = H == 1 ? D : x.stride(1);
+    if (x.stride(2) == 1 && token * es % 16 == 0 && head * es % 16 == 0) return {x, token, head};
+  }
+  return {x.clone(at::MemoryFormat::Contiguous), H * D, D};
+}
+
+// a table of angles as fp32 with 16-byte aligned rows, and their stride
+std::pair<Tensor, int64_t> table(const Tensor& t, int64_t D) {
+  Tensor u = t.scalar_type() == at::kFloat ? t : t.to(at::kFloat);
+  const bool several = u.size(0) > 1;
+  if (u.stride(1) != 1 || !at16(u.data_ptr()) || (several && (u.stride(0) % 4 || u.stride(0) < D / 2)))
+    u = u.clone(at::MemoryFormat::Contiguous);
+  return {u, several ? u.stride(0) : (D + 3) / 4 * 4};
+}
+
+struct Rope {
+  c10::Device dev{c10::kCPU};
+  int64_t T = 0, H = 0, Hk = 0, D = 0, stride = 0;
+  Tensor cos, sin, positions, q_weight, k_weight;
+};
+
+Rope rope_args(const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor& sin, const Tensor& positions,
+               const Tensor& q_weight, const Tensor& k_weight) {
+  if (q.dim() != 3 || k.dim() != 3) throw py::value_error("q must be [T, H, D] and k [T, H_kv, D]");
+  Rope a;
+  a.dev = one_device({&q, &k, &cos, &sin, &positions, &q_weight, &k_weight});
+  a.T = q.size(0), a.H = q.size(1), a.D = q.size(2), a.Hk = k.size(1);
+  if (k.size(0) != a.T || k.size(2) != a.D)
+    throw py::value_error(words("k must be [", a.T, ", H_kv, ", a.D, "], got ", k.sizes()));
+  if (k.scalar_type() != q.scalar_type()) throw py::type_error("q and k must share a dtype");
+  type_code(q);
+  if (q_weight.defined() != k_weight.defined()) throw py::value_error("q_weight and k_weight go together");
+  if (q_weight.defined()) {
+    type_code(q_weight);
+    want(q_weight, "q_weight", q_weight.scalar_type(), {a.D});
+    want(k_weight, "k_weight", q_weight.scalar_type(), {a.D});
+  }
+  if (a.D % 2) throw py::value_error(words("head_dim ", a.D, " is odd"));
+  if (cos.dim() != 2 || cos.sizes() != sin.sizes() || (cos.size(1) != a.D && cos.size(1) != a.D / 2))
+    throw py::value_error(words("cos and sin must be [rows, ", a.D, "] or [rows, ", a.D / 2, "], both alike"));
+  int64_t other;
+  std::tie(a.cos, a.stride) = table(cos, a.D);
+  std::tie(a.sin, other) = table(sin, a.D);
+  if (other != a.stride) {
+    a.cos = a.cos.contiguous(), a.sin = a.sin.contiguous();
+    a.stride = a.cos.stride(0);
+  }
+  a.positions = positions;
+  if (positions.defined()) {
+    if (positions.dim() != 1 || positions.size(0) != a.T ||
+        (positions.scalar_type() != at::kInt && positions.scalar_type() != at::kLong))
+      throw py::value_error(words("positions must be [", a.T, "] whole numbers"));
+    a.positions = positions.to(at::kInt).contiguous();
+    if (cos.size(0) == 0 && a.T) throw py::value_error("empty tables");
+  } else if (cos.size(0) < a.T) {
+    throw py::value_error(words("tables of ", cos.size(0), " rows for ", a.T, " tokens"));
+  }
+  a.q_weight = q_weight, a.k_weight = k_weight;
+  return a;
+}
+
+variable_list rope_forward(const Tensor& q, const Tensor& k, const Rope& a, double eps) {
+  Tensor qo = empty({a.T, a.H, a.D}, q.scalar_type(), a.dev), ko = empty({a.T, a.Hk, a.D}, q.scalar_type(), a.dev);
+  const Heads x = heads(q), y = heads(k);
+  const Launch launch(a.dev);
+  check(dsalt_qk_norm_rope(x.t.data_ptr(), y.t.data_ptr(), type_code(q), a.T, (int)a.H, (int)a.Hk, (int)a.D, x.token, x.head,
+                           y.token, y.head, ptr(a.q_weight), ptr(a.k_weight), a.q_weight.defined() ? type_code(a.q_weight) : 0,
+                           (float)eps, a.cos.data_ptr<float>(), a.sin.data_ptr<float>(), std::max<int64_t>(a.cos.size(0), 1),
+                           a.stride, static_cast<const int32_t*>(ptr(a.positions)), qo.data_ptr(), ko.data_ptr(),
+                           launch.stream),
+        "dsalt_qk_norm_rope");
+  return {qo, ko};
+}
+
+// q and k are kept as they came; the norms are formed again in the backward pass
+struct RopeNode : torch::autograd::Function<RopeNode> {
+  // the weights are arguments of their own (any tensor where there are none), so that the node sees them
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor&, const Tensor&,
+                               const Rope& a, double eps) {
+    ctx->save_for_backward({q, k, a.q_weight, a.k_weight, a.cos, a.sin, a.positions});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["stride"] = a.stride;
+    return rope_forward(q, k, a, eps);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    no_second_derivative();
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &q = s[0], &k = s[1], &q_weight = s[2], &k_weight = s[3], &cos = s[4], &sin = s[5], &positions = s[6];
+    const c10::Device dev = q.device();
+    const int64_t T = q.size(0), H = q.size(1), D = q.size(2), Hk = k.size(1);
+    const bool norm = q_weight.defined();
+    Tensor dq = empty({T, H, D}, q.scalar_type(), dev), dk = empty({T, Hk, D}, q.scalar_type(), dev), dwq, dwk, ws;
+    if (norm) {
+      dwq = empty({D}, q_weight.scalar_type(), dev), dwk = empty({D}, q_weight.scalar_type(), dev);
+      ws = workspace(dsalt_qk_norm_rope_bwd_workspace_bytes((int)D), dev);
+    }
+    const Heads x = heads(q), y = heads(k);
+    // an output that nothing used has no gradient
+    const Heads gx = heads(grads[0].defined() ? grads[0] : at::zeros_like(dq)),
+                gy = heads(grads[1].defined() ? grads[1] : at::zeros_like(dk));
+    const Launch launch(dev);
+    check(dsalt_qk_norm_rope_bwd(x.t.data_ptr(), y.t.data_ptr(), gx.t.data_ptr(), gy.t.data_ptr(), type_code(q), T, (int)H,
+                                 (int)Hk, (int)D, x.token, x.head, y.token, y.head, gx.token, gx.head, gy.token, gy.head,
+                                 ptr(q_weight), ptr(k_weight), norm ? type_code(q_weight) : 0,
+                                 (float)ctx->saved_data["eps"].toDouble(), cos.data_ptr<float>(), sin.data_ptr<float>(),
+                                 std::max<int64_t>(cos.size(0), 1), ctx->saved_data["stride"].toInt(),
+                                 static_cast<const int32_t*>(ptr(positions)), dq.data_ptr(), dk.data_ptr(), ptr(dwq), ptr(dwk),
+                                 ptr(ws), norm ? (size_t)ws.numel() : 0, launch.stream),
+          "dsalt_qk_norm_rope_bwd");
+    return {dq, dk, dwq, dwk, Tensor(), Tensor()};
+  }
+};
+
+bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor& sin,
+                                        const std::optional<Tensor>& positions, const std::optional<Tensor>& q_weight,
+                                        const std::optional<Tensor>& k_weight, double eps) {
+  const Tensor pos = positions.value_or(Tensor()), wq = q_weight.value_or(Tensor()), wk = k_weight.value_or(Tensor());
+  const Rope a = rope_args(q, k, cos, sin, pos, wq, wk);
+  const variable_list out = wants_grad({&q, &k, &wq, &wk})
+                                ? RopeNode::apply(q, k, wq.defined() ? wq : cos, wk.defined() ? wk : cos, a, eps)
+                                : rope_forward(q, k, a, eps);
+  return {out[0], out[1]};
+}
+
+// --------------------------------------------------------------------------- feed-forward
+// whether the rows are 16-byte aligned, or their length does not allow that anyway
+bool rows_aligned(const Tensor& t, int64_t stride) {
+  const int64_t es = t.element_size();
+  return t.size(1) * es % 16 || (at16(t.data_ptr()) && stride * es % 16 == 0);
+}
+std::pair<Tensor, int64_t> ffn_rows(const Tensor& x) {
+  auto [m, stride] = matrix(x);
+  if (!rows_aligned(m, stride)) return {m.clone(at::MemoryFormat::Contiguous), m.size(1)};
+  return {m, stride};
+}
+Tensor ffn_weight(const Tensor& w) {
+  if (!w.is_contiguous()) return w.contiguous();
+  return rows_aligned(w, w.size(1)) ? w : w.clone();
+}
+
+struct Ffn {
+  c10::Device dev{c10::kCPU};
+  int64_t d = 0, F = 0, d_out = 0;
+};
+Ffn ffn_args(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const Tensor& w_down) {
+  Ffn a;
+  a.dev = one_device({&x, &w_gate, &w_up, &w_down});
+  if (w_gate.dim() != 2 || w_down.dim() != 2 || x.dim() < 1)
+    throw py::value_error("x must be [..., d_model], w_gate and w_up [d_ff, d_model], w_down [d_out, d_ff]");
+  a.F = w_gate.size(0), a.d = w_gate.size(1), a.d_out = w_down.size(0);
+  if (x.size(-1) != a.d || w_up.sizes() != w_gate.sizes() || w_down.size(1) != a.F)
+    throw py::value_error(words("x ", x.sizes(), ", w_gate ", w_gate.sizes(), ", w_up ", w_up.sizes(), " and w_down ",
+                                w_down.sizes(), " do not fit together"));
+  const at::ScalarType type = x.scalar_type();
+  if (w_gate.scalar_type() != type || w_up.scalar_type() != type || w_down.scalar_type() != type)
+    throw py::type_error("x and the weights must share a dtype");
+  type_code(x);
+  return a;
+}
+
+struct Kept {
+  Tensor y, kept, exps;
+};
+// the rows of m; nothing is kept with DSALT_KEEP_NONE
+Kept ffn_forward(const Tensor& x, const Tensor& m, int64_t stride, const Tensor& w_gate, const Tensor& w_up,
+                 const Tensor& w_down, const Ffn& a, int act, int keep) {
+  const int64_t T = m.size(0);
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = a.d_out;
+  const int dt = type_code(m);
+  Kept k;
+  k.y = empty(shape, m.scalar_type(), a.dev);
+  if (keep != DSALT_KEEP_NONE) {
+    const int64_t pitch = dsalt_gated_ffn_pitch((int)a.F);
+    const bool coded = keep == DSALT_KEEP_8BIT;
+    k.kept = empty({coded ? 2 : 3, T, pitch}, coded ? at::kChar : m.scalar_type(), a.dev);
+    if (coded || dt != DSALT_F32) k.exps = empty({2, pitch / GROUP, T}, at::kByte, a.dev);
+  }
+  const Tensor ws = workspace(dsalt_gated_ffn_workspace_bytes(dt, T, (int)a.d, (int)a.F, (int)a.d_out), a.dev);
+  const Launch launch(a.dev);
+  check(dsalt_gated_ffn(m.data_ptr(), dt, T, (int)a.d, stride, w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
+                        (int)a.F, (int)a.d_out, act, keep, ptr(k.kept), static_cast<uint8_t*>(ptr(k.exps)), k.y.data_ptr(),
+                        ws.data_ptr(), (size_t)ws.numel(), launch.stream),
+        "dsalt_gated_ffn");
+  return k;
+}
+
+// Kept for the backward pass: gate's and up's sums and x, in 16 bits (fp32 inputs: as they are) or in 8. With
+// 16 the rows that the last product read are kept too; with 8 they are formed again.
+struct FfnNode : torch::autograd::Function<FfnNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_gate, const Tensor& w_up,
+                               const Tensor& w_down, int64_t act, int64_t keep) {
+    const Ffn a = ffn_args(x, w_gate, w_up, w_down);
+    auto [m, stride] = ffn_rows(x);
+    const Tensor wg = ffn_weight(w_gate), wu = ffn_weight(w_up), wd = ffn_weight(w_down);
+    const Kept k = ffn_forward(x, m, stride, wg, wu, wd, a, (int)act, (int)keep);
+    Tensor x_exps;
+    if (!w_gate.requires_grad() && !w_up.requires_grad()) m = Tensor();  // only their gradients read it
+    else if (keep == DSALT_KEEP_8BIT && m.numel()) std::tie(m, x_exps) = pack_rows(m, stride, a.dev);
+    ctx->save_for_backward({m, x_exps, k.kept, k.exps, wg, wu, wd});
+    ctx->saved_data["stride"] = stride;
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["keep"] = keep;
+    ctx->saved_data["shape"] = x.sizes().vec();
+    return {k.y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    no_second_derivative();
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &x_exps = s[1], &kept = s[2], &exps = s[3], &wg = s[4], &wu = s[5], &wd = s[6];
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    const c10::Device dev = wg.device();
+    const int64_t T = kept.size(1), F = wg.size(0), d = wg.size(1), d_out = wd.size(0);
+    const int keep = (int)ctx->saved_data["keep"].toInt(), dt = type_code(wg);
+    const auto [dy, dy_stride] = ffn_rows(grads[0].reshape({T, d_out}));
+    Tensor dx, dwg, dwu, dwd;
+    if (ctx->needs_input_grad(0)) dx = empty(ctx->saved_data["shape"].toIntVector(), wg.scalar_type(), dev);
+    const bool both = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
+    if (both) dwg = empty({F, d}, wg.scalar_type(), dev), dwu = empty({F, d}, wg.scalar_type(), dev);
+    if (ctx->needs_input_grad(3)) dwd = empty({d_out, F}, wg.scalar_type(), dev);
+    const Tensor ws = workspace(dsalt_gated_ffn_bwd_workspace_bytes(dt, T, (int)d, (int)F, (int)d_out, keep), dev);
+    const Launch launch(dev);
+    check(dsalt_gated_ffn_bwd(dy.data_ptr(), dt, T, (int)d, dy_stride, ptr(x), ctx->saved_data["stride"].toInt(),
+                              static_cast<const uint8_t*>(ptr(x_exps)), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), (int)F,
+                              (int)d_out, (int)ctx->saved_data["act"].toInt(), keep, kept.data_ptr(),
+                              static_cast<const uint8_t*>(ptr(exps)), ptr(dx), ptr(dwg), ptr(dwu), ptr(dwd), ws.data_ptr(),
+                              (size_t)ws.numel(), launch.stream),
+          "dsalt_gated_ffn_bwd");
+    return {dx, ctx->needs_input_grad(1) ? dwg : Tensor(), ctx->needs_input_grad(2) ? dwu : Tensor(), dwd, Tensor(), Tensor()};
+  }
+};
+
+Tensor gated_ffn(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const Tensor& w_down, int act, int keep) {
+  const Ffn a = ffn_args(x, w_gate, w_up, w_down);
+  if (wants_grad({&x, &w_gate, &w_up, &w_down})) return FfnNode::apply(x, w_gate, w_up, w_down, (int64_t)act, (int64_t)keep)[0];
+  const at::NoGradGuard no_grad;
+  const auto [m, stride] = ffn_rows(x);
+  return ffn_forward(x, m, stride, ffn_weight(w_gate), ffn_weight(w_up), ffn_weight(w_down), a, act, DSALT_KEEP_NONE).y;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("pack8", &pack8);
+  m.def("unpack8", &unpack8);
+  m.def("qk_norm_rope", &qk_norm_rope);
+  m.def("gated_ffn", &gated_ffn);
+}
