@@ -25,6 +25,7 @@ namespace dsalt {
 namespace ffn {
 namespace {
 
+constexpr int SUMS_COL = 128 * 4;  // bytes of a column of partial sums
 constexpr int PAIR_M = 256, CTA_M = 128, PAIR_N = 256, KB = 64;
 constexpr int OPERAND_BYTES = CTA_M * KB * 2, STAGE_BYTES = 2 * OPERAND_BYTES;
 constexpr int BOX = 32, BOX_BYTES = 32 * BOX * 2;  // a warp's staged outputs: 32 rows of 32 columns
@@ -58,8 +59,10 @@ struct Args {
 };
 
 // ---------------------------------------------------------------- pair-wide forms
+// relaxed: it says that the accumulator has been read (tcgen05.wait::ld has returned); a release would wait for the
+// thread's stores to memory, some 1600 cycles a tile
 __device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // load into this CTA's shared memory, counted on a barrier of the pair
 __device__ __forceinline__ void load_2d(uint32_t dst, const void* map, uint32_t bar, int c0, int c1) {
@@ -68,6 +71,12 @@ __device__ __forceinline__ void load_2d(uint32_t dst, const void* map, uint32_t 
       "[%2];" ::"r"(dst),
       "l"(map), "r"(bar), "r"(c0), "r"(c1)
       : "memory");
+}
+// bytes of this CTA's shared memory to another's, counted on a barrier there
+__device__ __forceinline__ void copy_to_cta(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "r"(src), "r"(bytes), "r"(bar)
+               : "memory");
 }
 __device__ __forceinline__ void store_2d(const void* map, uint32_t src, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src),
@@ -79,7 +88,6 @@ template <int N>
 __device__ __forceinline__ void store_wait_read() {
   asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ void store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void pair_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -117,7 +125,7 @@ struct Shape {
 };
 template <int STAGES>
 struct Bars {
-  uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], kept_full[EPI_WARPS][3];
+  uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], kept_full[EPI_WARPS][3], sums;
   uint32_t tmem;
 };
 
@@ -240,6 +248,12 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int pair = blockIdx.x / 2 / split, pairs = gridDim.x / 2 / split;  // or cluster and clusters
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
+  if (threadIdx.x == 96) {  // of the first tile
+    const Job& job = args.job[find_tile<NJ>(args, pair).job];
+    tma_prefetch_desc(&job.a[0]);
+    tma_prefetch_desc(&job.b[EPI == GATE_UP ? rank : 0]);
+    if constexpr (EPI != GATE_UP) tma_prefetch_desc(&job.c[0]);
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&bars.full[i], 1);
@@ -249,6 +263,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&bars.acc_full[i], 1);
       mbar_init(&bars.acc_empty[i], 2 * EPI_WARPS);
     }
+    mbar_init(&bars.sums, 1);
     if constexpr (EPI == GRADS)
       for (int i = 0; i < EPI_WARPS * 3; ++i) mbar_init(&bars.kept_full[i / 3][i % 3], 1);
     fence_barrier_init();
@@ -413,6 +428,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       };
       const uint32_t mine = ta + side * S::COLS;
+      auto acc_read = [&]() {  // the accumulator may be overwritten
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_remote(in_cta(smem_u32(&bars.acc_empty[acc]), leader));
+      };
       if constexpr (EPI == GRADS) {
         rows[0] = rows[1], cols[0] = cols[1];
         look_ahead(t + pairs);
@@ -431,6 +451,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           float d[32];
           take_acc<32>(r, d);
           if (c + 32 < S::COLS) ask_acc<32>(mine + c + 32, r);
+          else acc_read();
           uint32_t to = from;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
@@ -479,6 +500,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (half + 1 < S::COLS / 32) {
             ask_acc<32>(mine + 32, rg);
             ask_acc<32>(mine + PAIR_N / 2 + 32, ru);
+          } else {
+            acc_read();
           }
           const bool in = row < args.kept.T && col + 32 * half < args.kept.pitch;
           if constexpr (KEEP != DSALT_KEEP_NONE) {
@@ -511,10 +534,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           float d[BOX];
           take_acc<BOX>(r, d);
           if (c + BOX < S::COLS) ask_acc<BOX>(mine + c + BOX, r);
-          if (split > 1) {  // sums of this part of K, as [column][row], where the operands were
+          else acc_read();
+          if (split > 1) {  // sums of this part of K, column by column, where the operands were
 #pragma unroll
             for (int i = 0; i < BOX; ++i)
-              asm volatile("st.shared.f32 [%0], %1;" ::"r"(base + ((side * S::COLS + c + i) * CTA_M + quad * 32 + lane) * 4),
+              asm volatile("st.shared.f32 [%0], %1;" ::"r"(base + (side * S::COLS + c + i) * SUMS_COL + (quad * 32 + lane) * 4),
                            "f"(d[i])
                            : "memory");
             continue;
@@ -524,45 +548,50 @@ __global__ void __launch_bounds__(THREADS, 1)
           send(to, col0 + c);
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) arrive_remote(in_cta(smem_u32(&bars.acc_empty[acc]), leader));
     }
-    if (lane == 0) store_wait_all();
+    if (lane == 0) store_wait_read<0>();
     __syncwarp();
   }
   tc_fence_before();
   if constexpr (EPI == PLAIN) {
     if (split > 1) {
-      // the parts' sums, in the order of the parts: each pair adds up and stores its share of the columns
-      cluster_sync();
+      // Each pair adds up and stores its share of the columns: the others' sums of it are copied over,
+      // whole columns at a time, behind its own (threads that read them where they are took 7000 cycles).
+      fence_proxy_async_smem();
+      cluster_sync();  // every part has its sums, and no operand is read any more
+      auto first = [&](int p) { return p * 32 / split; };  // groups of 8 columns
+      const int lo = first(part), groups = first(part + 1) - lo;
+      const uint32_t inbox = base + PAIR_N * SUMS_COL;
+      if (threadIdx.x == 0) {
+        mbar_arrive_expect_tx(&bars.sums, (split - 1) * groups * 8 * SUMS_COL);
+        for (int p = 0; p < split; ++p)
+          if (p != part) {
+            const int n = first(p + 1) - first(p), place = part < p ? part : part - 1;
+            copy_to_cta(in_cta(inbox + place * n * 8 * SUMS_COL, 2 * p + rank), base + first(p) * 8 * SUMS_COL, n * 8 * SUMS_COL,
+                        in_cta(smem_u32(&bars.sums), 2 * p + rank));
+          }
+      }
       const Tile tile = find_tile<NJ>(args, pair);
       const Job& job = args.job[tile.job];
       const int row = warp % 4 * 32 + lane, m = tile.m * PAIR_M + (int)rank * CTA_M + row;
-      const int lo = part * 32 / split, hi = (part + 1) * 32 / split;  // in groups of 8 columns
-#pragma unroll 2
-      for (int g = lo + warp / 4; g < hi; g += THREADS / 128) {
-        float v[4][8];  // all parts' loads under way at once
+      if (mbar_wait(&bars.sums, 0, args.err, 60))
+        for (int g = warp / 4; g < groups; g += THREADS / 128) {
+          float v[8] = {};
+          for (int p = 0; p < split; ++p) {  // in the order of the parts
+            const uint32_t from =
+                (p == part ? base + lo * 8 * SUMS_COL : inbox + (p < part ? p : p - 1) * groups * 8 * SUMS_COL) + row * 4;
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const uint32_t from = in_cta(base + (g * 8 * CTA_M + row) * 4, 2 * (p < split ? p : 0) + rank);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            v[p][i] = 0.f;
-            if (p < split)
-              asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[p][i]) : "r"(from + i * CTA_M * 4) : "memory");
+            for (int i = 0; i < 8; ++i) {
+              float x;
+              asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(from + (g * 8 + i) * SUMS_COL) : "memory");
+              v[i] += x;
+            }
           }
+          const int n = tile.n * PAIR_N + (lo + g) * 8;
+          if (m < job.rows && n < job.cols)
+            *reinterpret_cast<uint4*>(static_cast<T*>(job.out) + (int64_t)m * job.cols + n) = make_uint4(
+                narrow2<T>(v[0], v[1]), narrow2<T>(v[2], v[3]), narrow2<T>(v[4], v[5]), narrow2<T>(v[6], v[7]));
         }
-#pragma unroll
-        for (int p = 1; p < 4; ++p)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[0][i] += v[p][i];
-        const int n = tile.n * PAIR_N + g * 8;
-        if (m < job.rows && n < job.cols)
-          *reinterpret_cast<uint4*>(static_cast<T*>(job.out) + (int64_t)m * job.cols + n) =
-              make_uint4(narrow2<T>(v[0][0], v[0][1]), narrow2<T>(v[0][2], v[0][3]), narrow2<T>(v[0][4], v[0][5]),
-                         narrow2<T>(v[0][6], v[0][7]));
-      }
     }
   }
   __syncthreads();
@@ -593,7 +622,7 @@ int launch_pair(Args<NJ>& a, const Ffn& f, bool after, const char* what) {
   static std::atomic<uint64_t> ready{0};
   constexpr int bytes = Shape<EPI, KEEP>::SMEM_BYTES, PAIRS = 74;
   static_assert(sizeof(Bars<6>) <= 512 && bytes <= 232448, "shared memory of a block");
-  static_assert(EPI != PLAIN || Shape<EPI, KEEP>::STAGES * STAGE_BYTES >= CTA_M * PAIR_N * 4, "the sums of a part do not fit");
+  static_assert(EPI != PLAIN || bytes >= 1024 + 512 + (PAIR_N + 3 * PAIR_N / 4) * SUMS_COL, "the sums of a part do not fit");
   auto kernel = ffn_pair_kernel<EPI, A_MN, B_MN, T, ACT, KEEP, NJ>;
   if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), bytes, ready)) return rc;
   a.tiles = 0;
