@@ -5,8 +5,8 @@
 //              will be wanted;  y = h Wd^T
 //   backward   dh = dy Wd -> epilogue: dg = dh up act'(gate), du = dh act(gate), of 8-bit
 //              activations h again;
-//              dx = dg Wg + du Wu (one sum over both);  dWg = dg^T x, dWu = du^T x, dWd = dy^T h (one
-//              launch, so that the tiles of the three fill the GPU together)
+//              dx = dg Wg + du Wu (one sum over both);  dWg = dg^T x, dWu = du^T x, dWd = dy^T h, all
+//              in one launch
 //
 // Two CTAs share a tile of 256 x 256 outputs (tcgen05.mma of the pair: each holds 128 rows of A
 // and 128 of B, and reads the other's B through it), 64 values of K and 32 KB a CTA in a stage. The
@@ -31,8 +31,10 @@ constexpr int OPERAND_BYTES = CTA_M * KB * 2, STAGE_BYTES = 2 * OPERAND_BYTES;
 constexpr int BOX = 32, BOX_BYTES = 32 * BOX * 2;  // a warp's staged outputs: 32 rows of 32 columns
 constexpr int EPI_WARPS = 8, THREADS = 32 * (4 + EPI_WARPS);  // 16 warps in the first epilogue: no faster
 constexpr uint32_t TMEM_COLS = 512;
+constexpr int PAIRS = 74;  // of SMs
 constexpr int GROUP_M = 4;  // tiles of 256 rows whose A stays in L2 while N is walked; 1 to 16 differ by 2 %
 
+enum Order { ALONG = 0, ACROSS = 1, BY_JOB = 2 };  // how K of A lies: along its rows, across them
 enum Epilogue { PLAIN = 0, GATE_UP = 1, GRADS = 2 };
 
 struct alignas(64) Job {
@@ -40,6 +42,7 @@ struct alignas(64) Job {
   CUtensorMap c[3];
   int tiles_m, tiles_n, blocks0, blocks;  // blocks of K in the first segment and in all
   int rows, cols;                         // of the outputs
+  int a_across;                           // K of A lies across its rows (where jobs differ)
   void* out;                              // of c[0], for a plain store's sums of several parts
 };
 struct Kept {
@@ -53,6 +56,9 @@ struct Args {
   Job job[NJ];
   CUtensorMap kept_map[2];  // gate's and up's, where they are read
   Kept kept;
+  // Tiles are dealt round robin, or (of two kinds of jobs) the first `dealt` are, then each pair takes its extra
+  // ones of the others and then `rounds` in turn with the other pairs
+  int dealt, rounds, extra[PAIRS + 1];
   int tiles, split;  // split > 1: a cluster of so many pairs shares a tile, each takes a part of K
   uint32_t idesc;
   int* err;
@@ -132,6 +138,18 @@ struct Bars {
 struct Tile {
   int job, m, n;
 };
+// the i-th tile of a pair, or -1
+template <int NJ>
+__device__ __forceinline__ int tile_of(const Args<NJ>& a, int pair, int pairs, int i) {
+  const int t = pair + i * pairs;
+  if (t < a.dealt) return t;
+  if (a.dealt == a.tiles) return -1;
+  int k = i - (pair < a.dealt ? (a.dealt - pair + pairs - 1) / pairs : 0);
+  const int n = a.extra[pair + 1] - a.extra[pair];
+  if (k < n) return a.dealt + a.rounds * pairs + a.extra[pair] + k;
+  k -= n;
+  return k < a.rounds ? a.dealt + k * pairs + pair : -1;
+}
 template <int NJ>
 __device__ __forceinline__ Tile find_tile(const Args<NJ>& a, int t) {
   int j = 0;
@@ -233,7 +251,7 @@ __device__ __forceinline__ void kept_values(uint32_t box, int lane, int half, fl
 }
 
 // ---------------------------------------------------------------- the kernel
-template <int EPI, bool A_MN, bool B_MN, typename T, int ACT, int KEEP, int NJ>
+template <int EPI, int A_ORDER, bool B_MN, typename T, int ACT, int KEEP, int NJ>
 __global__ void __launch_bounds__(THREADS, 1)
     ffn_pair_kernel(const __grid_constant__ Args<NJ> args) {
   using S = Shape<EPI, KEEP>;
@@ -286,7 +304,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       int s = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = pair; ok && t < args.tiles; t += pairs) {
+      for (int i = 0, t; ok && (t = tile_of<NJ>(args, pair, pairs, i)) >= 0; ++i) {
         const Tile tile = find_tile<NJ>(args, t);
         const Job& job = args.job[tile.job];
         const int m0 = tile.m * PAIR_M + (int)rank * CTA_M;
@@ -303,7 +321,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           const uint32_t a = base + s * STAGE_BYTES, b = a + OPERAND_BYTES;
           const CUtensorMap* ma = &job.a[seg];
           const CUtensorMap* mb = &job.b[EPI == GATE_UP ? (int)rank : seg];
-          if constexpr (A_MN) {
+          if (A_ORDER == ACROSS || (A_ORDER == BY_JOB && job.a_across)) {
             load_2d(a, ma, full, m0, k);
             load_2d(a + OPERAND_BYTES / 2, ma, full, m0 + 64, k);
           } else {
@@ -328,12 +346,14 @@ __global__ void __launch_bounds__(THREADS, 1)
       int s = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = pair; ok && t < args.tiles; t += pairs, ++it) {
+      for (int t; ok && (t = tile_of<NJ>(args, pair, pairs, it)) >= 0; ++it) {
         const Tile tile = find_tile<NJ>(args, t);
         const int all = args.job[tile.job].blocks, blocks = (part + 1) * all / split - part * all / split, acc = it & 1;
         if (!mbar_wait(&bars.acc_empty[acc], ((it >> 1) & 1) ^ 1, args.err, 62)) break;
         tc_fence_after();
         const uint32_t d = tmem + acc * PAIR_N;
+        const bool across = A_ORDER == ACROSS || (A_ORDER == BY_JOB && args.job[tile.job].a_across);
+        const uint32_t idesc = args.idesc | (across ? 1u << 15 : 0u);
         for (int kb = 0; kb < blocks; ++kb) {
           if (!mbar_wait(&bars.full[s], phase, args.err, 63)) {
             ok = false;
@@ -344,9 +364,9 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int ks = 0; ks < KB / 16; ++ks) {
             // K along rows of 128 bytes: 16 values are 32 bytes on; across: 16 rows of 128 bytes
-            const uint64_t da = A_MN ? sw128_desc(a + ks * 2048, OPERAND_BYTES / 2, 1024) : sw128_desc(a + ks * 32, 16, 1024);
+            const uint64_t da = across ? sw128_desc(a + ks * 2048, OPERAND_BYTES / 2, 1024) : sw128_desc(a + ks * 32, 16, 1024);
             const uint64_t db = B_MN ? sw128_desc(b + ks * 2048, OPERAND_BYTES / 2, 1024) : sw128_desc(b + ks * 32, 16, 1024);
-            pair_mma(d, da, db, args.idesc, kb | ks);
+            pair_mma(d, da, db, idesc, kb | ks);
           }
           pair_commit(&bars.empty[s], leader);
           if (++s == STAGES) {
@@ -404,7 +424,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int n = 0; n < (S::IN_PLACE ? 2 : 3); ++n) ask_kept(n, CHUNKS + n);
       __syncwarp();
     }
-    for (int t = pair; t < args.tiles; t += pairs, ++it) {
+    for (int t; (t = tile_of<NJ>(args, pair, pairs, it)) >= 0; ++it) {
       const Tile tile = find_tile<NJ>(args, t);
       const Job& job = args.job[tile.job];
       const int acc = it & 1;
@@ -616,30 +636,75 @@ void size_job(Job& j, int64_t M, int64_t N, int64_t K, int tile_n) {
   j.cols = (int)N;
 }
 
+// Where a plain store's tiles leave half of the pairs idle, K is split over 2 to 4 pairs of a cluster, as far as
+// all clusters run at once: of 4, 6 and 8 CTAs of this size the GPU holds 33, 22 and 15 (its processing
+// clusters have odd numbers of SMs left over). 24 tiles of K = 2048: two parts 12 us, three 25, one 16.
+int split_for(int tiles, int blocks) {
+  constexpr int AT_ONCE[5] = {0, PAIRS, 33, 22, 15};
+  int split = 1;
+  while (split < 4 && tiles <= AT_ONCE[split + 1] && 4 * (split + 1) <= blocks) ++split;
+  return split;
+}
+// blocks of K that the longest-working pair goes through
+int64_t rounds_of(int tiles, int blocks) {
+  const int split = split_for(tiles, blocks);
+  return split > 1 ? ceil_div(blocks, split) : (int64_t)ceil_div(tiles, PAIRS) * blocks;
+}
+
+// Of the weights' and x's gradients, which differ in length: the longer tiles are dealt round robin, the shorter
+// ones so that all pairs end together. (Two launches leave pairs idle at the end of each: 341 us against 332 at
+// 32768 x 768 -> 2048.)
+void deal(Args<4>& a) {
+  const Job& x = a.job[a.job[0].a_across ? 3 : 0];
+  const Job* first_w = a.job + (a.job[0].a_across ? 0 : 1);
+  const Job& w = first_w[first_w->tiles_m ? 0 : 1];
+  const int x_tiles = x.tiles_m * x.tiles_n, w_tiles = a.tiles - x_tiles;
+  if (!x_tiles || !w_tiles) return;
+  const bool x_first = &x == &a.job[0];
+  // what a tile costs: its blocks of K and about eight more for its epilogue
+  const int64_t first_cost = (x_first ? x : w).blocks + 8, cost = (x_first ? w : x).blocks + 8;
+  a.dealt = x_first ? x_tiles : w_tiles;
+  const int others = a.tiles - a.dealt;
+  int64_t load[PAIRS], low = 0, high = 0;
+  for (int p = 0; p < PAIRS; ++p) {
+    load[p] = (p < a.dealt ? (a.dealt - p + PAIRS - 1) / PAIRS : 0) * first_cost;
+    high = load[p] > high ? load[p] : high;
+  }
+  high += (others / PAIRS + 1) * cost;
+  auto fits = [&](int64_t level, int p) { return level > load[p] ? (int)((level - load[p]) / cost) : 0; };
+  while (low < high) {  // the lowest level at which all find a place
+    const int64_t level = (low + high) / 2;
+    int64_t n = 0;
+    for (int p = 0; p < PAIRS; ++p) n += fits(level, p);
+    if (n >= others) high = level;
+    else low = level + 1;
+  }
+  int counts[PAIRS], left = -others;
+  for (int p = 0; p < PAIRS; ++p) left += counts[p] = fits(low, p);
+  for (int p = 0; left > 0; p = (p + 1) % PAIRS)
+    if (counts[p] > 0) --counts[p], --left;
+  a.rounds = counts[0];
+  for (int p = 1; p < PAIRS; ++p) a.rounds = counts[p] < a.rounds ? counts[p] : a.rounds;
+  for (int p = 0; p < PAIRS; ++p) a.extra[p + 1] = a.extra[p] + counts[p] - a.rounds;
+}
+template <int NJ>
+void deal(Args<NJ>&) {}
+
 // `after`: the launch before it in the stream is one of this call, whose end it may overlap
-template <int EPI, bool A_MN, bool B_MN, typename T, int ACT, int KEEP, int NJ>
+template <int EPI, int A_ORDER, bool B_MN, typename T, int ACT, int KEEP, int NJ>
 int launch_pair(Args<NJ>& a, const Ffn& f, bool after, const char* what) {
   static std::atomic<uint64_t> ready{0};
-  constexpr int bytes = Shape<EPI, KEEP>::SMEM_BYTES, PAIRS = 74;
+  constexpr int bytes = Shape<EPI, KEEP>::SMEM_BYTES;
   static_assert(sizeof(Bars<6>) <= 512 && bytes <= 232448, "shared memory of a block");
   static_assert(EPI != PLAIN || bytes >= 1024 + 512 + (PAIR_N + 3 * PAIR_N / 4) * SUMS_COL, "the sums of a part do not fit");
-  auto kernel = ffn_pair_kernel<EPI, A_MN, B_MN, T, ACT, KEEP, NJ>;
+  auto kernel = ffn_pair_kernel<EPI, A_ORDER, B_MN, T, ACT, KEEP, NJ>;
   if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), bytes, ready)) return rc;
   a.tiles = 0;
-  int blocks = 1 << 30;
-  for (int i = 0; i < NJ; ++i)
-    if (a.job[i].tiles_m) {
-      a.tiles += a.job[i].tiles_m * a.job[i].tiles_n;
-      blocks = a.job[i].blocks < blocks ? a.job[i].blocks : blocks;
-    }
-  // Where the tiles leave half of the pairs idle, K is split over 2 to 4 pairs of a cluster, as far as all
-  // clusters run at once: of 4, 6 and 8 CTAs of this size the GPU holds 33, 22 and 15 (its processing
-  // clusters have odd numbers of SMs left over). 24 tiles of K = 2048: two parts 12 us, three 25, one 16.
-  constexpr int AT_ONCE[5] = {0, PAIRS, 33, 22, 15};
-  a.split = 1;
-  if (EPI == PLAIN)
-    while (a.split < 4 && a.tiles <= AT_ONCE[a.split + 1] && 4 * (a.split + 1) <= blocks) ++a.split;
-  a.idesc = umma_idesc_f16(f.dtype == DSALT_BF16 ? 1 : 0, A_MN, B_MN, PAIR_M, PAIR_N);
+  for (int i = 0; i < NJ; ++i) a.tiles += a.job[i].tiles_m * a.job[i].tiles_n;
+  if (a.split < 1) a.split = EPI == PLAIN ? split_for(a.tiles, a.job[0].blocks) : 1;
+  a.idesc = umma_idesc_f16(f.dtype == DSALT_BF16 ? 1 : 0, 0, B_MN, PAIR_M, PAIR_N);
+  a.dealt = a.tiles;
+  if (NJ == 4 && a.split == 1 && a.tiles > PAIRS) deal(a);
   a.err = device_status_ptr();
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * a.split * (a.split > 1 || a.tiles < PAIRS ? a.tiles : PAIRS));
@@ -667,7 +732,7 @@ int gate_up(const Ffn& f) {
       (rc = operand(&j.b[1], f.w_up, f, f.F, f.d, f.d, false)))
     return rc;
   a.kept = {f.kept, f.exps, f.h, f.T, f.pitch};
-  return launch_pair<GATE_UP, false, false, T, ACT, KEEP, 1>(a, f, false, "gated_ffn gate and up launch");
+  return launch_pair<GATE_UP, ALONG, false, T, ACT, KEEP, 1>(a, f, false, "gated_ffn gate and up launch");
 }
 
 template <typename T, int ACT>
@@ -683,7 +748,7 @@ int forward(const Ffn& f) {
       (rc = operand(&j.b[0], f.w_down, f, f.d_out, f.F, f.F, false)) || (rc = output(&j.c[0], f.y, f, f.T, f.d_out, f.d_out)))
     return rc;
   j.out = f.y;
-  return launch_pair<PLAIN, false, false, T, 0, 0, 1>(a, f, true, "gated_ffn down launch");
+  return launch_pair<PLAIN, ALONG, false, T, 0, 0, 1>(a, f, true, "gated_ffn down launch");
 }
 
 template <typename T, int ACT, int KEEP>
@@ -703,12 +768,13 @@ int grads(const Ffn& f) {
                                       : make_map(&a.kept_map[i], p, f.dtype, f.T, f.pitch, f.pitch, 32, BOX)))
       return rc;
   }
-  return launch_pair<GRADS, false, true, T, ACT, KEEP, 1>(a, f, false, "gated_ffn_bwd hidden gradients launch");
+  return launch_pair<GRADS, ALONG, true, T, ACT, KEEP, 1>(a, f, false, "gated_ffn_bwd hidden gradients launch");
 }
 
 int weight_job(Job& j, const Ffn& f, const void* a, int64_t M, int64_t a_stride, const void* b, int64_t N, int64_t b_stride,
                void* c) {
   size_job(j, M, N, f.T, PAIR_N);
+  j.a_across = 1;
   int rc;
   if ((rc = operand(&j.a[0], a, f, f.T, M, a_stride, true)) || (rc = operand(&j.b[0], b, f, f.T, N, b_stride, true))) return rc;
   j.out = c;
@@ -719,25 +785,43 @@ template <typename T, int ACT>
 int backward(const Ffn& f) {
   int rc = f.keep == DSALT_KEEP_8BIT ? grads<T, ACT, DSALT_KEEP_8BIT>(f) : grads<T, ACT, DSALT_KEEP_INPUT>(f);
   if (rc) return rc;
-  if (f.dx) {
-    Args<1> a{};
-    Job& j = a.job[0];
-    size_job(j, f.T, f.d, f.F, PAIR_N);
-    j.blocks = 2 * j.blocks0;
-    if ((rc = operand(&j.a[0], f.dg, f, f.T, f.F, f.pitch, false)) || (rc = operand(&j.a[1], f.du, f, f.T, f.F, f.pitch, false)) ||
-        (rc = operand(&j.b[0], f.w_gate, f, f.F, f.d, f.d, true)) || (rc = operand(&j.b[1], f.w_up, f, f.F, f.d, f.d, true)) ||
-        (rc = output(&j.c[0], f.dx, f, f.T, f.d, f.d)))
+  if (!f.dx && !f.dw_gate && !f.dw_down) return DSALT_OK;
+  // x's gradient, of 2 d_ff, and the weights', of T values of K: in one launch, the longer ones first, or in two
+  // where the few long tiles of one would outlast the rest. That and the cut of K, and with it the sums' order,
+  // are the same whichever gradients are wanted.
+  const int x_blocks = 2 * ceil_div(f.F, KB), w_blocks = ceil_div(f.T, KB), F_tiles = ceil_div(f.F, PAIR_N);
+  const int x_tiles = ceil_div(f.T, PAIR_M) * ceil_div(f.d, PAIR_N);
+  const int w_tiles = ceil_div(f.d_out, PAIR_M) * F_tiles + 2 * F_tiles * ceil_div(f.d, PAIR_N);
+  const int tiles = x_tiles + w_tiles, longest = x_blocks > w_blocks ? x_blocks : w_blocks;
+  const int split = split_for(tiles, x_blocks < w_blocks ? x_blocks : w_blocks);
+  const int64_t even = ((int64_t)x_tiles * x_blocks + (int64_t)w_tiles * w_blocks) / PAIRS;
+  const int64_t one = split > 1 ? ceil_div(longest, split) : tiles > PAIRS && even > longest ? even : longest;
+  const bool together = one <= rounds_of(x_tiles, x_blocks) + rounds_of(w_tiles, w_blocks) + 16;  // 16: a launch
+  const bool x_first = x_blocks > w_blocks;
+  for (int launch = 0; launch < (together ? 1 : 2); ++launch) {
+    Args<4> a{};
+    const bool xs = f.dx && (together || launch == 0), ws = (f.dw_down || f.dw_gate) && (together || launch == 1);
+    if (!xs && !ws) continue;
+    a.split = together ? split : launch == 0 ? split_for(x_tiles, x_blocks) : split_for(w_tiles, w_blocks);
+    Job* w = a.job + (x_first ? 1 : 0);
+    for (int i = 0; i < 3; ++i) w[i].a_across = 1;
+    if (xs) {
+      Job& j = a.job[x_first ? 0 : 3];
+      size_job(j, f.T, f.d, f.F, PAIR_N);
+      j.blocks = 2 * j.blocks0;
+      j.out = f.dx;
+      if ((rc = operand(&j.a[0], f.dg, f, f.T, f.F, f.pitch, false)) || (rc = operand(&j.a[1], f.du, f, f.T, f.F, f.pitch, false)) ||
+          (rc = operand(&j.b[0], f.w_gate, f, f.F, f.d, f.d, true)) || (rc = operand(&j.b[1], f.w_up, f, f.F, f.d, f.d, true)) ||
+          (rc = output(&j.c[0], f.dx, f, f.T, f.d, f.d)))
+        return rc;
+    }
+    if (ws && f.dw_down && (rc = weight_job(w[0], f, f.dy, f.d_out, f.dy_stride, f.h, f.F, f.pitch, f.dw_down))) return rc;
+    if (ws && f.dw_gate && ((rc = weight_job(w[1], f, f.dg, f.F, f.pitch, f.x, f.d, f.x_stride, f.dw_gate)) ||
+                            (rc = weight_job(w[2], f, f.du, f.F, f.pitch, f.x, f.d, f.x_stride, f.dw_up))))
       return rc;
-    j.out = f.dx;
-    if ((rc = launch_pair<PLAIN, false, true, T, 0, 0, 1>(a, f, true, "gated_ffn_bwd dx launch"))) return rc;
+    if ((rc = launch_pair<PLAIN, BY_JOB, true, T, 0, 0, 4>(a, f, true, "gated_ffn_bwd gradients launch"))) return rc;
   }
-  if (!f.dw_gate && !f.dw_down) return DSALT_OK;
-  Args<3> a{};
-  if (f.dw_down && (rc = weight_job(a.job[0], f, f.dy, f.d_out, f.dy_stride, f.h, f.F, f.pitch, f.dw_down))) return rc;
-  if (f.dw_gate && ((rc = weight_job(a.job[1], f, f.dg, f.F, f.pitch, f.x, f.d, f.x_stride, f.dw_gate)) ||
-                    (rc = weight_job(a.job[2], f, f.du, f.F, f.pitch, f.x, f.d, f.x_stride, f.dw_up))))
-    return rc;
-  return launch_pair<PLAIN, true, true, T, 0, 0, 3>(a, f, true, "gated_ffn_bwd weights launch");
+  return DSALT_OK;
 }
 
 template <typename T>
