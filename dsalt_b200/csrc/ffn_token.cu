@@ -15,7 +15,13 @@ namespace dsalt {
 namespace ffn {
 namespace {
 
-constexpr int ROWS = 16, WARPS = 8, THREADS = 32 * WARPS, BATCH = 4, TOKENS = 8, MAX_SPLIT = 8;
+constexpr int ROWS = 16, TOKENS = 8, MAX_SPLIT = 8;
+// The second product has few rows and a long K: twice the warps to a block, each with twice the loads under
+// way, so that one token's weights wait in registers for h and clusters are rarely needed
+template <bool GATED>
+struct Block {
+  static constexpr int WARPS = GATED ? 8 : 16, THREADS = 32 * WARPS, BATCH = GATED ? 4 : 8;
+};
 
 struct TokenArgs {
   const void* w[2];
@@ -46,7 +52,8 @@ __device__ __forceinline__ uint4 load_once(const void* p) {  // weights: not kep
 }
 
 template <bool GATED, typename T, int ACT>
-__global__ void __launch_bounds__(THREADS) ffn_token_kernel(const __grid_constant__ TokenArgs a) {
+__global__ void __launch_bounds__(Block<GATED>::THREADS) ffn_token_kernel(const __grid_constant__ TokenArgs a) {
+  constexpr int WARPS = Block<GATED>::WARPS, THREADS = Block<GATED>::THREADS, BATCH = Block<GATED>::BATCH;
   constexpr int MATS = GATED ? 2 : 1, SUMS = MATS * ROWS * TOKENS;
   __shared__ float part[WARPS][SUMS];
   __shared__ float total[SUMS];
@@ -138,12 +145,13 @@ __global__ void __launch_bounds__(THREADS) ffn_token_kernel(const __grid_constan
 template <bool GATED, typename T, int ACT>
 int launch_token(TokenArgs& a, const Ffn& f, const char* what) {
   const int tiles = ceil_div(a.rows, ROWS);
-  // clusters where the tiles alone do not fill the SMs; every warp has a batch to load
+  // clusters where the tiles would leave more than half of the SMs idle and every warp has several batches
   a.split = 1;
-  while (a.split < MAX_SPLIT && a.split * tiles < 148 && 2 * a.split * WARPS * BATCH * 32 <= a.K) a.split *= 2;
+  while (a.split < MAX_SPLIT && a.split * tiles < 64 && 2 * a.split * Block<GATED>::WARPS * Block<GATED>::BATCH * 32 <= a.K)
+    a.split *= 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(tiles * a.split);
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(Block<GATED>::THREADS);
   cfg.stream = f.stream;
   cudaLaunchAttribute attr[2]{};
   attr[0].id = cudaLaunchAttributeClusterDimension;
