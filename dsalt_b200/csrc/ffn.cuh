@@ -80,7 +80,7 @@ struct Ffn {
 
 // 16-bit types whose sizes are multiples of 8 and whose operands' rows are 16-byte aligned
 int run_tensor_cores(const Ffn& f, bool backward);
-int forward_tokens(const Ffn& f);  // up to 8 tokens, nothing kept
+int forward_tokens(const Ffn& f);  // up to 16 tokens, nothing kept
 int forward_few(const Ffn& f);     // few tokens, nothing kept
 
 }  // namespace ffn

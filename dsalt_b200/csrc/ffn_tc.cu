@@ -838,11 +838,16 @@ int run_tensor_cores(const Ffn& f, bool back) {
   int dev = 0;
   int rc;
   if ((rc = check_cuda(cudaGetDevice(&dev), "current device")) || (rc = check_cuda(cudaSetDevice(dev), "current device"))) return rc;
-  // Measured (us, weights not in L2), 2048 -> 11008 and 768 -> 2048: a token's path, that of few tokens and
-  // this file's at 8 tokens 41 | 43 | 98 and 14 | 18 | 33, at 16 tokens 49 | 41 | 98 and 14 | 18 | 31; at 256 tokens
-  // the last two 92 | 98 and 33 | 32
-  if (!back && f.keep == DSALT_KEEP_NONE && f.T <= 8) return forward_tokens(f);
-  if (!back && f.keep == DSALT_KEEP_NONE && f.T <= 256) return forward_few(f);
+  // Measured (us, weights not in L2), a stream past tokens | tiles for few tokens | this file, at
+  //   768 -> 2048:  8 tokens 8.3 | 14 | 27; 16 tokens 8.3 | 14 | 27; 32 tokens 14 | 14 | 27; 256 tokens - | 27 | 27
+  //   1024 -> 4096: 8 tokens 10 | 16 | 31; 16 tokens 12 | 17 | 31; 32 tokens 20 | 18 | 31; 256 tokens - | 31 | 31
+  //   2048 -> 11008: 8 tokens 29 | 31 | 72; 16 tokens 36 | 32 | 72; 32 tokens 62 | 33 | 72; 256 tokens - | 81 | 76
+  // Nine to sixteen tokens cost the stream 0.21 us a MB of weights, the tiles 0.14 and 4 us more.
+  if (!back && f.keep == DSALT_KEEP_NONE) {
+    const int64_t weights = (int64_t)f.F * (2 * f.d + f.d_out);
+    if (f.T <= 8 || (f.T <= 16 && weights <= 40000000)) return forward_tokens(f);
+    if (f.T < 256) return forward_few(f);
+  }
   return f.dtype == DSALT_BF16 ? run_typed<__nv_bfloat16>(f, back) : run_typed<__half>(f, back);
 }
 

@@ -1,4 +1,4 @@
-// The gated feed-forward block for up to eight tokens (bf16, fp16): a stream of weights past them.
+// The gated feed-forward block for up to sixteen tokens (bf16, fp16): a stream of weights past them.
 //
 //   h = act(x Wg^T) (x Wu^T), then y = h Wd^T
 //
@@ -15,7 +15,7 @@ namespace dsalt {
 namespace ffn {
 namespace {
 
-constexpr int ROWS = 16, TOKENS = 8, MAX_SPLIT = 8;
+constexpr int ROWS = 16, MAX_SPLIT = 8;
 // The second product has few rows and a long K: twice the warps to a block, each with twice the loads under
 // way, so that one token's weights wait in registers for h and clusters are rarely needed
 template <bool GATED>
@@ -51,12 +51,13 @@ __device__ __forceinline__ uint4 load_once(const void* p) {  // weights: not kep
   return v;
 }
 
-template <bool GATED, typename T, int ACT>
+// NT: groups of 8 tokens
+template <bool GATED, int NT, typename T, int ACT>
 __global__ void __launch_bounds__(Block<GATED>::THREADS) ffn_token_kernel(const __grid_constant__ TokenArgs a) {
   constexpr int WARPS = Block<GATED>::WARPS, THREADS = Block<GATED>::THREADS, BATCH = Block<GATED>::BATCH;
-  constexpr int MATS = GATED ? 2 : 1, SUMS = MATS * ROWS * TOKENS;
+  constexpr int MATS = GATED ? 2 : 1, TOKENS = 8 * NT, SUMS = MATS * ROWS * TOKENS;
   __shared__ float part[WARPS][SUMS];
-  __shared__ float total[SUMS];
+  float* total = part[0];  // of all warps
   if constexpr (GATED) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const int rank = a.split > 1 ? (int)cluster_rank() : 0, f0 = blockIdx.x / a.split * ROWS;
@@ -71,7 +72,7 @@ __global__ void __launch_bounds__(Block<GATED>::THREADS) ffn_token_kernel(const 
     for (int i = 0; i < 2; ++i)  // rows behind the last are read as the last and not stored
       row[m][i] = static_cast<const T*>(a.w[m]) + (int64_t)min(f0 + g + 8 * i, a.rows - 1) * a.K + 8 * t;
 
-  float acc[MATS][4] = {};
+  float acc[MATS][NT][4] = {};
   bool waited = false;
   for (int c0 = lo; c0 < hi; c0 += BATCH) {
     uint4 w[BATCH][MATS][2] = {};
@@ -91,12 +92,16 @@ __global__ void __launch_bounds__(Block<GATED>::THREADS) ffn_token_kernel(const 
     for (int b = 0; b < BATCH; ++b) {
       const int k = (c0 + b) * 32 + 8 * t;
       const bool in = c0 + b < hi && k < a.K;
-      uint4 x = {};
-      if (in && g < a.T) x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + g * a.x_stride + k);
 #pragma unroll
-      for (int m = 0; m < MATS; ++m) {
-        mma_16816<T>(acc[m], w[b][m][0].x, w[b][m][1].x, w[b][m][0].y, w[b][m][1].y, x.x, x.y);
-        mma_16816<T>(acc[m], w[b][m][0].z, w[b][m][1].z, w[b][m][0].w, w[b][m][1].w, x.z, x.w);
+      for (int n = 0; n < NT; ++n) {
+        uint4 x = {};
+        if (in && 8 * n + g < a.T)
+          x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (8 * n + g) * a.x_stride + k);
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) {
+          mma_16816<T>(acc[m][n], w[b][m][0].x, w[b][m][1].x, w[b][m][0].y, w[b][m][1].y, x.x, x.y);
+          mma_16816<T>(acc[m][n], w[b][m][0].z, w[b][m][1].z, w[b][m][0].w, w[b][m][1].w, x.z, x.w);
+        }
       }
     }
   }
@@ -106,7 +111,10 @@ __global__ void __launch_bounds__(Block<GATED>::THREADS) ffn_token_kernel(const 
 #pragma unroll
   for (int m = 0; m < MATS; ++m)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) part[warp][(m * TOKENS + 2 * t + (i & 1)) * ROWS + g + 8 * (i >> 1)] = acc[m][i];
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        part[warp][(m * TOKENS + 8 * n + 2 * t + (i & 1)) * ROWS + g + 8 * (i >> 1)] = acc[m][n][i];
   __syncthreads();
   for (int i = threadIdx.x; i < SUMS; i += THREADS) {
     float v = 0.f;
@@ -142,7 +150,7 @@ __global__ void __launch_bounds__(Block<GATED>::THREADS) ffn_token_kernel(const 
   if (a.split > 1) cluster_sync();  // the others' reads of this block's sums
 }
 
-template <bool GATED, typename T, int ACT>
+template <bool GATED, int NT, typename T, int ACT>
 int launch_token(TokenArgs& a, const Ffn& f, const char* what) {
   const int tiles = ceil_div(a.rows, ROWS);
   // clusters where the tiles would leave more than half of the SMs idle and every warp has several batches
@@ -161,20 +169,25 @@ int launch_token(TokenArgs& a, const Ffn& f, const char* what) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = GATED ? 1 : 2;
-  return check_cuda(cudaLaunchKernelEx(&cfg, ffn_token_kernel<GATED, T, ACT>, a), what);
+  return check_cuda(cudaLaunchKernelEx(&cfg, ffn_token_kernel<GATED, NT, T, ACT>, a), what);
+}
+
+template <int NT, typename T, int ACT>
+int tokens(const Ffn& f) {
+  TokenArgs a{{f.w_gate, f.w_up}, f.x, f.h, f.x_stride, f.pitch, (int)f.T, f.F, f.d, 1};
+  if (int rc = launch_token<true, NT, T, ACT>(a, f, "gated_ffn gate and up launch")) return rc;
+  TokenArgs b{{f.w_down, f.w_down}, f.h, f.y, f.pitch, f.d_out, (int)f.T, f.d_out, f.F, 1};
+  return launch_token<false, NT, T, 0>(b, f, "gated_ffn down launch");
 }
 
 template <typename T, int ACT>
-int tokens(const Ffn& f) {
-  TokenArgs a{{f.w_gate, f.w_up}, f.x, f.h, f.x_stride, f.pitch, (int)f.T, f.F, f.d, 1};
-  if (int rc = launch_token<true, T, ACT>(a, f, "gated_ffn gate and up launch")) return rc;
-  TokenArgs b{{f.w_down, f.w_down}, f.h, f.y, f.pitch, f.d_out, (int)f.T, f.d_out, f.F, 1};
-  return launch_token<false, T, 0>(b, f, "gated_ffn down launch");
+int tokens_n(const Ffn& f) {
+  return f.T <= 8 ? tokens<1, T, ACT>(f) : tokens<2, T, ACT>(f);
 }
 
 template <typename T>
 int tokens_typed(const Ffn& f) {
-  return f.act == DSALT_ACT_SILU ? tokens<T, DSALT_ACT_SILU>(f) : tokens<T, DSALT_ACT_GELU>(f);
+  return f.act == DSALT_ACT_SILU ? tokens_n<T, DSALT_ACT_SILU>(f) : tokens_n<T, DSALT_ACT_GELU>(f);
 }
 
 }  // namespace

@@ -116,6 +116,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) qk_norm_rope_kernel(const __g
     const int64_t t = in ? item / (uint32_t)s.chunks : 0;
     const int h0 = in ? (int)(item - (uint32_t)t * s.chunks) * HEADS : 0;
     const int n = in && held ? min(HEADS, s.heads - h0) : 0;
+    int64_t p = a.pos && n > 0 ? __ldg(a.pos + t) : t;
     const T* x = static_cast<const T*>(s.x) + t * s.x_token + h0 * s.x_head + col;
     uint4 xr[HEADS][2] = {}, dr[HEADS][2] = {};
 #pragma unroll
@@ -135,7 +136,6 @@ __global__ void __launch_bounds__(THREADS, PER_SM) qk_norm_rope_kernel(const __g
     }
     float c[V] = {}, sn[V] = {};
     if (n > 0) {
-      int64_t p = a.pos ? a.pos[t] : t;
       if (p < 0 || p >= a.table_rows) {  // reported, and read as the table's first row
         report_device_error(a.err, 51);
         p = 0;

@@ -7,6 +7,8 @@
 // training step's head norms over 24000 tokens.
 #include <torch/extension.h>
 
+#include <limits>
+
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -189,7 +191,9 @@ Rope rope_args(const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor
     if (positions.dim() != 1 || positions.size(0) != a.T ||
         (positions.scalar_type() != at::kInt && positions.scalar_type() != at::kLong))
       throw py::value_error(words("positions must be [", a.T, "] whole numbers"));
-    a.positions = positions.to(at::kInt).contiguous();
+    if (positions.scalar_type() == at::kLong)  // what 32 bits do not hold stays outside the tables
+      a.positions = positions.clamp(-1, std::numeric_limits<int32_t>::max()).to(at::kInt);
+    a.positions = a.positions.contiguous();
     if (cos.size(0) == 0 && a.T) throw py::value_error("empty tables");
   } else if (cos.size(0) < a.T) {
     throw py::value_error(words("tables of ", cos.size(0), " rows for ", a.T, " tokens"));

@@ -256,6 +256,9 @@ def test_rope_position_outside_the_tables_is_reported(Y):
     got = Y.qk_norm_rope(q, k, cos, sin, positions=torch.tensor([8, 7, -1], device="cuda"))
     assert ops.device_status() == 51 and ops.device_status() == 0
     assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    far = torch.tensor([1 << 32, 7, -(1 << 40)], device="cuda")   # not what 32 bits would make of them
+    got = Y.qk_norm_rope(q, k, cos, sin, positions=far)
+    assert ops.device_status() == 51 and all(torch.equal(a, b) for a, b in zip(got, ref))
 
 
 def test_rope_refusals(Y):
@@ -380,7 +383,9 @@ def ffn_inputs(T, d, F, d_out, dtype, seed=0):
 @pytest.mark.parametrize("T,d,F,d_out,act", [
     (1, 64, 96, 64, "silu"), (1, 8, 8, 8, "gelu"), (3, 72, 40, 24, "silu"), (17, 256, 768, 256, "gelu"),
     (64, 512, 1408, 512, "silu"), (127, 128, 136, 200, "silu"), (300, 264, 520, 136, "gelu"), (513, 768, 2048, 768, "silu"),
-    (1000, 200, 328, 200, "silu"), (2500, 512, 1408, 512, "silu"), (4100, 264, 2824, 520, "gelu")])
+    (1000, 200, 328, 200, "silu"), (2500, 512, 1408, 512, "silu"), (4100, 264, 2824, 520, "gelu"),
+    (8, 520, 264, 1032, "silu"), (9, 1024, 2816, 72, "gelu"), (16, 200, 5504, 520, "silu"), (255, 72, 4104, 264, "silu"),
+    (256, 1032, 520, 520, "gelu"), (40, 2056, 1000, 2048, "silu"), (6000, 72, 200, 72, "silu"), (1100, 256, 4104, 256, "silu")])
 def test_ffn_matches_the_oracle(Y, dtype, keep, T, d, F, d_out, act):
     x, wg, wu, wd, dy = ffn_inputs(T, d, F, d_out, TYPES[dtype])
     check_ffn(Y, x, wg, wu, wd, act, keep, dy)
