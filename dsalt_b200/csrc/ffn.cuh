@@ -1,4 +1,4 @@
-// Shared by the kernels of the gated feed-forward block (ffn.cu, ffn_tc.cu).
+// Shared by the kernels of the gated feed-forward block (ffn.cu, ffn_tc.cu, ffn_few.cu, ffn_token.cu).
 #pragma once
 
 #include "pack8.cuh"
@@ -21,7 +21,7 @@ __device__ __forceinline__ float sigmoid(float g) { return reciprocal(1.f + ex2_
 // added up with others of the size of u): p by Hastings' approximation (Abramowitz and Stegun 7.1.26),
 // off by 7.5e-8 at most, with the exponential that the derivative needs as well; CUDA's function, which
 // keeps the relative error of far negative g, takes about three times the instructions (first epilogue of
-// 1999 x 768 -> 2048: 30 us against 25).
+// 1999 x 768 -> 2048: 30 us against 20).
 __device__ __forceinline__ float share_below(float g, float e) {  // e = exp(-g^2 / 2)
   const float t = reciprocal(fmaf(0.3275911f * 0.70710678f, fabsf(g), 1.f));
   const float tail =

@@ -18,7 +18,10 @@
 //
 // Bound by what an SM can take from L2, 64 bytes a cycle: a stage of 32 KB feeds 512 cycles of products, so
 // at the tensor cores' full rate the operands alone fill that path (85 to 90 % of the rate is reached),
-// and what an epilogue writes and reads (up to 6 and 4 bytes for each of T x d_ff values) comes on top.
+// and what an epilogue writes and reads (up to 6 and 4 bytes for each of T x d_ff values) comes on top. Long runs
+// are bound by the power limit, under which the clock falls from 1.9 to 1.4 GHz. Measured, bf16: 32768 x 2048 ->
+// 11008 forward 2.79 ms (1590 TFLOP/s) cold and 3.13 ms (1420) in a row; 32768 x 768 -> 2048 forward, 16 bits kept,
+// and backward 692 us (1340 TFLOP/s); 16384 x 1024 -> 4096, 8 bits kept, 944 us (1310); 1999 x 768 -> 2048 33 us.
 #include "ffn_tc.cuh"
 
 namespace dsalt {
@@ -115,9 +118,10 @@ __device__ __forceinline__ void pair_commit(uint64_t* bar, uint32_t leader) {
 // What an epilogue keeps in shared memory, and the stages that this leaves for the operands. The first
 // product's writes its rows from registers. A plain store stages its output for the store engine, in four
 // sets of boxes. The backward's has what was kept brought in by the load engine, a warp's 32 rows x 32
-// columns of gate and of up at a time, three of them under way (read row by row by the threads it took
-// 165 us at 32768 x 768 -> 2048, 148 so); codes of 16 bits are replaced by
-// the gradients where they lie, codes of 8 have a set of boxes for three outputs besides.
+// columns of gate and of up at a time, three of them under way (hidden gradients of
+// 32768 x 768 -> 2048: read row by row by the threads 165 us, so 148, and 123 since accumulators are given back
+// early); codes of 16 bits are replaced by the gradients where they lie, codes of 8 have a set of boxes for three
+// outputs besides.
 template <int EPI, int KEEP>
 struct Shape {
   static constexpr bool IN_PLACE = EPI == GRADS && KEEP == DSALT_KEEP_INPUT;
@@ -638,7 +642,8 @@ void size_job(Job& j, int64_t M, int64_t N, int64_t K, int tile_n) {
 
 // Where a plain store's tiles leave half of the pairs idle, K is split over 2 to 4 pairs of a cluster, as far as
 // all clusters run at once: of 4, 6 and 8 CTAs of this size the GPU holds 33, 22 and 15 (its processing
-// clusters have odd numbers of SMs left over). 24 tiles of K = 2048: two parts 12 us, three 25, one 16.
+// clusters have odd numbers of SMs left over). 1999 x 768 -> 2048 (24 tiles of
+// K = 2048 in the second product), both launches: one part 40 us, two 33, three 43.
 int split_for(int tiles, int blocks) {
   constexpr int AT_ONCE[5] = {0, PAIRS, 33, 22, 15};
   int split = 1;
