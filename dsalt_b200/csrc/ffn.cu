@@ -1,7 +1,8 @@
 // The gated feed-forward block y = (act(x Wg^T) * (x Wu^T)) Wd^T and its gradients
 // (dsalt_gated_ffn, dsalt_gated_ffn_bwd): arguments, workspaces, and the path for what the tensor
-// cores do not take: fp32 inputs, and sizes that are not multiples of 8. That path is plain: products on the CUDA cores in fp32 (128 x 128 tiles, 8 x 8 outputs a thread), the
-// activation and its gradient as kernels of their own between them.
+// cores do not take: fp32 inputs, and sizes that are not multiples of 8. That path is plain: products on the
+// CUDA cores in fp32 (128 x 128 tiles, 8 x 8 outputs a thread), the activation and its gradient as kernels of their
+// own between them.
 #include "ffn.cuh"
 
 namespace dsalt {

@@ -71,6 +71,14 @@ void no_second_derivative() {
   TORCH_CHECK(!at::GradMode::is_enabled(), "dsalt_b200 operators have no second derivative");  // create_graph=True
 }
 
+// A tensor that was kept for the backward pass: hooks on saved tensors may give back one of other strides, which is
+// copied; anything else is an error.
+Tensor saved(const Tensor& t, const char* name, at::ScalarType type, at::IntArrayRef shape, c10::Device dev) {
+  TORCH_CHECK(t.defined() && t.device() == dev && t.scalar_type() == type && t.sizes() == shape, "the saved ", name,
+              " came back as another tensor");
+  return t.is_contiguous() ? t : t.contiguous();
+}
+
 // The tensor's device as the current one, and its current stream, while a call is made
 struct Launch {
   c10::cuda::CUDAGuard guard;
@@ -222,15 +230,20 @@ struct RopeNode : torch::autograd::Function<RopeNode> {
                                const Rope& a, double eps) {
     ctx->save_for_backward({q, k, a.q_weight, a.k_weight, a.cos, a.sin, a.positions});
     ctx->saved_data["eps"] = eps;
-    ctx->saved_data["stride"] = a.stride;
     return rope_forward(q, k, a, eps);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     no_second_derivative();
     const variable_list s = ctx->get_saved_variables();
-    const Tensor &q = s[0], &k = s[1], &q_weight = s[2], &k_weight = s[3], &cos = s[4], &sin = s[5], &positions = s[6];
-    const c10::Device dev = q.device();
-    const int64_t T = q.size(0), H = q.size(1), D = q.size(2), Hk = k.size(1);
+    const Tensor &q = s[0], &k = s[1];
+    TORCH_CHECK(q.defined() && k.defined() && s[4].defined() && s[5].defined() && q.dim() == 3 && k.dim() == 3 &&
+                    (!grads[0].defined() || grads[0].sizes() == q.sizes()) &&
+                    (!grads[1].defined() || grads[1].sizes() == k.sizes()),
+                "the saved heads came back as other tensors");
+    const Rope a = rope_args(q, k, s[4], s[5], s[6], s[2], s[3]);
+    const Tensor &q_weight = a.q_weight, &k_weight = a.k_weight, &cos = a.cos, &sin = a.sin, &positions = a.positions;
+    const c10::Device dev = a.dev;
+    const int64_t T = a.T, H = a.H, D = a.D, Hk = a.Hk;
     const bool norm = q_weight.defined();
     Tensor dq = empty({T, H, D}, q.scalar_type(), dev), dk = empty({T, Hk, D}, q.scalar_type(), dev), dwq, dwk, ws;
     if (norm) {
@@ -246,7 +259,7 @@ struct RopeNode : torch::autograd::Function<RopeNode> {
                                  (int)Hk, (int)D, x.token, x.head, y.token, y.head, gx.token, gx.head, gy.token, gy.head,
                                  ptr(q_weight), ptr(k_weight), norm ? type_code(q_weight) : 0,
                                  (float)ctx->saved_data["eps"].toDouble(), cos.data_ptr<float>(), sin.data_ptr<float>(),
-                                 std::max<int64_t>(cos.size(0), 1), ctx->saved_data["stride"].toInt(),
+                                 std::max<int64_t>(cos.size(0), 1), a.stride,
                                  static_cast<const int32_t*>(ptr(positions)), dq.data_ptr(), dk.data_ptr(), ptr(dwq), ptr(dwk),
                                  ptr(ws), norm ? (size_t)ws.numel() : 0, launch.stream),
           "dsalt_qk_norm_rope_bwd");
@@ -348,29 +361,50 @@ struct FfnNode : torch::autograd::Function<FfnNode> {
     if (!w_gate.requires_grad() && !w_up.requires_grad()) m = Tensor();  // only their gradients read it
     else if (keep == DSALT_KEEP_8BIT && m.numel()) std::tie(m, x_exps) = pack_rows(m, stride, a.dev);
     ctx->save_for_backward({m, x_exps, k.kept, k.exps, wg, wu, wd});
-    ctx->saved_data["stride"] = stride;
     ctx->saved_data["act"] = act;
     ctx->saved_data["keep"] = keep;
     ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["d_ff"] = a.F;
     return {k.y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     no_second_derivative();
     const variable_list s = ctx->get_saved_variables();
-    const Tensor &x = s[0], &x_exps = s[1], &kept = s[2], &exps = s[3], &wg = s[4], &wu = s[5], &wd = s[6];
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
-    const c10::Device dev = wg.device();
-    const int64_t T = kept.size(1), F = wg.size(0), d = wg.size(1), d_out = wd.size(0);
-    const int keep = (int)ctx->saved_data["keep"].toInt(), dt = type_code(wg);
+    const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+    const int64_t F = ctx->saved_data["d_ff"].toInt(), d = shape.back(), d_out = grads[0].size(-1);
+    const int64_t T = d_out ? grads[0].numel() / d_out : 0, pitch = dsalt_gated_ffn_pitch((int)F);
+    const int keep = (int)ctx->saved_data["keep"].toInt();
+    const bool coded = keep == DSALT_KEEP_8BIT;
+    const c10::Device dev = grads[0].device();
+    const at::ScalarType type = grads[0].scalar_type();
+    const int dt = type_code(grads[0]);
+    const Tensor kept = saved(s[2], "activations", coded ? at::kChar : type, {coded ? 2 : 3, T, pitch}, dev);
+    const Tensor wg = ffn_weight(saved(s[4], "gate weight", type, {F, d}, dev)),
+                 wu = ffn_weight(saved(s[5], "up weight", type, {F, d}, dev)),
+                 wd = ffn_weight(saved(s[6], "down weight", type, {d_out, F}, dev));
+    Tensor x, x_exps, exps;
+    if (coded || type != at::kFloat) exps = saved(s[3], "scales", at::kByte, {2, pitch / GROUP, T}, dev);
+    int64_t x_stride = d;
+    if (s[0].defined()) {
+      if (coded && T) {
+        x = saved(s[0], "codes", at::kChar, {T, d}, dev);
+        x_exps = saved(s[1], "scales", at::kByte, {T, (d + GROUP - 1) / GROUP}, dev);
+      } else {
+        TORCH_CHECK(s[0].device() == dev && s[0].scalar_type() == type && s[0].dim() == 2 && s[0].size(0) == T && s[0].size(1) == d,
+                    "the saved input came back as another tensor");
+        std::tie(x, x_stride) = ffn_rows(s[0]);
+      }
+    }
     const auto [dy, dy_stride] = ffn_rows(grads[0].reshape({T, d_out}));
     Tensor dx, dwg, dwu, dwd;
-    if (ctx->needs_input_grad(0)) dx = empty(ctx->saved_data["shape"].toIntVector(), wg.scalar_type(), dev);
+    if (ctx->needs_input_grad(0)) dx = empty(shape, type, dev);
     const bool both = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
-    if (both) dwg = empty({F, d}, wg.scalar_type(), dev), dwu = empty({F, d}, wg.scalar_type(), dev);
-    if (ctx->needs_input_grad(3)) dwd = empty({d_out, F}, wg.scalar_type(), dev);
+    if (both) dwg = empty({F, d}, type, dev), dwu = empty({F, d}, type, dev);
+    if (ctx->needs_input_grad(3)) dwd = empty({d_out, F}, type, dev);
     const Tensor ws = workspace(dsalt_gated_ffn_bwd_workspace_bytes(dt, T, (int)d, (int)F, (int)d_out, keep), dev);
     const Launch launch(dev);
-    check(dsalt_gated_ffn_bwd(dy.data_ptr(), dt, T, (int)d, dy_stride, ptr(x), ctx->saved_data["stride"].toInt(),
+    check(dsalt_gated_ffn_bwd(dy.data_ptr(), dt, T, (int)d, dy_stride, ptr(x), x_stride,
                               static_cast<const uint8_t*>(ptr(x_exps)), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), (int)F,
                               (int)d_out, (int)ctx->saved_data["act"].toInt(), keep, kept.data_ptr(),
                               static_cast<const uint8_t*>(ptr(exps)), ptr(dx), ptr(dwg), ptr(dwu), ptr(dwd), ws.data_ptr(),

@@ -2,6 +2,7 @@
 views, missing gradients, streams, captured steps, autocast, long axes, the decoder stack."""
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from oracle import layers_oracle as O
 
@@ -152,6 +153,63 @@ def test_a_weight_changed_between_forward_and_backward_is_noticed(Y):
         leaves[3].add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+# ------------------------------------------------------------------ saved tensors that others handle
+def ffn_step(Y, keep):
+    """A training step whose input is a view of rows wider than it has."""
+    g = gen(31)
+    wide = normal(g, 300, 200).requires_grad_(True)
+    weights = [t.requires_grad_(True) for t in ffn_leaves(g, 1, 64, 104)[1:]]
+    dy = normal(g, 300, 64)
+    return [wide, *weights], lambda: (Y.gated_ffn(wide[:, 72:136], *weights, keep=keep),), (dy,)
+
+
+def rope_step(Y, dtype):
+    """Heads that are views of one projection, tables that are views of wider ones."""
+    g = gen(32)
+    qkv = normal(g, 65, 6, 32, dtype=dtype).requires_grad_(True)
+    w = [(torch.rand(32, device="cuda", generator=g) + 0.5).requires_grad_(True) for _ in range(2)]
+    angles = normal(g, 90, 48, dtype=torch.float32)
+    pos = torch.randint(0, 90, (65,), device="cuda", generator=g)
+    call = lambda: Y.qk_norm_rope(qkv[:, :4], qkv[:, 4:5], angles[:, :32].cos(), angles[:, 16:].sin(), positions=pos,  # noqa: E731
+                                  q_weight=w[0], k_weight=w[1])
+    return [qkv, *w], call, (normal(g, 65, 4, 32, dtype=dtype), normal(g, 65, 1, 32, dtype=dtype))
+
+
+STEPS = [(ffn_step, "16bit"), (ffn_step, "8bit"), (rope_step, torch.bfloat16), (rope_step, torch.float32)]
+
+
+@pytest.mark.parametrize("make,kind", STEPS)
+def test_backward_from_saved_tensors_of_other_strides(Y, make, kind):
+    leaves, call, douts = make(Y, kind)
+    ref = torch.autograd.grad(call(), leaves, douts)
+    with torch.autograd.graph.save_on_cpu():  # they come back contiguous
+        out = call()
+    got = torch.autograd.grad(out, leaves, douts)
+    again = torch.autograd.grad(torch.utils.checkpoint.checkpoint(lambda: call(), use_reentrant=False), leaves, douts)
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(ref, got, again))
+
+
+@pytest.mark.parametrize("make,kind", STEPS)
+@pytest.mark.parametrize("spoil", [lambda t: t.cpu(), lambda t: t.narrow(0, 0, t.shape[0] - 1), lambda t: t.double()],
+                         ids=["elsewhere", "shorter", "wider"])
+def test_backward_from_other_saved_tensors_is_refused(Y, make, kind, spoil):
+    leaves, call, douts = make(Y, kind)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: spoil(t)):
+        out = call()
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, leaves, douts)
+    assert status() == 0
+
+
+@pytest.mark.parametrize("make,kind", STEPS)
+def test_a_second_backward_pass_of_one_graph_is_the_first_again(Y, make, kind):
+    leaves, call, douts = make(Y, kind)
+    out = call()
+    first = torch.autograd.grad(out, leaves, douts, retain_graph=True)
+    second = torch.autograd.grad(out, leaves, douts)
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
 
 
 # ------------------------------------------------------------------ streams and captured steps
