@@ -8,7 +8,7 @@
 // and a long K: the CTAs of a cluster share 128 rows and take equal parts of K, and add up their fp32 sums
 // through each other's shared memory in the order of their ranks (results repeat bit for bit). It is
 // launched while the first one runs and asks for its first weights before it waits for h. 64 tokens, 2048 ->
-// 11008 in bf16 (135 MB of weights): 36 us in a row, 3.8 TB/s; memory's own rate gives 21.
+// 11008 in bf16 (135 MB of weights): 33 us in a row, 4.1 TB/s; memory's own rate gives 21.
 #include "ffn_tc.cuh"
 
 namespace dsalt {
@@ -16,6 +16,7 @@ namespace ffn {
 namespace {
 
 constexpr int ROWS = 128, KB = 64, THREADS = 128, MAX_STAGES = 12, MAX_SPLIT = 8, MAX_SMEM = 226 * 1024;
+constexpr int HALF_SMEM = 228 * 1024 / 2 - 1024 - 256;  // of two CTAs an SM, beside what each keeps for itself
 
 struct FewArgs {
   CUtensorMap w[2], x;      // weights (gate's and up's, or one twice) and tokens
@@ -38,6 +39,12 @@ struct FewBars {
 __device__ __forceinline__ float2 load_peer2(uint32_t addr) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ float2 load_own2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
   return v;
 }
 
@@ -142,15 +149,27 @@ __global__ void __launch_bounds__(THREADS) ffn_few_kernel(const __grid_constant_
   if constexpr (GATED) __syncthreads();
   else cluster_sync();
 
-  for (int t = rank * 4 + warp; t < here; t += 4 * a.split) {
-    T* out = static_cast<T*>(a.out) + (t0 + t) * a.out_stride + f0;
-    if constexpr (GATED) {  // all of K is here
-      const int r = 2 * lane;
-      if (r < a.box && f0 + r < a.rows) {
-        const float2 g = load_peer2(base + (t * ROWS + r) * 4), u = load_peer2(base + (t * ROWS + a.box + r) * 4);
-        *reinterpret_cast<uint32_t*>(out + r) = narrow2<T>(activate<ACT, true>(g.x) * u.x, activate<ACT, true>(g.y) * u.y);
+  if constexpr (GATED) {  // all of K is here
+    constexpr int BATCH = 4;  // tokens whose sums are asked for at once
+    const int r = 2 * lane;
+    if (r < a.box && f0 + r < a.rows)
+      for (int t = warp; t < here; t += 4 * BATCH) {
+        float2 g[BATCH], u[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+          if (t + 4 * i < here) {
+            g[i] = load_own2(base + ((t + 4 * i) * ROWS + r) * 4);
+            u[i] = load_own2(base + ((t + 4 * i) * ROWS + a.box + r) * 4);
+          }
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+          if (t + 4 * i < here)
+            *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (t0 + t + 4 * i) * a.out_stride + f0 + r) =
+                narrow2<T>(activate<ACT, true>(g[i].x) * u[i].x, activate<ACT, true>(g[i].y) * u[i].y);
       }
-    } else {
+  } else {
+    for (int t = rank * 4 + warp; t < here; t += 4 * a.split) {
+      T* out = static_cast<T*>(a.out) + (t0 + t) * a.out_stride + f0;
       float2 v[2][MAX_SPLIT];
 #pragma unroll
       for (int c = 0; c < MAX_SPLIT; ++c)
@@ -172,11 +191,22 @@ __global__ void __launch_bounds__(THREADS) ffn_few_kernel(const __grid_constant_
 }
 
 // ---------------------------------------------------------------- host side
-// how a product of `rows` features, T tokens and K is cut: tiles of weights and of tokens, parts of K, stages
+// How a product of `rows` features, T tokens and K is cut: tiles of weights and of tokens, parts of K, stages.
+//
+// Two CTAs an SM, where the sums leave room for that: the second product's first loads, and clusters of eight,
+// find room beside others (one CTA an SM with twice the stages took 16 % longer at 64 tokens, 2048 -> 11008).
+// Tokens are cut as finely as lets all CTAs run at once, to 48 (second product: 64) of them: weights that several CTAs read
+// come from L2, and what a CTA does for each of its tokens after its products is seen by nobody else. (One tile
+// of up to 256 tokens | so cut, us: 64 tokens 768 -> 2048 13.9 | 12.6, 128 tokens 1024 -> 4096 20.8 | 17.8, 192
+// tokens 2048 -> 5504 44 | 29, 128 tokens 2048 -> 11008 41 | 36.4.)
 void cut(FewArgs& a, bool gated, int rows, int64_t T, int K, int& tiles, int& token_tiles) {
   constexpr int SMS = 148;
-  token_tiles = ceil_div(T, 256);
+  tiles = ceil_div(rows, gated ? ROWS / 2 : ROWS);
+  const int most = 2 * SMS / tiles, wanted = ceil_div(T, gated ? 48 : 64), least = ceil_div(T, 256);
+  token_tiles = wanted < most ? wanted : most;
+  if (token_tiles < least) token_tiles = least;
   a.tokens = ceil_div(ceil_div(T, token_tiles), 16) * 16;
+  token_tiles = ceil_div(T, a.tokens);
   a.tmem_cols = 32;
   while ((int)a.tmem_cols < a.tokens) a.tmem_cols *= 2;
   a.rows = rows;
@@ -184,23 +214,25 @@ void cut(FewArgs& a, bool gated, int rows, int64_t T, int K, int& tiles, int& to
   a.box = ROWS / 2;
   a.split = 1;
   if (gated) {
-    // an SM reads its tiles' weights from memory and the tokens, at about twice the rate, from L2
+    // An SM reads its tiles' weights from memory and the tokens, at about twice the rate, from L2; each two
+    // tiles that it works on at once have a start and an end besides, of some thousand cycles (here in rows of
+    // weights, which take K / 12 cycles each)
     int best = 1 << 30;
     for (int box = ROWS / 2; box >= 8; box -= 8) {
-      const int cost = ceil_div((int64_t)ceil_div(rows, box) * token_tiles, SMS) * (2 * box + a.tokens / 2);
+      const int n = ceil_div((int64_t)ceil_div(rows, box) * token_tiles, SMS);
+      const int cost = n * (2 * box + a.tokens / 2) + (n + 1) / 2 * ((2000 + 15 * a.tokens) * 12 / K);
       if (cost < best) best = cost, a.box = box;
     }
     tiles = ceil_div(rows, a.box);
   } else {
-    tiles = ceil_div(rows, ROWS);
-    while (a.split < MAX_SPLIT && 2 * a.split * tiles * token_tiles <= 2 * SMS && 8 * a.split <= a.blocks) a.split *= 2;
+    // clusters that all run at once: 36 of 8 or 72 of 4, two CTAs an SM, do not (16 us against 21 at 384 tokens,
+    // 768 -> 2048)
+    while (a.split < MAX_SPLIT && 2 * a.split * tiles * token_tiles <= 256 && 8 * a.split <= a.blocks) a.split *= 2;
   }
-  // Two CTAs an SM, where the sums leave room for that: the second product's first loads, and clusters of
-  // eight, find room beside others (one CTA an SM with twice the stages: 57 us against 49 at 64 tokens, 2048 ->
-  // 11008, weights not in L2, when this was chosen; 47 since). The products read 128 rows from the start of the last stage on; the stages later hold the sums.
+  // the products read 128 rows from the start of the last stage on; the stages later hold the sums
   const int stage = (2 * a.box + a.tokens) * KB * 2, behind = (ROWS - 2 * a.box) * KB * 2, sums = a.tokens * ROWS * 4;
-  const bool two = 1024 + behind + (sums > 3 * stage ? sums : 3 * stage) <= MAX_SMEM / 2;
-  a.stages = ((two ? MAX_SMEM / 2 : MAX_SMEM) - 1024 - behind) / stage;
+  const bool two = 1024 + (sums > 2 * stage + behind ? sums : 2 * stage + behind) <= HALF_SMEM;
+  a.stages = ((two ? HALF_SMEM : MAX_SMEM) - 1024 - behind) / stage;
   a.stages = a.stages < MAX_STAGES ? a.stages : MAX_STAGES;
   a.smem = 1024 + a.stages * stage + behind;
   if (a.smem < 1024 + sums) a.smem = 1024 + sums;

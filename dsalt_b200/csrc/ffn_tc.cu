@@ -843,15 +843,19 @@ int run_tensor_cores(const Ffn& f, bool back) {
   int dev = 0;
   int rc;
   if ((rc = check_cuda(cudaGetDevice(&dev), "current device")) || (rc = check_cuda(cudaSetDevice(dev), "current device"))) return rc;
-  // Measured (us, weights not in L2), a stream past tokens | tiles for few tokens | this file, at
-  //   768 -> 2048:  8 tokens 8.3 | 14 | 27; 16 tokens 8.3 | 14 | 27; 32 tokens 14 | 14 | 27; 256 tokens - | 27 | 27
-  //   1024 -> 4096: 8 tokens 10 | 16 | 31; 16 tokens 12 | 17 | 31; 32 tokens 20 | 18 | 31; 256 tokens - | 31 | 31
-  //   2048 -> 11008: 8 tokens 29 | 31 | 72; 16 tokens 36 | 32 | 72; 32 tokens 62 | 33 | 72; 256 tokens - | 81 | 76
-  // Nine to sixteen tokens cost the stream 0.21 us a MB of weights, the tiles 0.14 and 4 us more.
+  // Measured (us in a row, weights not in L2), a stream past tokens | tiles for few tokens | this file, at
+  //   512 -> 1408:   256 tokens - | 12.7 | 20; 1024 tokens - | 15.6 | 21; 1536 - | 19 | 22; 2560 - | 27 | 25
+  //   768 -> 2048:   16 tokens 7.5 | 11.7 | 21; 64 tokens - | 12.6 | 21; 256 - | 15.6 | 23; 1024 - | 22 | 25; 1536 - | 31 | 28
+  //   1024 -> 4096:  16 tokens 10.4 | 14.8 | 25; 64 tokens - | 15.9 | 26; 256 - | 20 | 26; 512 - | 24 | 28; 896 - | 42 | 35
+  //   2048 -> 5504:  64 tokens - | 24 | 34; 256 - | 32 | 35; 384 - | 39 | 46; 544 - | 61 | 49
+  //   2048 -> 11008: 16 tokens 36 | 29.7 | 54; 64 tokens - | 33 | 54; 192 - | 45 | 54; 224 - | 58 | 54
+  //   4096 -> 28672: 64 tokens - | 131 | 169; 128 - | 139 | 170; 160 - | 175 | 171
+  // Nine to sixteen tokens cost the stream 0.21 us a MB of weights, the tiles 0.14 and 4 us more. The tiles win
+  // while their CTAs run at once, two an SM with some 128 tokens each: that is T d_ff.
   if (!back && f.keep == DSALT_KEEP_NONE) {
     const int64_t weights = (int64_t)f.F * (2 * f.d + f.d_out);
     if (f.T <= 8 || (f.T <= 16 && weights <= 40000000)) return forward_tokens(f);
-    if (f.T < 256) return forward_few(f);
+    if (f.T <= 128 || (f.T <= 2048 && f.T * f.F <= 2300000)) return forward_few(f);
   }
   return f.dtype == DSALT_BF16 ? run_typed<__nv_bfloat16>(f, back) : run_typed<__half>(f, back);
 }

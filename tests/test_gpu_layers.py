@@ -391,6 +391,17 @@ def test_ffn_matches_the_oracle(Y, dtype, keep, T, d, F, d_out, act):
     check_ffn(Y, x, wg, wu, wd, act, keep, dy)
 
 
+# where the forms without gradients meet, and where they are cut differently
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,d,F,d_out", [
+    (48, 136, 1032, 72), (49, 136, 1032, 72), (64, 136, 1032, 2048), (65, 136, 1032, 2048), (128, 72, 19000, 64),
+    (129, 72, 19000, 64), (193, 1024, 1048, 264), (640, 200, 1048, 264), (208, 72, 11008, 136), (209, 72, 11008, 136),
+    (2048, 200, 1048, 264), (2049, 200, 1048, 264), (300, 64, 264, 9000), (1500, 2048, 8, 8)])
+def test_ffn_at_the_borders_of_its_forms(Y, dtype, T, d, F, d_out):
+    x, wg, wu, wd, dy = ffn_inputs(T, d, F, d_out, TYPES[dtype])
+    check_ffn(Y, x, wg, wu, wd, "silu", "16bit", dy)
+
+
 @pytest.mark.parametrize("dtype,keep", [("bf16", "16bit"), ("fp16", "8bit"), ("fp32", "8bit")])
 @pytest.mark.parametrize("T,d,F,d_out", [(5, 7, 9, 3), (130, 33, 65, 129), (2, 64, 100, 64), (9, 65, 64, 64)])
 def test_ffn_of_odd_sizes(Y, dtype, keep, T, d, F, d_out):
