@@ -58,7 +58,8 @@ def _build_torch_side() -> None:
     from torch.utils.cpp_extension import include_paths, library_paths
     cuda = os.path.dirname(os.path.dirname(nvcc()))
     include = [*include_paths(), sysconfig.get_path("include"), os.path.join(cuda, "include")]
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_torch_layers",
+    # the g++ that nvcc takes too: another one may link a C++ library of its own beside torch's
+    cmd = [shutil.which("g++") or os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_torch_layers",
            "-D_GLIBCXX_USE_CXX11_ABI=1", *[a for p in include for a in ("-isystem", p)], "-I", os.path.join(ROOT, "include"),
            TORCH_SOURCE, "-o", TORCH_LIB + ".tmp", "-L" + OUT_DIR, "-ldsalt_b200", "-Wl,-rpath,$ORIGIN",
            *["-L" + p for p in library_paths()], "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]

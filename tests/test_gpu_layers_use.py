@@ -320,6 +320,26 @@ def test_pack_beyond_32_bit_offsets(Y):
     assert torch.equal(back[-1].double(), O.held(x[-1:].double())[0]) and torch.equal(back[0], back[-2])
 
 
+def test_rope_beyond_32_bit_offsets(Y):
+    g = gen(27)
+    T, H, D = 270_000, 32, 256  # 2.2e9 values
+    q = torch.empty(T, H, D, device="cuda", dtype=torch.bfloat16).normal_(generator=g).requires_grad_(True)
+    k = normal(g, T, 1, D).requires_grad_(True)
+    angles, pos = normal(g, 50, D // 2, dtype=torch.float32), torch.arange(T, device="cuda", dtype=torch.int32) % 50
+    w = [(torch.rand(D, device="cuda", generator=g) + 0.5) for _ in range(2)]
+
+    def step(rows):
+        out = Y.qk_norm_rope(q[rows], k[rows], angles.cos(), angles.sin(), positions=pos[rows], q_weight=w[0], k_weight=w[1])
+        return (*out, *torch.autograd.grad(out, (q, k), (q.detach()[rows].flip(1), k.detach()[rows])))
+
+    all_of_it = step(slice(None))
+    for rows in (slice(T - 100, None), slice(262_100, 262_200)):  # behind 2^31 values, across them
+        alone = step(rows)
+        assert all(torch.equal(a[rows], b) for a, b in zip(all_of_it[:2], alone[:2]))
+        assert all(torch.equal(a[rows], b[rows]) for a, b in zip(all_of_it[2:], alone[2:]))
+    assert status() == 0
+
+
 # ------------------------------------------------------------------ registered forms
 def test_opcheck_registered_forms():
     import dsalt_b200  # noqa: F401
