@@ -20,7 +20,7 @@
 // at the tensor cores' full rate the operands alone fill that path (85 to 90 % of the rate is reached),
 // and what an epilogue writes and reads (up to 6 and 4 bytes for each of T x d_ff values) comes on top. Long runs
 // are bound by the power limit, under which the clock falls from 1.9 to 1.4 GHz. Measured, bf16: 32768 x 2048 ->
-// 11008 forward 2.79 ms (1590 TFLOP/s) cold and 3.13 ms (1420) in a row; 32768 x 768 -> 2048 forward, 16 bits kept,
+// 11008 forward 2.76 ms (1610 TFLOP/s) cold and 3.13 to 3.25 ms (1360 to 1420) in a row; 32768 x 768 -> 2048 forward, 16 bits kept,
 // and backward 692 us (1340 TFLOP/s); 16384 x 1024 -> 4096, 8 bits kept, 944 us (1310); 1999 x 768 -> 2048 33 us.
 #include "ffn_tc.cuh"
 
@@ -35,7 +35,7 @@ constexpr int BOX = 32, BOX_BYTES = 32 * BOX * 2;  // a warp's staged outputs: 3
 constexpr int EPI_WARPS = 8, THREADS = 32 * (4 + EPI_WARPS);  // 16 warps in the first epilogue: no faster
 constexpr uint32_t TMEM_COLS = 512;
 constexpr int PAIRS = 74;  // of SMs
-constexpr int GROUP_M = 4;  // tiles of 256 rows whose A stays in L2 while N is walked; 1 to 16 differ by 2 %
+constexpr int64_t HALF_L2 = 60 << 20;
 
 enum Order { ALONG = 0, ACROSS = 1, BY_JOB = 2 };  // how K of A lies: along its rows, across them
 enum Epilogue { PLAIN = 0, GATE_UP = 1, GRADS = 2 };
@@ -44,6 +44,7 @@ struct alignas(64) Job {
   CUtensorMap a[2], b[2];  // of both segments of K; the first product: gate's and up's rows
   CUtensorMap c[3];
   int tiles_m, tiles_n, blocks0, blocks;  // blocks of K in the first segment and in all
+  int group;                              // tiles of 256 rows whose A stays in L2 while N is walked
   int rows, cols;                         // of the outputs
   int a_across;                           // K of A lies across its rows (where jobs differ)
   void* out;                              // of c[0], for a plain store's sums of several parts
@@ -166,8 +167,8 @@ __device__ __forceinline__ Tile find_tile(const Args<NJ>& a, int t) {
     }
   }
   const int tm = a.job[j].tiles_m, tn = a.job[j].tiles_n;
-  const int group = t / (GROUP_M * tn), first = group * GROUP_M, rows = min(GROUP_M, tm - first);
-  const int r = t - group * GROUP_M * tn;
+  const int high = a.job[j].group, group = t / (high * tn), first = group * high, rows = min(high, tm - first);
+  const int r = t - group * high * tn;
   return {j, first + r % rows, r / rows};
 }
 
@@ -636,6 +637,12 @@ void size_job(Job& j, int64_t M, int64_t N, int64_t K, int tile_n) {
   j.tiles_m = ceil_div(M, PAIR_M);
   j.tiles_n = ceil_div(N, tile_n);
   j.blocks0 = j.blocks = ceil_div(K, KB);
+  // Columns of tiles are walked once for every `group` of 256 rows. Where the walked operand (the first product's:
+  // gate's and up's) is more than half of L2, it comes from memory each time, so that it should be seldom: 32768 x
+  // 2048 -> 11008 in a row, which the power limit bounds, 3.71 ms with 4, 3.61 with 8, 3.49 with 16, 3.55 with 24. Smaller ones
+  // stay in L2, and 4, which share A among more pairs, are as fast or faster (16384 x 1024 -> 4096, training: 1105 us
+  // against 1125 with 16).
+  j.group = N * K * (tile_n == PAIR_N ? 2 : 4) > HALF_L2 ? 16 : 4;
   j.rows = (int)M;
   j.cols = (int)N;
 }
