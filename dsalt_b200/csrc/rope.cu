@@ -156,6 +156,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) qk_norm_rope_kernel(const __g
 #pragma unroll
         for (int i = 0; i < V; ++i) q += xa[i] * xa[i] + xb[i] * xb[i];
         r = 1.f / sqrtf(group_sum<G>(q) * inv_d + a.eps);
+        if (j >= n) r = 0.f;  // no head here: with eps = 0 an infinity, which would reach the weights' sums as NaN
       }
       float oa[V], ob[V];
       if constexpr (!BWD) {
