@@ -89,18 +89,16 @@ __global__ void __launch_bounds__(THREADS) act_kernel(const float* __restrict__ 
     if (sizeof(T) == 4 && keep == DSALT_KEEP_INPUT) {
       static_cast<float*>(kept)[at] = a;
       static_cast<float*>(kept)[plane + at] = b;
-    } else if (keep != DSALT_KEEP_NONE) {
-      const uint32_t top_a = __reduce_max_sync(0xffffffffu, __float_as_uint(a) & 0x7fffffffu);
-      const uint32_t top_b = __reduce_max_sync(0xffffffffu, __float_as_uint(b) & 0x7fffffffu);
-      const bool wide = keep == DSALT_KEEP_INPUT;
-      const uint32_t sa = wide ? scale_byte16(top_a) : scale_byte(top_a), sb = wide ? scale_byte16(top_b) : scale_byte(top_b);
-      if (wide) {
-        static_cast<uint16_t*>(kept)[at] = (uint16_t)code_bits16(a, inverse_scale(sa));
-        static_cast<uint16_t*>(kept)[plane + at] = (uint16_t)code_bits16(b, inverse_scale(sb));
-      } else {
-        static_cast<int8_t*>(kept)[at] = (int8_t)code_of(a, sa);
-        static_cast<int8_t*>(kept)[plane + at] = (int8_t)code_of(b, sb);
-      }
+    } else if (keep == DSALT_KEEP_INPUT) {
+      uint16_t* to = static_cast<uint16_t*>(kept) + at;
+      to[0] = (uint16_t)upper_halves(a, 0.f);
+      to[plane] = (uint16_t)upper_halves(b, 0.f);
+      to[2 * plane] = (uint16_t)third_bytes(a, b);
+    } else if (keep == DSALT_KEEP_8BIT) {
+      const uint32_t sa = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(a) & 0x7fffffffu));
+      const uint32_t sb = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(b) & 0x7fffffffu));
+      static_cast<int8_t*>(kept)[at] = (int8_t)code_of(a, sa);
+      static_cast<int8_t*>(kept)[plane + at] = (int8_t)code_of(b, sb);
       if (lane == 0) {
         exps[i % groups * T_ + i / groups] = (uint8_t)sa;
         exps[(groups + i % groups) * T_ + i / groups] = (uint8_t)sb;
@@ -120,13 +118,15 @@ __global__ void __launch_bounds__(THREADS) act_grad_kernel(const float* __restri
     if (sizeof(T) == 4 && keep == DSALT_KEEP_INPUT) {
       a = static_cast<const float*>(kept)[at];
       b = static_cast<const float*>(kept)[total + at];
+    } else if (keep == DSALT_KEEP_INPUT) {
+      const uint16_t* w = static_cast<const uint16_t*>(kept) + at;
+      a = held24<0, 0>(w[0], w[2 * total]);
+      b = held24<0, 1>(w[total], w[2 * total]);
     } else {
       const int8_t* c = static_cast<const int8_t*>(kept);
-      const int16_t* w = static_cast<const int16_t*>(kept);
-      const bool wide = keep == DSALT_KEEP_INPUT;
       const int64_t scale = at % pitch / GROUP8 * T_ + at / pitch;
-      a = (float)(wide ? w[at] : c[at]) * scale_of(exps[scale]);
-      b = (float)(wide ? w[total + at] : c[total + at]) * scale_of(exps[pitch / GROUP8 * T_ + scale]);
+      a = (float)c[at] * scale_of(exps[scale]);
+      b = (float)c[total + at] * scale_of(exps[pitch / GROUP8 * T_ + scale]);
     }
     const float d = at % pitch < F ? dh[at] : 0.f;
     float v, dv;
@@ -158,6 +158,9 @@ int blocks_for(int64_t threads) {
   return (int)(b < 148 * 32 ? b : 148 * 32);
 }
 
+// whether the product of gate and up, the last product's operand, is kept, or formed again by the backward pass
+bool keeps_h(int dtype, int keep) { return dtype == DSALT_F32 && keep == DSALT_KEEP_INPUT; }
+
 template <typename T, int ACT>
 int forward_plain(const Ffn& f) {
   float* g = f.wide;
@@ -180,7 +183,7 @@ int backward_plain(const Ffn& f) {
   const Product dh = {{{f.dy, f.dy_stride, 1}}, {{f.w_down, 1, f.F}}, 1, f.T, f.F, f.d_out, f.pitch};
   if ((rc = product<T, float>(dh, f.wide, f.stream, "gated_ffn_bwd product launch"))) return rc;
   act_grad_kernel<T, ACT><<<blocks_for(f.T * f.pitch), THREADS, 0, f.stream>>>(
-      f.wide, f.T, f.F, f.pitch, f.kept, f.exps, f.keep, f.keep == DSALT_KEEP_8BIT ? static_cast<T*>(f.h) : nullptr,
+      f.wide, f.T, f.F, f.pitch, f.kept, f.exps, f.keep, keeps_h(f.dtype, f.keep) ? nullptr : static_cast<T*>(f.h),
       static_cast<T*>(f.dg), static_cast<T*>(f.du));
   if ((rc = check_cuda(cudaGetLastError(), "gated_ffn_bwd activation launch"))) return rc;
   if (f.dx) {
@@ -216,7 +219,7 @@ int run(const Ffn& f, bool backward) {
 
 size_t a256(size_t v) { return (v + 255) & ~(size_t)255; }
 size_t elem_bytes(int dtype) { return dtype == DSALT_F32 ? 4 : 2; }
-// whether what is kept of gate and up are codes with scales
+// whether the caller has to give a place for scales (with 24 bits nothing is written there)
 bool scaled(int dtype, int keep) { return keep == DSALT_KEEP_8BIT || (keep == DSALT_KEEP_INPUT && dtype != DSALT_F32); }
 // what the tensor cores take; their operands' rows have to be 16-byte aligned
 bool tensor_cores(int dtype, int d, int F, int d_out) { return dtype != DSALT_F32 && d % 8 == 0 && F % 8 == 0 && d_out % 8 == 0; }
@@ -276,7 +279,7 @@ int dsalt_gated_ffn(const void* x, int dtype, int64_t T, int d_model, int64_t x_
   f.pitch = pitch_of(d_ff);
   f.w_gate = w_gate, f.w_up = w_up, f.w_down = w_down, f.x = x, f.x_stride = T > 1 ? x_stride : d_model, f.kept = kept, f.exps = kept_exps;
   f.y = y;
-  f.h = keep == DSALT_KEEP_INPUT ? static_cast<char*>(kept) + 2 * T * f.pitch * elem_bytes(dtype) : workspace;
+  f.h = keeps_h(dtype, keep) ? static_cast<char*>(kept) + 2 * T * f.pitch * elem_bytes(dtype) : workspace;
   f.wide = reinterpret_cast<float*>(static_cast<char*>(workspace) + a256((size_t)T * f.pitch * elem_bytes(dtype)));
   f.stream = static_cast<cudaStream_t>(stream);
   if (int rc = check_rows(FN, f)) return rc;
@@ -286,8 +289,8 @@ int dsalt_gated_ffn(const void* x, int dtype, int64_t T, int d_model, int64_t x_
 size_t dsalt_gated_ffn_bwd_workspace_bytes(int dtype, int64_t T, int d_model, int d_ff, int d_out, int keep) {
   if (check("gated_ffn_bwd", dtype, T, d_model, d_ff, d_out, 0, keep)) return 0;
   const size_t n = (size_t)T * pitch_of(d_ff);
-  // dg and du; of 8-bit activations h and x as well; the plain path's dh
-  return (keep == DSALT_KEEP_8BIT ? 3 : 2) * a256(n * elem_bytes(dtype)) +
+  // dg and du, h where it was not kept; x where it was kept in 8 bits; the plain path's dh
+  return (keeps_h(dtype, keep) ? 2 : 3) * a256(n * elem_bytes(dtype)) +
          (keep == DSALT_KEEP_8BIT ? a256((size_t)T * d_model * elem_bytes(dtype)) : 0) +
          (tensor_cores(dtype, d_model, d_ff, d_out) ? 0 : a256(n * sizeof(float))) + 256;
 }
@@ -328,9 +331,10 @@ int dsalt_gated_ffn_bwd(const void* dy, int dtype, int64_t T, int d_model, int64
   const size_t n = a256((size_t)T * f.pitch * es);
   char* ws = static_cast<char*>(workspace);
   f.dg = ws, f.du = ws + n;
-  char* wide_x = ws + 3 * n;
-  f.wide = reinterpret_cast<float*>(coded ? wide_x + a256((size_t)T * d_model * es) : ws + 2 * n);
-  f.h = coded ? ws + 2 * n : static_cast<char*>(f.kept) + 2 * T * f.pitch * es;
+  const bool kept_h = keeps_h(dtype, keep);
+  char* wide_x = ws + (kept_h ? 2 : 3) * n;
+  f.wide = reinterpret_cast<float*>(coded ? wide_x + a256((size_t)T * d_model * es) : wide_x);
+  f.h = kept_h ? static_cast<char*>(f.kept) + 2 * T * f.pitch * es : ws + 2 * n;
   f.x = coded ? nullptr : x, f.x_stride = T > 1 ? x_stride : d_model;
   if (int rc = check_rows(FN, f)) return rc;
   if (coded && dw_gate) {

@@ -47,6 +47,24 @@ __device__ __forceinline__ void activate_grad(float g, float& a, float& da) {
   }
 }
 
+// What a backward pass of 16-bit inputs reads of gate's and up's sums: 24 of their 32 bits, each value by itself (codes
+// with a scale for 32 neighbours, of 16 bits, held a feature 2^10 times smaller than one beside it worse than
+// its own type does, and none beside an infinity). Three planes of 16 bits: gate's upper halves, up's, and both third bytes.
+// The fourth byte is read as the third again: 0 where a value has no more bits, else off by less than 2^-15 of
+// the value, to either side.
+__device__ __forceinline__ uint32_t upper_halves(float a, float b) {
+  return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+}
+__device__ __forceinline__ uint32_t third_bytes(float gate, float up) {  // in the lower half
+  return __byte_perm(__float_as_uint(gate), __float_as_uint(up), 0x0051);
+}
+// value COL (0, 1) of a pair of gate's (UP = 0) or up's
+template <int COL, int UP>
+__device__ __forceinline__ float held24(uint32_t upper, uint32_t third) {
+  constexpr uint32_t L = 4 + 2 * COL + UP;
+  return __uint_as_float(__byte_perm(upper, third, ((2 * COL + 1) << 12) | ((2 * COL) << 8) | (L << 4) | L));
+}
+
 inline int64_t pitch_of(int64_t d_ff) { return (d_ff + GROUP8 - 1) / GROUP8 * GROUP8; }
 
 // One call's sizes and operands. Rows of h, dg, du and of what is kept are `pitch` values long.
@@ -60,7 +78,7 @@ struct Ffn {
   const void* w_down;
   const void* x;
   int64_t x_stride;
-  void* kept;       // gate's and up's [2, T, pitch], as fp32 or as codes of 16 bits with h behind them, or codes of 8
+  void* kept;       // [3, T, pitch]: gate, up and h in fp32, or gate and up in 24 bits; [2, T, pitch] codes of 8
   uint8_t* exps;    // [2, pitch / 32, T] of codes
   // forward
   void* y;

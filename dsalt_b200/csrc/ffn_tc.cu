@@ -18,7 +18,7 @@
 //
 // Bound by what an SM can take from L2, 64 bytes a cycle: a stage of 32 KB feeds 512 cycles of products, so
 // at the tensor cores' full rate the operands alone fill that path (85 to 90 % of the rate is reached),
-// and what an epilogue writes and reads (up to 6 and 4 bytes for each of T x d_ff values) comes on top. Long runs
+// and what an epilogue writes and reads (up to 8 and 6 bytes for each of T x d_ff values) comes on top. Long runs
 // are bound by the power limit, under which the clock falls from 1.9 to 1.4 GHz. Measured, bf16: 32768 x 2048 ->
 // 11008 forward 2.76 ms (1610 TFLOP/s) cold and 3.13 to 3.25 ms (1360 to 1420) in a row; 32768 x 768 -> 2048 forward, 16 bits kept,
 // and backward 692 us (1340 TFLOP/s); 16384 x 1024 -> 4096, 8 bits kept, 944 us (1310); 1999 x 768 -> 2048 33 us.
@@ -50,7 +50,7 @@ struct alignas(64) Job {
   void* out;                              // of c[0], for a plain store's sums of several parts
 };
 struct Kept {
-  void* p;           // gate's and up's [2, T, pitch]
+  void* p;           // gate's and up's codes [2, T, pitch], or their 24 bits [3, T, pitch]
   uint8_t* exps;     // their scales [2, pitch / 32, T]: the lanes of a warp, rows of a tile, find theirs side by side
   void* h;           // [T, pitch]
   int64_t T, pitch;
@@ -121,8 +121,9 @@ __device__ __forceinline__ void pair_commit(uint64_t* bar, uint32_t leader) {
 // sets of boxes. The backward's has what was kept brought in by the load engine, a warp's 32 rows x 32
 // columns of gate and of up at a time, three of them under way (hidden gradients of
 // 32768 x 768 -> 2048: read row by row by the threads 165 us, so 148, and 123 since accumulators are given back
-// early); codes of 16 bits are replaced by the gradients where they lie, codes of 8 have a set of boxes for three
-// outputs besides.
+// early, with two codes of 16 bits a value; 162 with 24 bits each and h formed again, 850 MB of memory traffic where there were
+// 558). The upper halves of 24 bits are replaced by the gradients where they lie, the third bytes and h go
+// through registers; codes of 8 bits have a set of boxes for three outputs besides.
 template <int EPI, int KEEP>
 struct Shape {
   static constexpr bool IN_PLACE = EPI == GRADS && KEEP == DSALT_KEEP_INPUT;
@@ -212,24 +213,11 @@ __device__ __forceinline__ uint32_t largest_of(const float (&f)[GROUP8]) {
   for (int i = 1; i < 4; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top[0]) : "f"(top[i]));
   return __float_as_uint(top[0]) & 0x7fffffffu;
 }
-// a group of 32 columns of a row: its scale byte and its codes of 8 or 16 bits
-template <int WORDS>
-__device__ __forceinline__ uint32_t form_codes(const float (&f)[GROUP8], uint32_t (&w)[WORDS]) {
-  const uint32_t top = largest_of(f);
-  const uint32_t s = WORDS == 8 ? scale_byte(top) : scale_byte16(top);
-  if constexpr (WORDS == 8) pack_codes<GROUP8>(f, s, w);
-  else pack_codes16<GROUP8>(f, s, w);
-  return s;
-}
-template <int WORDS>
-__device__ __forceinline__ void store_codes(void* p, const uint32_t (&w)[WORDS]) {
-#pragma unroll
-  for (int i = 0; i < WORDS; i += 8) {
-    uint32_t part[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) part[j] = w[i + j];
-    store_32b(static_cast<char*>(p) + 4 * i, part);
-  }
+// 32 bytes of what the forward pass kept
+__device__ __forceinline__ void load_32b(uint32_t (&w)[8], const void* p) {
+  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(__cvta_generic_to_global(p)));
 }
 
 __device__ __forceinline__ uint4 load_shared(uint32_t at) {
@@ -238,20 +226,23 @@ __device__ __forceinline__ uint4 load_shared(uint32_t at) {
   return v;
 }
 // values 16 half .. 16 half + 15 of a row of a box of codes, as the load engine wrote it
-template <int KEEP>
-__device__ __forceinline__ void kept_values(uint32_t box, int lane, int half, float scale, float (&f)[16]) {
-  if constexpr (KEEP == DSALT_KEEP_8BIT) {
-    const uint4 v = load_shared(box + lane * 32 + half * 16);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    unpack_codes<16>(w, scale, f);
-  } else {
-    uint32_t w[8];
+__device__ __forceinline__ void coded_values(uint32_t box, int lane, int half, float scale, float (&f)[16]) {
+  const uint4 v = load_shared(box + lane * 32 + half * 16);
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  unpack_codes<16>(w, scale, f);
+}
+// the same of a box of upper halves, with their third bytes
+template <int UP>
+__device__ __forceinline__ void held_values(uint32_t box, int lane, int half, const uint32_t (&third)[8], float (&f)[16]) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint4 v = load_shared(box + lane * 64 + (((2 * half + i) ^ ((lane >> 1) & 3)) << 4));
-      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+  for (int i = 0; i < 2; ++i) {
+    const uint4 v = load_shared(box + lane * 64 + (((2 * half + i) ^ ((lane >> 1) & 3)) << 4));
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f[8 * i + 2 * j] = held24<0, UP>(w[j], third[4 * i + j]);
+      f[8 * i + 2 * j + 1] = held24<1, UP>(w[j], third[4 * i + j]);
     }
-    unpack_codes16<16>(w, scale, f);
   }
 }
 
@@ -411,7 +402,15 @@ __global__ void __launch_bounds__(THREADS, 1)
       load_own_2d(to, &args.kept_map[0], &kept_full[n % 3], col, row);
       load_own_2d(to + S::KEPT_BOX, &args.kept_map[1], &kept_full[n % 3], col, row);
     };
-    uint32_t sg = 127, su = 127;
+    // of codes the scales of a chunk, of 24 bits the third bytes of half of one, which are asked for a chunk ahead
+    uint32_t sg = 127, su = 127, third[2][8] = {};
+    auto ask_third = [&](int c, int half) {
+      const bool next = c >= CHUNKS;
+      const int64_t row = (next ? rows[1] : rows[0]) + lane, col = (next ? cols[1] - CHUNKS * 32 : cols[0]) + c * 32;
+      if ((!next || more) && row < args.kept.T && col < args.kept.pitch)
+        load_32b(third[half],
+                 static_cast<const uint16_t*>(args.kept.p) + (2 * args.kept.T + row) * args.kept.pitch + col + 16 * half);
+    };
     auto ask_scales = [&](int c) {
       const bool next = c >= CHUNKS;
       const int64_t row = (next ? rows[1] : rows[0]) + lane, group = ((next ? cols[1] - CHUNKS * 32 : cols[0]) + c * 32) / GROUP8;
@@ -424,7 +423,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     };
     if constexpr (EPI == GRADS) {
       look_ahead(pair);
-      ask_scales(CHUNKS);
+      if constexpr (KEEP == DSALT_KEEP_8BIT) {
+        ask_scales(CHUNKS);
+      } else {
+        ask_third(CHUNKS, 0);
+        ask_third(CHUNKS, 1);
+      }
       if (lane == 0)
         for (int n = 0; n < (S::IN_PLACE ? 2 : 3); ++n) ask_kept(n, CHUNKS + n);
       __syncwarp();
@@ -471,7 +475,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           const int n = it * CHUNKS + c / 32;
           const uint32_t from = kept_boxes + n % 3 * 2 * S::KEPT_BOX;
           const float scale_g = scale_of(sg), scale_u = scale_of(su);
-          ask_scales(c / 32 + 1);
+          if constexpr (KEEP == DSALT_KEEP_8BIT) ask_scales(c / 32 + 1);
           if (!(ok = mbar_wait(&kept_full[n % 3], n / 3 & 1, args.err, 65))) break;
           float d[32];
           take_acc<32>(r, d);
@@ -481,8 +485,14 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             float a[16], b[16], e[16];
-            kept_values<KEEP>(from, lane, half, scale_g, a);
-            kept_values<KEEP>(from + S::KEPT_BOX, lane, half, scale_u, b);
+            if constexpr (KEEP == DSALT_KEEP_8BIT) {
+              coded_values(from, lane, half, scale_g, a);
+              coded_values(from + S::KEPT_BOX, lane, half, scale_u, b);
+            } else {
+              held_values<0>(from, lane, half, third[half], a);
+              held_values<1>(from + S::KEPT_BOX, lane, half, third[half], b);
+              ask_third(c / 32 + 1, half);
+            }
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               float v, dv;
@@ -495,7 +505,13 @@ __global__ void __launch_bounds__(THREADS, 1)
               if (half == 0) to = next_boxes();
             stage_row<T, 16>(to, lane, a, 16 * half);
             stage_row<T, 16>(to + BOX_BYTES, lane, e, 16 * half);
-            if constexpr (!S::IN_PLACE) stage_row<T, 16>(to + 2 * BOX_BYTES, lane, b, 16 * half);
+            if constexpr (S::IN_PLACE) {
+              const int64_t row = row0 + lane;
+              if (row < args.kept.T && cols[0] + c < args.kept.pitch)
+                store_row<T, 16>(static_cast<T*>(args.kept.h) + row * args.kept.pitch + cols[0] + c + 16 * half, b);
+            } else {
+              stage_row<T, 16>(to + 2 * BOX_BYTES, lane, b, 16 * half);
+            }
           }
           send(to, cols[0] + c);
           if (lane == 0) {
@@ -529,19 +545,38 @@ __global__ void __launch_bounds__(THREADS, 1)
             acc_read();
           }
           const bool in = row < args.kept.T && col + 32 * half < args.kept.pitch;
-          if constexpr (KEEP != DSALT_KEEP_NONE) {
-            constexpr int WORDS = KEEP == DSALT_KEEP_8BIT ? 8 : 16;
-            uint32_t c[WORDS];
-            char* codes = static_cast<char*>(args.kept.p) + (at + 32 * half) * (WORDS / 8);
-            uint32_t s = form_codes(g, c);
+          if constexpr (KEEP == DSALT_KEEP_8BIT) {
+            uint32_t c[8];
+            char* codes = static_cast<char*>(args.kept.p) + at + 32 * half;
+            uint32_t s = scale_byte(largest_of(g));
+            pack_codes<GROUP8>(g, s, c);
             if (in) {
-              store_codes(codes, c);
+              store_32b(codes, c);
               args.kept.exps[(col / GROUP8 + half) * args.kept.T + row] = (uint8_t)s;
             }
-            s = form_codes(u, c);
+            s = scale_byte(largest_of(u));
+            pack_codes<GROUP8>(u, s, c);
             if (in) {
-              store_codes(codes + plane * (WORDS / 8), c);
+              store_32b(codes + plane, c);
               args.kept.exps[((args.kept.pitch + col) / GROUP8 + half) * args.kept.T + row] = (uint8_t)s;
+            }
+          } else if constexpr (KEEP == DSALT_KEEP_INPUT) {
+            uint16_t* to = static_cast<uint16_t*>(args.kept.p) + at + 32 * half;
+#pragma unroll
+            for (int i = 0; i < 32; i += 16) {
+              uint32_t wg[8], wu[8], w3[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const int k = i + 2 * j;
+                wg[j] = upper_halves(g[k], g[k + 1]);
+                wu[j] = upper_halves(u[k], u[k + 1]);
+                w3[j] = __byte_perm(third_bytes(g[k], u[k]), third_bytes(g[k + 1], u[k + 1]), 0x5410);
+              }
+              if (in) {
+                store_32b(to + i, wg);
+                store_32b(to + plane + i, wu);
+                store_32b(to + 2 * plane + i, w3);
+              }
             }
           }
 #pragma unroll

@@ -81,33 +81,6 @@ __device__ __forceinline__ void unpack_codes(const uint32_t (&w)[N / 4], float s
   for (int i = 0; i < N; ++i) f[i] = (float)(int8_t)(w[i / 4] >> (8 * (i % 4))) * scale;
 }
 
-// The same with codes of 16 bits, for what a backward pass of 16-bit inputs reads: s = max(E - 14, 1), E the
-// exponent field of the largest plus half a step, so that no code reaches 32768. A value is off by
-// 2^-16 of the group's largest at most, where its own rounding to bf16 would be off by 2^-9 (fp16:
-// 2^-12) of itself.
-__device__ __forceinline__ uint32_t scale_byte16(uint32_t top) {
-  const int e = (int)((top + 0x100u) >> 23);
-  return e >= 255 ? 255u : (uint32_t)max(e - 14, 1);
-}
-__device__ __forceinline__ uint32_t code_bits16(float x, float inv) { return __float_as_uint(fmaf(x, inv, 12582912.f)); }
-template <int N>
-__device__ __forceinline__ void pack_codes16(const float (&f)[N], uint32_t s, uint32_t (&w)[N / 2]) {
-  const float inv = inverse_scale(s);
-#pragma unroll
-  for (int i = 0; i < N / 2; ++i) w[i] = __byte_perm(code_bits16(f[2 * i], inv), code_bits16(f[2 * i + 1], inv), 0x5410);
-}
-// code + 32768 behind the bits of 2^23, times the scale less (2^23 + 32768) times the scale: exact
-template <int N>
-__device__ __forceinline__ void unpack_codes16(const uint32_t (&w)[N / 2], float scale, float (&f)[N]) {
-  const float less = -8421376.f * scale;
-#pragma unroll
-  for (int i = 0; i < N / 2; ++i) {
-    const uint32_t u = w[i] ^ 0x80008000u;
-    f[2 * i] = fmaf(__uint_as_float(__byte_perm(u, 0x4b00u, 0x5410)), scale, less);
-    f[2 * i + 1] = fmaf(__uint_as_float(__byte_perm(u, 0x4b00u, 0x5432)), scale, less);
-  }
-}
-
 int launch_pack8(const void* x, int dtype, int64_t rows, int64_t cols, int64_t x_stride, int8_t* codes, uint8_t* exps,
                  cudaStream_t stream);
 int launch_unpack8(const int8_t* codes, const uint8_t* exps, int64_t rows, int64_t cols, void* out, int dtype,

@@ -337,19 +337,19 @@ Kept ffn_forward(const Tensor& x, const Tensor& m, int64_t stride, const Tensor&
     const int64_t pitch = dsalt_gated_ffn_pitch((int)a.F);
     const bool coded = keep == DSALT_KEEP_8BIT;
     k.kept = empty({coded ? 2 : 3, T, pitch}, coded ? at::kChar : m.scalar_type(), a.dev);
-    if (coded || dt != DSALT_F32) k.exps = empty({2, pitch / GROUP, T}, at::kByte, a.dev);
+    if (coded) k.exps = empty({2, pitch / GROUP, T}, at::kByte, a.dev);
   }
   const Tensor ws = workspace(dsalt_gated_ffn_workspace_bytes(dt, T, (int)a.d, (int)a.F, (int)a.d_out), a.dev);
   const Launch launch(a.dev);
   check(dsalt_gated_ffn(m.data_ptr(), dt, T, (int)a.d, stride, w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
-                        (int)a.F, (int)a.d_out, act, keep, ptr(k.kept), static_cast<uint8_t*>(ptr(k.exps)), k.y.data_ptr(),
+                        (int)a.F, (int)a.d_out, act, keep, ptr(k.kept), static_cast<uint8_t*>(ptr(k.exps.defined() ? k.exps : k.kept)), k.y.data_ptr(),
                         ws.data_ptr(), (size_t)ws.numel(), launch.stream),
         "dsalt_gated_ffn");
   return k;
 }
 
-// Kept for the backward pass: gate's and up's sums and x, in 16 bits (fp32 inputs: as they are) or in 8. With
-// 16 the rows that the last product read are kept too; with 8 they are formed again.
+// Kept for the backward pass: gate's and up's sums and x, in 24 bits and as it is, or in 8 bits. The rows that
+// the last product read are formed again; of fp32 inputs everything is kept as it is, those rows too.
 struct FfnNode : torch::autograd::Function<FfnNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_gate, const Tensor& w_up,
                                const Tensor& w_down, int64_t act, int64_t keep) {
@@ -384,7 +384,7 @@ struct FfnNode : torch::autograd::Function<FfnNode> {
                  wu = ffn_weight(saved(s[5], "up weight", type, {F, d}, dev)),
                  wd = ffn_weight(saved(s[6], "down weight", type, {d_out, F}, dev));
     Tensor x, x_exps, exps;
-    if (coded || type != at::kFloat) exps = saved(s[3], "scales", at::kByte, {2, pitch / GROUP, T}, dev);
+    if (coded) exps = saved(s[3], "scales", at::kByte, {2, pitch / GROUP, T}, dev);
     int64_t x_stride = d;
     if (s[0].defined()) {
       if (coded && T) {
@@ -407,7 +407,7 @@ struct FfnNode : torch::autograd::Function<FfnNode> {
     check(dsalt_gated_ffn_bwd(dy.data_ptr(), dt, T, (int)d, dy_stride, ptr(x), x_stride,
                               static_cast<const uint8_t*>(ptr(x_exps)), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), (int)F,
                               (int)d_out, (int)ctx->saved_data["act"].toInt(), keep, kept.data_ptr(),
-                              static_cast<const uint8_t*>(ptr(exps)), ptr(dx), ptr(dwg), ptr(dwu), ptr(dwd), ws.data_ptr(),
+                              static_cast<const uint8_t*>(ptr(exps.defined() ? exps : kept)), ptr(dx), ptr(dwg), ptr(dwu), ptr(dwd), ws.data_ptr(),
                               (size_t)ws.numel(), launch.stream),
           "dsalt_gated_ffn_bwd");
     return {dx, ctx->needs_input_grad(1) ? dwg : Tensor(), ctx->needs_input_grad(2) ? dwu : Tensor(), dwd, Tensor(), Tensor()};

@@ -71,8 +71,9 @@ def gated_ffn(x, w_gate, w_up, w_down, *, activation: str = "silu", keep: str = 
 
     ``activation`` is ``"silu"`` or ``"gelu"`` (by the error function). Differentiable in all four;
     ``keep`` says in what form the backward pass finds ``x``, ``x Wgᵀ`` and ``x Wuᵀ``: ``"16bit"``, ``x`` as it is
-    and the others in 16 bits with a scale for 32 values (fp32 inputs: fp32), or ``"8bit"``, as
-    :func:`pack8` holds them (a third of the memory; the gradients are then those at the held values). bf16
+    and the others each with 16 significant bits, in three bytes (fp32 inputs: fp32), or ``"8bit"``, as
+    :func:`pack8` holds them (a third of the memory; the gradients are then those at the held values, and a value
+    that is not finite is one for its group of 32). bf16
     and fp16 run on the tensor cores where sizes are multiples of 8; fp32 and other sizes on the CUDA
     cores. Under autocast all four are cast first, as a linear layer's are."""
     if activation not in ACTIVATIONS:

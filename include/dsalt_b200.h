@@ -459,10 +459,11 @@ int dsalt_qk_norm_rope_bwd(const void* q, const void* k, const void* dq_out, con
  *   [T, d_out], contiguous, all of dtype. The product of gate and up is rounded to dtype before the
  *   last product; sums are fp32. activation: DSALT_ACT_SILU, or DSALT_ACT_GELU (by the error function).
  * keep: what the backward pass needs goes to kept, in rows of pitch = dsalt_gated_ffn_pitch(d_ff) values, a
- *   multiple of 32. DSALT_KEEP_INPUT: [3, T, pitch] of dtype's size, x Wg^T, x Wu^T (fp32 as it is; of 16-bit
- *   types codes of 16 bits, 32 values to a scale in kept_exps [2, pitch / 32, T], whose step is at most
- *   2^-14 of the largest) and the product's rows. DSALT_KEEP_8BIT: [2, T, pitch] bytes, the first two
- *   as codes with scales in kept_exps (likewise), as dsalt_pack8 forms them. kept and workspace 256-byte aligned.
+ *   multiple of 32. DSALT_KEEP_INPUT: [3, T, pitch] of dtype's size: of fp32 x Wg^T, x Wu^T and the product's
+ *   rows; of 16-bit types the upper halves of x Wg^T and of x Wu^T in fp32, then the third byte of each (an up's behind
+ *   its gate's), so that every value is held to 2^-15 of itself (kept_exps must be given here too; nothing
+ *   is written there). DSALT_KEEP_8BIT: [2, T, pitch] bytes, x Wg^T and x Wu^T as codes with scales in
+ *   kept_exps [2, pitch / 32, T], as dsalt_pack8 forms them. kept and workspace 256-byte aligned.
  * dsalt_gated_ffn_bwd: the gradients (contiguous, of dtype; null: not wanted, dw_gate and dw_up go
  *   together) from dy [T, d_out] (row stride dy_stride). With DSALT_KEEP_8BIT x holds the codes and
  *   x_exps the scales of dsalt_pack8 (contiguous), else x is the forward's. x may be null where dw_gate is.
