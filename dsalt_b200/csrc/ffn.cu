@@ -120,8 +120,8 @@ __global__ void __launch_bounds__(THREADS) act_grad_kernel(const float* __restri
       b = static_cast<const float*>(kept)[total + at];
     } else if (keep == DSALT_KEEP_INPUT) {
       const uint16_t* w = static_cast<const uint16_t*>(kept) + at;
-      a = held24<0, 0>(w[0], w[2 * total]);
-      b = held24<0, 1>(w[total], w[2 * total]);
+      a = held24<0>(w[0], w[2 * total]).x;
+      b = held24<1>(w[total], w[2 * total]).x;
     } else {
       const int8_t* c = static_cast<const int8_t*>(kept);
       const int64_t scale = at % pitch / GROUP8 * T_ + at / pitch;

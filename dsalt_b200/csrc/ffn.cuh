@@ -50,19 +50,19 @@ __device__ __forceinline__ void activate_grad(float g, float& a, float& da) {
 // What a backward pass of 16-bit inputs reads of gate's and up's sums: 24 of their 32 bits, each value by itself (codes
 // with a scale for 32 neighbours, of 16 bits, held a feature 2^10 times smaller than one beside it worse than
 // its own type does, and none beside an infinity). Three planes of 16 bits: gate's upper halves, up's, and both third bytes.
-// The fourth byte is read as the third again: 0 where a value has no more bits, else off by less than 2^-15 of
-// the value, to either side.
+// The fourth byte is cut off: sums of at most 16 significant bits are held exactly, others are off by less than
+// 2^-15 of themselves, towards zero (the mean, 2^-16, is far below the rounding of their gradients to 16 bits).
 __device__ __forceinline__ uint32_t upper_halves(float a, float b) {
   return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
 }
 __device__ __forceinline__ uint32_t third_bytes(float gate, float up) {  // in the lower half
   return __byte_perm(__float_as_uint(gate), __float_as_uint(up), 0x0051);
 }
-// value COL (0, 1) of a pair of gate's (UP = 0) or up's
-template <int COL, int UP>
-__device__ __forceinline__ float held24(uint32_t upper, uint32_t third) {
-  constexpr uint32_t L = 4 + 2 * COL + UP;
-  return __uint_as_float(__byte_perm(upper, third, ((2 * COL + 1) << 12) | ((2 * COL) << 8) | (L << 4) | L));
+// gate's (UP = 0) or up's two values of a pair of columns
+template <int UP>
+__device__ __forceinline__ float2 held24(uint32_t upper, uint32_t third) {
+  const uint32_t t = UP ? __byte_perm(third, 0u, 0x4341) : third & 0x00ff00ffu;  // byte, zero, byte, zero
+  return make_float2(__uint_as_float(__byte_perm(upper, t, 0x1045)), __uint_as_float(__byte_perm(upper, t, 0x3267)));
 }
 
 inline int64_t pitch_of(int64_t d_ff) { return (d_ff + GROUP8 - 1) / GROUP8 * GROUP8; }

@@ -240,8 +240,8 @@ __device__ __forceinline__ void held_values(uint32_t box, int lane, int half, co
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      f[8 * i + 2 * j] = held24<0, UP>(w[j], third[4 * i + j]);
-      f[8 * i + 2 * j + 1] = held24<1, UP>(w[j], third[4 * i + j]);
+      const float2 v = held24<UP>(w[j], third[4 * i + j]);
+      f[8 * i + 2 * j] = v.x, f[8 * i + 2 * j + 1] = v.y;
     }
   }
 }

@@ -95,3 +95,22 @@ def test_held_values_are_within_their_stated_bound(T, d, F):
     tol = tol + 2.0 ** -11 * h.abs() + 2.0 ** -18 * h.abs() + 2.0 ** -24   # as an operand; the activation
     assert ((got[0].double() - h).abs() <= tol * (1 + 2.0 ** -10)).all()
     assert all(torch.equal(got[0], row) for row in got)
+
+
+@pytest.mark.parametrize("size", [8, 3])
+def test_sums_of_few_bits_are_held_exactly(size):
+    """Gates that fp16 holds, where silu's derivative changes its sign: the gradient of x shows the slightest change of them."""
+    from dsalt_b200 import layers
+    v = torch.linspace(-1.32, -1.24, 100, device="cuda").half()
+    x, w = torch.zeros(100, size, device="cuda").half(), torch.zeros(3, size, size, device="cuda").half()
+    x[:, 0], x[:, 1] = v, 1
+    w[0, 0, 0], w[1, 0, 1], w[2, 0, 0] = 1, 1024, 1
+    leaf = x.clone().requires_grad_(True)
+    dy = torch.zeros(100, size, device="cuda").half()
+    dy[:, 0] = 1
+    dx, = torch.autograd.grad(layers.gated_ffn(leaf, *w), leaf, dy)
+    g = v.double()
+    p, dp = O.share(g, "silu")
+    ref = 1024 * (p + g * dp)
+    # half a step of fp16, and some ten operations in 32 bits on terms of the size of p
+    assert ((dx[:, 0].double() - ref).abs() <= 2.0 ** -11 * ref.abs() + 1024 * 2.0 ** -20 * p).all()
