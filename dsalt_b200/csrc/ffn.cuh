@@ -13,12 +13,9 @@ __device__ __forceinline__ float reciprocal(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// 1 / (1 + e^-g), to some 2^-21 of itself; below the normal range 0
-__device__ __forceinline__ float sigmoid(float g) { return reciprocal(1.f + ex2_approx(-LOG2E * g)); }
-
 // act(g) and act'(g) in fp32. silu: g p with p = 1 / (1 + e^-g); gelu: g p with p the normal
-// distribution's share below g. FAST (the tensor cores' epilogues, whose results are rounded to 16 bits): with the
-// exponential that the derivative needs as well, the share below -x as e^(-x^2/2) t P(t), t = 1 / (1 + 0.302 x), the
+// distribution's share below g. By CUDA's functions, or FAST (the tensor cores' epilogues, whose results are rounded
+// to 16 bits). FAST gelu: with the exponential that the derivative needs as well, the share below -x as e^(-x^2/2) t P(t), t = 1 / (1 + 0.302 x), the
 // form of Hastings' approximations. P has six terms, fitted by linear programming for its relative error, which stays
 // below 2^-16 where the share is small and below 2^-18 for x < 2 (Hastings' own five terms, Abramowitz
 // and Stegun 7.1.26, hold 7.5e-8 of the whole, which at g = -5 is 1.6e-3 of the value: three half steps of fp16).
@@ -33,20 +30,41 @@ __device__ __forceinline__ float share_below(float g, float e) {  // e = exp(-g^
   const float tail = e * t * p;
   return g < 0.f ? tail : 1.f - tail;
 }
+// p = 1 / (1 + e^-g) and 1 - p. FAST: p to some 2^-21 of itself near 0; the argument's rounding grows with it, to 2^-20
+// at -20 and 2^-18 at -80; below the normal range 0.
+template <bool FAST>
+__device__ __forceinline__ float2 sigmoid(float g) {
+  if constexpr (FAST) {
+    const float p = reciprocal(1.f + ex2_approx(-LOG2E * g));
+    return make_float2(p, 1.f - p);
+  } else {
+    const float e = expf(-fabsf(g)), large = 1.f / (1.f + e), small = e * large;
+    return g < 0.f ? make_float2(small, large) : make_float2(large, small);
+  }
+}
 template <int ACT, bool FAST>
 __device__ __forceinline__ float activate(float g) {
-  if constexpr (ACT == DSALT_ACT_SILU) return g * sigmoid(g);
+  if constexpr (ACT == DSALT_ACT_SILU) return g * sigmoid<FAST>(g).x;
   else if constexpr (FAST) return g * share_below(g, ex2_approx(-0.5f * LOG2E * g * g));
   else return g * normcdff(g);
 }
 template <int ACT, bool FAST>
 __device__ __forceinline__ void activate_grad(float g, float& a, float& da) {
   if constexpr (ACT == DSALT_ACT_SILU) {
-    const float p = sigmoid(g);
-    a = g * p;
-    da = fmaf(a, 1.f - p, p);
+    const float2 p = sigmoid<FAST>(g);
+    a = g * p.x;
+    da = fmaf(a, p.y, p.x);
   } else {
-    const float e = ex2_approx(-0.5f * LOG2E * g * g), p = FAST ? share_below(g, e) : normcdff(g);
+    float e, p;
+    if constexpr (FAST) {
+      e = ex2_approx(-0.5f * LOG2E * g * g);
+      p = share_below(g, e);
+    } else {
+      const float square = g * g;  // what its rounding leaves out counts where it is large
+      e = expf(-0.5f * square);
+      if (e > 0.f) e = fmaf(-0.5f * fmaf(g, g, -square), e, e);
+      p = normcdff(g);
+    }
     a = g * p;
     da = fmaf(g * 0.3989422804014327f, e, p);
   }

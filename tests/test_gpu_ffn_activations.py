@@ -26,6 +26,24 @@ def probe(v, size, up, dtype, keep, grad=True):
     return out
 
 
+def test_activations_of_fp32_inputs():
+    v = torch.cat([torch.linspace(-87, 87, 4001), torch.linspace(-13, 13, 4001), torch.linspace(-1e-3, 1e-3, 101)]).cuda()
+    got = probe(v, 2, 1.0, torch.float32, "16bit")
+    g = v.double()
+    for act, (y, dx) in got.items():
+        p, dp = O.share(g, act)
+        far = (g * p).abs() >= 2.0 ** -126   # below it fewer bits are left
+        # silu: an exponential of two steps of 2^-23, three operations of half a step; gelu: CUDA's distribution function
+        # of five steps, or an exponential and a product, and three operations
+        tol = {"silu": 2.0 ** -21, "gelu": 2.0 ** -20}[act]
+        over = ((y.double() - g * p).abs() - tol * (g * p).abs())[far]
+        assert (over <= 0).all(), (act, float(g[far][over.argmax()]))
+        size = p + (g * dp).abs()
+        far = size >= 2.0 ** -120
+        over = ((dx.double() - (p + g * dp)).abs() - tol * size)[far]
+        assert (over <= 0).all(), (act, float(g[far][over.argmax()]))
+
+
 @pytest.mark.parametrize("T", [8, 16, 100, 6000])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("grad", [True, False])
