@@ -25,7 +25,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import layers
-from .module import DSALTAttention
+from .module import DSALTAttention, longest_sequence
 from .serving import MAX_VOCAB, PagedCache, sample_tokens
 
 
@@ -216,6 +216,7 @@ class DSALTLMHeadModel(nn.Module):
             x = x.to(torch.get_autocast_dtype("cuda"))
         cu_h = [int(c) for c in (cu_list if cu_list is not None else cu_seqlens.detach().cpu().tolist())]
         attn0 = self.layers[0].attn
+        longest_sequence(cu_h, attn0.rope_cos.shape[0])
         pos = torch.cat([torch.arange(cu_h[i + 1] - cu_h[i], device=x.device) for i in range(len(cu_h) - 1)])
         rope_cs = (attn0.rope_cos.to(x.device)[pos], attn0.rope_sin.to(x.device)[pos])
         for layer in self.layers:

@@ -89,6 +89,15 @@ def apply_rotary_emb(q, k, cos, sin):
     return q * cos + rot(q) * sin, k * cos + rot(k) * sin
 
 
+def longest_sequence(cu_h, max_seq_len: int) -> int:
+    """The longest sequence of a pack (``cu_h``: its borders), which the tables of angles have to reach: a
+    ``ValueError`` on the host, where an index beyond them would be read as another on the device or end its context."""
+    longest = max((b - a for a, b in zip(cu_h, cu_h[1:])), default=0)
+    if longest > max_seq_len:
+        raise ValueError(f"a sequence of {longest} tokens is beyond max_seq_len {max_seq_len}")
+    return longest
+
+
 class HeadNorm(nn.Module):
     """The weight of a head's RMS norm (applied by :func:`dsalt_b200.layers.qk_norm_rope`)."""
 
@@ -156,6 +165,8 @@ class DSALTAttention(nn.Module):
     def _qkv(self, x, cu_h, total_len, device, rope_cs):
         """Projections and RoPE (``_packed`` ``:566-589``); kv heads stay grouped."""
         T, H, Hkv, D = total_len, self.n_heads, self.n_kv_heads, self.head_dim
+        if rope_cs is None:
+            longest_sequence(cu_h, self.rope_cos.shape[0])
         q = self.q_proj(x).view(T, H, D)
         k = self.k_proj(x).view(T, Hkv, D)
         v = self.v_proj(x).view(T, Hkv, D)
