@@ -92,7 +92,7 @@ def apply_rotary_emb(q, k, cos, sin):
 def longest_sequence(cu_h, max_seq_len: int) -> int:
     """The longest sequence of a pack (``cu_h``: its borders), which the tables of angles have to reach: a
     ``ValueError`` on the host, where an index beyond them would be read as another on the device or end its context."""
-    longest = max((b - a for a, b in zip(cu_h, cu_h[1:])), default=0)
+    longest = max([0] + [b - a for a, b in zip(cu_h, cu_h[1:])])  # a list: as a traced module has it
     if longest > max_seq_len:
         raise ValueError(f"a sequence of {longest} tokens is beyond max_seq_len {max_seq_len}")
     return longest
