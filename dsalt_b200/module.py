@@ -165,8 +165,7 @@ class DSALTAttention(nn.Module):
     def _qkv(self, x, cu_h, total_len, device, rope_cs):
         """Projections and RoPE (``_packed`` ``:566-589``); kv heads stay grouped."""
         T, H, Hkv, D = total_len, self.n_heads, self.n_kv_heads, self.head_dim
-        if rope_cs is None:
-            longest_sequence(cu_h, self.rope_cos.shape[0])
+        longest = None if rope_cs is not None else longest_sequence(cu_h, self.rope_cos.shape[0])
         q = self.q_proj(x).view(T, H, D)
         k = self.k_proj(x).view(T, Hkv, D)
         v = self.v_proj(x).view(T, Hkv, D)
@@ -175,7 +174,9 @@ class DSALTAttention(nn.Module):
                 return *self._norm_rope(q, k, *rope_cs, None), v
             pos = torch.cat([torch.arange(cu_h[i + 1] - cu_h[i], device=device, dtype=torch.int32)
                              for i in range(len(cu_h) - 1)])
-            return *self._norm_rope(q, k, self.rope_cos.to(device), self.rope_sin.to(device), pos), v
+            # the rows and the half that are read: in 16 bits they are converted, and a backward pass keeps that
+            cos, sin = (t[:longest, :D // 2].to(device) for t in (self.rope_cos, self.rope_sin))
+            return *self._norm_rope(q, k, cos, sin, pos), v
         if rope_cs is None:
             pos = torch.cat([torch.arange(cu_h[i + 1] - cu_h[i], device=device) for i in range(len(cu_h) - 1)])
             cos, sin = self.rope_cos.to(device)[pos], self.rope_sin.to(device)[pos]
