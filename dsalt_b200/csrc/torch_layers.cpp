@@ -71,6 +71,12 @@ void no_second_derivative() {
   TORCH_CHECK(!at::GradMode::is_enabled(), "dsalt_b200 operators have no second derivative");  // create_graph=True
 }
 
+// A dual tensor need not require a gradient, so that the call would go past the node and lose its tangent
+void no_forward_mode(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), "dsalt_b200 operators have no forward-mode derivative");
+}
+
 // A tensor that was kept for the backward pass: hooks on saved tensors may give back one of other strides, which is
 // copied; anything else is an error.
 Tensor saved(const Tensor& t, const char* name, at::ScalarType type, at::IntArrayRef shape, c10::Device dev) {
@@ -278,6 +284,7 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const 
                                         const std::optional<Tensor>& positions, const std::optional<Tensor>& q_weight,
                                         const std::optional<Tensor>& k_weight, double eps) {
   const Tensor pos = positions.value_or(Tensor()), wq = q_weight.value_or(Tensor()), wk = k_weight.value_or(Tensor());
+  no_forward_mode({&q, &k, &cos, &sin, &wq, &wk});
   const Rope a = rope_args(q, k, cos, sin, pos, wq, wk);
   const variable_list out = wants_grad({&q, &k, &wq, &wk})
                                 ? RopeNode::apply(q, k, wq.defined() ? wq : cos, wk.defined() ? wk : cos, a, eps)
@@ -415,6 +422,7 @@ struct FfnNode : torch::autograd::Function<FfnNode> {
 };
 
 Tensor gated_ffn(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const Tensor& w_down, int act, int keep) {
+  no_forward_mode({&x, &w_gate, &w_up, &w_down});
   const Ffn a = ffn_args(x, w_gate, w_up, w_down);
   if (wants_grad({&x, &w_gate, &w_up, &w_down})) return FfnNode::apply(x, w_gate, w_up, w_down, (int64_t)act, (int64_t)keep)[0];
   const at::NoGradGuard no_grad;

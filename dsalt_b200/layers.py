@@ -9,7 +9,8 @@
 The reference norms and rotates nothing but by elementwise torch operations
 (``dsalt/kernels/window_utils.py:73-88``) and runs its block's MLP as three linear layers
 (``dsalt/modules/dsalt_transformer.py``). As in :mod:`dsalt_b200.serving`, tensors must be CUDA
-tensors of one device and every call launches on its current stream; none synchronises. Checks,
+tensors of one device and every call launches on its current stream; none synchronises. Gradients are
+those of one backward pass: second and forward-mode derivatives are refused. Checks,
 outputs and autograd nodes are compiled (``csrc/torch_layers.cpp``): the calls are short.
 """
 from __future__ import annotations
