@@ -25,15 +25,17 @@ constexpr int64_t GROUP = 32;
 template <typename... Args>
 std::string words(const Args&... args) { return c10::str(args...); }
 
-void check(int rc, const char* fn) {
+// `python`: the call came from Python, not from autograd's own threads
+void check(int rc, const char* fn, bool python) {
   if (rc == DSALT_OK) return;
   const std::string msg = dsalt_last_error();
-  if (PyGILState_Check()) {
+  if (python) {
+    const py::gil_scoped_acquire gil;
     const py::object cls = py::module_::import("dsalt_b200._lib").attr("DsaltError");
     PyErr_SetObject(cls.ptr(), cls(rc, fn, msg).ptr());
     throw py::error_already_set();
   }
-  TORCH_CHECK(false, fn, " failed (status ", rc, "): ", msg);  // in autograd's own threads
+  TORCH_CHECK(false, fn, " failed (status ", rc, "): ", msg);
 }
 
 int type_code(const Tensor& t) {
@@ -109,7 +111,7 @@ std::tuple<Tensor, Tensor> pack_rows(const Tensor& m, int64_t stride, c10::Devic
   const Launch launch(dev);
   check(dsalt_pack8(m.data_ptr(), type_code(m), rows, n, stride, codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(),
                     launch.stream),
-        "dsalt_pack8");
+        "dsalt_pack8", true);
   return {codes, exps};
 }
 
@@ -139,7 +141,7 @@ Tensor unpack8(const Tensor& codes, const Tensor& exps, int dtype) {
   const Launch launch(dev);
   check(dsalt_unpack8(codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), n ? codes.numel() / n : 0, n, out.data_ptr(), dtype,
                       launch.stream),
-        "dsalt_unpack8");
+        "dsalt_unpack8", true);
   return out;
 }
 
@@ -225,7 +227,7 @@ variable_list rope_forward(const Tensor& q, const Tensor& k, const Rope& a, doub
                            (float)eps, a.cos.data_ptr<float>(), a.sin.data_ptr<float>(), std::max<int64_t>(a.cos.size(0), 1),
                            a.stride, static_cast<const int32_t*>(ptr(a.positions)), qo.data_ptr(), ko.data_ptr(),
                            launch.stream),
-        "dsalt_qk_norm_rope");
+        "dsalt_qk_norm_rope", true);
   return {qo, ko};
 }
 
@@ -268,7 +270,7 @@ struct RopeNode : torch::autograd::Function<RopeNode> {
                                  std::max<int64_t>(cos.size(0), 1), a.stride,
                                  static_cast<const int32_t*>(ptr(positions)), dq.data_ptr(), dk.data_ptr(), ptr(dwq), ptr(dwk),
                                  ptr(ws), norm ? (size_t)ws.numel() : 0, launch.stream),
-          "dsalt_qk_norm_rope_bwd");
+          "dsalt_qk_norm_rope_bwd", false);
     return {dq, dk, dwq, dwk, Tensor(), Tensor()};
   }
 };
@@ -351,7 +353,7 @@ Kept ffn_forward(const Tensor& x, const Tensor& m, int64_t stride, const Tensor&
   check(dsalt_gated_ffn(m.data_ptr(), dt, T, (int)a.d, stride, w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
                         (int)a.F, (int)a.d_out, act, keep, ptr(k.kept), static_cast<uint8_t*>(ptr(k.exps.defined() ? k.exps : k.kept)), k.y.data_ptr(),
                         ws.data_ptr(), (size_t)ws.numel(), launch.stream),
-        "dsalt_gated_ffn");
+        "dsalt_gated_ffn", true);
   return k;
 }
 
@@ -416,7 +418,7 @@ struct FfnNode : torch::autograd::Function<FfnNode> {
                               (int)d_out, (int)ctx->saved_data["act"].toInt(), keep, kept.data_ptr(),
                               static_cast<const uint8_t*>(ptr(exps.defined() ? exps : kept)), ptr(dx), ptr(dwg), ptr(dwu), ptr(dwd), ws.data_ptr(),
                               (size_t)ws.numel(), launch.stream),
-          "dsalt_gated_ffn_bwd");
+          "dsalt_gated_ffn_bwd", false);
     return {dx, ctx->needs_input_grad(1) ? dwg : Tensor(), ctx->needs_input_grad(2) ? dwu : Tensor(), dwd, Tensor(), Tensor()};
   }
 };
@@ -433,8 +435,10 @@ Tensor gated_ffn(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, cons
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-  m.def("pack8", &pack8);
-  m.def("unpack8", &unpack8);
-  m.def("qk_norm_rope", &qk_norm_rope);
-  m.def("gated_ffn", &gated_ffn);
+  // without the interpreter's lock: a launch waits where the queue is full, and what it waits for may need the lock
+  const py::call_guard<py::gil_scoped_release> free;
+  m.def("pack8", &pack8, free);
+  m.def("unpack8", &unpack8, free);
+  m.def("qk_norm_rope", &qk_norm_rope, free);
+  m.def("gated_ffn", &gated_ffn, free);
 }
