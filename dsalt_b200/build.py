@@ -47,26 +47,50 @@ def build(force: bool = False, verbose: bool = False) -> str:
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh"))] + [header]
     if force or not _newer(LIB, deps):
         _build_kernels(verbose)
-    if force or not _newer(TORCH_LIB, [TORCH_SOURCE, header]):
+    if force or not _newer(TORCH_LIB, [TORCH_SOURCE, header]) or _noted() != _torch_of():
         _build_torch_side()
     return LIB
 
 
+def _torch_of() -> str:
+    """What torch's side is compiled against: its classes have other layouts in another torch."""
+    import torch
+    return f"torch {torch.__version__}, C++11 ABI {int(torch._C._GLIBCXX_USE_CXX11_ABI)}, python {sys.version.split()[0]}"
+
+
+def _noted() -> str:
+    try:
+        with open(TORCH_LIB + ".torch") as f:
+            return f.read()
+    except OSError:
+        return ""
+
+
 def _build_torch_side() -> None:
+    _run_compiler(TORCH_LIB + ".tmp")
+    os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+    with open(TORCH_LIB + ".torch", "w") as f:
+        f.write(_torch_of())
+
+
+def _torch_command(target: str) -> list:
     import sysconfig
 
+    import torch
     from torch.utils.cpp_extension import include_paths, library_paths
     cuda = os.path.dirname(os.path.dirname(nvcc()))
     include = [*include_paths(), sysconfig.get_path("include"), os.path.join(cuda, "include")]
     # the g++ that nvcc takes too: another one may link a C++ library of its own beside torch's
-    cmd = [shutil.which("g++") or os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_torch_layers",
-           "-D_GLIBCXX_USE_CXX11_ABI=1", *[a for p in include for a in ("-isystem", p)], "-I", os.path.join(ROOT, "include"),
-           TORCH_SOURCE, "-o", TORCH_LIB + ".tmp", "-L" + OUT_DIR, "-ldsalt_b200", "-Wl,-rpath,$ORIGIN",
+    return [shutil.which("g++") or os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_torch_layers",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[a for p in include for a in ("-isystem", p)], "-I", os.path.join(ROOT, "include"),
+           TORCH_SOURCE, "-o", target, "-L" + OUT_DIR, "-ldsalt_b200", "-Wl,-rpath,$ORIGIN",
            *["-L" + p for p in library_paths()], "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
+
+
+def _run_compiler(target: str) -> None:
+    res = subprocess.run(_torch_command(target), capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError("g++ failed:\n" + res.stderr[-8000:])
-    os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
 
 
 def _build_kernels(verbose: bool) -> None:
