@@ -231,6 +231,30 @@ variable_list rope_forward(const Tensor& q, const Tensor& k, const Rope& a, doub
   return {qo, ko};
 }
 
+// the gradients of q, k and the weights (undefined where there are none) from those of the outputs, of which one that
+// nothing used is undefined
+variable_list rope_backward(const Tensor& dq_out, const Tensor& dk_out, const Tensor& q, const Tensor& k, const Rope& a,
+                            double eps, bool python) {
+  const int64_t T = a.T, H = a.H, D = a.D, Hk = a.Hk;
+  const bool norm = a.q_weight.defined();
+  Tensor dq = empty({T, H, D}, q.scalar_type(), a.dev), dk = empty({T, Hk, D}, q.scalar_type(), a.dev), dwq, dwk, ws;
+  if (norm) {
+    dwq = empty({D}, a.q_weight.scalar_type(), a.dev), dwk = empty({D}, a.q_weight.scalar_type(), a.dev);
+    ws = workspace(dsalt_qk_norm_rope_bwd_workspace_bytes((int)D), a.dev);
+  }
+  const Heads x = heads(q), y = heads(k);
+  const Heads gx = heads(dq_out.defined() ? dq_out : at::zeros_like(dq)), gy = heads(dk_out.defined() ? dk_out : at::zeros_like(dk));
+  const Launch launch(a.dev);
+  check(dsalt_qk_norm_rope_bwd(x.t.data_ptr(), y.t.data_ptr(), gx.t.data_ptr(), gy.t.data_ptr(), type_code(q), T, (int)H,
+                               (int)Hk, (int)D, x.token, x.head, y.token, y.head, gx.token, gx.head, gy.token, gy.head,
+                               ptr(a.q_weight), ptr(a.k_weight), norm ? type_code(a.q_weight) : 0, (float)eps,
+                               a.cos.data_ptr<float>(), a.sin.data_ptr<float>(), std::max<int64_t>(a.cos.size(0), 1), a.stride,
+                               static_cast<const int32_t*>(ptr(a.positions)), dq.data_ptr(), dk.data_ptr(), ptr(dwq), ptr(dwk),
+                               ptr(ws), norm ? (size_t)ws.numel() : 0, launch.stream),
+        "dsalt_qk_norm_rope_bwd", python);
+  return {dq, dk, dwq, dwk};
+}
+
 // q and k are kept as they came; the norms are formed again in the backward pass
 struct RopeNode : torch::autograd::Function<RopeNode> {
   // the weights are arguments of their own (any tensor where there are none), so that the node sees them
@@ -248,30 +272,10 @@ struct RopeNode : torch::autograd::Function<RopeNode> {
                     (!grads[0].defined() || grads[0].sizes() == q.sizes()) &&
                     (!grads[1].defined() || grads[1].sizes() == k.sizes()),
                 "the saved heads came back as other tensors");
-    const Rope a = rope_args(q, k, s[4], s[5], s[6], s[2], s[3]);
-    const Tensor &q_weight = a.q_weight, &k_weight = a.k_weight, &cos = a.cos, &sin = a.sin, &positions = a.positions;
-    const c10::Device dev = a.dev;
-    const int64_t T = a.T, H = a.H, D = a.D, Hk = a.Hk;
-    const bool norm = q_weight.defined();
-    Tensor dq = empty({T, H, D}, q.scalar_type(), dev), dk = empty({T, Hk, D}, q.scalar_type(), dev), dwq, dwk, ws;
-    if (norm) {
-      dwq = empty({D}, q_weight.scalar_type(), dev), dwk = empty({D}, q_weight.scalar_type(), dev);
-      ws = workspace(dsalt_qk_norm_rope_bwd_workspace_bytes((int)D), dev);
-    }
-    const Heads x = heads(q), y = heads(k);
-    // an output that nothing used has no gradient
-    const Heads gx = heads(grads[0].defined() ? grads[0] : at::zeros_like(dq)),
-                gy = heads(grads[1].defined() ? grads[1] : at::zeros_like(dk));
-    const Launch launch(dev);
-    check(dsalt_qk_norm_rope_bwd(x.t.data_ptr(), y.t.data_ptr(), gx.t.data_ptr(), gy.t.data_ptr(), type_code(q), T, (int)H,
-                                 (int)Hk, (int)D, x.token, x.head, y.token, y.head, gx.token, gx.head, gy.token, gy.head,
-                                 ptr(q_weight), ptr(k_weight), norm ? type_code(q_weight) : 0,
-                                 (float)ctx->saved_data["eps"].toDouble(), cos.data_ptr<float>(), sin.data_ptr<float>(),
-                                 std::max<int64_t>(cos.size(0), 1), a.stride,
-                                 static_cast<const int32_t*>(ptr(positions)), dq.data_ptr(), dk.data_ptr(), ptr(dwq), ptr(dwk),
-                                 ptr(ws), norm ? (size_t)ws.numel() : 0, launch.stream),
-          "dsalt_qk_norm_rope_bwd", false);
-    return {dq, dk, dwq, dwk, Tensor(), Tensor()};
+    variable_list d = rope_backward(grads[0], grads[1], q, k, rope_args(q, k, s[4], s[5], s[6], s[2], s[3]),
+                                    ctx->saved_data["eps"].toDouble(), false);
+    d.resize(6);
+    return d;
   }
 };
 
@@ -292,6 +296,22 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const 
                                 ? RopeNode::apply(q, k, wq.defined() ? wq : cos, wk.defined() ? wk : cos, a, eps)
                                 : rope_forward(q, k, a, eps);
   return {out[0], out[1]};
+}
+
+// the gradients for a registered operator, whose outputs are all tensors: empty where there is no weight
+variable_list qk_norm_rope_grads(const Tensor& dq_out, const Tensor& dk_out, const Tensor& q, const Tensor& k, const Tensor& cos,
+                                 const Tensor& sin, const std::optional<Tensor>& positions, const std::optional<Tensor>& q_weight,
+                                 const std::optional<Tensor>& k_weight, double eps) {
+  const at::NoGradGuard no_grad;
+  const Rope a = rope_args(q, k, cos, sin, positions.value_or(Tensor()), q_weight.value_or(Tensor()), k_weight.value_or(Tensor()));
+  one_device({&q, &dq_out, &dk_out});
+  if (dq_out.sizes() != q.sizes() || dk_out.sizes() != k.sizes()) throw py::value_error("gradients must have the shapes of q and k");
+  if (dq_out.scalar_type() != q.scalar_type() || dk_out.scalar_type() != q.scalar_type())
+    throw py::type_error("gradients must have the dtype of q and k");
+  variable_list d = rope_backward(dq_out, dk_out, q, k, a, eps, true);
+  for (Tensor& t : d)
+    if (!t.defined()) t = empty({0}, q.scalar_type(), a.dev);
+  return d;
 }
 
 // --------------------------------------------------------------------------- feed-forward
@@ -357,6 +377,34 @@ Kept ffn_forward(const Tensor& x, const Tensor& m, int64_t stride, const Tensor&
   return k;
 }
 
+// x as the weights' gradients read it: rows, or codes and their scales
+struct Rows {
+  Tensor t;
+  int64_t stride;
+  Tensor exps;
+};
+// the gradients of x and the weights that are wanted
+variable_list ffn_backward(const Tensor& grad, const Rows& x, const Kept& k, const Tensor& wg, const Tensor& wu, const Tensor& wd,
+                           const Ffn& a, at::IntArrayRef x_shape, int act, int keep, const bool (&wanted)[4], bool python) {
+  const at::ScalarType type = grad.scalar_type();
+  const int dt = type_code(grad);
+  const int64_t T = grad.numel() / a.d_out;
+  const auto [dy, dy_stride] = ffn_rows(grad.reshape({T, a.d_out}));
+  Tensor dx, dwg, dwu, dwd;
+  if (wanted[0]) dx = empty(x_shape, type, a.dev);
+  if (wanted[1] || wanted[2]) dwg = empty({a.F, a.d}, type, a.dev), dwu = empty({a.F, a.d}, type, a.dev);
+  if (wanted[3]) dwd = empty({a.d_out, a.F}, type, a.dev);
+  const Tensor ws = workspace(dsalt_gated_ffn_bwd_workspace_bytes(dt, T, (int)a.d, (int)a.F, (int)a.d_out, keep), a.dev);
+  const Launch launch(a.dev);
+  check(dsalt_gated_ffn_bwd(dy.data_ptr(), dt, T, (int)a.d, dy_stride, ptr(x.t), x.stride,
+                            static_cast<const uint8_t*>(ptr(x.exps)), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), (int)a.F,
+                            (int)a.d_out, act, keep, k.kept.data_ptr(),
+                            static_cast<const uint8_t*>(ptr(k.exps.defined() ? k.exps : k.kept)), ptr(dx), ptr(dwg), ptr(dwu),
+                            ptr(dwd), ws.data_ptr(), (size_t)ws.numel(), launch.stream),
+        "dsalt_gated_ffn_bwd", python);
+  return {dx, wanted[1] ? dwg : Tensor(), wanted[2] ? dwu : Tensor(), dwd};
+}
+
 // Kept for the backward pass: gate's and up's sums and x, in 24 bits and as it is, or in 8 bits. The rows that
 // the last product read are formed again; of fp32 inputs everything is kept as it is, those rows too.
 struct FfnNode : torch::autograd::Function<FfnNode> {
@@ -387,7 +435,6 @@ struct FfnNode : torch::autograd::Function<FfnNode> {
     const bool coded = keep == DSALT_KEEP_8BIT;
     const c10::Device dev = grads[0].device();
     const at::ScalarType type = grads[0].scalar_type();
-    const int dt = type_code(grads[0]);
     const Tensor kept = saved(s[2], "activations", coded ? at::kChar : type, {coded ? 2 : 3, T, pitch}, dev);
     const Tensor wg = ffn_weight(saved(s[4], "gate weight", type, {F, d}, dev)),
                  wu = ffn_weight(saved(s[5], "up weight", type, {F, d}, dev)),
@@ -405,21 +452,11 @@ struct FfnNode : torch::autograd::Function<FfnNode> {
         std::tie(x, x_stride) = ffn_rows(s[0]);
       }
     }
-    const auto [dy, dy_stride] = ffn_rows(grads[0].reshape({T, d_out}));
-    Tensor dx, dwg, dwu, dwd;
-    if (ctx->needs_input_grad(0)) dx = empty(shape, type, dev);
-    const bool both = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
-    if (both) dwg = empty({F, d}, type, dev), dwu = empty({F, d}, type, dev);
-    if (ctx->needs_input_grad(3)) dwd = empty({d_out, F}, type, dev);
-    const Tensor ws = workspace(dsalt_gated_ffn_bwd_workspace_bytes(dt, T, (int)d, (int)F, (int)d_out, keep), dev);
-    const Launch launch(dev);
-    check(dsalt_gated_ffn_bwd(dy.data_ptr(), dt, T, (int)d, dy_stride, ptr(x), x_stride,
-                              static_cast<const uint8_t*>(ptr(x_exps)), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), (int)F,
-                              (int)d_out, (int)ctx->saved_data["act"].toInt(), keep, kept.data_ptr(),
-                              static_cast<const uint8_t*>(ptr(exps.defined() ? exps : kept)), ptr(dx), ptr(dwg), ptr(dwu), ptr(dwd), ws.data_ptr(),
-                              (size_t)ws.numel(), launch.stream),
-          "dsalt_gated_ffn_bwd", false);
-    return {dx, ctx->needs_input_grad(1) ? dwg : Tensor(), ctx->needs_input_grad(2) ? dwu : Tensor(), dwd, Tensor(), Tensor()};
+    const bool wanted[4] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2), ctx->needs_input_grad(3)};
+    variable_list out = ffn_backward(grads[0], {x, x_stride, x_exps}, {Tensor(), kept, exps}, wg, wu, wd, {dev, d, F, d_out},
+                                     shape, (int)ctx->saved_data["act"].toInt(), keep, wanted, false);
+    out.resize(6);
+    return out;
   }
 };
 
@@ -432,6 +469,28 @@ Tensor gated_ffn(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, cons
   return ffn_forward(x, m, stride, ffn_weight(w_gate), ffn_weight(w_up), ffn_weight(w_down), a, act, DSALT_KEEP_NONE).y;
 }
 
+// The gradients for a registered operator, which keeps its inputs alone: what the backward pass reads is formed again.
+// Empty where one is not wanted.
+variable_list gated_ffn_grads(const Tensor& dy, const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const Tensor& w_down,
+                              int act, std::vector<bool> wanted) {
+  const at::NoGradGuard no_grad;
+  const Ffn a = ffn_args(x, w_gate, w_up, w_down);
+  one_device({&x, &dy});
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = a.d_out;
+  if (dy.sizes() != at::IntArrayRef(shape)) throw py::value_error(words("the gradient must have shape ", shape, ", got ", dy.sizes()));
+  if (dy.scalar_type() != x.scalar_type()) throw py::type_error("the gradient must have the dtype of x");
+  if (wanted.size() != 4) throw py::value_error("wanted names x and three weights");
+  const auto [m, stride] = ffn_rows(x);
+  const Tensor wg = ffn_weight(w_gate), wu = ffn_weight(w_up), wd = ffn_weight(w_down);
+  const Kept k = ffn_forward(x, m, stride, wg, wu, wd, a, act, DSALT_KEEP_INPUT);
+  const bool which[4] = {wanted[0], wanted[1], wanted[2], wanted[3]};
+  variable_list d = ffn_backward(dy, {m, stride, Tensor()}, k, wg, wu, wd, a, x.sizes(), act, DSALT_KEEP_INPUT, which, true);
+  for (Tensor& t : d)
+    if (!t.defined()) t = empty({0}, x.scalar_type(), a.dev);
+  return d;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -441,4 +500,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("unpack8", &unpack8, free);
   m.def("qk_norm_rope", &qk_norm_rope, free);
   m.def("gated_ffn", &gated_ffn, free);
+  m.def("qk_norm_rope_grads", &qk_norm_rope_grads, free);
+  m.def("gated_ffn_grads", &gated_ffn_grads, free);
 }

@@ -13,7 +13,9 @@ keeps its kernels opaque (``_dynamo_opaque``, ``dsalt/kernels/dsalt_triton_attn.
   numbers and the log-probability)
 
 * ``torch.ops.dsalt_b200.qk_norm_rope`` / ``gated_ffn`` / ``pack8`` / ``unpack8``
-  → the functions of :mod:`dsalt_b200.layers` of these names, without gradients
+  → the functions of :mod:`dsalt_b200.layers` of these names. The first two have gradients, formed by
+  ``qk_norm_rope_backward`` and ``gated_ffn_backward``: a graph keeps their inputs alone, and the
+  backward pass forms again what else it reads
 
 ``cu_list`` (the host copy of ``cu_seqlens``) is an ``int[]`` argument: the kernels size
 their launches and workspaces from it, so a compiled graph is specialised on the packing.
@@ -26,6 +28,7 @@ from typing import List, Optional
 
 import torch
 
+from . import _lib as L
 from . import layers
 from . import ops
 from . import serving
@@ -140,6 +143,34 @@ def _(q, k, cos, sin, positions, q_weight, k_weight, eps):
     return [q.new_empty(q.shape), k.new_empty(k.shape)]
 
 
+@torch.library.custom_op("dsalt_b200::qk_norm_rope_backward", mutates_args=())
+def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor,
+                          sin: torch.Tensor, positions: Optional[torch.Tensor], q_weight: Optional[torch.Tensor],
+                          k_weight: Optional[torch.Tensor], eps: float) -> List[torch.Tensor]:
+    return L.torch_layers().qk_norm_rope_grads(dq, dk, q, k, cos, sin, positions, q_weight, k_weight, eps)
+
+
+@qk_norm_rope_backward.register_fake
+def _(dq, dk, q, k, cos, sin, positions, q_weight, k_weight, eps):
+    return [q.new_empty(q.shape), k.new_empty(k.shape),
+            *(q.new_empty(0) if w is None else w.new_empty(w.shape) for w in (q_weight, k_weight))]
+
+
+def _keep_heads(ctx, inputs, output):
+    *tensors, ctx.eps = inputs
+    ctx.save_for_backward(*tensors)
+
+
+def _heads_backward(ctx, grads):
+    q, k, cos, sin, positions, q_weight, k_weight = ctx.saved_tensors
+    dq, dk = (torch.zeros_like(t) if d is None else d for d, t in zip(grads, (q, k)))
+    dq, dk, dwq, dwk = torch.ops.dsalt_b200.qk_norm_rope_backward(dq, dk, q, k, cos, sin, positions, q_weight, k_weight, ctx.eps)
+    return dq, dk, None, None, None, *((None, None) if q_weight is None else (dwq, dwk)), None
+
+
+qk_norm_rope.register_autograd(_heads_backward, setup_context=_keep_heads)
+
+
 @torch.library.custom_op("dsalt_b200::gated_ffn", mutates_args=())
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
               activation: str) -> torch.Tensor:
@@ -149,6 +180,34 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 @gated_ffn.register_fake
 def _(x, w_gate, w_up, w_down, activation):
     return x.new_empty(x.shape[:-1] + (w_down.shape[0],))
+
+
+@torch.library.custom_op("dsalt_b200::gated_ffn_backward", mutates_args=())
+def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+                       activation: str, wanted: List[bool]) -> List[torch.Tensor]:
+    ts = x, w_gate, w_up, w_down
+    cast = (t.to(dy.dtype) for t in ts)  # as autocast had them in the forward pass
+    grads = L.torch_layers().gated_ffn_grads(dy, *cast, layers.ACTIVATIONS[activation], wanted)
+    return [g.to(t.dtype) for g, t in zip(grads, ts)]
+
+
+@gated_ffn_backward.register_fake
+def _(dy, x, w_gate, w_up, w_down, activation, wanted):
+    return [t.new_empty(t.shape if w else 0) for t, w in zip((x, w_gate, w_up, w_down), wanted)]
+
+
+def _keep_ffn(ctx, inputs, output):
+    *tensors, ctx.activation = inputs
+    ctx.save_for_backward(*tensors)
+
+
+def _ffn_backward(ctx, dy):
+    wanted = list(ctx.needs_input_grad[:4])
+    grads = torch.ops.dsalt_b200.gated_ffn_backward(dy, *ctx.saved_tensors, ctx.activation, wanted)
+    return *(g if w else None for g, w in zip(grads, wanted)), None
+
+
+gated_ffn.register_autograd(_ffn_backward, setup_context=_keep_ffn)
 
 
 @torch.library.custom_op("dsalt_b200::pack8", mutates_args=())
