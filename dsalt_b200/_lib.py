@@ -75,6 +75,7 @@ SIGNATURES = {
                                                                                          _I64] + [_P] * 6 + [_SZ, _P]),
     "dsalt_gated_ffn_pitch": (_I64, [_I]),
     "dsalt_gated_ffn_workspace_bytes": (_SZ, [_I, _I64, _I, _I, _I]),
+    "dsalt_gated_ffn_keep_workspace_bytes": (_SZ, [_I, _I64, _I, _I, _I, _I]),
     "dsalt_gated_ffn": (_I, [_P, _I, _I64, _I, _I64, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _SZ, _P]),
     "dsalt_gated_ffn_bwd_workspace_bytes": (_SZ, [_I, _I64, _I, _I, _I, _I]),
     "dsalt_gated_ffn_bwd": (_I, [_P, _I, _I64, _I, _I64, _P, _I64, _P, _P, _P, _P, _I, _I, _I, _I] + [_P] * 7

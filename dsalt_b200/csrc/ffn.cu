@@ -73,9 +73,9 @@ __global__ void __launch_bounds__(THREADS) product_kernel(const Product p, TO* _
       if (m0 + tm + i < p.M && n0 + tn + j < p.N) c[(m0 + tm + i) * p.c_stride + n0 + tn + j] = from_float<TO>(acc[i][j]);
 }
 
-// a warp per 32 columns of a row: h and what is kept
+// a warp per 32 columns of a row: h and what is kept (of fp32: g and u lie there already, but for the columns behind F)
 template <typename T, int ACT>
-__global__ void __launch_bounds__(THREADS) act_kernel(const float* __restrict__ g, const float* __restrict__ u, int64_t T_,
+__global__ void __launch_bounds__(THREADS) act_kernel(const float* g, const float* u, int64_t T_,
                                                       int F, int64_t pitch, T* __restrict__ h, void* kept,
                                                       uint8_t* __restrict__ exps, int keep) {
   const int lane = threadIdx.x % 32;
@@ -87,8 +87,7 @@ __global__ void __launch_bounds__(THREADS) act_kernel(const float* __restrict__ 
     const float a = in ? g[at] : 0.f, b = in ? u[at] : 0.f;
     h[at] = from_float<T>(activate<ACT, false>(a) * b);
     if (sizeof(T) == 4 && keep == DSALT_KEEP_INPUT) {
-      static_cast<float*>(kept)[at] = a;
-      static_cast<float*>(kept)[plane + at] = b;
+      if (!in) static_cast<float*>(kept)[at] = static_cast<float*>(kept)[plane + at] = 0.f;
     } else if (keep == DSALT_KEEP_INPUT) {
       uint16_t* to = static_cast<uint16_t*>(kept) + at;
       to[0] = (uint16_t)upper_halves(a, 0.f);
@@ -163,8 +162,9 @@ bool keeps_h(int dtype, int keep) { return dtype == DSALT_F32 && keep == DSALT_K
 
 template <typename T, int ACT>
 int forward_plain(const Ffn& f) {
-  float* g = f.wide;
-  float* u = f.wide + f.T * f.pitch;
+  // of fp32 inputs that keep their activations the sums are formed where they are kept
+  float* g = keeps_h(f.dtype, f.keep) ? static_cast<float*>(f.kept) : f.wide;
+  float* u = g + f.T * f.pitch;
   int rc;
   for (int i = 0; i < 2; ++i) {
     const Product p = {{{f.x, f.x_stride, 1}}, {{i ? f.w_up : f.w_gate, f.d, 1}}, 1, f.T, f.F, f.d, f.pitch};
@@ -257,7 +257,12 @@ extern "C" {
 int64_t dsalt_gated_ffn_pitch(int d_ff) { return d_ff < 1 ? 0 : pitch_of(d_ff); }
 
 size_t dsalt_gated_ffn_workspace_bytes(int dtype, int64_t T, int d_model, int d_ff, int d_out) {
-  if (check("gated_ffn", dtype, T, d_model, d_ff, d_out, 0, 0)) return 0;
+  return dsalt_gated_ffn_keep_workspace_bytes(dtype, T, d_model, d_ff, d_out, DSALT_KEEP_NONE);
+}
+
+size_t dsalt_gated_ffn_keep_workspace_bytes(int dtype, int64_t T, int d_model, int d_ff, int d_out, int keep) {
+  if (check("gated_ffn", dtype, T, d_model, d_ff, d_out, 0, keep)) return 0;
+  if (keeps_h(dtype, keep)) return 256;
   const size_t n = (size_t)T * pitch_of(d_ff);
   return a256(n * elem_bytes(dtype)) + (tensor_cores(dtype, d_model, d_ff, d_out) ? 0 : a256(2 * n * sizeof(float))) + 256;
 }
@@ -272,7 +277,7 @@ int dsalt_gated_ffn(const void* x, int dtype, int64_t T, int d_model, int64_t x_
   if (!x || !w_gate || !w_up || !w_down || !y || !workspace || (keep && !kept) || (scaled(dtype, keep) && !kept_exps))
     return fail(DSALT_ERR_INVALID, "%s: null pointer", FN);
   if (off256(kept) || off256(workspace)) return fail(DSALT_ERR_INVALID, "%s: kept and workspace must be 256-byte aligned", FN);
-  if (workspace_bytes < dsalt_gated_ffn_workspace_bytes(dtype, T, d_model, d_ff, d_out))
+  if (workspace_bytes < dsalt_gated_ffn_keep_workspace_bytes(dtype, T, d_model, d_ff, d_out, keep))
     return fail(DSALT_ERR_WORKSPACE, "%s: workspace of %zu bytes is too small", FN, workspace_bytes);
   Ffn f{};
   f.dtype = dtype, f.act = activation, f.keep = keep, f.T = T, f.d = d_model, f.F = d_ff, f.d_out = d_out;

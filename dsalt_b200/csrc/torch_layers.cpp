@@ -368,7 +368,7 @@ Kept ffn_forward(const Tensor& x, const Tensor& m, int64_t stride, const Tensor&
     k.kept = empty({coded ? 2 : 3, T, pitch}, coded ? at::kChar : m.scalar_type(), a.dev);
     if (coded) k.exps = empty({2, pitch / GROUP, T}, at::kByte, a.dev);
   }
-  const Tensor ws = workspace(dsalt_gated_ffn_workspace_bytes(dt, T, (int)a.d, (int)a.F, (int)a.d_out), a.dev);
+  const Tensor ws = workspace(dsalt_gated_ffn_keep_workspace_bytes(dt, T, (int)a.d, (int)a.F, (int)a.d_out, keep), a.dev);
   const Launch launch(a.dev);
   check(dsalt_gated_ffn(m.data_ptr(), dt, T, (int)a.d, stride, w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
                         (int)a.F, (int)a.d_out, act, keep, ptr(k.kept), static_cast<uint8_t*>(ptr(k.exps.defined() ? k.exps : k.kept)), k.y.data_ptr(),

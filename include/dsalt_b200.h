@@ -477,6 +477,8 @@ int dsalt_qk_norm_rope_bwd(const void* q, const void* k, const void* dq_out, con
 #define DSALT_KEEP_8BIT 2
 int64_t dsalt_gated_ffn_pitch(int d_ff);
 size_t dsalt_gated_ffn_workspace_bytes(int dtype, int64_t T, int d_model, int d_ff, int d_out);
+/* with what is kept: DSALT_KEEP_INPUT of fp32 needs almost none */
+size_t dsalt_gated_ffn_keep_workspace_bytes(int dtype, int64_t T, int d_model, int d_ff, int d_out, int keep);
 int dsalt_gated_ffn(const void* x, int dtype, int64_t T, int d_model, int64_t x_stride, const void* w_gate,
                     const void* w_up, const void* w_down, int d_ff, int d_out, int activation, int keep, void* kept,
                     uint8_t* kept_exps, void* y, void* workspace, size_t workspace_bytes, void* stream);
