@@ -37,3 +37,39 @@ def test_a_full_launch_queue_does_not_stop_other_threads(name):
     worker.join()
     torch.cuda.synchronize()
     assert longest < 0.2, f"another thread stood still for {longest:.2f} s"
+
+
+def test_calls_reach_what_is_written_in_python():
+    """Without the lock: anomaly detection, hooks on saved tensors and a mode that sees every operation take it themselves."""
+    import dsalt_b200 as D
+    from torch.utils._python_dispatch import TorchDispatchMode
+    x = torch.randn(40, 64, device="cuda").bfloat16().requires_grad_(True)
+    w = [torch.randn(64, 64, device="cuda").bfloat16().mul_(0.1).requires_grad_(True) for _ in range(3)]
+    n = torch.ones(64, device="cuda", requires_grad=True)
+    t = torch.randn(40, 64, device="cuda")
+
+    def step():
+        y = D.gated_ffn(x, *w, keep="8bit").view(40, 1, 64)
+        q, k = D.qk_norm_rope(y, y, t, t, q_weight=n, k_weight=n)
+        return [q.detach(), *torch.autograd.grad((q, k), [x, *w, n], (q.detach(), k.detach()))]
+
+    class Seen(TorchDispatchMode):
+        names = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    ref = step()
+    packed = []
+    with torch.autograd.detect_anomaly(check_nan=False):
+        runs = [step()]
+    with torch.autograd.graph.saved_tensors_hooks(lambda s: packed.append(s) or s, lambda s: s):
+        runs.append(step())
+    with Seen():
+        runs.append(step())
+    assert packed and Seen.names
+    for got in runs:
+        assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    with pytest.raises(D.DsaltError):
+        D.qk_norm_rope(torch.ones(4, 1, 20, device="cuda"), torch.ones(4, 1, 20, device="cuda"), t[:4, :20], t[:4, :20])
