@@ -8,7 +8,7 @@
 // and a long K: the CTAs of a cluster share 128 rows and take equal parts of K, and add up their fp32 sums
 // through each other's shared memory in the order of their ranks (results repeat bit for bit). It is
 // launched while the first one runs and asks for its first weights before it waits for h. 64 tokens, 2048 ->
-// 11008 in bf16 (135 MB of weights): 33 us in a row, 4.1 TB/s; memory's own rate gives 21.
+// 11008 in bf16 (135 MB of weights): 34 to 35 us in a row, 3.9 TB/s; memory's own rate gives 21.
 #include "ffn_tc.cuh"
 
 namespace dsalt {

@@ -3,8 +3,7 @@
 //
 //   forward    gate, up = x [Wg | Wu]^T -> epilogue: h = act(gate) up, gate and up kept if a gradient
 //              will be wanted;  y = h Wd^T
-//   backward   dh = dy Wd -> epilogue: dg = dh up act'(gate), du = dh act(gate), of 8-bit
-//              activations h again;
+//   backward   dh = dy Wd -> epilogue: dg = dh up act'(gate), du = dh act(gate), and h again;
 //              dx = dg Wg + du Wu (one sum over both);  dWg = dg^T x, dWu = du^T x, dWd = dy^T h, all
 //              in one launch
 //
@@ -19,9 +18,9 @@
 // Bound by what an SM can take from L2, 64 bytes a cycle: a stage of 32 KB feeds 512 cycles of products, so
 // at the tensor cores' full rate the operands alone fill that path (85 to 90 % of the rate is reached),
 // and what an epilogue writes and reads (up to 8 and 6 bytes for each of T x d_ff values) comes on top. Long runs
-// are bound by the power limit, under which the clock falls from 1.9 to 1.4 GHz. Measured, bf16: 32768 x 2048 ->
-// 11008 forward 2.76 ms (1610 TFLOP/s) cold and 3.13 to 3.25 ms (1360 to 1420) in a row; 32768 x 768 -> 2048 forward, 16 bits kept,
-// and backward 692 us (1340 TFLOP/s); 16384 x 1024 -> 4096, 8 bits kept, 944 us (1310); 1999 x 768 -> 2048 33 us.
+// are bound by the power limit, under which the clock falls from 1.9 to 1.3 GHz. Measured, bf16, a call alone and in a row: 32768 x
+// 2048 -> 11008 forward 2.9 ms (1530 TFLOP/s) and 3.3 (1330); 32768 x 768 -> 2048 forward, 16 bits kept, and backward
+// 0.78 and 0.94 (1180 and 990); 16384 x 1024 -> 4096, 8 bits kept, 0.96 and 1.12 (1290 and 1100); 1999 x 768 -> 2048 30 us.
 #include "ffn_tc.cuh"
 
 namespace dsalt {
@@ -674,9 +673,11 @@ void size_job(Job& j, int64_t M, int64_t N, int64_t K, int tile_n) {
   j.blocks0 = j.blocks = ceil_div(K, KB);
   // Columns of tiles are walked once for every `group` of 256 rows. Where the walked operand (the first product's:
   // gate's and up's) is more than half of L2, it comes from memory each time, so that it should be seldom: 32768 x
-  // 2048 -> 11008 in a row, which the power limit bounds, 3.71 ms with 4, 3.61 with 8, 3.49 with 16, 3.55 with 24. Smaller ones
-  // stay in L2, and 4, which share A among more pairs, are as fast or faster (16384 x 1024 -> 4096, training: 1105 us
-  // against 1125 with 16).
+  // 2048 -> 11008 in a row, which the power limit bounds, on one GPU 3.71 ms with 4, 3.61 with 8, 3.49 with 16, 3.55 with 24 (3.3
+  // with 16 on others). Smaller ones stay in L2, and 4, which share A among more pairs, are as fast or faster (16384 x 1024 ->
+  // 4096, training: 1105 us against 1125 with 16). Of x's gradient one of the two segments counts: with both, 16384 x
+  // 2048 -> 11008, 16384 x 1536 -> 12288 and 8192 x 2048 -> 8192 would get 16, and their training steps take as long
+  // (5.6, 5.1, 2.1 ms either way).
   j.group = N * K * (tile_n == PAIR_N ? 2 : 4) > HALF_L2 ? 16 : 4;
   j.rows = (int)M;
   j.cols = (int)N;
@@ -892,8 +893,10 @@ int run_tensor_cores(const Ffn& f, bool back) {
   //   2048 -> 5504:  64 tokens - | 24 | 34; 256 - | 32 | 35; 384 - | 39 | 46; 544 - | 61 | 49
   //   2048 -> 11008: 16 tokens 36 | 29.7 | 54; 64 tokens - | 33 | 54; 192 - | 45 | 54; 224 - | 58 | 54
   //   4096 -> 28672: 64 tokens - | 131 | 169; 128 - | 139 | 170; 160 - | 175 | 171
-  // Nine to sixteen tokens cost the stream 0.21 us a MB of weights, the tiles 0.14 and 4 us more. The tiles win
-  // while their CTAs run at once, two an SM with some 128 tokens each: that is T d_ff.
+  // Nine to sixteen tokens, stream | tiles by millions of weights: 19 M 12.7 | 17.0, 25 M 14.4 | 20.0 (d_ff = 2 d) and 18.6 | 19.2,
+  // 34 M 21.6 | 22.2, 41 M 23.5 | 23.7 (16 tokens 24.4 | 24.0), 53 M 33 | 27.5: they meet at 40 M. The tiles for few tokens win
+  // over this file's while their CTAs run at once, two an SM with some 128 tokens each: that is T d_ff (measured for d_ff
+  // of 2.7 to 7 times d only).
   if (!back && f.keep == DSALT_KEEP_NONE) {
     const int64_t weights = (int64_t)f.F * (2 * f.d + f.d_out);
     if (f.T <= 8 || (f.T <= 16 && weights <= 40000000)) return forward_tokens(f);

@@ -8,8 +8,8 @@
 // products, and the same 16 bytes of a token. All loads of BATCH x 32 values of K are under way before the
 // first is used. The warps of a block, and the blocks of a cluster, take parts of K; their sums are
 // added in the order of their ranks (results repeat bit for bit). The second product is launched while the
-// first one runs and loads its first weights before it waits for h. One token in bf16: 1024 -> 4096 (25 MB
-// of weights) 10.4 us, 2048 -> 11008 (135 MB) 27 us, 5 TB/s.
+// first one runs and loads its first weights before it waits for h. One token in bf16, weights from
+// memory: 1024 -> 4096 (25 MB) 8.8 us, 2048 -> 11008 (135 MB) 27 us, 5 TB/s.
 #include "ffn_tc.cuh"
 
 namespace dsalt {

@@ -104,8 +104,8 @@ class RMSENorm(nn.Module):
 
 class SwiGLUFFN(nn.Module):
     """``down(silu(gate(x)) * up(x))``: by library products, or (``kind`` ``"fused"``, ``"fused_8bit"``) by
-    :func:`dsalt_b200.layers.gated_ffn`, whose backward pass finds its activations in the weights' dtype or
-    in 8 bits."""
+    :func:`dsalt_b200.layers.gated_ffn`, whose backward pass finds its activations with 16 significant
+    bits or in 8 (fp32: as they are). Compiled, it keeps its input alone and forms the rest again."""
 
     def __init__(self, d_model: int, d_ff: int, dropout: float = 0.0, kind: str = "library"):
         super().__init__()
