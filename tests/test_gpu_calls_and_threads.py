@@ -73,3 +73,38 @@ def test_calls_reach_what_is_written_in_python():
         assert all(torch.equal(a, b) for a, b in zip(got, ref))
     with pytest.raises(D.DsaltError):
         D.qk_norm_rope(torch.ones(4, 1, 20, device="cuda"), torch.ones(4, 1, 20, device="cuda"), t[:4, :20], t[:4, :20])
+
+
+def test_two_threads_at_once():
+    import dsalt_b200 as D
+
+    def inputs(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        new = lambda *s: torch.randn(*s, device="cuda", generator=g).bfloat16().mul_(0.2).requires_grad_(True)  # noqa: E731
+        T = 300 + 200 * seed
+        return [new(T, 128), new(264, 128), new(264, 128), new(64, 264)], torch.ones(64, device="cuda"), torch.randn(T, 64, device="cuda")
+
+    def step(leaves, n, t):
+        y = D.gated_ffn(*leaves).view(-1, 1, 64)
+        q, k = D.qk_norm_rope(y, y, t, t, q_weight=n, k_weight=n)
+        with torch.no_grad():
+            z = D.gated_ffn(*leaves)
+        return [q.detach(), z, *torch.autograd.grad((q, k), leaves, (q.detach(), k.detach())), *D.pack8(z)]
+
+    sets = [inputs(i) for i in range(2)]
+    ref = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                if not all(torch.equal(a, b) for a, b in zip(step(*sets[i]), ref[i])):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and D.device_status() == 0
